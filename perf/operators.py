@@ -245,7 +245,8 @@ def _dropout_plain(st):
 def _tokens(x):
     """(whole numbers -127 .. 127, one scale per row) of float32 rows."""
     most = x.abs().amax(1, keepdim=True)
-    return (x * torch.where(most > 0, 127 / most, torch.zeros_like(most))).round(), most / 127
+    top = torch.full_like(most, 127)  # a tensor: a number's quotient is formed from its reciprocal, one rounding more
+    return (x * torch.where(most > 0, top / most, torch.zeros_like(most))).round(), most / top
 
 
 def _int8_product(x, codes, scale, bias):
