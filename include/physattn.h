@@ -664,6 +664,89 @@ int pa_layernorm_backward(int dtype, int64_t rows, int64_t C, const void *x, con
 int pa_layernorm_backward_add(int dtype, int64_t rows, int64_t C, const void *x, const void *dy, const void *add,
                               const float *gamma, float eps, void *dx, float *partials, float *grads, void *stream);
 
+/* ---- gated feed-forward block, dropout + add + LayerNorm, 8-bit integer Linears (no reference counterpart) ------------- */
+
+/* Activations: those of the reference's Mlp (physicsnemo/nn/module/mlp_layers.py:139-173 with its table of names). */
+#define PA_ACT_NONE 0
+#define PA_ACT_GELU 1 /* erf form */
+#define PA_ACT_RELU 2
+#define PA_ACT_SILU 3
+#define PA_ACT_SIGMOID 4
+#define PA_ACT_TANH 5
+
+/* Tensors of this section may start on any element boundary and have any width; rows that are not whole 16-byte units are
+ * copied to padded ones in the workspace, which must be 16-byte aligned.  C, F up to 2^18. */
+
+/* y = residual + w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down over rows of C with F hidden units.  Weights in the
+ * activations' type (dtype: PA_F32 or PA_BF16), biases float32, each NULL if there is none. */
+typedef struct pa_gated_params {
+  const void *w_gate;  /* (F, C) */
+  const float *b_gate; /* (F) or NULL */
+  const void *w_up;    /* (F, C) */
+  const float *b_up;   /* (F) or NULL */
+  const void *w_down;  /* (C, F) */
+  const float *b_down; /* (C) or NULL */
+} pa_gated_params;
+/* residual (rows, C) or NULL; y may be residual itself, but not x. */
+int64_t pa_gated_mlp_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F);
+int pa_gated_mlp_forward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
+                         const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
+/* Its gradients from dy and x; the hidden layer is formed again.  Weight gradients in the weights' type, bias gradients
+ * float32, each NULL if not wanted; dx (rows, C) or NULL.  (The gradient of residual is dy.)  Sums in a fixed order. */
+typedef struct pa_gated_grads {
+  void *w_gate;
+  float *b_gate;
+  void *w_up;
+  float *b_up;
+  void *w_down;
+  float *b_down;
+} pa_gated_grads;
+int64_t pa_gated_mlp_backward_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F);
+int pa_gated_mlp_backward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
+                          const void *dy, void *dx, const pa_gated_grads *grads, void *workspace, int64_t workspace_bytes,
+                          void *stream);
+
+/* y = residual + dropout(x), and with `normed` its LayerNorm (of the unrounded sum), over rows of C up to 2^23.  Element (r, c)
+ * is kept, and scaled by 1 / (1 - p), where word c % 4 of Philox4x32-10 of the counter (c / 4, r mod 2^32, r / 2^32,
+ * offset mod 2^32) under the seed is at least p 2^32 (rounded); an element that is dropped contributes zero whatever it holds.
+ * rng: two int64 in device memory, seed and offset.  p from 0 to 1.  residual or NULL; normed, gamma, beta: all or none;
+ * stats (rows, 2) float32, for the backward pass, or NULL. */
+int pa_dropout_add_norm(int dtype, int64_t rows, int64_t C, const void *x, const void *residual, double p, const int64_t *rng,
+                        void *y, const float *gamma, const float *beta, float eps, void *normed, float *stats, void *stream);
+/* Its backward pass under the same rng values: ds = dy + the LayerNorm's input gradient for d_normed; d_residual = ds,
+ * dx = ds kept and scaled; grads (2, C) float32 = d gamma, d beta.  dy or NULL (zero); d_normed NULL: no LayerNorm, and y,
+ * stats, gamma, d_residual and grads are not used.  dx, d_residual, grads: NULL if not wanted. */
+int64_t pa_dropout_add_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t C);
+int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *y,
+                                 const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
+                                 float *grads, void *workspace, int64_t workspace_bytes, void *stream);
+/* taken <- state, then state's offset + 1: the values one call and its backward pass use. */
+int pa_dropout_advance(int64_t *state, int64_t *taken, void *stream);
+
+/* q = rint(127 x / max |x|) per row as int8 and scale = max |x| / 127 (float32): rows of x of K elements; q's rows are ldq
+ * bytes apart (at least K, a multiple of 8; q 8-byte aligned), zeros behind the K-th.  A row of zeros has scale 0; one with an infinity or NaN has scale NaN. */
+int pa_int8_quantize_rows(int dtype, int64_t rows, int64_t K, const void *x, void *q, int64_t ldq, float *scale, void *stream);
+/* y = act(q_x q_w^T scaled by both scales + bias) + residual: x (rows, K) is quantised as above, w (N, K) int8 with w_scale (N)
+ * float32; bias (N) or NULL; residual, y (rows, N) in dtype.  K up to 131 072 (the sums stay below 2^31), N up to 2^18. */
+int64_t pa_int8_linear_workspace_bytes(int dtype, int64_t rows, int64_t K, int64_t N);
+int pa_int8_linear(int dtype, int64_t rows, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act,
+                   const void *x, const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
+/* pa_gated_mlp_forward on 8-bit weights and activations, the hidden layer quantised per row like x. */
+typedef struct pa_int8_gated_params {
+  const void *w_gate;  /* (F, C) int8 */
+  const float *s_gate; /* (F) */
+  const float *b_gate; /* (F) or NULL */
+  const void *w_up;
+  const float *s_up;
+  const float *b_up;
+  const void *w_down;  /* (C, F) int8 */
+  const float *s_down; /* (C) */
+  const float *b_down; /* (C) or NULL */
+} pa_int8_gated_params;
+int64_t pa_int8_gated_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F);
+int pa_int8_gated(int dtype, int64_t rows, int64_t C, int64_t F, const pa_int8_gated_params *p, int act, const void *x,
+                  const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- whole layer ------------------------------------------------------------------------------ */
 
 /* Replaces PhysicsAttentionBase.forward (PA.py:501-558), plus=False, use_te=False, dropout off.

@@ -229,3 +229,29 @@ def block_forward(p, fx, heads, dim_head, last_layer, variant="irregular", spati
         h3 = layer_norm(fx, p["ln_mlp2.0.weight"], p["ln_mlp2.0.bias"])
         return np.einsum("bnc,oc->bno", h3, _f64(p["ln_mlp2.1.weight"])) + _f64(p["ln_mlp2.1.bias"])
     return fx
+
+
+# ---- counter-based dropout (no reference counterpart: the reference uses nn.Dropout) ----
+
+
+def philox4x32(counter, key, rounds: int = 10):
+    """Philox4x32 (Salmon et al., SC 2011): four arrays of counter words and two of key words -> four arrays of words."""
+    c = [np.asarray(w, dtype=np.uint64) for w in counter]
+    k = [int(w) & 0xFFFFFFFF for w in key]
+    low, shift = np.uint64(0xFFFFFFFF), np.uint64(32)
+    for _ in range(rounds):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)  # of 32-bit words: they fit 64 bits
+        c = [(b >> shift) ^ c[1] ^ np.uint64(k[0]), b & low, (a >> shift) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def dropout_keep(seed: int, offset: int, rows, C: int, p: float):
+    """Boolean (len(rows), C): the elements of the given row numbers that dropout of probability p keeps."""
+    rows = np.asarray(rows, dtype=np.uint64)[:, None]
+    quads = np.arange((C + 3) // 4, dtype=np.uint64)[None, :]
+    one = np.ones((rows.shape[0], quads.shape[1]), dtype=np.uint64)
+    seed, offset = seed % 2 ** 64, offset % 2 ** 32
+    words = philox4x32((quads * one, (rows & np.uint64(0xFFFFFFFF)) * one, (rows >> np.uint64(32)) * one, np.uint64(offset) * one),
+                       (seed & 0xFFFFFFFF, seed >> 32))
+    return (np.stack(words, -1) >= np.uint64(round(p * 2 ** 32))).reshape(rows.shape[0], -1)[:, :C]

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_int64, c_void_p
 
 import torch  # noqa: F401  (must be imported first: its HIP runtime is the one the library binds to)
 
@@ -43,10 +43,14 @@ EXPORTED = [
     "pa_preprocess_query", "pa_preprocess_workspace_bytes", "pa_preprocess_forward",
     "pa_block_query", "pa_block_workspace_bytes", "pa_block_forward", "pa_markers_enabled",
     "pa_mfma_project_softmax_reduce_clocked", "pa_weight_grad_workspace_bytes", "pa_weight_grad",
+    "pa_gated_mlp_workspace_bytes", "pa_gated_mlp_forward", "pa_gated_mlp_backward_workspace_bytes", "pa_gated_mlp_backward",
+    "pa_dropout_add_norm", "pa_dropout_add_norm_backward_workspace_bytes", "pa_dropout_add_norm_backward", "pa_dropout_advance",
+    "pa_int8_quantize_rows", "pa_int8_linear_workspace_bytes", "pa_int8_linear", "pa_int8_gated_workspace_bytes", "pa_int8_gated",
 ]
 
 PA_TRAIN_SAVED, PA_TRAIN_FORWARD, PA_TRAIN_BACKWARD, PA_TRAIN_GRADS = range(4)
 PA_GRAD_LINEAR1, PA_GRAD_LINEAR2 = 1, 2
+ACTS = {None: 0, "gelu": 1, "relu": 2, "silu": 3, "sigmoid": 4, "tanh": 5}  # PA_ACT_*
 PA_BUF_BLOB, PA_BUF_FX_PACK, PA_BUF_W_PACK, PA_BUF_PARTIALS, PA_BUF_TOKP = range(5)
 
 
@@ -88,6 +92,18 @@ class PaGaleParams(Structure):
     _fields_ = [(n, c_void_p) for n in ("cross_q_weight", "cross_q_bias", "cross_k_weight", "cross_k_bias",
                                         "cross_v_weight", "cross_v_bias", "state_mixing", "concat_project_weight",
                                         "concat_project_bias")]
+
+
+class PaGatedParams(Structure):
+    _fields_ = [(n, c_void_p) for n in ("w_gate", "b_gate", "w_up", "b_up", "w_down", "b_down")]
+
+
+class PaGatedGrads(Structure):
+    _fields_ = [(n, c_void_p) for n in ("w_gate", "b_gate", "w_up", "b_up", "w_down", "b_down")]
+
+
+class PaInt8GatedParams(Structure):
+    _fields_ = [(n, c_void_p) for n in ("w_gate", "s_gate", "b_gate", "w_up", "s_up", "b_up", "w_down", "s_down", "b_down")]
 
 
 class PaBlockTail(Structure):
@@ -324,6 +340,32 @@ def load() -> ctypes.CDLL:
     lib.pa_layernorm_backward.argtypes = [c_int, c_int64, c_int64] + [c_void_p] * 3 + [c_float] + [c_void_p] * 3
     lib.pa_layernorm_backward_add.restype = c_int
     lib.pa_layernorm_backward_add.argtypes = [c_int, c_int64, c_int64] + [c_void_p] * 4 + [c_float] + [c_void_p] * 4
+    rows3 = [c_int, c_int64, c_int64, c_int64]
+    for name in ("pa_gated_mlp_workspace_bytes", "pa_gated_mlp_backward_workspace_bytes", "pa_int8_linear_workspace_bytes",
+                 "pa_int8_gated_workspace_bytes"):
+        getattr(lib, name).restype = c_int64
+        getattr(lib, name).argtypes = rows3
+    lib.pa_gated_mlp_forward.restype = c_int
+    lib.pa_gated_mlp_forward.argtypes = rows3 + [POINTER(PaGatedParams), c_int] + [c_void_p] * 4 + [c_int64, c_void_p]
+    lib.pa_gated_mlp_backward.restype = c_int
+    lib.pa_gated_mlp_backward.argtypes = rows3 + [POINTER(PaGatedParams), c_int] + [c_void_p] * 3 + [
+        POINTER(PaGatedGrads), c_void_p, c_int64, c_void_p]
+    lib.pa_dropout_add_norm.restype = c_int
+    lib.pa_dropout_add_norm.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_double] + [c_void_p] * 4 + [
+        c_float] + [c_void_p] * 3
+    lib.pa_dropout_add_norm_backward_workspace_bytes.restype = c_int64
+    lib.pa_dropout_add_norm_backward_workspace_bytes.argtypes = [c_int, c_int64, c_int64]
+    lib.pa_dropout_add_norm_backward.restype = c_int
+    lib.pa_dropout_add_norm_backward.argtypes = [c_int, c_int64, c_int64] + [c_void_p] * 5 + [c_double] + [c_void_p] * 5 + [
+        c_int64, c_void_p]
+    lib.pa_dropout_advance.restype = c_int
+    lib.pa_dropout_advance.argtypes = [c_void_p] * 3
+    lib.pa_int8_quantize_rows.restype = c_int
+    lib.pa_int8_quantize_rows.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]
+    lib.pa_int8_linear.restype = c_int
+    lib.pa_int8_linear.argtypes = rows3 + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int64, c_void_p]
+    lib.pa_int8_gated.restype = c_int
+    lib.pa_int8_gated.argtypes = rows3 + [POINTER(PaInt8GatedParams), c_int] + [c_void_p] * 4 + [c_int64, c_void_p]
     _lib = lib
     return lib
 

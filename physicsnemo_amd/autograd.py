@@ -1019,3 +1019,78 @@ def layer_norm(x: torch.Tensor, ln: torch.nn.LayerNorm) -> torch.Tensor:
     if _layer_norm_served(x, ln):
         return LayerNormFunction.apply(x.contiguous(), ln.weight, ln.bias, ln.eps)
     return ln(x)
+
+
+class GatedMlpFunction(torch.autograd.Function):
+    """`functional.gated_mlp_forward`, differentiable w.r.t. x, the residual and the six parameters.  The hidden layer is not
+    kept: the backward forms it again from x."""
+
+    @staticmethod
+    def forward(ctx, x, residual, w_gate, b_gate, w_up, b_up, w_down, b_down, act):
+        params = (w_gate, b_gate, w_up, b_up, w_down, b_down)
+        kernel = [None if p is None else p.detach().to(x.dtype if p.ndim == 2 else torch.float32).contiguous() for p in params]
+        ctx.act, ctx.param_dtypes = act, [None if p is None else p.dtype for p in params]
+        ctx.save_for_backward(x, *kernel[:5])
+        return PF.gated_mlp_forward(x, *kernel, act=act, residual=residual)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, *kernel = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dy = dy.to(x.dtype).contiguous()
+        dx, *grads = PF.gated_mlp_backward(x, dy, *kernel, act=ctx.act, wanted=(need[0], *need[2:8]))
+        grads = [None if g is None else g.to(t) for g, t in zip(grads, ctx.param_dtypes)]
+        return (dx, dy if need[1] else None, *grads, None)
+
+
+def gated_mlp(x, w_gate, b_gate, w_up, b_up, w_down, b_down, act: str | None = "silu", residual=None) -> torch.Tensor:
+    """Differentiable gated feed-forward block, `functional.gated_mlp_forward` in x's type (bfloat16 or float32): parameters
+    of other types are cast, strided inputs copied."""
+    x = x.contiguous()
+    residual = None if residual is None else residual.to(x.dtype).contiguous()
+    return GatedMlpFunction.apply(x, residual, w_gate, b_gate, w_up, b_up, w_down, b_down, act)
+
+
+class DropoutAddNormFunction(torch.autograd.Function):
+    """`functional.dropout_add_norm`, differentiable w.r.t. x, the residual and the LayerNorm's parameters; the backward forms
+    the mask again from the seed and offset, of which it keeps a copy's values."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, rng, ln_weight, ln_bias, eps):
+        ctx.set_materialize_grads(False)
+        ctx.p, ctx.has_residual = p, residual is not None
+        if ln_weight is None:
+            ctx.save_for_backward(rng)
+            ctx.ln_dtypes = None
+            return PF.dropout_add_norm(x, residual, p, rng)
+        w32 = ln_weight.detach().float().contiguous()
+        y, normed, stats = PF.dropout_add_norm(x, residual, p, rng, w32, ln_bias.detach().float().contiguous(), eps, True)
+        ctx.save_for_backward(rng, y, stats, w32)
+        ctx.ln_dtypes = (ln_weight.dtype, ln_bias.dtype)
+        return y, normed
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, d_normed=None):
+        need = ctx.needs_input_grad
+        if dy is None and d_normed is None:
+            return (None,) * 7
+        rng, *saved = ctx.saved_tensors
+        like = saved[0] if saved else dy
+        dy = None if dy is None else dy.to(like.dtype).contiguous()
+        if d_normed is None:
+            dx, dr, _, _ = PF.dropout_add_norm_backward(dy, None, None, None, None, ctx.p, rng, need[0], need[1])
+            return dx, dr, None, None, None, None, None
+        y, stats, w32 = saved
+        dx, dr, dg, db = PF.dropout_add_norm_backward(dy, d_normed.to(y.dtype).contiguous(), y, stats, w32, ctx.p, rng, need[0],
+                                                      need[1], need[4] or need[5])
+        return (dx, dr, None, None, dg.to(ctx.ln_dtypes[0]) if need[4] else None, db.to(ctx.ln_dtypes[1]) if need[5] else None, None)
+
+
+def dropout_add_norm(x, residual, p: float, rng, ln_weight=None, ln_bias=None, ln_eps: float = 1e-5):
+    """Differentiable `functional.dropout_add_norm`: y, or (y, LayerNorm(y)) with ln_weight.  `rng` must keep its values until
+    the backward pass has run (`functional.dropout_advance` hands out a copy per call)."""
+    x = x.contiguous()
+    residual = None if residual is None else residual.to(x.dtype).contiguous()
+    return DropoutAddNormFunction.apply(x, residual, p, rng, ln_weight, ln_bias, ln_eps)

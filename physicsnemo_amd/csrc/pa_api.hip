@@ -360,7 +360,7 @@ int mfma_layer(const pa_shape &s, const pa_params &p, const void *blob, const vo
 
 extern "C" {
 
-int pa_version(void) { return 112; }
+int pa_version(void) { return 113; }
 
 int pa_set_compute_units(int n) {
   if (n < 0 || n > 4096) return PA_ERR_DIMS;
@@ -1882,6 +1882,147 @@ int pa_layer_forward_plus(int dtype, const pa_shape *shape, const pa_params *p, 
   if ((rc = pa::general::out_linear(dtype, s, *p, out_x, y, st))) return rc;
   if (tail_active(tail)) rc = pa::general::residual_ln(dtype, s, y, *tail, st);
   return rc;
+}
+
+// ---- gated feed-forward block, dropout + add + LayerNorm, 8-bit integer Linears ----
+static bool act_ok(int act) { return act >= PA_ACT_NONE && act <= PA_ACT_TANH; }
+
+static int check_gated(int dtype, int64_t rows, int64_t C, int64_t F) {
+  if (rows <= 0 || C <= 0 || F <= 0) return PA_ERR_DIMS;
+  return pa::gated::supported(dtype, rows, C, F) ? PA_OK : PA_ERR_UNSUPPORTED;
+}
+
+int64_t pa_gated_mlp_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F) {
+  if (int rc = check_gated(dtype, rows, C, F)) return rc;
+  return pa::gated::forward_workspace_bytes(dtype, rows, C, F);
+}
+
+int pa_gated_mlp_forward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
+                         const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_gated_mlp_forward");
+  const int64_t need = pa_gated_mlp_workspace_bytes(dtype, rows, C, F);
+  if (need < 0) return (int)need;
+  if (!act_ok(act)) return PA_ERR_UNSUPPORTED;
+  if (!p || !p->w_gate || !p->w_up || !p->w_down || !x || !y || !workspace) return PA_ERR_NULL;
+  if (!aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::gated::forward(dtype, rows, C, F, *p, act, x, residual, y, workspace, compute_units(), static_cast<hipStream_t>(stream));
+}
+
+int64_t pa_gated_mlp_backward_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F) {
+  if (int rc = check_gated(dtype, rows, C, F)) return rc;
+  return pa::gated::backward_workspace_bytes(dtype, rows, C, F, compute_units());
+}
+
+int pa_gated_mlp_backward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
+                          const void *dy, void *dx, const pa_gated_grads *grads, void *workspace, int64_t workspace_bytes,
+                          void *stream) {
+  Range entry("pa_gated_mlp_backward");
+  const int64_t need = pa_gated_mlp_backward_workspace_bytes(dtype, rows, C, F);
+  if (need < 0) return (int)need;
+  if (!act_ok(act)) return PA_ERR_UNSUPPORTED;
+  if (!p || !p->w_gate || !p->w_up || !p->w_down || !x || !dy || !grads || !workspace) return PA_ERR_NULL;
+  if (!aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::gated::backward(dtype, rows, C, F, *p, act, x, dy, dx, *grads, workspace, compute_units(),
+                             static_cast<hipStream_t>(stream));
+}
+
+static int check_dropout(int dtype, int64_t rows, int64_t C) {
+  if (rows <= 0 || C <= 0) return PA_ERR_DIMS;
+  if ((dtype != PA_F32 && dtype != PA_BF16) || rows > PA_MAX_ROWS || C > 1 << 23) return PA_ERR_UNSUPPORTED;
+  return rows > ((int64_t)1 << 60) / C ? PA_ERR_UNSUPPORTED : PA_OK;
+}
+
+int pa_dropout_add_norm(int dtype, int64_t rows, int64_t C, const void *x, const void *residual, double p, const int64_t *rng,
+                        void *y, const float *gamma, const float *beta, float eps, void *normed, float *stats, void *stream) {
+  Range entry("pa_dropout_add_norm");
+  int rc = check_dropout(dtype, rows, C);
+  if (rc) return rc;
+  if (!(p >= 0.0 && p <= 1.0)) return PA_ERR_DIMS;
+  if (!x || !rng || !y || (normed && (!gamma || !beta))) return PA_ERR_NULL;
+  return pa::dropout::forward(dtype, rows, C, x, residual, p, rng, y, gamma, beta, eps, normed, stats, compute_units(),
+                              static_cast<hipStream_t>(stream));
+}
+
+int64_t pa_dropout_add_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t C) {
+  if (int rc = check_dropout(dtype, rows, C)) return rc;
+  return pa::dropout::backward_workspace_bytes(dtype, rows, C, compute_units());
+}
+
+int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *y,
+                                 const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
+                                 float *grads, void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_dropout_add_norm_backward");
+  const int64_t need = pa_dropout_add_norm_backward_workspace_bytes(dtype, rows, C);
+  if (need < 0) return (int)need;
+  if (!(p >= 0.0 && p <= 1.0)) return PA_ERR_DIMS;
+  if (!rng || (!dy && !d_normed)) return PA_ERR_NULL;
+  if (d_normed && (!y || !stats || !gamma || (grads && !workspace))) return PA_ERR_NULL;
+  if (d_normed && grads && !aligned16(workspace)) return PA_ERR_ALIGN;
+  if (d_normed && grads && workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::dropout::backward(dtype, rows, C, dy, d_normed, y, stats, gamma, p, rng, dx, d_residual, grads, workspace,
+                               compute_units(), static_cast<hipStream_t>(stream));
+}
+
+int pa_dropout_advance(int64_t *state, int64_t *taken, void *stream) {
+  if (!state || !taken) return PA_ERR_NULL;
+  return pa::dropout::advance(state, taken, static_cast<hipStream_t>(stream));
+}
+
+static int check_int8(int dtype, int64_t rows, int64_t K, int64_t N) {
+  if (rows <= 0 || K <= 0 || N <= 0) return PA_ERR_DIMS;
+  return pa::int8::supported(dtype, rows, K, N) ? PA_OK : PA_ERR_UNSUPPORTED;
+}
+
+int pa_int8_quantize_rows(int dtype, int64_t rows, int64_t K, const void *x, void *q, int64_t ldq, float *scale, void *stream) {
+  Range entry("pa_int8_quantize_rows");
+  if (int rc = check_int8(dtype, rows, K, 1)) return rc;
+  if (ldq < K || ldq % 8 != 0) return PA_ERR_DIMS;
+  if (ldq > 2 * K + 4096) return PA_ERR_UNSUPPORTED;
+  if (!x || !q || !scale) return PA_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(q) % 8 != 0) return PA_ERR_ALIGN;
+  return pa::int8::quantize_rows(dtype, rows, K, x, K, q, ldq, scale, static_cast<hipStream_t>(stream));
+}
+
+int64_t pa_int8_linear_workspace_bytes(int dtype, int64_t rows, int64_t K, int64_t N) {
+  if (int rc = check_int8(dtype, rows, K, N)) return rc;
+  return pa::int8::linear_workspace_bytes(rows, K, N);
+}
+
+int pa_int8_linear(int dtype, int64_t rows, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act,
+                   const void *x, const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_int8_linear");
+  const int64_t need = pa_int8_linear_workspace_bytes(dtype, rows, K, N);
+  if (need < 0) return (int)need;
+  if (!act_ok(act)) return PA_ERR_UNSUPPORTED;
+  if (!w || !w_scale || !x || !y || !workspace) return PA_ERR_NULL;
+  if (!aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::int8::linear(dtype, rows, K, N, w, w_scale, bias, act, x, residual, y, workspace, compute_units(),
+                          static_cast<hipStream_t>(stream));
+}
+
+static int check_int8_gated(int dtype, int64_t rows, int64_t C, int64_t F) {
+  const int rc = check_int8(dtype, rows, C, F);
+  return rc ? rc : check_int8(dtype, rows, F, C);
+}
+
+int64_t pa_int8_gated_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F) {
+  if (int rc = check_int8_gated(dtype, rows, C, F)) return rc;
+  return pa::int8::gated_workspace_bytes(dtype, rows, C, F);
+}
+
+int pa_int8_gated(int dtype, int64_t rows, int64_t C, int64_t F, const pa_int8_gated_params *p, int act, const void *x,
+                  const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_int8_gated");
+  const int64_t need = pa_int8_gated_workspace_bytes(dtype, rows, C, F);
+  if (need < 0) return (int)need;
+  if (!act_ok(act)) return PA_ERR_UNSUPPORTED;
+  if (!p || !p->w_gate || !p->s_gate || !p->w_up || !p->s_up || !p->w_down || !p->s_down || !x || !y || !workspace) return PA_ERR_NULL;
+  if (!aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::int8::gated(dtype, rows, C, F, *p, act, x, residual, y, workspace, compute_units(), static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

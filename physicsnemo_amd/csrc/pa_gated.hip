@@ -1,0 +1,316 @@
+// Gated feed-forward block, y = residual + W_down (act(W_gate x + b_gate) * (W_up x + b_up)) + b_down, and its backward pass:
+//   h  = act(g) u                     g = W_gate x + b_gate,  u = W_up x + b_up
+//   dh = W_down^T dy                  dg = dh u act'(g),      du = dh act(g)
+//   dx = W_gate^T dg + W_up^T du,     d W_gate = dg^T x, d W_up = du^T x, d W_down = dy^T h, d b = column sums
+// Both input products, the activation and the factor are one kernel (kGated); the backward forms g and u again beside dh
+// (kBack: 4 C F operations per row more, against 4 F elements per row written by the forward and read back), so the forward
+// leaves nothing behind.  Sums and all that happens between two products are float32; h, dg and du are rounded once, to the
+// activations' type, as operands of the next product.
+//
+// Operands whose rows are not whole 16-byte units (odd widths, views off a boundary) are copied to padded rows first, with the
+// transposed weights of the backward pass in the same launch.
+#include "pa_common.h"
+#include "pa_host.h"
+#include "pa_tile.h"
+
+namespace pa {
+namespace gated {
+
+using tile::Args;
+using tile::Layout;
+using tile::Space;
+using tile::up;
+using tile::whole_rows;
+
+// ---------------------------------------------------------------------------------------------------------------
+// lay_out_kernel: up to eight matrices copied into rows of whole units, zeros behind their last column, or transposed.  A
+// workgroup moves 64 x 64 elements; transposed ones turn in LDS.
+// ---------------------------------------------------------------------------------------------------------------
+template <class U>  // unsigned integer of the elements' size
+__global__ __launch_bounds__(256) void lay_out_kernel(Layout a) {
+  __shared__ U turn[64][65];
+  Layout::One o = a.m[0];
+#pragma unroll
+  for (int k = 1; k < Layout::kMost; ++k)
+    if (k < a.count && (int64_t)blockIdx.x >= a.m[k].first) o = a.m[k];
+  const int64_t block = (int64_t)blockIdx.x - o.first;
+  const int across = (o.width + 63) / 64, c0 = (int)(block % across) * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int64_t r0 = block / across * 64;
+  const U *src = static_cast<const U *>(o.src);
+  U *dst = static_cast<U *>(o.dst);
+  if (!o.turned) {
+    for (int k = y; k < 64; k += 4) {
+      const int64_t r = r0 + k;
+      if (r < o.rows && c0 + x < o.width) dst[r * o.ld + c0 + x] = c0 + x < o.cols ? src[r * o.src_ld + c0 + x] : U(0);
+    }
+    return;
+  }
+  for (int k = y; k < 64; k += 4)  // row c0 + k of src is column c0 + k of dst
+    turn[k][x] = c0 + k < o.cols && r0 + x < o.rows ? src[(int64_t)(c0 + k) * o.src_ld + r0 + x] : U(0);
+  __syncthreads();
+  for (int k = y; k < 64; k += 4)
+    if (r0 + k < o.rows && c0 + x < o.width) dst[(r0 + k) * o.ld + c0 + x] = turn[x][k];
+}
+
+}  // namespace gated
+
+namespace tile {
+int lay_out(const Layout &a, size_t elem, hipStream_t st) {
+  using gated::lay_out_kernel;
+  if (a.count == 0) return PA_OK;
+  if (a.blocks > 0x7fffffff) return PA_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)a.blocks);
+  if (elem == 1) hipLaunchKernelGGL(lay_out_kernel<uint8_t>, grid, dim3(256), 0, st, a);
+  else if (elem == 2) hipLaunchKernelGGL(lay_out_kernel<uint16_t>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(lay_out_kernel<uint32_t>, grid, dim3(256), 0, st, a);
+  return launch_status();
+}
+
+}  // namespace tile
+
+namespace gated {
+
+// ---------------------------------------------------------------------------------------------------------------
+// totals_kernel: partial products of the row-axis kernels added up in a fixed order, cropped to the parameter's size and
+// rounded to its type, all gradients in one launch.  A workgroup takes 256 neighbouring elements of a partial's rows, every
+// fourth partial per wave, four elements per lane.
+// ---------------------------------------------------------------------------------------------------------------
+struct Totals {
+  static constexpr int kMost = 6;
+  struct One {
+    const float *src;  // [G][..][ld], stride elements between partials
+    void *dst;         // (rows, cols)
+    int64_t stride, n, first;
+    int G, cols, ld, bytes;
+  } r[kMost];
+  int count = 0;
+  int64_t blocks = 0;
+  void add(const float *src, int64_t G, int64_t stride, int64_t ld, void *dst, int64_t rows, int64_t cols, int bytes) {
+    if (!dst) return;
+    r[count++] = One{src, dst, stride, rows * ld, blocks, (int)G, (int)cols, (int)ld, bytes};
+    blocks += (rows * ld + 255) / 256;
+  }
+};
+
+__global__ __launch_bounds__(256) void totals_kernel(Totals a) {
+  __shared__ float part[4][256];
+  Totals::One o = a.r[0];
+#pragma unroll
+  for (int k = 1; k < Totals::kMost; ++k)
+    if (k < a.count && (int64_t)blockIdx.x >= a.r[k].first) o = a.r[k];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t e0 = ((int64_t)blockIdx.x - o.first) * 256;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {  // element e0 + 64 j + lane: whole lines, whatever the alignment
+    const int64_t e = e0 + 64 * j + lane;
+    float s = 0.f;
+    if (e < o.n) {
+      const float *p = o.src + e;
+      int g = wave;
+      for (; g + 12 < o.G; g += 16) {
+        const float v0 = p[g * o.stride], v1 = p[(g + 4) * o.stride], v2 = p[(g + 8) * o.stride], v3 = p[(g + 12) * o.stride];
+        s += (v0 + v1) + (v2 + v3);
+      }
+      for (; g < o.G; g += 4) s += p[g * o.stride];
+    }
+    part[wave][64 * j + lane] = s;
+  }
+  __syncthreads();
+  const int64_t e = e0 + threadIdx.x;
+  if (e >= o.n) return;
+  const int64_t row = e / o.ld;
+  const int col = (int)(e - row * o.ld);
+  if (col >= o.cols) return;
+  const float v = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+  if (o.bytes == 2) static_cast<uint16_t *>(o.dst)[row * o.cols + col] = f32_to_bf16_bits(v);
+  else static_cast<float *>(o.dst)[row * o.cols + col] = v;
+}
+
+// ================================================================================================
+// host side
+// ================================================================================================
+// rows of `width` elements as the tile kernels read them: as they lie, or a padded copy queued in `lay`
+struct Rows {
+  const void *p;
+  int64_t ld;  // bytes
+  int units;
+};
+static Rows rows_of(const void *p, int64_t rows, int64_t width, int64_t elem, bool copy, Space &ws, Layout *lay) {
+  const int64_t padded = up(width, 16 / elem);
+  Rows r{p, padded * elem, (int)(padded * elem / 16)};
+  if (copy) {
+    void *dst = ws.take(rows * padded * elem);
+    if (lay) lay->add(p, width, dst, rows, width, padded, padded, false);
+    r.p = dst;
+  }
+  return r;
+}
+
+template <class E, class TO, tile::Kind KIND>
+static int product(const Args &a, int num_cu, hipStream_t st) {
+  return tile::launch_tiles<E, TO, KIND, 2, 2, 2, 2, 2>(a, num_cu, st);
+}
+
+// The forward's workspace: h, and padded copies of what is not laid out in whole units.  The plan depends on the pointers'
+// alignment; the query answers for the worst case.
+template <class E, class TO>
+static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *residual, void *y,
+                   char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
+  constexpr int64_t e = E::kBytes, U = 16 / e;
+  const bool plan = bytes != nullptr;
+  Space ws{workspace};
+  Layout lay;
+  const int64_t Fp = up(F, U);
+  auto copied = [&](const void *q, int64_t width) { return plan || !whole_rows(q, width, e); };
+  void *h = ws.take(M * Fp * e);
+  const Rows xr = rows_of(x, M, C, e, copied(x, C), ws, &lay);
+  const Rows wg = rows_of(p.w_gate, F, C, e, copied(p.w_gate, C), ws, &lay);
+  const Rows wu = rows_of(p.w_up, F, C, e, copied(p.w_up, C), ws, &lay);
+  const Rows wd = rows_of(p.w_down, C, F, e, copied(p.w_down, F), ws, &lay);
+  if (plan) return *bytes = ws.used, PA_OK;
+  if (int rc = tile::lay_out(lay, e, st)) return rc;
+  Args a{};
+  a.X = xr.p, a.ldx = xr.ld, a.units = xr.units;
+  a.W[0] = wg.p, a.W[1] = wu.p, a.ldw = wg.ld;
+  a.M = M, a.N = (int)F, a.limit = (int)Fp;
+  a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+  a.out = h, a.ldo = Fp, a.act = act;
+  if (int rc = product<E, TO, tile::kGated>(a, num_cu, st)) return rc;
+  Args d{};
+  d.X = h, d.ldx = Fp * e, d.units = (int)(Fp * e / 16);
+  d.W[0] = wd.p, d.ldw = wd.ld;
+  d.M = M, d.N = d.limit = (int)C;
+  d.bias[0] = p.b_down;
+  d.residual = residual, d.out = y, d.ldo = C;
+  d.vec = whole_rows(y, C, e) && (!residual || aligned16(residual));
+  return product<E, TO, tile::kPlain>(d, num_cu, st);
+}
+
+static constexpr int64_t kMaxWidth = 1 << 18;  // 256 rows of two hidden layers of it stay below 2^31 bytes
+
+bool supported(int dtype, int64_t M, int64_t C, int64_t F) {
+  return (dtype == PA_F32 || dtype == PA_BF16) && M > 0 && C > 0 && F > 0 && M <= PA_MAX_ROWS && C <= kMaxWidth && F <= kMaxWidth &&
+         M <= ((int64_t)1 << 60) / (16 * (C > F ? C : F));
+}
+
+int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F) {
+  int64_t bytes = 0;
+  const pa_gated_params p{};
+  if (dtype == PA_F32) forward<tile::F32, float>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  else forward<tile::Bf16, bf16>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  return bytes;
+}
+
+int forward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *residual, void *y,
+            void *workspace, int num_cu, hipStream_t st) {
+  char *ws = static_cast<char *>(workspace);
+  if (dtype == PA_F32) return forward<tile::F32, float>(M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
+  return forward<tile::Bf16, bf16>(M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
+}
+
+// partial results of a row-axis product of `oa` by `ob` columns, and of the column sums of its first operand
+struct Partials {
+  int64_t G;
+  float *product, *sums;
+};
+template <class E>
+static Partials partials_of(int64_t M, int64_t oa, int64_t ob, int num_cu, Space &ws) {
+  Partials r{};
+  if (E::kBytes == 2) r.G = wgrad::chunks_for(M, ((oa + 255) / 256) * ((ob + 255) / 256), oa * ob, num_cu);
+  else r.G = gemm::cols_gemm_f32_chunks(M, oa, ob, num_cu);
+  r.product = static_cast<float *>(ws.take(r.G * oa * ob * 4));
+  r.sums = static_cast<float *>(ws.take(r.G * oa * 4));
+  return r;
+}
+template <class E>
+static int rows_product(const Partials &r, const void *A, int64_t oa, const void *B, int64_t ob, int64_t M, int num_cu, hipStream_t st) {
+  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, r.sums, st);
+  return gemm::cols_gemm_f32(A, oa, oa, B, ob, ob, M, nullptr, r.product, r.sums, num_cu, st);
+}
+
+template <class E, class TO>
+static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *dy, void *dx,
+                    const pa_gated_grads &out, char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
+  constexpr int64_t e = E::kBytes, U = 16 / e, LEAST = e == 4 ? 16 : 8;  // narrowest operand of the row-axis kernels
+  const bool plan = bytes != nullptr;
+  Space ws{workspace};
+  Layout lay;
+  const int64_t Cp = up(C < LEAST ? LEAST : C, U), Fp = up(F < LEAST ? LEAST : F, U);
+  const bool copy_x = plan || C != Cp || !aligned16(x), copy_dy = plan || C != Cp || !aligned16(dy);
+  void *dgu = ws.take(M * 2 * Fp * e), *h = ws.take(M * Fp * e);
+  auto padded = [&](const void *q, int64_t rows, int64_t cols, int64_t ld, bool copy) {
+    Rows r{q, ld * e, (int)(ld * e / 16)};
+    if (copy) {
+      void *dst = ws.take(rows * ld * e);
+      lay.add(q, cols, dst, rows, cols, ld, ld, false);
+      r.p = dst;
+    }
+    return r;
+  };
+  const Rows xr = padded(x, M, C, Cp, copy_x), dyr = padded(dy, M, C, Cp, copy_dy);
+  const bool copy_w = plan || C != Cp || !aligned16(p.w_gate) || !aligned16(p.w_up);
+  const Rows wg = padded(p.w_gate, F, C, Cp, copy_w), wu = padded(p.w_up, F, C, Cp, copy_w);
+  // W_down^T (F, Cp), and [W_gate; W_up]^T (C, 2 Fp): hidden units past F are zero columns
+  void *wd_t = ws.take(F * Cp * e), *w_t = ws.take(C * 2 * Fp * e);
+  const Partials in = partials_of<E>(M, 2 * Fp, Cp, num_cu, ws), down = partials_of<E>(M, Cp, Fp, num_cu, ws);
+  if (plan) return *bytes = ws.used, PA_OK;
+  lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
+  if (dx) {
+    lay.add(p.w_gate, C, w_t, C, F, Fp, 2 * Fp, true);
+    lay.add(p.w_up, C, static_cast<char *>(w_t) + Fp * e, C, F, Fp, 2 * Fp, true);
+  }
+  int rc = tile::lay_out(lay, e, st);
+  if (rc) return rc;
+  Args a{};
+  a.X = xr.p, a.ldx = xr.ld, a.units = xr.units;
+  a.X2 = dyr.p, a.ldx2 = dyr.ld, a.units2 = dyr.units;
+  a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
+  a.M = M, a.N = (int)F, a.limit = (int)Fp;
+  a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+  a.out = dgu, a.ldo = 2 * Fp, a.out2 = h, a.ldh = Fp, a.act = act;
+  if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
+  if (dx) {
+    Args d{};
+    d.X = dgu, d.ldx = 2 * Fp * e, d.units = (int)(2 * Fp * e / 16);
+    d.W[0] = w_t, d.ldw = 2 * Fp * e;
+    d.M = M, d.N = d.limit = (int)C;
+    d.out = dx, d.ldo = C;
+    d.vec = whole_rows(dx, C, e);
+    if ((rc = product<E, TO, tile::kPlain>(d, num_cu, st))) return rc;
+  }
+  Totals totals;
+  if (out.w_gate || out.w_up || out.b_gate || out.b_up) {
+    if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, num_cu, st))) return rc;
+    totals.add(in.product, in.G, 2 * Fp * Cp, Cp, out.w_gate, F, C, e);
+    totals.add(in.product + Fp * Cp, in.G, 2 * Fp * Cp, Cp, out.w_up, F, C, e);
+    totals.add(in.sums, in.G, 2 * Fp, F, out.b_gate, 1, F, 4);
+    totals.add(in.sums + Fp, in.G, 2 * Fp, F, out.b_up, 1, F, 4);
+  }
+  if (out.w_down || out.b_down) {
+    if ((rc = rows_product<E>(down, dyr.p, Cp, h, Fp, M, num_cu, st))) return rc;
+    totals.add(down.product, down.G, Cp * Fp, Fp, out.w_down, C, F, e);
+    totals.add(down.sums, down.G, Cp, C, out.b_down, 1, C, 4);
+  }
+  if (totals.count == 0) return PA_OK;
+  hipLaunchKernelGGL(totals_kernel, dim3((unsigned)totals.blocks), dim3(256), 0, st, totals);
+  return launch_status();
+}
+
+int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu) {
+  int64_t bytes = 0;
+  const pa_gated_params p{};
+  const pa_gated_grads g{};
+  if (dtype == PA_F32) backward<tile::F32, float>(M, C, F, p, 0, nullptr, nullptr, nullptr, g, nullptr, &bytes, num_cu, nullptr);
+  else backward<tile::Bf16, bf16>(M, C, F, p, 0, nullptr, nullptr, nullptr, g, nullptr, &bytes, num_cu, nullptr);
+  return bytes;
+}
+
+int backward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *dy, void *dx,
+             const pa_gated_grads &out, void *workspace, int num_cu, hipStream_t st) {
+  char *ws = static_cast<char *>(workspace);
+  if (dtype == PA_F32) return backward<tile::F32, float>(M, C, F, p, act, x, dy, dx, out, ws, nullptr, num_cu, st);
+  return backward<tile::Bf16, bf16>(M, C, F, p, act, x, dy, dx, out, ws, nullptr, num_cu, st);
+}
+
+}  // namespace gated
+}  // namespace pa

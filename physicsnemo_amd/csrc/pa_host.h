@@ -125,6 +125,7 @@ int product(int dtype, int64_t M, const void *A, int64_t lda, int64_t OA, const 
 int launch_wide(const void *A, int64_t lda, int64_t OA, const void *B, int64_t ldb, int64_t OB, int64_t M, int64_t G,
                 const pa_shape *grid, float *partials, float *col_sums, hipStream_t st);
 int sum_rows(const float *src, int64_t rows, int64_t n, float *dst, hipStream_t st);
+int64_t chunks_for(int64_t M, int64_t tiles, int64_t n, int num_cu);  // partial results of a product of `tiles` workgroups
 int64_t output_backward_workspace_bytes(const pa_shape &s, int num_cu);
 int output_backward(const pa_shape &s, const void *w_pack, const void *dy, const float *out_token, const void *w_out,
                     void *workspace, float *d_out_token, float *d_w_out, float *d_b_out, int num_cu, hipStream_t st);
@@ -155,6 +156,40 @@ int forward(const pa_shape &s, const pa_params &p, const void *x, void *y, const
 int backward(const pa_shape &s, const void *x, const void *dy, const void *saved, void *dx, float *grads, void *workspace,
              int num_cu, hipStream_t st);
 }  // namespace train_f32
+
+namespace gated {
+// gated feed-forward block: see pa_gated_mlp_forward / _backward
+bool supported(int dtype, int64_t M, int64_t C, int64_t F);
+int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F);
+int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu);
+int forward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *residual, void *y,
+            void *workspace, int num_cu, hipStream_t st);
+int backward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *dy, void *dx,
+             const pa_gated_grads &out, void *workspace, int num_cu, hipStream_t st);
+}  // namespace gated
+
+namespace int8 {
+// products of 8-bit integers: see pa_int8_*
+bool supported(int dtype, int64_t M, int64_t K, int64_t N);
+int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, hipStream_t st);
+int64_t linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act, const void *x,
+           const void *residual, void *y, void *workspace, int num_cu, hipStream_t st);
+int64_t gated_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F);
+int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated_params &p, int act, const void *x, const void *residual,
+          void *y, void *workspace, int num_cu, hipStream_t st);
+}  // namespace int8
+
+namespace dropout {
+// dropout + residual add + LayerNorm: see pa_dropout_add_norm*
+int advance(int64_t *state, int64_t *taken, hipStream_t st);
+int forward(int dtype, int64_t M, int64_t C, const void *x, const void *residual, double p, const int64_t *rng, void *y,
+            const float *gamma, const float *beta, float eps, void *normed, float *stats, int num_cu, hipStream_t st);
+int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int num_cu);
+int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_normed, const void *y, const float *stats,
+             const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual, float *grads, void *workspace, int num_cu,
+             hipStream_t st);
+}  // namespace dropout
 
 namespace general {
 int dequant_e4m3(const void *in, const float *scale, void *out, int64_t rows, int64_t cols, hipStream_t st);

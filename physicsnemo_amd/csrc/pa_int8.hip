@@ -1,0 +1,248 @@
+// Products of 8-bit integers with one float32 scale per token (row of activations) and per output channel (row of weights):
+//   q = rint(127 x / max |x|) per row, s = max |x| / 127;  y = act(s s_w (q . q_w) + b) + residual
+// The sums of whole numbers are exact in 32 bits up to 131 072 terms of 127 x 127.  int8 matrix instructions have twice the
+// rate of bf16 ones and the operands half the bytes, so the products run on the tile kernel of pa_tile.h with stages of 128
+// elements.
+#include "pa_common.h"
+#include "pa_host.h"
+#include "pa_tile.h"
+
+namespace pa {
+namespace int8 {
+
+using tile::Args;
+using tile::Layout;
+using tile::Space;
+using tile::u32x2;
+using tile::u32x4;
+using tile::up;
+using tile::whole_rows;
+
+// eight neighbouring elements as float32, zeros past `left`
+template <bool VEC>
+__device__ __forceinline__ void load8(const bf16 *p, int64_t left, float (&v)[8]) {
+  if (VEC && left >= 8) {
+    const u32x4 w = *reinterpret_cast<const u32x4 *>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t b = w[j];
+      v[2 * j] = __uint_as_float(b << 16), v[2 * j + 1] = __uint_as_float(b & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? load_as_f32(p + j) : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load8(const float *p, int64_t left, float (&v)[8]) {
+  if (VEC && left >= 8) {
+    const tile::f32x4 a = *reinterpret_cast<const tile::f32x4 *>(p), b = *reinterpret_cast<const tile::f32x4 *>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.f;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// quantize_rows_kernel: a wave per row, eight elements per lane and step; rows of up to 512 NCH elements stay in registers
+// between the maximum and the rounding, longer ones are read again.  The maximum runs over the bits of |x|, in which NaN lies
+// above infinity above the numbers: a row with one of them gets scale NaN, which is what a product with it would be.
+// ---------------------------------------------------------------------------------------------------------------
+struct Quantize {
+  const void *x;
+  int64_t M, K, ldx, ldq;  // elements; bytes
+  uint8_t *q;
+  float *scale;
+};
+
+template <class T, int NCH, bool VEC>
+__global__ __launch_bounds__(256) void quantize_rows_kernel(Quantize a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= a.M) return;
+  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+  float v[NCH][8];
+  uint32_t most = 0;
+  auto larger = [&](const float (&w)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t b = __float_as_uint(w[j]) & 0x7fffffffu;
+      most = b > most ? b : most;
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) {
+    const int64_t k = c * 512 + lane * 8;
+    load8<VEC>(x + k, a.K - k, v[c]);
+    larger(v[c]);
+  }
+  for (int64_t k = NCH * 512 + lane * 8; k < a.K; k += 512) {
+    float w[8];
+    load8<VEC>(x + k, a.K - k, w);
+    larger(w);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const uint32_t b = (uint32_t)__shfl_xor((int)most, off, 64);
+    most = b > most ? b : most;
+  }
+  const bool finite = most < 0x7f800000u;
+  const float top = __uint_as_float(most);
+  const float lift = top < 0x1p-100f ? 0x1p100f : 1.f;  // 127 / top stays finite
+  const float inv = finite && most > 0 ? 127.f / (top * lift) : 0.f;
+  auto store = [&](int64_t k, const float (&w)[8]) {
+    if (k >= a.ldq) return;
+    u32x2 out = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float r = fminf(fmaxf(rintf(w[j] * lift * inv), -127.f), 127.f);
+      const uint32_t code = finite ? (uint32_t)((int)r & 0xff) : 0u;
+      if (j < 4) out[0] |= code << (8 * j);
+      else out[1] |= code << (8 * (j - 4));
+    }
+    *reinterpret_cast<u32x2 *>(a.q + row * a.ldq + k) = out;
+  };
+#pragma unroll
+  for (int c = 0; c < NCH; ++c) store(c * 512 + lane * 8, v[c]);
+  for (int64_t k = NCH * 512 + lane * 8; k < a.ldq; k += 512) {
+    float w[8];
+    load8<VEC>(x + k, a.K - k, w);
+    store(k, w);
+  }
+  if (lane == 0) a.scale[row] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
+}
+
+static constexpr int64_t kMaxTerms = 131072;  // 127 x 127 of them stay below 2^31
+
+bool supported(int dtype, int64_t M, int64_t K, int64_t N) {
+  return (dtype == PA_F32 || dtype == PA_BF16) && M > 0 && K > 0 && N > 0 && M <= (int64_t)1 << 32 && K <= kMaxTerms && N <= 1 << 18;
+}
+
+template <class T>
+static int quantize(const Quantize &a, bool vec, hipStream_t st) {
+  const int64_t blocks = (a.M + 3) / 4;
+  if (blocks > 0x7fffffff) return PA_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)blocks), wg(256);
+  if (vec && a.K <= 512) hipLaunchKernelGGL((quantize_rows_kernel<T, 1, true>), grid, wg, 0, st, a);
+  else if (vec) hipLaunchKernelGGL((quantize_rows_kernel<T, 4, true>), grid, wg, 0, st, a);
+  else if (a.K <= 512) hipLaunchKernelGGL((quantize_rows_kernel<T, 1, false>), grid, wg, 0, st, a);
+  else hipLaunchKernelGGL((quantize_rows_kernel<T, 4, false>), grid, wg, 0, st, a);
+  return launch_status();
+}
+
+int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, hipStream_t st) {
+  const Quantize a{x, M, K, ldx, ldq, static_cast<uint8_t *>(q), scale};
+  const bool vec = whole_rows(x, ldx, dtype == PA_F32 ? 4 : 2);
+  return dtype == PA_F32 ? quantize<float>(a, vec, st) : quantize<bf16>(a, vec, st);
+}
+
+template <class TO, tile::Kind KIND>
+static int product(const Args &a, int num_cu, hipStream_t st) {
+  return tile::launch_tiles<tile::I8, TO, KIND, 2, 2, 2, 2, 2>(a, num_cu, st);
+}
+
+// codes of a weight (rows, width) as the tile kernel reads them: as they lie, or copied to rows of whole units
+static const void *codes_of(const void *w, int64_t rows, int64_t width, bool plan, Space &ws, Layout &lay) {
+  if (!plan && whole_rows(w, width, 1)) return w;
+  void *dst = ws.take(rows * up(width, 16));
+  lay.add(w, width, dst, rows, width, up(width, 16), up(width, 16), false);
+  return dst;
+}
+
+struct Tokens {
+  uint8_t *q;
+  float *scale;
+};
+static Tokens tokens(int64_t M, int64_t K, Space &ws) {
+  return {static_cast<uint8_t *>(ws.take(M * up(K, 16))), static_cast<float *>(ws.take(M * 4))};
+}
+
+template <class TO>
+static int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act,
+                  const void *x, const void *residual, void *y, char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
+  Space ws{workspace};
+  Layout lay;
+  const Tokens q = tokens(M, K, ws);
+  const void *codes = codes_of(w, N, K, bytes != nullptr, ws, lay);
+  if (bytes) return *bytes = ws.used, PA_OK;
+  int rc = tile::lay_out(lay, 1, st);
+  if (!rc) rc = quantize_rows(dtype, M, K, x, K, q.q, up(K, 16), q.scale, st);
+  if (rc) return rc;
+  Args a{};
+  a.X = q.q, a.ldx = a.ldw = up(K, 16), a.units = (int)(up(K, 16) / 16);
+  a.W[0] = codes;
+  a.M = M, a.N = a.limit = (int)N;
+  a.bias[0] = bias, a.sx = q.scale, a.sw[0] = w_scale;
+  a.residual = residual, a.out = y, a.ldo = N, a.act = act;
+  a.vec = whole_rows(y, N, sizeof(TO)) && (!residual || aligned16(residual));
+  return product<TO, tile::kPlain>(a, num_cu, st);
+}
+
+int64_t linear_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+  int64_t bytes = 0;
+  linear<float>(PA_F32, M, K, N, nullptr, nullptr, nullptr, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  return bytes;
+}
+
+int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act, const void *x,
+           const void *residual, void *y, void *workspace, int num_cu, hipStream_t st) {
+  char *ws = static_cast<char *>(workspace);
+  if (dtype == PA_F32) return linear<float>(dtype, M, K, N, w, w_scale, bias, act, x, residual, y, ws, nullptr, num_cu, st);
+  return linear<bf16>(dtype, M, K, N, w, w_scale, bias, act, x, residual, y, ws, nullptr, num_cu, st);
+}
+
+// The gated block: x's codes against W_gate and W_up in one product, the hidden layer in the activations' type (its largest
+// value per row is known when the row is complete), its codes against W_down.
+template <class TO>
+static int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated_params &p, int act, const void *x,
+                 const void *residual, void *y, char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
+  Space ws{workspace};
+  Layout lay;
+  const bool plan = bytes != nullptr;
+  const int64_t Fp = up(F, 16 / sizeof(TO)), Kc = up(C, 16), Kf = up(F, 16);
+  void *h = ws.take(M * Fp * sizeof(TO));
+  const Tokens qx = tokens(M, C, ws), qh = tokens(M, F, ws);
+  const void *gate = codes_of(p.w_gate, F, C, plan, ws, lay), *upw = codes_of(p.w_up, F, C, plan, ws, lay),
+             *down = codes_of(p.w_down, C, F, plan, ws, lay);
+  if (plan) return *bytes = ws.used, PA_OK;
+  int rc = tile::lay_out(lay, 1, st);
+  if (!rc) rc = quantize_rows(dtype, M, C, x, C, qx.q, Kc, qx.scale, st);
+  if (rc) return rc;
+  Args a{};
+  a.X = qx.q, a.ldx = a.ldw = Kc, a.units = (int)(Kc / 16);
+  a.W[0] = gate, a.W[1] = upw;
+  a.M = M, a.N = (int)F, a.limit = (int)Fp;
+  a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+  a.sx = qx.scale, a.sw[0] = p.s_gate, a.sw[1] = p.s_up;
+  a.out = h, a.ldo = Fp, a.act = act;
+  if ((rc = product<TO, tile::kGated>(a, num_cu, st))) return rc;
+  if ((rc = quantize_rows(dtype, M, F, h, Fp, qh.q, Kf, qh.scale, st))) return rc;
+  Args d{};
+  d.X = qh.q, d.ldx = d.ldw = Kf, d.units = (int)(Kf / 16);
+  d.W[0] = down;
+  d.M = M, d.N = d.limit = (int)C;
+  d.bias[0] = p.b_down, d.sx = qh.scale, d.sw[0] = p.s_down;
+  d.residual = residual, d.out = y, d.ldo = C;
+  d.vec = whole_rows(y, C, sizeof(TO)) && (!residual || aligned16(residual));
+  return product<TO, tile::kPlain>(d, num_cu, st);
+}
+
+int64_t gated_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F) {
+  int64_t bytes = 0;
+  const pa_int8_gated_params p{};
+  if (dtype == PA_F32) gated<float>(dtype, M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  else gated<bf16>(dtype, M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  return bytes;
+}
+
+int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated_params &p, int act, const void *x, const void *residual,
+          void *y, void *workspace, int num_cu, hipStream_t st) {
+  char *ws = static_cast<char *>(workspace);
+  if (dtype == PA_F32) return gated<float>(dtype, M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
+  return gated<bf16>(dtype, M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
+}
+
+}  // namespace int8
+}  // namespace pa

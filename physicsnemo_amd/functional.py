@@ -6,6 +6,7 @@ kernels on torch's current stream.  `params` is the dict produced by
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
 from ctypes import byref
 from functools import lru_cache
 from typing import NamedTuple
@@ -1136,3 +1137,273 @@ def ball_query(points: torch.Tensor, queries: torch.Tensor, radius: float, max_n
     else:
         raise ValueError(f"unknown ball_query method {method!r}")
     return (idx, out, counts, dists) if return_dists else (idx, out, counts)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# gated feed-forward block, dropout + add + LayerNorm, 8-bit integer Linears
+# ---------------------------------------------------------------------------------------------------------------------
+
+
+def _on(device: torch.device):
+    """The library launches on the current device: make `device` that for the call where it is not."""
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _act_code(act: str | None) -> int:
+    try:
+        return _lib.ACTS[act]
+    except (KeyError, TypeError):
+        raise ValueError(f"activation {act!r} not found; available are {[a for a in _lib.ACTS if a]} and None") from None
+
+
+def _same_device(x, *others):
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"all tensors have to be on the input's device ({x.device}), got one on {t.device}")
+
+
+def _expect(t, what: str, shape, dtype):
+    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+        raise ValueError(f"{what} has to be {dtype} of shape {tuple(shape)}, got {t.dtype} of shape {tuple(t.shape)}")
+
+
+def _sized(code: int, what: str) -> int:
+    if code < 0:
+        _lib.check(int(code), what)
+    return int(code)
+
+
+def _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, b_down):
+    """(rows, C, F) after checking that the parameters belong together and to x."""
+    _need_cuda(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
+    _same_device(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
+    _lib.dtype_code(x.dtype)
+    if x.ndim < 1 or w_gate.ndim != 2:
+        raise ValueError("x needs a last axis of channels and w_gate the shape (F, C)")
+    C, F = x.shape[-1], w_gate.shape[0]
+    for name, w, shape in (("w_gate", w_gate, (F, C)), ("w_up", w_up, (F, C)), ("w_down", w_down, (C, F))):
+        _expect(w, name, shape, x.dtype)
+    for name, b, n in (("b_gate", b_gate, F), ("b_up", b_up, F), ("b_down", b_down, C)):
+        _expect(b, name, (n,), torch.float32)
+    if C == 0 or F == 0:
+        raise ValueError("the gated block needs at least one channel and one hidden unit")
+    return x.numel() // C, C, F
+
+
+def gated_mlp_forward(x, w_gate, b_gate, w_up, b_up, w_down, b_down, act: str | None = "silu", residual=None):
+    """y = w_down . (act(w_gate . x + b_gate) * (w_up . x + b_up)) + b_down [+ residual] over the last axis of x.
+
+    x (..., C) bfloat16 or float32; w_gate, w_up (F, C) and w_down (C, F) in the same type; biases float32 or None; `act`
+    one of "silu", "gelu" (erf form), "relu", "sigmoid", "tanh", None.  Any widths."""
+    rows, C, F = _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
+    code = _act_code(act)
+    _need_cuda(residual)
+    _same_device(x, residual)
+    _expect(residual, "residual", x.shape, x.dtype)
+    y = torch.empty_like(x)
+    if rows == 0:
+        return y
+    lib, dtype = _lib.load(), _lib.dtype_code(x.dtype)
+    with _on(x.device):
+        nbytes = _sized(lib.pa_gated_mlp_workspace_bytes(dtype, rows, C, F), "pa_gated_mlp_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        params = _lib.PaGatedParams(*map(_lib.ptr, (w_gate, b_gate, w_up, b_up, w_down, b_down)))
+        _lib.check(lib.pa_gated_mlp_forward(dtype, rows, C, F, byref(params), code, x.data_ptr(), _lib.ptr(residual), y.data_ptr(),
+                                            workspace.data_ptr(), nbytes, _lib.current_stream_ptr(x.device)), "pa_gated_mlp_forward")
+    return y
+
+
+def gated_mlp_backward(x, dy, w_gate, b_gate, w_up, b_up, w_down, act: str | None = "silu", wanted=(True,) * 7):
+    """Gradients of `gated_mlp_forward` for dy: (dx, d w_gate, d b_gate, d w_up, d b_up, d w_down, d b_down), weight gradients
+    in the weights' type, bias gradients float32; `wanted` says which of the seven are formed, the others are None."""
+    rows, C, F = _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, None)
+    code = _act_code(act)
+    _need_cuda(dy)
+    _same_device(x, dy)
+    _expect(dy, "dy", x.shape, x.dtype)
+    shapes = (x.shape, (F, C), (F,), (F, C), (F,), (C, F), (C,))
+    types = (x.dtype, x.dtype, torch.float32, x.dtype, torch.float32, x.dtype, torch.float32)
+    make = torch.empty if rows else torch.zeros
+    out = [make(s, dtype=t, device=x.device) if w else None for s, t, w in zip(shapes, types, wanted)]
+    if rows == 0 or not any(wanted):
+        return tuple(out)
+    lib, dtype = _lib.load(), _lib.dtype_code(x.dtype)
+    with _on(x.device):
+        nbytes = _sized(lib.pa_gated_mlp_backward_workspace_bytes(dtype, rows, C, F), "pa_gated_mlp_backward_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        params = _lib.PaGatedParams(*map(_lib.ptr, (w_gate, b_gate, w_up, b_up, w_down, None)))
+        grads = _lib.PaGatedGrads(*map(_lib.ptr, out[1:]))
+        _lib.check(lib.pa_gated_mlp_backward(dtype, rows, C, F, byref(params), code, x.data_ptr(), dy.data_ptr(), _lib.ptr(out[0]),
+                                             byref(grads), workspace.data_ptr(), nbytes, _lib.current_stream_ptr(x.device)),
+                   "pa_gated_mlp_backward")
+    return tuple(out)
+
+
+def _dropout_args(x, p, rng, *rows):
+    _need_cuda(x, rng, *rows)
+    _same_device(x, rng, *rows)
+    _lib.dtype_code(x.dtype)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, got {p}")
+    _expect(rng, "rng (seed, offset)", (2,), torch.int64)
+    if x.ndim < 1:
+        raise ValueError("x needs a last axis of channels")
+    for t in rows:
+        _expect(t, "a tensor of rows", x.shape, x.dtype)
+
+
+def dropout_add_norm(x, residual, p: float, rng, ln_weight=None, ln_bias=None, ln_eps: float = 1e-5, return_stats: bool = False):
+    """y = residual + dropout(x) in one pass, the mask formed from `rng` and never stored; returns y, or
+    (y, LayerNorm(y)) when ln_weight is given (of the unrounded sum; float32 ln_weight and ln_bias).  residual None: dropout
+    alone.  rng: int64 tensor (seed, offset) on the device; the same values, shape and p give the same mask (see
+    `pa_dropout_add_norm` for how).  With `return_stats` mean and 1 / std of the rows (rows, 2), which the backward pass
+    reads, are appended.  x (..., C) bfloat16 or float32."""
+    _dropout_args(x, p, rng, residual)
+    C = x.shape[-1]
+    if (ln_weight is None) != (ln_bias is None):
+        raise ValueError("ln_weight and ln_bias are given together")
+    _need_cuda(ln_weight, ln_bias)
+    _same_device(x, ln_weight, ln_bias)
+    _expect(ln_weight, "ln_weight", (C,), torch.float32)
+    _expect(ln_bias, "ln_bias", (C,), torch.float32)
+    rows = x.numel() // C if C else 0
+    y = torch.empty_like(x)
+    normed = torch.empty_like(x) if ln_weight is not None else None
+    stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if return_stats and normed is not None else None
+    if rows:
+        with _on(x.device):
+            _lib.check(_lib.load().pa_dropout_add_norm(
+                _lib.dtype_code(x.dtype), rows, C, x.data_ptr(), _lib.ptr(residual), p, rng.data_ptr(), y.data_ptr(),
+                _lib.ptr(ln_weight), _lib.ptr(ln_bias), float(ln_eps), _lib.ptr(normed), _lib.ptr(stats),
+                _lib.current_stream_ptr(x.device)), "pa_dropout_add_norm")
+    out = y if normed is None else (y, normed)
+    return (*out, stats) if stats is not None else out
+
+
+def dropout_add_norm_backward(dy, d_normed, y, stats, ln_weight, p: float, rng, need_dx: bool = True, need_residual: bool = True,
+                              need_ln: bool = True):
+    """(dx, d residual, d ln_weight, d ln_bias) of `dropout_add_norm` under the rng values it ran with, from the gradients
+    of y and of the normalised rows (dy None: zero; d_normed None: no LayerNorm, y, stats and ln_weight are not used,
+    d residual is dy itself and the LayerNorm's gradients None)."""
+    rows_like = dy if d_normed is None else d_normed
+    if rows_like is None:
+        raise ValueError("dy or d_normed has to be given")
+    norm = d_normed is not None
+    _dropout_args(rows_like, p, rng, dy, d_normed, *((y,) if norm else ()))
+    C = rows_like.shape[-1]
+    rows = rows_like.numel() // C if C else 0
+    device = rows_like.device
+    if norm:
+        _need_cuda(stats, ln_weight)
+        _same_device(rows_like, stats, ln_weight)
+        if y is None or stats is None or ln_weight is None:
+            raise ValueError("a gradient of the normalised rows needs y, stats and ln_weight")
+        _expect(stats, "stats", (rows, 2), torch.float32)
+        _expect(ln_weight, "ln_weight", (C,), torch.float32)
+    dx = torch.empty_like(rows_like) if need_dx else None
+    d_residual = (torch.empty_like(rows_like) if norm else dy) if need_residual else None
+    grads = (torch.empty if rows else torch.zeros)(2, C, dtype=torch.float32, device=device) if norm and need_ln else None
+    if rows and (dx is not None or norm):
+        lib, code = _lib.load(), _lib.dtype_code(rows_like.dtype)
+        with _on(device):
+            nbytes = _sized(lib.pa_dropout_add_norm_backward_workspace_bytes(code, rows, C),
+                            "pa_dropout_add_norm_backward_workspace_bytes") if grads is not None else 0
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            _lib.check(lib.pa_dropout_add_norm_backward(
+                code, rows, C, _lib.ptr(dy), _lib.ptr(d_normed), _lib.ptr(y) if norm else None, _lib.ptr(stats) if norm else None,
+                _lib.ptr(ln_weight) if norm else None, p, rng.data_ptr(), _lib.ptr(dx), _lib.ptr(d_residual) if norm else None,
+                _lib.ptr(grads), workspace.data_ptr(), nbytes, _lib.current_stream_ptr(device)), "pa_dropout_add_norm_backward")
+    return (dx, d_residual, *((None, None) if grads is None else (grads[0], grads[1])))
+
+
+def dropout_advance(state):
+    """The (seed, offset) pair for one call: a copy of `state`, whose offset goes up by one; one small launch, in a captured graph
+    on every replay."""
+    _need_cuda(state)
+    _expect(state, "state (seed, offset)", (2,), torch.int64)
+    taken = torch.empty_like(state)
+    with _on(state.device):
+        _lib.check(_lib.load().pa_dropout_advance(state.data_ptr(), taken.data_ptr(), _lib.current_stream_ptr(state.device)),
+                   "pa_dropout_advance")
+    return taken
+
+
+def quantize_int8(x):
+    """(int8 codes, float32 scale per row) of the rows of x (..., K): codes rint(127 x / max |x|), scale max |x| / 127.
+    For a weight (N, K) that is one scale per output channel.  A row of zeros has scale 0, one with an infinity or NaN
+    scale NaN."""
+    _need_cuda(x)
+    if x.ndim < 1 or x.shape[-1] == 0:
+        raise ValueError("x needs a last axis with at least one element")
+    K = x.shape[-1]
+    rows = x.numel() // K
+    padded = (K + 7) // 8 * 8
+    q = torch.empty(*x.shape[:-1], padded, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    code = _lib.dtype_code(x.dtype)
+    if rows:
+        with _on(x.device):
+            _lib.check(_lib.load().pa_int8_quantize_rows(code, rows, K, x.data_ptr(), q.data_ptr(), padded, scale.data_ptr(),
+                                                         _lib.current_stream_ptr(x.device)), "pa_int8_quantize_rows")
+    return (q if padded == K else q[..., :K].contiguous()), scale
+
+
+def _int8_weight(x, name, w, scale, bias, shape):
+    _need_cuda(w, scale, bias)
+    _same_device(x, w, scale, bias)
+    _expect(w, f"w_{name}", shape, torch.int8)
+    _expect(scale, f"the scale of w_{name}", shape[:1], torch.float32)
+    _expect(bias, f"the bias of w_{name}", shape[:1], torch.float32)
+
+
+def linear_int8(x, weight, weight_scale, bias=None, act: str | None = None, residual=None):
+    """y = act(weight . x + bias) [+ residual] with an 8-bit weight (N, K) int8, one float32 scale per output channel
+    (`quantize_int8` of the weight), and x (..., K) bfloat16 or float32 rounded to 8 bits per token on the way; the sums of
+    products are exact.  bias (N) float32 or None.  For inference: it has no gradient."""
+    _need_cuda(x, residual)
+    _same_device(x, residual)
+    dtype, code = _lib.dtype_code(x.dtype), _act_code(act)
+    if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] == 0 or weight.shape[0] == 0:
+        raise ValueError("x needs a last axis of channels and weight the shape (N, K)")
+    N, K = weight.shape[0], x.shape[-1]
+    _int8_weight(x, "weight", weight, weight_scale, bias, (N, K))
+    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+    _expect(residual, "residual", y.shape, x.dtype)
+    rows = x.numel() // K
+    if rows == 0:
+        return y
+    lib = _lib.load()
+    with _on(x.device):
+        nbytes = _sized(lib.pa_int8_linear_workspace_bytes(dtype, rows, K, N), "pa_int8_linear_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        _lib.check(lib.pa_int8_linear(dtype, rows, K, N, weight.data_ptr(), weight_scale.data_ptr(), _lib.ptr(bias), code,
+                                      x.data_ptr(), _lib.ptr(residual), y.data_ptr(), workspace.data_ptr(), nbytes,
+                                      _lib.current_stream_ptr(x.device)), "pa_int8_linear")
+    return y
+
+
+def gated_mlp_int8(x, w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, b_down, act: str | None = "silu", residual=None):
+    """`gated_mlp_forward` on 8-bit weights (int8 with one float32 scale per output channel, `quantize_int8`) and activations
+    rounded to 8 bits per token, the hidden layer likewise.  For inference: it has no gradient."""
+    _need_cuda(x, residual)
+    _same_device(x, residual)
+    dtype, code = _lib.dtype_code(x.dtype), _act_code(act)
+    if x.ndim < 1 or w_gate.ndim != 2 or x.shape[-1] == 0 or w_gate.shape[0] == 0:
+        raise ValueError("x needs a last axis of channels and w_gate the shape (F, C)")
+    C, F = x.shape[-1], w_gate.shape[0]
+    _int8_weight(x, "gate", w_gate, s_gate, b_gate, (F, C))
+    _int8_weight(x, "up", w_up, s_up, b_up, (F, C))
+    _int8_weight(x, "down", w_down, s_down, b_down, (C, F))
+    _expect(residual, "residual", x.shape, x.dtype)
+    y = torch.empty_like(x)
+    rows = x.numel() // C
+    if rows == 0:
+        return y
+    lib = _lib.load()
+    with _on(x.device):
+        nbytes = _sized(lib.pa_int8_gated_workspace_bytes(dtype, rows, C, F), "pa_int8_gated_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        params = _lib.PaInt8GatedParams(*map(_lib.ptr, (w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, b_down)))
+        _lib.check(lib.pa_int8_gated(dtype, rows, C, F, byref(params), code, x.data_ptr(), _lib.ptr(residual), y.data_ptr(),
+                                     workspace.data_ptr(), nbytes, _lib.current_stream_ptr(x.device)), "pa_int8_gated")
+    return y
