@@ -148,7 +148,7 @@ static Rows rows_of(const void *p, int64_t rows, int64_t width, int64_t elem, bo
 
 template <class E, class TO, tile::Kind KIND>
 static int product(const Args &a, int num_cu, hipStream_t st) {
-  return tile::launch_tiles<E, TO, KIND, 2, 2, 2, 2, 2>(a, num_cu, st);
+  return tile::launch<E, TO, KIND>(a, num_cu, st);
 }
 
 // The forward's workspace: h, and padded copies of what is not laid out in whole units.  The plan depends on the pointers'

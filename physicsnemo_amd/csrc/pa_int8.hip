@@ -140,7 +140,7 @@ int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, v
 
 template <class TO, tile::Kind KIND>
 static int product(const Args &a, int num_cu, hipStream_t st) {
-  return tile::launch_tiles<tile::I8, TO, KIND, 2, 2, 2, 2, 2>(a, num_cu, st);
+  return tile::launch<tile::I8, TO, KIND>(a, num_cu, st);
 }
 
 // codes of a weight (rows, width) as the tile kernel reads them: as they lie, or copied to rows of whole units

@@ -61,7 +61,7 @@ __device__ __forceinline__ void act_values(int act, f32x16 &v) {
   switch (act) {
     case kGelu:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = gelu_fit(v[r]);
+      for (int r = 0; r < 16; ++r) v[r] = gelu_tail(v[r]);
       break;
     case kRelu:  // NaN passes, as torch's does
 #pragma unroll
@@ -89,10 +89,9 @@ __device__ __forceinline__ void act_slopes(int act, f32x16 &v, f32x16 &slope) {
     case kGelu:
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float x = v[r];
-        const GeluParts p = gelu_parts(x);
-        slope[r] = gelu_grad(x, p);
-        v[r] = x * p.phi;
+        float d;
+        v[r] = gelu_tail_slope(v[r], d);
+        slope[r] = d;
       }
       break;
     case kRelu:
@@ -157,69 +156,86 @@ struct Args {
   int mt, nt;                    // tiles
 };
 
-// four neighbouring floats (p on any float); past the last of n that one again
-__device__ __forceinline__ f32x4 quad_at(const float *p, int col, int n, bool whole) {
-  typedef float f32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
-  if (whole) return *reinterpret_cast<const f32x4_at4 *>(p + col);
-  f32x4 v;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = p[col + j < n ? col + j : n - 1];
-  return v;
-}
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned kNowhere = 0x80000000u;  // an offset past every buffer below: loads give zero, stores are dropped
 
-__device__ __forceinline__ f32x4 widen4(const float *p) { return *reinterpret_cast<const f32x4 *>(p); }
-__device__ __forceinline__ f32x4 widen4(const bf16 *p) {
-  const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
-  const uint32_t a = w[0], b = w[1];
-  return f32x4{__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u), __uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)};
-}
-
-// columns col .. col + 31 (below limit) of this lane's row; row points at the row's column 0
-template <bool VEC>
-__device__ __forceinline__ void store_tile(const f32x16 &v, bf16 *row, int col, int limit, int g, bool ok) {
-  if constexpr (VEC) {
-    u32x4 s0, s1;
-    mfma::tile_natural(v, s0, s1);
-    const int c = col + 16 * g;
-    if (ok && c < limit) *reinterpret_cast<u32x4 *>(row + c) = s0;
-    if (ok && c + 8 < limit) *reinterpret_cast<u32x4 *>(row + c + 8) = s1;
-  } else {
+// 16-byte stores of a 32 x 32 tile: this lane's row at byte offset `at`, columns col .. col + 31 below limit.  Neighbouring
+// columns of a row come from both halves of the wave: a lane's 16 bytes lie beside its partner's.
+__device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, unsigned at, int col, int limit, int g, const bf16 *) {
+  uint32_t p[4][2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int c = col + rowmap(r, g);
-      if (ok && c < limit) row[c].bits = mfma::to_bf16_bits(v[r]);
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) p[q][w] = pack2(v[4 * q + 2 * w], v[4 * q + 2 * w + 1]);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u32x4 s;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const auto r = __builtin_amdgcn_permlane32_swap(p[2 * h][w], p[2 * h + 1][w], false, false);
+      s[w] = r[0], s[2 + w] = r[1];
     }
+    const int c = col + 16 * h + 8 * g;
+    __builtin_amdgcn_raw_buffer_store_b128(s, out, c < limit ? at + 2 * c : kNowhere, 0, 0);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store_tile(const f32x16 &v, float *row, int col, int limit, int g, bool ok) {
+__device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, unsigned at, int col, int limit, int g, const float *) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int c = col + 8 * q + 4 * g;
-    if constexpr (VEC) {
-      if (ok && c < limit) *reinterpret_cast<f32x4 *>(row + c) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-    } else {
+    u32x4 s;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (ok && c + j < limit) row[c + j] = v[4 * q + j];
-    }
+    for (int j = 0; j < 4; ++j) s[j] = __float_as_uint(v[4 * q + j]);
+    __builtin_amdgcn_raw_buffer_store_b128(s, out, c < limit ? at + 4 * c : kNowhere, 0, 0);
   }
 }
+template <class T>
+constexpr int kTileStores = sizeof(T) == 2 ? 2 : 4;
 
-// accumulators to float32: int8 sums take their scales; then the bias.  Columns past N hold something of column N - 1.
+// four neighbouring elements of a row of the residual, as they lie and as float32
+template <class T>
+struct Quad;
+template <>
+struct Quad<bf16> {
+  u32x2 w;
+  __device__ __forceinline__ void load(const Buffer &in, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b64(in, at, 0, 0); }
+  __device__ __forceinline__ float operator[](int j) const {
+    const uint32_t b = w[j >> 1];
+    return __uint_as_float(j & 1 ? b & 0xffff0000u : b << 16);
+  }
+};
+template <>
+struct Quad<float> {
+  u32x4 w;
+  __device__ __forceinline__ void load(const Buffer &in, unsigned at) { w = __builtin_amdgcn_raw_buffer_load_b128(in, at, 0, 0); }
+  __device__ __forceinline__ float operator[](int j) const {
+    const uint32_t b = w[j];
+    return __uint_as_float(b);
+  }
+};
+
+// one float per lane, to dst + 4 lane
+__device__ __forceinline__ void load_word_to_lds(const float *p, unsigned dst) {
+  asm volatile(
+      "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %0, off" ::"v"(p), "s"(dst)
+      : "memory");
+}
+
+// accumulators to float32: int8 sums take their scales; then the bias.  `side` points at the tile's 32 biases, `scale` at its
+// 32 scales.
 template <class E>
-__device__ __forceinline__ f32x16 values_of(const typename E::Acc &acc, const Args &a, int which, int col, int g, float sx) {
+__device__ __forceinline__ f32x16 values_of(const typename E::Acc &acc, const float *side, const float *scale, int g, float sx) {
   f32x16 v;
-  const bool whole = col + 32 <= a.N;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int c = col + 8 * q + 4 * g;
-    f32x4 b = {0.f, 0.f, 0.f, 0.f}, s = b;
-    if (a.bias[which]) b = quad_at(a.bias[which], c, a.N, whole);
-    if constexpr (E::kBytes == 1) s = quad_at(a.sw[which], c, a.N, whole) * sx;
+    const f32x4 b = *reinterpret_cast<const f32x4 *>(side + 8 * q + 4 * g);
+    f32x4 s = {1.f, 1.f, 1.f, 1.f};
+    if constexpr (E::kBytes == 1) s = *reinterpret_cast<const f32x4 *>(scale + 8 * q + 4 * g) * sx;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if constexpr (E::kBytes == 1) v[4 * q + j] = (float)acc[4 * q + j] * s[j] + b[j];
+      if constexpr (E::kBytes == 1) v[4 * q + j] = fmaf((float)acc[4 * q + j], s[j], b[j]);
       else v[4 * q + j] = acc[4 * q + j] + b[j];
     }
   }
@@ -229,22 +245,41 @@ __device__ __forceinline__ f32x16 values_of(const typename E::Acc &acc, const Ar
 // ---------------------------------------------------------------------------------------------------------------
 // rows_tile_kernel.  A workgroup of WM x WN waves owns tiles of BM rows x BN weight rows; a wave's part is TM x TN tiles of
 // 32 x 32.  kGated and kBack take 32 rows of W0 and the 32 rows of W1 in turn, so that a wave holds both factors of its
-// hidden units.  Stages of 128 bytes of every row pass through two LDS buffers, filled by direct global -> LDS loads while
-// the stage before is multiplied, one barrier per stage; the stages of a workgroup's tiles form one sequence, so that the
-// first stage of a tile arrives behind the last products and the stores of the one before.
-// Position p of row r holds the row's unit p ^ (r / 2 % 8): the 16 lanes of an access phase fall on all 64 banks.
+// hidden units.  Stages of UPS units of every row pass through a ring of RING LDS buffers, filled RING - 1 stages ahead by
+// direct global -> LDS loads, one barrier per stage; the stages of a workgroup's tiles form one sequence, so that the
+// first stages of a tile arrive behind the last products and the stores of the one before.
+// Position p of row r holds the row's unit p ^ (r / 4 % 4) (UPS = 4) or p ^ (r / 2 % 8) (UPS = 8): the 16 lanes of an access
+// phase fall on all 64 banks.
 // Units past a row's last one repeat it and are left out of the products; rows past the last row repeat it and are not stored.
+// What the epilogue needs besides (biases; int8: both scales) arrives in LDS with a tile's first stage, a buffer per tile.
+// Loads and stores are counted in order: the stores of a tile leave behind the first AHEAD stages of the next one and must not be
+// waited for with those, so the vector paths issue every store, with an offset past the buffer where there is nothing to
+// store, and the waits of a tile's first stages leave that many operations more in flight.
 // Tiles are dealt out to the XCDs (= workgroup id mod 8) in eight equal runs with the columns running fastest, so that the
 // workgroups of an L2 share rows of X and W.
 // ---------------------------------------------------------------------------------------------------------------
-template <class E, class TO, Kind KIND, int WM, int WN, int TM, int TN, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
-  constexpr int WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
+template <int WM_, int WN_, int TM_, int TN_, int UPS_, int RING_, int OCC_>
+struct Config {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, UPS = UPS_, RING = RING_, OCC = OCC_;  // OCC: waves per SIMD
+  static constexpr int WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
+  static constexpr int STAGE = (BM + BN) * 16 * UPS;
+  static constexpr int side(int bytes) { return bytes == 1 ? 2 * BN + BM : BN; }  // floats
+  static constexpr int lds(int bytes) { return RING * (STAGE + 4 * side(bytes)); }
+};
+
+template <class E, class TO, Kind KIND, class CFG>
+__global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Args a) {
+  constexpr int WM = CFG::WM, TM = CFG::TM, TN = CFG::TN, WAVES = CFG::WAVES, BM = CFG::BM, BN = CFG::BN, UPS = CFG::UPS;
+  constexpr int RING = CFG::RING, AHEAD = RING - 1, GROUP = 64 / UPS;  // rows of one load
   constexpr bool DUAL = KIND != kPlain;
-  constexpr int NX = BM / 8 / WAVES, NW = BN / 8 / WAVES, TN2 = TN / 2;  // groups of 8 rows a wave fetches
-  static_assert(BM % (8 * WAVES) == 0 && BN % (16 * WAVES) == 0, "whole groups");
+  constexpr int NX = BM / GROUP / WAVES, NW = BN / GROUP / WAVES, TN2 = TN / 2;  // loads a wave issues
+  static_assert(BM % (GROUP * WAVES) == 0 && BN % (GROUP * WAVES) == 0, "whole groups");
   static_assert(!DUAL || TN % 2 == 0, "pairs of tiles");
-  constexpr unsigned STAGE = (BM + BN) * 128;
+  constexpr unsigned STAGE = CFG::STAGE, SIDE = CFG::side(E::kBytes);
+  static_assert(BM % 64 == 0 && BN % 64 == 0, "whole loads of 64 floats");
+  // stores a wave leaves behind a tile
+  constexpr int STORES = kTileStores<TO> * TM * (KIND == kPlain ? TN : KIND == kGated ? TN2 : 3 * TN2), YOUNGER = (AHEAD - 1) * (NX + NW);
+  constexpr int LEFT = YOUNGER + STORES < 63 ? YOUNGER + STORES : 63;
   using Acc = typename E::Acc;
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
@@ -257,20 +292,21 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
   int t = (int)((int64_t)total * xcd / 8) + (blockIdx.x >> 3);
   if (t >= last) return;
 
-  const int nk1 = (a.units + 7) / 8, nk = nk1 + (KIND == kBack ? (a.units2 + 7) / 8 : 0);
+  const int nk1 = (a.units + UPS - 1) / UPS, nk = nk1 + (KIND == kBack ? (a.units2 + UPS - 1) / UPS : 0);
 
-  // ---- the loads run one stage ahead of the products ----
-  int lt = t, lk = 0;       // tile and stage that are fetched next
-  unsigned buf = 0;         // where they go
+  // ---- the loads run RING - 1 stages ahead of the products ----
+  int lt = t, lk = 0;  // tile and stage that are fetched next
+  unsigned buf = 0;    // where they go
+  int sbuf = 0;        // and the side data
   unsigned offx[NX], offw[NW];
   const char *xbase = nullptr, *wbase[2] = {nullptr, nullptr};
-  const int frow = lane >> 3;
+  const int frow = lane / UPS, fpos = lane % UPS;
   auto uniform = [](const char *p) {  // what is the same for every lane, in scalar registers
     const uint64_t v = (uint64_t)(uintptr_t)p;
     return reinterpret_cast<const char *>((uintptr_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
                                                       (uint32_t)__builtin_amdgcn_readfirstlane((int)v)));
   };
-  auto unit_of = [&](int row) { return (lane & 7) ^ ((row >> 1) & 7); };
+  auto swizzle = [](int row) { return UPS == 8 ? (row >> 1) & 7 : (row >> 2) & 3; };
   auto place = [&](bool second) {  // offsets of tile lt: rows of X and W (second: of X2 and W[2])
     const int tm = lt / a.nt, tn = lt - tm * a.nt;
     const int64_t m0 = (int64_t)tm * BM, ldx = second ? a.ldx2 : a.ldx, ldw = second ? a.ldw2 : a.ldw;
@@ -280,45 +316,67 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
     if constexpr (DUAL) wbase[1] = static_cast<const char *>(a.W[1]) + n0 * ldw;
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
-      const int row = (wave * NX + q) * 8 + frow, r = row < have ? row : have - 1;
-      offx[q] = (unsigned)(r * ldx) + 16 * unit_of(row);
+      const int row = (wave * NX + q) * GROUP + frow, r = row < have ? row : have - 1;
+      offx[q] = (unsigned)(r * ldx) + 16 * (fpos ^ swizzle(row));
     }
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
-      const int row = second ? (wave * (NW / 2) + (q < NW / 2 ? q : 0)) * 8 + frow : (wave * NW + q) * 8 + frow;
+      const int row = (wave * NW + q) * GROUP + frow;
       const int col = DUAL && !second ? (row >> 6) * 32 + (row & 31) : row, c = col < haven ? col : haven - 1;
-      offw[q] = (unsigned)(c * ldw) + 16 * unit_of(row);
+      offw[q] = (unsigned)(c * ldw) + 16 * (fpos ^ swizzle(row));
     }
   };
   auto fetch = [&]() {
-    if (lt >= last) return;
-    const bool second = KIND == kBack && lk >= nk1;
-    if (lk == 0 || (KIND == kBack && lk == nk1)) place(second);
-    const int kb = second ? lk - nk1 : lk, left = (second ? a.units2 : a.units) - 8 * kb;
+    const bool none = lt >= last;  // past the last tile: the last stage again, so that every stage counts the same loads
+    const bool second = KIND == kBack && (none ? nk1 < nk : lk >= nk1);
+    if (!none && (lk == 0 || (KIND == kBack && lk == nk1))) place(second);
+    const int kb = none ? (second ? nk - nk1 : nk1) - 1 : second ? lk - nk1 : lk, left = (second ? a.units2 : a.units) - UPS * kb;
     const unsigned dst = (unsigned)(uintptr_t)smem + buf;
     // units past the row's last one: that one again; the products leave them out
     auto past = [&](int unit) { return 16u * (unsigned)(unit >= left ? unit - left + 1 : 0); };
-    const unsigned past_even = past((lane & 7) ^ (frow >> 1)), past_odd = past((lane & 7) ^ (frow >> 1) ^ 4);
+    const unsigned past_even = past(fpos ^ swizzle(frow)), past_odd = past(fpos ^ swizzle(frow + GROUP));
+    if (!none && lk == 0) {
+      const int n0 = (lt % a.nt) * CN;
+      const int64_t m0 = (int64_t)(lt / a.nt) * BM;
+      for (int k = wave; k < (int)SIDE / 64; k += WAVES) {
+        const int at = 64 * k + lane;
+        const float *p;
+        if (64 * k < 2 * BN) {
+          const int v = 64 * k < BN ? at : at - BN, which = DUAL ? (v >> 5) & 1 : 0, col = n0 + (DUAL ? (v >> 6) * 32 + (v & 31) : v);
+          const float *from = 64 * k < BN ? a.bias[which] : a.sw[which];
+          p = from ? from + (col < a.N ? col : a.N - 1) : reinterpret_cast<const float *>(&mfma::kZeroUnit);
+        } else {
+          const int64_t m = m0 + at - 2 * BN;
+          p = a.sx + (m < a.M ? m : a.M - 1);
+        }
+        load_word_to_lds(p, (unsigned)(uintptr_t)smem + RING * STAGE + 4 * (sbuf * SIDE + 64 * k));
+      }
+      sbuf = sbuf + 1 == RING ? 0 : sbuf + 1;
+    }
     auto off_of = [&](unsigned off, int grp) { return (int)(off - (grp & 1 ? past_odd : past_even)); };
-    const char *xs = uniform(xbase + (int64_t)kb * 128);
+    const char *xs = uniform(xbase + (int64_t)kb * (16 * UPS)), *ws0 = uniform(wbase[0] + (int64_t)kb * (16 * UPS));
+    const char *ws1 = DUAL ? uniform(wbase[1] + (int64_t)kb * (16 * UPS)) : ws0;
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
       const int grp = wave * NX + q;
       load_unit_to_lds(xs, off_of(offx[q], grp), dst + grp * 1024);
     }
-    const char *ws0 = uniform(wbase[0] + (int64_t)kb * 128), *ws1 = DUAL ? uniform(wbase[1] + (int64_t)kb * 128) : ws0;
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
-      if (second && q >= NW / 2) break;
-      const int grp = second ? wave * (NW / 2) + q : wave * NW + q;
-      load_unit_to_lds(DUAL && !second && (grp & 4) ? ws1 : ws0, off_of(offw[q], grp), dst + BM * 128 + grp * 1024);
+      const int grp = wave * NW + q;
+      // second: half as many rows; in a longer ring the other loads are made all the same, so that every stage counts as many
+      if (AHEAD == 1 && second && grp * GROUP >= BN / 2) continue;
+      load_unit_to_lds(DUAL && !second && (grp & (32 / GROUP)) ? ws1 : ws0, off_of(offw[q], grp), dst + BM * 16 * UPS + grp * 1024);
     }
-    buf ^= STAGE;
-    if (++lk == nk) lk = 0, lt += step;
+    buf = buf + STAGE == RING * STAGE ? 0 : buf + STAGE;
+    if (!none && ++lk == nk) lk = 0, lt += step;
   };
 
-  fetch();
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) fetch();
   unsigned cur = 0;
+  int cside = 0;
+  bool stored = false;  // the tile before left exactly STORES stores
   for (; t < last; t += step) {
     Acc acc[TM][TN], acc2[KIND == kBack ? TM : 1][KIND == kBack ? TN2 : 1];
 #pragma unroll
@@ -335,26 +393,30 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc2[m][n][r] = 0;
     }
-    const int swz = (i >> 1) & 7;
+    const int swz = swizzle(i);
+    int at_stage = 0;
     auto next_stage = [&]() {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the stage has landed
-      __syncthreads();                                  // everyone's; and everyone is past the stage before
+      // this wave's share of the stage has landed; the younger stages and, at first, the stores of the tile before stay in flight
+      if (stored && at_stage < AHEAD) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(YOUNGER) : "memory");
+      ++at_stage;
+      __syncthreads();  // everyone's; and everyone is past the stage before
       fetch();
     };
-    auto multiply = [&](auto &to, auto tn_, auto whole_, int left, int wrow) {  // left: units of the stage, 8 where `whole`
+    auto multiply = [&](auto &to, auto tn_, auto whole_, int left, int wrow) {  // left: units of the stage, UPS where `whole`
       constexpr int T = decltype(tn_)::value;
       constexpr bool WHOLE = decltype(whole_)::value;
-      const u32x4 *xs = smem + cur / 16 + (wm * TM * 32 + i) * 8;
-      const u32x4 *ws = smem + cur / 16 + (BM + wrow + i) * 8;
+      const u32x4 *xs = smem + cur / 16 + (wm * TM * 32 + i) * UPS;
+      const u32x4 *ws = smem + cur / 16 + (BM + wrow + i) * UPS;
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
+      for (int ks = 0; ks < UPS / 2; ++ks) {
         if (!WHOLE && 2 * ks >= left) break;
         const int at = (2 * ks + g) ^ swz;
         u32x4 w[T], x[TM];
 #pragma unroll
-        for (int n = 0; n < T; ++n) w[n] = ws[n * 256 + at];
+        for (int n = 0; n < T; ++n) w[n] = ws[n * 32 * UPS + at];
 #pragma unroll
-        for (int m = 0; m < TM; ++m) x[m] = xs[m * 256 + at];
+        for (int m = 0; m < TM; ++m) x[m] = xs[m * 32 * UPS + at];
         if (!WHOLE && 2 * ks + 1 >= left && g == 1) {
 #pragma unroll
           for (int n = 0; n < T; ++n) w[n] = u32x4{0u, 0u, 0u, 0u};
@@ -366,13 +428,13 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
 #pragma unroll
           for (int n = 0; n < T; ++n) to[m][n] = E::mma(w[n], x[m], to[m][n]);
       }
-      cur ^= STAGE;
+      cur = cur + STAGE == RING * STAGE ? 0 : cur + STAGE;
     };
     auto reduce = [&](auto &to, auto tn_, int units, int wrow) {
 #pragma clang loop unroll(disable)
-      for (; units >= 8; units -= 8) {
+      for (; units >= UPS; units -= UPS) {
         next_stage();
-        multiply(to, tn_, std::true_type{}, 8, wrow);
+        multiply(to, tn_, std::true_type{}, UPS, wrow);
       }
       if (units > 0) {
         next_stage();
@@ -384,44 +446,73 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
 
     // ---- what follows the product, in registers ----
     const int tm = t / a.nt, tn = t - tm * a.nt;
+    const float *side = reinterpret_cast<const float *>(smem) + RING * STAGE / 4 + cside * SIDE;
+    cside = cside + 1 == RING ? 0 : cside + 1;
+    const int64_t m0 = (int64_t)tm * BM;
+    const int have = (int)(a.M - m0 < BM ? a.M - m0 : BM);
+    auto rows_at = [&](const void *p, int64_t ld) {  // the tile's rows of an output; past them loads give zero, stores are dropped
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform(static_cast<const char *>(p) + m0 * ld * sizeof(TO))), 0,
+                                               (int)(have * ld * sizeof(TO)), 0x00027000);
+    };
+    const TO *type = nullptr;
+    auto bias_of = [&](int n) { return side + (wn * TN + n) * 32; };  // of the wave's n-th tile of weight rows
+    auto scale_of = [&](int n) { return side + BN + (wn * TN + n) * 32; };
+    stored = KIND != kPlain || a.vec;
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
-      const int64_t row = (int64_t)tm * BM + (wm * TM + m) * 32 + i;
-      const bool ok = row < a.M;
-      const float sx = E::kBytes == 1 ? a.sx[ok ? row : a.M - 1] : 1.f;
+      const int rl = (wm * TM + m) * 32 + i;  // row of the tile
+      const float sx = E::kBytes == 1 ? side[2 * BN + rl] : 1.f;
+      const unsigned at = (unsigned)(rl * a.ldo * sizeof(TO));
       if constexpr (KIND == kPlain) {
+        if (a.vec) {
+          const Buffer out = rows_at(a.out, a.ldo);
+          // the residual's loads run one tile ahead
+          Quad<TO> add[2][4];
+          const Buffer res = rows_at(a.residual ? a.residual : a.out, a.ldo);
+          auto ask = [&](int n) {
+            if (a.residual) {
 #pragma unroll
-        for (int n = 0; n < TN; ++n) {
-          const int col = tn * CN + (wn * TN + n) * 32;
-          f32x16 v = values_of<E>(acc[m][n], a, 0, col, g, sx);
-          act_values(a.act, v);
-          TO *out = static_cast<TO *>(a.out) + row * a.ldo;
-          if (a.residual) {
-            const TO *res = static_cast<const TO *>(a.residual) + row * a.ldo;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int c = col + 8 * q + 4 * g;
-              f32x4 add = {0.f, 0.f, 0.f, 0.f};
-              if (a.vec) {
-                if (ok && c < a.N) add = widen4(res + c);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (ok && c + j < a.N) add[j] = load_as_f32(res + c + j);
+              for (int q = 0; q < 4; ++q) {
+                const int c = tn * CN + (wn * TN + n) * 32 + 8 * q + 4 * g;
+                add[n & 1][q].load(res, c < a.N ? at + (unsigned)sizeof(TO) * c : kNowhere);
               }
+            }
+          };
+          ask(0);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) v[4 * q + j] += add[j];
+          for (int n = 0; n < TN; ++n) {
+            if (n + 1 < TN) ask(n + 1);
+            f32x16 v = values_of<E>(acc[m][n], bias_of(n), scale_of(n), g, sx);
+            act_values(a.act, v);
+            if (a.residual) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] += add[n & 1][r / 4][r % 4];
+            }
+            store_tile(v, out, at, tn * CN + (wn * TN + n) * 32, a.N, g, type);
+          }
+        } else {  // rows that are not whole units: element by element
+          const int64_t row = m0 + rl;
+#pragma unroll
+          for (int n = 0; n < TN; ++n) {
+            f32x16 v = values_of<E>(acc[m][n], bias_of(n), scale_of(n), g, sx);
+            act_values(a.act, v);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int c = tn * CN + (wn * TN + n) * 32 + rowmap(r, g);
+              if (rl < have && c < a.N) {
+                const float add = a.residual ? load_as_f32(static_cast<const TO *>(a.residual) + row * a.ldo + c) : 0.f;
+                store_from_f32(static_cast<TO *>(a.out) + row * a.ldo + c, v[r] + add);
+              }
             }
           }
-          if (a.vec) store_tile<true>(v, out, col, a.N, g, ok);
-          else store_tile<false>(v, out, col, a.N, g, ok);
         }
       } else {
+        const Buffer out = rows_at(a.out, a.ldo);
 #pragma unroll
         for (int n = 0; n < TN2; ++n) {
           const int col = tn * CN + (wn * TN2 + n) * 32;
-          f32x16 gate = values_of<E>(acc[m][2 * n], a, 0, col, g, sx);
-          f32x16 up = values_of<E>(acc[m][2 * n + 1], a, 1, col, g, sx);
+          f32x16 gate = values_of<E>(acc[m][2 * n], bias_of(2 * n), scale_of(2 * n), g, sx);
+          f32x16 up = values_of<E>(acc[m][2 * n + 1], bias_of(2 * n + 1), scale_of(2 * n + 1), g, sx);
           const bool whole = col + 32 <= a.N;
           auto cut = [&](f32x16 &v) {  // weight rows past the last one were repeated
             if (!whole) {
@@ -434,8 +525,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) gate[r] *= up[r];
             cut(gate);
-            store_tile<true>(gate, static_cast<TO *>(a.out) + row * a.ldo, col, a.limit, g, ok);
+            store_tile(gate, out, at, col, a.limit, g, type);
           } else {
+            const Buffer hidden = rows_at(a.out2, a.ldh);
             f32x16 slope, d = acc2[m][n];
             act_slopes(a.act, gate, slope);
             f32x16 h;
@@ -446,32 +538,53 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void rows_tile_kernel(Args a) {
               gate[r] *= d[r];
             }
             cut(h), cut(slope), cut(gate);
-            TO *out = static_cast<TO *>(a.out) + row * a.ldo;
-            store_tile<true>(slope, out, col, a.limit, g, ok);
-            store_tile<true>(gate, out + a.ldh, col, a.limit, g, ok);
-            store_tile<true>(h, static_cast<TO *>(a.out2) + row * a.ldh, col, a.limit, g, ok);
+            store_tile(slope, out, at, col, a.limit, g, type);
+            store_tile(gate, out, at + (unsigned)(a.ldh * sizeof(TO)), col, a.limit, g, type);
+            store_tile(h, hidden, (unsigned)(rl * a.ldh * sizeof(TO)), col, a.limit, g, type);
           }
         }
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is landing in LDS when the workgroup ends
 }
 
-template <class E, class TO, Kind KIND, int WM, int WN, int TM, int TN, int OCC>
+template <class E, class TO, Kind KIND, class CFG>
 int launch_tiles(Args a, int num_cu, hipStream_t st) {
-  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, CN = KIND == kPlain ? BN : BN / 2;
-  constexpr size_t lds = 2 * (BM + BN) * 128;
-  const int64_t mt = (a.M + BM - 1) / BM, nt = (a.N + CN - 1) / CN;
+  constexpr int CN = KIND == kPlain ? CFG::BN : CFG::BN / 2;
+  constexpr size_t lds = CFG::lds(E::kBytes);
+  static_assert(lds <= kMaxLdsBytes, "the ring fits a workgroup");
+  const int64_t mt = (a.M + CFG::BM - 1) / CFG::BM, nt = (a.N + CN - 1) / CN;
   if (mt * nt > (int64_t)1 << 30) return PA_ERR_UNSUPPORTED;
   a.mt = (int)mt, a.nt = (int)nt;
-  const int per_cu = (int)(kMaxLdsBytes / lds) < OCC * 4 / (WM * WN) ? (int)(kMaxLdsBytes / lds) : OCC * 4 / (WM * WN);
+  constexpr int by_lds = (int)(kMaxLdsBytes / lds), by_waves = CFG::OCC * 4 / CFG::WAVES, per_cu = by_lds < by_waves ? by_lds : by_waves;
   int64_t grid = (int64_t)num_cu * (per_cu < 1 ? 1 : per_cu);
   if (grid > mt * nt) grid = mt * nt;
   grid = (grid + 7) / 8 * 8;  // every XCD the same number
-  auto kernel = rows_tile_kernel<E, TO, KIND, WM, WN, TM, TN, OCC>;
+  auto kernel = rows_tile_kernel<E, TO, KIND, CFG>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WM * WN), lds, st, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * CFG::WAVES), lds, st, a);
   return launch_status();
+}
+
+// Tiles of 256 x 256 (kBack: 128 x 256) for large products, 128 x 128 and two workgroups per CU where those leave CUs idle, 64 x 64
+// where the product is small.  Taken by the weight rows and rows that the busiest CU has to work off, smaller tiles counted
+// dearer for the operands they fetch again.  Measured at 256 / 128 (us): 131 072 rows, 1 024 -> 256 bf16 107 / 117, 2 048 -> 256
+// 162 / 189, 256 -> 2 x 1 024 201 / 227; 100 003 rows, 1 368 -> 512 247 / 234; int8 131 072 rows 2 048 -> 512 144 / 193; float32
+// 28 900 rows, 512 -> 128 126 / 43.
+template <class E, class TO, Kind KIND>
+int launch(const Args &a, int num_cu, hipStream_t st) {
+  using Large = typename std::conditional<KIND == kBack, Config<2, 4, 2, 2, 8, 3, 2>, Config<4, 2, 2, 4, 8, 2, 2>>::type;
+  using Medium = Config<2, 2, 2, 2, 8, 2, 2>;
+  using Small = Config<2, 1, 1, 2, 8, 3, 2>;
+  auto cost = [&](int64_t bm, int64_t bn, double dearer) {
+    const int64_t cn = KIND == kPlain ? bn : bn / 2, tiles = ((a.M + bm - 1) / bm) * ((a.N + cn - 1) / cn);
+    return (double)((tiles + num_cu - 1) / num_cu) * bm * bn * dearer;
+  };
+  const double l = cost(Large::BM, Large::BN, 1.0), m = cost(Medium::BM, Medium::BN, 1.13), s = cost(Small::BM, Small::BN, 1.5);
+  if (l <= m && l <= s) return launch_tiles<E, TO, KIND, Large>(a, num_cu, st);
+  if (m <= s) return launch_tiles<E, TO, KIND, Medium>(a, num_cu, st);
+  return launch_tiles<E, TO, KIND, Small>(a, num_cu, st);
 }
 
 // ---- host side of the calls that use the products ----
