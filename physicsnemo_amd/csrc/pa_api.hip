@@ -1982,7 +1982,8 @@ int pa_int8_quantize_rows(int dtype, int64_t rows, int64_t K, const void *x, voi
   if (ldq > 2 * K + 4096) return PA_ERR_UNSUPPORTED;
   if (!x || !q || !scale) return PA_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(q) % 8 != 0) return PA_ERR_ALIGN;
-  return pa::int8::quantize_rows(dtype, rows, K, x, K, q, ldq, scale, static_cast<hipStream_t>(stream));
+  return pa::int8::quantize_rows(dtype, rows, K, x, K, q, ldq, scale, compute_units(),
+                                 static_cast<hipStream_t>(stream));
 }
 
 int64_t pa_int8_linear_workspace_bytes(int dtype, int64_t rows, int64_t K, int64_t N) {

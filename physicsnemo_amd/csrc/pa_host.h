@@ -171,7 +171,8 @@ int backward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &
 namespace int8 {
 // products of 8-bit integers: see pa_int8_*
 bool supported(int dtype, int64_t M, int64_t K, int64_t N);
-int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, hipStream_t st);
+int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, int num_cu,
+                  hipStream_t st);
 int64_t linear_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, const float *w_scale, const float *bias, int act, const void *x,
            const void *residual, void *y, void *workspace, int num_cu, hipStream_t st);

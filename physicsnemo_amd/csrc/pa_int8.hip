@@ -45,10 +45,34 @@ __device__ __forceinline__ void load8(const float *p, int64_t left, float (&v)[8
   }
 }
 
+// largest value over groups of LANES neighbouring lanes, in every lane
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  auto larger = [](uint32_t x, uint32_t y) { return x > y ? x : y; };
+  auto step = [&](uint32_t x, auto ctrl) {
+    constexpr int c = decltype(ctrl)::value;
+    return larger(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, c, 0xf, 0xf, true));
+  };
+  v = step(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  v = step(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  v = step(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v = step(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  if constexpr (LANES >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = larger(r[0], r[1]);
+  }
+  return v;
+}
+
 // ---------------------------------------------------------------------------------------------------------------
-// quantize_rows_kernel: a wave per row, eight elements per lane and step; rows of up to 512 NCH elements stay in registers
-// between the maximum and the rounding, longer ones are read again.  The maximum runs over the bits of |x|, in which NaN lies
-// above infinity above the numbers: a row with one of them gets scale NaN, which is what a product with it would be.
+// quantize_rows_kernel: LANES lanes per row, eight elements per lane and step; rows of up to 8 LANES NCH elements stay in
+// registers between the maximum and the rounding, longer ones are read again.  A wave has ROWS sets of rows in flight.  The
+// maximum runs over the bits of |x|, in which NaN lies above infinity above the numbers: a row with one of them gets scale NaN,
+// which is what a product with it would be.  Bound by HBM.
 // ---------------------------------------------------------------------------------------------------------------
 struct Quantize {
   const void *x;
@@ -57,61 +81,69 @@ struct Quantize {
   float *scale;
 };
 
-template <class T, int NCH, bool VEC>
+template <class T, int LANES, int NCH, int ROWS, bool VEC>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(Quantize a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= a.M) return;
-  const T *x = static_cast<const T *>(a.x) + row * a.ldx;
-  float v[NCH][8];
-  uint32_t most = 0;
-  auto larger = [&](const float (&w)[8]) {
+  constexpr int SPAN = LANES * 8, PER = 256 / LANES;  // elements of a step; rows of a workgroup
+  const int lane = threadIdx.x % LANES, first = threadIdx.x / LANES;
+  const T *x = static_cast<const T *>(a.x);
+  const int64_t stride = (int64_t)gridDim.x * PER;
+  for (int64_t base = (int64_t)blockIdx.x * PER + first; base < a.M; base += ROWS * stride) {
+    float v[ROWS][NCH][8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t b = __float_as_uint(w[j]) & 0x7fffffffu;
-      most = b > most ? b : most;
+    for (int r = 0; r < ROWS; ++r) {
+      const int64_t row = base + r * stride;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) {
+        const int64_t k = c * SPAN + lane * 8;
+        load8<VEC>(x + row * a.ldx + k, row < a.M ? a.K - k : 0, v[r][c]);
+      }
     }
-  };
 #pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int64_t k = c * 512 + lane * 8;
-    load8<VEC>(x + k, a.K - k, v[c]);
-    larger(v[c]);
-  }
-  for (int64_t k = NCH * 512 + lane * 8; k < a.K; k += 512) {
-    float w[8];
-    load8<VEC>(x + k, a.K - k, w);
-    larger(w);
-  }
+    for (int r = 0; r < ROWS; ++r) {
+      const int64_t row = base + r * stride;
+      if (row >= a.M) break;
+      uint32_t most = 0;
+      auto larger = [&](const float (&w)[8]) {
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const uint32_t b = (uint32_t)__shfl_xor((int)most, off, 64);
-    most = b > most ? b : most;
-  }
-  const bool finite = most < 0x7f800000u;
-  const float top = __uint_as_float(most);
-  const float lift = top < 0x1p-100f ? 0x1p100f : 1.f;  // 127 / top stays finite
-  const float inv = finite && most > 0 ? 127.f / (top * lift) : 0.f;
-  auto store = [&](int64_t k, const float (&w)[8]) {
-    if (k >= a.ldq) return;
-    u32x2 out = {0u, 0u};
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __float_as_uint(w[j]) & 0x7fffffffu;
+          most = b > most ? b : most;
+        }
+      };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float r = fminf(fmaxf(rintf(w[j] * lift * inv), -127.f), 127.f);
-      const uint32_t code = finite ? (uint32_t)((int)r & 0xff) : 0u;
-      if (j < 4) out[0] |= code << (8 * j);
-      else out[1] |= code << (8 * (j - 4));
+      for (int c = 0; c < NCH; ++c) larger(v[r][c]);
+      for (int64_t k = NCH * SPAN + lane * 8; k < a.K; k += SPAN) {
+        float w[8];
+        load8<VEC>(x + row * a.ldx + k, a.K - k, w);
+        larger(w);
+      }
+      most = lanes_max<LANES>(most);
+      const bool finite = most < 0x7f800000u;
+      const float top = __uint_as_float(most);
+      const float lift = top < 0x1p-100f ? 0x1p100f : 1.f;  // 127 / top stays finite
+      const float inv = finite && most > 0 ? 127.f / (top * lift) : 0.f;
+      auto store = [&](int64_t k, const float (&w)[8]) {
+        if (k >= a.ldq) return;
+        u32x2 out = {0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float r = fminf(fmaxf(rintf(w[j] * lift * inv), -127.f), 127.f);
+          const uint32_t code = finite ? (uint32_t)((int)r & 0xff) : 0u;
+          if (j < 4) out[0] |= code << (8 * j);
+          else out[1] |= code << (8 * (j - 4));
+        }
+        *reinterpret_cast<u32x2 *>(a.q + row * a.ldq + k) = out;
+      };
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) store(c * SPAN + lane * 8, v[r][c]);
+      for (int64_t k = NCH * SPAN + lane * 8; k < a.ldq; k += SPAN) {
+        float w[8];
+        load8<VEC>(x + row * a.ldx + k, a.K - k, w);
+        store(k, w);
+      }
+      if (lane == 0) a.scale[row] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
     }
-    *reinterpret_cast<u32x2 *>(a.q + row * a.ldq + k) = out;
-  };
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) store(c * 512 + lane * 8, v[c]);
-  for (int64_t k = NCH * 512 + lane * 8; k < a.ldq; k += 512) {
-    float w[8];
-    load8<VEC>(x + k, a.K - k, w);
-    store(k, w);
   }
-  if (lane == 0) a.scale[row] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
 }
 
 static constexpr int64_t kMaxTerms = 131072;  // 127 x 127 of them stay below 2^31
@@ -120,22 +152,27 @@ bool supported(int dtype, int64_t M, int64_t K, int64_t N) {
   return (dtype == PA_F32 || dtype == PA_BF16) && M > 0 && K > 0 && N > 0 && M <= (int64_t)1 << 32 && K <= kMaxTerms && N <= 1 << 18;
 }
 
-template <class T>
-static int quantize(const Quantize &a, bool vec, hipStream_t st) {
-  const int64_t blocks = (a.M + 3) / 4;
-  if (blocks > 0x7fffffff) return PA_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)blocks), wg(256);
-  if (vec && a.K <= 512) hipLaunchKernelGGL((quantize_rows_kernel<T, 1, true>), grid, wg, 0, st, a);
-  else if (vec) hipLaunchKernelGGL((quantize_rows_kernel<T, 4, true>), grid, wg, 0, st, a);
-  else if (a.K <= 512) hipLaunchKernelGGL((quantize_rows_kernel<T, 1, false>), grid, wg, 0, st, a);
-  else hipLaunchKernelGGL((quantize_rows_kernel<T, 4, false>), grid, wg, 0, st, a);
-  return launch_status();
+template <class T, bool VEC>
+static int quantize(const Quantize &a, int num_cu, hipStream_t st) {
+  auto go = [&](auto kernel, int64_t per) {
+    int64_t grid = (a.M + per - 1) / per;
+    if (grid > 8 * (int64_t)num_cu) grid = 8 * (int64_t)num_cu;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
+    return launch_status();
+  };
+  const int64_t w = a.ldq;  // zeros behind the last element are written by the lanes that would hold them
+  if (w <= 128) return go(quantize_rows_kernel<T, 16, 1, 4, VEC>, 16);
+  if (w <= 256) return go(quantize_rows_kernel<T, 32, 1, 4, VEC>, 8);
+  if (w <= 512) return go(quantize_rows_kernel<T, 64, 1, 4, VEC>, 4);
+  return go(quantize_rows_kernel<T, 64, 4, 1, VEC>, 4);
 }
 
-int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, hipStream_t st) {
+int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, int num_cu,
+                  hipStream_t st) {
   const Quantize a{x, M, K, ldx, ldq, static_cast<uint8_t *>(q), scale};
   const bool vec = whole_rows(x, ldx, dtype == PA_F32 ? 4 : 2);
-  return dtype == PA_F32 ? quantize<float>(a, vec, st) : quantize<bf16>(a, vec, st);
+  if (dtype == PA_F32) return vec ? quantize<float, true>(a, num_cu, st) : quantize<float, false>(a, num_cu, st);
+  return vec ? quantize<bf16, true>(a, num_cu, st) : quantize<bf16, false>(a, num_cu, st);
 }
 
 template <class TO, tile::Kind KIND>
@@ -168,7 +205,7 @@ static int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, con
   const void *codes = codes_of(w, N, K, bytes != nullptr, ws, lay);
   if (bytes) return *bytes = ws.used, PA_OK;
   int rc = tile::lay_out(lay, 1, st);
-  if (!rc) rc = quantize_rows(dtype, M, K, x, K, q.q, up(K, 16), q.scale, st);
+  if (!rc) rc = quantize_rows(dtype, M, K, x, K, q.q, up(K, 16), q.scale, num_cu, st);
   if (rc) return rc;
   Args a{};
   a.X = q.q, a.ldx = a.ldw = up(K, 16), a.units = (int)(up(K, 16) / 16);
@@ -208,7 +245,7 @@ static int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated
              *down = codes_of(p.w_down, C, F, plan, ws, lay);
   if (plan) return *bytes = ws.used, PA_OK;
   int rc = tile::lay_out(lay, 1, st);
-  if (!rc) rc = quantize_rows(dtype, M, C, x, C, qx.q, Kc, qx.scale, st);
+  if (!rc) rc = quantize_rows(dtype, M, C, x, C, qx.q, Kc, qx.scale, num_cu, st);
   if (rc) return rc;
   Args a{};
   a.X = qx.q, a.ldx = a.ldw = Kc, a.units = (int)(Kc / 16);
@@ -218,7 +255,7 @@ static int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated
   a.sx = qx.scale, a.sw[0] = p.s_gate, a.sw[1] = p.s_up;
   a.out = h, a.ldo = Fp, a.act = act;
   if ((rc = product<TO, tile::kGated>(a, num_cu, st))) return rc;
-  if ((rc = quantize_rows(dtype, M, F, h, Fp, qh.q, Kf, qh.scale, st))) return rc;
+  if ((rc = quantize_rows(dtype, M, F, h, Fp, qh.q, Kf, qh.scale, num_cu, st))) return rc;
   Args d{};
   d.X = qh.q, d.ldx = d.ldw = Kf, d.units = (int)(Kf / 16);
   d.W[0] = down;
