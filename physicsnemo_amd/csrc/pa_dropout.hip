@@ -62,39 +62,50 @@ __device__ __forceinline__ void apply(const Mask &m, const Stream &s, int64_t ro
   }
 }
 
-// ---- VEC neighbouring elements of a row; VEC = 16 bytes of them: rows are whole units, else element by element ----
+// ---- VEC neighbouring elements of a row, 16 bytes; UNITS: rows are whole 16-byte units.  Rows that are not start on any
+// element: the same 16-byte accesses without that alignment, element by element at a row's end ----
+typedef u32x4 unit_at4 __attribute__((aligned(4)));
+typedef u32x4 unit_at2 __attribute__((aligned(2)));
+template <class T, bool UNITS>
+using UnitAt = typename std::conditional<UNITS, u32x4, typename std::conditional<sizeof(T) == 4, unit_at4, unit_at2>::type>::type;
+
 template <class T, int VEC, bool UNITS>
 __device__ __forceinline__ void load(const T *row, int col, int C, float (&v)[VEC]) {
-  if constexpr (UNITS && sizeof(T) == 2) {
-    u32x4 w = {0u, 0u, 0u, 0u};
-    if (col < C) w = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(row + col));
+  static_assert(VEC * sizeof(T) == 16, "one access");
+  typedef UnitAt<T, UNITS> unit_at;
+  u32x4 w = {0u, 0u, 0u, 0u};
+  if (UNITS ? col < C : col + VEC <= C) {
+    w = __builtin_nontemporal_load(reinterpret_cast<const unit_at *>(row + col));
+  } else if (!UNITS && col < C) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t b = w[j];
-      v[2 * j] = __uint_as_float(b << 16), v[2 * j + 1] = __uint_as_float(b & 0xffff0000u);
+    for (int j = 0; j < VEC; ++j) {
+      if constexpr (sizeof(T) == 2) w[j / 2] |= (col + j < C ? (uint32_t)row[col + j].bits : 0u) << (16 * (j & 1));
+      else w[j] = col + j < C ? __float_as_uint(row[col + j]) : 0u;
     }
-  } else if constexpr (UNITS) {
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    f32x4 w = {0.f, 0.f, 0.f, 0.f};
-    if (col < C) w = __builtin_nontemporal_load(reinterpret_cast<const f32x4 *>(row + col));
+  }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = w[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = col + j < C ? load_as_f32(row + col + j) : 0.f;
+  for (int j = 0; j < VEC; ++j) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t b = w[j / 2];
+      v[j] = __uint_as_float(j & 1 ? b & 0xffff0000u : b << 16);
+    } else {
+      const uint32_t b = w[j];
+      v[j] = __uint_as_float(b);
+    }
   }
 }
 template <class T, int VEC, bool UNITS>
 __device__ __forceinline__ void store(T *row, int col, int C, const float (&v)[VEC]) {
-  if constexpr (UNITS && sizeof(T) == 2) {
+  typedef UnitAt<T, UNITS> unit_at;
+  if (UNITS ? col < C : col + VEC <= C) {
     u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = mfma::pack2(v[2 * j], v[2 * j + 1]);
-    if (col < C) __builtin_nontemporal_store(w, reinterpret_cast<u32x4 *>(row + col));
-  } else if constexpr (UNITS) {
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    if (col < C) __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, reinterpret_cast<f32x4 *>(row + col));
-  } else {
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 2) w[j] = mfma::pack2(v[2 * j], v[2 * j + 1]);
+      else w[j] = __float_as_uint(v[j]);
+    }
+    __builtin_nontemporal_store(w, reinterpret_cast<unit_at *>(row + col));
+  } else if (!UNITS) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j)
       if (col + j < C) store_from_f32(row + col + j, v[j]);
@@ -455,7 +466,7 @@ static Shape shape_of(int dtype, int64_t C, bool aligned) {
   Shape s{};
   const int per = dtype == PA_F32 ? 4 : 8;
   s.units = aligned && C % per == 0;
-  s.vec = s.units ? per : 4;
+  s.vec = per;
   const int64_t q = (C + s.vec - 1) / s.vec;
   if (q <= 64) {
     s.pieces = 1;
@@ -515,7 +526,7 @@ static int launch(const Args &a, const Shape &s, bool forward, bool norm, int nu
 
 static int launch(int dtype, const Args &a, const Shape &s, bool forward, bool norm, int num_cu, hipStream_t st) {
   if (dtype == PA_F32) return s.units ? launch<float, 4, true>(a, s, forward, norm, num_cu, st) : launch<float, 4, false>(a, s, forward, norm, num_cu, st);
-  return s.units ? launch<bf16, 8, true>(a, s, forward, norm, num_cu, st) : launch<bf16, 4, false>(a, s, forward, norm, num_cu, st);
+  return s.units ? launch<bf16, 8, true>(a, s, forward, norm, num_cu, st) : launch<bf16, 8, false>(a, s, forward, norm, num_cu, st);
 }
 
 int advance(int64_t *state, int64_t *taken, hipStream_t st) {
