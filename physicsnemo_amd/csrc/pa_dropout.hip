@@ -131,6 +131,17 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// the same over the 256 lanes of a workgroup, through four floats of LDS; all of it calls this
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, float *red) {
+  if constexpr (LANES <= 64) return lanes_sum<LANES>(v);
+  v = lanes_sum<64>(v);
+  __syncthreads();  // the sum before has been read
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 struct Args {
   const void *x, *residual, *y, *dy, *dn;
   void *out_y, *out_n, *dx, *d_residual;
@@ -144,7 +155,7 @@ struct Args {
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// rows_forward_kernel, rows_backward_kernel.  LANES lanes share a row, each NCH pieces of VEC neighbouring columns, so that a row
+// rows_forward_kernel, rows_backward_kernel.  LANES lanes (256: the workgroup) share a row, each NCH pieces of VEC neighbouring columns, so that a row
 // is read once and stays in registers; a workgroup of four waves walks the rows.  In the backward pass a lane adds d gamma and d beta
 // of its columns up over all its rows; the workgroup's sums become one partial result, added up in a fixed order by one more
 // small launch.  Bound by HBM: (3 + norm) element reads and writes forward, 5 backward; the generator's twenty 32 x 32 bit
@@ -152,6 +163,7 @@ struct Args {
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int VEC, bool UNITS, int LANES, int NCH, bool NORM>
 __global__ __launch_bounds__(256) void rows_forward_kernel(Args a) {
+  __shared__ float wide[4];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   constexpr int ROWS = 256 / LANES;
   const int C = a.C;
@@ -189,7 +201,7 @@ __global__ __launch_bounds__(256) void rows_forward_kernel(Args a) {
       for (int j = 0; j < VEC; ++j) sum += s[k][j];
     }
     if constexpr (NORM) {
-      const float mean = lanes_sum<LANES>(sum) * inv;
+      const float mean = group_sum<LANES>(sum, wide) * inv;
       float sq = 0.f;
 #pragma unroll
       for (int k = 0; k < NCH; ++k)
@@ -198,7 +210,7 @@ __global__ __launch_bounds__(256) void rows_forward_kernel(Args a) {
           const float d = (k * LANES + lane) * VEC + j < C ? s[k][j] - mean : 0.f;
           sq = fmaf(d, d, sq);
         }
-      const float rstd = 1.f / sqrtf(lanes_sum<LANES>(sq) * inv + a.eps);
+      const float rstd = 1.f / sqrtf(group_sum<LANES>(sq, wide) * inv + a.eps);
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         float n[VEC];
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(256) void rows_forward_kernel(Args a) {
 template <class T, int VEC, bool UNITS, int LANES, int NCH, bool NORM>
 __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
   constexpr int ROWS = 256 / LANES, WIDE = LANES * NCH * VEC;
-  __shared__ float red[NORM ? 4 * WIDE : 1];
+  __shared__ float red[NORM && LANES <= 64 ? 4 * WIDE : 4];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int C = a.C;
   const float inv = 1.f / (float)C;
@@ -262,8 +274,8 @@ __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
           s2 = fmaf(t[k][j], xh[k][j], s2);
         }
       }
-      s1 = lanes_sum<LANES>(s1) * inv;
-      s2 = lanes_sum<LANES>(s2) * inv;
+      s1 = group_sum<LANES>(s1, red) * inv;
+      s2 = group_sum<LANES>(s2, red) * inv;
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
 #pragma unroll
@@ -282,6 +294,16 @@ __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
   }
   if constexpr (NORM) {
     if (!a.partials) return;
+    if constexpr (LANES > 64) {  // a column is one lane's
+#pragma unroll
+      for (int k = 0; k < NCH; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int c = (k * LANES + lane) * VEC + j;
+          if (c < C) a.partials[(int64_t)blockIdx.x * 2 * C + c] = dg[k][j], a.partials[((int64_t)blockIdx.x * 2 + 1) * C + c] = db[k][j];
+        }
+      return;
+    }
     const int wave = threadIdx.x >> 6;
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
@@ -471,9 +493,9 @@ static Shape shape_of(int dtype, int64_t C, bool aligned) {
   if (q <= 64) {
     s.pieces = 1;
     for (s.lanes = 8; s.lanes < q; s.lanes *= 2) {}
-  } else if (q <= 512) {
-    s.lanes = 64;
-    s.pieces = q <= 128 ? 2 : q <= 256 ? 4 : 8;
+  } else if (q <= 1024) {
+    s.lanes = q <= 256 ? 64 : 256;
+    s.pieces = q <= 128 || (q > 256 && q <= 512) ? 2 : 4;
   }
   return s;
 }
@@ -509,7 +531,8 @@ static int launch(const Args &a, const Shape &s, bool forward, bool norm, int nu
   else if (s.lanes == 64 && s.pieces == 1) launch_rows<T, VEC, UNITS, 64, 1>(a, forward, norm, grid, st);
   else if (s.lanes == 64 && s.pieces == 2) launch_rows<T, VEC, UNITS, 64, 2>(a, forward, norm, grid, st);
   else if (s.lanes == 64 && s.pieces == 4) launch_rows<T, VEC, UNITS, 64, 4>(a, forward, norm, grid, st);
-  else if (s.lanes == 64) launch_rows<T, VEC, UNITS, 64, 8>(a, forward, norm, grid, st);
+  else if (s.lanes == 256 && s.pieces == 2) launch_rows<T, VEC, UNITS, 256, 2>(a, forward, norm, grid, st);
+  else if (s.lanes == 256) launch_rows<T, VEC, UNITS, 256, 4>(a, forward, norm, grid, st);
   else {
     const dim3 g((unsigned)grid), b(kWideThreads);
     if (forward && norm) hipLaunchKernelGGL((long_rows_forward_kernel<T, VEC, UNITS, true>), g, b, 0, st, a);
