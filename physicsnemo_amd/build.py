@@ -16,7 +16,7 @@ OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libphysattn.so")
 SOURCES = ["pa_api.hip", "pa_general.hip", "pa_mfma.hip", "pa_mlp.hip", "pa_mlp_bwd.hip", "pa_norm_bwd.hip", "pa_backward.hip", "pa_gemm.hip", "pa_wgrad.hip", "pa_train.hip", "pa_train_f32.hip", "pa_mfma_bwd.hip",
            "pa_layer_point.hip", "pa_mfma_staged.hip", "pa_gale.hip", "pa_flare.hip", "pa_ball_query.hip", "pa_noalloc.hip", "pa_conv.hip", "pa_rows_f32.hip", "pa_narrow_f32.hip", "pa_points_f32.hip",
-           "pa_gated.hip", "pa_int8.hip", "pa_dropout.hip"]
+           "pa_gated.hip", "pa_gated_rows.hip", "pa_int8.hip", "pa_dropout.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
@@ -25,7 +25,7 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 # flags of single files; the reason stands at the top of the file
-FILE_FLAGS = {"pa_layer_point.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {"pa_layer_point.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "pa_gated_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _headers_mtime() -> float:

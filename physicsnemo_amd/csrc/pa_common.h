@@ -81,14 +81,18 @@ __device__ __forceinline__ float gelu_grad(float x, const GeluParts &p) { return
 // The same from one transcendental instruction: Phi(-a) = 2^P(a), a = |x|, P of degree 6 fitted to log2 Phi(-a) over 0 <= a <= 6
 // for the smallest error of a Phi(-a), and GELU(x) = max(x, 0) - a Phi(-a).  GELU is within 2.5e-7 of the exact one everywhere.  P has its
 // turning point past 12; at 10, where a stops, a Phi(-a) is 1e-20.
-__device__ __forceinline__ float gelu_lower_tail(float a) {  // Phi(-a), 0 <= a <= 10
+__device__ __forceinline__ float gelu_lower_tail_upper_terms(float a) {
   float p = fmaf(3.2733779e-05f, a, -7.60096567e-04f);
   p = fmaf(p, a, 8.03007988e-03f);
-  p = fmaf(p, a, -5.32984358e-02f);
+  return fmaf(p, a, -5.32984358e-02f);
+}
+__device__ __forceinline__ float gelu_lower_tail_lower_terms(float a, float p) {
   p = fmaf(p, a, -4.58887012e-01f);
   p = fmaf(p, a, -1.15115055f);
-  p = fmaf(p, a, -1.0000004f);
-  return __builtin_amdgcn_exp2f(p);
+  return fmaf(p, a, -1.0000004f);
+}
+__device__ __forceinline__ float gelu_lower_tail(float a) {  // Phi(-a), 0 <= a <= 10
+  return __builtin_amdgcn_exp2f(gelu_lower_tail_lower_terms(a, gelu_lower_tail_upper_terms(a)));
 }
 __device__ __forceinline__ float gelu_tail_arg(float x) { return fabsf(x) > 10.f ? 10.f : fabsf(x); }  // NaN stays
 __device__ __forceinline__ float gelu_tail(float x) {

@@ -2,7 +2,8 @@
 //   h  = act(g) u                     g = W_gate x + b_gate,  u = W_up x + b_up
 //   dh = W_down^T dy                  dg = dh u act'(g),      du = dh act(g)
 //   dx = W_gate^T dg + W_up^T du,     d W_gate = dg^T x, d W_up = du^T x, d W_down = dy^T h, d b = column sums
-// Both input products, the activation and the factor are one kernel (kGated); the backward forms g and u again beside dh
+// Both input products, the activation and the factor are one kernel (kGated); for many bf16 rows of up to 256 channels all three
+// products are (pa_gated_rows.hip).  The backward forms g and u again beside dh
 // (kBack: 4 C F operations per row more, against 4 F elements per row written by the forward and read back), so the forward
 // leaves nothing behind.  Sums and all that happens between two products are float32; h, dg and du are rounded once, to the
 // activations' type, as operands of the next product.
@@ -146,6 +147,14 @@ static Rows rows_of(const void *p, int64_t rows, int64_t width, int64_t elem, bo
   return r;
 }
 
+// pa_gated_rows.hip
+bool rows_supported(int64_t C, int64_t F);
+int64_t rows_worth(int64_t M, int64_t C, int num_cu);
+int64_t rows_blob_bytes(int64_t C, int64_t F);
+int rows_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st);
+int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float *b_down, int act, const void *x, const void *residual,
+                 void *y, int num_cu, hipStream_t st);
+
 template <class E, class TO, tile::Kind KIND>
 static int product(const Args &a, int num_cu, hipStream_t st) {
   return tile::launch<E, TO, KIND>(a, num_cu, st);
@@ -162,6 +171,19 @@ static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, in
   Layout lay;
   const int64_t Fp = up(F, U);
   auto copied = [&](const void *q, int64_t width) { return plan || !whole_rows(q, width, e); };
+  int64_t done = 0;  // rows of the kernel that keeps the hidden layer on chip
+  if (e == 2 && C % 8 == 0 && rows_supported(C, F)) {
+    void *blob = ws.take(rows_blob_bytes(C, F));
+    if (!plan && aligned16(x) && aligned16(y) && aligned16(residual)) done = rows_worth(M, C, num_cu);
+    if (done > 0) {
+      int rc = rows_pack(C, F, p, blob, st);
+      if (!rc) rc = rows_forward(done, C, F, blob, p.b_down, act, x, residual, y, num_cu, st);
+      if (rc || done == M) return rc;
+    }
+  }
+  auto behind = [&](const void *q) { return q ? static_cast<const char *>(q) + done * C * e : nullptr; };
+  x = behind(x), residual = behind(residual), y = const_cast<char *>(behind(y));
+  M -= done;
   void *h = ws.take(M * Fp * e);
   const Rows xr = rows_of(x, M, C, e, copied(x, C), ws, &lay);
   const Rows wg = rows_of(p.w_gate, F, C, e, copied(p.w_gate, C), ws, &lay);

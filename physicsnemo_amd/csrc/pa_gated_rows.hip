@@ -1,0 +1,339 @@
+// The gated feed-forward block with the hidden layer on chip, bf16 rows of up to 256 channels (see pa_gated.hip for the formulas):
+// a wave owns 32 rows and all their channels, the weights stream past it in slots of 32 hidden units.  x is read once and y
+// written once, where the two products of the tile kernel pass 4 F bytes per row through memory.
+#include "pa_common.h"
+#include "pa_host.h"
+#include "pa_tile.h"
+
+namespace pa {
+namespace gated {
+
+using mfma::f32x16;
+using mfma::load_unit_to_lds;
+using mfma::mma;
+using mfma::pack2;
+using mfma::rowmap;
+using mfma::static_for;
+using mfma::u32x4;
+using tile::Buffer;
+
+__host__ __device__ __forceinline__ int chunks_of(int F) { return (F + 63) / 64 * 2; }
+
+// ---------------------------------------------------------------------------------------------------------------
+// rows_pack_kernel: slot c = 0 .. NCH of the weight stream (NCH: chunks of 32 hidden units, an even number), (6 CT + 1) KB: for every k-step the fragments of W_up's and W_gate's
+// rows 32 c .. + 31; then W_down's columns 32 (c - 1) .. + 31, k half major, its reduction index in the order in which the
+// hidden layer leaves the accumulators (kperm); then 32 biases of each of the two.  What lies outside the matrices is zero.
+// ---------------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void rows_pack_kernel(const uint16_t *__restrict__ wg, const uint16_t *__restrict__ wu,
+                                                        const uint16_t *__restrict__ wd, const float *__restrict__ bg,
+                                                        const float *__restrict__ bu, u32x4 *__restrict__ blob, int C, int F, int CT) {
+  const int KS = 2 * CT, SU = (6 * CT + 1) * 64, NCH = chunks_of(F);
+  const int64_t total = (int64_t)(NCH + 1) * SU;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
+    const int c = (int)(u / SU), r = (int)(u - (int64_t)c * SU), frag = r >> 6, lane = r & 63, i = lane & 31, g = lane >> 5;
+    u32x4 e = {0u, 0u, 0u, 0u};
+    if (frag < 2 * KS) {
+      const uint16_t *w = frag & 1 ? wg : wu;
+      const int row = 32 * c + i, col = 16 * (frag >> 1) + 8 * g;
+      if (row < F) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + j < C) e[j / 2] |= (uint32_t)w[(int64_t)row * C + col + j] << (16 * (j & 1));
+      }
+    } else if (frag < 2 * KS + 2 * CT) {
+      const int t = frag - 2 * KS, kk = t / CT, row = 32 * (t % CT) + i;
+      if (c > 0 && row < C) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int col = 32 * (c - 1) + mfma::kperm(kk, g, j);
+          if (col < F) e[j / 2] |= (uint32_t)wd[(int64_t)row * F + col] << (16 * (j & 1));
+        }
+      }
+    } else if (lane < 16) {
+      const float *b = lane < 8 ? bu : bg;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 32 * c + 4 * (lane & 7) + j;
+        if (b && at < F) e[j] = __float_as_uint(b[at]);
+      }
+    }
+    blob[u] = e;
+  }
+}
+
+struct RowsArgs {
+  const u32x4 *blob;
+  const uint16_t *x, *residual;
+  const float *b_down;
+  uint16_t *y;
+  int64_t M, nblocks;
+  int C, F, act;
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// rows_forward_kernel<CT>: rows of up to 32 CT channels.  Per slot c a wave runs
+//   u(c)^T = W_up[chunk c] x^T + b_up and g(c)^T = W_gate[chunk c] x^T + b_gate, in turn          4 CT MFMAs
+//     with h(c - 1) = act(g) u of the chunk before formed behind them, 16 values in 32 pieces; two sets of accumulators take turns
+//   y^T += W_down[:, chunk c - 1] h(c - 1)^T                                                      2 CT MFMAs
+// Two LDS buffers, one barrier per slot.  CT = 8: one wave per SIMD with 512 registers (y 128, x 64, two sets of g and u 64);
+// narrower rows: two.
+// ---------------------------------------------------------------------------------------------------------------
+// One value of h in four pieces, so that what a piece depends on lies a step of the matrix instructions behind it.
+template <int ACT>
+struct Gate {
+  float x, t, q;
+  __device__ __forceinline__ void piece0(float v) {
+    x = v;
+    if constexpr (ACT == tile::kSilu) {
+      t = -kLog2e * v;
+    } else if constexpr (ACT == tile::kGelu) {
+      t = gelu_tail_arg(v);
+      q = gelu_lower_tail_upper_terms(t);
+    }
+  }
+  __device__ __forceinline__ void piece1() {
+    if constexpr (ACT == tile::kSilu) t = __builtin_amdgcn_exp2f(t);
+    else if constexpr (ACT == tile::kGelu) q = __builtin_amdgcn_exp2f(gelu_lower_tail_lower_terms(t, q));
+  }
+  __device__ __forceinline__ void piece2() {
+    if constexpr (ACT == tile::kSilu) t = __builtin_amdgcn_rcpf(1.f + t);
+    else if constexpr (ACT == tile::kGelu) x = fmaxf(x, 0.f);
+  }
+  __device__ __forceinline__ float piece3(float up, int act) const {
+    if constexpr (ACT == tile::kSilu) return x * t * up;
+    else if constexpr (ACT == tile::kGelu) return fmaf(-t, q, x) * up;
+    switch (act) {
+      case tile::kRelu: return (x < 0.f ? 0.f : x) * up;
+      case tile::kSigmoid: return tile::sigmoid(x) * up;
+      case tile::kTanh: return tanhf(x) * up;
+      default: return x * up;
+    }
+  }
+};
+
+template <int CT, int ACT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void rows_forward_kernel(RowsArgs a) {
+  constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
+  extern __shared__ u32x4 smem[];
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int NCH = chunks_of(a.F), C = a.C;
+  float *bd = reinterpret_cast<float *>(smem + 2 * SU);  // b_down
+  for (int k = threadIdx.x; k < 32 * CT; k += 64 * WAVES) bd[k] = a.b_down && k < C ? a.b_down[k] : 0.f;
+  __syncthreads();
+  auto fetch = [&](int buf, int c) {  // this wave's share of slot c, 1 KB at a time
+    const u32x4 *src = a.blob + (int64_t)c * SU;
+    const unsigned dst = (unsigned)(uintptr_t)(smem + buf * SU);
+#pragma unroll
+    for (int k = 0; k < (NF + 1 + WAVES - 1) / WAVES; ++k) {
+      const int part = k * WAVES + wave;
+      if (part < NF + 1) load_unit_to_lds(src + part * 64, lane * 16, dst + part * 1024);
+    }
+  };
+  u32x4 xb[KS];
+  auto load_rows = [&](int64_t mb) {
+    int64_t r = mb * ROWS + wave * 32 + i;
+    if (r >= a.M) r = a.M - 1;
+    const uint16_t *src = a.x + r * C;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int col = 16 * ks + 8 * g;
+      xb[ks] = *reinterpret_cast<const u32x4 *>(src + (col < C ? col : 0));  // past the last channel: W's columns are zero there
+      if (32 * CT > C && col >= C) xb[ks] = u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  int buf = 0;
+  fetch(0, 0);
+  load_rows(blockIdx.x);
+  for (int64_t mb = blockIdx.x; mb < a.nblocks; mb += gridDim.x) {
+    f32x16 yacc[CT], ga[2], ua[2];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const tile::f32x4 b = *reinterpret_cast<const tile::f32x4 *>(bd + 32 * ct + 8 * q + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) yacc[ct][4 * q + j] = b[j];
+      }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ga[1][r] = ua[1][r] = 0.f;  // no chunk before the first: act(0) 0 = 0
+    auto slot = [&](int c, auto set_) {
+      constexpr int now = decltype(set_)::value, old = 1 - now;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the slot has landed
+      __syncthreads();                                  // everyone's, and the other buffer is free
+      const u32x4 *wb = smem + buf * SU + lane;
+      const float *bias = reinterpret_cast<const float *>(smem + buf * SU + NF * 64);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
+        const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ua[now][4 * q + j] = bu[j], ga[now][4 * q + j] = bg[j];
+      }
+      constexpr int AHEAD = 4, RING = AHEAD + 1;
+      u32x4 fr[RING], hop[2];
+      static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = wb[decltype(q)::value * 64]; });
+      Gate<ACT> gate[4];
+      float even = 0.f;
+      auto tick = [&](auto t_) {  // pieces of values T, T - 1, T - 2, T - 3
+        constexpr int T = decltype(t_)::value;
+        if constexpr (T >= 3 && T < 19) {
+          constexpr int J = T - 3;
+          const float h = gate[J % 4].piece3(ua[old][J], a.act);
+          if constexpr (J % 2 == 0) even = h;
+          else hop[J / 8][J / 2 % 4] = pack2(even, h);
+        }
+        if constexpr (T >= 2 && T < 18) gate[(T - 2) % 4].piece2();
+        if constexpr (T >= 1 && T < 17) gate[(T - 1) % 4].piece1();
+        if constexpr (T < 16) gate[T % 4].piece0(ga[old][T]);
+      };
+      // the 19 ticks are done before step 5 CT, which reads the upper half of h; the lower half, ready at tick 11, is read from step 4 CT on
+      auto behind = [&](auto s_) {
+        constexpr int S = decltype(s_)::value;
+        if constexpr (S < 5 * CT) {
+          if constexpr (CT == 8) {
+            if constexpr (S % 2 == 0) tick(std::integral_constant<int, S / 2>{});
+          } else {
+            static_for<4 / CT>([&](auto p_) { tick(std::integral_constant<int, S * (4 / CT) + decltype(p_)::value>{}); });
+          }
+        }
+      };
+      static_for<NF>([&](auto s_) {
+        constexpr int S = decltype(s_)::value;
+        if constexpr (S + AHEAD < NF) fr[(S + AHEAD) % RING] = wb[(S + AHEAD) * 64];
+        if constexpr (S >= 2 * KS) {
+          constexpr int t = S - 2 * KS;
+          yacc[t % CT] = mma(fr[S % RING], hop[t / CT], yacc[t % CT]);
+        } else if constexpr (S % 2 == 0) {
+          ua[now] = mma(fr[S % RING], xb[S / 2], ua[now]);
+        } else {
+          ga[now] = mma(fr[S % RING], xb[S / 2], ga[now]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        behind(s_);
+        if constexpr (S == 1) fetch(buf ^ 1, c + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      buf ^= 1;
+    };
+#pragma clang loop unroll(disable)
+    for (int c = 0; c < NCH; c += 2) {
+      slot(c, std::integral_constant<int, 0>{});
+      slot(c + 1, std::integral_constant<int, 1>{});
+    }
+    {  // the last chunk's share of y
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      const u32x4 *wb = smem + buf * SU + 2 * KS * 64 + lane;
+      fetch(buf ^ 1, 0);  // the first slot of the next block
+      u32x4 hop[2];
+      auto value = [&](int j) {
+        Gate<ACT> v;
+        v.piece0(ga[1][j]);
+        v.piece1();
+        v.piece2();
+        return v.piece3(ua[1][j], a.act);
+      };
+#pragma unroll
+      for (int j = 0; j < 16; j += 2) hop[j / 8][j / 2 % 4] = pack2(value(j), value(j + 1));
+#pragma unroll
+      for (int t = 0; t < 2 * CT; ++t) yacc[t % CT] = mma(wb[t * 64], hop[t / CT], yacc[t % CT]);
+      buf ^= 1;
+    }
+
+    const int64_t row0 = mb * ROWS + wave * 32;
+    const int64_t next = mb + gridDim.x;
+    load_rows(next < a.nblocks ? next : mb);
+    const int have = (int)(a.M - row0 < 32 ? (a.M > row0 ? a.M - row0 : 0) : 32);
+    auto rows_at = [&](const uint16_t *p) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p) + row0 * C, 0, have * C * 2, 0x00027000);
+    };
+    const Buffer out = rows_at(a.y), res = rows_at(a.residual ? a.residual : a.y);
+    tile::Quad<bf16> add[2][4];
+    auto ask = [&](int ct) {
+      if (a.residual) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int col = 32 * ct + 8 * q + 4 * g;
+          add[ct & 1][q].load(res, col < C ? (unsigned)(i * C + col) * 2 : tile::kNowhere);
+        }
+      }
+    };
+    ask(0);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      if (ct + 1 < CT) ask(ct + 1);
+      f32x16 v = yacc[ct];
+      if (a.residual) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[r] += add[ct & 1][r / 4][r % 4];
+      }
+      tile::store_tile(v, out, (unsigned)(i * C) * 2, 32 * ct, C, g, static_cast<const bf16 *>(nullptr));
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is landing in LDS when the workgroup ends
+}
+
+// ================================================================================================
+// host side
+// ================================================================================================
+static int channel_tiles(int64_t C) { return C <= 64 ? 2 : C <= 128 ? 4 : 8; }
+static int waves_of(int64_t C) { return C <= 128 ? 8 : 4; }
+
+bool rows_supported(int64_t C, int64_t F) { return C <= 256 && F <= 1 << 18; }
+
+// How many of M rows this kernel takes.  A round is one block of 32 rows per wave on every CU; less than a round costs as much, and the
+// tile kernels then have the smaller pieces: C = 256, F = 1024, rows / tiles (us): 16 384 rows 64 / 45, 32 768 74 / 78, 262 144 474 /
+// 582; C = 128, F = 512: 16 384 33 / 21, 32 768 34 / 34, 262 144 126 / 225.  Rows past the whole rounds go to the tile kernels where they
+// are less than half a round.
+int64_t rows_worth(int64_t M, int64_t C, int num_cu) {
+  const int64_t block = 32 * waves_of(C), blocks = (M + block - 1) / block, rounds = blocks / num_cu, over = blocks - rounds * num_cu;
+  if (2 * over >= num_cu && (rounds > 0 || 10 * over >= (C <= 128 ? 6 : 9) * num_cu)) return M;
+  const int64_t rows = rounds * num_cu * block;
+  return rows < M ? rows : M;
+}
+int64_t rows_blob_bytes(int64_t C, int64_t F) { return (chunks_of((int)F) + 1) * (6 * channel_tiles(C) + 1) * 1024; }
+
+template <int CT, int ACT, int WAVES>
+static int launch_rows(const RowsArgs &a, int num_cu, hipStream_t st) {
+  constexpr size_t lds = 2 * (6 * CT + 1) * 1024 + 32 * CT * 4;
+  auto kernel = rows_forward_kernel<CT, ACT, WAVES>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  const int64_t grid = a.nblocks < num_cu ? a.nblocks : num_cu;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
+  return launch_status();
+}
+template <int CT, int WAVES>
+static int launch_rows(const RowsArgs &a, int num_cu, hipStream_t st) {
+  if (a.act == tile::kSilu) return launch_rows<CT, tile::kSilu, WAVES>(a, num_cu, st);
+  if (a.act == tile::kGelu) return launch_rows<CT, tile::kGelu, WAVES>(a, num_cu, st);
+  return launch_rows<CT, -1, WAVES>(a, num_cu, st);
+}
+
+int rows_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st) {
+  const int64_t units = rows_blob_bytes(C, F) / 16;
+  const int64_t blocks = (units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096;
+  hipLaunchKernelGGL(rows_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const uint16_t *>(p.w_gate),
+                     static_cast<const uint16_t *>(p.w_up), static_cast<const uint16_t *>(p.w_down), p.b_gate, p.b_up,
+                     static_cast<u32x4 *>(blob), (int)C, (int)F, channel_tiles(C));
+  return launch_status();
+}
+
+// rows 0 .. M - 1 on the weights of rows_pack
+int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float *b_down, int act, const void *x, const void *residual,
+                 void *y, int num_cu, hipStream_t st) {
+  RowsArgs a{};
+  a.blob = static_cast<const u32x4 *>(blob);
+  a.x = static_cast<const uint16_t *>(x), a.residual = static_cast<const uint16_t *>(residual), a.y = static_cast<uint16_t *>(y);
+  a.b_down = b_down;
+  a.M = M, a.nblocks = (M + 32 * waves_of(C) - 1) / (32 * waves_of(C));
+  a.C = (int)C, a.F = (int)F, a.act = act;
+  switch (channel_tiles(C)) {
+    case 2: return launch_rows<2, 8>(a, num_cu, st);
+    case 4: return launch_rows<4, 8>(a, num_cu, st);
+    default: return launch_rows<8, 4>(a, num_cu, st);
+  }
+}
+
+}  // namespace gated
+}  // namespace pa

@@ -93,6 +93,28 @@ def test_values_and_gradients(rows, C, F, dtype):
         check(g, v, t, what)
 
 
+@pytest.mark.parametrize("act", list(ACTS))
+@pytest.mark.parametrize("rows,C,F", [(39_400, 32, 33), (65_539, 64, 96), (66_000, 96, 200), (40_001, 128, 64), (32_700, 200, 70),
+                                      (33_000, 256, 130)])
+def test_many_rows(rows, C, F, act):
+    """Enough rows for the kernel that keeps the hidden layer on chip, with and without rows left over for the tile kernels."""
+    announce("gated many rows", rows, C, F, act)
+    st = make(rows, C, F, torch.bfloat16, bias=F % 2 == 0, seed=C)
+    values, tols = derived(st, act, torch.bfloat16)
+    gpu = on_gpu(st)
+    params = [gpu[n] for n in NAMES]
+    check(PF.gated_mlp_forward(gpu["x"], *params, act=act, residual=gpu["residual"]), values[0], tols[0], "y")
+    y = PF.gated_mlp_forward(gpu["x"], *params, act=act)
+    bare = values[0] - st["residual"].double()  # rounded relative to itself, not to its sum with the residual
+    check(y, bare, tols[0] + torch.finfo(torch.bfloat16).eps / 2 * bare.abs(), "y without a residual")
+    x = gpu["x"].clone()
+    x[17, 3], x[rows - 1, 0] = float("nan"), float("inf")
+    hit = PF.gated_mlp_forward(x, *params, act=act)
+    clean = torch.ones(rows, dtype=torch.bool, device="cuda")
+    clean[17] = clean[rows - 1] = False
+    assert torch.equal(hit[clean], y[clean]) and torch.isnan(hit[17]).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", list(ACTS))
 def test_activations(act, dtype):
