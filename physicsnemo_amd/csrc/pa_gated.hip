@@ -154,6 +154,10 @@ int64_t rows_blob_bytes(int64_t C, int64_t F);
 int rows_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st);
 int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float *b_down, int act, const void *x, const void *residual,
                  void *y, int num_cu, hipStream_t st);
+int64_t hidden_blob_bytes(int64_t C, int64_t F);
+int hidden_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st);
+int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void *blob, int act, const void *x, const void *dy, void *dgu,
+                         void *h, int num_cu, hipStream_t st);
 
 template <class E, class TO, tile::Kind KIND>
 static int product(const Args &a, int num_cu, hipStream_t st) {
@@ -169,7 +173,7 @@ static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, in
   const bool plan = bytes != nullptr;
   Space ws{workspace};
   Layout lay;
-  const int64_t Fp = up(F, U);
+  const int64_t Fp = up(F, 32 / e);  // the hidden layer's columns: whole 32-byte groups
   auto copied = [&](const void *q, int64_t width) { return plan || !whole_rows(q, width, e); };
   int64_t done = 0;  // rows of the kernel that keeps the hidden layer on chip
   if (e == 2 && C % 8 == 0 && rows_supported(C, F)) {
@@ -184,7 +188,7 @@ static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, in
   auto behind = [&](const void *q) { return q ? static_cast<const char *>(q) + done * C * e : nullptr; };
   x = behind(x), residual = behind(residual), y = const_cast<char *>(behind(y));
   M -= done;
-  void *h = ws.take(M * Fp * e);
+  void *h = ws.take(up(M, tile::kGroupRows) * Fp * e);
   const Rows xr = rows_of(x, M, C, e, copied(x, C), ws, &lay);
   const Rows wg = rows_of(p.w_gate, F, C, e, copied(p.w_gate, C), ws, &lay);
   const Rows wu = rows_of(p.w_up, F, C, e, copied(p.w_up, C), ws, &lay);
@@ -199,7 +203,7 @@ static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, in
   a.out = h, a.ldo = Fp, a.act = act;
   if (int rc = product<E, TO, tile::kGated>(a, num_cu, st)) return rc;
   Args d{};
-  d.X = h, d.ldx = Fp * e, d.units = (int)(Fp * e / 16);
+  d.X = h, d.ldx = Fp * e, d.units = wd.units, d.x_groups = tile::kGrouped<TO>;
   d.W[0] = wd.p, d.ldw = wd.ld;
   d.M = M, d.N = d.limit = (int)C;
   d.bias[0] = p.b_down;
@@ -245,8 +249,9 @@ static Partials partials_of(int64_t M, int64_t oa, int64_t ob, int num_cu, Space
   return r;
 }
 template <class E>
-static int rows_product(const Partials &r, const void *A, int64_t oa, const void *B, int64_t ob, int64_t M, int num_cu, hipStream_t st) {
-  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, r.sums, st);
+static int rows_product(const Partials &r, const void *A, int64_t oa, const void *B, int64_t ob, int64_t M, int groups, int num_cu,
+                        hipStream_t st) {  // groups: 1 if A, 2 if B is a matrix of the hidden layer
+  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, r.sums, st, groups);
   return gemm::cols_gemm_f32(A, oa, oa, B, ob, ob, M, nullptr, r.product, r.sums, num_cu, st);
 }
 
@@ -257,9 +262,10 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   const bool plan = bytes != nullptr;
   Space ws{workspace};
   Layout lay;
-  const int64_t Cp = up(C < LEAST ? LEAST : C, U), Fp = up(F < LEAST ? LEAST : F, U);
+  const int64_t Cp = up(C < LEAST ? LEAST : C, U), Fp = up(F < LEAST ? LEAST : F, 32 / e);
   const bool copy_x = plan || C != Cp || !aligned16(x), copy_dy = plan || C != Cp || !aligned16(dy);
-  void *dgu = ws.take(M * 2 * Fp * e), *h = ws.take(M * Fp * e);
+  const int64_t Mp = up(M, tile::kGroupRows);
+  void *dgu = ws.take(Mp * 2 * Fp * e), *h = ws.take(Mp * Fp * e);
   auto padded = [&](const void *q, int64_t rows, int64_t cols, int64_t ld, bool copy) {
     Rows r{q, ld * e, (int)(ld * e / 16)};
     if (copy) {
@@ -270,30 +276,42 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     return r;
   };
   const Rows xr = padded(x, M, C, Cp, copy_x), dyr = padded(dy, M, C, Cp, copy_dy);
+  // rows of the kernel that owns them, which has the weights in an order of its own
+  const bool by_rows = e == 2 && rows_supported(Cp, F);
+  const int64_t done = by_rows && !plan ? rows_worth(M, Cp, num_cu) : 0, rest = M - done;
+  void *blob = by_rows ? ws.take(hidden_blob_bytes(C, F)) : nullptr;
   const bool copy_w = plan || C != Cp || !aligned16(p.w_gate) || !aligned16(p.w_up);
-  const Rows wg = padded(p.w_gate, F, C, Cp, copy_w), wu = padded(p.w_up, F, C, Cp, copy_w);
+  const Rows wg = padded(p.w_gate, F, C, Cp, copy_w && rest > 0), wu = padded(p.w_up, F, C, Cp, copy_w && rest > 0);
   // W_down^T (F, Cp), and [W_gate; W_up]^T (C, 2 Fp): hidden units past F are zero columns
   void *wd_t = ws.take(F * Cp * e), *w_t = ws.take(C * 2 * Fp * e);
   const Partials in = partials_of<E>(M, 2 * Fp, Cp, num_cu, ws), down = partials_of<E>(M, Cp, Fp, num_cu, ws);
   if (plan) return *bytes = ws.used, PA_OK;
-  lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
+  if (rest > 0) lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
   if (dx) {
     lay.add(p.w_gate, C, w_t, C, F, Fp, 2 * Fp, true);
     lay.add(p.w_up, C, static_cast<char *>(w_t) + Fp * e, C, F, Fp, 2 * Fp, true);
   }
   int rc = tile::lay_out(lay, e, st);
   if (rc) return rc;
-  Args a{};
-  a.X = xr.p, a.ldx = xr.ld, a.units = xr.units;
-  a.X2 = dyr.p, a.ldx2 = dyr.ld, a.units2 = dyr.units;
-  a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
-  a.M = M, a.N = (int)F, a.limit = (int)Fp;
-  a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
-  a.out = dgu, a.ldo = 2 * Fp, a.out2 = h, a.ldh = Fp, a.act = act;
-  if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
+  if (done > 0) {
+    rc = hidden_pack(C, F, p, blob, st);
+    if (!rc) rc = rows_hidden_backward(done, Cp, F, Fp, blob, act, xr.p, dyr.p, dgu, h, num_cu, st);
+    if (rc) return rc;
+  }
+  if (rest > 0) {
+    auto from = [&](const void *q, int64_t ld) { return const_cast<char *>(static_cast<const char *>(q)) + done * ld; };
+    Args a{};
+    a.X = from(xr.p, xr.ld), a.ldx = xr.ld, a.units = xr.units;
+    a.X2 = from(dyr.p, dyr.ld), a.ldx2 = dyr.ld, a.units2 = dyr.units;
+    a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
+    a.M = rest, a.N = (int)F, a.limit = (int)Fp;
+    a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+    a.out = from(dgu, 2 * Fp * e), a.ldo = 2 * Fp, a.out2 = from(h, Fp * e), a.ldh = Fp, a.act = act;
+    if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
+  }
   if (dx) {
     Args d{};
-    d.X = dgu, d.ldx = 2 * Fp * e, d.units = (int)(2 * Fp * e / 16);
+    d.X = dgu, d.ldx = 2 * Fp * e, d.units = (int)(2 * Fp * e / 16), d.x_groups = tile::kGrouped<TO>;
     d.W[0] = w_t, d.ldw = 2 * Fp * e;
     d.M = M, d.N = d.limit = (int)C;
     d.out = dx, d.ldo = C;
@@ -302,14 +320,14 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   }
   Totals totals;
   if (out.w_gate || out.w_up || out.b_gate || out.b_up) {
-    if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, num_cu, st))) return rc;
+    if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, 1, num_cu, st))) return rc;
     totals.add(in.product, in.G, 2 * Fp * Cp, Cp, out.w_gate, F, C, e);
     totals.add(in.product + Fp * Cp, in.G, 2 * Fp * Cp, Cp, out.w_up, F, C, e);
     totals.add(in.sums, in.G, 2 * Fp, F, out.b_gate, 1, F, 4);
     totals.add(in.sums + Fp, in.G, 2 * Fp, F, out.b_up, 1, F, 4);
   }
   if (out.w_down || out.b_down) {
-    if ((rc = rows_product<E>(down, dyr.p, Cp, h, Fp, M, num_cu, st))) return rc;
+    if ((rc = rows_product<E>(down, dyr.p, Cp, h, Fp, M, 2, num_cu, st))) return rc;
     totals.add(down.product, down.G, Cp * Fp, Fp, out.w_down, C, F, e);
     totals.add(down.sums, down.G, Cp, C, out.b_down, 1, C, 4);
   }

@@ -274,6 +274,254 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is landing in LDS when the workgroup ends
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// hidden_pack_kernel: slot c = 0 .. NCH - 1 of the backward's weight stream, (6 CT + 1) KB: for every k-step the fragments of
+// W_up's and W_gate's rows 32 c .. + 31 and of W_down's columns 32 c .. + 31 (reduction over its rows); 32 biases of W_up and W_gate.
+// ---------------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void hidden_pack_kernel(const uint16_t *__restrict__ wg, const uint16_t *__restrict__ wu,
+                                                          const uint16_t *__restrict__ wd, const float *__restrict__ bg,
+                                                          const float *__restrict__ bu, u32x4 *__restrict__ blob, int C, int F, int CT) {
+  const int SU = (6 * CT + 1) * 64, NCH = chunks_of(F);
+  const int64_t total = (int64_t)NCH * SU;
+  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < total; u += (int64_t)gridDim.x * 256) {
+    const int c = (int)(u / SU), r = (int)(u - (int64_t)c * SU), frag = r >> 6, lane = r & 63, i = lane & 31, g = lane >> 5;
+    u32x4 e = {0u, 0u, 0u, 0u};
+    if (frag < 6 * CT) {
+      const int which = frag % 3, row = 32 * c + i, col = 16 * (frag / 3) + 8 * g;
+      if (row < F) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + j < C) {
+            const uint16_t v = which == 2 ? wd[(int64_t)(col + j) * F + row] : (which ? wg : wu)[(int64_t)row * C + col + j];
+            e[j / 2] |= (uint32_t)v << (16 * (j & 1));
+          }
+      }
+    } else if (lane < 16) {
+      const float *b = lane < 8 ? bu : bg;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 32 * c + 4 * (lane & 7) + j;
+        if (b && at < F) e[j] = __float_as_uint(b[at]);
+      }
+    }
+    blob[u] = e;
+  }
+}
+
+struct HiddenArgs {
+  const u32x4 *blob;
+  const uint16_t *x, *dy;
+  uint16_t *dgu, *h;  // (M, 2 Fp): dg, du; (M, Fp); in column groups (pa_tile.h), whole blocks of 32 rows
+  int64_t M, nblocks;
+  int C, F, Fp, act;
+};
+
+// One hidden unit of a row in five pieces: h = act(g) u, dg = d u act'(g), du = d act(g).
+template <int ACT>
+struct Slope {
+  float x, a, s, t;
+  __device__ __forceinline__ void piece0(float v) {
+    x = v;
+    if constexpr (ACT == tile::kSilu) {
+      t = -kLog2e * v;
+    } else if constexpr (ACT == tile::kGelu) {
+      a = gelu_tail_arg(v);
+      s = gelu_lower_tail_upper_terms(a);
+    }
+  }
+  __device__ __forceinline__ void piece1() {
+    if constexpr (ACT == tile::kSilu) {
+      t = __builtin_amdgcn_exp2f(t);
+    } else if constexpr (ACT == tile::kGelu) {
+      s = gelu_lower_tail_lower_terms(a, s);
+      t = a * a * (-0.5f * kLog2e);
+    }
+  }
+  __device__ __forceinline__ void piece2() {
+    if constexpr (ACT == tile::kSilu) {
+      s = __builtin_amdgcn_rcpf(1.f + t);
+    } else if constexpr (ACT == tile::kGelu) {
+      s = __builtin_amdgcn_exp2f(s);
+      t = __builtin_amdgcn_exp2f(t);
+    }
+  }
+  __device__ __forceinline__ void piece3(int act) {  // a <- act(g), s and t what the derivative needs besides
+    if constexpr (ACT == tile::kSilu) {
+      a = x * s;
+      t = 1.f - s;
+    } else if constexpr (ACT == tile::kGelu) {
+      const float phi = x > 0.f ? 1.f - s : s;
+      a = fmaf(-a, s, fmaxf(x, 0.f));
+      s = phi;
+    } else {
+      switch (act) {
+        case tile::kRelu: a = x < 0.f ? 0.f : x, s = x > 0.f ? 1.f : 0.f; break;
+        case tile::kSigmoid: a = tile::sigmoid(x), s = a * (1.f - a); break;
+        case tile::kTanh: a = tanhf(x), s = fmaf(-a, a, 1.f); break;
+        default: a = x, s = 1.f;
+      }
+    }
+  }
+  __device__ __forceinline__ void piece4(float up, float d, float &h, float &dg, float &du) const {
+    float slope = s;
+    if constexpr (ACT == tile::kSilu) slope = fmaf(a, t, s);
+    else if constexpr (ACT == tile::kGelu) slope = fmaf(x * 0.3989422804014327f, t, s);
+    h = a * up;
+    dg = d * up * slope;
+    du = d * a;
+  }
+};
+
+// ---------------------------------------------------------------------------------------------------------------
+// rows_hidden_backward_kernel<CT>: the hidden layer of the backward pass for rows of up to 32 CT channels.  Per slot c a wave runs
+//   u(c)^T = W_up[chunk c] x^T + b_up, g(c)^T = W_gate[chunk c] x^T + b_gate, d(c)^T = W_down[:, chunk c]^T dy^T     6 CT MFMAs
+// in turn, with h, dg and du of the chunk before formed behind them, 16 values in five pieces each; two sets of accumulators take
+// turns.  Results of two chunks leave together, 2 KB in one piece each (pa_tile.h).  Bound by HBM, 4 C + 6 F bytes per row.
+// ---------------------------------------------------------------------------------------------------------------
+template <int CT, int ACT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void rows_hidden_backward_kernel(
+    HiddenArgs a) {
+  constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
+  constexpr int STORES = 12;  // of two chunks
+  extern __shared__ u32x4 smem[];
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int NCH = chunks_of(a.F), C = a.C;
+  auto fetch = [&](int buf, int c) {  // this wave's share of slot c, 1 KB at a time
+    const u32x4 *src = a.blob + (int64_t)c * SU;
+    const unsigned dst = (unsigned)(uintptr_t)(smem + buf * SU);
+#pragma unroll
+    for (int k = 0; k < (NF + 1 + WAVES - 1) / WAVES; ++k) {
+      const int part = k * WAVES + wave;
+      if (part < NF + 1) load_unit_to_lds(src + part * 64, lane * 16, dst + part * 1024);
+    }
+  };
+  u32x4 xb[KS], db[KS];
+  auto load_rows = [&](int64_t mb) {
+    int64_t r = mb * ROWS + wave * 32 + i;
+    if (r >= a.M) r = a.M - 1;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int col = 16 * ks + 8 * g, at = col < C ? col : 0;
+      xb[ks] = *reinterpret_cast<const u32x4 *>(a.x + r * C + at);
+      db[ks] = *reinterpret_cast<const u32x4 *>(a.dy + r * C + at);
+      if (32 * CT > C && col >= C) xb[ks] = db[ks] = u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  int buf = 0;
+  fetch(0, 0);
+  load_rows(blockIdx.x);
+  for (int64_t mb = blockIdx.x; mb < a.nblocks; mb += gridDim.x) {
+    const int64_t row0 = mb * ROWS + wave * 32;
+    const int have = (int)(a.M - row0 < 32 ? (a.M > row0 ? a.M - row0 : 0) : 32);
+    const Buffer out = __builtin_amdgcn_make_buffer_rsrc(a.dgu + row0 * 2 * a.Fp, 0, have > 0 ? 32 * 2 * a.Fp * 2 : 0, 0x00027000);
+    const Buffer hidden = __builtin_amdgcn_make_buffer_rsrc(a.h + row0 * a.Fp, 0, have > 0 ? 32 * a.Fp * 2 : 0, 0x00027000);
+    f32x16 ga[2], ua[2], da[2];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) ga[1][r] = ua[1][r] = da[1][r] = 0.f;
+    uint32_t packed[2][3][8];  // of the chunks of a pair: dg, du, h
+    auto store_pair = [&](int c) {  // chunks c, c + 1
+#pragma unroll
+      for (int which = 0; which < 3; ++which)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            u32x4 s;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const auto r = __builtin_amdgcn_permlane32_swap(packed[k][which][4 * half + w], packed[k][which][4 * half + 2 + w], false, false);
+              s[w] = r[0], s[2 + w] = r[1];
+            }
+            const int col = 32 * (c + k) + 16 * half + 8 * g;
+            const unsigned at = (unsigned)(((which == 1 ? a.Fp : 0) + 32 * (c + k) + 16 * half) * 64 + i * 32 + g * 16);
+            __builtin_amdgcn_raw_buffer_store_b128(s, which < 2 ? out : hidden, col < a.Fp ? at : tile::kNowhere, 0, 0);
+          }
+    };
+    auto slot = [&](int c, auto set_) {
+      constexpr int now = decltype(set_)::value, old = 1 - now;
+      // this wave's share of the slot has landed; the stores that left behind it stay in flight
+      if (now == 1 && c > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();  // everyone's, and the other buffer is free
+      const u32x4 *wb = smem + buf * SU + lane;
+      const float *bias = reinterpret_cast<const float *>(smem + buf * SU + NF * 64);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
+        const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ua[now][4 * q + j] = bu[j], ga[now][4 * q + j] = bg[j], da[now][4 * q + j] = 0.f;
+      }
+      constexpr int AHEAD = 4, RING = AHEAD + 1;
+      u32x4 fr[RING];
+      static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = wb[decltype(q)::value * 64]; });
+      Slope<ACT> v[5];
+      float even[3];
+      auto tick = [&](auto t_) {  // pieces of values T .. T - 4
+        constexpr int T = decltype(t_)::value;
+        if constexpr (T >= 4 && T < 20) {
+          constexpr int J = T - 4;
+          float h, dg, du;
+          v[J % 5].piece4(ua[old][J], da[old][J], h, dg, du);
+          if constexpr (J % 2 == 0) {
+            even[0] = dg, even[1] = du, even[2] = h;
+          } else {
+            packed[old][0][J / 2] = pack2(even[0], dg);
+            packed[old][1][J / 2] = pack2(even[1], du);
+            packed[old][2][J / 2] = pack2(even[2], h);
+          }
+        }
+        if constexpr (T >= 3 && T < 19) v[(T - 3) % 5].piece3(a.act);
+        if constexpr (T >= 2 && T < 18) v[(T - 2) % 5].piece2();
+        if constexpr (T >= 1 && T < 17) v[(T - 1) % 5].piece1();
+        if constexpr (T < 16) v[T % 5].piece0(ga[old][T]);
+      };
+      static_for<NF>([&](auto s_) {
+        constexpr int S = decltype(s_)::value;
+        if constexpr (S + AHEAD < NF) fr[(S + AHEAD) % RING] = wb[(S + AHEAD) * 64];
+        if constexpr (S % 3 == 0) ua[now] = mma(fr[S % RING], xb[S / 3], ua[now]);
+        else if constexpr (S % 3 == 1) ga[now] = mma(fr[S % RING], xb[S / 3], ga[now]);
+        else da[now] = mma(fr[S % RING], db[S / 3], da[now]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (CT == 8) {
+          if constexpr (S % 2 == 0) tick(std::integral_constant<int, S / 2>{});
+        } else {
+          static_for<4 / CT>([&](auto p_) { tick(std::integral_constant<int, S * (4 / CT) + decltype(p_)::value>{}); });
+        }
+        if constexpr (S == 1) fetch(buf ^ 1, c + 1 < NCH ? c + 1 : 0);  // past the last slot: the first of the next block
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      if (now == 0 && c > 0) store_pair(c - 2);
+      buf ^= 1;
+    };
+#pragma clang loop unroll(disable)
+    for (int c = 0; c < NCH; c += 2) {
+      slot(c, std::integral_constant<int, 0>{});
+      slot(c + 1, std::integral_constant<int, 1>{});
+    }
+    const int64_t next = mb + gridDim.x;
+    load_rows(next < a.nblocks ? next : mb);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {  // the last chunk
+      float o[2][3];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        Slope<ACT> v;
+        v.piece0(ga[1][j + k]);
+        v.piece1();
+        v.piece2();
+        v.piece3(a.act);
+        v.piece4(ua[1][j + k], da[1][j + k], o[k][2], o[k][0], o[k][1]);
+      }
+#pragma unroll
+      for (int which = 0; which < 3; ++which) packed[1][which][j / 2] = pack2(o[0][which], o[1][which]);
+    }
+    store_pair(NCH - 2);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is landing in LDS when the workgroup ends
+}
+
 // ================================================================================================
 // host side
 // ================================================================================================
@@ -292,7 +540,7 @@ int64_t rows_worth(int64_t M, int64_t C, int num_cu) {
   const int64_t rows = rounds * num_cu * block;
   return rows < M ? rows : M;
 }
-int64_t rows_blob_bytes(int64_t C, int64_t F) { return (chunks_of((int)F) + 1) * (6 * channel_tiles(C) + 1) * 1024; }
+int64_t rows_blob_bytes(int64_t C, int64_t F) { return (int64_t)(chunks_of((int)F) + 1) * (6 * channel_tiles(C) + 1) * 1024; }
 
 template <int CT, int ACT, int WAVES>
 static int launch_rows(const RowsArgs &a, int num_cu, hipStream_t st) {
@@ -332,6 +580,49 @@ int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float 
     case 2: return launch_rows<2, 8>(a, num_cu, st);
     case 4: return launch_rows<4, 8>(a, num_cu, st);
     default: return launch_rows<8, 4>(a, num_cu, st);
+  }
+}
+
+// ---- the backward's hidden layer ----
+int64_t hidden_blob_bytes(int64_t C, int64_t F) { return (int64_t)chunks_of((int)F) * (6 * channel_tiles(C) + 1) * 1024; }
+
+template <int CT, int ACT, int WAVES>
+static int launch_hidden(const HiddenArgs &a, int num_cu, hipStream_t st) {
+  constexpr size_t lds = 2 * (6 * CT + 1) * 1024;
+  auto kernel = rows_hidden_backward_kernel<CT, ACT, WAVES>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  const int64_t grid = a.nblocks < num_cu ? a.nblocks : num_cu;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(64 * WAVES), lds, st, a);
+  return launch_status();
+}
+template <int CT, int WAVES>
+static int launch_hidden(const HiddenArgs &a, int num_cu, hipStream_t st) {
+  if (a.act == tile::kSilu) return launch_hidden<CT, tile::kSilu, WAVES>(a, num_cu, st);
+  if (a.act == tile::kGelu) return launch_hidden<CT, tile::kGelu, WAVES>(a, num_cu, st);
+  return launch_hidden<CT, -1, WAVES>(a, num_cu, st);
+}
+
+int hidden_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st) {
+  const int64_t units = hidden_blob_bytes(C, F) / 16;
+  const int64_t blocks = (units + 255) / 256 < 4096 ? (units + 255) / 256 : 4096;
+  hipLaunchKernelGGL(hidden_pack_kernel, dim3((unsigned)blocks), dim3(256), 0, st, static_cast<const uint16_t *>(p.w_gate),
+                     static_cast<const uint16_t *>(p.w_up), static_cast<const uint16_t *>(p.w_down), p.b_gate, p.b_up,
+                     static_cast<u32x4 *>(blob), (int)C, (int)F, channel_tiles(C));
+  return launch_status();
+}
+
+int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void *blob, int act, const void *x, const void *dy, void *dgu,
+                         void *h, int num_cu, hipStream_t st) {
+  HiddenArgs a{};
+  a.blob = static_cast<const u32x4 *>(blob);
+  a.x = static_cast<const uint16_t *>(x), a.dy = static_cast<const uint16_t *>(dy);
+  a.dgu = static_cast<uint16_t *>(dgu), a.h = static_cast<uint16_t *>(h);
+  a.M = M, a.nblocks = (M + 32 * waves_of(C) - 1) / (32 * waves_of(C));
+  a.C = (int)C, a.F = (int)F, a.Fp = (int)Fp, a.act = act;
+  switch (channel_tiles(C)) {
+    case 2: return launch_hidden<2, 8>(a, num_cu, st);
+    case 4: return launch_hidden<4, 8>(a, num_cu, st);
+    default: return launch_hidden<8, 4>(a, num_cu, st);
   }
 }
 

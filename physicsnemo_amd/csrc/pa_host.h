@@ -123,7 +123,8 @@ int product(int dtype, int64_t M, const void *A, int64_t lda, int64_t OA, const 
             Sums *later = nullptr);  // later: the totals are left to its launch
 // the bf16 tile kernel alone, G partial results
 int launch_wide(const void *A, int64_t lda, int64_t OA, const void *B, int64_t ldb, int64_t OB, int64_t M, int64_t G,
-                const pa_shape *grid, float *partials, float *col_sums, hipStream_t st);
+                const pa_shape *grid, float *partials, float *col_sums, hipStream_t st,
+                int groups = 0);  // no grid; 1: A, 2: B in groups of 16 columns (rows of whole groups, whole blocks of 32 rows)
 int sum_rows(const float *src, int64_t rows, int64_t n, float *dst, hipStream_t st);
 int64_t chunks_for(int64_t M, int64_t tiles, int64_t n, int num_cu);  // partial results of a product of `tiles` workgroups
 int64_t output_backward_workspace_bytes(const pa_shape &s, int num_cu);

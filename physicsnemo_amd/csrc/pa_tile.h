@@ -160,6 +160,14 @@ enum Kind {
            // out[:, :ldh] = d u act'(g), out[:, ldh:] = d act(g), out2 = act(g) u
 };
 
+// The hidden layer's matrices are written and read by kernels of this library alone, and lie in groups of 32 bytes of columns where
+// the type is bf16: [32 rows][column group][row][32 bytes].  A wave's 32 x 32 tile is then 2 KB in one piece; as rows it
+// is 32 pieces of 64 bytes, kilobytes apart, which memory takes at half the rate (131 072 rows of 3 x 1 024 values: 476 us as
+// rows, 326 in groups).
+template <class T>
+constexpr bool kGrouped = sizeof(T) == 2;
+constexpr int64_t kGroupRows = 32;
+
 struct Args {
   const void *X, *X2;            // rows of activations; a row is `units` units of 16 bytes, ldx / ldx2 bytes apart
   const void *W[3];              // rows of weights, ldw / ldw2 (W[2]) bytes apart
@@ -173,6 +181,7 @@ struct Args {
   void *out, *out2;
   int64_t ldo, ldh;              // elements between rows of out (residual alike); of out2, and from dg to du
   int act;
+  bool x_groups;                 // X lies in column groups
   bool vec;                      // out and residual start on 16 bytes and their rows are whole units apart
   int mt, nt;                    // tiles
 };
@@ -181,7 +190,9 @@ typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr unsigned kNowhere = 0x80000000u;  // an offset past every buffer below: loads give zero, stores are dropped
 
 // 16-byte stores of a 32 x 32 tile: this lane's row at byte offset `at`, columns col .. col + 31 below limit.  Neighbouring
-// columns of a row come from both halves of the wave: a lane's 16 bytes lie beside its partner's.
+// columns of a row come from both halves of the wave: a lane's 16 bytes lie beside its partner's.  GROUPS: `at` is the row's place in
+// its column groups.
+template <bool GROUPS = false>
 __device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, unsigned at, int col, int limit, int g, const bf16 *) {
   uint32_t p[4][2];
 #pragma unroll
@@ -197,10 +208,13 @@ __device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, u
       s[w] = r[0], s[2 + w] = r[1];
     }
     const int c = col + 16 * h + 8 * g;
-    __builtin_amdgcn_raw_buffer_store_b128(s, out, c < limit ? at + 2 * c : kNowhere, 0, 0);
+    const unsigned place = GROUPS ? at + 64 * (col + 16 * h) + 16 * g : at + 2 * c;
+    __builtin_amdgcn_raw_buffer_store_b128(s, out, c < limit ? place : kNowhere, 0, 0);
   }
 }
+template <bool GROUPS = false>
 __device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, unsigned at, int col, int limit, int g, const float *) {
+  static_assert(!GROUPS, "float32 lies as rows");
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int c = col + 8 * q + 4 * g;
@@ -338,7 +352,9 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
       const int row = (wave * NX + q) * GROUP + frow, r = row < have ? row : have - 1;
-      offx[q] = (unsigned)(r * ldx) + 16 * (fpos ^ swizzle(row));
+      const int unit = fpos ^ swizzle(row);
+      offx[q] = KIND == kPlain && a.x_groups ? (unsigned)((r & ~31) * ldx + (r & 31) * 32 + (unit >> 1) * 1024 + (unit & 1) * 16)
+                                             : (unsigned)(r * ldx) + 16 * unit;
     }
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
@@ -375,12 +391,21 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
       sbuf = sbuf + 1 == RING ? 0 : sbuf + 1;
     }
     auto off_of = [&](unsigned off, int grp) { return (int)(off - (grp & 1 ? past_odd : past_even)); };
-    const char *xs = uniform(xbase + (int64_t)kb * (16 * UPS)), *ws0 = uniform(wbase[0] + (int64_t)kb * (16 * UPS));
+    unsigned xpast_even = past_even, xpast_odd = past_odd;
+    if (KIND == kPlain && a.x_groups) {
+      auto past_groups = [&](int unit) {
+        const int to = unit >= left ? left - 1 : unit;
+        return (unsigned)(((unit >> 1) - (to >> 1)) * 1024 + ((unit & 1) - (to & 1)) * 16);
+      };
+      xpast_even = past_groups(fpos ^ swizzle(frow)), xpast_odd = past_groups(fpos ^ swizzle(frow + GROUP));
+    }
+    const int64_t xstep = KIND == kPlain && a.x_groups ? 512 * UPS : 16 * UPS;
+    const char *xs = uniform(xbase + (int64_t)kb * xstep), *ws0 = uniform(wbase[0] + (int64_t)kb * (16 * UPS));
     const char *ws1 = DUAL ? uniform(wbase[1] + (int64_t)kb * (16 * UPS)) : ws0;
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
       const int grp = wave * NX + q;
-      load_unit_to_lds(xs, off_of(offx[q], grp), dst + grp * 1024);
+      load_unit_to_lds(xs, (int)(offx[q] - (grp & 1 ? xpast_odd : xpast_even)), dst + grp * 1024);
     }
 #pragma unroll
     for (int q = 0; q < NW; ++q) {
@@ -553,7 +578,17 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           }
         }
       } else {
-        const Buffer out = rows_at(a.out, a.ldo);
+        constexpr bool GROUPS = kGrouped<TO> && E::kBytes == 2;
+        auto rows_or_blocks_at = [&](const void *p, int64_t ld) {  // whole blocks of 32 rows: what lies past the last row is never read as a value
+          const int rows = GROUPS ? (have + 31) & ~31 : have;
+          return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(uniform(static_cast<const char *>(p) + m0 * ld * sizeof(TO))), 0,
+                                                   (int)(rows * ld * sizeof(TO)), 0x00027000);
+        };
+        auto place_of = [&](int64_t ld) {  // of this lane's row
+          return GROUPS ? (unsigned)((rl & ~31) * ld * sizeof(TO) + (rl & 31) * 32) : (unsigned)(rl * ld * sizeof(TO));
+        };
+        const Buffer out = rows_or_blocks_at(a.out, a.ldo);
+        const unsigned at_out = place_of(a.ldo);
 #pragma unroll
         for (int n = 0; n < TN2; ++n) {
           const int col = tn * CN + (wn * TN2 + n) * 32;
@@ -571,9 +606,9 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
 #pragma unroll
             for (int r = 0; r < 16; ++r) gate[r] *= up[r];
             cut(gate);
-            store_tile(gate, out, at, col, a.limit, g, type);
+            store_tile<GROUPS>(gate, out, at_out, col, a.limit, g, type);
           } else {
-            const Buffer hidden = rows_at(a.out2, a.ldh);
+            const Buffer hidden = rows_or_blocks_at(a.out2, a.ldh);
             f32x16 slope, d = acc2[m][n];
             act_slopes(a.act, gate, slope);
             f32x16 h;
@@ -584,9 +619,9 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
               gate[r] *= d[r];
             }
             cut(h), cut(slope), cut(gate);
-            store_tile(slope, out, at, col, a.limit, g, type);
-            store_tile(gate, out, at + (unsigned)(a.ldh * sizeof(TO)), col, a.limit, g, type);
-            store_tile(h, hidden, (unsigned)(rl * a.ldh * sizeof(TO)), col, a.limit, g, type);
+            store_tile<GROUPS>(slope, out, at_out, col, a.limit, g, type);
+            store_tile<GROUPS>(gate, out, at_out + (unsigned)(a.ldh * sizeof(TO)) * (GROUPS ? 32 : 1), col, a.limit, g, type);
+            store_tile<GROUPS>(h, hidden, place_of(a.ldh), col, a.limit, g, type);
           }
         }
       }

@@ -56,9 +56,14 @@ struct Args {
 // are copied as they lie, the 16-byte units permuted within a chunk so that the transposing reads of a half-wave (4
 // points x 4 groups of slices x 2 chunks) fall on all banks: unit (p, g) of chunk c at position 32 g + (p ^ 4 g ^ 8 (c & 1)).
 // Slice weights of points beyond N are zero, so B's rows there only need to be readable; col_sums are B's columns.
-template <int MODE>
+// GROUPS (mode 0): bit 0 A, bit 1 B: the operand lies in groups of 16 columns, [32 rows][column group][row][16 columns], as the
+// hidden layer's kernels leave it (pa_tile.h).  A load takes a group's 1 KB as it lies, the rows of odd groups in the order
+// r ^ 4, so that the two groups a half-wave reads from fall on different halves of the banks.
+template <int MODE, int GROUPS = 0>
 __global__ __launch_bounds__(512) void wgrad_kernel(Args a) {
   constexpr bool CONV = MODE == 1, PACKED = MODE == 2;
+  constexpr bool GA = GROUPS & 1, GB = GROUPS & 2;
+  static_assert(GROUPS == 0 || MODE == 0, "plain rows otherwise");
   typedef short v4i16 __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) v4i16 *lds_v4i16;
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -95,6 +100,17 @@ __global__ __launch_bounds__(512) void wgrad_kernel(Args a) {
     ua[k] = oa0 + unit * 8 < a.OA ? oa0 + unit * 8 : oa0;
     ub[k] = ob0 + unit * 8 < a.OB ? ob0 + unit * 8 : ob0;
   }
+  // by groups: this wave takes the groups 2 wave and 2 wave + 1 of the block, lane l the half l % 2 of row (l / 2) ^ 4 (group % 2)
+  int64_t gofs_a[2], gofs_b[2];
+  if constexpr (GROUPS != 0) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int row = (lane >> 1) ^ (4 * k);
+      const int ca = oa0 + 16 * (2 * wave + k), cb = ob0 + 16 * (2 * wave + k);
+      gofs_a[k] = (int64_t)((ca < a.OA ? ca : oa0) >> 4) * 512 + row * 16 + 8 * (lane & 1);
+      gofs_b[k] = (int64_t)((cb < a.OB ? cb : ob0) >> 4) * 512 + row * 16 + 8 * (lane & 1);
+    }
+  }
   const unsigned lds0 = (unsigned)(uintptr_t)ring + wave * 2048;
   // Convolution: the neighbour of row m at this tap is row m + shift where it lies inside the grid.  The grid coordinates
   // of a lane's two rows are divided out once and then advanced by the 32 rows of a stage with carries.
@@ -126,10 +142,13 @@ __global__ __launch_bounds__(512) void wgrad_kernel(Args a) {
           const int c = 2 * wave + k, cs = oa0 + 16 * c < a.OA ? oa0 / 16 + c : oa0 / 16;
           pa[k] = reinterpret_cast<const uint16_t *>(a.pack + ((int64_t)batch * a.tpb + blk) * a.tile_units + cs * 64 +
                                                      32 * g + (i ^ (4 * g) ^ (8 * k)));
+        } else if constexpr (GA) {
+          pa[k] = a.A + blk * 32 * a.lda + gofs_a[k];
         } else {
           pa[k] = a.A + mc * a.lda + ua[k];
         }
-        pb[k] = a.B + ((int64_t)batch * a.M + mc) * a.ldb + ub[k];
+        if constexpr (GB) pb[k] = a.B + blk * 32 * a.ldb + gofs_b[k];
+        else pb[k] = a.B + ((int64_t)batch * a.M + mc) * a.ldb + ub[k];
         if constexpr (CONV) {
           const int ii = ci[k] + du, jj = cj[k] + dv, ll = cl[k] + dz;
           const bool in = m < a.M && (unsigned)ii < (unsigned)gh && (unsigned)jj < (unsigned)gw && (unsigned)ll < (unsigned)gd;
@@ -153,6 +172,14 @@ __global__ __launch_bounds__(512) void wgrad_kernel(Args a) {
     const char *p = base + row_off + 16 * ks * 512 + 64 * ((col >> 5) ^ rr);
     const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16)(uintptr_t)p));
     const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16)(uintptr_t)(p + 4 * 512)));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  // by groups: the same rows and columns at [group][row][16 columns]
+  auto group_operand = [&](const char *base, int ks, int col) {
+    const char *p = base + ((col >> 4) + q1) * 1024 + (16 * ks + ((8 * g + rr) ^ (4 * q1))) * 32 + 8 * (l16 & 3);
+    const char *p4 = base + ((col >> 4) + q1) * 1024 + (16 * ks + ((8 * g + rr + 4) ^ (4 * q1))) * 32 + 8 * (l16 & 3);
+    const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16)(uintptr_t)p));
+    const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16)(uintptr_t)p4));
     return u32x4{lo[0], lo[1], hi[0], hi[1]};
   };
   // packed A: points 16 ks + 8 g + l16 / 4 (+ 4), group l16 % 4 of the chunk's four groups of four slices
@@ -198,9 +225,15 @@ __global__ __launch_bounds__(512) void wgrad_kernel(Args a) {
     for (int ks = 0; ks < 2; ++ks) {
       u32x4 af[2], bf[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) af[u] = PACKED ? packed_operand(at, ks, wa + 32 * u) : operand(at, ks, wa + 32 * u);
+      for (int u = 0; u < 2; ++u) {
+        if constexpr (GA) af[u] = group_operand(at, ks, wa + 32 * u);
+        else af[u] = PACKED ? packed_operand(at, ks, wa + 32 * u) : operand(at, ks, wa + 32 * u);
+      }
 #pragma unroll
-      for (int v = 0; v < 4; ++v) bf[v] = operand(bt, ks, wb + 32 * v);
+      for (int v = 0; v < 4; ++v) {
+        if constexpr (GB) bf[v] = group_operand(bt, ks, wb + 32 * v);
+        else bf[v] = operand(bt, ks, wb + 32 * v);
+      }
       if (valid < 32) {  // the last rows of all: those beyond M hold a repeated row and must not count, infinite or not
 #pragma unroll
         for (int v = 0; v < 4; ++v) bf[v] = masked(bf[v], ks, valid);
@@ -620,7 +653,7 @@ static int launch_narrow(const NarrowArgs &a, int64_t G, hipStream_t st) {
 }
 
 int launch_wide(const void *A, int64_t lda, int64_t OA, const void *B, int64_t ldb, int64_t OB, int64_t M, int64_t G,
-                const pa_shape *grid, float *partials, float *col_sums, hipStream_t st) {
+                const pa_shape *grid, float *partials, float *col_sums, hipStream_t st, int groups) {
   Args a{};
   a.A = static_cast<const uint16_t *>(A);
   a.B = static_cast<const uint16_t *>(B);
@@ -632,7 +665,7 @@ int launch_wide(const void *A, int64_t lda, int64_t OA, const void *B, int64_t l
   a.ny = (int)((OA + 255) / 256);
   a.nz = (int)((OB + 255) / 256) * a.grid.taps;
   a.partials = partials, a.col_sums = col_sums;
-  auto kernel = grid ? wgrad_kernel<1> : wgrad_kernel<0>;
+  auto kernel = grid ? wgrad_kernel<1> : groups == 1 ? wgrad_kernel<0, 1> : groups == 2 ? wgrad_kernel<0, 2> : wgrad_kernel<0>;
   const size_t lds = (size_t)kStages * kStageBytes;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)((G * a.ny * a.nz + 7) / 8 * 8)), dim3(512), lds, st, a);

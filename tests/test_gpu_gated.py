@@ -107,6 +107,8 @@ def test_many_rows(rows, C, F, act):
     y = PF.gated_mlp_forward(gpu["x"], *params, act=act)
     bare = values[0] - st["residual"].double()  # rounded relative to itself, not to its sum with the residual
     check(y, bare, tols[0] + torch.finfo(torch.bfloat16).eps / 2 * bare.abs(), "y without a residual")
+    for what, g, v, t in zip(("dx",) + NAMES, PF.gated_mlp_backward(gpu["x"], gpu["dy"], *params[:5], act=act), values[1:], tols[1:]):
+        check(g, v, t, what)
     x = gpu["x"].clone()
     x[17, 3], x[rows - 1, 0] = float("nan"), float("inf")
     hit = PF.gated_mlp_forward(x, *params, act=act)
