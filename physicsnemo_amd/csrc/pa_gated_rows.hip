@@ -78,6 +78,13 @@ struct RowsArgs {
 // Two LDS buffers, one barrier per slot.  CT = 8: one wave per SIMD with 512 registers (y 128, x 64, two sets of g and u 64);
 // narrower rows: two.
 // ---------------------------------------------------------------------------------------------------------------
+// Twenty ticks of vector work spread evenly behind the first 5 CT matrix instructions of a slot: those behind step S.
+template <int S, int CT, class F>
+__device__ __forceinline__ void ticks_behind(F &&tick) {
+  constexpr int first = (4 * S + CT - 1) / CT, end = (4 * (S + 1) + CT - 1) / CT;
+  static_for<end - first>([&](auto p_) { tick(std::integral_constant<int, first + decltype(p_)::value>{}); });
+}
+
 // One value of h in four pieces, so that what a piece depends on lies a step of the matrix instructions behind it.
 template <int ACT>
 struct Gate {
@@ -87,13 +94,13 @@ struct Gate {
     if constexpr (ACT == tile::kSilu) {
       t = -kLog2e * v;
     } else if constexpr (ACT == tile::kGelu) {
-      t = gelu_tail_arg(v);
-      q = gelu_lower_tail_upper_terms(t);
+      t = fabsf(v);
+      q = gelu_short_upper_terms(t);
     }
   }
   __device__ __forceinline__ void piece1() {
     if constexpr (ACT == tile::kSilu) t = __builtin_amdgcn_exp2f(t);
-    else if constexpr (ACT == tile::kGelu) q = __builtin_amdgcn_exp2f(gelu_lower_tail_lower_terms(t, q));
+    else if constexpr (ACT == tile::kGelu) q = __builtin_amdgcn_exp2f(gelu_short_lower_terms(t, q));
   }
   __device__ __forceinline__ void piece2() {
     if constexpr (ACT == tile::kSilu) t = __builtin_amdgcn_rcpf(1.f + t);
@@ -190,13 +197,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       // the 19 ticks are done before step 5 CT, which reads the upper half of h; the lower half, ready at tick 11, is read from step 4 CT on
       auto behind = [&](auto s_) {
         constexpr int S = decltype(s_)::value;
-        if constexpr (S < 5 * CT) {
-          if constexpr (CT == 8) {
-            if constexpr (S % 2 == 0) tick(std::integral_constant<int, S / 2>{});
-          } else {
-            static_for<4 / CT>([&](auto p_) { tick(std::integral_constant<int, S * (4 / CT) + decltype(p_)::value>{}); });
-          }
-        }
+        ticks_behind<S, CT>(tick);
       };
       static_for<NF>([&](auto s_) {
         constexpr int S = decltype(s_)::value;
@@ -484,11 +485,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
         else if constexpr (S % 3 == 1) ga[now] = mma(fr[S % RING], xb[S / 3], ga[now]);
         else da[now] = mma(fr[S % RING], db[S / 3], da[now]);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (CT == 8) {
-          if constexpr (S % 2 == 0) tick(std::integral_constant<int, S / 2>{});
-        } else {
-          static_for<4 / CT>([&](auto p_) { tick(std::integral_constant<int, S * (4 / CT) + decltype(p_)::value>{}); });
-        }
+        ticks_behind<S, CT>(tick);
         if constexpr (S == 1) fetch(buf ^ 1, c + 1 < NCH ? c + 1 : 0);  // past the last slot: the first of the next block
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -525,18 +522,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
 // ================================================================================================
 // host side
 // ================================================================================================
-static int channel_tiles(int64_t C) { return C <= 64 ? 2 : C <= 128 ? 4 : 8; }
+// tiles of 32 channels; five and six of them, rare widths, run as seven
+static int channel_tiles(int64_t C) { const int t = (int)((C + 31) / 32); return t == 5 || t == 6 ? 7 : t; }
 static int waves_of(int64_t C) { return C <= 128 ? 8 : 4; }
 
 bool rows_supported(int64_t C, int64_t F) { return C <= 256 && F <= 1 << 18; }
 
-// How many of M rows this kernel takes.  A round is one block of 32 rows per wave on every CU; less than a round costs as much, and the
-// tile kernels then have the smaller pieces: C = 256, F = 1024, rows / tiles (us): 16 384 rows 64 / 45, 32 768 74 / 78, 262 144 474 /
-// 582; C = 128, F = 512: 16 384 33 / 21, 32 768 34 / 34, 262 144 126 / 225.  Rows past the whole rounds go to the tile kernels where they
-// are less than half a round.
+// How many of M rows these kernels take.  A round is one block of 32 rows per wave on every CU; part of one costs as much, and the
+// tile kernels then have the smaller pieces.  Wide rows take long for a block, so that they need most of a round; rows of up to 64
+// channels are worth it always.  Forward, rows + 4 us for the weights / tiles (us): C = 256, F = 1024: 16 384 rows 59 / 45,
+// 32 768 71 / 78, 262 144 474 / 582; C = 200, F = 800: 32 768 43 / 60; C = 128, F = 512: 16 384 28 / 21, 32 768 28 / 34, 262 144
+// 124 / 225; C = 64, F = 256: 2 000 13 / 19, 32 768 13 / 20.  Rows past the whole rounds go to the tile kernels where they are less
+// than half a round.
 int64_t rows_worth(int64_t M, int64_t C, int num_cu) {
+  static const int least[9] = {0, 0, 0, 25, 45, 0, 0, 75, 85};  // per cent of a round, by channel tiles
   const int64_t block = 32 * waves_of(C), blocks = (M + block - 1) / block, rounds = blocks / num_cu, over = blocks - rounds * num_cu;
-  if (2 * over >= num_cu && (rounds > 0 || 10 * over >= (C <= 128 ? 6 : 9) * num_cu)) return M;
+  if (rounds == 0 ? 100 * over >= least[channel_tiles(C)] * num_cu : 2 * over >= num_cu) return M;
   const int64_t rows = rounds * num_cu * block;
   return rows < M ? rows : M;
 }
@@ -577,8 +578,11 @@ int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float 
   a.M = M, a.nblocks = (M + 32 * waves_of(C) - 1) / (32 * waves_of(C));
   a.C = (int)C, a.F = (int)F, a.act = act;
   switch (channel_tiles(C)) {
+    case 1: return launch_rows<1, 8>(a, num_cu, st);
     case 2: return launch_rows<2, 8>(a, num_cu, st);
+    case 3: return launch_rows<3, 8>(a, num_cu, st);
     case 4: return launch_rows<4, 8>(a, num_cu, st);
+    case 7: return launch_rows<7, 4>(a, num_cu, st);
     default: return launch_rows<8, 4>(a, num_cu, st);
   }
 }
@@ -620,8 +624,11 @@ int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void
   a.M = M, a.nblocks = (M + 32 * waves_of(C) - 1) / (32 * waves_of(C));
   a.C = (int)C, a.F = (int)F, a.Fp = (int)Fp, a.act = act;
   switch (channel_tiles(C)) {
+    case 1: return launch_hidden<1, 8>(a, num_cu, st);
     case 2: return launch_hidden<2, 8>(a, num_cu, st);
+    case 3: return launch_hidden<3, 8>(a, num_cu, st);
     case 4: return launch_hidden<4, 8>(a, num_cu, st);
+    case 7: return launch_hidden<7, 4>(a, num_cu, st);
     default: return launch_hidden<8, 4>(a, num_cu, st);
   }
 }

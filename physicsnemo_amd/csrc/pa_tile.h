@@ -78,11 +78,12 @@ enum Act { kNone = 0, kGelu = 1, kRelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5, 
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v)); }
 
+template <bool SHORT>  // rounded to bf16 next
 __device__ __forceinline__ void act_values(int act, f32x16 &v) {
   switch (act) {
     case kGelu:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = gelu_tail(v[r]);
+      for (int r = 0; r < 16; ++r) v[r] = SHORT ? gelu_short(v[r]) : gelu_tail(v[r]);
       break;
     case kRelu:  // NaN passes, as torch's does
 #pragma unroll
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           for (int n = 0; n < TN; ++n) {
             if (n + 1 < TN) ask(n + 1);
             f32x16 v = values_of<E>(acc[m][n], bias_of(n), scale_of(n), g, sx);
-            act_values(a.act, v);
+            act_values<sizeof(TO) == 2>(a.act, v);
             if (a.residual) {
 #pragma unroll
               for (int r = 0; r < 16; ++r) v[r] += add[n & 1][r / 4][r % 4];
@@ -566,7 +567,7 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
 #pragma unroll
           for (int n = 0; n < TN; ++n) {
             f32x16 v = values_of<E>(acc[m][n], bias_of(n), scale_of(n), g, sx);
-            act_values(a.act, v);
+            act_values<sizeof(TO) == 2>(a.act, v);
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int c = tn * CN + (wn * TN + n) * 32 + rowmap(r, g);
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
             }
           };
           if constexpr (KIND == kGated) {
-            act_values(a.act, gate);
+            act_values<sizeof(TO) == 2>(a.act, gate);
 #pragma unroll
             for (int r = 0; r < 16; ++r) gate[r] *= up[r];
             cut(gate);
@@ -651,21 +652,57 @@ int launch_tiles(Args a, int num_cu, hipStream_t st) {
 // Tiles of 256 x 256 (kBack: 128 x 256) for large products, 128 x 128 and two workgroups per CU where those leave CUs idle, 64 x 64
 // where the product is small.  Taken by the weight rows and rows that the busiest CU has to work off, smaller tiles counted
 // dearer for the operands they fetch again.  Measured at 256 / 128 (us): 131 072 rows, 1 024 -> 256 bf16 107 / 117, 2 048 -> 256
-// 162 / 189, 256 -> 2 x 1 024 201 / 227; 100 003 rows, 1 368 -> 512 247 / 234; int8 131 072 rows 2 048 -> 512 144 / 193; float32
-// 28 900 rows, 512 -> 128 126 / 43.
+// 162 / 189, 256 -> 2 x 1 024 201 / 227; int8 131 072 rows 2 048 -> 512 144 / 193; float32 28 900 rows, 512 -> 128 126 / 43.
+// Rows past whole rounds of large tiles go to a launch of smaller ones where that is the shorter way: 100 003 rows, 1 368 -> 512,
+// three rounds and 1 699 rows: 254 -> 214 us.
+struct Plan {
+  int64_t rows;  // on tiles of `size`; the rest on tiles of their own
+  int size;      // 0 large, 1 medium, 2 small
+  double cost;   // in stages of a large tile
+};
+inline Plan plan_of(int64_t M, int64_t N, int64_t stages, bool back, bool pairs, int num_cu, bool split) {
+  const double launch = 2.5;  // of one more launch: about 8 us
+  auto cost = [&](int64_t rows, int64_t bm, int64_t bn, double dearer) {
+    const int64_t cn = pairs ? bn / 2 : bn, tiles = ((rows + bm - 1) / bm) * ((N + cn - 1) / cn);
+    return (double)((tiles + num_cu - 1) / num_cu) * bm * bn * dearer * stages / 65536;
+  };
+  const int64_t bm = back ? 128 : 256;
+  const double of[3] = {cost(M, bm, 256, 1.0), cost(M, 128, 128, 1.13), cost(M, 64, 64, 1.5)};
+  Plan p{M, of[0] <= of[1] && of[0] <= of[2] ? 0 : of[1] <= of[2] ? 1 : 2, 0.0};
+  p.cost = of[p.size];
+  if (split) {
+    const int64_t cn = pairs ? 128 : 256, nt = (N + cn - 1) / cn, rounds = (M / bm) * nt / num_cu, rows = rounds * num_cu / nt * bm;
+    if (rounds > 0 && rows < M) {
+      const double c = cost(rows, bm, 256, 1.0) + launch + plan_of(M - rows, N, stages, back, pairs, num_cu, false).cost;
+      if (c < p.cost) return Plan{rows, 0, c};
+    }
+  }
+  return p;
+}
+
 template <class E, class TO, Kind KIND>
-int launch(const Args &a, int num_cu, hipStream_t st) {
+int launch(Args a, int num_cu, hipStream_t st) {
   using Large = typename std::conditional<KIND == kBack, Config<2, 4, 2, 2, 8, 3, 2>, Config<4, 2, 2, 4, 8, 2, 2>>::type;
   using Medium = Config<2, 2, 2, 2, 8, 2, 2>;
   using Small = Config<2, 1, 1, 2, 8, 3, 2>;
-  auto cost = [&](int64_t bm, int64_t bn, double dearer) {
-    const int64_t cn = KIND == kPlain ? bn : bn / 2, tiles = ((a.M + bm - 1) / bm) * ((a.N + cn - 1) / cn);
-    return (double)((tiles + num_cu - 1) / num_cu) * bm * bn * dearer;
+  const int64_t stages = (a.units + 7) / 8 + (KIND == kBack ? (a.units2 + 7) / 8 : 0);
+  auto run = [&](const Args &t, int size) {
+    if (size == 0) return launch_tiles<E, TO, KIND, Large>(t, num_cu, st);
+    if (size == 1) return launch_tiles<E, TO, KIND, Medium>(t, num_cu, st);
+    return launch_tiles<E, TO, KIND, Small>(t, num_cu, st);
   };
-  const double l = cost(Large::BM, Large::BN, 1.0), m = cost(Medium::BM, Medium::BN, 1.13), s = cost(Small::BM, Small::BN, 1.5);
-  if (l <= m && l <= s) return launch_tiles<E, TO, KIND, Large>(a, num_cu, st);
-  if (m <= s) return launch_tiles<E, TO, KIND, Medium>(a, num_cu, st);
-  return launch_tiles<E, TO, KIND, Small>(a, num_cu, st);
+  const Plan p = plan_of(a.M, a.N, stages, KIND == kBack, KIND != kPlain, num_cu, true);
+  Args rest = a;
+  a.M = p.rows;
+  int rc = run(a, p.size);
+  if (rc || p.rows == rest.M) return rc;
+  auto past = [&](const void *q, int64_t row) { return q ? const_cast<char *>(static_cast<const char *>(q)) + p.rows * row : nullptr; };
+  rest.M -= p.rows;
+  rest.X = past(a.X, a.ldx), rest.X2 = past(a.X2, a.ldx2);
+  rest.sx = a.sx ? a.sx + p.rows : nullptr;
+  rest.residual = past(a.residual, a.ldo * (int64_t)sizeof(TO));
+  rest.out = past(a.out, a.ldo * (int64_t)sizeof(TO)), rest.out2 = past(a.out2, a.ldh * (int64_t)sizeof(TO));
+  return run(rest, plan_of(rest.M, a.N, stages, KIND == kBack, KIND != kPlain, num_cu, false).size);
 }
 
 // ---- host side of the calls that use the products ----
