@@ -714,11 +714,11 @@ int pa_gated_mlp_backward(int dtype, int64_t rows, int64_t C, int64_t F, const p
 int pa_dropout_add_norm(int dtype, int64_t rows, int64_t C, const void *x, const void *residual, double p, const int64_t *rng,
                         void *y, const float *gamma, const float *beta, float eps, void *normed, float *stats, void *stream);
 /* Its backward pass under the same rng values: ds = dy + the LayerNorm's input gradient for d_normed; d_residual = ds,
- * dx = ds kept and scaled; grads (2, C) float32 = d gamma, d beta.  dy or NULL (zero); d_normed NULL: no LayerNorm, and y,
- * stats, gamma, d_residual and grads are not used.  dx, d_residual, grads: NULL if not wanted. */
+ * dx = ds kept and scaled; grads (2, C) float32 = d gamma, d beta.  dy or NULL (zero); d_normed NULL: no LayerNorm, and x,
+ * residual, stats, gamma, d_residual and grads are not used.  dx, d_residual, grads: NULL if not wanted. */
 int64_t pa_dropout_add_norm_backward_workspace_bytes(int dtype, int64_t rows, int64_t C);
-int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *y,
-                                 const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
+int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *x,
+                                 const void *residual, const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
                                  float *grads, void *workspace, int64_t workspace_bytes, void *stream);
 /* taken <- state, then state's offset + 1: the values one call and its backward pass use. */
 int pa_dropout_advance(int64_t *state, int64_t *taken, void *stream);

@@ -356,7 +356,7 @@ def load() -> ctypes.CDLL:
     lib.pa_dropout_add_norm_backward_workspace_bytes.restype = c_int64
     lib.pa_dropout_add_norm_backward_workspace_bytes.argtypes = [c_int, c_int64, c_int64]
     lib.pa_dropout_add_norm_backward.restype = c_int
-    lib.pa_dropout_add_norm_backward.argtypes = [c_int, c_int64, c_int64] + [c_void_p] * 5 + [c_double] + [c_void_p] * 5 + [
+    lib.pa_dropout_add_norm_backward.argtypes = [c_int, c_int64, c_int64] + [c_void_p] * 6 + [c_double] + [c_void_p] * 5 + [
         c_int64, c_void_p]
     lib.pa_dropout_advance.restype = c_int
     lib.pa_dropout_advance.argtypes = [c_void_p] * 3

@@ -1059,14 +1059,14 @@ class DropoutAddNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, rng, ln_weight, ln_bias, eps):
         ctx.set_materialize_grads(False)
-        ctx.p, ctx.has_residual = p, residual is not None
+        ctx.p, ctx.dtype = p, x.dtype
         if ln_weight is None:
             ctx.save_for_backward(rng)
             ctx.ln_dtypes = None
             return PF.dropout_add_norm(x, residual, p, rng)
         w32 = ln_weight.detach().float().contiguous()
         y, normed, stats = PF.dropout_add_norm(x, residual, p, rng, w32, ln_bias.detach().float().contiguous(), eps, True)
-        ctx.save_for_backward(rng, y, stats, w32)
+        ctx.save_for_backward(rng, x, residual, stats, w32)
         ctx.ln_dtypes = (ln_weight.dtype, ln_bias.dtype)
         return y, normed
 
@@ -1077,14 +1077,13 @@ class DropoutAddNormFunction(torch.autograd.Function):
         if dy is None and d_normed is None:
             return (None,) * 7
         rng, *saved = ctx.saved_tensors
-        like = saved[0] if saved else dy
-        dy = None if dy is None else dy.to(like.dtype).contiguous()
+        dy = None if dy is None else dy.to(ctx.dtype).contiguous()
         if d_normed is None:
-            dx, dr, _, _ = PF.dropout_add_norm_backward(dy, None, None, None, None, ctx.p, rng, need[0], need[1])
+            dx, dr, _, _ = PF.dropout_add_norm_backward(dy, None, None, None, None, None, ctx.p, rng, need[0], need[1])
             return dx, dr, None, None, None, None, None
-        y, stats, w32 = saved
-        dx, dr, dg, db = PF.dropout_add_norm_backward(dy, d_normed.to(y.dtype).contiguous(), y, stats, w32, ctx.p, rng, need[0],
-                                                      need[1], need[4] or need[5])
+        x, residual, stats, w32 = saved
+        dx, dr, dg, db = PF.dropout_add_norm_backward(dy, d_normed.to(ctx.dtype).contiguous(), x, residual, stats, w32, ctx.p, rng,
+                                                      need[0], need[1], need[4] or need[5])
         return (dx, dr, None, None, dg.to(ctx.ln_dtypes[0]) if need[4] else None, db.to(ctx.ln_dtypes[1]) if need[5] else None, None)
 
 

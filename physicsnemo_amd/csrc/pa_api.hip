@@ -1950,18 +1950,18 @@ int64_t pa_dropout_add_norm_backward_workspace_bytes(int dtype, int64_t rows, in
   return pa::dropout::backward_workspace_bytes(dtype, rows, C, compute_units());
 }
 
-int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *y,
-                                 const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
+int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void *dy, const void *d_normed, const void *x,
+                                 const void *residual, const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual,
                                  float *grads, void *workspace, int64_t workspace_bytes, void *stream) {
   Range entry("pa_dropout_add_norm_backward");
   const int64_t need = pa_dropout_add_norm_backward_workspace_bytes(dtype, rows, C);
   if (need < 0) return (int)need;
   if (!(p >= 0.0 && p <= 1.0)) return PA_ERR_DIMS;
   if (!rng || (!dy && !d_normed)) return PA_ERR_NULL;
-  if (d_normed && (!y || !stats || !gamma || (grads && !workspace))) return PA_ERR_NULL;
+  if (d_normed && (!x || !stats || !gamma || (grads && !workspace))) return PA_ERR_NULL;
   if (d_normed && grads && !aligned16(workspace)) return PA_ERR_ALIGN;
   if (d_normed && grads && workspace_bytes < need) return PA_ERR_WORKSPACE;
-  return pa::dropout::backward(dtype, rows, C, dy, d_normed, y, stats, gamma, p, rng, dx, d_residual, grads, workspace,
+  return pa::dropout::backward(dtype, rows, C, dy, d_normed, x, residual, stats, gamma, p, rng, dx, d_residual, grads, workspace,
                                compute_units(), static_cast<hipStream_t>(stream));
 }
 

@@ -1,15 +1,16 @@
 // Dropout, residual add and LayerNorm of rows in one pass, forward and backward, with a mask that is formed from a counter on
 // both ways and never stored:
 //   y = residual + keep x / (1 - p),  n = (y - mean) rstd gamma + beta
-//   ds = dy + rstd (t - mean_c(t) - xh mean_c(t xh)),  t = dn gamma,  xh = (y - mean) rstd
+//   ds = dy + rstd (t - mean_c(t) - xh mean_c(t xh)),  t = dn gamma,  xh = (s - mean) rstd,  s the sum before its rounding to y
 //   d residual = ds,  dx = keep ds / (1 - p),  d gamma = sum_rows dn xh,  d beta = sum_rows dn
 // keep(r, c): word c % 4 of Philox4x32-10 (J. K. Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", SC 2011) of the
 // counter (c / 4, r mod 2^32, r / 2^32, offset) under the 64-bit seed is at least p 2^32.  It depends on the element's place
 // alone, not on types, alignment or launches.  Seed and offset are read from device memory, so that a captured graph draws a
 // new mask on every replay when the offset is advanced in it.
 //
-// Sums, statistics and all arithmetic are float32.  n is formed from the sum before its rounding to y, the backward pass takes
-// xh from the rounded y with the statistics of the unrounded rows.
+// Sums, statistics and all arithmetic are float32.  n is formed from the sum before its rounding to y, and the backward pass forms
+// that sum again from x and the residual, which costs one read more than y and keeps d gamma as exact as float32 sums are (from
+// the rounded y: 2e-3 off).
 #include "pa_common.h"
 #include "pa_host.h"
 #include "pa_mfma_ops.h"
@@ -50,16 +51,25 @@ __device__ __forceinline__ Stream stream_of(const Mask &m) {
   const uint64_t seed = (uint64_t)m.rng[0];
   return {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)m.rng[1]};
 }
-// v[j] <- keep ? v[j] * scale : 0 for the VEC columns from col (a multiple of 4) of a row
+// which of the VEC columns from col (a multiple of 4) of a row are kept, a bit each
 template <int VEC>
-__device__ __forceinline__ void apply(const Mask &m, const Stream &s, int64_t row, int col, float (&v)[VEC]) {
-  if (m.all) return;
+__device__ __forceinline__ uint32_t kept(const Mask &m, const Stream &s, int64_t row, int col) {
+  if (m.all) return 0xffu;
+  if (m.none) return 0u;
+  uint32_t bits = 0;
 #pragma unroll
   for (int q = 0; q < VEC / 4; ++q) {
     const Words w = philox((uint32_t)(col >> 2) + q, (uint32_t)row, (uint32_t)((uint64_t)row >> 32), s.offset, s.k0, s.k1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[4 * q + j] = w.w[j] >= m.threshold && !m.none ? v[4 * q + j] * m.scale : 0.f;
+    for (int j = 0; j < 4; ++j) bits |= w.w[j] >= m.threshold ? 1u << (4 * q + j) : 0u;
   }
+  return bits;
+}
+// v[j] <- keep ? v[j] * scale : 0
+template <int VEC>
+__device__ __forceinline__ void apply(uint32_t bits, float scale, float (&v)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[j] = bits >> j & 1u ? v[j] * scale : 0.f;
 }
 
 // ---- VEC neighbouring elements of a row, 16 bytes; UNITS: rows are whole 16-byte units.  Rows that are not start on any
@@ -143,7 +153,7 @@ __device__ __forceinline__ float group_sum(float v, float *red) {
 }
 
 struct Args {
-  const void *x, *residual, *y, *dy, *dn;
+  const void *x, *residual, *dy, *dn;
   void *out_y, *out_n, *dx, *d_residual;
   const float *gamma, *beta;
   float *stats;     // (M, 2): mean, rstd
@@ -158,7 +168,7 @@ struct Args {
 // rows_forward_kernel, rows_backward_kernel.  LANES lanes (256: the workgroup) share a row, each NCH pieces of VEC neighbouring columns, so that a row
 // is read once and stays in registers; a workgroup of four waves walks the rows.  In the backward pass a lane adds d gamma and d beta
 // of its columns up over all its rows; the workgroup's sums become one partial result, added up in a fixed order by one more
-// small launch.  Bound by HBM: (3 + norm) element reads and writes forward, 5 backward; the generator's twenty 32 x 32 bit
+// small launch.  Bound by HBM: (3 + norm) element reads and writes forward, 6 backward; the generator's twenty 32 x 32 bit
 // products per four elements run behind them.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int VEC, bool UNITS, int LANES, int NCH, bool NORM>
@@ -191,7 +201,7 @@ __global__ __launch_bounds__(256) void rows_forward_kernel(Args a) {
       float r[VEC];
       load<T, VEC, UNITS>(static_cast<const T *>(a.x) + at, col, C, s[k]);
       if (a.residual) load<T, VEC, UNITS>(static_cast<const T *>(a.residual) + at, col, C, r);
-      apply(a.mask, rng, row, col, s[k]);
+      apply(kept<VEC>(a.mask, rng, row, col), a.mask.scale, s[k]);
       if (a.residual) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) s[k][j] += r[j];
@@ -245,6 +255,7 @@ __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
   for (int64_t row = (int64_t)blockIdx.x * ROWS + group; row < a.M; row += (int64_t)gridDim.x * ROWS) {
     const int64_t at = row * C;
     float ds[NCH][VEC];
+    uint32_t bits[NCH];
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int col = (k * LANES + lane) * VEC;
@@ -262,11 +273,15 @@ __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         const int col = (k * LANES + lane) * VEC;
-        load<T, VEC, UNITS>(static_cast<const T *>(a.y) + at, col, C, xh[k]);
+        float r[VEC];
+        load<T, VEC, UNITS>(static_cast<const T *>(a.x) + at, col, C, xh[k]);
         load<T, VEC, UNITS>(static_cast<const T *>(a.dn) + at, col, C, t[k]);
+        if (a.residual) load<T, VEC, UNITS>(static_cast<const T *>(a.residual) + at, col, C, r);
+        bits[k] = kept<VEC>(a.mask, rng, row, col);
+        apply(bits[k], a.mask.scale, xh[k]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          xh[k][j] = (xh[k][j] - mean) * rstd;
+          xh[k][j] = ((a.residual ? xh[k][j] + r[j] : xh[k][j]) - mean) * rstd;
           dg[k][j] = fmaf(t[k][j], xh[k][j], dg[k][j]);
           db[k][j] += t[k][j];
           t[k][j] *= gamma[k][j];  // 0 past the last column
@@ -287,7 +302,8 @@ __global__ __launch_bounds__(256) void rows_backward_kernel(Args a) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         const int col = (k * LANES + lane) * VEC;
-        apply(a.mask, rng, row, col, ds[k]);
+        if constexpr (!NORM) bits[k] = kept<VEC>(a.mask, rng, row, col);
+        apply(bits[k], a.mask.scale, ds[k]);
         store<T, VEC, UNITS>(static_cast<T *>(a.dx) + at, col, C, ds[k]);
       }
     }
@@ -348,7 +364,7 @@ __global__ __launch_bounds__(kWideThreads) void long_rows_forward_kernel(Args a)
     auto sums = [&](int col, float (&s)[VEC]) {
       float r[VEC];
       load<T, VEC, UNITS>(static_cast<const T *>(a.x) + at, col, C, s);
-      apply(a.mask, rng, row, col, s);
+      apply(kept<VEC>(a.mask, rng, row, col), a.mask.scale, s);
       if (!a.residual) return;
       load<T, VEC, UNITS>(static_cast<const T *>(a.residual) + at, col, C, r);
 #pragma unroll
@@ -399,14 +415,19 @@ __global__ __launch_bounds__(kWideThreads) void long_rows_backward_kernel(Args a
   for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
     const int64_t at = row * C;
     float mean = 0.f, rstd = 0.f, s1 = 0.f, s2 = 0.f;
-    auto parts = [&](int col, float (&t)[VEC], float (&xh)[VEC]) {
-      load<T, VEC, UNITS>(static_cast<const T *>(a.y) + at, col, C, xh);
+    auto parts = [&](int col, float (&t)[VEC], float (&xh)[VEC]) {  // returns which columns are kept
+      float r[VEC];
+      load<T, VEC, UNITS>(static_cast<const T *>(a.x) + at, col, C, xh);
       load<T, VEC, UNITS>(static_cast<const T *>(a.dn) + at, col, C, t);
+      if (a.residual) load<T, VEC, UNITS>(static_cast<const T *>(a.residual) + at, col, C, r);
+      const uint32_t bits = kept<VEC>(a.mask, rng, row, col);
+      apply(bits, a.mask.scale, xh);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        xh[j] = (xh[j] - mean) * rstd;
+        xh[j] = ((a.residual ? xh[j] + r[j] : xh[j]) - mean) * rstd;
         t[j] *= col + j < C ? a.gamma[col + j] : 0.f;
       }
+      return bits;
     };
     float t[VEC], xh[VEC];
     if constexpr (NORM) {
@@ -421,6 +442,7 @@ __global__ __launch_bounds__(kWideThreads) void long_rows_backward_kernel(Args a
     }
     for (int col = threadIdx.x * VEC; col < C; col += kWideThreads * VEC) {
       float ds[VEC];
+      uint32_t bits = 0;
       if (a.dy) {
         load<T, VEC, UNITS>(static_cast<const T *>(a.dy) + at, col, C, ds);
       } else {
@@ -428,13 +450,14 @@ __global__ __launch_bounds__(kWideThreads) void long_rows_backward_kernel(Args a
         for (int j = 0; j < VEC; ++j) ds[j] = 0.f;
       }
       if constexpr (NORM) {
-        parts(col, t, xh);
+        bits = parts(col, t, xh);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) ds[j] = fmaf(rstd, t[j] - s1 - xh[j] * s2, ds[j]);
         if (a.d_residual) store<T, VEC, UNITS>(static_cast<T *>(a.d_residual) + at, col, C, ds);
       }
       if (a.dx) {
-        apply(a.mask, rng, row, col, ds);
+        if constexpr (!NORM) bits = kept<VEC>(a.mask, rng, row, col);
+        apply(bits, a.mask.scale, ds);
         store<T, VEC, UNITS>(static_cast<T *>(a.dx) + at, col, C, ds);
       }
     }
@@ -447,10 +470,14 @@ __global__ __launch_bounds__(256) void long_rows_grads_kernel(Args a, int64_t pe
   const int c = blockIdx.y * 256 + threadIdx.x;
   if (c >= a.C) return;
   const int64_t r0 = (int64_t)blockIdx.x * per, r1 = r0 + per < a.M ? r0 + per : a.M;
+  const Stream rng = stream_of(a.mask);
   float dg = 0.f, db = 0.f;
   for (int64_t r = r0; r < r1; ++r) {
     const float t = load_as_f32(static_cast<const T *>(a.dn) + r * a.C + c);
-    const float xh = (load_as_f32(static_cast<const T *>(a.y) + r * a.C + c) - a.stats[2 * r]) * a.stats[2 * r + 1];
+    const bool keep = kept<4>(a.mask, rng, r, c & ~3) >> (c & 3) & 1u;
+    const float s = (keep ? load_as_f32(static_cast<const T *>(a.x) + r * a.C + c) * a.mask.scale : 0.f) +
+                    (a.residual ? load_as_f32(static_cast<const T *>(a.residual) + r * a.C + c) : 0.f);
+    const float xh = (s - a.stats[2 * r]) * a.stats[2 * r + 1];
     dg = fmaf(t, xh, dg);
     db += t;
   }
@@ -577,15 +604,15 @@ int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int num_cu) {
   return most * 2 * C * 4;
 }
 
-int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_normed, const void *y, const float *stats,
-             const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual, float *grads, void *workspace, int num_cu,
+int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_normed, const void *x, const void *residual,
+             const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual, float *grads, void *workspace, int num_cu,
              hipStream_t st) {
   Args a{};
-  a.dy = dy, a.dn = d_normed, a.y = y, a.dx = dx, a.d_residual = d_residual;
+  a.dy = dy, a.dn = d_normed, a.x = x, a.residual = residual, a.dx = dx, a.d_residual = d_residual;
   a.gamma = gamma, a.stats = const_cast<float *>(stats);
   a.partials = grads ? static_cast<float *>(workspace) : nullptr;
   a.M = M, a.C = (int)C, a.mask = mask_of(p, rng);
-  const bool aligned = aligned16(dy) && aligned16(d_normed) && aligned16(y) && aligned16(dx) && aligned16(d_residual);
+  const bool aligned = aligned16(dy) && aligned16(d_normed) && aligned16(x) && aligned16(residual) && aligned16(dx) && aligned16(d_residual);
   const Shape s = shape_of(dtype, C, aligned);
   int rc = launch(dtype, a, s, false, d_normed != nullptr, num_cu, st);
   if (!rc && grads && d_normed) rc = wgrad::sum_rows(a.partials, partials_of(s, M, C, num_cu), 2 * C, grads, st);

@@ -188,8 +188,8 @@ int advance(int64_t *state, int64_t *taken, hipStream_t st);
 int forward(int dtype, int64_t M, int64_t C, const void *x, const void *residual, double p, const int64_t *rng, void *y,
             const float *gamma, const float *beta, float eps, void *normed, float *stats, int num_cu, hipStream_t st);
 int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int num_cu);
-int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_normed, const void *y, const float *stats,
-             const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual, float *grads, void *workspace, int num_cu,
+int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_normed, const void *x, const void *residual,
+             const float *stats, const float *gamma, double p, const int64_t *rng, void *dx, void *d_residual, float *grads, void *workspace, int num_cu,
              hipStream_t st);
 }  // namespace dropout
 

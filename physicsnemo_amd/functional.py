@@ -1280,24 +1280,24 @@ def dropout_add_norm(x, residual, p: float, rng, ln_weight=None, ln_bias=None, l
     return (*out, stats) if stats is not None else out
 
 
-def dropout_add_norm_backward(dy, d_normed, y, stats, ln_weight, p: float, rng, need_dx: bool = True, need_residual: bool = True,
-                              need_ln: bool = True):
+def dropout_add_norm_backward(dy, d_normed, x, residual, stats, ln_weight, p: float, rng, need_dx: bool = True,
+                              need_residual: bool = True, need_ln: bool = True):
     """(dx, d residual, d ln_weight, d ln_bias) of `dropout_add_norm` under the rng values it ran with, from the gradients
-    of y and of the normalised rows (dy None: zero; d_normed None: no LayerNorm, y, stats and ln_weight are not used,
+    of y and of the normalised rows (dy None: zero; d_normed None: no LayerNorm: x, residual, stats and ln_weight are not used,
     d residual is dy itself and the LayerNorm's gradients None)."""
     rows_like = dy if d_normed is None else d_normed
     if rows_like is None:
         raise ValueError("dy or d_normed has to be given")
     norm = d_normed is not None
-    _dropout_args(rows_like, p, rng, dy, d_normed, *((y,) if norm else ()))
+    if norm and (x is None or stats is None or ln_weight is None):
+        raise ValueError("a gradient of the normalised rows needs x, stats and ln_weight")
+    _dropout_args(rows_like, p, rng, dy, d_normed, *((x, residual) if norm else ()))
     C = rows_like.shape[-1]
     rows = rows_like.numel() // C if C else 0
     device = rows_like.device
     if norm:
         _need_cuda(stats, ln_weight)
         _same_device(rows_like, stats, ln_weight)
-        if y is None or stats is None or ln_weight is None:
-            raise ValueError("a gradient of the normalised rows needs y, stats and ln_weight")
         _expect(stats, "stats", (rows, 2), torch.float32)
         _expect(ln_weight, "ln_weight", (C,), torch.float32)
     dx = torch.empty_like(rows_like) if need_dx else None
@@ -1309,10 +1309,11 @@ def dropout_add_norm_backward(dy, d_normed, y, stats, ln_weight, p: float, rng, 
             nbytes = _sized(lib.pa_dropout_add_norm_backward_workspace_bytes(code, rows, C),
                             "pa_dropout_add_norm_backward_workspace_bytes") if grads is not None else 0
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            used = [_lib.ptr(t) if norm else None for t in (x, residual, stats, ln_weight)]
             _lib.check(lib.pa_dropout_add_norm_backward(
-                code, rows, C, _lib.ptr(dy), _lib.ptr(d_normed), _lib.ptr(y) if norm else None, _lib.ptr(stats) if norm else None,
-                _lib.ptr(ln_weight) if norm else None, p, rng.data_ptr(), _lib.ptr(dx), _lib.ptr(d_residual) if norm else None,
-                _lib.ptr(grads), workspace.data_ptr(), nbytes, _lib.current_stream_ptr(device)), "pa_dropout_add_norm_backward")
+                code, rows, C, _lib.ptr(dy), _lib.ptr(d_normed), *used, p, rng.data_ptr(), _lib.ptr(dx),
+                _lib.ptr(d_residual) if norm else None, _lib.ptr(grads), workspace.data_ptr(), nbytes,
+                _lib.current_stream_ptr(device)), "pa_dropout_add_norm_backward")
     return (dx, d_residual, *((None, None) if grads is None else (grads[0], grads[1])))
 
 

@@ -65,9 +65,9 @@ def test_arguments_of_dropout():
     assert call(x=None) == call(rng=None) == call(y=None) == call(n=P) == call(n=P, gamma=P) == call(n=P, beta=P) == -1
     need = lib.pa_dropout_add_norm_backward_workspace_bytes(1, 1000, 64)
     assert need > 0 and lib.pa_dropout_add_norm_backward_workspace_bytes(1, 0, 64) == -2
-    back = lambda dy=P, dn=P, y=P, stats=P, gamma=P, p=0.5, rng=P, grads=P, ws=P, n=need: lib.pa_dropout_add_norm_backward(
-        1, 1000, 64, dy, dn, y, stats, gamma, p, rng, P, P, grads, ws, n, None)
-    assert back(dy=None, dn=None) == back(rng=None) == back(y=None) == back(stats=None) == back(gamma=None) == back(ws=None) == -1
+    back = lambda dy=P, dn=P, x=P, stats=P, gamma=P, p=0.5, rng=P, grads=P, ws=P, n=need: lib.pa_dropout_add_norm_backward(
+        1, 1000, 64, dy, dn, x, None, stats, gamma, p, rng, P, P, grads, ws, n, None)
+    assert back(dy=None, dn=None) == back(rng=None) == back(x=None) == back(stats=None) == back(gamma=None) == back(ws=None) == -1
     assert back(p=2.0) == -2 and back(ws=ctypes.c_void_p(4)) == -4 and back(n=need - 1) == -5
     assert lib.pa_dropout_advance(None, P, None) == lib.pa_dropout_advance(P, None, None) == -1
 
@@ -99,7 +99,7 @@ def test_tensors_on_the_cpu_are_refused():
     x, w, v = torch.zeros(4, 8), torch.zeros(8, 8), torch.zeros(8)
     state, codes = torch.zeros(2, dtype=torch.int64), torch.zeros(8, 8, dtype=torch.int8)
     for call in (lambda: PF.gated_mlp_forward(x, w, v, w, v, w, v), lambda: PF.gated_mlp_backward(x, x, w, v, w, v, w),
-                 lambda: PF.dropout_add_norm(x, x, 0.1, state), lambda: PF.dropout_add_norm_backward(x, None, None, None, None, 0.1, state),
+                 lambda: PF.dropout_add_norm(x, x, 0.1, state), lambda: PF.dropout_add_norm_backward(x, None, None, None, None, None, 0.1, state),
                  lambda: PF.dropout_advance(state), lambda: PF.quantize_int8(x), lambda: PF.linear_int8(x, codes, v),
                  lambda: PF.gated_mlp_int8(x, codes, v, v, codes, v, v, codes, v, v)):
         with pytest.raises(RuntimeError, match="GPU tensors only"):
