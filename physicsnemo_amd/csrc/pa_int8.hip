@@ -79,6 +79,7 @@ struct Quantize {
   int64_t M, K, ldx, ldq;  // elements; bytes
   uint8_t *q;
   float *scale;
+  uint32_t *clear;  // (M) set to zero, or NULL
 };
 
 template <class T, int LANES, int NCH, int ROWS, bool VEC>
@@ -142,6 +143,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(Quantize a) {
         store(k, w);
       }
       if (lane == 0) a.scale[row] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
+      if (lane == 0 && a.clear) a.clear[row] = 0u;
     }
   }
 }
@@ -167,12 +169,15 @@ static int quantize(const Quantize &a, int num_cu, hipStream_t st) {
   return go(quantize_rows_kernel<T, 64, 4, 1, VEC>, 4);
 }
 
-int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, int num_cu,
-                  hipStream_t st) {
-  const Quantize a{x, M, K, ldx, ldq, static_cast<uint8_t *>(q), scale};
-  const bool vec = whole_rows(x, ldx, dtype == PA_F32 ? 4 : 2);
+static int quantize(int dtype, const Quantize &a, int num_cu, hipStream_t st) {
+  const bool vec = whole_rows(a.x, a.ldx, dtype == PA_F32 ? 4 : 2);
   if (dtype == PA_F32) return vec ? quantize<float, true>(a, num_cu, st) : quantize<float, false>(a, num_cu, st);
   return vec ? quantize<bf16, true>(a, num_cu, st) : quantize<bf16, false>(a, num_cu, st);
+}
+
+int quantize_rows(int dtype, int64_t M, int64_t K, const void *x, int64_t ldx, void *q, int64_t ldq, float *scale, int num_cu,
+                  hipStream_t st) {
+  return quantize(dtype, Quantize{x, M, K, ldx, ldq, static_cast<uint8_t *>(q), scale, nullptr}, num_cu, st);
 }
 
 template <class TO, tile::Kind KIND>
@@ -230,22 +235,25 @@ int linear(int dtype, int64_t M, int64_t K, int64_t N, const void *w, const floa
   return linear<bf16>(dtype, M, K, N, w, w_scale, bias, act, x, residual, y, ws, nullptr, num_cu, st);
 }
 
-// The gated block: x's codes against W_gate and W_up in one product, the hidden layer in the activations' type (its largest
-// value per row is known when the row is complete), its codes against W_down.
+// The gated block: x's codes against W_gate and W_up in one product, the hidden layer's codes against W_down.  A row's scale is known
+// when the row is complete, and the product is formed twice, first for the largest value of each row and then for the codes: the
+// hidden layer is in memory as codes alone.  Kept in bf16 between one product and its quantisation it would be rounded twice,
+// which moves the output by 0.9 % of itself (the codes' own rounding: 0.3); in float32 its 8 F bytes per row
+// cost as much as the second product.
 template <class TO>
 static int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated_params &p, int act, const void *x,
                  const void *residual, void *y, char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
   Space ws{workspace};
   Layout lay;
   const bool plan = bytes != nullptr;
-  const int64_t Fp = up(F, 16 / sizeof(TO)), Kc = up(C, 16), Kf = up(F, 16);
-  void *h = ws.take(M * Fp * sizeof(TO));
-  const Tokens qx = tokens(M, C, ws), qh = tokens(M, F, ws);
+  const int64_t Kc = up(C, 16), Kf = up(F, 16), Fp = up(F, 32), Mp = up(M, tile::kGroupRows);
+  const Tokens qx = tokens(M, C, ws), qh = tokens(Mp, Fp, ws);
+  uint32_t *peak = static_cast<uint32_t *>(ws.take(M * 4));
   const void *gate = codes_of(p.w_gate, F, C, plan, ws, lay), *upw = codes_of(p.w_up, F, C, plan, ws, lay),
              *down = codes_of(p.w_down, C, F, plan, ws, lay);
   if (plan) return *bytes = ws.used, PA_OK;
   int rc = tile::lay_out(lay, 1, st);
-  if (!rc) rc = quantize_rows(dtype, M, C, x, C, qx.q, Kc, qx.scale, num_cu, st);
+  if (!rc) rc = quantize(dtype, Quantize{x, M, C, C, Kc, qx.q, qx.scale, peak}, num_cu, st);
   if (rc) return rc;
   Args a{};
   a.X = qx.q, a.ldx = a.ldw = Kc, a.units = (int)(Kc / 16);
@@ -253,11 +261,12 @@ static int gated(int dtype, int64_t M, int64_t C, int64_t F, const pa_int8_gated
   a.M = M, a.N = (int)F, a.limit = (int)Fp;
   a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
   a.sx = qx.scale, a.sw[0] = p.s_gate, a.sw[1] = p.s_up;
-  a.out = h, a.ldo = Fp, a.act = act;
-  if ((rc = product<TO, tile::kGated>(a, num_cu, st))) return rc;
-  if ((rc = quantize_rows(dtype, M, F, h, Fp, qh.q, Kf, qh.scale, num_cu, st))) return rc;
+  a.act = act, a.peak = peak;
+  if ((rc = product<TO, tile::kPeak>(a, num_cu, st))) return rc;
+  a.out = qh.q, a.ldo = Fp, a.row_scale = qh.scale;
+  if ((rc = product<TO, tile::kCodes>(a, num_cu, st))) return rc;
   Args d{};
-  d.X = qh.q, d.ldx = d.ldw = Kf, d.units = (int)(Kf / 16);
+  d.X = qh.q, d.ldx = Fp, d.ldw = Kf, d.units = (int)(Kf / 16), d.x_groups = true;
   d.W[0] = down;
   d.M = M, d.N = d.limit = (int)C;
   d.bias[0] = p.b_down, d.sx = qh.scale, d.sw[0] = p.s_down;

@@ -159,6 +159,8 @@ enum Kind {
   kGated,  // out = act(X W0^T + b0) * (X W1^T + b1)
   kBack,   // the gated block's hidden layer again, g = X W0^T + b0, u = X W1^T + b1, and d = X2 W2^T:
            // out[:, :ldh] = d u act'(g), out[:, ldh:] = d act(g), out2 = act(g) u
+  kPeak,   // int8: peak[m] = max over n of |act(X W0^T + b0) * (X W1^T + b1)|, as bits
+  kCodes,  // the same products again, out = rint(127 of them / peak) as int8 in column groups, row_scale = peak / 127
 };
 
 // The hidden layer's matrices are written and read by kernels of this library alone, and lie in groups of 32 bytes of columns where
@@ -178,6 +180,8 @@ struct Args {
   int N, limit;                  // columns; columns N .. limit - 1 are written as zeros (limit: a multiple of a unit's elements, or N)
   const float *bias[2];          // or NULL
   const float *sx, *sw[2];       // int8: scale per row of X, per row of W
+  uint32_t *peak;                // kPeak, kCodes
+  float *row_scale;              // kCodes
   const void *residual;          // (M, N), kPlain, or NULL
   void *out, *out2;
   int64_t ldo, ldh;              // elements between rows of out (residual alike); of out2, and from dg to du
@@ -299,8 +303,9 @@ struct Config {
   static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_, UPS = UPS_, RING = RING_, OCC = OCC_;  // OCC: waves per SIMD
   static constexpr int WAVES = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32;
   static constexpr int STAGE = (BM + BN) * 16 * UPS;
-  static constexpr int side(int bytes) { return bytes == 1 ? 2 * BN + BM : BN; }  // floats
-  static constexpr int lds(int bytes) { return RING * (STAGE + 4 * side(bytes)); }
+  // floats: biases; int8: scales of W, of X; kCodes: peaks
+  static constexpr int side(int bytes, Kind kind) { return BN + (bytes == 1 ? BN + BM : 0) + (kind == kCodes ? BM : 0); }
+  static constexpr int lds(int bytes, Kind kind) { return RING * (STAGE + 4 * side(bytes, kind)); }
 };
 
 template <class E, class TO, Kind KIND, class CFG>
@@ -311,10 +316,11 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
   constexpr int NX = BM / GROUP / WAVES, NW = BN / GROUP / WAVES, TN2 = TN / 2;  // loads a wave issues
   static_assert(BM % (GROUP * WAVES) == 0 && BN % (GROUP * WAVES) == 0, "whole groups");
   static_assert(!DUAL || TN % 2 == 0, "pairs of tiles");
-  constexpr unsigned STAGE = CFG::STAGE, SIDE = CFG::side(E::kBytes);
+  constexpr unsigned STAGE = CFG::STAGE, SIDE = CFG::side(E::kBytes, KIND);
   static_assert(BM % 64 == 0 && BN % 64 == 0, "whole loads of 64 floats");
   // stores a wave leaves behind a tile
-  constexpr int STORES = kTileStores<TO> * TM * (KIND == kPlain ? TN : KIND == kGated ? TN2 : 3 * TN2), YOUNGER = (AHEAD - 1) * (NX + NW);
+  constexpr int STORES = KIND == kPeak ? 0 : KIND == kCodes ? TM * TN2 : kTileStores<TO> * TM * (KIND == kPlain ? TN : KIND == kGated ? TN2 : 3 * TN2);
+  constexpr int YOUNGER = (AHEAD - 1) * (NX + NW);
   constexpr int LEFT = YOUNGER + STORES < 63 ? YOUNGER + STORES : 63;
   using Acc = typename E::Acc;
   extern __shared__ u32x4 smem[];
@@ -384,8 +390,9 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           const float *from = 64 * k < BN ? a.bias[which] : a.sw[which];
           p = from ? from + (col < a.N ? col : a.N - 1) : reinterpret_cast<const float *>(&mfma::kZeroUnit);
         } else {
-          const int64_t m = m0 + at - 2 * BN;
-          p = a.sx + (m < a.M ? m : a.M - 1);
+          const bool peaks = KIND == kCodes && 64 * k >= 2 * BN + BM;
+          const int64_t m = m0 + at - 2 * BN - (peaks ? BM : 0);
+          p = (peaks ? reinterpret_cast<const float *>(a.peak) : a.sx) + (m < a.M ? m : a.M - 1);
         }
         load_word_to_lds(p, (unsigned)(uintptr_t)smem + RING * STAGE + 4 * (sbuf * SIDE + 64 * k));
       }
@@ -529,7 +536,8 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
     const TO *type = nullptr;
     auto bias_of = [&](int n) { return side + (wn * TN + n) * 32; };  // of the wave's n-th tile of weight rows
     auto scale_of = [&](int n) { return side + BN + (wn * TN + n) * 32; };
-    stored = KIND != kPlain || a.vec;
+    // kPeak leaves none; row_scale's stores of kCodes come on top
+    stored = KIND == kGated || KIND == kBack || KIND == kCodes || (KIND == kPlain && a.vec);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       const int rl = (wm * TM + m) * 32 + i;  // row of the tile
@@ -577,6 +585,57 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
               }
             }
           }
+        }
+      } else if constexpr (KIND == kPeak || KIND == kCodes) {
+        // both passes run the same operations on the same sums: no code passes 127
+        const uint32_t top_bits = KIND == kCodes ? __float_as_uint(side[2 * BN + BM + rl]) : 0u;
+        const float top = __uint_as_float(top_bits);
+        const bool finite = top_bits < 0x7f800000u;
+        const float by = finite && top >= 0x1p-100f ? 127.f / top : 0.f;  // a smaller layer counts as zero
+        uint32_t most = 0;
+        const Buffer out = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<char *>(uniform(static_cast<const char *>(a.out) + m0 * a.ldo)), 0, (int)(((have + 31) & ~31) * a.ldo), 0x00027000);
+#pragma unroll
+        for (int n = 0; n < TN2; ++n) {
+          const int col = tn * CN + (wn * TN2 + n) * 32;
+          f32x16 h = values_of<E>(acc[m][2 * n], bias_of(2 * n), scale_of(2 * n), g, sx);
+          const f32x16 up = values_of<E>(acc[m][2 * n + 1], bias_of(2 * n + 1), scale_of(2 * n + 1), g, sx);
+          act_values<sizeof(TO) == 2>(a.act, h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) h[r] *= up[r];
+          if (col + 32 > a.N) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) h[r] = col + rowmap(r, g) < a.N ? h[r] : 0.f;
+          }
+          if constexpr (KIND == kPeak) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const uint32_t b = __float_as_uint(h[r]) & 0x7fffffffu;
+              most = b > most ? b : most;
+            }
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              int c[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) c[j] = (int)rintf(h[4 * q + j] * by);
+              const uint32_t lo = __builtin_amdgcn_perm((uint32_t)c[1], (uint32_t)c[0], 0x0c0c0400u);
+              w[q] = __builtin_amdgcn_perm((uint32_t)c[3], (uint32_t)c[2], 0x04000c0cu) | lo;
+            }
+            const auto r0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+            const u32x4 s = {r0[0], r0[1], r1[0], r1[1]};
+            const unsigned place = (unsigned)((rl & ~31) * a.ldo + (rl & 31) * 32 + 32 * col + 16 * g);
+            __builtin_amdgcn_raw_buffer_store_b128(s, out, col + 16 * g < a.limit ? place : kNowhere, 0, 0);
+          }
+        }
+        if constexpr (KIND == kPeak) {
+          const auto r = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+          most = r[0] > r[1] ? r[0] : r[1];
+          if (g == 0 && rl < have) atomicMax(a.peak + m0 + rl, most);  // a maximum: the order does not matter
+        } else if (tn == 0 && wn == 0 && g == 0 && rl < have) {
+          a.row_scale[m0 + rl] = finite ? top / 127.f : __uint_as_float(0x7fc00000u);
         }
       } else {
         constexpr bool GROUPS = kGrouped<TO> && E::kBytes == 2;
@@ -634,7 +693,7 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
 template <class E, class TO, Kind KIND, class CFG>
 int launch_tiles(Args a, int num_cu, hipStream_t st) {
   constexpr int CN = KIND == kPlain ? CFG::BN : CFG::BN / 2;
-  constexpr size_t lds = CFG::lds(E::kBytes);
+  constexpr size_t lds = CFG::lds(E::kBytes, KIND);
   static_assert(lds <= kMaxLdsBytes, "the ring fits a workgroup");
   const int64_t mt = (a.M + CFG::BM - 1) / CFG::BM, nt = (a.N + CN - 1) / CN;
   if (mt * nt > (int64_t)1 << 30) return PA_ERR_UNSUPPORTED;
@@ -700,8 +759,9 @@ int launch(Args a, int num_cu, hipStream_t st) {
   rest.M -= p.rows;
   rest.X = past(a.X, a.ldx), rest.X2 = past(a.X2, a.ldx2);
   rest.sx = a.sx ? a.sx + p.rows : nullptr;
+  rest.peak = a.peak ? a.peak + p.rows : nullptr, rest.row_scale = a.row_scale ? a.row_scale + p.rows : nullptr;
   rest.residual = past(a.residual, a.ldo * (int64_t)sizeof(TO));
-  rest.out = past(a.out, a.ldo * (int64_t)sizeof(TO)), rest.out2 = past(a.out2, a.ldh * (int64_t)sizeof(TO));
+  rest.out = past(a.out, a.ldo * (int64_t)(KIND == kCodes ? 1 : sizeof(TO))), rest.out2 = past(a.out2, a.ldh * (int64_t)sizeof(TO));
   return run(rest, plan_of(rest.M, a.N, stages, KIND == kBack, KIND != kPlain, num_cu, false).size);
 }
 
