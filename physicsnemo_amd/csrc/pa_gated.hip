@@ -127,6 +127,22 @@ __global__ __launch_bounds__(256) void totals_kernel(Totals a) {
   else static_cast<float *>(o.dst)[row * o.cols + col] = v;
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// tile_sums_kernel: the column sums that the hidden layer's kernels leave per 32 rows, [tiles][n], to [gridDim.y][n].
+// ---------------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void tile_sums_kernel(const float *__restrict__ src, float *__restrict__ dst, int64_t tiles, int n) {
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= n) return;
+  const int64_t per = (tiles + gridDim.y - 1) / gridDim.y, t0 = blockIdx.y * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  float s[8] = {};
+  int64_t t = t0;
+  for (; t + 8 <= t1; t += 8)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s[k] += src[(t + k) * n + e];
+  for (; t < t1; ++t) s[0] += src[t * n + e];
+  dst[(int64_t)blockIdx.y * n + e] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
+
 // ================================================================================================
 // host side
 // ================================================================================================
@@ -157,7 +173,7 @@ int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float 
 int64_t hidden_blob_bytes(int64_t C, int64_t F);
 int hidden_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipStream_t st);
 int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void *blob, int act, const void *x, const void *dy, void *dgu,
-                         void *h, int num_cu, hipStream_t st);
+                         void *h, float *sums, int num_cu, hipStream_t st);
 
 template <class E, class TO, tile::Kind KIND>
 static int product(const Args &a, int num_cu, hipStream_t st) {
@@ -251,7 +267,7 @@ static Partials partials_of(int64_t M, int64_t oa, int64_t ob, int num_cu, Space
 template <class E>
 static int rows_product(const Partials &r, const void *A, int64_t oa, const void *B, int64_t ob, int64_t M, int groups, int num_cu,
                         hipStream_t st) {  // groups: 1 if A, 2 if B is a matrix of the hidden layer
-  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, r.sums, st, groups);
+  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, groups == 1 ? nullptr : r.sums, st, groups);
   return gemm::cols_gemm_f32(A, oa, oa, B, ob, ob, M, nullptr, r.product, r.sums, num_cu, st);
 }
 
@@ -285,6 +301,10 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   // W_down^T (F, Cp), and [W_gate; W_up]^T (C, 2 Fp): hidden units past F are zero columns
   void *wd_t = ws.take(F * Cp * e), *w_t = ws.take(C * 2 * Fp * e);
   const Partials in = partials_of<E>(M, 2 * Fp, Cp, num_cu, ws), down = partials_of<E>(M, Cp, Fp, num_cu, ws);
+  // bf16: dg and du are rounded for their products, their column sums are not
+  const int64_t tiles = (M + 31) / 32, parts = tiles < 1024 ? (tiles + 31) / 32 : 32;
+  float *sums = e == 2 ? static_cast<float *>(ws.take(tiles * 2 * Fp * 4)) : nullptr;
+  float *sum_parts = e == 2 ? static_cast<float *>(ws.take(parts * 2 * Fp * 4)) : nullptr;
   if (plan) return *bytes = ws.used, PA_OK;
   if (rest > 0) lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
   if (dx) {
@@ -295,7 +315,7 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   if (rc) return rc;
   if (done > 0) {
     rc = hidden_pack(C, F, p, blob, st);
-    if (!rc) rc = rows_hidden_backward(done, Cp, F, Fp, blob, act, xr.p, dyr.p, dgu, h, num_cu, st);
+    if (!rc) rc = rows_hidden_backward(done, Cp, F, Fp, blob, act, xr.p, dyr.p, dgu, h, sums, num_cu, st);
     if (rc) return rc;
   }
   if (rest > 0) {
@@ -306,6 +326,7 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
     a.M = rest, a.N = (int)F, a.limit = (int)Fp;
     a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+    a.sums = out.b_gate || out.b_up ? reinterpret_cast<float *>(from(sums, 2 * Fp * 4 / 32)) : nullptr;
     a.out = from(dgu, 2 * Fp * e), a.ldo = 2 * Fp, a.out2 = from(h, Fp * e), a.ldh = Fp, a.act = act;
     if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
   }
@@ -323,8 +344,14 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, 1, num_cu, st))) return rc;
     totals.add(in.product, in.G, 2 * Fp * Cp, Cp, out.w_gate, F, C, e);
     totals.add(in.product + Fp * Cp, in.G, 2 * Fp * Cp, Cp, out.w_up, F, C, e);
-    totals.add(in.sums, in.G, 2 * Fp, F, out.b_gate, 1, F, 4);
-    totals.add(in.sums + Fp, in.G, 2 * Fp, F, out.b_up, 1, F, 4);
+    if (e == 2 && (out.b_gate || out.b_up)) {
+      hipLaunchKernelGGL(tile_sums_kernel, dim3((unsigned)((2 * Fp + 255) / 256), (unsigned)parts), dim3(256), 0, st, sums, sum_parts, tiles,
+                         (int)(2 * Fp));
+      if ((rc = launch_status())) return rc;
+    }
+    const float *db = e == 2 ? sum_parts : in.sums;
+    totals.add(db, e == 2 ? parts : in.G, 2 * Fp, F, out.b_gate, 1, F, 4);
+    totals.add(db + Fp, e == 2 ? parts : in.G, 2 * Fp, F, out.b_up, 1, F, 4);
   }
   if (out.w_down || out.b_down) {
     if ((rc = rows_product<E>(down, dyr.p, Cp, h, Fp, M, 2, num_cu, st))) return rc;

@@ -313,6 +313,7 @@ struct HiddenArgs {
   const u32x4 *blob;
   const uint16_t *x, *dy;
   uint16_t *dgu, *h;  // (M, 2 Fp): dg, du; (M, Fp); in column groups (pa_tile.h), whole blocks of 32 rows
+  float *sums;        // per 32 rows the column sums of dg and du before their rounding, (2 Fp)
   int64_t M, nblocks;
   int C, F, Fp, act;
 };
@@ -377,13 +378,15 @@ struct Slope {
 // rows_hidden_backward_kernel<CT>: the hidden layer of the backward pass for rows of up to 32 CT channels.  Per slot c a wave runs
 //   u(c)^T = W_up[chunk c] x^T + b_up, g(c)^T = W_gate[chunk c] x^T + b_gate, d(c)^T = W_down[:, chunk c]^T dy^T     6 CT MFMAs
 // in turn, with h, dg and du of the chunk before formed behind them, 16 values in five pieces each; two sets of accumulators take
-// turns.  Results of two chunks leave together, 2 KB in one piece each (pa_tile.h).  Bound by HBM, 4 C + 6 F bytes per row.
+// turns.  A chunk's results leave 2 KB in one piece each (pa_tile.h); the column sums of dg
+// and du, for the bias gradients, are formed before their rounding.  Bound by HBM, 4 C + 6 F bytes per row.
 // ---------------------------------------------------------------------------------------------------------------
+__host__ __device__ constexpr int value_at(int t) { return t / 2 % 4 * 4 + t / 8 * 2 + t % 2; }
 template <int CT, int ACT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void rows_hidden_backward_kernel(
     HiddenArgs a) {
   constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
-  constexpr int STORES = 12;  // of two chunks
+  constexpr int STORES = 6 + 1;  // of a chunk
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -407,6 +410,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       xb[ks] = *reinterpret_cast<const u32x4 *>(a.x + r * C + at);
       db[ks] = *reinterpret_cast<const u32x4 *>(a.dy + r * C + at);
       if (32 * CT > C && col >= C) xb[ks] = db[ks] = u32x4{0u, 0u, 0u, 0u};
+      if (mb * ROWS + wave * 32 + i >= a.M) db[ks] = u32x4{0u, 0u, 0u, 0u};  // a repeated row: of no gradient
     }
   };
   int buf = 0;
@@ -420,29 +424,48 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     f32x16 ga[2], ua[2], da[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) ga[1][r] = ua[1][r] = da[1][r] = 0.f;
-    uint32_t packed[2][3][8];  // of the chunks of a pair: dg, du, h
-    auto store_pair = [&](int c) {  // chunks c, c + 1
+    uint32_t packed[3][8];  // of a chunk: dg, du, h
+    auto store_chunk = [&](int c) {
 #pragma unroll
       for (int which = 0; which < 3; ++which)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int half = 0; half < 2; ++half) {
+          u32x4 s;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            u32x4 s;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const auto r = __builtin_amdgcn_permlane32_swap(packed[k][which][4 * half + w], packed[k][which][4 * half + 2 + w], false, false);
-              s[w] = r[0], s[2 + w] = r[1];
-            }
-            const int col = 32 * (c + k) + 16 * half + 8 * g;
-            const unsigned at = (unsigned)(((which == 1 ? a.Fp : 0) + 32 * (c + k) + 16 * half) * 64 + i * 32 + g * 16);
-            __builtin_amdgcn_raw_buffer_store_b128(s, which < 2 ? out : hidden, col < a.Fp ? at : tile::kNowhere, 0, 0);
+          for (int w = 0; w < 2; ++w) {
+            const auto r = __builtin_amdgcn_permlane32_swap(packed[which][4 * half + w], packed[which][4 * half + 2 + w], false, false);
+            s[w] = r[0], s[2 + w] = r[1];
           }
+          const int col = 32 * c + 16 * half + 8 * g;
+          const unsigned at = (unsigned)(((which == 1 ? a.Fp : 0) + 32 * c + 16 * half) * 64 + i * 32 + g * 16);
+          __builtin_amdgcn_raw_buffer_store_b128(s, which < 2 ? out : hidden, col < a.Fp ? at : tile::kNowhere, 0, 0);
+        }
+    };
+    // Column sums on their way (tile::column_sums).  Values are taken in an order that keeps few of them: the four q of columns
+    // j = 0, 1, then of 2, 3.
+    float held[2][2], half[2][2];
+    tile::f32x4 total;
+    auto add_up = [&](auto j_, float dg, float du) {  // value J of the chunk's 16 in this lane
+      constexpr int q = decltype(j_)::value / 4, j = decltype(j_)::value % 4;
+      if constexpr (q % 2 == 0) {
+        held[0][j % 2] = dg, held[1][j % 2] = du;
+      } else {
+        const float s0 = tile::exchange_add<0>(held[0][j % 2], dg, lane), s1 = tile::exchange_add<0>(held[1][j % 2], du, lane);
+        if constexpr (q == 1) half[0][j % 2] = s0, half[1][j % 2] = s1;
+        else
+          total[j] = tile::both_add(tile::exchange_add<1>(half[0][j % 2], s0, lane), tile::exchange_add<1>(half[1][j % 2], s1, lane), lane);
+      }
+    };
+    const Buffer sums = __builtin_amdgcn_make_buffer_rsrc(a.sums + row0 / 32 * 2 * a.Fp, 0, have > 0 ? 2 * a.Fp * 4 : 0, 0x00027000);
+    auto store_sums = [&](int c) {
+      const int col = 32 * c + 8 * (lane & 3) + 4 * g;
+      const unsigned at = (unsigned)((i & 4 ? a.Fp : 0) + col) * 4;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, total), sums, i < 8 && col < a.Fp ? at : tile::kNowhere, 0, 0);
     };
     auto slot = [&](int c, auto set_) {
       constexpr int now = decltype(set_)::value, old = 1 - now;
       // this wave's share of the slot has landed; the stores that left behind it stay in flight
-      if (now == 1 && c > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+      if (c > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();  // everyone's, and the other buffer is free
       const u32x4 *wb = smem + buf * SU + lane;
@@ -462,21 +485,22 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       auto tick = [&](auto t_) {  // pieces of values T .. T - 4
         constexpr int T = decltype(t_)::value;
         if constexpr (T >= 4 && T < 20) {
-          constexpr int J = T - 4;
+          constexpr int J = value_at(T - 4);
           float h, dg, du;
-          v[J % 5].piece4(ua[old][J], da[old][J], h, dg, du);
+          v[(T - 4) % 5].piece4(ua[old][J], da[old][J], h, dg, du);
+          add_up(std::integral_constant<int, J>{}, dg, du);
           if constexpr (J % 2 == 0) {
             even[0] = dg, even[1] = du, even[2] = h;
           } else {
-            packed[old][0][J / 2] = pack2(even[0], dg);
-            packed[old][1][J / 2] = pack2(even[1], du);
-            packed[old][2][J / 2] = pack2(even[2], h);
+            packed[0][J / 2] = pack2(even[0], dg);
+            packed[1][J / 2] = pack2(even[1], du);
+            packed[2][J / 2] = pack2(even[2], h);
           }
         }
         if constexpr (T >= 3 && T < 19) v[(T - 3) % 5].piece3(a.act);
         if constexpr (T >= 2 && T < 18) v[(T - 2) % 5].piece2();
         if constexpr (T >= 1 && T < 17) v[(T - 1) % 5].piece1();
-        if constexpr (T < 16) v[T % 5].piece0(ga[old][T]);
+        if constexpr (T < 16) v[T % 5].piece0(ga[old][value_at(T)]);
       };
       static_for<NF>([&](auto s_) {
         constexpr int S = decltype(s_)::value;
@@ -489,7 +513,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
         if constexpr (S == 1) fetch(buf ^ 1, c + 1 < NCH ? c + 1 : 0);  // past the last slot: the first of the next block
         __builtin_amdgcn_sched_barrier(0);
       });
-      if (now == 0 && c > 0) store_pair(c - 2);
+      if (now == 1 || c > 0) store_sums(c - 1), store_chunk(c - 1);
       buf ^= 1;
     };
 #pragma clang loop unroll(disable)
@@ -499,22 +523,26 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     }
     const int64_t next = mb + gridDim.x;
     load_rows(next < a.nblocks ? next : mb);
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {  // the last chunk
-      float o[2][3];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        Slope<ACT> v;
-        v.piece0(ga[1][j + k]);
-        v.piece1();
-        v.piece2();
-        v.piece3(a.act);
-        v.piece4(ua[1][j + k], da[1][j + k], o[k][2], o[k][0], o[k][1]);
+    float even[3];
+    static_for<16>([&](auto j_) {  // the last chunk
+      constexpr int J = value_at(decltype(j_)::value);
+      float h, dg, du;
+      Slope<ACT> v;
+      v.piece0(ga[1][J]);
+      v.piece1();
+      v.piece2();
+      v.piece3(a.act);
+      v.piece4(ua[1][J], da[1][J], h, dg, du);
+      add_up(std::integral_constant<int, J>{}, dg, du);
+      if constexpr (J % 2 == 0) {
+        even[0] = dg, even[1] = du, even[2] = h;
+      } else {
+        packed[0][J / 2] = pack2(even[0], dg);
+        packed[1][J / 2] = pack2(even[1], du);
+        packed[2][J / 2] = pack2(even[2], h);
       }
-#pragma unroll
-      for (int which = 0; which < 3; ++which) packed[1][which][j / 2] = pack2(o[0][which], o[1][which]);
-    }
-    store_pair(NCH - 2);
+    });
+    store_sums(NCH - 1), store_chunk(NCH - 1);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing is landing in LDS when the workgroup ends
 }
@@ -616,8 +644,9 @@ int hidden_pack(int64_t C, int64_t F, const pa_gated_params &p, void *blob, hipS
 }
 
 int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void *blob, int act, const void *x, const void *dy, void *dgu,
-                         void *h, int num_cu, hipStream_t st) {
+                         void *h, float *sums, int num_cu, hipStream_t st) {
   HiddenArgs a{};
+  a.sums = sums;
   a.blob = static_cast<const u32x4 *>(blob);
   a.x = static_cast<const uint16_t *>(x), a.dy = static_cast<const uint16_t *>(dy);
   a.dgu = static_cast<uint16_t *>(dgu), a.h = static_cast<uint16_t *>(h);

@@ -183,6 +183,7 @@ struct Args {
   uint32_t *peak;                // kPeak, kCodes
   float *row_scale;              // kCodes
   const void *residual;          // (M, N), kPlain, or NULL
+  float *sums;                   // kBack, bf16: per 32 rows the column sums of dg and du before their rounding, (2 ldh), or NULL
   void *out, *out2;
   int64_t ldo, ldh;              // elements between rows of out (residual alike); of out2, and from dg to du
   int act;
@@ -229,6 +230,35 @@ __device__ __forceinline__ void store_tile(const f32x16 &v, const Buffer &out, u
     __builtin_amdgcn_raw_buffer_store_b128(s, out, c < limit ? at + 4 * c : kNowhere, 0, 0);
   }
 }
+// ---- sums over the 32 rows (lanes) of two 32 x 32 tiles of the same 32 columns (16 registers and both halves of the wave) ----
+// First pairs of registers in exchange for pairs of lanes, then the two tiles, then over the lanes that are left: 3 instructions per
+// pair of values where adding each over the lanes takes 10.  In the end lane (i, g) holds columns 8 q + 4 g .. + 3, q = i % 4, of the
+// second tile where bit 2 of i is set.
+template <int BIT>  // 0 .. 2, of the lane
+__device__ __forceinline__ float exchange_add(float even, float odd, int lane) {
+  constexpr int CTRL = BIT == 0 ? 0xB1 : BIT == 1 ? 0x4E : 0x124;  // quad_perm [1,0,3,2], [2,3,0,1], row_ror 4
+  const bool upper = lane >> BIT & 1;
+  const float keep = upper ? odd : even, send = upper ? even : odd;
+  return keep + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(send), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float both_add(float first, float second, int lane) {
+  float v = exchange_add<2>(first, second, lane);
+  v += __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), 0x128, 0xf, 0xf, true));  // row_ror 8
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ f32x4 column_sums(const f32x16 &v, const f32x16 &w, int lane) {
+  f32x4 s;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    auto four = [&](const f32x16 &x) {
+      return exchange_add<1>(exchange_add<0>(x[j], x[4 + j], lane), exchange_add<0>(x[8 + j], x[12 + j], lane), lane);
+    };
+    s[j] = both_add(four(v), four(w), lane);
+  }
+  return s;
+}
+
 template <class T>
 constexpr int kTileStores = sizeof(T) == 2 ? 2 : 4;
 
@@ -670,6 +700,10 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           } else {
             const Buffer hidden = rows_or_blocks_at(a.out2, a.ldh);
             f32x16 slope, d = acc2[m][n];
+            if (rl >= have) {  // a repeated row: of no gradient
+#pragma unroll
+              for (int r = 0; r < 16; ++r) d[r] = 0.f;
+            }
             act_slopes(a.act, gate, slope);
             f32x16 h;
 #pragma unroll
@@ -679,6 +713,12 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
               gate[r] *= d[r];
             }
             cut(h), cut(slope), cut(gate);
+            if (E::kBytes == 2 && a.sums) {
+              const f32x4 s = column_sums(slope, gate, lane);
+              const int c = col + 8 * (lane & 3) + 4 * g;
+              if (i < 8 && c < a.limit && (wm * TM + m) * 32 < have)
+                *reinterpret_cast<f32x4 *>(a.sums + (m0 / 32 + wm * TM + m) * 2 * a.ldh + (i & 4 ? a.ldh : 0) + c) = s;
+            }
             store_tile<GROUPS>(slope, out, at_out, col, a.limit, g, type);
             store_tile<GROUPS>(gate, out, at_out + (unsigned)(a.ldh * sizeof(TO)) * (GROUPS ? 32 : 1), col, a.limit, g, type);
             store_tile<GROUPS>(h, hidden, place_of(a.ldh), col, a.limit, g, type);
@@ -759,6 +799,7 @@ int launch(Args a, int num_cu, hipStream_t st) {
   rest.M -= p.rows;
   rest.X = past(a.X, a.ldx), rest.X2 = past(a.X2, a.ldx2);
   rest.sx = a.sx ? a.sx + p.rows : nullptr;
+  rest.sums = a.sums ? a.sums + p.rows / 32 * 2 * a.ldh : nullptr;
   rest.peak = a.peak ? a.peak + p.rows : nullptr, rest.row_scale = a.row_scale ? a.row_scale + p.rows : nullptr;
   rest.residual = past(a.residual, a.ldo * (int64_t)sizeof(TO));
   rest.out = past(a.out, a.ldo * (int64_t)(KIND == kCodes ? 1 : sizeof(TO))), rest.out2 = past(a.out2, a.ldh * (int64_t)sizeof(TO));
