@@ -7,6 +7,7 @@ from .physics_attention import (  # noqa: F401
 )
 from .context_projector import (BQWarp, ContextProjector, GeometricFeatureProcessor,  # noqa: F401
                                 MultiScaleFeatureExtractor, StructuredContextProjector)
+from .feedforward import CounterDropout, GatedMlp  # noqa: F401
 from .flare import FLARE, FLAREBlock, FLAREModel, GALE_FA  # noqa: F401
 from .gale import GALE, GALEBlock, GALEStructuredMesh2D, GALEStructuredMesh3D  # noqa: F401
 from .geotransolver import GeoTransolver, GlobalContextBuilder  # noqa: F401

@@ -24,7 +24,7 @@ import torch.nn as nn
 
 from . import functional as PF
 from .autograd import FlareFunction
-from .transolver import Mlp, Transolver, TransolverBlock
+from .transolver import Transolver, TransolverBlock, block_mlp
 
 
 class FLARE(nn.Module):
@@ -322,7 +322,7 @@ class FLAREBlock(TransolverBlock):
         self.Attn = FLARE(hidden_dim, heads=num_heads, dim_head=hidden_dim // num_heads, dropout=dropout,
                           n_global_queries=n_global_queries, use_te=use_te)
         self.ln_mlp1 = nn.Sequential(nn.LayerNorm(hidden_dim),
-                                     Mlp(hidden_dim, hidden_dim * mlp_ratio, hidden_dim, act))
+                                     block_mlp(hidden_dim, hidden_dim * mlp_ratio, act))
         if last_layer:
             self.ln_mlp2 = nn.Sequential(nn.LayerNorm(hidden_dim), nn.Linear(hidden_dim, out_dim))
         self._mlp_cache = {}

@@ -15,13 +15,16 @@ With gradients required the per-point stages run on the layer's forward / backwa
 """
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 import torch.nn as nn
 
 from . import functional as PF
 from . import autograd as PA
 from .autograd import GALEFunction, GALEPlusFunction
-from .transolver import Mlp, TransolverBlock
+from .feedforward import GatedMlp, counter_dropout
+from .transolver import Mlp, TransolverBlock, block_mlp
 from .physics_attention import (
     PhysicsAttentionIrregularMesh,
     PhysicsAttentionStructuredMesh2D,
@@ -272,7 +275,7 @@ class GALEBlock(nn.Module):
             self.Attn = GALEStructuredMesh3D(hidden_dim, spatial_shape=tuple(int(v) for v in spatial_shape), **common)
         else:
             raise ValueError(f"spatial_shape must be None, length-2, or length-3; got {spatial_shape!r}")
-        self.ln_mlp1 = nn.Sequential(nn.LayerNorm(hidden_dim), Mlp(hidden_dim, hidden_dim * mlp_ratio, hidden_dim, act))
+        self.ln_mlp1 = nn.Sequential(nn.LayerNorm(hidden_dim), block_mlp(hidden_dim, hidden_dim * mlp_ratio, act))
         self.attn_dropout = None
         self.ffn_dropout = None
         self._mlp_cache: dict = {}
@@ -284,15 +287,29 @@ class GALEBlock(nn.Module):
     _mlp_is_plain = TransolverBlock._mlp_is_plain
     _mlp_kernel_serves = TransolverBlock._mlp_kernel_serves
     _mlp_residual = TransolverBlock._mlp_residual
+    int8_mlp = None
+    use_int8_mlp = TransolverBlock.use_int8_mlp
+    use_counter_dropout = TransolverBlock.use_counter_dropout
 
-    def _one(self, fx: torch.Tensor, attn: torch.Tensor, needs_grad: bool) -> torch.Tensor:
-        fx1, mlp = attn + fx, self.ln_mlp1[1]
-        if needs_grad and type(mlp) is Mlp and PA.unhooked(mlp):
-            return PA.norm_mlp_residual(fx1, self.ln_mlp1[0], mlp.layers)
-        normed = PA.layer_norm(fx1, self.ln_mlp1[0])
+    def _one(self, fx: torch.Tensor, attn: torch.Tensor, needs_grad: bool, drop=None) -> torch.Tensor:
+        """The block behind the attention layer; with `drop` the layer's dropout is still to be applied."""
+        mlp = self.ln_mlp1[1]
+        if drop is not None:
+            fx1, normed = drop.add_norm(attn, fx, self.ln_mlp1[0])
+            if needs_grad and type(mlp) is Mlp and PA.unhooked(mlp):
+                return PA.mlp_residual(normed, fx1, mlp.layers)[0]
+        else:
+            fx1 = attn + fx
+            if needs_grad and type(mlp) is Mlp and PA.unhooked(mlp):
+                return PA.norm_mlp_residual(fx1, self.ln_mlp1[0], mlp.layers)
+            normed = PA.layer_norm(fx1, self.ln_mlp1[0])
         if not needs_grad and self._mlp_kernel_serves(normed):
             packed, b1, b2 = self._mlp_kernel_packed(normed.device, normed.dtype)
             return PF.mlp_forward_packed(normed, packed, b1, b2, residual=fx1.to(normed.dtype).contiguous())
+        if not needs_grad and self.int8_mlp is not None:
+            return self._mlp_residual(fx1, normed, None)[0]
+        if type(mlp) is GatedMlp and PA.unhooked(mlp):
+            return mlp(normed, fx1)
         return mlp(normed) + fx1
 
     def forward_chain(self, fx: tuple, normed_in, global_context: torch.Tensor | None, next_ln: nn.LayerNorm | None):
@@ -327,5 +344,7 @@ class GALEBlock(nn.Module):
                                                   any(p.requires_grad for p in self.parameters()))
         if not needs_grad and torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") == torch.bfloat16:
             fx = tuple(t.to(torch.bfloat16) for t in fx)  # inference: the residual stream in the compute type
-        attn = self.Attn(tuple(PA.layer_norm(t, self.ln_1) for t in fx), global_context)
-        return [self._one(t, a, needs_grad) for t, a in zip(fx, attn)]
+        drop = counter_dropout(self.Attn)
+        with drop.left_out() if drop is not None else nullcontext():
+            attn = self.Attn(tuple(PA.layer_norm(t, self.ln_1) for t in fx), global_context)
+        return [self._one(t, a, needs_grad, drop) for t, a in zip(fx, attn)]

@@ -18,6 +18,7 @@ import torch.nn as nn
 
 from . import autograd as PA
 from .context_projector import ContextProjector, MultiScaleFeatureExtractor, StructuredContextProjector
+from .feedforward import plain_act
 from .gale import GALEBlock
 from .transolver import Mlp, Transolver
 
@@ -145,7 +146,7 @@ class GeoTransolver(nn.Module):
         if len(functional_dims) != len(out_dims):
             raise ValueError(f"functional_dim and out_dim must be the same length, but instead got "
                              f"{len(functional_dims)} and {len(out_dims)}")
-        self.preprocess = nn.ModuleList([Mlp(f, n_hidden * 2, n_hidden, act) for f in functional_dims])
+        self.preprocess = nn.ModuleList([Mlp(f, n_hidden * 2, n_hidden, plain_act(act)) for f in functional_dims])
         self.n_hidden = n_hidden
         effective_hidden = n_hidden + n_hidden_local * len(self.radii) if include_local_features else n_hidden
         self.blocks = nn.ModuleList([
@@ -160,6 +161,9 @@ class GeoTransolver(nn.Module):
         self.time_input = time_input
         if time_input:
             self.time_fc = nn.Sequential(nn.Linear(n_hidden, n_hidden), nn.SiLU(), nn.Linear(n_hidden, n_hidden))
+
+    use_int8_mlp = Transolver.use_int8_mlp
+    use_counter_dropout = Transolver.use_counter_dropout
 
     def _flatten(self, t: torch.Tensor, name: str) -> torch.Tensor:
         n = int(math.prod(self.structured_shape))

@@ -21,6 +21,7 @@ import torch.nn as nn
 from . import functional as PF
 from .autograd import (LayerResidualFunction, LayerResidualNormFunction, PhysicsAttentionFunction, PhysicsAttentionMfmaFunction,
                        PhysicsAttentionPlusFunction, PhysicsAttentionPlusMfmaFunction, _aligned, unhooked)
+from .feedforward import CounterDropout
 
 __all__ = ["PhysicsAttentionBase", "PhysicsAttentionIrregularMesh", "PhysicsAttentionStructuredMesh2D",
            "PhysicsAttentionStructuredMesh3D"]
@@ -43,7 +44,7 @@ def _parameter(module: nn.Module, name: str) -> torch.Tensor:
 
 def _identity_dropout(m: nn.Module) -> bool:
     """True where calling m returns its argument and nothing else happens."""
-    return (type(m) is nn.Dropout and "forward" not in m.__dict__ and not (m.training and m.p > 0) and unhooked(m) and
+    return (type(m) in (nn.Dropout, CounterDropout) and "forward" not in m.__dict__ and not (m.training and m.p > 0) and unhooked(m) and
             not torch.nn.modules.module._has_any_global_hook())
 
 

@@ -22,6 +22,7 @@ import torch.nn as nn
 from . import autograd as PA
 from . import checkpoint as _ckpt
 from . import functional as PF
+from .feedforward import GATED_ACTS, CounterDropout, GatedMlp, Int8Mlp, counter_dropout, plain_act
 from .physics_attention import (PhysicsAttentionBase, PhysicsAttentionIrregularMesh, PhysicsAttentionStructuredMesh2D,
                                 PhysicsAttentionStructuredMesh3D)
 
@@ -94,6 +95,12 @@ class Mlp(nn.Module):
         return (PA.mlp(x, self.layers) if needs_grad else self.layers(x)), None
 
 
+def block_mlp(features: int, hidden_features: int, act: str) -> nn.Module:
+    """A block's MLP: `Mlp`, or for "swiglu", "geglu", "reglu" and "glu" a `GatedMlp`."""
+    gate = GATED_ACTS.get(act.lower())
+    return Mlp(features, hidden_features, features, act) if gate is None else GatedMlp(features, hidden_features, gate)
+
+
 class PositionalEmbedding(nn.Module):
     """Timestep features [cos(t f_k) | sin(t f_k)], f_k = max_positions^(-k / (C/2)) (reference
     physicsnemo/nn/module/embedding_layers.py:67-152 with the arguments Transolver passes, transolver.py:532-538)."""
@@ -118,6 +125,7 @@ class TransolverBlock(nn.Module):
     """LayerNorm -> PhysicsAttention -> +residual -> LayerNorm -> MLP -> +residual [-> LayerNorm -> Linear]."""
 
     fp8_weights = False  # class default for subclasses with constructors of their own; see use_fp8_weights()
+    int8_mlp: Int8Mlp | None = None  # see use_int8_mlp()
 
     def __init__(self, num_heads: int, hidden_dim: int, dropout: float, act: str = "gelu", mlp_ratio: int = 4,
                  last_layer: bool = False, out_dim: int = 1, slice_num: int = 32,
@@ -136,7 +144,7 @@ class TransolverBlock(nn.Module):
         else:
             raise ValueError(
                 f"Unexpected length of spatial shape encountered in Transolver_block: {len(spatial_shape)}. Expected 2 or 3.")
-        self.ln_mlp1 = nn.Sequential(nn.LayerNorm(hidden_dim), Mlp(hidden_dim, hidden_dim * mlp_ratio, hidden_dim, act))
+        self.ln_mlp1 = nn.Sequential(nn.LayerNorm(hidden_dim), block_mlp(hidden_dim, hidden_dim * mlp_ratio, act))
         if last_layer:
             self.ln_mlp2 = nn.Sequential(nn.LayerNorm(hidden_dim), nn.Linear(hidden_dim, out_dim))
         self._mlp_cache: dict = {}
@@ -147,10 +155,36 @@ class TransolverBlock(nn.Module):
         (scale = max|row| / 448): the attention layer's three projections (`PhysicsAttentionBase.use_fp8_weights`)
         and the two Linears of the MLP.  The kernels expand them to bf16 operands; activations stay bf16.  No
         counterpart in the reference."""
+        if enabled and (self.int8_mlp is not None or type(self.ln_mlp1[1]) is GatedMlp):
+            raise ValueError("fp8 weights are for a block whose MLP is a plain one outside use_int8_mlp; the attention layer "
+                             "alone takes them by Attn.use_fp8_weights")
         self.Attn.use_fp8_weights(enabled)
         self.fp8_weights = bool(enabled)
         self._mlp_cache = {}
         return self
+
+    def use_int8_mlp(self, enabled: bool = True):
+        """Inference with the MLP's products in 8 bits: weights rounded to int8 with one scale per output channel, once per
+        parameter set, and the rows on their way in with one scale each (`functional.linear_int8`, `gated_mlp_int8`); bfloat16
+        and float32 rows on the GPU.  Training runs as without it.  No counterpart in the reference."""
+        if enabled and self.fp8_weights:
+            raise ValueError("the block's MLP holds fp8 weights; use_fp8_weights(False) first")
+        if enabled and Int8Mlp.linears(self.ln_mlp1[1]) is None:
+            raise ValueError("the block's MLP is not Linear, activation, Linear or a GatedMlp, without hooks")
+        self.int8_mlp = Int8Mlp() if enabled else None
+        return self
+
+    def use_counter_dropout(self, seed: int, offset: int = 0):
+        """Training with the attention output's dropout from a counter-based generator (`CounterDropout`), in one kernel with
+        the residual add and the LayerNorm behind it.  The masks are others than torch's."""
+        self.Attn.out_dropout = CounterDropout(self.Attn.out_dropout.p, seed, offset).train(self.Attn.out_dropout.training)
+        return self
+
+    def _dropped_residual_norm(self, drop: CounterDropout, x_in: torch.Tensor, fx: torch.Tensor):
+        """(fx + dropout(Attn(x_in)), ln_mlp1[0] of it)."""
+        with drop.left_out():
+            y = self.Attn(x_in)
+        return drop.add_norm(y, fx, self.ln_mlp1[0])
 
     # ---------------------------------------------------------------- fused MLP (pa_mlp_forward)
     def _mlp_kernel_params(self, device, dtype=torch.bfloat16):
@@ -189,9 +223,9 @@ class TransolverBlock(nn.Module):
 
     def _mlp_is_plain(self) -> bool:
         """True where calling ln_mlp1[1] is Linear, GELU, Linear on its own parameters and nothing more, as the kernels
-        compute it: no hooks (weight normalisation forms the weight in one), no replaced or parametrised module."""
+        compute it: no hooks (weight normalisation forms the weight in one), no replaced or parametrised module, not in 8 bits."""
         mlp = self.ln_mlp1[1]
-        if type(mlp) is not Mlp or len(mlp.layers) != 3:
+        if type(mlp) is not Mlp or len(mlp.layers) != 3 or self.int8_mlp is not None:
             return False
         lin1, act, lin2 = mlp.layers
         return (type(lin1) is type(lin2) is nn.Linear and type(act) is nn.GELU and act.approximate == "none" and
@@ -238,7 +272,10 @@ class TransolverBlock(nn.Module):
             x_in, fx = (normed_in, fx) if normed_in is not None else PA.layer_norm_residual(fx, self.ln_1)
             pair, ln2, mlp = None, self.ln_mlp1[0], self.ln_mlp1[1]
             apart = type(mlp) is Mlp and PA.unhooked(mlp) and PA.norm_mlp_fused(fx, ln2, mlp.layers)
-            if isinstance(self.Attn, PhysicsAttentionBase):
+            drop = counter_dropout(self.Attn)
+            if drop is not None:
+                pair, apart = self._dropped_residual_norm(drop, x_in, fx), False
+            elif isinstance(self.Attn, PhysicsAttentionBase):
                 pair = self.Attn.forward_block_with_grad(x_in, fx, ln2, apart)
             if pair is not None and apart:
                 return PA.norm_mlp_residual_of(*pair, ln2, mlp.layers, next_ln)
@@ -246,10 +283,15 @@ class TransolverBlock(nn.Module):
                 normed, fx1 = PA.layer_norm_residual(self.Attn(x_in) + fx, self.ln_mlp1[0])
             else:
                 fx1, normed = pair
+            if type(mlp) is GatedMlp and PA.unhooked(mlp):
+                return mlp(normed, fx1), None
             if type(mlp) is not Mlp or not PA.unhooked(mlp):
                 return mlp(normed) + fx1, None
             return PA.mlp_residual(normed, fx1, mlp.layers, next_ln)
         x_in = normed_in if normed_in is not None else self.ln_1(fx)
+        drop = counter_dropout(self.Attn)
+        if drop is not None:
+            return self._mlp_residual(*self._dropped_residual_norm(drop, x_in, fx), next_ln)
         whole = self._whole_block(x_in, fx, next_ln)
         if whole is not None:
             return whole
@@ -308,8 +350,18 @@ class TransolverBlock(nn.Module):
             return PF.mlp_forward_packed(normed, packed, b1, b2, residual=fx1,
                                          ln_weight=next_ln.weight.detach().float().contiguous(),
                                          ln_bias=next_ln.bias.detach().float().contiguous(), ln_eps=next_ln.eps)
-        # MLP shapes the fused kernel does not serve: tensor-op MLP, then residual add (+ the next LayerNorm) in one pass
-        if self.fp8_weights and normed.is_cuda and normed.dtype == torch.bfloat16:
+        # MLPs the fused kernel does not serve: the MLP, then residual add (+ the next LayerNorm) in one pass
+        mlp, own = self.ln_mlp1[1], None
+        within = fx1 if next_ln is None and fx1.dtype == normed.dtype and fx1.shape == normed.shape else None
+        if self.int8_mlp is not None:
+            own = self.int8_mlp(mlp, normed, within)
+        if own is None and type(mlp) is GatedMlp and PA.unhooked(mlp):
+            own = mlp(normed, within)
+        if own is not None and within is not None:
+            return own, None
+        if own is not None:
+            h = own
+        elif self.fp8_weights and normed.is_cuda and normed.dtype == torch.bfloat16:
             w1, b1, w2, b2 = self._mlp_kernel_params(normed.device)
             F = torch.nn.functional
             h = F.linear(self.ln_mlp1[1].layers[1](F.linear(normed, w1, b1.to(normed.dtype))), w2, b2.to(normed.dtype))
@@ -340,7 +392,8 @@ class TransolverBlock(nn.Module):
 
 
 class Transolver(nn.Module):
-    """Transolver model (reference :447-736) built on the HIP PhysicsAttention layer."""
+    """Transolver model (reference :447-736) built on the HIP PhysicsAttention layer.  Beside the reference's activations
+    `act` takes "swiglu", "geglu", "reglu" and "glu": blocks with a `GatedMlp`, the preprocess Mlp with the gate's activation."""
 
     def __init__(self, functional_dim: int, out_dim: int, embedding_dim: int | None = None, n_layers: int = 4,
                  n_hidden: int = 256, dropout: float = 0.0, n_head: int = 8, act: str = "gelu", mlp_ratio: int = 4,
@@ -376,7 +429,7 @@ class Transolver(nn.Module):
             if embedding_dim is None:
                 raise ValueError("Transolver requires embedding_dim when unified_pos=False")
             self.embedding_dim = embedding_dim
-        self.preprocess = Mlp(functional_dim + self.embedding_dim, n_hidden * 2, n_hidden, act)
+        self.preprocess = Mlp(functional_dim + self.embedding_dim, n_hidden * 2, n_hidden, plain_act(act))
         self.time_input = time_input
         self.n_hidden = n_hidden
         if time_input:  # timestep embedding and its projection (reference :531-543)
@@ -466,6 +519,19 @@ class Transolver(nn.Module):
         the preprocess Mlp, the LayerNorms, the slice / qkv projections and the output head stay in higher precision."""
         for block in self.blocks:
             block.use_fp8_weights(enabled)
+        return self
+
+    def use_int8_mlp(self, enabled: bool = True):
+        """Inference with the products of every block's MLP in 8 bits (`TransolverBlock.use_int8_mlp`)."""
+        for block in self.blocks:
+            block.use_int8_mlp(enabled)
+        return self
+
+    def use_counter_dropout(self, seed: int):
+        """Every block's dropout from a counter-based generator (`TransolverBlock.use_counter_dropout`) of one seed: block k
+        counts its calls from k 2^40."""
+        for k, block in enumerate(self.blocks):
+            block.use_counter_dropout(seed, k << 40)
         return self
 
     def initialize_weights(self) -> None:

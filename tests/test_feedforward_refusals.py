@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+import physicsnemo_amd as pn
 from oracle import numpy_oracle as no
 from physicsnemo_amd import _lib
 from physicsnemo_amd import functional as PF
@@ -120,3 +121,63 @@ def test_mask_is_a_function_of_the_place():
     for other in (no.dropout_keep(4, 4, np.arange(64), 64, 0.5), no.dropout_keep(3, 5, np.arange(64), 64, 0.5),
                   no.dropout_keep(3, 4, np.arange(64) + 2 ** 32, 64, 0.5)):
         assert 0.4 < (other == full).mean() < 0.6
+
+
+def test_gated_module_on_the_cpu_is_the_formula():
+    for act, f in (("silu", torch.nn.functional.silu), ("gelu", torch.nn.functional.gelu), ("relu", torch.relu),
+                   ("sigmoid", torch.sigmoid), ("tanh", torch.tanh), (None, lambda t: t)):
+        mlp = pn.GatedMlp(6, 10, act, bias=act != "relu")
+        x, r = torch.randn(3, 6), torch.randn(3, 6)
+        lin = torch.nn.functional.linear
+        h = f(lin(x, mlp.gate.weight, mlp.gate.bias)) * lin(x, mlp.up.weight, mlp.up.bias)
+        assert torch.equal(mlp(x, r), lin(h, mlp.down.weight, mlp.down.bias) + r)
+    with pytest.raises(KeyError, match="not found"):
+        pn.GatedMlp(6, 10, "swish")
+
+
+@pytest.mark.parametrize("cls", [pn.Transolver, pn.FLAREModel])
+def test_models_of_gated_blocks(cls, tmp_path):
+    make = lambda act: cls(functional_dim=3, out_dim=2, embedding_dim=2, n_layers=2, n_hidden=32, dropout=0.1, n_head=4, act=act, use_te=False)
+    for act, gate, module in (("swiglu", "silu", torch.nn.SiLU), ("geglu", "gelu", torch.nn.GELU), ("reglu", "relu", torch.nn.ReLU),
+                              ("GLU", "sigmoid", torch.nn.Sigmoid)):
+        model = make(act)
+        assert all(type(b.ln_mlp1[1]) is pn.GatedMlp and b.ln_mlp1[1].act == gate for b in model.blocks)
+        assert type(model.preprocess.layers[1]) is module
+    model.save(str(tmp_path / "gated.mdlus"))
+    again = cls.from_checkpoint(str(tmp_path / "gated.mdlus"))
+    assert all(torch.equal(a, b) for a, b in zip(model.state_dict().values(), again.state_dict().values()))
+    assert type(make("gelu").blocks[0].ln_mlp1[1]) is pn.Mlp
+    with pytest.raises(KeyError, match="not found"):
+        make("swish")
+    keys = list(model.state_dict())
+    assert list(model.use_counter_dropout(5).state_dict()) == keys
+    assert [b.Attn.out_dropout.state.tolist() for b in model.blocks] == [[5, 0], [5, 1 << 40]]
+    assert [b.Attn.out_dropout.p for b in model.blocks] == [0.1, 0.1]
+
+
+def test_blocks_refuse_what_does_not_go_together():
+    plain, gated = (pn.TransolverBlock(4, 32, 0.1, act=act, use_te=False) for act in ("gelu", "swiglu"))
+    with pytest.raises(ValueError, match="fp8 weights"):
+        gated.use_fp8_weights()
+    with pytest.raises(ValueError, match="fp8 weights"):
+        plain.use_int8_mlp().use_fp8_weights()
+    plain.use_int8_mlp(False).use_fp8_weights()
+    with pytest.raises(ValueError, match="fp8 weights"):
+        plain.use_int8_mlp()
+    plain.use_fp8_weights(False)
+    plain.ln_mlp1[1].layers[0].register_forward_hook(lambda *a: None)
+    with pytest.raises(ValueError, match="without hooks"):
+        plain.use_int8_mlp()
+    gated.ln_mlp1[1].up = torch.nn.Identity()
+    with pytest.raises(ValueError, match="without hooks"):
+        gated.use_int8_mlp()
+
+
+def test_counter_dropout_off_the_gpu():
+    drop = pn.CounterDropout(0.5)
+    with pytest.raises(RuntimeError, match="GPU tensors only"):
+        drop(torch.zeros(4))
+    x = torch.zeros(4)
+    assert drop.eval()(x) is x and pn.CounterDropout(0.0)(x) is x
+    with pytest.raises(ValueError):
+        pn.CounterDropout(1.5)
