@@ -39,18 +39,33 @@ __global__ __launch_bounds__(256) void lay_out_kernel(Layout a) {
   const int64_t r0 = block / across * 64;
   const U *src = static_cast<const U *>(o.src);
   U *dst = static_cast<U *>(o.dst);
+  U v[16];  // all of a thread's loads before its first store: places outside are read at the nearest inside
   if (!o.turned) {
-    for (int k = y; k < 64; k += 4) {
-      const int64_t r = r0 + k;
-      if (r < o.rows && c0 + x < o.width) dst[r * o.ld + c0 + x] = c0 + x < o.cols ? src[r * o.src_ld + c0 + x] : U(0);
+    const int c = c0 + x < o.cols ? c0 + x : o.cols - 1;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int64_t r = r0 + y + 4 * k;
+      v[k] = src[(r < o.rows ? r : o.rows - 1) * o.src_ld + c];
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int64_t r = r0 + y + 4 * k;
+      if (r < o.rows && c0 + x < o.width) dst[r * o.ld + c0 + x] = c0 + x < o.cols ? v[k] : U(0);
     }
     return;
   }
-  for (int k = y; k < 64; k += 4)  // row c0 + k of src is column c0 + k of dst
-    turn[k][x] = c0 + k < o.cols && r0 + x < o.rows ? src[(int64_t)(c0 + k) * o.src_ld + r0 + x] : U(0);
+  const int64_t r = r0 + x < o.rows ? r0 + x : o.rows - 1;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {  // row c of src is column c of dst
+    const int c = c0 + y + 4 * k;
+    v[k] = src[(int64_t)(c < o.cols ? c : o.cols - 1) * o.src_ld + r];
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) turn[y + 4 * k][x] = c0 + y + 4 * k < o.cols ? v[k] : U(0);
   __syncthreads();
-  for (int k = y; k < 64; k += 4)
-    if (r0 + k < o.rows && c0 + x < o.width) dst[(r0 + k) * o.ld + c0 + x] = turn[x][k];
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (r0 + y + 4 * k < o.rows && c0 + x < o.width) dst[(r0 + y + 4 * k) * o.ld + c0 + x] = turn[x][y + 4 * k];
 }
 
 }  // namespace gated
@@ -101,21 +116,23 @@ __global__ __launch_bounds__(256) void totals_kernel(Totals a) {
     if (k < a.count && (int64_t)blockIdx.x >= a.r[k].first) o = a.r[k];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t e0 = ((int64_t)blockIdx.x - o.first) * 256;
+  float s[4] = {};  // of elements e0 + 64 j + lane: whole lines, whatever the alignment; past the end the last one again
+  const float *p[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {  // element e0 + 64 j + lane: whole lines, whatever the alignment
-    const int64_t e = e0 + 64 * j + lane;
-    float s = 0.f;
-    if (e < o.n) {
-      const float *p = o.src + e;
-      int g = wave;
-      for (; g + 12 < o.G; g += 16) {
-        const float v0 = p[g * o.stride], v1 = p[(g + 4) * o.stride], v2 = p[(g + 8) * o.stride], v3 = p[(g + 12) * o.stride];
-        s += (v0 + v1) + (v2 + v3);
-      }
-      for (; g < o.G; g += 4) s += p[g * o.stride];
-    }
-    part[wave][64 * j + lane] = s;
+  for (int j = 0; j < 4; ++j) p[j] = o.src + (e0 + 64 * j + lane < o.n ? e0 + 64 * j + lane : o.n - 1);
+  int g = wave;
+  for (; g + 4 < o.G; g += 8) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = p[j & 3][(g + (j & 4)) * o.stride];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += v[j] + v[4 + j];
   }
+  if (g < o.G)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] += p[j][g * o.stride];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) part[wave][64 * j + lane] = s[j];
   __syncthreads();
   const int64_t e = e0 + threadIdx.x;
   if (e >= o.n) return;
@@ -302,7 +319,7 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   void *wd_t = ws.take(F * Cp * e), *w_t = ws.take(C * 2 * Fp * e);
   const Partials in = partials_of<E>(M, 2 * Fp, Cp, num_cu, ws), down = partials_of<E>(M, Cp, Fp, num_cu, ws);
   // bf16: dg and du are rounded for their products, their column sums are not
-  const int64_t tiles = (M + 31) / 32, parts = tiles < 1024 ? (tiles + 31) / 32 : 32;
+  const int64_t tiles = (M + 31) / 32, parts = tiles < 2048 ? (tiles + 31) / 32 : 64;
   float *sums = e == 2 ? static_cast<float *>(ws.take(tiles * 2 * Fp * 4)) : nullptr;
   float *sum_parts = e == 2 ? static_cast<float *>(ws.take(parts * 2 * Fp * 4)) : nullptr;
   if (plan) return *bytes = ws.used, PA_OK;

@@ -1156,14 +1156,17 @@ def _act_code(act: str | None) -> int:
         raise ValueError(f"activation {act!r} not found; available are {[a for a in _lib.ACTS if a]} and None") from None
 
 
-def _same_device(x, *others):
-    for t in others:
-        if t is not None and t.device != x.device:
-            raise ValueError(f"all tensors have to be on the input's device ({x.device}), got one on {t.device}")
+def _together(x, *others):
+    """Everything on x's GPU and contiguous."""
+    device = x.device
+    for t in (x, *others):
+        if t is not None and not (t.is_cuda and t.is_contiguous() and t.device == device):
+            _need_cuda(x, *others)
+            raise ValueError(f"all tensors have to be on the input's device ({device}), got one on {t.device}")
 
 
-def _expect(t, what: str, shape, dtype):
-    if t is not None and (tuple(t.shape) != tuple(shape) or t.dtype != dtype):
+def _expect(t, what: str, shape: tuple, dtype):
+    if t is not None and (t.shape != shape or t.dtype != dtype):
         raise ValueError(f"{what} has to be {dtype} of shape {tuple(shape)}, got {t.dtype} of shape {tuple(t.shape)}")
 
 
@@ -1173,10 +1176,9 @@ def _sized(code: int, what: str) -> int:
     return int(code)
 
 
-def _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, b_down):
-    """(rows, C, F) after checking that the parameters belong together and to x."""
-    _need_cuda(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
-    _same_device(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
+def _gated_sizes(x, rows, w_gate, b_gate, w_up, b_up, w_down, b_down):
+    """(rows, C, F) after checking that the parameters, and `rows` like x's, belong together and to x."""
+    _together(x, rows, w_gate, b_gate, w_up, b_up, w_down, b_down)
     _lib.dtype_code(x.dtype)
     if x.ndim < 1 or w_gate.ndim != 2:
         raise ValueError("x needs a last axis of channels and w_gate the shape (F, C)")
@@ -1195,10 +1197,8 @@ def gated_mlp_forward(x, w_gate, b_gate, w_up, b_up, w_down, b_down, act: str | 
 
     x (..., C) bfloat16 or float32; w_gate, w_up (F, C) and w_down (C, F) in the same type; biases float32 or None; `act`
     one of "silu", "gelu" (erf form), "relu", "sigmoid", "tanh", None.  Any widths."""
-    rows, C, F = _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, b_down)
+    rows, C, F = _gated_sizes(x, residual, w_gate, b_gate, w_up, b_up, w_down, b_down)
     code = _act_code(act)
-    _need_cuda(residual)
-    _same_device(x, residual)
     _expect(residual, "residual", x.shape, x.dtype)
     y = torch.empty_like(x)
     if rows == 0:
@@ -1216,10 +1216,8 @@ def gated_mlp_forward(x, w_gate, b_gate, w_up, b_up, w_down, b_down, act: str | 
 def gated_mlp_backward(x, dy, w_gate, b_gate, w_up, b_up, w_down, act: str | None = "silu", wanted=(True,) * 7):
     """Gradients of `gated_mlp_forward` for dy: (dx, d w_gate, d b_gate, d w_up, d b_up, d w_down, d b_down), weight gradients
     in the weights' type, bias gradients float32; `wanted` says which of the seven are formed, the others are None."""
-    rows, C, F = _gated_sizes(x, w_gate, b_gate, w_up, b_up, w_down, None)
+    rows, C, F = _gated_sizes(x, dy, w_gate, b_gate, w_up, b_up, w_down, None)
     code = _act_code(act)
-    _need_cuda(dy)
-    _same_device(x, dy)
     _expect(dy, "dy", x.shape, x.dtype)
     shapes = (x.shape, (F, C), (F,), (F, C), (F,), (C, F), (C,))
     types = (x.dtype, x.dtype, torch.float32, x.dtype, torch.float32, x.dtype, torch.float32)
@@ -1240,8 +1238,7 @@ def gated_mlp_backward(x, dy, w_gate, b_gate, w_up, b_up, w_down, act: str | Non
 
 
 def _dropout_args(x, p, rng, *rows):
-    _need_cuda(x, rng, *rows)
-    _same_device(x, rng, *rows)
+    _together(x, rng, *rows)
     _lib.dtype_code(x.dtype)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability has to be between 0 and 1, got {p}")
@@ -1262,8 +1259,7 @@ def dropout_add_norm(x, residual, p: float, rng, ln_weight=None, ln_bias=None, l
     C = x.shape[-1]
     if (ln_weight is None) != (ln_bias is None):
         raise ValueError("ln_weight and ln_bias are given together")
-    _need_cuda(ln_weight, ln_bias)
-    _same_device(x, ln_weight, ln_bias)
+    _together(x, ln_weight, ln_bias)
     _expect(ln_weight, "ln_weight", (C,), torch.float32)
     _expect(ln_bias, "ln_bias", (C,), torch.float32)
     rows = x.numel() // C if C else 0
@@ -1296,8 +1292,7 @@ def dropout_add_norm_backward(dy, d_normed, x, residual, stats, ln_weight, p: fl
     rows = rows_like.numel() // C if C else 0
     device = rows_like.device
     if norm:
-        _need_cuda(stats, ln_weight)
-        _same_device(rows_like, stats, ln_weight)
+        _together(rows_like, stats, ln_weight)
         _expect(stats, "stats", (rows, 2), torch.float32)
         _expect(ln_weight, "ln_weight", (C,), torch.float32)
     dx = torch.empty_like(rows_like) if need_dx else None
@@ -1350,8 +1345,7 @@ def quantize_int8(x):
 
 
 def _int8_weight(x, name, w, scale, bias, shape):
-    _need_cuda(w, scale, bias)
-    _same_device(x, w, scale, bias)
+    _together(x, w, scale, bias)
     _expect(w, f"w_{name}", shape, torch.int8)
     _expect(scale, f"the scale of w_{name}", shape[:1], torch.float32)
     _expect(bias, f"the bias of w_{name}", shape[:1], torch.float32)
@@ -1361,8 +1355,7 @@ def linear_int8(x, weight, weight_scale, bias=None, act: str | None = None, resi
     """y = act(weight . x + bias) [+ residual] with an 8-bit weight (N, K) int8, one float32 scale per output channel
     (`quantize_int8` of the weight), and x (..., K) bfloat16 or float32 rounded to 8 bits per token on the way; the sums of
     products are exact.  bias (N) float32 or None.  For inference: it has no gradient."""
-    _need_cuda(x, residual)
-    _same_device(x, residual)
+    _together(x, residual)
     dtype, code = _lib.dtype_code(x.dtype), _act_code(act)
     if x.ndim < 1 or weight.ndim != 2 or x.shape[-1] == 0 or weight.shape[0] == 0:
         raise ValueError("x needs a last axis of channels and weight the shape (N, K)")
@@ -1386,8 +1379,7 @@ def linear_int8(x, weight, weight_scale, bias=None, act: str | None = None, resi
 def gated_mlp_int8(x, w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, b_down, act: str | None = "silu", residual=None):
     """`gated_mlp_forward` on 8-bit weights (int8 with one float32 scale per output channel, `quantize_int8`) and activations
     rounded to 8 bits per token, the hidden layer likewise.  For inference: it has no gradient."""
-    _need_cuda(x, residual)
-    _same_device(x, residual)
+    _together(x, residual)
     dtype, code = _lib.dtype_code(x.dtype), _act_code(act)
     if x.ndim < 1 or w_gate.ndim != 2 or x.shape[-1] == 0 or w_gate.shape[0] == 0:
         raise ValueError("x needs a last axis of channels and w_gate the shape (F, C)")
