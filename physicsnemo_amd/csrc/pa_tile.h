@@ -78,28 +78,29 @@ enum Act { kNone = 0, kGelu = 1, kRelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5, 
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v)); }
 
-template <bool SHORT>  // rounded to bf16 next
-__device__ __forceinline__ void act_values(int act, f32x16 &v) {
+template <bool SHORT, class V>  // SHORT: rounded to bf16 next
+__device__ __forceinline__ void act_values(int act, V &v) {
+  constexpr int N = sizeof(V) / 4;
   switch (act) {
     case kGelu:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = SHORT ? gelu_short(v[r]) : gelu_tail(v[r]);
+      for (int r = 0; r < N; ++r) v[r] = SHORT ? gelu_short(v[r]) : gelu_tail(v[r]);
       break;
     case kRelu:  // NaN passes, as torch's does
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = v[r] < 0.f ? 0.f : v[r];
+      for (int r = 0; r < N; ++r) v[r] = v[r] < 0.f ? 0.f : v[r];
       break;
     case kSilu:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] *= sigmoid(v[r]);
+      for (int r = 0; r < N; ++r) v[r] *= sigmoid(v[r]);
       break;
     case kSigmoid:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = sigmoid(v[r]);
+      for (int r = 0; r < N; ++r) v[r] = sigmoid(v[r]);
       break;
     case kTanh:
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = tanhf(v[r]);
+      for (int r = 0; r < N; ++r) v[r] = tanhf(v[r]);
       break;
     default: break;
   }
@@ -748,6 +749,162 @@ int launch_tiles(Args a, int num_cu, hipStream_t st) {
   return launch_status();
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// few_rows_kernel.  Products of so few rows that tiles of them leave most CUs idle while each works through the whole reduction,
+// a stage behind the other.  A workgroup of eight waves forms 32 rows x 32 columns (kGated: both factors of them); each wave takes an
+// eighth of the reduction, operands straight from memory to registers, CHUNK steps of loads in flight and no barrier; the eight
+// sums meet in LDS and are added in the order of the waves.  Tiles are dealt out to the XCDs in eight equal runs with the rows running
+// fastest, so that the workgroups of an L2 share columns of W.
+// ---------------------------------------------------------------------------------------------------------------
+template <class E, class TO, Kind KIND>
+__global__ __launch_bounds__(512) void few_rows_kernel(Args a) {
+  constexpr int UNITS = E::kBytes == 4 ? 4 : 2, HALVES = UNITS / 2, PAIR = KIND == kGated ? 2 : 1;  // units of a step; products
+  constexpr int CHUNK = (E::kBytes == 4 ? 8 : 16) / PAIR;
+  using Acc = typename E::Acc;
+  extern __shared__ u32x4 smem[];  // [wave][product][q][lane]
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8, tn = tile / a.mt, tm = tile - tn * a.mt;
+  if (tn >= a.nt) return;
+  const int64_t m = (int64_t)tm * 32 + i;
+  const int n = tn * 32 + i < a.N ? tn * 32 + i : a.N - 1;
+  const char *xp = static_cast<const char *>(a.X) + (a.x_groups ? (int64_t)tm * 32 * a.ldx + i * 32 : (m < a.M ? m : a.M - 1) * a.ldx);
+  const char *wp[PAIR];
+#pragma unroll
+  for (int k = 0; k < PAIR; ++k) wp[k] = static_cast<const char *>(a.W[k]) + n * a.ldw;
+  const int steps = (a.units + UNITS - 1) / UNITS, per = (steps + 7) / 8, first = wave * per, last = first + per < steps ? first + per : steps;
+  Acc acc[PAIR];
+#pragma unroll
+  for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[k][r] = 0;
+#pragma clang loop unroll(disable)
+  for (int s = first; s < last; s += CHUNK) {
+    u32x4 x[CHUNK][HALVES], w[PAIR][CHUNK][HALVES];
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) {
+      if (s + c >= last) break;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        const int want = UNITS * (s + c) + 2 * h + g, u = want < a.units ? want : a.units - 1;
+        x[c][h] = *reinterpret_cast<const u32x4 *>(xp + (a.x_groups ? u / 2 * 1024 + u % 2 * 16 : u * 16));
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) w[k][c][h] = *reinterpret_cast<const u32x4 *>(wp[k] + u * 16);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNK; ++c) {
+      if (s + c >= last) break;
+      if (UNITS * (s + c + 1) > a.units) {
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+          if (UNITS * (s + c) + 2 * h + g >= a.units) {
+            x[c][h] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int k = 0; k < PAIR; ++k) w[k][c][h] = u32x4{0u, 0u, 0u, 0u};
+          }
+      }
+      if constexpr (E::kBytes == 4) {
+        const typename E::Parts xs = E::split(x[c][0], x[c][1]);
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) acc[k] = E::mma(E::split(w[k][c][0], w[k][c][1]), xs, acc[k]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < PAIR; ++k) acc[k] = E::mma(w[k][c][0], x[c][0], acc[k]);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < PAIR; ++k)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      u32x4 v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const auto r = acc[k][4 * q + j];
+        v[j] = __builtin_bit_cast(uint32_t, r);
+      }
+      smem[((wave * PAIR + k) * 4 + q) * 64 + lane] = v;
+    }
+  __syncthreads();
+  if (wave >= 4) return;
+  const int q = wave, col = tn * 32 + 8 * q + 4 * g;
+  const float sx = E::kBytes == 1 && m < a.M ? a.sx[m] : 1.f;
+  f32x4 v[PAIR];
+#pragma unroll
+  for (int k = 0; k < PAIR; ++k) {
+    using Sum = typename std::conditional<E::kBytes == 1, int, float>::type;
+    Sum sum[4] = {};
+#pragma unroll
+    for (int from = 0; from < 8; ++from) {
+      const u32x4 t = smem[((from * PAIR + k) * 4 + q) * 64 + lane];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t bits = t[j];
+        sum[j] += __builtin_bit_cast(Sum, bits);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool in = col + j < a.N;
+      const float bias = a.bias[k] && in ? a.bias[k][col + j] : 0.f;
+      if constexpr (E::kBytes == 1) v[k][j] = fmaf((float)sum[j], (in ? a.sw[k][col + j] : 0.f) * sx, bias);
+      else v[k][j] = sum[j] + bias;
+    }
+  }
+  act_values<sizeof(TO) == 2>(a.act, v[0]);
+  if (m >= a.M) return;
+  if constexpr (KIND == kGated) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[0][j] = col + j < a.N ? v[0][j] * v[1][j] : 0.f;
+    if (col >= a.limit) return;
+    char *to = static_cast<char *>(a.out) + (kGrouped<TO> ? m / 32 * 32 * a.ldo * 2 + col / 16 * 1024 + m % 32 * 32 + col % 16 * 2
+                                                           : (m * a.ldo + col) * (int64_t)sizeof(TO));
+    if constexpr (sizeof(TO) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack2(v[0][0], v[0][1]), pack2(v[0][2], v[0][3])};
+    else *reinterpret_cast<f32x4 *>(to) = v[0];
+  } else {
+    TO *to = static_cast<TO *>(a.out) + m * a.ldo + col;
+    const TO *add = a.residual ? static_cast<const TO *>(a.residual) + m * a.ldo + col : nullptr;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (add && col + j < a.N) v[0][j] += load_as_f32(add + j);
+    if (a.vec) {  // whole units: four columns or none
+      if (col >= a.N) return;
+      if constexpr (sizeof(TO) == 2) *reinterpret_cast<u32x2 *>(to) = u32x2{pack2(v[0][0], v[0][1]), pack2(v[0][2], v[0][3])};
+      else *reinterpret_cast<f32x4 *>(to) = v[0];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < a.N) store_from_f32(to + j, v[0][j]);
+    }
+  }
+}
+
+// Whether it is the shorter way, in us behind the launch: what a wave works through one after the other, its eighth of the reduction
+// for every round of workgroups over the CUs, against all stages of a 64 x 64 tile.  Measured, tiles / few rows:
+// bf16 2 048 -> 512, 64 rows 17.9 / 8.8, 1 000 (two rounds) 18.0 / 17.1, 1 500 17.8 / 25.0; 512 -> 2 x 2 048, 64 rows 6.5 / 6.9;
+// float32 2 048 -> 512, 64 rows 75.6 / 21.9, 1 500 77.6 / 68.5, 2 000 77.9 / 89.3, 512 -> 2 x 2 048, 64 rows 21.6 / 10.1, 400 32.7 /
+// 36.4; int8 512 -> 2 048, 64 rows 6.0 / 4.3, 400 6.3 / 9.5, 2 048 -> 512, 64 rows 11.0 / 7.6, 600 11.3 / 12.3.
+template <class E, Kind KIND>
+bool few_rows_worth(const Args &a, int64_t stages, int num_cu) {
+  const double step = E::kBytes == 4 ? 1.2 : 0.4;  // of a tile's stage and of a wave's step alike
+  const int64_t units = E::kBytes == 4 ? 4 : 2, per = ((a.units + units - 1) / units + 7) / 8;
+  const int64_t groups = ((a.M + 31) / 32) * ((a.N + 31) / 32), columns = KIND == kGated ? 32 : 64;
+  const int64_t tiles = ((a.M + 63) / 64) * ((a.N + columns - 1) / columns);
+  const int64_t rounds = (groups + num_cu - 1) / num_cu, of_tiles = (tiles + num_cu - 1) / num_cu;
+  return rounds * (1.5 + step * per * (KIND == kGated ? 2 : 1)) <= 1.5 + step * stages * of_tiles;
+}
+
+template <class E, class TO, Kind KIND>
+int launch_few_rows(Args a, hipStream_t st) {
+  constexpr size_t lds = 8 * (KIND == kGated ? 2 : 1) * 4 * 1024;
+  a.mt = (int)((a.M + 31) / 32), a.nt = (a.N + 31) / 32;
+  auto kernel = few_rows_kernel<E, TO, KIND>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(((int64_t)a.nt * a.mt + 7) / 8 * 8)), dim3(512), lds, st, a);
+  return launch_status();
+}
+
 // Tiles of 256 x 256 (kBack: 128 x 256) for large products, 128 x 128 and two workgroups per CU where those leave CUs idle, 64 x 64
 // where the product is small.  Taken by the weight rows and rows that the busiest CU has to work off, smaller tiles counted
 // dearer for the operands they fetch again.  Measured at 256 / 128 (us): 131 072 rows, 1 024 -> 256 bf16 107 / 117, 2 048 -> 256
@@ -785,6 +942,8 @@ int launch(Args a, int num_cu, hipStream_t st) {
   using Medium = Config<2, 2, 2, 2, 8, 2, 2>;
   using Small = Config<2, 1, 1, 2, 8, 3, 2>;
   const int64_t stages = (a.units + 7) / 8 + (KIND == kBack ? (a.units2 + 7) / 8 : 0);
+  if constexpr (KIND == kPlain || (KIND == kGated && E::kBytes != 1))
+    if (few_rows_worth<E, KIND>(a, stages, num_cu)) return launch_few_rows<E, TO, KIND>(a, st);
   auto run = [&](const Args &t, int size) {
     if (size == 0) return launch_tiles<E, TO, KIND, Large>(t, num_cu, st);
     if (size == 1) return launch_tiles<E, TO, KIND, Medium>(t, num_cu, st);
