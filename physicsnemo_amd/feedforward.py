@@ -84,7 +84,7 @@ class CounterDropout(nn.Dropout):
     """Dropout whose mask is a function of (seed, offset) and of the element's place (`functional.dropout_add_norm`): it is never
     stored, the backward pass forms it again, and every call takes the next offset, in a captured graph every replay.
 
-    `state` is the int64 pair (seed, next offset).  It is no entry of the state dict; to go on after a restart with the masks
+    `state` is the int64 pair (seed, next offset); masks come again after 2^32 calls.  It is no entry of the state dict; to go on after a restart with the masks
     that would have come next, save it and set it again.  Processes that train together take different seeds.  Calls of one
     module run on one stream at a time.  A backward pass that runs the module again (activation checkpointing) would draw
     another mask and is refused."""

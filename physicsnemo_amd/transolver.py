@@ -528,10 +528,10 @@ class Transolver(nn.Module):
         return self
 
     def use_counter_dropout(self, seed: int):
-        """Every block's dropout from a counter-based generator (`TransolverBlock.use_counter_dropout`) of one seed: block k
-        counts its calls from k 2^40."""
+        """Every block's dropout from a counter-based generator (`TransolverBlock.use_counter_dropout`), block k under
+        seed + k 2^32: seeds below 2^32 give every block of every process masks of its own."""
         for k, block in enumerate(self.blocks):
-            block.use_counter_dropout(seed, k << 40)
+            block.use_counter_dropout((seed + (k << 32) + 2 ** 63) % 2 ** 64 - 2 ** 63)
         return self
 
     def initialize_weights(self) -> None:

@@ -151,7 +151,8 @@ def test_models_of_gated_blocks(cls, tmp_path):
         make("swish")
     keys = list(model.state_dict())
     assert list(model.use_counter_dropout(5).state_dict()) == keys
-    assert [b.Attn.out_dropout.state.tolist() for b in model.blocks] == [[5, 0], [5, 1 << 40]]
+    assert [b.Attn.out_dropout.state.tolist() for b in model.blocks] == [[5, 0], [5 + (1 << 32), 0]]
+    assert model.use_counter_dropout(2 ** 63 - 1).blocks[1].Attn.out_dropout.state.tolist() == [-(2 ** 63) + 2 ** 32 - 1, 0]
     assert [b.Attn.out_dropout.p for b in model.blocks] == [0.1, 0.1]
 
 

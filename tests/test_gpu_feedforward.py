@@ -287,7 +287,10 @@ def test_models_train_and_serve(kind):
     first, second = step(), step()
     assert all(bool(torch.isfinite(t).all()) for t in first)
     assert not torch.equal(first[0], second[0])
-    assert [b.Attn.out_dropout.state.tolist() for b in model.blocks] == [[21, 2], [21, (1 << 40) + 2]]
+    assert [b.Attn.out_dropout.state.tolist() for b in model.blocks] == [[21, 2], [21 + (1 << 32), 2]]
+    ones = torch.ones(64, 64, device=DEV)
+    masks = [PF.dropout_add_norm(ones, None, 0.5, b.Attn.out_dropout.state) for b in model.blocks]
+    assert 0.4 < float((masks[0] == masks[1]).float().mean()) < 0.6  # 4 096 fair coins: 0.5 within 0.1 by 12 of their deviations
     for b in model.blocks:
         b.Attn.out_dropout.state = b.Attn.out_dropout.state - torch.tensor([0, 2], device=DEV)
     again = step()
