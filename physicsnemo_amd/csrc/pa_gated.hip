@@ -343,7 +343,7 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
     a.M = rest, a.N = (int)F, a.limit = (int)Fp;
     a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
-    a.sums = out.b_gate || out.b_up ? reinterpret_cast<float *>(from(sums, 2 * Fp * 4 / 32)) : nullptr;
+    a.sums = e == 2 && (out.b_gate || out.b_up) ? reinterpret_cast<float *>(from(sums, 2 * Fp * 4 / 32)) : nullptr;
     a.out = from(dgu, 2 * Fp * e), a.ldo = 2 * Fp, a.out2 = from(h, Fp * e), a.ldh = Fp, a.act = act;
     if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
   }
@@ -357,11 +357,14 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     if ((rc = product<E, TO, tile::kPlain>(d, num_cu, st))) return rc;
   }
   Totals totals;
-  if (out.w_gate || out.w_up || out.b_gate || out.b_up) {
+  const bool in_biases = out.b_gate || out.b_up;
+  if (out.w_gate || out.w_up || (e == 4 && in_biases)) {
     if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, 1, num_cu, st))) return rc;
     totals.add(in.product, in.G, 2 * Fp * Cp, Cp, out.w_gate, F, C, e);
     totals.add(in.product + Fp * Cp, in.G, 2 * Fp * Cp, Cp, out.w_up, F, C, e);
-    if (e == 2 && (out.b_gate || out.b_up)) {
+  }
+  if (in_biases) {
+    if (e == 2) {
       hipLaunchKernelGGL(tile_sums_kernel, dim3((unsigned)((2 * Fp + 255) / 256), (unsigned)parts), dim3(256), 0, st, sums, sum_parts, tiles,
                          (int)(2 * Fp));
       if ((rc = launch_status())) return rc;

@@ -410,7 +410,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       xb[ks] = *reinterpret_cast<const u32x4 *>(a.x + r * C + at);
       db[ks] = *reinterpret_cast<const u32x4 *>(a.dy + r * C + at);
       if (32 * CT > C && col >= C) xb[ks] = db[ks] = u32x4{0u, 0u, 0u, 0u};
-      if (mb * ROWS + wave * 32 + i >= a.M) db[ks] = u32x4{0u, 0u, 0u, 0u};  // a repeated row: of no gradient
+      if (mb * ROWS + wave * 32 + i >= a.M) xb[ks] = db[ks] = u32x4{0u, 0u, 0u, 0u};  // a repeated row: of no gradient
     }
   };
   int buf = 0;

@@ -701,10 +701,6 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           } else {
             const Buffer hidden = rows_or_blocks_at(a.out2, a.ldh);
             f32x16 slope, d = acc2[m][n];
-            if (rl >= have) {  // a repeated row: of no gradient
-#pragma unroll
-              for (int r = 0; r < 16; ++r) d[r] = 0.f;
-            }
             act_slopes(a.act, gate, slope);
             f32x16 h;
 #pragma unroll
@@ -715,6 +711,10 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
             }
             cut(h), cut(slope), cut(gate);
             if (E::kBytes == 2 && a.sums) {
+              if (rl >= have) {  // a repeated row
+#pragma unroll
+                for (int r = 0; r < 16; ++r) slope[r] = gate[r] = 0.f;
+              }
               const f32x4 s = column_sums(slope, gate, lane);
               const int c = col + 8 * (lane & 3) + 4 * g;
               if (i < 8 && c < a.limit && (wm * TM + m) * 32 < have)
@@ -881,7 +881,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Args a) {
 }
 
 // Whether it is the shorter way, in us behind the launch: what a wave works through one after the other, its eighth of the reduction
-// for every round of workgroups over the CUs, against all stages of a 64 x 64 tile.  Measured, tiles / few rows:
+// for every round of workgroups over the CUs, against all stages of a 64 x 64 tile, as long as those are one round.  Measured, tiles
+// / few rows:
 // bf16 2 048 -> 512, 64 rows 17.9 / 8.8, 1 000 (two rounds) 18.0 / 17.1, 1 500 17.8 / 25.0; 512 -> 2 x 2 048, 64 rows 6.5 / 6.9;
 // float32 2 048 -> 512, 64 rows 75.6 / 21.9, 1 500 77.6 / 68.5, 2 000 77.9 / 89.3, 512 -> 2 x 2 048, 64 rows 21.6 / 10.1, 400 32.7 /
 // 36.4; int8 512 -> 2 048, 64 rows 6.0 / 4.3, 400 6.3 / 9.5, 2 048 -> 512, 64 rows 11.0 / 7.6, 600 11.3 / 12.3.
@@ -891,8 +892,8 @@ bool few_rows_worth(const Args &a, int64_t stages, int num_cu) {
   const int64_t units = E::kBytes == 4 ? 4 : 2, per = ((a.units + units - 1) / units + 7) / 8;
   const int64_t groups = ((a.M + 31) / 32) * ((a.N + 31) / 32), columns = KIND == kGated ? 32 : 64;
   const int64_t tiles = ((a.M + 63) / 64) * ((a.N + columns - 1) / columns);
-  const int64_t rounds = (groups + num_cu - 1) / num_cu, of_tiles = (tiles + num_cu - 1) / num_cu;
-  return rounds * (1.5 + step * per * (KIND == kGated ? 2 : 1)) <= 1.5 + step * stages * of_tiles;
+  const int64_t rounds = (groups + num_cu - 1) / num_cu;
+  return tiles <= num_cu && rounds * (1.5 + step * per * (KIND == kGated ? 2 : 1)) <= 1.5 + step * stages;
 }
 
 template <class E, class TO, Kind KIND>

@@ -304,6 +304,23 @@ def test_models_train_and_serve(kind):
         assert torch.equal(call(model.use_int8_mlp(False), fx, emb), plain)
 
 
+@pytest.mark.parametrize("act", ["swiglu", "geglu", "reglu", "glu"])
+@pytest.mark.parametrize("kind", ["transolver", "flare", "geotransolver"])
+def test_models_of_gated_blocks_are_their_tensor_ops(kind, act):
+    """In float32, against the same model with hooks on its gated MLPs, which then run as tensor ops: within the 1e-4 that float32
+    models are held to everywhere."""
+    announce("model, gated", kind, act)
+    model = make_model(kind, act).to(DEV).eval()
+    fx, emb = torch.randn(2, 70, 3, device=DEV), torch.randn(2, 70, 2, device=DEV)
+    with torch.no_grad():
+        y, seen = call(model, fx, emb), []
+        for b in model.blocks:
+            b.ln_mlp1[1].gate.register_forward_hook(lambda *a: seen.append(1))
+        want = call(model, fx, emb)
+    assert len(seen) == len(model.blocks)
+    assert float((y - want).norm()) <= 1e-4 * float(want.norm())
+
+
 def test_a_captured_training_step_draws_new_masks():
     """Forward and backward of a block in a graph: every replay is the eager step of the same counter, bit for bit."""
     announce("block, captured training step")

@@ -207,6 +207,22 @@ def test_infinities_and_nan_stay_in_their_rows(where):
     assert torch.equal(y[~hit], clean[~hit]) and not torch.isfinite(y[hit]).any()
 
 
+@pytest.mark.parametrize("rows,C,F", [(33, 24, 40), (40_001, 128, 64)])
+def test_bias_gradients_with_an_infinite_last_row(rows, C, F):
+    """Rows are worked off in blocks; what fills the last one takes no part: inf x 0 of it would be NaN."""
+    announce("gated, infinite last row", rows, C, F)
+    st = make(rows, C, F, torch.bfloat16, seed=21)
+    st["x"][-1, 0] = float("inf")
+    st["w_gate"][:, 0] = st["w_gate"][:, 0].abs() + 0.25
+    st["w_up"][:, 0] = st["w_up"][:, 0].abs() + 0.25
+    gpu = on_gpu(st)
+    grads = PF.gated_mlp_backward(gpu["x"], gpu["dy"], *[gpu[n] for n in NAMES[:5]], act=None, wanted=(False, False, True, False, True, False, False))
+    sign = torch.sign(st["dy"][-1].double() @ st["w_down"].double())  # of d h in the last row, whose g and u are + infinity
+    assert bool((sign != 0).all())
+    for got in (grads[2], grads[4]):
+        assert torch.equal(got.double().cpu(), sign * float("inf"))
+
+
 def test_no_rows_and_wanted_gradients():
     announce("gated empty")
     st = on_gpu(make(6, 16, 24, torch.float32))
