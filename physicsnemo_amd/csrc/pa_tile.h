@@ -371,8 +371,10 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
   int lt = t, lk = 0;  // tile and stage that are fetched next
   unsigned buf = 0;    // where they go
   int sbuf = 0;        // and the side data
+  int left = 0;        // units of its rows from its first on
   unsigned offx[NX], offw[NW];
-  const char *xbase = nullptr, *wbase[2] = {nullptr, nullptr};
+  const char *xs = nullptr, *ws0 = nullptr, *ws1 = nullptr;
+  const int64_t xstep = KIND == kPlain && a.x_groups ? 512 * UPS : 16 * UPS;
   const int frow = lane / UPS, fpos = lane % UPS;
   auto uniform = [](const char *p) {  // what is the same for every lane, in scalar registers
     const uint64_t v = (uint64_t)(uintptr_t)p;
@@ -384,9 +386,10 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
     const int tm = lt / a.nt, tn = lt - tm * a.nt;
     const int64_t m0 = (int64_t)tm * BM, ldx = second ? a.ldx2 : a.ldx, ldw = second ? a.ldw2 : a.ldw;
     const int have = (int)(a.M - m0 < BM ? a.M - m0 : BM), n0 = tn * CN, haven = a.N - n0;
-    xbase = static_cast<const char *>(second ? a.X2 : a.X) + m0 * ldx;
-    wbase[0] = static_cast<const char *>(second ? a.W[2] : a.W[0]) + n0 * ldw;
-    if constexpr (DUAL) wbase[1] = static_cast<const char *>(a.W[1]) + n0 * ldw;
+    left = second ? a.units2 : a.units;
+    xs = uniform(static_cast<const char *>(second ? a.X2 : a.X) + m0 * ldx);
+    ws0 = uniform(static_cast<const char *>(second ? a.W[2] : a.W[0]) + n0 * ldw);
+    if constexpr (DUAL) ws1 = uniform(static_cast<const char *>(a.W[1]) + n0 * ldw);
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
       const int row = (wave * NX + q) * GROUP + frow, r = row < have ? row : have - 1;
@@ -405,11 +408,8 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
     const bool none = lt >= last;  // past the last tile: the last stage again, so that every stage counts the same loads
     const bool second = KIND == kBack && (none ? nk1 < nk : lk >= nk1);
     if (!none && (lk == 0 || (KIND == kBack && lk == nk1))) place(second);
-    const int kb = none ? (second ? nk - nk1 : nk1) - 1 : second ? lk - nk1 : lk, left = (second ? a.units2 : a.units) - UPS * kb;
+    else if (!none) left -= UPS, xs += xstep, ws0 += 16 * UPS, ws1 += DUAL ? 16 * UPS : 0;
     const unsigned dst = (unsigned)(uintptr_t)smem + buf;
-    // units past the row's last one: that one again; the products leave them out
-    auto past = [&](int unit) { return 16u * (unsigned)(unit >= left ? unit - left + 1 : 0); };
-    const unsigned past_even = past(fpos ^ swizzle(frow)), past_odd = past(fpos ^ swizzle(frow + GROUP));
     if (!none && lk == 0) {
       const int n0 = (lt % a.nt) * CN;
       const int64_t m0 = (int64_t)(lt / a.nt) * BM;
@@ -429,29 +429,34 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
       }
       sbuf = sbuf + 1 == RING ? 0 : sbuf + 1;
     }
-    auto off_of = [&](unsigned off, int grp) { return (int)(off - (grp & 1 ? past_odd : past_even)); };
-    unsigned xpast_even = past_even, xpast_odd = past_odd;
-    if (KIND == kPlain && a.x_groups) {
-      auto past_groups = [&](int unit) {
-        const int to = unit >= left ? left - 1 : unit;
-        return (unsigned)(((unit >> 1) - (to >> 1)) * 1024 + ((unit & 1) - (to & 1)) * 16);
+    auto load = [&](auto x_off, auto w_off) {
+#pragma unroll
+      for (int q = 0; q < NX; ++q) {
+        const int grp = wave * NX + q;
+        load_unit_to_lds(xs, (int)x_off(offx[q], grp), dst + grp * 1024);
+      }
+#pragma unroll
+      for (int q = 0; q < NW; ++q) {
+        const int grp = wave * NW + q;
+        // second: half as many rows; in a longer ring the other loads are made all the same, so that every stage counts as many
+        if (AHEAD == 1 && second && grp * GROUP >= BN / 2) continue;
+        load_unit_to_lds(DUAL && !second && (grp & (32 / GROUP)) ? ws1 : ws0, (int)w_off(offw[q], grp), dst + BM * 16 * UPS + grp * 1024);
+      }
+    };
+    if (left >= UPS) {
+      auto as_it_is = [](unsigned off, int) { return off; };
+      load(as_it_is, as_it_is);
+    } else {  // units past the row's last one: that one again; the products leave them out
+      const int unit[2] = {fpos ^ swizzle(frow), fpos ^ swizzle(frow + GROUP)};
+      auto w_off = [&](unsigned off, int grp) {
+        const int u = unit[grp & 1];
+        return off - 16u * (unsigned)(u >= left ? u - left + 1 : 0);
       };
-      xpast_even = past_groups(fpos ^ swizzle(frow)), xpast_odd = past_groups(fpos ^ swizzle(frow + GROUP));
-    }
-    const int64_t xstep = KIND == kPlain && a.x_groups ? 512 * UPS : 16 * UPS;
-    const char *xs = uniform(xbase + (int64_t)kb * xstep), *ws0 = uniform(wbase[0] + (int64_t)kb * (16 * UPS));
-    const char *ws1 = DUAL ? uniform(wbase[1] + (int64_t)kb * (16 * UPS)) : ws0;
-#pragma unroll
-    for (int q = 0; q < NX; ++q) {
-      const int grp = wave * NX + q;
-      load_unit_to_lds(xs, (int)(offx[q] - (grp & 1 ? xpast_odd : xpast_even)), dst + grp * 1024);
-    }
-#pragma unroll
-    for (int q = 0; q < NW; ++q) {
-      const int grp = wave * NW + q;
-      // second: half as many rows; in a longer ring the other loads are made all the same, so that every stage counts as many
-      if (AHEAD == 1 && second && grp * GROUP >= BN / 2) continue;
-      load_unit_to_lds(DUAL && !second && (grp & (32 / GROUP)) ? ws1 : ws0, off_of(offw[q], grp), dst + BM * 16 * UPS + grp * 1024);
+      auto x_off = [&](unsigned off, int grp) {
+        const int u = unit[grp & 1], to = u >= left ? left - 1 : u;
+        return KIND == kPlain && a.x_groups ? off - (unsigned)(((u >> 1) - (to >> 1)) * 1024 + ((u & 1) - (to & 1)) * 16) : w_off(off, grp);
+      };
+      load(x_off, w_off);
     }
     buf = buf + STAGE == RING * STAGE ? 0 : buf + STAGE;
     if (!none && ++lk == nk) lk = 0, lt += step;
