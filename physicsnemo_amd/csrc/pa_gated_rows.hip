@@ -121,11 +121,14 @@ struct Gate {
 template <int CT, int ACT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void rows_forward_kernel(RowsArgs a) {
   constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
+  constexpr bool ALONE = WAVES == 4;  // one wave per SIMD
+  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 3;
+  static_assert(!ALONE || NF % RING == 0, "a slot's fragments begin where the last one's end");
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int NCH = chunks_of(a.F), C = a.C;
-  float *bd = reinterpret_cast<float *>(smem + 2 * SU);  // b_down
+  float *bd = reinterpret_cast<float *>(smem + BUFFERS * SU);  // b_down
   for (int k = threadIdx.x; k < 32 * CT; k += 64 * WAVES) bd[k] = a.b_down && k < C ? a.b_down[k] : 0.f;
   __syncthreads();
   auto fetch = [&](int buf, int c) {  // this wave's share of slot c, 1 KB at a time
@@ -149,11 +152,35 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       if (32 * CT > C && col >= C) xb[ks] = u32x4{0u, 0u, 0u, 0u};
     }
   };
+  auto next_of = [](int b) { return b + 1 == BUFFERS ? 0 : b + 1; };
   int buf = 0;
+  u32x4 fr[RING];
+  f32x16 ga[2], ua[2];
+  auto biases = [&](int b, auto set_) {  // of the slot in buffer b, to accumulators SET
+    constexpr int set = decltype(set_)::value;
+    const float *bias = reinterpret_cast<const float *>(smem + b * SU + NF * 64);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
+      const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ua[set][4 * q + j] = bu[j], ga[set][4 * q + j] = bg[j];
+    }
+  };
+  auto begin = [&](int b, auto set_) {
+    static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = smem[b * SU + decltype(q)::value * 64 + lane]; });
+    biases(b, set_);
+  };
   fetch(0, 0);
+  if (ALONE) fetch(1, 1);
   load_rows(blockIdx.x);
+  if (ALONE) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    begin(0, std::integral_constant<int, 0>{});
+  }
   for (int64_t mb = blockIdx.x; mb < a.nblocks; mb += gridDim.x) {
-    f32x16 yacc[CT], ga[2], ua[2];
+    f32x16 yacc[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
@@ -166,20 +193,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     for (int r = 0; r < 16; ++r) ga[1][r] = ua[1][r] = 0.f;  // no chunk before the first: act(0) 0 = 0
     auto slot = [&](int c, auto set_) {
       constexpr int now = decltype(set_)::value, old = 1 - now;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the slot has landed
-      __syncthreads();                                  // everyone's, and the other buffer is free
-      const u32x4 *wb = smem + buf * SU + lane;
-      const float *bias = reinterpret_cast<const float *>(smem + buf * SU + NF * 64);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
-        const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ua[now][4 * q + j] = bu[j], ga[now][4 * q + j] = bg[j];
+      if constexpr (!ALONE) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the slot has landed
+        __syncthreads();                                  // everyone's, and the other buffer is free
+        begin(buf, set_);
       }
-      constexpr int AHEAD = 4, RING = AHEAD + 1;
-      u32x4 fr[RING], hop[2];
-      static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = wb[decltype(q)::value * 64]; });
+      const u32x4 *wb = smem + buf * SU + lane;
+      u32x4 hop[2];
       Gate<ACT> gate[4];
       float even = 0.f;
       auto tick = [&](auto t_) {  // pieces of values T, T - 1, T - 2, T - 3
@@ -202,6 +222,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       static_for<NF>([&](auto s_) {
         constexpr int S = decltype(s_)::value;
         if constexpr (S + AHEAD < NF) fr[(S + AHEAD) % RING] = wb[(S + AHEAD) * 64];
+        else if constexpr (ALONE) fr[(S + AHEAD) % RING] = smem[next_of(buf) * SU + (S + AHEAD - NF) * 64 + lane];
         if constexpr (S >= 2 * KS) {
           constexpr int t = S - 2 * KS;
           yacc[t % CT] = mma(fr[S % RING], hop[t / CT], yacc[t % CT]);
@@ -212,10 +233,16 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
         }
         __builtin_amdgcn_sched_barrier(0);
         behind(s_);
-        if constexpr (S == 1) fetch(buf ^ 1, c + 1);
+        if constexpr (!ALONE && S == 1) fetch(buf ^ 1, c + 1);
+        if constexpr (ALONE && S == MEET) {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's share of the next slot has landed
+          __syncthreads();                                  // everyone's, and the buffer of the slot before is free
+          fetch(next_of(next_of(buf)), c + 2 <= NCH ? c + 2 : c + 1 - NCH);
+        }
+        if constexpr (ALONE && S == NF - AHEAD) biases(next_of(buf), std::integral_constant<int, old>{});
         __builtin_amdgcn_sched_barrier(0);
       });
-      buf ^= 1;
+      buf = next_of(buf);
     };
 #pragma clang loop unroll(disable)
     for (int c = 0; c < NCH; c += 2) {
@@ -226,7 +253,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       const u32x4 *wb = smem + buf * SU + 2 * KS * 64 + lane;
-      fetch(buf ^ 1, 0);  // the first slot of the next block
+      if (ALONE) fetch(next_of(next_of(buf)), 1);
+      else fetch(buf ^ 1, 0);  // the first slot of the next block
       u32x4 hop[2];
       auto value = [&](int j) {
         Gate<ACT> v;
@@ -239,7 +267,8 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       for (int j = 0; j < 16; j += 2) hop[j / 8][j / 2 % 4] = pack2(value(j), value(j + 1));
 #pragma unroll
       for (int t = 0; t < 2 * CT; ++t) yacc[t % CT] = mma(wb[t * 64], hop[t / CT], yacc[t % CT]);
-      buf ^= 1;
+      buf = next_of(buf);
+      if (ALONE) begin(buf, std::integral_constant<int, 0>{});
     }
 
     const int64_t row0 = mb * ROWS + wave * 32;
@@ -387,6 +416,9 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     HiddenArgs a) {
   constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
   constexpr int STORES = 6 + 1;  // of a chunk
+  constexpr bool ALONE = WAVES == 4;
+  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 3;
+  static_assert(!ALONE || NF % RING == 0, "a slot's fragments begin where the last one's end");
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -413,15 +445,38 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       if (mb * ROWS + wave * 32 + i >= a.M) xb[ks] = db[ks] = u32x4{0u, 0u, 0u, 0u};  // a repeated row: of no gradient
     }
   };
+  auto next_of = [](int b) { return b + 1 == BUFFERS ? 0 : b + 1; };
   int buf = 0;
+  u32x4 fr[RING];
+  f32x16 ga[2], ua[2], da[2];
+  auto biases = [&](int b, auto set_) {
+    constexpr int set = decltype(set_)::value;
+    const float *bias = reinterpret_cast<const float *>(smem + b * SU + NF * 64);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
+      const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ua[set][4 * q + j] = bu[j], ga[set][4 * q + j] = bg[j], da[set][4 * q + j] = 0.f;
+    }
+  };
+  auto begin = [&](int b, auto set_) {
+    static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = smem[b * SU + decltype(q)::value * 64 + lane]; });
+    biases(b, set_);
+  };
   fetch(0, 0);
+  if (ALONE) fetch(1, 1);
   load_rows(blockIdx.x);
+  if (ALONE) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    begin(0, std::integral_constant<int, 0>{});
+  }
   for (int64_t mb = blockIdx.x; mb < a.nblocks; mb += gridDim.x) {
     const int64_t row0 = mb * ROWS + wave * 32;
     const int have = (int)(a.M - row0 < 32 ? (a.M > row0 ? a.M - row0 : 0) : 32);
     const Buffer out = __builtin_amdgcn_make_buffer_rsrc(a.dgu + row0 * 2 * a.Fp, 0, have > 0 ? 32 * 2 * a.Fp * 2 : 0, 0x00027000);
     const Buffer hidden = __builtin_amdgcn_make_buffer_rsrc(a.h + row0 * a.Fp, 0, have > 0 ? 32 * a.Fp * 2 : 0, 0x00027000);
-    f32x16 ga[2], ua[2], da[2];
 #pragma unroll
     for (int r = 0; r < 16; ++r) ga[1][r] = ua[1][r] = da[1][r] = 0.f;
     uint32_t packed[3][8];  // of a chunk: dg, du, h
@@ -465,21 +520,13 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
     auto slot = [&](int c, auto set_) {
       constexpr int now = decltype(set_)::value, old = 1 - now;
       // this wave's share of the slot has landed; the stores that left behind it stay in flight
-      if (c > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();  // everyone's, and the other buffer is free
-      const u32x4 *wb = smem + buf * SU + lane;
-      const float *bias = reinterpret_cast<const float *>(smem + buf * SU + NF * 64);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const tile::f32x4 bu = *reinterpret_cast<const tile::f32x4 *>(bias + 8 * q + 4 * g);
-        const tile::f32x4 bg = *reinterpret_cast<const tile::f32x4 *>(bias + 32 + 8 * q + 4 * g);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) ua[now][4 * q + j] = bu[j], ga[now][4 * q + j] = bg[j], da[now][4 * q + j] = 0.f;
+      if constexpr (!ALONE) {
+        if (c > 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // everyone's, and the other buffer is free
+        begin(buf, set_);
       }
-      constexpr int AHEAD = 4, RING = AHEAD + 1;
-      u32x4 fr[RING];
-      static_for<AHEAD>([&](auto q) { fr[decltype(q)::value] = wb[decltype(q)::value * 64]; });
+      const u32x4 *wb = smem + buf * SU + lane;
       Slope<ACT> v[5];
       float even[3];
       auto tick = [&](auto t_) {  // pieces of values T .. T - 4
@@ -505,16 +552,25 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
       static_for<NF>([&](auto s_) {
         constexpr int S = decltype(s_)::value;
         if constexpr (S + AHEAD < NF) fr[(S + AHEAD) % RING] = wb[(S + AHEAD) * 64];
+        else if constexpr (ALONE) fr[(S + AHEAD) % RING] = smem[next_of(buf) * SU + (S + AHEAD - NF) * 64 + lane];
         if constexpr (S % 3 == 0) ua[now] = mma(fr[S % RING], xb[S / 3], ua[now]);
         else if constexpr (S % 3 == 1) ga[now] = mma(fr[S % RING], xb[S / 3], ga[now]);
         else da[now] = mma(fr[S % RING], db[S / 3], da[now]);
         __builtin_amdgcn_sched_barrier(0);
         ticks_behind<S, CT>(tick);
-        if constexpr (S == 1) fetch(buf ^ 1, c + 1 < NCH ? c + 1 : 0);  // past the last slot: the first of the next block
+        if constexpr (!ALONE && S == 1) fetch(buf ^ 1, c + 1 < NCH ? c + 1 : 0);  // past the last slot: the first of the next block
+        if constexpr (ALONE && S == MEET) {
+          // this wave's share of the next slot has landed; no stores came behind it in slot 0
+          if (c == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STORES) : "memory");
+          __syncthreads();  // everyone's, and the buffer of the slot before is free
+          fetch(next_of(next_of(buf)), c + 2 < NCH ? c + 2 : c + 2 - NCH);
+        }
+        if constexpr (ALONE && S == NF - AHEAD) biases(next_of(buf), std::integral_constant<int, old>{});
         __builtin_amdgcn_sched_barrier(0);
       });
       if (now == 1 || c > 0) store_sums(c - 1), store_chunk(c - 1);
-      buf ^= 1;
+      buf = next_of(buf);
     };
 #pragma clang loop unroll(disable)
     for (int c = 0; c < NCH; c += 2) {
@@ -573,7 +629,7 @@ int64_t rows_blob_bytes(int64_t C, int64_t F) { return (int64_t)(chunks_of((int)
 
 template <int CT, int ACT, int WAVES>
 static int launch_rows(const RowsArgs &a, int num_cu, hipStream_t st) {
-  constexpr size_t lds = 2 * (6 * CT + 1) * 1024 + 32 * CT * 4;
+  constexpr size_t lds = (WAVES == 4 ? 3 : 2) * (6 * CT + 1) * 1024 + 32 * CT * 4;
   auto kernel = rows_forward_kernel<CT, ACT, WAVES>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   const int64_t grid = a.nblocks < num_cu ? a.nblocks : num_cu;
@@ -620,7 +676,7 @@ int64_t hidden_blob_bytes(int64_t C, int64_t F) { return (int64_t)chunks_of((int
 
 template <int CT, int ACT, int WAVES>
 static int launch_hidden(const HiddenArgs &a, int num_cu, hipStream_t st) {
-  constexpr size_t lds = 2 * (6 * CT + 1) * 1024;
+  constexpr size_t lds = (WAVES == 4 ? 3 : 2) * (6 * CT + 1) * 1024;
   auto kernel = rows_hidden_backward_kernel<CT, ACT, WAVES>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   const int64_t grid = a.nblocks < num_cu ? a.nblocks : num_cu;
