@@ -75,8 +75,11 @@ struct RowsArgs {
 //   u(c)^T = W_up[chunk c] x^T + b_up and g(c)^T = W_gate[chunk c] x^T + b_gate, in turn          4 CT MFMAs
 //     with h(c - 1) = act(g) u of the chunk before formed behind them, 16 values in 32 pieces; two sets of accumulators take turns
 //   y^T += W_down[:, chunk c - 1] h(c - 1)^T                                                      2 CT MFMAs
-// Two LDS buffers, one barrier per slot.  CT = 8: one wave per SIMD with 512 registers (y 128, x 64, two sets of g and u 64);
-// narrower rows: two.
+// CT = 8: one wave per SIMD with 512 registers (y 128, x 64, two sets of g and u 64); narrower rows: two.  One barrier per slot:
+// two waves per SIMD meet at its beginning and cover each other (two LDS buffers); a wave alone has the next slot's data a
+// slot earlier (three) and its first fragments and biases in registers, and meets the others behind its first products
+// (262 144 x 256, F = 1 024: 549 -> 517 us; meeting behind step 10 of 48 530; with two waves per SIMD the registers that this takes cost more than it gives,
+// 262 144 x 128, F = 512, backward 197 -> 245).
 // ---------------------------------------------------------------------------------------------------------------
 // Twenty ticks of vector work spread evenly behind the first 5 CT matrix instructions of a slot: those behind step S.
 template <int S, int CT, class F>
@@ -122,7 +125,7 @@ template <int CT, int ACT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) void rows_forward_kernel(RowsArgs a) {
   constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
   constexpr bool ALONE = WAVES == 4;  // one wave per SIMD
-  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 3;
+  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 1;
   static_assert(!ALONE || NF % RING == 0, "a slot's fragments begin where the last one's end");
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
@@ -407,8 +410,9 @@ struct Slope {
 // rows_hidden_backward_kernel<CT>: the hidden layer of the backward pass for rows of up to 32 CT channels.  Per slot c a wave runs
 //   u(c)^T = W_up[chunk c] x^T + b_up, g(c)^T = W_gate[chunk c] x^T + b_gate, d(c)^T = W_down[:, chunk c]^T dy^T     6 CT MFMAs
 // in turn, with h, dg and du of the chunk before formed behind them, 16 values in five pieces each; two sets of accumulators take
-// turns.  A chunk's results leave 2 KB in one piece each (pa_tile.h); the column sums of dg
-// and du, for the bias gradients, are formed before their rounding.  Bound by HBM, 4 C + 6 F bytes per row.
+// turns.  A chunk's results leave 2 KB in one piece each (pa_tile.h); the column sums of dg and du, for the bias gradients, are
+// formed before their rounding.  Buffers and barriers as in rows_forward_kernel.  131 072 x 256, F = 1 024: 362 us for 940 MB and 206
+// GFLOP; vector instructions 37 %, matrix pipes 26 % of the time, waits 28 %.
 // ---------------------------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int value_at(int t) { return t / 2 % 4 * 4 + t / 8 * 2 + t % 2; }
 template <int CT, int ACT, int WAVES>
@@ -417,7 +421,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
   constexpr int KS = 2 * CT, SU = (6 * CT + 1) * 64, NF = 6 * CT, ROWS = 32 * WAVES;
   constexpr int STORES = 6 + 1;  // of a chunk
   constexpr bool ALONE = WAVES == 4;
-  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 3;
+  constexpr int BUFFERS = ALONE ? 3 : 2, AHEAD = 4, RING = ALONE ? 6 : AHEAD + 1, MEET = 1;
   static_assert(!ALONE || NF % RING == 0, "a slot's fragments begin where the last one's end");
   extern __shared__ u32x4 smem[];
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5;
