@@ -386,3 +386,27 @@ def test_running_again_inside_a_backward_pass_is_refused():
     y = torch.utils.checkpoint.checkpoint(block, x, use_reentrant=False)
     with pytest.raises(RuntimeError, match="another mask"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("C,rows,tail", [(512, 4_300_000, 300_000), (256, 275 * 32_768, 32_768)])
+def test_elements_past_32_bits(C, rows, tail):
+    """The last rows of a call of more than 2^31 elements are those of a call of their own (of so many rows that the same kernels
+    take them: every element is summed in the same order)."""
+    announce("elements past 32 bits", C, rows)
+    torch.manual_seed(10)
+    F, dtype = 64, torch.bfloat16
+    params = [torch.randn(F, C, device=DEV).to(dtype) / 16, torch.randn(F, device=DEV), torch.randn(F, C, device=DEV).to(dtype) / 16,
+              torch.randn(F, device=DEV), torch.randn(C, F, device=DEV).to(dtype) / 8, torch.randn(C, device=DEV)]
+    x = torch.empty(rows, C, device=DEV, dtype=dtype).normal_()
+    last = x[-tail:].clone()
+    y = PF.gated_mlp_forward(x, *params, residual=x)[-tail:].clone()
+    assert torch.equal(y, PF.gated_mlp_forward(last, *params, residual=last))
+    dx = PF.gated_mlp_backward(x, x, *params[:5], wanted=(True,) + (False,) * 6)[0][-tail:].clone()
+    assert torch.equal(dx, PF.gated_mlp_backward(last, last, *params[:5], wanted=(True,) + (False,) * 6)[0])
+    q = [t for k in (0, 2, 4) for t in (*PF.quantize_int8(params[k]), params[k + 1])]
+    y = PF.gated_mlp_int8(x, *q, residual=x)[-tail:].clone()
+    assert torch.equal(y, PF.gated_mlp_int8(last, *q, residual=last))
+    del y, dx
+    gamma, rng = torch.ones(C, device=DEV), torch.tensor([1, 2], device=DEV)
+    _, n = PF.dropout_add_norm(x, x, 0.0, rng, gamma, gamma)
+    assert torch.equal(n[-tail:], PF.dropout_add_norm(last, last, 0.0, rng, gamma, gamma)[1])
