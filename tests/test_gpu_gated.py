@@ -77,7 +77,8 @@ def check(got, want, tol, what):
 
 
 SIZES = [(1, 1, 1), (1, 8, 8), (3, 7, 5), (2, 33, 65), (31, 64, 128), (33, 32, 96), (64, 96, 130), (127, 128, 512), (129, 200, 533),
-         (300, 256, 1024), (257, 257, 100), (65, 512, 1365), (1000, 64, 170), (5, 1024, 40), (700, 24, 2050)]
+         (300, 256, 1024), (257, 257, 100), (65, 512, 1365), (1000, 64, 170), (5, 1024, 40), (700, 24, 2050),
+         (2500, 200, 533), (4000, 96, 260), (3001, 257, 130), (9000, 40, 72)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -80,7 +80,8 @@ def check(got, want, tol, what):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows,K,N", [(1, 1, 1), (1, 16, 8), (2, 17, 3), (31, 64, 33), (33, 100, 130), (64, 256, 1024), (130, 512, 512),
-                                      (257, 130, 96), (70, 2048, 64), (5, 33000, 20), (1000, 32, 250)])
+                                      (257, 130, 96), (70, 2048, 64), (5, 33000, 20), (1000, 32, 250), (3001, 100, 700), (9000, 40, 33),
+                                      (2500, 320, 257)])
 def test_linear(rows, K, N, dtype):
     announce("linear_int8", rows, K, N, dtype)
     gen = torch.Generator().manual_seed(rows)
