@@ -412,7 +412,7 @@ struct Slope {
 // in turn, with h, dg and du of the chunk before formed behind them, 16 values in five pieces each; two sets of accumulators take
 // turns.  A chunk's results leave 2 KB in one piece each (pa_tile.h); the column sums of dg and du, for the bias gradients, are
 // formed before their rounding.  Buffers and barriers as in rows_forward_kernel.  131 072 x 256, F = 1 024: 362 us for 940 MB and 206
-// GFLOP; vector instructions 37 %, matrix pipes 26 % of the time, waits 28 %.
+// GFLOP; vector instructions 38 %, matrix pipes 28 % of the time, waits 21 %.
 // ---------------------------------------------------------------------------------------------------------------
 __host__ __device__ constexpr int value_at(int t) { return t / 2 % 4 * 4 + t / 8 * 2 + t % 2; }
 template <int CT, int ACT, int WAVES>
