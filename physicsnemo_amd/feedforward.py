@@ -52,17 +52,10 @@ class GatedMlp(nn.Module):
         return [p for lin in self.linears() for p in (lin.weight, lin.bias)]
 
     def _kernel_params(self, dtype: torch.dtype, device: torch.device):
-        """The six parameters for the kernels (weights in `dtype`, biases in float32), cached until one changes."""
-        params = self.parameters_in_order()
-        stamp = (dtype, device) + tuple(None if p is None else (p.data_ptr(), p._version, p.dtype) for p in params)
-        cache = self.__dict__.setdefault("_kernel_cache", {})
-        if cache.get("stamp") != stamp:
-            with torch.no_grad():
-                cache["params"] = [None if p is None else
-                                   p.detach().to(device=device, dtype=dtype if p.ndim == 2 else torch.float32).contiguous().clone()
-                                   for p in params]
-            cache["stamp"] = stamp
-        return cache["params"]
+        """The six parameters for the kernels, weights in `dtype` and biases in float32: themselves where they are that, else
+        cast for this call.  Nothing is kept: writes through `.data` would leave what is kept behind, unseen."""
+        return [None if p is None else p.to(device=device, dtype=dtype if p.ndim == 2 else torch.float32).contiguous()
+                for p in self.parameters_in_order()]
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         dtype = PA.compute_dtype(x)
