@@ -137,10 +137,24 @@ def counter_dropout(attn: nn.Module) -> CounterDropout | None:
 
 
 class Int8Mlp:
-    """8-bit weights of a block's Mlp or GatedMlp, made once per parameter set, and the MLP on them."""
+    """8-bit weights of a block's Mlp or GatedMlp, made once per parameter set, and the MLP on them.
+
+    A set is told by its parameters' addresses, versions and types, and holds the parameters, so that no address comes twice.  A
+    write through `.data` changes none of the three: `refresh` after it.  The codes are complete before the call that makes
+    them returns, for streams and captures that use them later; a set that a capture meets unmade is made in the graph, on
+    every replay, and not kept; one that a graph reads stays allocated (`of_graphs`).  Copies start without codes."""
 
     def __init__(self):
-        self._stamp = self._weights = None
+        self.of_graphs: list = []  # codes that a captured graph reads
+        self._stamp = self._weights = self._held = None
+        self._streams: set = set()
+
+    def __reduce__(self):
+        return Int8Mlp, ()
+
+    def refresh(self):
+        """Round the weights again on the next call."""
+        self._stamp = None
 
     @staticmethod
     def linears(mlp: nn.Module):
@@ -157,15 +171,31 @@ class Int8Mlp:
         return lins, act
 
     def _of(self, lins, device):
+        with PF._on(device):
+            return self._of_current_device(lins, device)
+
+    def _of_current_device(self, lins, device):
         params = [p for lin in lins for p in (lin.weight, lin.bias)]
         stamp = (device,) + tuple(None if p is None else (p.data_ptr(), p._version, p.dtype) for p in params)
+        stream, capturing = torch.cuda.current_stream(device), torch.cuda.is_current_stream_capturing()
         if self._stamp != stamp:
             with torch.no_grad():
-                self._weights = [
+                weights = [
                     (*PF.quantize_int8(lin.weight.detach().to(device=device, dtype=torch.float32).contiguous()),
                      None if lin.bias is None else lin.bias.detach().to(device=device, dtype=torch.float32).contiguous().clone())
                     for lin in lins]
+            if capturing:
+                return weights
+            stream.synchronize()
+            self._weights, self._held, self._streams = weights, [None if p is None else p.detach() for p in params], {stream}
             self._stamp = stamp
+        elif capturing:
+            if not any(w is self._weights for w in self.of_graphs):
+                self.of_graphs.append(self._weights)
+        elif stream not in self._streams:  # the codes' memory is not reused before this stream's work on them is done
+            for t in (t for w in self._weights for t in w if t is not None):
+                t.record_stream(stream)
+            self._streams.add(stream)
         return self._weights
 
     def __call__(self, mlp: nn.Module, x: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor | None:

@@ -166,12 +166,18 @@ class TransolverBlock(nn.Module):
     def use_int8_mlp(self, enabled: bool = True):
         """Inference with the MLP's products in 8 bits: weights rounded to int8 with one scale per output channel, once per
         parameter set, and the rows on their way in with one scale each (`functional.linear_int8`, `gated_mlp_int8`); bfloat16
-        and float32 rows on the GPU.  Training runs as without it.  No counterpart in the reference."""
+        and float32 rows on the GPU.  Training runs as without it.  Called again it rounds the weights again, which a write
+        through `.data` asks for; other writes are noticed.  No counterpart in the reference."""
         if enabled and self.fp8_weights:
             raise ValueError("the block's MLP holds fp8 weights; use_fp8_weights(False) first")
         if enabled and Int8Mlp.linears(self.ln_mlp1[1]) is None:
             raise ValueError("the block's MLP is not Linear, activation, Linear or a GatedMlp, without hooks")
-        self.int8_mlp = Int8Mlp() if enabled else None
+        if enabled and self.int8_mlp is not None:
+            self.int8_mlp.refresh()
+        else:
+            if self.int8_mlp is not None:
+                self._int8_of_graphs = getattr(self, "_int8_of_graphs", []) + self.int8_mlp.of_graphs
+            self.int8_mlp = Int8Mlp() if enabled else None
         return self
 
     def use_counter_dropout(self, seed: int, offset: int = 0):
