@@ -159,11 +159,15 @@ class Int8Mlp:
     @staticmethod
     def linears(mlp: nn.Module):
         """(Linears, activation's name) of an MLP that runs in 8 bits, or None: hooks, replaced modules, other activations."""
+        from .transolver import Mlp  # which imports this file
+
         if type(mlp) is GatedMlp:
             lins, act, modules = mlp.linears(), mlp.act, (mlp,)
         else:
-            layers = getattr(mlp, "layers", None)
-            if layers is None or len(layers) != 3 or type(layers[1]) not in _NAMES or getattr(layers[1], "approximate", "none") != "none":
+            if type(mlp) is not Mlp:
+                return None
+            layers = mlp.layers
+            if len(layers) != 3 or type(layers[1]) not in _NAMES or getattr(layers[1], "approximate", "none") != "none":
                 return None
             lins, act, modules = (layers[0], layers[2]), _NAMES[type(layers[1])], (mlp, layers, layers[1])
         if not (all(type(lin) is nn.Linear for lin in lins) and PA.unhooked(*modules, *lins)):

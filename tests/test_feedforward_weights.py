@@ -130,3 +130,28 @@ def test_blocks_keep_what_graphs_read_and_copies_make_their_own(on_cpu):
     again = pickle.loads(pickle.dumps(codes))
     assert twin.int8_mlp is not codes and not twin.int8_mlp.of_graphs and not again.of_graphs
     assert block.use_int8_mlp(False).int8_mlp is None and block._int8_of_graphs[0] is kept
+
+
+class Halved(pn.Mlp):
+    def forward(self, x):
+        return super().forward(x) / 2
+
+
+class Skipping(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.layers = torch.nn.ModuleList([torch.nn.Linear(32, 64), torch.nn.GELU(), torch.nn.Linear(64, 32)])
+
+    def forward(self, x):
+        return x + self.layers[2](self.layers[1](self.layers[0](x)))
+
+
+@pytest.mark.parametrize("replaced", [Halved(32, 64, 32), Skipping(), torch.nn.Sequential(torch.nn.Linear(32, 32))])
+def test_only_the_blocks_own_mlps_run_in_8_bits(replaced):
+    """A module that computes something else from three layers keeps its own forward."""
+    assert Int8Mlp.linears(replaced) is None
+    block = pn.TransolverBlock(4, 32, 0.0, use_te=False)
+    assert Int8Mlp.linears(block.ln_mlp1[1])[1] == "gelu"
+    block.ln_mlp1[1] = replaced
+    with pytest.raises(ValueError, match="not Linear, activation, Linear"):
+        block.use_int8_mlp()
