@@ -78,8 +78,8 @@ class CounterDropout(nn.Dropout):
     stored, the backward pass forms it again, and every call takes the next offset, in a captured graph every replay.
 
     `state` is the int64 pair (seed, next offset); masks come again after 2^32 calls.  It is no entry of the state dict; to go on after a restart with the masks
-    that would have come next, save it and set it again.  Processes that train together take different seeds.  Calls of one
-    module run on one stream at a time.  A backward pass that runs the module again (activation checkpointing) would draw
+    that would have come next, save it and set it again.  It moves to the input's device with the first call, which a capture
+    refuses.  Processes that train together take different seeds.  Calls of one module run on one stream at a time.  A backward pass that runs the module again (activation checkpointing) would draw
     another mask and is refused."""
 
     def __init__(self, p: float = 0.5, seed: int = 0, offset: int = 0):
@@ -100,6 +100,9 @@ class CounterDropout(nn.Dropout):
         if torch._C._current_graph_task_id() != -1:
             raise RuntimeError("CounterDropout ran again inside a backward pass, where it would draw another mask")
         if self.state.device != x.device:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"CounterDropout's state is on {self.state.device}: run the module once on {x.device}, or move "
+                                   "its state there, before the capture")
             self.state = self.state.to(x.device)
         return PF.dropout_advance(self.state)
 

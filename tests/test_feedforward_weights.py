@@ -155,3 +155,13 @@ def test_only_the_blocks_own_mlps_run_in_8_bits(replaced):
     block.ln_mlp1[1] = replaced
     with pytest.raises(ValueError, match="not Linear, activation, Linear"):
         block.use_int8_mlp()
+
+
+def test_counters_do_not_move_inside_a_capture(monkeypatch):
+    """The copy to the GPU belongs before the capture: in it the state would be a copy of the graph, set back by every replay."""
+    rows = type("Rows", (), {"is_cuda": True, "device": torch.device("cuda", 0)})()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    drop = pn.CounterDropout(0.5, seed=3)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        drop._next(rows)
+    assert drop.state.tolist() == [3, 0]
