@@ -107,11 +107,11 @@ struct Gate {
   }
   __device__ __forceinline__ void piece2() {
     if constexpr (ACT == tile::kSilu) t = __builtin_amdgcn_rcpf(1.f + t);
-    else if constexpr (ACT == tile::kGelu) x = fmaxf(x, 0.f);
+    else if constexpr (ACT == tile::kGelu) x = gelu_from_tail(x, q);
   }
   __device__ __forceinline__ float piece3(float up, int act) const {
     if constexpr (ACT == tile::kSilu) return x * t * up;
-    else if constexpr (ACT == tile::kGelu) return fmaf(-t, q, x) * up;
+    else if constexpr (ACT == tile::kGelu) return x * up;
     switch (act) {
       case tile::kRelu: return (x < 0.f ? 0.f : x) * up;
       case tile::kSigmoid: return tile::sigmoid(x) * up;
@@ -359,15 +359,15 @@ struct Slope {
     if constexpr (ACT == tile::kSilu) {
       t = -kLog2e * v;
     } else if constexpr (ACT == tile::kGelu) {
-      a = gelu_tail_arg(v);
-      s = gelu_lower_tail_upper_terms(a);
+      a = fabsf(v);
+      s = gelu_short_upper_terms(a);
     }
   }
   __device__ __forceinline__ void piece1() {
     if constexpr (ACT == tile::kSilu) {
       t = __builtin_amdgcn_exp2f(t);
     } else if constexpr (ACT == tile::kGelu) {
-      s = gelu_lower_tail_lower_terms(a, s);
+      s = gelu_short_lower_terms(a, s);
       t = a * a * (-0.5f * kLog2e);
     }
   }
@@ -384,9 +384,8 @@ struct Slope {
       a = x * s;
       t = 1.f - s;
     } else if constexpr (ACT == tile::kGelu) {
-      const float phi = x > 0.f ? 1.f - s : s;
-      a = fmaf(-a, s, fmaxf(x, 0.f));
-      s = phi;
+      a = gelu_from_tail(x, s);
+      s = gelu_slope_from_tail(x, s, t);
     } else {
       switch (act) {
         case tile::kRelu: a = x < 0.f ? 0.f : x, s = x > 0.f ? 1.f : 0.f; break;
@@ -399,7 +398,6 @@ struct Slope {
   __device__ __forceinline__ void piece4(float up, float d, float &h, float &dg, float &du) const {
     float slope = s;
     if constexpr (ACT == tile::kSilu) slope = fmaf(a, t, s);
-    else if constexpr (ACT == tile::kGelu) slope = fmaf(x * 0.3989422804014327f, t, s);
     h = a * up;
     dg = d * up * slope;
     du = d * a;

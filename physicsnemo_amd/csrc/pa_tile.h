@@ -84,7 +84,7 @@ __device__ __forceinline__ void act_values(int act, V &v) {
   switch (act) {
     case kGelu:
 #pragma unroll
-      for (int r = 0; r < N; ++r) v[r] = SHORT ? gelu_short(v[r]) : gelu_tail(v[r]);
+      for (int r = 0; r < N; ++r) v[r] = SHORT ? gelu_short(v[r]) : gelu_full(v[r]);
       break;
     case kRelu:  // NaN passes, as torch's does
 #pragma unroll
@@ -107,13 +107,14 @@ __device__ __forceinline__ void act_values(int act, V &v) {
 }
 
 // v <- act(v), slope <- act'(v)
+template <bool SHORT>
 __device__ __forceinline__ void act_slopes(int act, f32x16 &v, f32x16 &slope) {
   switch (act) {
     case kGelu:
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         float d;
-        v[r] = gelu_tail_slope(v[r], d);
+        v[r] = SHORT ? gelu_short_slope(v[r], d) : gelu_full_slope(v[r], d);
         slope[r] = d;
       }
       break;
@@ -784,7 +785,7 @@ __global__ __launch_bounds__(64 * CFG::WAVES, CFG::OCC) void rows_tile_kernel(Ar
           } else {
             const Buffer hidden = rows_or_blocks_at(a.out2, a.ldh);
             f32x16 slope, d = acc2[m][n];
-            act_slopes(a.act, gate, slope);
+            act_slopes<sizeof(TO) == 2>(a.act, gate, slope);
             f32x16 h;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
