@@ -1894,7 +1894,7 @@ static int check_gated(int dtype, int64_t rows, int64_t C, int64_t F) {
 
 int64_t pa_gated_mlp_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F) {
   if (int rc = check_gated(dtype, rows, C, F)) return rc;
-  return pa::gated::forward_workspace_bytes(dtype, rows, C, F);
+  return pa::gated::forward_workspace_bytes(dtype, rows, C, F, compute_units());
 }
 
 int pa_gated_mlp_forward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,

@@ -197,52 +197,70 @@ static int product(const Args &a, int num_cu, hipStream_t st) {
   return tile::launch<E, TO, KIND>(a, num_cu, st);
 }
 
-// The forward's workspace: h, and padded copies of what is not laid out in whole units.  The plan depends on the pointers'
-// alignment; the query answers for the worst case.
+// The forward's workspace: packed weights of the kernel that keeps the hidden layer on chip, h of the rows that the tile kernels
+// take, and padded copies of what is not laid out in whole units.  The query does not know the pointers.  Rows whose width is
+// whole units are off a boundary only as views are, and then run in pieces of kLooseRows rows, so that no call has to bring
+// room for copies of all rows, or for the hidden layer of rows that have it on chip.  (262 144 x 256, F = 1 024, bf16: 87 MB instead of
+// 674; of rows off a boundary a piece costs two or three launches.)
+static constexpr int64_t kLooseRows = 32768;
+
 template <class E, class TO>
 static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *residual, void *y,
                    char *workspace, int64_t *bytes, int num_cu, hipStream_t st) {
-  constexpr int64_t e = E::kBytes, U = 16 / e;
-  const bool plan = bytes != nullptr;
+  constexpr int64_t e = E::kBytes;
+  const bool plan = bytes != nullptr, whole = C * e % 16 == 0, on_chip = e == 2 && whole && rows_supported(C, F);
+  const bool loose = whole && !plan && !(aligned16(x) && aligned16(y) && aligned16(residual));
+  const bool copy_x = plan ? !whole : !whole_rows(x, C, e);
   Space ws{workspace};
   Layout lay;
-  const int64_t Fp = up(F, 32 / e);  // the hidden layer's columns: whole 32-byte groups
-  auto copied = [&](const void *q, int64_t width) { return plan || !whole_rows(q, width, e); };
-  int64_t done = 0;  // rows of the kernel that keeps the hidden layer on chip
-  if (e == 2 && C % 8 == 0 && rows_supported(C, F)) {
-    void *blob = ws.take(rows_blob_bytes(C, F));
-    if (!plan && aligned16(x) && aligned16(y) && aligned16(residual)) done = rows_worth(M, C, num_cu);
-    if (done > 0) {
-      int rc = rows_pack(C, F, p, blob, st);
-      if (!rc) rc = rows_forward(done, C, F, blob, p.b_down, act, x, residual, y, num_cu, st);
-      if (rc || done == M) return rc;
-    }
+  const int64_t Fp = up(F, 32 / e), Cp = up(C, 16 / e);  // the hidden layer's columns: whole 32-byte groups
+  void *blob = on_chip ? ws.take(rows_blob_bytes(C, F)) : nullptr;
+  const int64_t done = on_chip && !loose ? rows_worth(M, C, num_cu) : 0;
+  if (done > 0 && !plan) {
+    int rc = rows_pack(C, F, p, blob, st);
+    if (!rc) rc = rows_forward(done, C, F, blob, p.b_down, act, x, residual, y, num_cu, st);
+    if (rc || done == M) return rc;
   }
-  auto behind = [&](const void *q) { return q ? static_cast<const char *>(q) + done * C * e : nullptr; };
-  x = behind(x), residual = behind(residual), y = const_cast<char *>(behind(y));
-  M -= done;
-  void *h = ws.take(up(M, tile::kGroupRows) * Fp * e);
-  const Rows xr = rows_of(x, M, C, e, copied(x, C), ws, &lay);
-  const Rows wg = rows_of(p.w_gate, F, C, e, copied(p.w_gate, C), ws, &lay);
-  const Rows wu = rows_of(p.w_up, F, C, e, copied(p.w_up, C), ws, &lay);
-  const Rows wd = rows_of(p.w_down, C, F, e, copied(p.w_down, F), ws, &lay);
+  auto room = [&](Space &s, int64_t rows, bool copies, void *&h, void *&copy) {
+    h = s.take(up(rows, tile::kGroupRows) * Fp * e);
+    copy = copies ? s.take(rows * Cp * e) : nullptr;
+  };
+  const int64_t piece = M < kLooseRows ? M : kLooseRows, per = loose && (on_chip || copy_x) ? piece : M - done;
+  void *h, *copy;
+  if (plan) {
+    Space pieces = ws;
+    room(ws, per, copy_x, h, copy);
+    if (whole) room(pieces, piece, true, h, copy);
+    if (pieces.used > ws.used) ws.used = pieces.used;
+  } else {
+    room(ws, per, copy_x, h, copy);
+  }
+  auto weight = [&](const void *w, int64_t rows, int64_t width) { return rows_of(w, rows, width, e, plan || !whole_rows(w, width, e), ws, &lay); };
+  const Rows wg = weight(p.w_gate, F, C), wu = weight(p.w_up, F, C), wd = weight(p.w_down, C, F);
   if (plan) return *bytes = ws.used, PA_OK;
-  if (int rc = tile::lay_out(lay, e, st)) return rc;
-  Args a{};
-  a.X = xr.p, a.ldx = xr.ld, a.units = xr.units;
-  a.W[0] = wg.p, a.W[1] = wu.p, a.ldw = wg.ld;
-  a.M = M, a.N = (int)F, a.limit = (int)Fp;
-  a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
-  a.out = h, a.ldo = Fp, a.act = act;
-  if (int rc = product<E, TO, tile::kGated>(a, num_cu, st)) return rc;
-  Args d{};
-  d.X = h, d.ldx = Fp * e, d.units = wd.units, d.x_groups = tile::kGrouped<TO>;
-  d.W[0] = wd.p, d.ldw = wd.ld;
-  d.M = M, d.N = d.limit = (int)C;
-  d.bias[0] = p.b_down;
-  d.residual = residual, d.out = y, d.ldo = C;
-  d.vec = whole_rows(y, C, e) && (!residual || aligned16(residual));
-  return product<E, TO, tile::kPlain>(d, num_cu, st);
+  for (int64_t r0 = done; r0 < M; r0 += per) {
+    const int64_t rows = M - r0 < per ? M - r0 : per;
+    auto from = [&](const void *q) { return q ? static_cast<const char *>(q) + r0 * C * e : nullptr; };
+    if (copy_x) lay.add(from(x), C, copy, rows, C, Cp, Cp, false);
+    if (int rc = tile::lay_out(lay, e, st)) return rc;
+    lay = Layout{};  // the weights with the first piece
+    Args a{};
+    a.X = copy_x ? copy : from(x), a.ldx = Cp * e, a.units = (int)(Cp * e / 16);
+    a.W[0] = wg.p, a.W[1] = wu.p, a.ldw = wg.ld;
+    a.M = rows, a.N = (int)F, a.limit = (int)Fp;
+    a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+    a.out = h, a.ldo = Fp, a.act = act;
+    if (int rc = product<E, TO, tile::kGated>(a, num_cu, st)) return rc;
+    Args d{};
+    d.X = h, d.ldx = Fp * e, d.units = wd.units, d.x_groups = tile::kGrouped<TO>;
+    d.W[0] = wd.p, d.ldw = wd.ld;
+    d.M = rows, d.N = d.limit = (int)C;
+    d.bias[0] = p.b_down;
+    d.residual = from(residual), d.out = const_cast<char *>(from(y)), d.ldo = C;
+    d.vec = whole_rows(d.out, C, e) && (!residual || aligned16(d.residual));
+    if (int rc = product<E, TO, tile::kPlain>(d, num_cu, st)) return rc;
+  }
+  return PA_OK;
 }
 
 static constexpr int64_t kMaxWidth = 1 << 18;  // 256 rows of two hidden layers of it stay below 2^31 bytes
@@ -252,11 +270,11 @@ bool supported(int dtype, int64_t M, int64_t C, int64_t F) {
          M <= ((int64_t)1 << 60) / (16 * (C > F ? C : F));
 }
 
-int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F) {
+int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu) {
   int64_t bytes = 0;
   const pa_gated_params p{};
-  if (dtype == PA_F32) forward<tile::F32, float>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
-  else forward<tile::Bf16, bf16>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, 0, nullptr);
+  if (dtype == PA_F32) forward<tile::F32, float>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, num_cu, nullptr);
+  else forward<tile::Bf16, bf16>(M, C, F, p, 0, nullptr, nullptr, nullptr, nullptr, &bytes, num_cu, nullptr);
   return bytes;
 }
 

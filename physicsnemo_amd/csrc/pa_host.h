@@ -165,7 +165,7 @@ int backward(const pa_shape &s, const void *x, const void *dy, const void *saved
 namespace gated {
 // gated feed-forward block: see pa_gated_mlp_forward / _backward
 bool supported(int dtype, int64_t M, int64_t C, int64_t F);
-int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F);
+int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu);
 int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu);
 int forward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p, int act, const void *x, const void *residual, void *y,
             void *workspace, int num_cu, hipStream_t st);
