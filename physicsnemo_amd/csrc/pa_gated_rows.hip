@@ -608,8 +608,7 @@ __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVE
 // ================================================================================================
 // host side
 // ================================================================================================
-// tiles of 32 channels; five and six of them, rare widths, run as seven
-static int channel_tiles(int64_t C) { const int t = (int)((C + 31) / 32); return t == 5 || t == 6 ? 7 : t; }
+static int channel_tiles(int64_t C) { return (int)((C + 31) / 32); }
 static int waves_of(int64_t C) { return C <= 128 ? 8 : 4; }
 
 bool rows_supported(int64_t C, int64_t F) { return C <= 256 && F <= 1 << 18; }
@@ -618,10 +617,12 @@ bool rows_supported(int64_t C, int64_t F) { return C <= 256 && F <= 1 << 18; }
 // tile kernels then have the smaller pieces.  Wide rows take long for a block, so that they need most of a round; rows of up to 64
 // channels are worth it always.  Forward, rows + 4 us for the weights / tiles (us): C = 256, F = 1024: 16 384 rows 59 / 45,
 // 32 768 71 / 78, 262 144 474 / 582; C = 200, F = 800: 32 768 43 / 60; C = 128, F = 512: 16 384 28 / 21, 32 768 28 / 34, 262 144
-// 124 / 225; C = 64, F = 256: 2 000 13 / 19, 32 768 13 / 20.  Rows past the whole rounds go to the tile kernels where they are less
+// 124 / 225; C = 64, F = 256: 2 000 13 / 19, 32 768 13 / 20.  Forward and the hidden layer's backward together: C = 160, F = 640:
+// 20 480 rows 104 / 101, 24 576 108 / 113; C = 192, F = 768: 20 480 125 / 117, 24 576 132 / 132, 28 672 139 / 152.  (Run as seven
+// tiles, 262 144 rows of these two widths take 225 and 272 forward instead of 181 and 244.)  Rows past the whole rounds go to the tile kernels where they are less
 // than half a round.
 int64_t rows_worth(int64_t M, int64_t C, int num_cu) {
-  static const int least[9] = {0, 0, 0, 25, 45, 0, 0, 75, 85};  // per cent of a round, by channel tiles
+  static const int least[9] = {0, 0, 0, 25, 45, 65, 75, 75, 85};  // per cent of a round, by channel tiles
   const int64_t block = 32 * waves_of(C), blocks = (M + block - 1) / block, rounds = blocks / num_cu, over = blocks - rounds * num_cu;
   if (rounds == 0 ? 100 * over >= least[channel_tiles(C)] * num_cu : 2 * over >= num_cu) return M;
   const int64_t rows = rounds * num_cu * block;
@@ -668,6 +669,8 @@ int rows_forward(int64_t M, int64_t C, int64_t F, const void *blob, const float 
     case 2: return launch_rows<2, 8>(a, num_cu, st);
     case 3: return launch_rows<3, 8>(a, num_cu, st);
     case 4: return launch_rows<4, 8>(a, num_cu, st);
+    case 5: return launch_rows<5, 4>(a, num_cu, st);
+    case 6: return launch_rows<6, 4>(a, num_cu, st);
     case 7: return launch_rows<7, 4>(a, num_cu, st);
     default: return launch_rows<8, 4>(a, num_cu, st);
   }
@@ -715,6 +718,8 @@ int rows_hidden_backward(int64_t M, int64_t C, int64_t F, int64_t Fp, const void
     case 2: return launch_hidden<2, 8>(a, num_cu, st);
     case 3: return launch_hidden<3, 8>(a, num_cu, st);
     case 4: return launch_hidden<4, 8>(a, num_cu, st);
+    case 5: return launch_hidden<5, 4>(a, num_cu, st);
+    case 6: return launch_hidden<6, 4>(a, num_cu, st);
     case 7: return launch_hidden<7, 4>(a, num_cu, st);
     default: return launch_hidden<8, 4>(a, num_cu, st);
   }
