@@ -705,6 +705,18 @@ int64_t pa_gated_mlp_backward_workspace_bytes(int dtype, int64_t rows, int64_t C
 int pa_gated_mlp_backward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
                           const void *dy, void *dx, const pa_gated_grads *grads, void *workspace, int64_t workspace_bytes,
                           void *stream);
+/* How many of a forward call's rows, on 16-byte boundaries, run with the hidden layer on chip. */
+int64_t pa_gated_mlp_rows_on_chip(int dtype, int64_t rows, int64_t C, int64_t F);
+/* The kernels that the products of this section run on at a size, as two launches: launches[0] rows on tiles launches[1], then
+ * launches[2] rows (0: no second launch) on tiles launches[3].  Tiles by rows x weight rows: 0 256 x 256 (PA_PRODUCT_BACK
+ * 128 x 256), 1 128 x 128, 2 64 x 64, 3 32 x 32 with the reduction split (few rows).  bytes: 1 int8, 2 bf16, 4 float32; K the
+ * reduction's elements, K2 those of PA_PRODUCT_BACK's second product. */
+#define PA_PRODUCT_PLAIN 0 /* a Linear, w_down, dx */
+#define PA_PRODUCT_GATED 1 /* gate and up at once */
+#define PA_PRODUCT_BACK 2  /* the hidden layer's backward */
+#define PA_PRODUCT_PEAK 3  /* int8 gate and up, largest value per row */
+#define PA_PRODUCT_CODES 4 /* int8 gate and up, codes */
+int pa_product_launches(int bytes, int kind, int64_t rows, int64_t columns, int64_t K, int64_t K2, int64_t launches[4]);
 
 /* y = residual + dropout(x), and with `normed` its LayerNorm (of the unrounded sum), over rows of C up to 2^23.  Element (r, c)
  * is kept, and scaled by 1 / (1 - p), where word c % 4 of Philox4x32-10 of the counter (c / 4, r mod 2^32, r / 2^32,

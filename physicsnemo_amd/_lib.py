@@ -44,6 +44,7 @@ EXPORTED = [
     "pa_block_query", "pa_block_workspace_bytes", "pa_block_forward", "pa_markers_enabled",
     "pa_mfma_project_softmax_reduce_clocked", "pa_weight_grad_workspace_bytes", "pa_weight_grad",
     "pa_gated_mlp_workspace_bytes", "pa_gated_mlp_forward", "pa_gated_mlp_backward_workspace_bytes", "pa_gated_mlp_backward",
+    "pa_gated_mlp_rows_on_chip", "pa_product_launches",
     "pa_dropout_add_norm", "pa_dropout_add_norm_backward_workspace_bytes", "pa_dropout_add_norm_backward", "pa_dropout_advance",
     "pa_int8_quantize_rows", "pa_int8_linear_workspace_bytes", "pa_int8_linear", "pa_int8_gated_workspace_bytes", "pa_int8_gated",
 ]
@@ -350,6 +351,10 @@ def load() -> ctypes.CDLL:
     lib.pa_gated_mlp_backward.restype = c_int
     lib.pa_gated_mlp_backward.argtypes = rows3 + [POINTER(PaGatedParams), c_int] + [c_void_p] * 3 + [
         POINTER(PaGatedGrads), c_void_p, c_int64, c_void_p]
+    lib.pa_gated_mlp_rows_on_chip.restype = c_int64
+    lib.pa_gated_mlp_rows_on_chip.argtypes = rows3
+    lib.pa_product_launches.restype = c_int
+    lib.pa_product_launches.argtypes = [c_int, c_int] + [c_int64] * 4 + [POINTER(c_int64)]
     lib.pa_dropout_add_norm.restype = c_int
     lib.pa_dropout_add_norm.argtypes = [c_int, c_int64, c_int64, c_void_p, c_void_p, c_double] + [c_void_p] * 4 + [
         c_float] + [c_void_p] * 3

@@ -360,7 +360,7 @@ int mfma_layer(const pa_shape &s, const pa_params &p, const void *blob, const vo
 
 extern "C" {
 
-int pa_version(void) { return 113; }
+int pa_version(void) { return 114; }
 
 int pa_set_compute_units(int n) {
   if (n < 0 || n > 4096) return PA_ERR_DIMS;
@@ -1926,6 +1926,19 @@ int pa_gated_mlp_backward(int dtype, int64_t rows, int64_t C, int64_t F, const p
   if (workspace_bytes < need) return PA_ERR_WORKSPACE;
   return pa::gated::backward(dtype, rows, C, F, *p, act, x, dy, dx, *grads, workspace, compute_units(),
                              static_cast<hipStream_t>(stream));
+}
+
+int pa_product_launches(int bytes, int kind, int64_t rows, int64_t columns, int64_t K, int64_t K2, int64_t launches[4]) {
+  if (!launches) return PA_ERR_NULL;
+  if (rows <= 0 || columns <= 0 || K <= 0 || K2 < 0) return PA_ERR_DIMS;
+  if (rows > PA_MAX_ROWS || columns > 1 << 19 || K > 1 << 19 || K2 > 1 << 19) return PA_ERR_UNSUPPORTED;
+  auto units = [&](int64_t k) { return (k * bytes + 15) / 16; };
+  return pa::tile::launches_query(bytes, kind, rows, columns, units(K), units(K2), compute_units(), launches) ? PA_OK : PA_ERR_UNSUPPORTED;
+}
+
+int64_t pa_gated_mlp_rows_on_chip(int dtype, int64_t rows, int64_t C, int64_t F) {
+  if (int rc = check_gated(dtype, rows, C, F)) return rc;
+  return dtype == PA_BF16 && C % 8 == 0 && C <= 256 ? pa::gated::rows_worth(rows, C, compute_units()) : 0;
 }
 
 static int check_dropout(int dtype, int64_t rows, int64_t C) {

@@ -82,6 +82,14 @@ int lay_out(const Layout &a, size_t elem, hipStream_t st) {
   return launch_status();
 }
 
+bool launches_query(int bytes, int kind, int64_t M, int64_t N, int64_t units, int64_t units2, int num_cu, int64_t out[4]) {
+  if ((bytes != 1 && bytes != 2 && bytes != 4) || kind < kPlain || kind > kCodes) return false;
+  if ((bytes == 1 && (kind == kGated || kind == kBack)) || (bytes != 1 && kind >= kPeak)) return false;
+  const Launches l = launches_of(bytes, (Kind)kind, M, N, units, units2, num_cu);
+  for (int k = 0; k < 2; ++k) out[2 * k] = l.rows[k], out[2 * k + 1] = l.size[k];
+  return true;
+}
+
 }  // namespace tile
 
 namespace gated {

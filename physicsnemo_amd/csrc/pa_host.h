@@ -162,8 +162,13 @@ int backward(const pa_shape &s, const void *x, const void *dy, const void *saved
              int num_cu, hipStream_t st);
 }  // namespace train_f32
 
+namespace tile {
+bool launches_query(int bytes, int kind, int64_t M, int64_t N, int64_t units, int64_t units2, int num_cu, int64_t out[4]);  // pa_product_launches
+}  // namespace tile
+
 namespace gated {
 // gated feed-forward block: see pa_gated_mlp_forward / _backward
+int64_t rows_worth(int64_t M, int64_t C, int num_cu);
 bool supported(int dtype, int64_t M, int64_t C, int64_t F);
 int64_t forward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu);
 int64_t backward_workspace_bytes(int dtype, int64_t M, int64_t C, int64_t F, int num_cu);

@@ -970,14 +970,14 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Args a) {
 // bf16 2 048 -> 512, 64 rows 17.9 / 8.8, 1 000 (two rounds) 18.0 / 17.1, 1 500 17.8 / 25.0; 512 -> 2 x 2 048, 64 rows 6.5 / 6.9;
 // float32 2 048 -> 512, 64 rows 75.6 / 21.9, 1 500 77.6 / 68.5, 2 000 77.9 / 89.3, 512 -> 2 x 2 048, 64 rows 21.6 / 10.1, 400 32.7 /
 // 36.4; int8 512 -> 2 048, 64 rows 6.0 / 4.3, 400 6.3 / 9.5, 2 048 -> 512, 64 rows 11.0 / 7.6, 600 11.3 / 12.3.
-template <class E, Kind KIND>
-bool few_rows_worth(const Args &a, int64_t stages, int num_cu) {
-  const double step = E::kBytes == 4 ? 1.2 : 0.4;  // of a tile's stage and of a wave's step alike
-  const int64_t units = E::kBytes == 4 ? 4 : 2, per = ((a.units + units - 1) / units + 7) / 8;
-  const int64_t groups = ((a.M + 31) / 32) * ((a.N + 31) / 32), columns = KIND == kGated ? 32 : 64;
-  const int64_t tiles = ((a.M + 63) / 64) * ((a.N + columns - 1) / columns);
+inline bool few_rows_worth(int bytes, Kind kind, int64_t M, int64_t N, int64_t row_units, int64_t stages, int num_cu) {
+  if (kind != kPlain && !(kind == kGated && bytes != 1)) return false;
+  const double step = bytes == 4 ? 1.2 : 0.4;  // of a tile's stage and of a wave's step alike
+  const int64_t units = bytes == 4 ? 4 : 2, per = ((row_units + units - 1) / units + 7) / 8;
+  const int64_t groups = ((M + 31) / 32) * ((N + 31) / 32), columns = kind == kGated ? 32 : 64;
+  const int64_t tiles = ((M + 63) / 64) * ((N + columns - 1) / columns);
   const int64_t rounds = (groups + num_cu - 1) / num_cu;
-  return tiles <= num_cu && rounds * (1.5 + step * per * (KIND == kGated ? 2 : 1)) <= 1.5 + step * stages;
+  return tiles <= num_cu && rounds * (1.5 + step * per * (kind == kGated ? 2 : 1)) <= 1.5 + step * stages;
 }
 
 template <class E, class TO, Kind KIND>
@@ -1021,33 +1021,46 @@ inline Plan plan_of(int64_t M, int64_t N, int64_t stages, bool back, bool pairs,
   return p;
 }
 
+// The launches of a product: on tiles of `size` (3: few_rows_kernel) the first rows[0] rows, the rest on tiles of their own.
+struct Launches {
+  int64_t rows[2];
+  int size[2];
+};
+inline Launches launches_of(int bytes, Kind kind, int64_t M, int64_t N, int64_t units, int64_t units2, int num_cu) {
+  const bool back = kind == kBack, pairs = kind != kPlain;
+  const int64_t stages = (units + 7) / 8 + (back ? (units2 + 7) / 8 : 0);
+  if (few_rows_worth(bytes, kind, M, N, units, stages, num_cu)) return {{M, 0}, {3, 0}};
+  const Plan p = plan_of(M, N, stages, back, pairs, num_cu, true);
+  if (p.rows == M) return {{M, 0}, {p.size, 0}};
+  return {{p.rows, M - p.rows}, {p.size, plan_of(M - p.rows, N, stages, back, pairs, num_cu, false).size}};
+}
+
 template <class E, class TO, Kind KIND>
 int launch(Args a, int num_cu, hipStream_t st) {
   using Large = typename std::conditional<KIND == kBack, Config<2, 4, 2, 2, 8, 3, 2>, Config<4, 2, 2, 4, 8, 2, 2>>::type;
   using Medium = Config<2, 2, 2, 2, 8, 2, 2>;
   using Small = Config<2, 1, 1, 2, 8, 3, 2>;
-  const int64_t stages = (a.units + 7) / 8 + (KIND == kBack ? (a.units2 + 7) / 8 : 0);
+  const Launches l = launches_of(E::kBytes, KIND, a.M, a.N, a.units, a.units2, num_cu);
   if constexpr (KIND == kPlain || (KIND == kGated && E::kBytes != 1))
-    if (few_rows_worth<E, KIND>(a, stages, num_cu)) return launch_few_rows<E, TO, KIND>(a, st);
+    if (l.size[0] == 3) return launch_few_rows<E, TO, KIND>(a, st);
   auto run = [&](const Args &t, int size) {
     if (size == 0) return launch_tiles<E, TO, KIND, Large>(t, num_cu, st);
     if (size == 1) return launch_tiles<E, TO, KIND, Medium>(t, num_cu, st);
     return launch_tiles<E, TO, KIND, Small>(t, num_cu, st);
   };
-  const Plan p = plan_of(a.M, a.N, stages, KIND == kBack, KIND != kPlain, num_cu, true);
   Args rest = a;
-  a.M = p.rows;
-  int rc = run(a, p.size);
-  if (rc || p.rows == rest.M) return rc;
-  auto past = [&](const void *q, int64_t row) { return q ? const_cast<char *>(static_cast<const char *>(q)) + p.rows * row : nullptr; };
-  rest.M -= p.rows;
+  a.M = l.rows[0];
+  int rc = run(a, l.size[0]);
+  if (rc || l.rows[1] == 0) return rc;
+  auto past = [&](const void *q, int64_t row) { return q ? const_cast<char *>(static_cast<const char *>(q)) + l.rows[0] * row : nullptr; };
+  rest.M = l.rows[1];
   rest.X = past(a.X, a.ldx), rest.X2 = past(a.X2, a.ldx2);
-  rest.sx = a.sx ? a.sx + p.rows : nullptr;
-  rest.sums = a.sums ? a.sums + p.rows / 32 * 2 * a.ldh : nullptr;
-  rest.peak = a.peak ? a.peak + p.rows : nullptr, rest.row_scale = a.row_scale ? a.row_scale + p.rows : nullptr;
+  rest.sx = a.sx ? a.sx + l.rows[0] : nullptr;
+  rest.sums = a.sums ? a.sums + l.rows[0] / 32 * 2 * a.ldh : nullptr;
+  rest.peak = a.peak ? a.peak + l.rows[0] : nullptr, rest.row_scale = a.row_scale ? a.row_scale + l.rows[0] : nullptr;
   rest.residual = past(a.residual, a.ldo * (int64_t)sizeof(TO));
   rest.out = past(a.out, a.ldo * (int64_t)(KIND == kCodes ? 1 : sizeof(TO))), rest.out2 = past(a.out2, a.ldh * (int64_t)sizeof(TO));
-  return run(rest, plan_of(rest.M, a.N, stages, KIND == kBack, KIND != kPlain, num_cu, false).size);
+  return run(rest, l.size[1]);
 }
 
 // ---- host side of the calls that use the products ----
