@@ -7,6 +7,7 @@ from contextlib import contextmanager
 import torch
 import torch.nn as nn
 
+from . import _lib
 from . import autograd as PA
 from . import functional as PF
 
@@ -140,7 +141,8 @@ def counter_dropout(attn: nn.Module) -> CounterDropout | None:
 
 
 class Int8Mlp:
-    """8-bit weights of a block's Mlp or GatedMlp, made once per parameter set, and the MLP on them.
+    """8-bit weights of a block's Mlp or GatedMlp, made once per parameter set, and the MLP on them.  A GatedMlp's hidden layer goes
+    from float32 to codes; an Mlp is two Linears, between which it is rounded to the rows' type.
 
     A set is told by its parameters' addresses, versions and types, and holds the parameters, so that no address comes twice.  A
     write through `.data` changes none of the three: `refresh` after it.  The codes are complete before the call that makes
@@ -178,13 +180,15 @@ class Int8Mlp:
         return lins, act
 
     def _of(self, lins, device):
-        with PF._on(device):
-            return self._of_current_device(lins, device)
-
-    def _of_current_device(self, lins, device):
         params = [p for lin in lins for p in (lin.weight, lin.bias)]
         stamp = (device,) + tuple(None if p is None else (p.data_ptr(), p._version, p.dtype) for p in params)
-        stream, capturing = torch.cuda.current_stream(device), torch.cuda.is_current_stream_capturing()
+        if torch.cuda.current_device() != device.index:
+            with torch.cuda.device(device):
+                return self._of_current_device(lins, device, params, stamp)
+        return self._of_current_device(lins, device, params, stamp)
+
+    def _of_current_device(self, lins, device, params, stamp):
+        stream, capturing = _lib.current_stream_ptr(device), torch.cuda.is_current_stream_capturing()
         if self._stamp != stamp:
             with torch.no_grad():
                 weights = [
@@ -193,7 +197,7 @@ class Int8Mlp:
                     for lin in lins]
             if capturing:
                 return weights
-            stream.synchronize()
+            torch.cuda.current_stream(device).synchronize()
             self._weights, self._held, self._streams = weights, [None if p is None else p.detach() for p in params], {stream}
             self._stamp = stamp
         elif capturing:
@@ -201,7 +205,7 @@ class Int8Mlp:
                 self.of_graphs.append(self._weights)
         elif stream not in self._streams:  # the codes' memory is not reused before this stream's work on them is done
             for t in (t for w in self._weights for t in w if t is not None):
-                t.record_stream(stream)
+                t.record_stream(torch.cuda.current_stream(device))
             self._streams.add(stream)
         return self._weights
 

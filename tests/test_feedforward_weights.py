@@ -1,12 +1,12 @@
 """Which weights the feed-forward modules hand to the kernels: those of the moment of the call, however they were written."""
 import copy
 import pickle
-from contextlib import nullcontext
 
 import pytest
 import torch
 
 import physicsnemo_amd as pn
+from physicsnemo_amd import _lib
 from physicsnemo_amd import functional as PF
 from physicsnemo_amd.feedforward import Int8Mlp
 
@@ -61,8 +61,9 @@ def on_cpu(monkeypatch):
         return (w / scale[:, None]).round().to(torch.int8), scale
 
     monkeypatch.setattr(PF, "quantize_int8", quantize)
-    monkeypatch.setattr(PF, "_on", lambda device: nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: CPU.index)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: here.stream)
+    monkeypatch.setattr(_lib, "current_stream_ptr", lambda device: id(here.stream))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: here.capturing)
     monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, stream: here.recorded.append((t.data_ptr(), stream)))
     return here
