@@ -675,7 +675,8 @@ int pa_layernorm_backward_add(int dtype, int64_t rows, int64_t C, const void *x,
 #define PA_ACT_TANH 5
 
 /* Tensors of this section may start on any element boundary and have any width; rows that are not whole 16-byte units are
- * copied to padded ones in the workspace, which must be 16-byte aligned.  C, F up to 2^18. */
+ * copied to padded ones in the workspace, which must be 16-byte aligned.  C, F up to 2^18.
+ * float32 products are sums of bf16 products: good to 2^-22 of each term, and NaN where a term is infinite. */
 
 /* y = residual + w_down (act(w_gate x + b_gate) * (w_up x + b_up)) + b_down over rows of C with F hidden units.  Weights in the
  * activations' type (dtype: PA_F32 or PA_BF16), biases float32, each NULL if there is none. */
@@ -687,11 +688,13 @@ typedef struct pa_gated_params {
   const void *w_down;  /* (C, F) */
   const float *b_down; /* (C) or NULL */
 } pa_gated_params;
-/* residual (rows, C) or NULL; y may be residual itself, but not x. */
+/* residual (rows, C) or NULL; y may be residual itself, but not x.  The workspace has room for the hidden layer of the rows that do
+ * not keep it on chip, and for copies of rows whose width asks for them; rows off a boundary run in pieces. */
 int64_t pa_gated_mlp_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F);
 int pa_gated_mlp_forward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
                          const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
-/* Its gradients from dy and x; the hidden layer is formed again.  Weight gradients in the weights' type, bias gradients
+/* Its gradients from dy and x; the hidden layer is formed again.  The workspace has room for 3 F and, for x and dy off a boundary,
+ * 2 C elements a row.  Weight gradients in the weights' type, bias gradients
  * float32, each NULL if not wanted; dx (rows, C) or NULL.  (The gradient of residual is dy.)  Sums in a fixed order. */
 typedef struct pa_gated_grads {
   void *w_gate;
@@ -735,7 +738,7 @@ int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void 
 /* taken <- state, then state's offset + 1: the values one call and its backward pass use. */
 int pa_dropout_advance(int64_t *state, int64_t *taken, void *stream);
 
-/* q = rint(127 x / max |x|) per row as int8 and scale = max |x| / 127 (float32): rows of x of K elements; q's rows are ldq
+/* q = rint(x (127 / max |x|)) per row as int8 and scale = max |x| / 127, both quotients rounded to float32: rows of x of K elements; q's rows are ldq
  * bytes apart (at least K, a multiple of 8; q 8-byte aligned), zeros behind the K-th.  A row of zeros has scale 0; one with an infinity or NaN has scale NaN. */
 int pa_int8_quantize_rows(int dtype, int64_t rows, int64_t K, const void *x, void *q, int64_t ldq, float *scale, void *stream);
 /* y = act(q_x q_w^T scaled by both scales + bias) + residual: x (rows, K) is quantised as above, w (N, K) int8 with w_scale (N)

@@ -78,7 +78,7 @@ struct RowsArgs {
 // CT = 8: one wave per SIMD with 512 registers (y 128, x 64, two sets of g and u 64); narrower rows: two.  One barrier per slot:
 // two waves per SIMD meet at its beginning and cover each other (two LDS buffers); a wave alone has the next slot's data a
 // slot earlier (three) and its first fragments and biases in registers, and meets the others behind its first products
-// (262 144 x 256, F = 1 024: 549 -> 517 us; meeting behind step 10 of 48 530; with two waves per SIMD the registers that this takes cost more than it gives,
+// (262 144 x 256, F = 1 024, GELU of degree 5: 549 -> 517 us; meeting behind step 10 of 48 530; with two waves per SIMD the registers that this takes cost more than it gives,
 // 262 144 x 128, F = 512, backward 197 -> 245).
 // ---------------------------------------------------------------------------------------------------------------
 // Twenty ticks of vector work spread evenly behind the first 5 CT matrix instructions of a slot: those behind step S.

@@ -1,5 +1,6 @@
 // Products of 8-bit integers with one float32 scale per token (row of activations) and per output channel (row of weights):
-//   q = rint(127 x / max |x|) per row, s = max |x| / 127;  y = act(s s_w (q . q_w) + b) + residual
+//   q = rint(x (127 / max |x|)) per row, s = max |x| / 127;  y = act(s s_w (q . q_w) + b) + residual
+// Both quotients are rounded to float32: of a value half a step between two codes (max |x| / 2, say) either may be taken.
 // The sums of whole numbers are exact in 32 bits up to 131 072 terms of 127 x 127.  int8 matrix instructions have twice the
 // rate of bf16 ones and the operands half the bytes, so the products run on the tile kernel of pa_tile.h with stages of 128
 // elements.

@@ -33,8 +33,10 @@ struct Bf16 {
   static __device__ __forceinline__ Acc mma(u32x4 a, u32x4 b, Acc c) { return mfma::mma(a, b, c); }
 };
 // float32 as sums of three bf16 values (8 + 8 + 8 bits), six products of them: hi hi + hi mid + mid hi + hi lo + lo hi + mid mid.
-// What is left out is below 2^-24 of a product, the error of a float32 product itself.  Against float32 matrix
-// instructions: 192 cycles per 32 x 32 x 16 instead of 512, and 44 vector instructions per operand.
+// The first part is cut off, not rounded, so that the second is up to 2^-7 of the value and the third 2^-16: what is left out is
+// up to 2^-22 of a product (8 % of products of operands just above a power of two pass 2^-24, a float32 product's own error).
+// Parts of an infinity are not numbers, nor is their product with a part that is zero: a sum that holds one is NaN.  Against
+// float32 matrix instructions: 192 cycles per 32 x 32 x 16 instead of 512, and 44 vector instructions per operand.
 struct F32 {
   using Acc = f32x16;
   static constexpr int kBytes = 4;
@@ -73,8 +75,8 @@ struct I8 {
   }
 };
 
-// ---- activations of the library's Mlp (see pa_gated_act_code) ----
-enum Act { kNone = 0, kGelu = 1, kRelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5, kActs = 6 };
+// ---- activations: PA_ACT_* ----
+enum Act { kNone = 0, kGelu = 1, kRelu = 2, kSilu = 3, kSigmoid = 4, kTanh = 5 };
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v)); }
 

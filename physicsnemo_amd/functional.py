@@ -1196,7 +1196,8 @@ def gated_mlp_forward(x, w_gate, b_gate, w_up, b_up, w_down, b_down, act: str | 
     """y = w_down . (act(w_gate . x + b_gate) * (w_up . x + b_up)) + b_down [+ residual] over the last axis of x.
 
     x (..., C) bfloat16 or float32; w_gate, w_up (F, C) and w_down (C, F) in the same type; biases float32 or None; `act`
-    one of "silu", "gelu" (erf form), "relu", "sigmoid", "tanh", None.  Any widths."""
+    one of "silu", "gelu" (erf form), "relu", "sigmoid", "tanh", None.  Any widths.  In float32 an infinite term of a sum makes
+    it NaN (products run as sums of bf16 products)."""
     rows, C, F = _gated_sizes(x, residual, w_gate, b_gate, w_up, b_up, w_down, b_down)
     code = _act_code(act)
     _expect(residual, "residual", x.shape, x.dtype)
@@ -1325,7 +1326,8 @@ def dropout_advance(state):
 
 
 def quantize_int8(x):
-    """(int8 codes, float32 scale per row) of the rows of x (..., K): codes rint(127 x / max |x|), scale max |x| / 127.
+    """(int8 codes, float32 scale per row) of the rows of x (..., K): codes rint(x (127 / max |x|)), scale max |x| / 127, both
+    quotients rounded to float32.
     For a weight (N, K) that is one scale per output channel.  A row of zeros has scale 0, one with an infinity or NaN
     scale NaN."""
     _need_cuda(x)

@@ -103,3 +103,18 @@ def test_large_int8_linears(rows, K, N):
     x, (w, sw), b, res = draw(rows, K).bfloat16(), codes(draw(N, K)), draw(N), draw(rows, N).bfloat16()
     want, tol = linear64(x, w, sw, b, "gelu", res)
     check(PF.linear_int8(x, w, sw, b, "gelu", res), want.cpu(), tol.cpu(), "y")
+
+
+@pytest.mark.parametrize("rows,C,F", [(70, 64, 80), (1, 64, 80), (3000, 512, 700)])
+def test_float32_rows_that_are_not_finite(eight_cus, rows, C, F):
+    """They give rows that are not finite and change no other."""
+    announce("tiles, float32 not finite", rows, C, F)
+    gpu = on_gpu(make(rows, C, F, torch.float32, seed=5))
+    params = [gpu[n] for n in NAMES]
+    clean = PF.gated_mlp_forward(gpu["x"], *params, act="gelu")
+    for k, bad in enumerate((float("nan"), float("inf"), -float("inf"))):
+        x, row = gpu["x"].clone(), (rows - 1, 0, rows // 2)[k]
+        x[row, (0, C - 1, C // 2)[k]] = bad
+        y = PF.gated_mlp_forward(x, *params, act="gelu")
+        others = torch.arange(rows, device="cuda") != row
+        assert torch.equal(y[others], clean[others]) and not bool(torch.isfinite(y[row]).any())
