@@ -693,8 +693,8 @@ typedef struct pa_gated_params {
 int64_t pa_gated_mlp_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_t F);
 int pa_gated_mlp_forward(int dtype, int64_t rows, int64_t C, int64_t F, const pa_gated_params *p, int act, const void *x,
                          const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
-/* Its gradients from dy and x; the hidden layer is formed again.  The workspace has room for 3 F and, for x and dy off a boundary,
- * 2 C elements a row.  Weight gradients in the weights' type, bias gradients
+/* Its gradients from dy and x; the hidden layer is formed again.  The workspace has room for 3 F elements a row, for copies of x and
+ * dy where their width asks for them, and for partial weight gradients; rows off a boundary run in pieces.  Weight gradients in the weights' type, bias gradients
  * float32, each NULL if not wanted; dx (rows, C) or NULL.  (The gradient of residual is dy.)  Sums in a fixed order. */
 typedef struct pa_gated_grads {
   void *w_gate;

@@ -293,25 +293,55 @@ int forward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p
   return forward<tile::Bf16, bf16>(M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
 }
 
-// partial results of a row-axis product of `oa` by `ob` columns, and of the column sums of its first operand
+// partial results of a row-axis product of `oa` by `ob` columns, and of the column sums of its first operand: of `rows` of a
+// call's M rows, bf16 their share of the call's
+template <class E>
+static int64_t chunks_of(int64_t rows, int64_t M, int64_t oa, int64_t ob, int num_cu) {
+  if (E::kBytes == 4) return gemm::cols_gemm_f32_chunks(rows, oa, ob, num_cu);
+  const int64_t all = wgrad::chunks_for(M, ((oa + 255) / 256) * ((ob + 255) / 256), oa * ob, num_cu), share = rows == M ? all : all * rows / M;
+  return share < 1 ? 1 : share;
+}
 struct Partials {
-  int64_t G;
-  float *product, *sums;
+  int64_t G = 0, M = 0, oa = 0, ob = 0;  // G: how many there are so far
+  float *product = nullptr, *sums = nullptr;
 };
 template <class E>
-static Partials partials_of(int64_t M, int64_t oa, int64_t ob, int num_cu, Space &ws) {
-  Partials r{};
-  if (E::kBytes == 2) r.G = wgrad::chunks_for(M, ((oa + 255) / 256) * ((ob + 255) / 256), oa * ob, num_cu);
-  else r.G = gemm::cols_gemm_f32_chunks(M, oa, ob, num_cu);
-  r.product = static_cast<float *>(ws.take(r.G * oa * ob * 4));
-  r.sums = static_cast<float *>(ws.take(r.G * oa * 4));
+static Partials partials_of(int64_t M, int64_t rows, int64_t oa, int64_t ob, int num_cu, Space &ws) {
+  int64_t most = 0;
+  for (int64_t r0 = 0; r0 < M; r0 += rows) most += chunks_of<E>(M - r0 < rows ? M - r0 : rows, M, oa, ob, num_cu);
+  Partials r;
+  r.M = M, r.oa = oa, r.ob = ob;
+  r.product = static_cast<float *>(ws.take(most * oa * ob * 4));
+  r.sums = static_cast<float *>(ws.take(most * oa * 4));
   return r;
 }
 template <class E>
-static int rows_product(const Partials &r, const void *A, int64_t oa, const void *B, int64_t ob, int64_t M, int groups, int num_cu,
+static int rows_product(Partials &r, const void *A, const void *B, int64_t rows, int groups, int num_cu,
                         hipStream_t st) {  // groups: 1 if A, 2 if B is a matrix of the hidden layer
-  if (E::kBytes == 2) return wgrad::launch_wide(A, oa, oa, B, ob, ob, M, r.G, nullptr, r.product, groups == 1 ? nullptr : r.sums, st, groups);
-  return gemm::cols_gemm_f32(A, oa, oa, B, ob, ob, M, nullptr, r.product, r.sums, num_cu, st);
+  float *product = r.product + r.G * r.oa * r.ob, *sums = r.sums + r.G * r.oa;
+  const int64_t G = chunks_of<E>(rows, r.M, r.oa, r.ob, num_cu);
+  r.G += G;
+  if (E::kBytes == 2) return wgrad::launch_wide(A, r.oa, r.oa, B, r.ob, r.ob, rows, G, nullptr, product, groups == 1 ? nullptr : sums, st, groups);
+  return gemm::cols_gemm_f32(A, r.oa, r.oa, B, r.ob, r.ob, rows, nullptr, product, sums, num_cu, st);
+}
+
+// The backward's workspace: dg and du, h, transposed weights, partial weight gradients, and copies of what is not laid out in whole
+// units.  As in the forward, x and dy off a boundary run in pieces: as many rows each as leave room for their copies beside the
+// piece's hidden layer in what a call on boundaries needs for all rows (131 072 x 256, F = 1 024, bf16: 978 MB instead of 1 112;
+// 1 048 576 x 256, F = 256: 1 814 instead of 2 887).
+struct BackwardRoom {
+  void *dgu, *h, *x, *dy;
+  Partials in, down;
+};
+template <class E>
+static BackwardRoom backward_room(int64_t M, int64_t rows, int64_t Cp, int64_t Fp, bool copy_x, bool copy_dy, int num_cu, Space &ws) {
+  constexpr int64_t e = E::kBytes;
+  const int64_t whole = up(rows, tile::kGroupRows);
+  BackwardRoom r;
+  r.dgu = ws.take(whole * 2 * Fp * e), r.h = ws.take(whole * Fp * e);
+  r.x = copy_x ? ws.take(rows * Cp * e) : nullptr, r.dy = copy_dy ? ws.take(rows * Cp * e) : nullptr;
+  r.in = partials_of<E>(M, rows, 2 * Fp, Cp, num_cu, ws), r.down = partials_of<E>(M, rows, Cp, Fp, num_cu, ws);
+  return r;
 }
 
 template <class E, class TO>
@@ -322,70 +352,88 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   Space ws{workspace};
   Layout lay;
   const int64_t Cp = up(C < LEAST ? LEAST : C, U), Fp = up(F < LEAST ? LEAST : F, 32 / e);
-  const bool copy_x = plan || C != Cp || !aligned16(x), copy_dy = plan || C != Cp || !aligned16(dy);
-  const int64_t Mp = up(M, tile::kGroupRows);
-  void *dgu = ws.take(Mp * 2 * Fp * e), *h = ws.take(Mp * Fp * e);
-  auto padded = [&](const void *q, int64_t rows, int64_t cols, int64_t ld, bool copy) {
-    Rows r{q, ld * e, (int)(ld * e / 16)};
-    if (copy) {
-      void *dst = ws.take(rows * ld * e);
-      lay.add(q, cols, dst, rows, cols, ld, ld, false);
+  const bool whole = C == Cp, copy_x = !whole || !aligned16(x), copy_dy = !whole || !aligned16(dy);
+  // rows of a piece: all of them, or of x and dy off a boundary
+  int64_t piece = M * 3 * Fp / (3 * Fp + 2 * Cp) / tile::kGroupRows * tile::kGroupRows;
+  if (piece < kLooseRows) piece = M < kLooseRows ? M : kLooseRows;
+  const int64_t per = whole && !plan && (copy_x || copy_dy) ? piece : M;
+  Space loose = ws;
+  BackwardRoom room = backward_room<E>(M, per, Cp, Fp, copy_x, copy_dy, num_cu, ws);
+  if (plan && whole) {
+    backward_room<E>(M, piece, Cp, Fp, true, true, num_cu, loose);
+    if (loose.used > ws.used) ws.used = loose.used;
+  }
+  // rows of the kernel that owns them, which has the weights in an order of its own
+  const bool by_rows = e == 2 && rows_supported(Cp, F);
+  auto rows_done = [&](int64_t rows) { return by_rows && !plan ? rows_worth(rows, Cp, num_cu) : 0; };
+  const bool tiles_too = per < M || rows_done(M) < M;  // some rows may be the tile kernels'
+  void *blob = by_rows ? ws.take(hidden_blob_bytes(C, F)) : nullptr;
+  auto weight = [&](const void *w) {
+    Rows r{w, Cp * e, (int)(Cp * e / 16)};
+    if (plan || (tiles_too && (!whole || !aligned16(w)))) {
+      void *dst = ws.take(F * Cp * e);
+      if (!plan) lay.add(w, C, dst, F, C, Cp, Cp, false);
       r.p = dst;
     }
     return r;
   };
-  const Rows xr = padded(x, M, C, Cp, copy_x), dyr = padded(dy, M, C, Cp, copy_dy);
-  // rows of the kernel that owns them, which has the weights in an order of its own
-  const bool by_rows = e == 2 && rows_supported(Cp, F);
-  const int64_t done = by_rows && !plan ? rows_worth(M, Cp, num_cu) : 0, rest = M - done;
-  void *blob = by_rows ? ws.take(hidden_blob_bytes(C, F)) : nullptr;
-  const bool copy_w = plan || C != Cp || !aligned16(p.w_gate) || !aligned16(p.w_up);
-  const Rows wg = padded(p.w_gate, F, C, Cp, copy_w && rest > 0), wu = padded(p.w_up, F, C, Cp, copy_w && rest > 0);
+  const Rows wg = weight(p.w_gate), wu = weight(p.w_up);
   // W_down^T (F, Cp), and [W_gate; W_up]^T (C, 2 Fp): hidden units past F are zero columns
   void *wd_t = ws.take(F * Cp * e), *w_t = ws.take(C * 2 * Fp * e);
-  const Partials in = partials_of<E>(M, 2 * Fp, Cp, num_cu, ws), down = partials_of<E>(M, Cp, Fp, num_cu, ws);
   // bf16: dg and du are rounded for their products, their column sums are not
   const int64_t tiles = (M + 31) / 32, parts = tiles < 2048 ? (tiles + 31) / 32 : 64;
   float *sums = e == 2 ? static_cast<float *>(ws.take(tiles * 2 * Fp * 4)) : nullptr;
   float *sum_parts = e == 2 ? static_cast<float *>(ws.take(parts * 2 * Fp * 4)) : nullptr;
   if (plan) return *bytes = ws.used, PA_OK;
-  if (rest > 0) lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
+  if (tiles_too) lay.add(p.w_down, F, wd_t, F, C, Cp, Cp, true);
   if (dx) {
     lay.add(p.w_gate, C, w_t, C, F, Fp, 2 * Fp, true);
     lay.add(p.w_up, C, static_cast<char *>(w_t) + Fp * e, C, F, Fp, 2 * Fp, true);
   }
-  int rc = tile::lay_out(lay, e, st);
-  if (rc) return rc;
-  if (done > 0) {
-    rc = hidden_pack(C, F, p, blob, st);
-    if (!rc) rc = rows_hidden_backward(done, Cp, F, Fp, blob, act, xr.p, dyr.p, dgu, h, sums, num_cu, st);
-    if (rc) return rc;
-  }
-  if (rest > 0) {
-    auto from = [&](const void *q, int64_t ld) { return const_cast<char *>(static_cast<const char *>(q)) + done * ld; };
-    Args a{};
-    a.X = from(xr.p, xr.ld), a.ldx = xr.ld, a.units = xr.units;
-    a.X2 = from(dyr.p, dyr.ld), a.ldx2 = dyr.ld, a.units2 = dyr.units;
-    a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
-    a.M = rest, a.N = (int)F, a.limit = (int)Fp;
-    a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
-    a.sums = e == 2 && (out.b_gate || out.b_up) ? reinterpret_cast<float *>(from(sums, 2 * Fp * 4 / 32)) : nullptr;
-    a.out = from(dgu, 2 * Fp * e), a.ldo = 2 * Fp, a.out2 = from(h, Fp * e), a.ldh = Fp, a.act = act;
-    if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
-  }
-  if (dx) {
-    Args d{};
-    d.X = dgu, d.ldx = 2 * Fp * e, d.units = (int)(2 * Fp * e / 16), d.x_groups = tile::kGrouped<TO>;
-    d.W[0] = w_t, d.ldw = 2 * Fp * e;
-    d.M = M, d.N = d.limit = (int)C;
-    d.out = dx, d.ldo = C;
-    d.vec = whole_rows(dx, C, e);
-    if ((rc = product<E, TO, tile::kPlain>(d, num_cu, st))) return rc;
+  const bool in_biases = out.b_gate || out.b_up, in_weights = out.w_gate || out.w_up || (e == 4 && in_biases);
+  int rc = PA_OK;
+  bool packed = false;
+  for (int64_t r0 = 0; r0 < M; r0 += per) {
+    const int64_t rows = M - r0 < per ? M - r0 : per, done = rows_done(rows), rest = rows - done;
+    auto from = [](const void *q, int64_t row, int64_t ld) { return const_cast<char *>(static_cast<const char *>(q)) + row * ld; };
+    const void *xr = from(x, r0, C * e), *dyr = from(dy, r0, C * e);
+    if (copy_x) lay.add(xr, C, room.x, rows, C, Cp, Cp, false), xr = room.x;
+    if (copy_dy) lay.add(dyr, C, room.dy, rows, C, Cp, Cp, false), dyr = room.dy;
+    if ((rc = tile::lay_out(lay, e, st))) return rc;
+    lay = Layout{};  // the weights with the first piece
+    float *piece_sums = e == 2 ? sums + r0 / 32 * 2 * Fp : nullptr;
+    if (done > 0) {
+      if (!packed) rc = hidden_pack(C, F, p, blob, st);
+      packed = true;
+      if (!rc) rc = rows_hidden_backward(done, Cp, F, Fp, blob, act, xr, dyr, room.dgu, room.h, piece_sums, num_cu, st);
+      if (rc) return rc;
+    }
+    if (rest > 0) {
+      Args a{};
+      a.X = from(xr, done, Cp * e), a.ldx = Cp * e, a.units = (int)(Cp * e / 16);
+      a.X2 = from(dyr, done, Cp * e), a.ldx2 = Cp * e, a.units2 = a.units;
+      a.W[0] = wg.p, a.W[1] = wu.p, a.W[2] = wd_t, a.ldw = wg.ld, a.ldw2 = Cp * e;
+      a.M = rest, a.N = (int)F, a.limit = (int)Fp;
+      a.bias[0] = p.b_gate, a.bias[1] = p.b_up;
+      a.sums = e == 2 && in_biases ? piece_sums + done / 32 * 2 * Fp : nullptr;
+      a.out = from(room.dgu, done, 2 * Fp * e), a.ldo = 2 * Fp, a.out2 = from(room.h, done, Fp * e), a.ldh = Fp, a.act = act;
+      if ((rc = product<E, TO, tile::kBack>(a, num_cu, st))) return rc;
+    }
+    if (dx) {
+      Args d{};
+      d.X = room.dgu, d.ldx = 2 * Fp * e, d.units = (int)(2 * Fp * e / 16), d.x_groups = tile::kGrouped<TO>;
+      d.W[0] = w_t, d.ldw = 2 * Fp * e;
+      d.M = rows, d.N = d.limit = (int)C;
+      d.out = from(dx, r0, C * e), d.ldo = C;
+      d.vec = whole_rows(d.out, C, e);
+      if ((rc = product<E, TO, tile::kPlain>(d, num_cu, st))) return rc;
+    }
+    if (in_weights && (rc = rows_product<E>(room.in, room.dgu, xr, rows, 1, num_cu, st))) return rc;
+    if ((out.w_down || out.b_down) && (rc = rows_product<E>(room.down, dyr, room.h, rows, 2, num_cu, st))) return rc;
   }
   Totals totals;
-  const bool in_biases = out.b_gate || out.b_up;
-  if (out.w_gate || out.w_up || (e == 4 && in_biases)) {
-    if ((rc = rows_product<E>(in, dgu, 2 * Fp, xr.p, Cp, M, 1, num_cu, st))) return rc;
+  const Partials &in = room.in, &down = room.down;
+  if (in_weights) {
     totals.add(in.product, in.G, 2 * Fp * Cp, Cp, out.w_gate, F, C, e);
     totals.add(in.product + Fp * Cp, in.G, 2 * Fp * Cp, Cp, out.w_up, F, C, e);
   }
@@ -400,7 +448,6 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
     totals.add(db + Fp, e == 2 ? parts : in.G, 2 * Fp, F, out.b_up, 1, F, 4);
   }
   if (out.w_down || out.b_down) {
-    if ((rc = rows_product<E>(down, dyr.p, Cp, h, Fp, M, 2, num_cu, st))) return rc;
     totals.add(down.product, down.G, Cp * Fp, Fp, out.w_down, C, F, e);
     totals.add(down.sums, down.G, Cp, C, out.b_down, 1, C, 4);
   }

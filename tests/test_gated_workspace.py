@@ -42,3 +42,22 @@ def test_few_rows(lib):
         for C, F in ((64, 96), (256, 1024), (512, 1365), (257, 100)):
             for dtype, e in ((BF16, 2), (F32, 4)):
                 assert lib.pa_gated_mlp_workspace_bytes(dtype, rows, C, F) >= rows * (C + F) * e
+
+
+@pytest.mark.parametrize("dtype,C,F", [(BF16, 256, 1024), (BF16, 512, 1365), (BF16, 64, 64), (F32, 128, 512), (F32, 64, 40)])
+def test_the_backward_of_rows_of_whole_units_has_no_room_for_copies(lib, dtype, C, F):
+    """dg, du and h, a 32nd of two of them in float32 for the bias gradients (bf16), and partial weight gradients: at most two per CU
+    of 3 F C float32 values, in float32 for each of the pieces that rows off a boundary run in."""
+    e = 2 if dtype == BF16 else 4
+    group = 32 // e  # the hidden layer's columns come in 32 bytes
+    Fp = (F + group - 1) // group * group
+    for rows in (1 << 18, 1 << 20, 1 << 22):
+        hidden = rows * 3 * Fp * e + (rows // 32 * 2 * Fp * 4 if dtype == BF16 else 0)
+        need = lib.pa_gated_mlp_backward_workspace_bytes(dtype, rows, C, F)
+        assert hidden <= need
+        weights = 6 * (C + 32) * (Fp + 64) * e + (Fp * 2 * 4 * 64) + MB
+        pieces = 1 if dtype == BF16 else (3 * Fp + 2 * C) // (3 * Fp) + 2
+        assert need - hidden <= weights + pieces * 512 * (3 * Fp * C + 2 * Fp + C) * 4
+    grows = [lib.pa_gated_mlp_backward_workspace_bytes(dtype, rows, C, F) for rows in (1 << 24, 1 << 25)]
+    per_row = (grows[1] - grows[0]) / (1 << 24)
+    assert per_row <= 1.001 * (3 * Fp * e + (2 * Fp * 4 / 32 if dtype == BF16 else 0)) + 1

@@ -34,7 +34,8 @@ def call(x, params, residual, y):
 
 
 @pytest.mark.parametrize("rows,C,F,dtype", [(70_001, 64, 96, torch.bfloat16), (32_768, 72, 40, torch.bfloat16), (65_537, 32, 33, torch.bfloat16),
-                                            (33_000, 264, 72, torch.bfloat16), (40_000, 36, 50, torch.float32), (500, 256, 64, torch.bfloat16)])
+                                            (33_000, 264, 72, torch.bfloat16), (40_000, 36, 50, torch.float32), (500, 256, 64, torch.bfloat16),
+                                            (140_000, 64, 16, torch.bfloat16)])
 def test_rows_off_a_boundary(rows, C, F, dtype):
     announce("gated views", rows, C, F, dtype)
     st = make(rows, C, F, dtype, seed=rows)
@@ -54,6 +55,34 @@ def test_rows_off_a_boundary(rows, C, F, dtype):
     out = torch.zeros_like(x)
     call(x, params, residual, out)
     check(out, values[0], tols[0], "on boundaries")
+
+
+@pytest.mark.parametrize("rows,C,F,dtype", [(70_001, 64, 96, torch.bfloat16), (65_537, 32, 33, torch.bfloat16), (33_000, 264, 72, torch.bfloat16),
+                                            (40_000, 36, 50, torch.float32), (500, 256, 64, torch.bfloat16), (140_000, 64, 16, torch.bfloat16),
+                                            (90_000, 256, 256, torch.bfloat16)])
+def test_gradients_of_rows_off_a_boundary(rows, C, F, dtype):
+    """x, dy or both; the result's place as well; every gradient, and the biases' alone."""
+    announce("gated views, gradients", rows, C, F, dtype)
+    st = make(rows, C, F, dtype, seed=rows)
+    values, tols = derived(st, "silu", dtype)
+    gpu = on_gpu(st)
+    params = [gpu[n] for n in NAMES]
+    for xs, ys in ((shifted(gpu["x"]), gpu["dy"]), (gpu["x"], shifted(gpu["dy"])), (shifted(gpu["x"]), shifted(gpu["dy"]))):
+        got = PF.gated_mlp_backward(xs, ys, *params[:5])
+        for what, g, v, t in zip(("dx",) + NAMES, got, values[1:], tols[1:]):
+            check(g, v, t, what)
+    some = PF.gated_mlp_backward(xs, ys, *params[:5], wanted=(False, False, True, False, True, False, True))
+    assert all(torch.equal(some[k], got[k]) for k in (2, 4, 6)) and [g is None for g in some] == [True, True, False, True, False, True, False]
+    lib, code, guard = _lib.load(), _lib.dtype_code(dtype), 4096
+    nbytes = lib.pa_gated_mlp_backward_workspace_bytes(code, rows, C, F)
+    ws = torch.full((nbytes + guard,), 77, dtype=torch.uint8, device="cuda")
+    dx = shifted(torch.zeros_like(gpu["x"]))
+    p, grads = _lib.PaGatedParams(*map(_lib.ptr, params)), _lib.PaGatedGrads()
+    _lib.check(lib.pa_gated_mlp_backward(code, rows, C, F, ctypes.byref(p), _lib.ACTS["silu"], xs.data_ptr(), ys.data_ptr(), dx.data_ptr(),
+                                         ctypes.byref(grads), ws.data_ptr(), nbytes, _lib.current_stream_ptr(dx.device)), "pa_gated_mlp_backward")
+    check(dx, values[1], tols[1], "dx alone, off a boundary")
+    torch.cuda.synchronize()
+    assert bool((ws[nbytes:] == 77).all())
 
 
 def test_an_on_chip_call_takes_little_memory():
