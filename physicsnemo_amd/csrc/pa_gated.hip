@@ -10,6 +10,8 @@
 //
 // Operands whose rows are not whole 16-byte units (odd widths, views off a boundary) are copied to padded rows first, with the
 // transposed weights of the backward pass in the same launch.
+#include <algorithm>
+
 #include "pa_common.h"
 #include "pa_host.h"
 #include "pa_tile.h"
@@ -207,9 +209,10 @@ static int product(const Args &a, int num_cu, hipStream_t st) {
 
 // The forward's workspace: packed weights of the kernel that keeps the hidden layer on chip, h of the rows that the tile kernels
 // take, and padded copies of what is not laid out in whole units.  The query does not know the pointers.  Rows whose width is
-// whole units are off a boundary only as views are, and then run in pieces of kLooseRows rows, so that no call has to bring
-// room for copies of all rows, or for the hidden layer of rows that have it on chip.  (262 144 x 256, F = 1 024, bf16: 87 MB instead of
-// 674; of rows off a boundary a piece costs two or three launches.)
+// whole units are off a boundary only as views are, and then run in pieces, so that no call has to bring room for copies of all
+// rows, or for the hidden layer of rows that have it on chip: of kLooseRows rows for widths that keep it there (262 144 x 256, F = 1 024,
+// bf16: 87 MB instead of 674; off a boundary 627 -> 676 us), else of the multiple of it whose copies and hidden layer fit what all
+// rows' hidden layer takes (100 003 x 512, F = 1 365, bf16: 279 MB instead of 382; 550 -> 547 us; in equal halves 611).
 static constexpr int64_t kLooseRows = 32768;
 
 template <class E, class TO>
@@ -233,7 +236,8 @@ static int forward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, in
     h = s.take(up(rows, tile::kGroupRows) * Fp * e);
     copy = copies ? s.take(rows * Cp * e) : nullptr;
   };
-  const int64_t piece = M < kLooseRows ? M : kLooseRows, per = loose && (on_chip || copy_x) ? piece : M - done;
+  const int64_t piece = M <= kLooseRows ? M : std::max<int64_t>(on_chip ? 1 : M * Fp / (Fp + Cp) / kLooseRows, 1) * kLooseRows;
+  const int64_t per = loose && (on_chip || copy_x) ? piece : M - done;
   void *h, *copy;
   if (plan) {
     Space pieces = ws;
@@ -293,24 +297,22 @@ int forward(int dtype, int64_t M, int64_t C, int64_t F, const pa_gated_params &p
   return forward<tile::Bf16, bf16>(M, C, F, p, act, x, residual, y, ws, nullptr, num_cu, st);
 }
 
-// partial results of a row-axis product of `oa` by `ob` columns, and of the column sums of its first operand: of `rows` of a
-// call's M rows, bf16 their share of the call's
+// partial results of a row-axis product of `oa` by `ob` columns, and of the column sums of its first operand
 template <class E>
-static int64_t chunks_of(int64_t rows, int64_t M, int64_t oa, int64_t ob, int num_cu) {
+static int64_t chunks_of(int64_t rows, int64_t oa, int64_t ob, int num_cu) {
   if (E::kBytes == 4) return gemm::cols_gemm_f32_chunks(rows, oa, ob, num_cu);
-  const int64_t all = wgrad::chunks_for(M, ((oa + 255) / 256) * ((ob + 255) / 256), oa * ob, num_cu), share = rows == M ? all : all * rows / M;
-  return share < 1 ? 1 : share;
+  return wgrad::chunks_for(rows, ((oa + 255) / 256) * ((ob + 255) / 256), oa * ob, num_cu);
 }
 struct Partials {
-  int64_t G = 0, M = 0, oa = 0, ob = 0;  // G: how many there are so far
+  int64_t G = 0, oa = 0, ob = 0;  // G: how many there are so far
   float *product = nullptr, *sums = nullptr;
 };
 template <class E>
 static Partials partials_of(int64_t M, int64_t rows, int64_t oa, int64_t ob, int num_cu, Space &ws) {
-  int64_t most = 0;
-  for (int64_t r0 = 0; r0 < M; r0 += rows) most += chunks_of<E>(M - r0 < rows ? M - r0 : rows, M, oa, ob, num_cu);
+  const int64_t before = (M - 1) / rows;  // pieces before the last one
+  const int64_t most = (before > 0 ? before * chunks_of<E>(rows, oa, ob, num_cu) : 0) + chunks_of<E>(M - before * rows, oa, ob, num_cu);
   Partials r;
-  r.M = M, r.oa = oa, r.ob = ob;
+  r.oa = oa, r.ob = ob;
   r.product = static_cast<float *>(ws.take(most * oa * ob * 4));
   r.sums = static_cast<float *>(ws.take(most * oa * 4));
   return r;
@@ -319,16 +321,16 @@ template <class E>
 static int rows_product(Partials &r, const void *A, const void *B, int64_t rows, int groups, int num_cu,
                         hipStream_t st) {  // groups: 1 if A, 2 if B is a matrix of the hidden layer
   float *product = r.product + r.G * r.oa * r.ob, *sums = r.sums + r.G * r.oa;
-  const int64_t G = chunks_of<E>(rows, r.M, r.oa, r.ob, num_cu);
+  const int64_t G = chunks_of<E>(rows, r.oa, r.ob, num_cu);
   r.G += G;
   if (E::kBytes == 2) return wgrad::launch_wide(A, r.oa, r.oa, B, r.ob, r.ob, rows, G, nullptr, product, groups == 1 ? nullptr : sums, st, groups);
   return gemm::cols_gemm_f32(A, r.oa, r.oa, B, r.ob, r.ob, rows, nullptr, product, sums, num_cu, st);
 }
 
 // The backward's workspace: dg and du, h, transposed weights, partial weight gradients, and copies of what is not laid out in whole
-// units.  As in the forward, x and dy off a boundary run in pieces: as many rows each as leave room for their copies beside the
-// piece's hidden layer in what a call on boundaries needs for all rows (131 072 x 256, F = 1 024, bf16: 978 MB instead of 1 112;
-// 1 048 576 x 256, F = 256: 1 814 instead of 2 887).
+// units.  As in the forward, x and dy off a boundary run in pieces, as few as leave room for their copies beside a piece's
+// hidden layer, and for partial gradients of their own, in what a call on boundaries needs (131 072 x 256, F = 1 024, bf16: 978 MB
+// instead of 1 112; 1 048 576 x 256, F = 256: 1 814 instead of 2 887; off a boundary 262 144 x 256, F = 1 024: 1 690 -> 1 787 us).
 struct BackwardRoom {
   void *dgu, *h, *x, *dy;
   Partials in, down;
@@ -353,15 +355,21 @@ static int backward(int64_t M, int64_t C, int64_t F, const pa_gated_params &p, i
   Layout lay;
   const int64_t Cp = up(C < LEAST ? LEAST : C, U), Fp = up(F < LEAST ? LEAST : F, 32 / e);
   const bool whole = C == Cp, copy_x = !whole || !aligned16(x), copy_dy = !whole || !aligned16(dy);
-  // rows of a piece: all of them, or of x and dy off a boundary
-  int64_t piece = M * 3 * Fp / (3 * Fp + 2 * Cp) / tile::kGroupRows * tile::kGroupRows;
-  if (piece < kLooseRows) piece = M < kLooseRows ? M : kLooseRows;
-  const int64_t per = whole && !plan && (copy_x || copy_dy) ? piece : M;
-  Space loose = ws;
-  BackwardRoom room = backward_room<E>(M, per, Cp, Fp, copy_x, copy_dy, num_cu, ws);
-  if (plan && whole) {
-    backward_room<E>(M, piece, Cp, Fp, true, true, num_cu, loose);
-    if (loose.used > ws.used) ws.used = loose.used;
+  auto need = [&](int64_t rows, bool copies) {
+    Space s{nullptr};
+    backward_room<E>(M, rows, Cp, Fp, copies, copies, num_cu, s);
+    return s.used;
+  };
+  int64_t per = M;  // rows of a piece: all of them, or of x and dy off a boundary
+  if (whole && (plan || copy_x || copy_dy) && M > kLooseRows) {
+    const int64_t most = need(M, false);
+    for (int64_t n = 2; n == 2 || (per > kLooseRows && need(per, true) > most); n += n / 2) per = up((M + n - 1) / n, kLooseRows);
+  }
+  Space aligned = ws;
+  BackwardRoom room = backward_room<E>(M, per, Cp, Fp, whole && plan ? true : copy_x, whole && plan ? true : copy_dy, num_cu, ws);
+  if (plan) {
+    backward_room<E>(M, M, Cp, Fp, copy_x, copy_dy, num_cu, aligned);
+    if (aligned.used > ws.used) ws.used = aligned.used;
   }
   // rows of the kernel that owns them, which has the weights in an order of its own
   const bool by_rows = e == 2 && rows_supported(Cp, F);
