@@ -17,6 +17,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as PF
+from . import versions
 from .autograd import SliceTokensFunction
 from .physics_attention import _kernel_layout
 
@@ -56,7 +57,7 @@ class _SliceToContextMixin:
         named += [("in_project_slice_weight", self.in_project_slice.weight, False),
                   ("in_project_slice_bias", self.in_project_slice.bias, False),
                   ("temperature", self.temperature, False)]
-        stamp = (dtype, device) + tuple((p.data_ptr(), p._version, p.dtype) for _, p, _ in named)
+        stamp = (dtype, device) + versions.stamp(*(p for _, p, _ in named))
         if self._kernel_param_cache.get("stamp") == stamp:
             return self._kernel_param_cache["params"]
         with torch.no_grad():

@@ -10,6 +10,7 @@ import torch.nn as nn
 from . import _lib
 from . import autograd as PA
 from . import functional as PF
+from . import versions
 
 __all__ = ["GatedMlp", "CounterDropout"]
 
@@ -144,8 +145,8 @@ class Int8Mlp:
     """8-bit weights of a block's Mlp or GatedMlp, made once per parameter set, and the MLP on them.  A GatedMlp's hidden layer goes
     from float32 to codes; an Mlp is two Linears, between which it is rounded to the rows' type.
 
-    A set is told by its parameters' addresses, versions and types, and holds the parameters, so that no address comes twice.  A
-    write through `.data` changes none of the three: `refresh` after it.  The codes are complete before the call that makes
+    A set is told by its parameters (`versions.stamp`) and holds them, so that no address comes twice.  Writes through `.data` or by
+    a replayed graph are not noticed: `refresh` after them.  The codes are complete before the call that makes
     them returns, for streams and captures that use them later; a set that a capture meets unmade is made in the graph, on
     every replay, and not kept; one that a graph reads stays allocated (`of_graphs`).  Copies start without codes."""
 
@@ -181,7 +182,7 @@ class Int8Mlp:
 
     def _of(self, lins, device):
         params = [p for lin in lins for p in (lin.weight, lin.bias)]
-        stamp = (device,) + tuple(None if p is None else (p.data_ptr(), p._version, p.dtype) for p in params)
+        stamp = (device,) + versions.stamp(*params)
         if torch.cuda.current_device() != device.index:
             with torch.cuda.device(device):
                 return self._of_current_device(lins, device, params, stamp)

@@ -23,6 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as PF
+from . import versions
 from .autograd import FlareFunction
 from .transolver import Transolver, TransolverBlock, block_mlp
 
@@ -49,7 +50,7 @@ class FLARE(nn.Module):
         """The composed GEMM weights (in `dtype`; biases float32) and out_linear, cached per parameter version."""
         ps = [self.q_global, self.in_project_x.weight, self.in_project_x.bias, self.self_k.weight, self.self_k.bias,
               self.self_v.weight, self.self_v.bias, self.out_linear.weight, self.out_linear.bias]
-        stamp = (dtype, device) + tuple((p.data_ptr(), p._version) for p in ps)
+        stamp = (dtype, device) + versions.stamp(*ps)
         if self._cache.get("stamp") == stamp:
             return self._cache["params"]
         H, D, S, C = self.heads, self.dim_head, self.n_global_queries, self.dim

@@ -19,6 +19,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as PF
+from . import versions
 from .autograd import (LayerResidualFunction, LayerResidualNormFunction, PhysicsAttentionFunction, PhysicsAttentionMfmaFunction,
                        PhysicsAttentionPlusFunction, PhysicsAttentionPlusMfmaFunction, _aligned, unhooked)
 from .feedforward import CounterDropout
@@ -118,7 +119,7 @@ class PhysicsAttentionBase(nn.Module):
         named = [(name, _parameter(module, attr), attr == "weight" and name in _LARGE)
                  for name, module, attr in self._layer_parameters()]
         fp8 = self.fp8_weights and dtype == torch.bfloat16
-        stamp = (dtype, device, fp8) + tuple((p.data_ptr(), p._version, p.dtype) for _, p, _ in named)
+        stamp = (dtype, device, fp8) + versions.stamp(*(p for _, p, _ in named))
         hit = self._kernel_param_cache.get("stamp")
         if hit == stamp:
             return self._kernel_param_cache["params"]

@@ -22,6 +22,7 @@ import torch.nn as nn
 from . import autograd as PA
 from . import checkpoint as _ckpt
 from . import functional as PF
+from . import versions
 from .feedforward import GATED_ACTS, CounterDropout, GatedMlp, Int8Mlp, counter_dropout, plain_act
 from .physics_attention import (PhysicsAttentionBase, PhysicsAttentionIrregularMesh, PhysicsAttentionStructuredMesh2D,
                                 PhysicsAttentionStructuredMesh3D)
@@ -59,7 +60,7 @@ class Mlp(nn.Module):
         """Both weights in the activation dtype and both biases in float32, cached until a parameter changes."""
         lin1, lin2 = self.layers[0], self.layers[2]
         named = (lin1.weight, lin1.bias, lin2.weight, lin2.bias)
-        stamp = (dtype, device) + tuple((t.data_ptr(), t._version, t.dtype) for t in named)
+        stamp = (dtype, device) + versions.stamp(*named)
         cache = self.__dict__.setdefault("_kernel_cache", {})
         if cache.get("stamp") != stamp:
             with torch.no_grad():
@@ -166,8 +167,8 @@ class TransolverBlock(nn.Module):
     def use_int8_mlp(self, enabled: bool = True):
         """Inference with the MLP's products in 8 bits: weights rounded to int8 with one scale per output channel, once per
         parameter set, and the rows on their way in with one scale each (`functional.linear_int8`, `gated_mlp_int8`); bfloat16
-        and float32 rows on the GPU.  Training runs as without it.  Called again it rounds the weights again, which a write
-        through `.data` asks for; other writes are noticed.  No counterpart in the reference."""
+        and float32 rows on the GPU.  Training runs as without it.  Called again it rounds the weights again, which writes
+        through `.data` and by a replayed graph ask for; others are noticed.  No counterpart in the reference."""
         if enabled and self.fp8_weights:
             raise ValueError("the block's MLP holds fp8 weights; use_fp8_weights(False) first")
         if enabled and Int8Mlp.linears(self.ln_mlp1[1]) is None:
@@ -198,7 +199,7 @@ class TransolverBlock(nn.Module):
         cached until a parameter changes.  With fp8 weights enabled the bf16 values are the dequantised e4m3 weights."""
         lin1, lin2 = self.ln_mlp1[1].layers[0], self.ln_mlp1[1].layers[2]
         named = (lin1.weight, lin1.bias, lin2.weight, lin2.bias)
-        stamp = (device, dtype, self.fp8_weights) + tuple((t.data_ptr(), t._version, t.dtype) for t in named)
+        stamp = (device, dtype, self.fp8_weights) + versions.stamp(*named)
         if self._mlp_cache.get("stamp") != stamp:
             def big(w):
                 w = w.detach().to(device=device, dtype=torch.float32)
@@ -496,7 +497,7 @@ class Transolver(nn.Module):
 
     def _library_linear(self, x: torch.Tensor, lin: nn.Linear, gelu: bool = False) -> torch.Tensor:
         cache = self.__dict__.setdefault("_linear_cache", {})
-        stamp = (x.dtype, x.device, lin.weight.data_ptr(), lin.weight._version, lin.bias.data_ptr(), lin.bias._version)
+        stamp = (x.dtype, x.device) + versions.stamp(lin.weight, lin.bias)
         hit = cache.get(id(lin))
         if hit is None or hit[0] != stamp:
             with torch.no_grad():
@@ -509,7 +510,7 @@ class Transolver(nn.Module):
         """The preprocess Mlp's weights in the activation dtype and its biases in float32, cached until one changes."""
         lin1, lin2 = self.preprocess.layers[0], self.preprocess.layers[2]
         named = (lin1.weight, lin1.bias, lin2.weight, lin2.bias)
-        stamp = (dtype, device) + tuple((t.data_ptr(), t._version, t.dtype) for t in named)
+        stamp = (dtype, device) + versions.stamp(*named)
         cache = self.__dict__.setdefault("_preprocess_cache", {})
         if cache.get("stamp") != stamp:
             with torch.no_grad():

@@ -166,3 +166,17 @@ def test_counters_do_not_move_inside_a_capture(monkeypatch):
     with pytest.raises(RuntimeError, match="before the capture"):
         drop._next(rows)
     assert drop.state.tolist() == [3, 0]
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_codes_follow_an_optimiser(on_cpu, fused):
+    """Fused optimisers write parameters without a new version."""
+    mlp, codes = pn.GatedMlp(8, 12), Int8Mlp()
+    optimizer = torch.optim.AdamW(mlp.parameters(), lr=0.1, fused=fused)
+    for _ in range(3):
+        codes._of(mlp.linears(), CPU)
+        for p in mlp.parameters():
+            p.grad = torch.randn_like(p)
+        optimizer.step()
+        for (q, s, _), lin in zip(codes._of(mlp.linears(), CPU), mlp.linears()):
+            assert torch.equal(s, lin.weight.detach().abs().amax(-1) / 127)
