@@ -971,7 +971,8 @@ __global__ __launch_bounds__(512) void few_rows_kernel(Args a) {
 // / few rows:
 // bf16 2 048 -> 512, 64 rows 17.9 / 8.8, 1 000 (two rounds) 18.0 / 17.1, 1 500 17.8 / 25.0; 512 -> 2 x 2 048, 64 rows 6.5 / 6.9;
 // float32 2 048 -> 512, 64 rows 75.6 / 21.9, 1 500 77.6 / 68.5, 2 000 77.9 / 89.3, 512 -> 2 x 2 048, 64 rows 21.6 / 10.1, 400 32.7 /
-// 36.4; int8 512 -> 2 048, 64 rows 6.0 / 4.3, 400 6.3 / 9.5, 2 048 -> 512, 64 rows 11.0 / 7.6, 600 11.3 / 12.3.
+// 36.4; int8 512 -> 2 048, 64 rows 6.0 / 4.3, 400 6.3 / 9.5, 2 048 -> 512, 64 rows 11.0 / 7.6, 600 11.3 / 12.3.  The 8-bit gated pair has
+// no such form: its codes need the largest value of a whole row first.
 inline bool few_rows_worth(int bytes, Kind kind, int64_t M, int64_t N, int64_t row_units, int64_t stages, int num_cu) {
   if (kind != kPlain && !(kind == kGated && bytes != 1)) return false;
   const double step = bytes == 4 ? 1.2 : 0.4;  // of a tile's stage and of a wave's step alike
