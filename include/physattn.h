@@ -762,6 +762,78 @@ int64_t pa_int8_gated_workspace_bytes(int dtype, int64_t rows, int64_t C, int64_
 int pa_int8_gated(int dtype, int64_t rows, int64_t C, int64_t F, const pa_int8_gated_params *p, int act, const void *x,
                   const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- attention of points over their neighbours in an order of the points (no reference counterpart) -------------------- */
+
+/* Rows of heads: element (b, n, h, d) lies at data + b * batch + n * row + h * head + d, strides in elements, not negative (0 for
+ * a broadcast input).  Inputs may start on any element boundary and overlap; outputs are contiguous (B, N, heads, D). */
+typedef struct pa_heads {
+  const void *data;
+  int64_t batch, row, head;
+} pa_heads;
+
+/* Queries and keys normalised and turned: u = x (mean_d x^2 + eps)^(-1/2) weight, then pair p of u's channels, (a, b), becomes
+ * (a cos t - b sin t, a sin t + b cos t), t = sum_a positions[b, n, a] frequencies[a, p] (rounded only once it is within one turn).
+ * Pairs: (p, p + rotated / 2), with `interleaved` (2 p, 2 p + 1); channels behind `rotated` are not turned. */
+#define PA_POS_I32 0
+#define PA_POS_I64 1
+#define PA_POS_F32 2
+#define PA_MAX_AXES 8
+typedef struct pa_rotate_params {
+  int64_t B, N, Hq, Hk, D;   /* D up to PA_MAX_D */
+  int64_t rotated;           /* channels that are turned: even, up to D; 0: none, positions and frequencies are not used */
+  int64_t axes;              /* numbers a position has, up to PA_MAX_AXES */
+  int64_t position_batch;    /* elements from a batch's positions to the next one's: N * axes, or 0 if shared */
+  int position_type;         /* PA_POS_* */
+  int interleaved;
+  int norm;                  /* 0: u = x, the weights are not used */
+  double eps;
+  const void *positions;     /* (B or 1, N, axes) */
+  const float *frequencies;  /* (axes, rotated / 2) */
+  const float *q_weight;     /* (D) or NULL: ones */
+  const float *k_weight;
+} pa_rotate_params;
+int pa_norm_rotate(int dtype, const pa_rotate_params *p, const pa_heads *q, const pa_heads *k, void *q_out, void *k_out, void *stream);
+/* Its gradients from those of the results, d_q and d_k, and the inputs: dq, dk (contiguous, in dtype), d weights (D) float32, each NULL if not wanted.
+ * Sums in a fixed order. */
+int64_t pa_norm_rotate_backward_workspace_bytes(int dtype, const pa_rotate_params *p);
+int pa_norm_rotate_backward(int dtype, const pa_rotate_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *d_q,
+                            const pa_heads *d_k, void *dq, void *dk, float *d_q_weight, float *d_k_weight, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
+/* y_i = sum_j p_ij v_j, p_i the softmax over the visible j of scale q_i . k_j + bias[bucket(j - i), head], for points i of a sequence:
+ * j is visible to i if j <= i + right and (j >= i - left or j < sinks) and both lie in the sequence.  Query head h reads key head
+ * h / (Hq / Hk).  A row that sees nothing, or only scores of -inf, is zero, and so are its gradients.
+ * Buckets of the distance d = |j - i|, n = buckets of them for j <= i where right is 0; else n = buckets / 2 for j <= i and as many for j > i
+ * behind them.  With E = n / 2: d < E has bucket d, others E + the largest b < n - E with d >= E (distance / E)^(b / (n - E)). */
+#define PA_MAX_WINDOW_N (1ll << 29)
+#define PA_MAX_SINKS 128
+#define PA_MAX_BUCKETS 256
+#define PA_MAX_DISTANCE 2048
+typedef struct pa_window_params {
+  int64_t B, N, Hq, Hk, D; /* D up to PA_MAX_D; Hk divides Hq */
+  int64_t left, right;     /* PA_NO_BOUND or at least 0 */
+  int64_t sinks;
+  int64_t buckets, distance; /* buckets 0: no bias */
+  double scale;              /* positive */
+  const int32_t *lengths;    /* (B) points of each sequence, held to 0 .. N; NULL: N.  Rows behind them are not read, and zero in results */
+  const float *bias;         /* (buckets, Hq) */
+} pa_window_params;
+#define PA_NO_BOUND (-1)
+/* stats: (B, Hq, N) float32 for the backward pass, log2 of the softmax's denominators, or NULL. */
+int pa_window_attention(int dtype, const pa_window_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *v, void *y,
+                        float *stats, void *stream);
+/* Its gradients from dy, the inputs, y and stats: dq, dk, dv (contiguous, in dtype), d_bias (buckets, Hq) float32 or NULL.  Sums in a fixed order. */
+int64_t pa_window_attention_backward_workspace_bytes(int dtype, const pa_window_params *p, int want_bias);
+int pa_window_attention_backward(int dtype, const pa_window_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *v,
+                                 const void *y, const float *stats, const pa_heads *dy, void *dq, void *dk, void *dv, float *d_bias,
+                                 void *workspace, int64_t workspace_bytes, void *stream);
+/* The newest T points of each sequence over the keys and values of all its points so far, their own among them: p->N rows of k and v
+ * per sequence, lengths of which are points (needed here); q and y (B, T, Hq, D), query t the point lengths - T + t (before the first: a row of zeros); p->right = 0.
+ * Reads what the window leaves visible, nothing else. */
+int64_t pa_window_attention_step_workspace_bytes(int dtype, const pa_window_params *p, int64_t T);
+int pa_window_attention_step(int dtype, const pa_window_params *p, int64_t T, const pa_heads *q, const pa_heads *k, const pa_heads *v,
+                             void *y, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- whole layer ------------------------------------------------------------------------------ */
 
 /* Replaces PhysicsAttentionBase.forward (PA.py:501-558), plus=False, use_te=False, dropout off.

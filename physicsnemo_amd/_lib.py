@@ -45,6 +45,9 @@ EXPORTED = [
     "pa_mfma_project_softmax_reduce_clocked", "pa_weight_grad_workspace_bytes", "pa_weight_grad",
     "pa_gated_mlp_workspace_bytes", "pa_gated_mlp_forward", "pa_gated_mlp_backward_workspace_bytes", "pa_gated_mlp_backward",
     "pa_gated_mlp_rows_on_chip", "pa_product_launches",
+    "pa_norm_rotate", "pa_norm_rotate_backward_workspace_bytes", "pa_norm_rotate_backward",
+    "pa_window_attention", "pa_window_attention_backward_workspace_bytes", "pa_window_attention_backward",
+    "pa_window_attention_step_workspace_bytes", "pa_window_attention_step",
     "pa_dropout_add_norm", "pa_dropout_add_norm_backward_workspace_bytes", "pa_dropout_add_norm_backward", "pa_dropout_advance",
     "pa_int8_quantize_rows", "pa_int8_linear_workspace_bytes", "pa_int8_linear", "pa_int8_gated_workspace_bytes", "pa_int8_gated",
 ]
@@ -101,6 +104,21 @@ class PaGatedParams(Structure):
 
 class PaGatedGrads(Structure):
     _fields_ = [(n, c_void_p) for n in ("w_gate", "b_gate", "w_up", "b_up", "w_down", "b_down")]
+
+
+class PaHeads(Structure):
+    _fields_ = [("data", c_void_p), ("batch", c_int64), ("row", c_int64), ("head", c_int64)]
+
+
+class PaRotateParams(Structure):
+    _fields_ = [(n, c_int64) for n in ("B", "N", "Hq", "Hk", "D", "rotated", "axes", "position_batch")] + [
+        (n, c_int) for n in ("position_type", "interleaved", "norm")] + [("eps", c_double)] + [
+        (n, c_void_p) for n in ("positions", "frequencies", "q_weight", "k_weight")]
+
+
+class PaWindowParams(Structure):
+    _fields_ = [(n, c_int64) for n in ("B", "N", "Hq", "Hk", "D", "left", "right", "sinks", "buckets", "distance")] + [
+        ("scale", c_double), ("lengths", c_void_p), ("bias", c_void_p)]
 
 
 class PaInt8GatedParams(Structure):
@@ -371,6 +389,23 @@ def load() -> ctypes.CDLL:
     lib.pa_int8_linear.argtypes = rows3 + [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int64, c_void_p]
     lib.pa_int8_gated.restype = c_int
     lib.pa_int8_gated.argtypes = rows3 + [POINTER(PaInt8GatedParams), c_int] + [c_void_p] * 4 + [c_int64, c_void_p]
+    heads, pr, pw = POINTER(PaHeads), POINTER(PaRotateParams), POINTER(PaWindowParams)
+    lib.pa_norm_rotate.restype = c_int
+    lib.pa_norm_rotate.argtypes = [c_int, pr, heads, heads] + [c_void_p] * 3
+    lib.pa_norm_rotate_backward_workspace_bytes.restype = c_int64
+    lib.pa_norm_rotate_backward_workspace_bytes.argtypes = [c_int, pr]
+    lib.pa_norm_rotate_backward.restype = c_int
+    lib.pa_norm_rotate_backward.argtypes = [c_int, pr] + [heads] * 4 + [c_void_p] * 5 + [c_int64, c_void_p]
+    lib.pa_window_attention.restype = c_int
+    lib.pa_window_attention.argtypes = [c_int, pw] + [heads] * 3 + [c_void_p] * 3
+    lib.pa_window_attention_backward_workspace_bytes.restype = c_int64
+    lib.pa_window_attention_backward_workspace_bytes.argtypes = [c_int, pw, c_int]
+    lib.pa_window_attention_backward.restype = c_int
+    lib.pa_window_attention_backward.argtypes = [c_int, pw] + [heads] * 3 + [c_void_p] * 2 + [heads] + [c_void_p] * 5 + [c_int64, c_void_p]
+    lib.pa_window_attention_step_workspace_bytes.restype = c_int64
+    lib.pa_window_attention_step_workspace_bytes.argtypes = [c_int, pw, c_int64]
+    lib.pa_window_attention_step.restype = c_int
+    lib.pa_window_attention_step.argtypes = [c_int, pw, c_int64] + [heads] * 3 + [c_void_p] * 2 + [c_int64, c_void_p]
     _lib = lib
     return lib
 

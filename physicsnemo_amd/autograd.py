@@ -1093,3 +1093,68 @@ def dropout_add_norm(x, residual, p: float, rng, ln_weight=None, ln_bias=None, l
     x = x.contiguous()
     residual = None if residual is None else residual.to(x.dtype).contiguous()
     return DropoutAddNormFunction.apply(x, residual, p, rng, ln_weight, ln_bias, ln_eps)
+
+
+def _with_channels(t):
+    """`t` with its last axis contiguous, itself where it is."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+class NormRotateFunction(torch.autograd.Function):
+    """`functional.norm_rotate`, differentiable w.r.t. q, k and the weights; the backward pass forms the norms again from q and k."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved):
+        weights = [None if w is None else w.detach().float().contiguous() for w in (q_weight, k_weight)]
+        ctx.save_for_backward(q, k, *weights, positions, frequencies)
+        ctx.kind, ctx.weight_dtypes = (eps, norm, interleaved), [None if w is None else w.dtype for w in (q_weight, k_weight)]
+        return PF.norm_rotate(q, k, *weights, positions, frequencies, *ctx.kind)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_q, d_k):
+        q, k, *rest = ctx.saved_tensors
+        d_q, d_k = (_with_channels(d.to(q.dtype)) for d in (d_q, d_k))
+        dq, dk, *dw = PF.norm_rotate_backward(d_q, d_k, q, k, *rest, *ctx.kind, wanted=ctx.needs_input_grad[:4])
+        dw = [None if w is None else w.to(t) for w, t in zip(dw, ctx.weight_dtypes)]
+        return (dq, dk, *dw, None, None, None, None, None)
+
+
+def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, frequencies=None, eps: float = 1e-6, norm: bool = True,
+                interleaved: bool = False):
+    """Differentiable `functional.norm_rotate` (positions and frequencies have no gradient): weights of other types are cast, inputs whose
+    channels are not neighbours copied."""
+    for name, t in (("positions", positions), ("frequencies", frequencies)):
+        if t is not None and t.requires_grad:
+            raise ValueError(f"norm_rotate has no gradient for {name}")
+    return NormRotateFunction.apply(_with_channels(q), _with_channels(k), q_weight, k_weight, positions, frequencies, eps, norm, interleaved)
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    """`functional.window_attention`, differentiable w.r.t. q, k, v and the bias; the softmax is formed again in the backward pass from the kept
+    denominators."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, bias, lengths, window, sinks, scale, max_distance):
+        ctx.call = dict(window=window, sinks=sinks, scale=scale, max_distance=max_distance)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        bias = None if bias is None else bias.detach().float().contiguous()
+        y, stats = PF.window_attention(q, k, v, lengths=lengths, bias=bias, return_stats=True, **ctx.call)
+        ctx.save_for_backward(q, k, v, y, stats, bias, lengths)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        q, k, v, y, stats, bias, lengths = ctx.saved_tensors
+        dq, dk, dv, db = PF.window_attention_backward(_with_channels(dy.to(q.dtype)), q, k, v, y, stats, lengths=lengths, bias=bias,
+                                                      need_bias=ctx.needs_input_grad[3], **ctx.call)
+        need = ctx.needs_input_grad
+        db = None if db is None else db.to(ctx.bias_dtype)
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, db, None, None, None, None, None)
+
+
+def window_attention(q, k, v, window=(None, None), sinks: int = 0, scale: float | None = None, lengths=None, bias=None, max_distance: int = 128):
+    """Differentiable `functional.window_attention`: a bias of another type is cast, inputs whose channels are not neighbours copied."""
+    q, k, v = (_with_channels(t) for t in (q, k, v))
+    return WindowAttentionFunction.apply(q, k, v, bias, lengths, tuple(window), sinks, scale, max_distance)

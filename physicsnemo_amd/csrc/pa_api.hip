@@ -1,4 +1,5 @@
 // C ABI of libphysattn.so: argument validation, workspace carving and dispatch.  No kernels here.
+#include <initializer_list>
 #include <dlfcn.h>
 #include <stdlib.h>
 
@@ -1981,6 +1982,135 @@ int pa_dropout_add_norm_backward(int dtype, int64_t rows, int64_t C, const void 
 int pa_dropout_advance(int64_t *state, int64_t *taken, void *stream) {
   if (!state || !taken) return PA_ERR_NULL;
   return pa::dropout::advance(state, taken, static_cast<hipStream_t>(stream));
+}
+
+// rows of heads as an input: there, on an element boundary, strides not negative
+static int check_heads(int dtype, const pa_heads *h) {
+  if (!h || !h->data) return PA_ERR_NULL;
+  if (h->batch < 0 || h->row < 0 || h->head < 0) return PA_ERR_DIMS;
+  if (reinterpret_cast<uintptr_t>(h->data) % (dtype == PA_F32 ? 4 : 2) != 0) return PA_ERR_ALIGN;
+  return PA_OK;
+}
+static int check_all_heads(int dtype, std::initializer_list<const pa_heads *> all) {
+  for (const pa_heads *h : all)
+    if (int rc = check_heads(dtype, h)) return rc;
+  return PA_OK;
+}
+
+static int check_rotate(int dtype, const pa_rotate_params *p) {
+  if (!p) return PA_ERR_NULL;
+  if (dtype != PA_F32 && dtype != PA_BF16) return PA_ERR_UNSUPPORTED;
+  if (p->B <= 0 || p->N <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->D <= 0) return PA_ERR_DIMS;
+  if (p->rotated < 0 || p->rotated > p->D || p->rotated % 2 != 0) return PA_ERR_DIMS;
+  if (p->D > PA_MAX_D || p->Hq > 4096 || p->Hk > 4096 || p->B > PA_MAX_ROWS || p->N > PA_MAX_ROWS / p->B) return PA_ERR_UNSUPPORTED;
+  if (p->norm && !(p->eps >= 0.0 && p->eps < 1e30)) return PA_ERR_DIMS;
+  if (p->rotated > 0) {
+    if (p->axes <= 0 || (p->position_batch != 0 && p->position_batch != p->N * p->axes)) return PA_ERR_DIMS;
+    if (p->axes > PA_MAX_AXES || p->position_type < PA_POS_I32 || p->position_type > PA_POS_F32) return PA_ERR_UNSUPPORTED;
+    if (!p->positions || !p->frequencies) return PA_ERR_NULL;
+  }
+  return PA_OK;
+}
+
+int pa_norm_rotate(int dtype, const pa_rotate_params *p, const pa_heads *q, const pa_heads *k, void *q_out, void *k_out, void *stream) {
+  Range entry("pa_norm_rotate");
+  if (int rc = check_rotate(dtype, p)) return rc;
+  if (int rc = check_all_heads(dtype, {q, k})) return rc;
+  if (!q_out || !k_out) return PA_ERR_NULL;
+  return pa::rotate::forward(dtype, *p, *q, *k, q_out, k_out, compute_units(), static_cast<hipStream_t>(stream));
+}
+
+int64_t pa_norm_rotate_backward_workspace_bytes(int dtype, const pa_rotate_params *p) {
+  if (int rc = check_rotate(dtype, p)) return rc;
+  return pa::rotate::backward_workspace_bytes(*p, compute_units());
+}
+
+int pa_norm_rotate_backward(int dtype, const pa_rotate_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *d_q, const pa_heads *d_k,
+                            void *dq, void *dk, float *d_q_weight, float *d_k_weight, void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_norm_rotate_backward");
+  const int64_t need = pa_norm_rotate_backward_workspace_bytes(dtype, p);
+  if (need < 0) return (int)need;
+  if (int rc = check_all_heads(dtype, {q, k, d_q, d_k})) return rc;
+  if (d_q_weight || d_k_weight) {
+    if (!p->norm) return PA_ERR_UNSUPPORTED;
+    if (!workspace) return PA_ERR_NULL;
+    if (!aligned16(workspace)) return PA_ERR_ALIGN;
+    if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  }
+  return pa::rotate::backward(dtype, *p, *q, *k, *d_q, *d_k, dq, dk, d_q_weight, d_k_weight, static_cast<float *>(workspace), compute_units(),
+                              static_cast<hipStream_t>(stream));
+}
+
+static int check_window(int dtype, const pa_window_params *p) {
+  if (!p) return PA_ERR_NULL;
+  if (dtype != PA_F32 && dtype != PA_BF16) return PA_ERR_UNSUPPORTED;
+  if (p->B <= 0 || p->N <= 0 || p->Hq <= 0 || p->Hk <= 0 || p->D <= 0 || p->Hq % p->Hk != 0) return PA_ERR_DIMS;
+  if (p->left < PA_NO_BOUND || p->right < PA_NO_BOUND || p->sinks < 0 || p->buckets < 0) return PA_ERR_DIMS;
+  if (!(p->scale > 1e-30 && p->scale < 1e30)) return PA_ERR_DIMS;
+  if (p->D > PA_MAX_D || p->Hq > 4096 || p->N > PA_MAX_WINDOW_N || p->B > (1 << 24) || p->sinks > PA_MAX_SINKS) return PA_ERR_UNSUPPORTED;
+  // one workgroup per 128 rows of a head, and as many again for the first rows of each
+  if (((p->N + 127) / 128 + (p->N + 1023) / 1024) > ((1ll << 31) - 1) / (p->Hq * p->B)) return PA_ERR_UNSUPPORTED;
+  if (p->buckets > 0) {
+    const int64_t side = p->right != 0 ? p->buckets / 2 : p->buckets;
+    if (side < 2 || (p->right != 0 && p->buckets % 2 != 0) || p->distance <= side / 2) return PA_ERR_DIMS;
+    if (p->buckets > PA_MAX_BUCKETS || p->distance > PA_MAX_DISTANCE) return PA_ERR_UNSUPPORTED;
+    if (!p->bias) return PA_ERR_NULL;
+  }
+  return PA_OK;
+}
+
+int pa_window_attention(int dtype, const pa_window_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *v, void *y, float *stats,
+                        void *stream) {
+  Range entry("pa_window_attention");
+  if (int rc = check_window(dtype, p)) return rc;
+  if (int rc = check_all_heads(dtype, {q, k, v})) return rc;
+  if (!y) return PA_ERR_NULL;
+  return pa::window::forward(dtype, *p, *q, *k, *v, y, stats, static_cast<hipStream_t>(stream));
+}
+
+int64_t pa_window_attention_backward_workspace_bytes(int dtype, const pa_window_params *p, int want_bias) {
+  if (int rc = check_window(dtype, p)) return rc;
+  if (want_bias && p->buckets == 0) return PA_ERR_DIMS;
+  return pa::window::backward_workspace_bytes(dtype, *p, want_bias != 0);
+}
+
+int pa_window_attention_backward(int dtype, const pa_window_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *v, const void *y,
+                                 const float *stats, const pa_heads *dy, void *dq, void *dk, void *dv, float *d_bias, void *workspace,
+                                 int64_t workspace_bytes, void *stream) {
+  Range entry("pa_window_attention_backward");
+  const int64_t need = pa_window_attention_backward_workspace_bytes(dtype, p, d_bias != nullptr);
+  if (need < 0) return (int)need;
+  if (int rc = check_all_heads(dtype, {q, k, v, dy})) return rc;
+  if (!y || !stats || !dq || !dk || !dv || !workspace) return PA_ERR_NULL;
+  if (!aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::window::backward(dtype, *p, *q, *k, *v, y, stats, *dy, dq, dk, dv, d_bias, workspace, static_cast<hipStream_t>(stream));
+}
+
+static int check_step(int dtype, const pa_window_params *p, int64_t T) {
+  if (int rc = check_window(dtype, p)) return rc;
+  if (T <= 0 || T > p->N || p->right != 0) return PA_ERR_DIMS;
+  if (!p->lengths) return PA_ERR_NULL;
+  const int64_t G = p->Hq / p->Hk, tiles = (T * G + 31) / 32;
+  if (p->buckets * G > 16384 || T > (1 << 24) || tiles * 8 > ((1ll << 31) - 1) / (p->Hk * p->B)) return PA_ERR_UNSUPPORTED;
+  return PA_OK;
+}
+
+int64_t pa_window_attention_step_workspace_bytes(int dtype, const pa_window_params *p, int64_t T) {
+  if (int rc = check_step(dtype, p, T)) return rc;
+  return pa::window::step_workspace_bytes(dtype, *p, T, compute_units());
+}
+
+int pa_window_attention_step(int dtype, const pa_window_params *p, int64_t T, const pa_heads *q, const pa_heads *k, const pa_heads *v, void *y,
+                             void *workspace, int64_t workspace_bytes, void *stream) {
+  Range entry("pa_window_attention_step");
+  const int64_t need = pa_window_attention_step_workspace_bytes(dtype, p, T);
+  if (need < 0) return (int)need;
+  if (int rc = check_all_heads(dtype, {q, k, v})) return rc;
+  if (!y || (need > 0 && !workspace)) return PA_ERR_NULL;
+  if (need > 0 && !aligned16(workspace)) return PA_ERR_ALIGN;
+  if (workspace_bytes < need) return PA_ERR_WORKSPACE;
+  return pa::window::step(dtype, *p, T, *q, *k, *v, y, workspace, compute_units(), static_cast<hipStream_t>(stream));
 }
 
 static int check_int8(int dtype, int64_t rows, int64_t K, int64_t N) {

@@ -202,6 +202,25 @@ int backward(int dtype, int64_t M, int64_t C, const void *dy, const void *d_norm
              hipStream_t st);
 }  // namespace dropout
 
+namespace rotate {
+// queries and keys normalised and turned: see pa_norm_rotate*
+int forward(int dtype, const pa_rotate_params &p, const pa_heads &q, const pa_heads &k, void *q_out, void *k_out, int num_cu, hipStream_t st);
+int64_t backward_workspace_bytes(const pa_rotate_params &p, int num_cu);
+int backward(int dtype, const pa_rotate_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &d_q, const pa_heads &d_k, void *dq,
+             void *dk, float *d_q_weight, float *d_k_weight, float *workspace, int num_cu, hipStream_t st);
+}  // namespace rotate
+
+namespace window {
+// attention over a window and the first points: see pa_window_attention*
+int forward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, void *y, float *stats, hipStream_t st);
+int64_t backward_workspace_bytes(int dtype, const pa_window_params &p, bool want_bias);
+int backward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, const void *y, const float *stats,
+             const pa_heads &dy, void *dq, void *dk, void *dv, float *d_bias, void *workspace, hipStream_t st);
+int64_t step_workspace_bytes(int dtype, const pa_window_params &p, int64_t T, int num_cu);
+int step(int dtype, const pa_window_params &p, int64_t T, const pa_heads &q, const pa_heads &k, const pa_heads &v, void *y, void *workspace,
+         int num_cu, hipStream_t st);
+}  // namespace window
+
 namespace general {
 int dequant_e4m3(const void *in, const float *scale, void *out, int64_t rows, int64_t cols, hipStream_t st);
 int project_inputs(int dtype, const pa_shape &s, const pa_params &p, const void *x, void *x_mid, void *fx_mid,

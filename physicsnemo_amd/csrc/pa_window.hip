@@ -1,0 +1,471 @@
+// Attention of points over a window of their neighbours and a few first points, served: y_i = sum_j p_ij v_j, p_i the softmax over the
+// visible j of scale q_i . k_j (+ a bias by buckets of j - i).
+//
+// One pass over the visible keys with a running maximum and sum (in log2 units, so that a weight is one multiply-add and one exp2).
+// A wave owns 32 queries of a head, a lane one of them (with its partner 32 lanes on): the scores of a tile of keys are the rows of a
+// C tile, so that maximum and sum are per lane, and the weights go back into the product with the values as they lie.  Four waves share the
+// tiles of keys and values, two buffers in LDS, the next tile's loads under the present one's products.  Tiles that a wave's
+// queries do not see are skipped, and only tiles on an edge are masked.
+#include "pa_window.h"
+
+#include <math.h>
+
+namespace pa {
+namespace window {
+
+constexpr float kSlack = 8.f;  // log2: how far scores may rise above the reference maximum before sums are scaled again
+
+// The softmax of a wave's queries so far, and the values' sum under it
+template <int DB>
+struct Running {
+  f32x16 o[DB];
+  float m, l, off;  // reference maximum in units of z, this lane's share of the sum, -m cc (0 while nothing was seen)
+  __device__ __forceinline__ void start() {
+    zero(o);
+    m = -INFINITY, l = 0.f, off = 0.f;
+  }
+  // a tile's largest z of this lane's query: scales what is summed where it is far above the reference (for the whole wave at once)
+  __device__ __forceinline__ void raise(float most, float cc) {
+    if (!__any(most > m + kSlack / cc)) return;
+    const float now = fmaxf(m, most);
+    const float ref = now == -INFINITY ? 0.f : now;
+    const float alpha = __builtin_amdgcn_exp2f((m - ref) * cc);
+    m = now, off = -ref * cc;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+  }
+  __device__ __forceinline__ void weigh(f32x16 &z, float cc) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], cc, off));
+      sum += z[r];
+    }
+    l += sum;
+  }
+};
+
+__device__ __forceinline__ float most_of(const f32x16 &z) {
+  float m = z[0];
+#pragma unroll
+  for (int r = 1; r < 16; ++r) m = fmaxf(m, z[r]);
+  return m;
+}
+
+// bias (in log2 units, z with it) and mask of a tile of keys from k0 for the query at position i of a wave from q0
+template <bool BIAS>
+__device__ __forceinline__ void dress(const Args &a, int len, Sight sight, f32x16 &z, int q0, int i, int k0, int g, const float *table) {
+  if constexpr (BIAS) {
+    const Reach reach = reach_of(a.bias, k0 - q0 - 31, k0 + 31 - q0);
+    const int low = table_low(a.bias);
+    if (reach == kNear) {
+      const float *t = table + (k0 + 4 * g - i + low);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[8 * (r >> 2) + (r & 3)]);
+    } else {
+      const float far = reach == kFarBehind ? table[0] : table[table_size(a.bias) - 1];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+    }
+  }
+  if (sight == kSome) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = sees(a, len, i, k0 + rowmap(r, g)) ? z[r] : -INFINITY;
+  }
+}
+
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void forward_kernel(Args a) {
+  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
+  extern __shared__ u32x4 lds_raw[];
+  T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
+  float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
+  const int64_t work = own_work();
+  const int block = (int)(work % a.blocks), h = (int)(work / a.blocks % a.Hq), b = (int)(work / a.blocks / a.Hq);
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
+  using O = Ops<T, DP>;
+  Running<DP / 32> run;
+  run.start();
+  const float cc = BIAS ? 1.f : a.c;
+  if (q0 < len) {
+    const typename O::Rows own = O::rows(head_of<T>(a.q, b, h) + me * a.q.row, me < len, a.D, a.q.units, g);
+    const int hk = h / (a.Hq / a.Hk);
+    const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
+    const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
+    if constexpr (BIAS) fill_bias_table(a, h, table);
+    Stage<T, DP, KT, 256> ks, vs;
+    if (list.count > 0) {
+      ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
+      vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
+      ks.store(tiles, threadIdx.x);
+      vs.store(tiles + TILE, threadIdx.x);
+    }
+    __syncthreads();
+    for (int n = 0; n < list.count; ++n) {
+      const T *const kt = tiles + (n & 1) * 2 * TILE, *const vt = kt + TILE;
+      T *const next = tiles + ((n + 1) & 1) * 2 * TILE;
+      if (n + 1 < list.count) {
+        ks.load(a.k, keys, list[n + 1] * KT, len, a.D, threadIdx.x);
+        vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
+      }
+      const int k0 = list[n] * KT;
+      f32x16 z[SUB];
+      Sight sight[SUB];
+      float most = -INFINITY;
+      bool any = false;
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        sight[s] = sight_of(a, len, qw, k0 + 32 * s);
+        if (sight[s] == kNone) continue;
+        any = true;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[s][r] = 0.f;
+        z[s] = O::scores(kt + 32 * s * O::kStride, own, i, g, z[s]);
+        dress<BIAS>(a, len, sight[s], z[s], qw, me, k0 + 32 * s, g, table);
+        most = fmaxf(most, most_of(z[s]));
+      }
+      if (any) {
+        run.raise(half_max(most), cc);
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          if (sight[s] == kNone) continue;
+          run.weigh(z[s], cc);
+          O::outcome(vt + 32 * s * O::kStride, O::pack(z[s]), lane, run.o);
+        }
+      }
+      if (n + 1 < list.count) {
+        ks.store(next, threadIdx.x);
+        vs.store(next + TILE, threadIdx.x);
+      }
+      __syncthreads();
+    }
+  }
+  const float l = half_sum(run.l);
+  const bool some = me < len && l != 0.f;
+  T *const row = static_cast<T *>(a.y) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
+  store_rows<T, DP>(run.o, 1.f / l, some, row, me < a.N, a.D, a.out_units, g);
+  if (a.stats && g == 0 && me < a.N) a.stats[((int64_t)b * a.Hq + h) * a.N + me] = some ? log2f(l) - run.off : INFINITY;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// step: the newest T points over the cache.  The columns of a wave's tile are (new point, query head of the group) pairs that share a
+// key head; every wave of every part of the keys has tiles of its own (part + parts x n), keys straight to registers, values through a patch
+// of LDS of its own for the transposing read; waves are joined in LDS, parts by a second kernel.
+// ---------------------------------------------------------------------------------------------------------------
+// LDS accesses of a wave happen in order; this keeps the compiler from exchanging them
+__device__ __forceinline__ void wave_meets() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+struct StepArgs {
+  Args a;
+  int T, G, columns, column_tiles, parts;
+  float *part_o, *part_ml;  // [b][hk][column tile][part][32][DP], [..][32][2]
+};
+
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
+  using O = Ops<T, DP>;
+  constexpr int TILE = 32 * O::kStride, DB = DP / 32;
+  const Args &a = s.a;
+  extern __shared__ u32x4 lds_raw[];
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  T *const patch = reinterpret_cast<T *>(lds_raw) + wave * TILE;
+  float *const join = reinterpret_cast<float *>(lds_raw);              // after the last tile: [wave][column][DP]
+  float *const biases = join + (4 * TILE * sizeof(T) > 4 * 32 * DP * 4 ? TILE * sizeof(T) : 32 * DP * 4);  // [bucket][G]
+  uint8_t *const buckets = reinterpret_cast<uint8_t *>(biases + a.bias.buckets * s.G);                   // of distance 0 .. M
+  __shared__ float most_of_wave[4][32], sum_of_wave[4][32], sum_of_all[32];
+  int64_t work = blockIdx.x;
+  const int part = (int)(work % s.parts);
+  work /= s.parts;
+  const int ct = (int)(work % s.column_tiles);
+  work /= s.column_tiles;
+  const int hk = (int)(work % a.Hk), b = (int)(work / a.Hk);
+  const int len = length_of(a, b);
+  const int col = ct * 32 + i, t = col / s.G, gq = col - t * s.G, me = len - s.T + t;
+  const bool mine = col < s.columns && me >= 0;
+  const int t0 = ct * 32 / s.G, t1 = (ct * 32 + 31 < s.columns ? ct * 32 + 31 : s.columns - 1) / s.G;
+  const int first_q = len - s.T + t0 > 0 ? len - s.T + t0 : 0, last_q = len - s.T + t1;
+  const typename O::Rows own = O::rows(head_of<T>(a.q, b, hk * s.G + gq) + t * a.q.row, mine, a.D, a.q.units, g);
+  const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
+  Running<DB> run;
+  run.start();
+  const float cc = BIAS ? 1.f : a.c;
+  if constexpr (BIAS) {
+    for (int u = threadIdx.x; u < a.bias.buckets * s.G; u += 256)
+      biases[u] = bias_log2(a.bias.table[(int64_t)(u / s.G) * a.Hq + hk * s.G + u % s.G]);
+    for (int u = threadIdx.x; u <= a.bias.distance; u += 256) buckets[u] = (uint8_t)bucket_of(a.bias, u);
+    __syncthreads();
+  }
+  if (last_q >= 0) {
+    const Tiles list(a, len, first_q, last_q, 32);
+    const int by = 4 * s.parts;
+    int n = part * 4 + wave;
+    typename O::Rows next;
+    Stage<T, DP, 32, 64> vs;
+    auto fetch = [&](int at) {
+      const int k0 = list[at] * 32;
+      next = O::rows(keys + (k0 + i) * a.k.row, k0 + i < len, a.D, a.k.units, g);
+      vs.load(a.v, values, k0, len, a.D, lane);
+    };
+    if (n < list.count) fetch(n);
+    for (; n < list.count; n += by) {
+      const int k0 = list[n] * 32;
+      vs.store(patch, lane);
+      wave_meets();  // lanes read what others wrote
+      f32x16 z;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = 0.f;
+      z = O::scores(next, own, z);
+      if (n + by < list.count) fetch(n + by);
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          int d = me - (k0 + rowmap(r, g));
+          d = d < 0 ? 0 : d < a.bias.distance ? d : a.bias.distance;
+          z[r] = fmaf(z[r], a.c, biases[buckets[d] * s.G + gq]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[r] = mine && sees(a, len, me, k0 + rowmap(r, g)) ? z[r] : -INFINITY;
+      run.raise(half_max(most_of(z)), cc);
+      run.weigh(z, cc);
+      O::outcome(patch, O::pack(z), lane, run.o);
+      wave_meets();
+    }
+  }
+  // the four waves' results under one maximum
+  const float l = half_sum(run.l);
+  if (g == 0) most_of_wave[wave][i] = l != 0.f ? -run.off : -INFINITY, sum_of_wave[wave][i] = l;
+  __syncthreads();  // and all patches have been read
+  float top = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, most_of_wave[w][i]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    if (sum_of_wave[w][i] != 0.f) total += sum_of_wave[w][i] * __builtin_amdgcn_exp2f(most_of_wave[w][i] - ref);
+  const float scale = l != 0.f ? __builtin_amdgcn_exp2f(-run.off - ref) : 0.f;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) join[(wave * 32 + i) * DP + 32 * db + rowmap(r, g)] = l != 0.f ? run.o[db][r] * scale : 0.f;
+  const int64_t slot = (((int64_t)b * a.Hk + hk) * s.column_tiles + ct) * s.parts + part;
+  if (s.parts > 1 && wave == 0 && g == 0) {
+    s.part_ml[(slot * 32 + i) * 2] = top;
+    s.part_ml[(slot * 32 + i) * 2 + 1] = total;
+  }
+  if (wave == 0 && g == 0) sum_of_all[i] = total;
+  __syncthreads();
+  const int live = s.columns - ct * 32 < 32 ? s.columns - ct * 32 : 32;
+  for (int u = threadIdx.x; u < live * DP; u += 256) {
+    const int c = u / DP, d = u - c * DP;
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) o += join[(w * 32 + c) * DP + d];
+    if (s.parts > 1) {
+      s.part_o[(slot * 32 + c) * DP + d] = o;
+    } else if (d < a.D) {
+      const int column = ct * 32 + c, tt = column / s.G, hq = hk * s.G + column - tt * s.G;
+      const float sum = sum_of_all[c];
+      store_from_f32(static_cast<T *>(a.y) + (((int64_t)b * s.T + tt) * a.Hq + hq) * a.D + d, sum != 0.f ? o / sum : 0.f);
+    }
+  }
+}
+
+// joins the parts of the keys: a workgroup per (sequence, key head, column tile, four columns)
+template <class T, int DP>
+__global__ __launch_bounds__(256) void join_kernel(StepArgs s) {
+  const Args &a = s.a;
+  int64_t work = blockIdx.x;
+  const int quad = (int)(work % 8);
+  work /= 8;
+  const int c = quad * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int ct = (int)(work % s.column_tiles), hk = (int)(work / s.column_tiles % a.Hk), b = (int)(work / s.column_tiles / a.Hk);
+  const int column = ct * 32 + c;
+  if (column >= s.columns) return;
+  const int64_t slot = work * s.parts;
+  float top = -INFINITY;
+  for (int p = 0; p < s.parts; ++p) top = fmaxf(top, s.part_ml[((slot + p) * 32 + c) * 2]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  float total = 0.f, o[(DP + 63) / 64] = {};
+  for (int p = 0; p < s.parts; ++p) {
+    const float l = s.part_ml[((slot + p) * 32 + c) * 2 + 1];
+    if (l == 0.f) continue;
+    const float w = __builtin_amdgcn_exp2f(s.part_ml[((slot + p) * 32 + c) * 2] - ref);
+    total += l * w;
+#pragma unroll
+    for (int k = 0; k < (DP + 63) / 64; ++k)
+      if (lane + 64 * k < DP) o[k] += s.part_o[((slot + p) * 32 + c) * DP + lane + 64 * k] * w;
+  }
+  const int t = column / s.G, hq = hk * s.G + column - t * s.G;
+#pragma unroll
+  for (int k = 0; k < (DP + 63) / 64; ++k)
+    if (lane + 64 * k < a.D)
+      store_from_f32(static_cast<T *>(a.y) + (((int64_t)b * s.T + t) * a.Hq + hq) * a.D + lane + 64 * k, total != 0.f ? o[k] / total : 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+View make_view(int dtype, const pa_heads &h, int64_t D) {
+  const int64_t elem = dtype == PA_F32 ? 4 : 2, per = 16 / elem;
+  return {h.data, h.batch, h.row, h.head,
+          reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && h.batch % per == 0 && h.row % per == 0 && h.head % per == 0 && D % per == 0};
+}
+
+// Whether d >= E (M / E)^(b / L), that is d^L E^b >= M^b E^L: by logarithms where they tell, else by the whole numbers themselves
+// (up to 2 048^128 128^128: 2 304 bits)
+static bool reached(int64_t d, int64_t E, int64_t M, int L, int b) {
+  const double lhs = L * log((double)d) + b * log((double)E), rhs = b * log((double)M) + L * log((double)E);
+  if (fabs(lhs - rhs) > 1e-9 * (fabs(lhs) + 1)) return lhs > rhs;
+  constexpr int WORDS = 80;
+  uint32_t x[WORDS] = {1}, y[WORDS] = {1};
+  auto times = [](uint32_t *v, int64_t factor, int count) {
+    for (; count > 0; --count) {
+      uint64_t carry = 0;
+      for (int w = 0; w < WORDS; ++w) {
+        const uint64_t t = (uint64_t)v[w] * (uint64_t)factor + carry;
+        v[w] = (uint32_t)t;
+        carry = t >> 32;
+      }
+    }
+  };
+  times(x, d, L), times(x, E, b), times(y, M, b), times(y, E, L);
+  for (int w = WORDS - 1; w >= 0; --w)
+    if (x[w] != y[w]) return x[w] > y[w];
+  return true;
+}
+
+static BiasArgs make_bias(const pa_window_params &p) {
+  static thread_local BiasArgs last = {};  // the borders depend on the three numbers alone
+  static thread_local int64_t last_buckets = 0;
+  const bool both = p.right != 0;
+  if (p.buckets == 0) return BiasArgs{};
+  if (last_buckets != p.buckets || last.distance != (int)p.distance || last.both != both) {
+    BiasArgs b = {};
+    b.buckets = (int)p.buckets, b.distance = (int)p.distance, b.both = both;
+    b.side = both ? b.buckets / 2 : b.buckets;
+    b.exact = b.side / 2;
+    const int L = b.side - b.exact;
+    for (int k = 1; k < L; ++k) {
+      int d = (int)(b.exact * pow((double)b.distance / b.exact, (double)k / L)) - 1;
+      if (d < b.exact) d = b.exact;
+      while (!reached(d, b.exact, b.distance, L, k)) ++d;
+      b.borders[k - 1] = d;
+    }
+    last = b, last_buckets = p.buckets;
+  }
+  BiasArgs b = last;
+  b.table = p.bias;
+  return b;
+}
+
+Args make_args(int dtype, const pa_window_params &p) {
+  Args a = {};
+  a.N = (int)p.N, a.Hq = (int)p.Hq, a.Hk = (int)p.Hk, a.D = (int)p.D, a.B = (int)p.B;
+  a.left = p.left < 0 || p.left >= p.N ? kNoBound : (int)p.left;
+  a.right = p.right < 0 || p.right >= p.N ? kNoBound : (int)p.right;
+  a.sinks = a.left == kNoBound ? 0 : (int)p.sinks;  // all that lies behind is seen without them
+  a.scale = (float)p.scale, a.c = (float)(p.scale * 1.4426950408889634);
+  a.lengths = p.lengths;
+  a.bias = make_bias(p);
+  a.out_units = p.D % (dtype == PA_F32 ? 4 : 8) == 0;
+  a.blocks = (int)((p.N + 127) / 128);
+  return a;
+}
+
+template <class T, int DP, bool BIAS>
+static int launch_forward(const Args &a, hipStream_t st) {
+  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
+  auto kernel = forward_kernel<T, DP, BIAS>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);
+  return launch_status();
+}
+template <class T>
+static int forward_of(const Args &a, hipStream_t st) {
+  return by_width(a.D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    return a.bias.buckets ? launch_forward<T, DP, true>(a, st) : launch_forward<T, DP, false>(a, st);
+  });
+}
+
+int forward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, void *y, float *stats, hipStream_t st) {
+  Args a = make_args(dtype, p);
+  a.q = make_view(dtype, q, p.D), a.k = make_view(dtype, k, p.D), a.v = make_view(dtype, v, p.D);
+  a.y = y, a.stats = stats;
+  a.out_units = a.out_units && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+  return dtype == PA_F32 ? forward_of<float>(a, st) : forward_of<bf16>(a, st);
+}
+
+struct StepPlan {
+  int64_t column_tiles, parts, slots;
+  int DP;
+};
+// Parts of the keys: as many as fill the chip twice, but a tile of keys at least for each of a workgroup's waves
+static StepPlan step_plan(const pa_window_params &p, int64_t T, int num_cu) {
+  StepPlan s;
+  const int64_t G = p.Hq / p.Hk;
+  s.column_tiles = (T * G + 31) / 32;
+  int64_t seen = p.N;
+  if (p.left >= 0 && p.left + T + p.sinks < seen) seen = p.left + T + p.sinks;
+  const int64_t tiles = (seen + 31) / 32, base = p.B * p.Hk * s.column_tiles;
+  int64_t parts = (2 * (int64_t)num_cu + base - 1) / base;
+  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+  s.parts = parts < 1 ? 1 : parts;
+  s.slots = base * s.parts;
+  s.DP = p.D <= 32 ? 32 : p.D <= 64 ? 64 : 128;
+  return s;
+}
+int64_t step_workspace_bytes(int, const pa_window_params &p, int64_t T, int num_cu) {
+  const StepPlan s = step_plan(p, T, num_cu);
+  return s.parts > 1 ? s.slots * 32 * (s.DP + 2) * (int64_t)sizeof(float) : 0;
+}
+
+template <class T, int DP>
+static int launch_step(const StepArgs &s, hipStream_t st) {
+  const size_t patches = 4 * 32 * Ops<T, DP>::kStride * sizeof(T), joins = 4 * 32 * DP * sizeof(float);
+  size_t lds = patches > joins ? patches : joins;
+  if (s.a.bias.buckets) lds += (size_t)s.a.bias.buckets * s.G * sizeof(float) + (s.a.bias.distance + 4) / 4 * 4;
+  const int64_t base = (int64_t)s.a.B * s.a.Hk * s.column_tiles;
+  int rc = 0;
+  if (s.a.bias.buckets) {
+    auto kernel = step_kernel<T, DP, true>;
+    if ((rc = allow_dynamic_lds(kernel, lds))) return rc;
+    kernel<<<(unsigned)(base * s.parts), 256, lds, st>>>(s);
+  } else {
+    auto kernel = step_kernel<T, DP, false>;
+    if ((rc = allow_dynamic_lds(kernel, lds))) return rc;
+    kernel<<<(unsigned)(base * s.parts), 256, lds, st>>>(s);
+  }
+  if ((rc = launch_status()) || s.parts == 1) return rc;
+  join_kernel<T, DP><<<(unsigned)(base * 8), 256, 0, st>>>(s);
+  return launch_status();
+}
+
+int step(int dtype, const pa_window_params &p, int64_t T, const pa_heads &q, const pa_heads &k, const pa_heads &v, void *y, void *workspace,
+         int num_cu, hipStream_t st) {
+  const StepPlan plan = step_plan(p, T, num_cu);
+  StepArgs s = {};
+  s.a = make_args(dtype, p);
+  s.a.q = make_view(dtype, q, p.D), s.a.k = make_view(dtype, k, p.D), s.a.v = make_view(dtype, v, p.D);
+  s.a.y = y;
+  s.T = (int)T, s.G = (int)(p.Hq / p.Hk), s.columns = (int)(T * (p.Hq / p.Hk));
+  s.column_tiles = (int)plan.column_tiles, s.parts = (int)plan.parts;
+  s.part_o = static_cast<float *>(workspace);
+  s.part_ml = s.part_o + plan.slots * 32 * plan.DP;
+  return by_width(s.a.D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    return dtype == PA_F32 ? launch_step<float, DP>(s, st) : launch_step<bf16, DP>(s, st);
+  });
+}
+
+}  // namespace window
+}  // namespace pa

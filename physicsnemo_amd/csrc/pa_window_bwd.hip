@@ -1,0 +1,409 @@
+// Gradients of attention over a window: with p_ij formed again from the kept log2 of the softmax's denominators,
+//   delta_i = sum_j p_ij dp_ij = dy_i . y_i,  dp_ij = dy_i . v_j,  ds_ij = p_ij (dp_ij - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dy_i,  d bias[b] = sum over bucket b of ds_ij
+// in two passes, so that every sum has an owner and a fixed order: queries_kernel owns 32 queries a wave and goes over the keys they see
+// (delta, dq, d bias), keys_kernel owns 32 keys a wave and goes over the queries that see them and over the query heads that share
+// them (dk, dv).
+//
+// delta from y carries the roundings of the weights and of y (2^-9 of |dy| |v| for bf16), which is what dq, dk and dv of that type are
+// rounded to.  The bias gradient is float32, and its sums cancel: where it is wanted, the first kernel sums p dp before it goes over the keys again.
+#include "pa_window.h"
+
+namespace pa {
+namespace window {
+
+template <class T, int DP, bool BIAS, bool DBIAS>
+__global__ __launch_bounds__(256) void queries_kernel(Args a) {
+  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
+  extern __shared__ u32x4 lds_raw[];
+  T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
+  float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
+  const int entries = BIAS ? table_size(a.bias) : 0;
+  float *const sums = table + entries;  // DBIAS: [wave][offset]
+  const int64_t work = own_work();
+  const int block = (int)(work % a.blocks), h = (int)(work / a.blocks % a.Hq), b = (int)(work / a.blocks / a.Hq);
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
+  using O = Ops<T, DP>;
+  f32x16 dq[DP / 32];
+  zero(dq);
+  if constexpr (BIAS) fill_bias_table(a, h, table);
+  float *const mine = sums + wave * entries;
+  if constexpr (DBIAS)
+    for (int u = lane; u < entries; u += 64) mine[u] = 0.f;
+  float behind = 0.f, ahead = 0.f;
+  if (q0 < len) {
+    const typename O::Rows own = O::rows(head_of<T>(a.q, b, h) + me * a.q.row, me < len, a.D, a.q.units, g);
+    const typename O::Rows dy = O::rows(head_of<T>(a.dy, b, h) + me * a.dy.row, me < len, a.D, a.dy.units, g);
+    const int64_t at = ((int64_t)b * a.Hq + h) * a.N + me;
+    const float stat = me < len ? a.saved_stats[at] : INFINITY;
+    float delta = 0.f;
+    if constexpr (!DBIAS) {
+      const typename O::Rows y =
+          O::rows(static_cast<const T *>(a.saved_y) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D, me < len, a.D, a.out_units, g);
+      delta = half_sum(O::dot(y, dy));
+    }
+    const int hk = h / (a.Hq / a.Hk);
+    const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
+    const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
+    Stage<T, DP, KT, 256> ks, vs;
+    // one pass over the keys: f(sub-tile's keys, values, p, dp, first key)
+    auto pass = [&](auto &&f) {
+      __syncthreads();
+      if (list.count > 0) {
+        ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
+        vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
+        ks.store(tiles, threadIdx.x);
+        vs.store(tiles + TILE, threadIdx.x);
+      }
+      __syncthreads();
+      for (int n = 0; n < list.count; ++n) {
+        const T *const kt = tiles + (n & 1) * 2 * TILE, *const vt = kt + TILE;
+        T *const next = tiles + ((n + 1) & 1) * 2 * TILE;
+        if (n + 1 < list.count) {
+          ks.load(a.k, keys, list[n + 1] * KT, len, a.D, threadIdx.x);
+          vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
+        }
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          const int k0 = list[n] * KT + 32 * s;
+          const Sight sight = sight_of(a, len, qw, k0);
+          if (sight == kNone) continue;
+          f32x16 z, dp;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
+          z = O::scores(kt + 32 * s * O::kStride, own, i, g, z);
+          dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
+          const Reach reach = BIAS ? reach_of(a.bias, k0 - qw - 31, k0 + 31 - qw) : kNear;
+          if constexpr (BIAS) {
+            const int low = table_low(a.bias);
+            if (reach == kNear) {
+              const float *t = table + (k0 + 4 * g - me + low);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[8 * (r >> 2) + (r & 3)]);
+            } else {
+              const float far = reach == kFarBehind ? table[0] : table[entries - 1];
+#pragma unroll
+              for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], BIAS ? 1.f : a.c, -stat));
+          if (sight == kSome) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const bool ok = sees(a, len, me, k0 + rowmap(r, g));
+              z[r] = ok ? z[r] : 0.f;
+              dp[r] = ok ? dp[r] : 0.f;
+            }
+          }
+          f(kt + 32 * s * O::kStride, z, dp, k0, reach);
+        }
+        if (n + 1 < list.count) {
+          ks.store(next, threadIdx.x);
+          vs.store(next + TILE, threadIdx.x);
+        }
+        __syncthreads();
+      }
+    };
+    if constexpr (DBIAS) {
+      float part = 0.f;
+      pass([&](const T *, f32x16 &p, f32x16 &dp, int, Reach) {
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
+        part += sum;
+      });
+      delta = half_sum(part);
+    }
+    if (g == 0 && me < len) a.delta[at] = delta;
+    pass([&](const T *kt, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) p[r] *= dp[r] - delta;
+      if constexpr (DBIAS) {
+        if (reach == kNear) {
+          // the half-waves one after the other: within one, every lane has an offset of its own
+          float *t = mine + (k0 + 4 * g - me + table_low(a.bias));
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (g == half) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) unsafeAtomicAdd(t + 8 * (r >> 2) + (r & 3), p[r]);
+            }
+            __builtin_amdgcn_wave_barrier();
+          }
+        } else {
+          float sum = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += p[r];
+          if (reach == kFarBehind) behind += sum;
+          else ahead += sum;
+        }
+      }
+      O::outcome(kt, O::pack(p), lane, dq);
+    });
+  }
+  T *const row = static_cast<T *>(a.dq) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
+  store_rows<T, DP>(dq, a.scale, me < len, row, me < a.N, a.D, a.out_units, g);
+  if constexpr (DBIAS) {
+    // this workgroup's share of every bucket: waves added up by offset, then offsets by bucket, one bucket a wave at a time
+    __shared__ float far[2][4];
+    behind = wave_sum(behind), ahead = wave_sum(ahead);
+    if (lane == 0) far[0][wave] = behind, far[1][wave] = ahead;
+    __syncthreads();
+    for (int u = threadIdx.x; u < entries; u += 256) sums[u] = (sums[u] + sums[entries + u]) + (sums[2 * entries + u] + sums[3 * entries + u]);
+    __syncthreads();
+    float *const out = a.bias_parts + (((int64_t)b * a.blocks + block) * a.Hq + h) * a.bias.buckets;
+    const int low = table_low(a.bias), n = a.bias.side, E = a.bias.exact;
+    for (int bucket = wave; bucket < a.bias.buckets; bucket += 4) {
+      const bool forward = bucket >= n;
+      const int k = forward ? bucket - n : bucket;
+      const int from = k <= E ? k : a.bias.borders[k - E - 1];
+      const int past = k + 1 <= E ? k + 1 : k + 1 < n ? a.bias.borders[k - E] : a.bias.distance + kPad + 1;
+      float sum = 0.f;
+      for (int d = from + lane; d < past; d += 64) {
+        if (forward) sum += d > 0 ? sums[low + d] : 0.f;
+        else sum += sums[low - d];
+      }
+      sum = wave_sum(sum);
+      if (k == n - 1) sum += forward ? (far[1][0] + far[1][1]) + (far[1][2] + far[1][3]) : (far[0][0] + far[0][1]) + (far[0][2] + far[0][3]);
+      if (lane == 0) out[bucket] = sum;
+    }
+  }
+}
+
+// d bias: a workgroup per head and bucket, the query blocks' shares in 256 parts that are joined in order
+__global__ __launch_bounds__(256) void bias_sums_kernel(const float *parts, int64_t rows, int Hq, int buckets, float *d_bias) {
+  __shared__ float part[256];
+  const int h = blockIdx.x / buckets, bucket = blockIdx.x % buckets;
+  float sum = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += 256) sum += parts[(r * Hq + h) * buckets + bucket];
+  part[threadIdx.x] = sum;
+  for (int n = 128; n > 0; n >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < n) part[threadIdx.x] += part[threadIdx.x + n];
+  }
+  if (threadIdx.x == 0) d_bias[(int64_t)bucket * Hq + h] = part[0];
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// keys_kernel: block 0 of the keys, where it holds sinks, is seen by all queries behind them: its queries are cut into sink_chunks parts, each a
+// workgroup of its own whose sums are joined by sink_sums_kernel.
+// ---------------------------------------------------------------------------------------------------------------
+template <class T, int DP, bool BIAS>
+__global__ __launch_bounds__(256) void keys_kernel(Args a) {
+  constexpr int QT = tile_rows<T, DP>(), SUB = QT / 32, TILE = QT * Ops<T, DP>::kStride;
+  extern __shared__ u32x4 lds_raw[];
+  T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][queries, gradients][QT][stride]
+  float *const stats = reinterpret_cast<float *>(tiles + 4 * TILE);  // [buffer][log2 denominators, deltas][QT]
+  float *const table = stats + 4 * QT;
+  const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.Hq / a.Hk, chunks = a.sink_chunks, per_head = a.blocks - (chunks > 0) + chunks;
+  const int64_t work = own_work();
+  int block = (int)(work % per_head), chunk = -1;
+  const int hk = (int)(work / per_head % a.Hk), b = (int)(work / per_head / a.Hk);
+  if (chunks > 0) {
+    if (block < chunks) chunk = block, block = 0;
+    else block -= chunks - 1;
+  }
+  const int len = length_of(a, b), k0 = block * 128, kw = k0 + 32 * wave, me = kw + i;
+  using O = Ops<T, DP>;
+  f32x16 dk[DP / 32], dv[DP / 32];
+  zero(dk);
+  zero(dv);
+  if (k0 < len) {
+    const typename O::Rows key = O::rows(head_of<T>(a.k, b, hk) + me * a.k.row, me < len, a.D, a.k.units, g);
+    const typename O::Rows value = O::rows(head_of<T>(a.v, b, hk) + me * a.v.row, me < len, a.D, a.v.units, g);
+    // queries that see a key of the block: i >= j - right, and i <= j + left or j a sink
+    int first = k0 - a.right > 0 ? k0 - a.right : 0, last = k0 + 127 + a.left;
+    if (chunk >= 0 || last > len - 1) last = len - 1;
+    int t0 = first / QT, t1 = last / QT;  // tiles of queries
+    if (chunk >= 0) {
+      const int tiles_of_all = (a.N + QT - 1) / QT, each = (tiles_of_all + chunks - 1) / chunks;
+      t0 = t0 > chunk * each ? t0 : chunk * each;
+      t1 = t1 < chunk * each + each - 1 ? t1 : chunk * each + each - 1;
+    }
+    const int tiles_of_head = t1 - t0 + 1, count = tiles_of_head > 0 ? tiles_of_head * G : 0;
+    Stage<T, DP, QT, 256> qs, gs;
+    float stat = 0.f;
+    auto fetch = [&](int n) {
+      const int h = hk * G + n / tiles_of_head, from = (t0 + n % tiles_of_head) * QT;
+      qs.load(a.q, head_of<T>(a.q, b, h), from, len, a.D, threadIdx.x);
+      gs.load(a.dy, head_of<T>(a.dy, b, h), from, len, a.D, threadIdx.x);
+      if (threadIdx.x < 2 * QT) {
+        const int row = from + threadIdx.x % QT;
+        const float *src = (int)threadIdx.x < QT ? a.saved_stats : a.delta;
+        stat = row < len ? src[((int64_t)b * a.Hq + h) * a.N + row] : ((int)threadIdx.x < QT ? INFINITY : 0.f);
+      }
+    };
+    auto put = [&](int n) {
+      T *const to = tiles + (n & 1) * 2 * TILE;
+      qs.store(to, threadIdx.x);
+      gs.store(to + TILE, threadIdx.x);
+      if (threadIdx.x < 2 * QT) stats[(n & 1) * 2 * QT + threadIdx.x] = stat;
+    };
+    if (count > 0) fetch(0), put(0);
+    int filled = -1;
+    for (int n = 0; n < count; ++n) {
+      const int h = hk * G + n / tiles_of_head;
+      if (BIAS && h != filled) {
+        __syncthreads();  // the head before is done with
+        fill_bias_table(a, h, table);
+        filled = h;
+      }
+      __syncthreads();
+      const T *const qt = tiles + (n & 1) * 2 * TILE, *const gt = qt + TILE;
+      const float *const lse = stats + (n & 1) * 2 * QT, *const delta = lse + QT;
+      if (n + 1 < count) fetch(n + 1);
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        const int q0 = (t0 + n % tiles_of_head) * QT + 32 * s;
+        const Sight sight = sight_of(a, len, q0, kw);
+        if (sight == kNone) continue;
+        f32x16 z, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
+        z = O::scores(qt + 32 * s * O::kStride, key, i, g, z);
+        dp = O::scores(gt + 32 * s * O::kStride, value, i, g, dp);
+        if constexpr (BIAS) {
+          const Reach reach = reach_of(a.bias, kw - q0 - 31, kw + 31 - q0);
+          const int low = table_low(a.bias);
+          if (reach == kNear) {
+            const float *t = table + (me - q0 - 4 * g + low);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[-(8 * (r >> 2) + (r & 3))]);
+          } else {
+            const float far = reach == kFarBehind ? table[0] : table[table_size(a.bias) - 1];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4 *>(lse + 32 * s + 8 * q + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(z[4 * q + j], BIAS ? 1.f : a.c, -l4[j]));
+        }
+        if (sight == kSome) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const bool ok = sees(a, len, q0 + rowmap(r, g), me);
+            z[r] = ok ? z[r] : 0.f;
+            dp[r] = ok ? dp[r] : 0.f;
+          }
+        }
+        O::outcome(gt + 32 * s * O::kStride, O::pack(z), lane, dv);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 d4 = *reinterpret_cast<const f32x4 *>(delta + 32 * s + 8 * q + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[4 * q + j] *= dp[4 * q + j] - d4[j];
+        }
+        O::outcome(qt + 32 * s * O::kStride, O::pack(z), lane, dk);
+      }
+      if (n + 1 < count) put(n + 1);
+    }
+  }
+  if (chunk < 0) {
+    const int64_t at = (((int64_t)b * a.N + me) * a.Hk + hk) * a.D;
+    store_rows<T, DP>(dk, a.scale, me < len, static_cast<T *>(a.dk) + at, me < a.N, a.D, a.out_units, g);
+    store_rows<T, DP>(dv, 1.f, me < len, static_cast<T *>(a.dv) + at, me < a.N, a.D, a.out_units, g);
+    return;
+  }
+  // [b][hk][chunk][dk, dv][128][D]
+  float *const part = a.sink_parts + (((int64_t)b * a.Hk + hk) * chunks + chunk) * 2 * 128 * a.D + (32 * wave + i) * a.D;
+  store_rows<float, DP>(dk, a.scale, me < len, part, true, a.D, a.D % 4 == 0, g);
+  store_rows<float, DP>(dv, 1.f, me < len, part + 128 * a.D, true, a.D, a.D % 4 == 0, g);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
+  const int64_t per = 2 * 128 * (int64_t)a.D, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (int64_t)a.B * a.Hk * per) return;
+  const int64_t head = e / per, at = e - head * per;
+  const float *p = a.sink_parts + head * a.sink_chunks * per + at;
+  float sum = 0.f;
+  for (int c = 0; c < a.sink_chunks; ++c) sum += p[c * per];
+  const int b = (int)(head / a.Hk), hk = (int)(head % a.Hk), side = (int)(at / (128 * a.D));
+  const int row = (int)(at / a.D % 128), d = (int)(at % a.D);
+  T *const out = static_cast<T *>(side ? a.dv : a.dk);
+  if (row < a.N) store_from_f32(out + (((int64_t)b * a.N + row) * a.Hk + hk) * a.D + d, sum);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------------------------------------------
+template <class T, int DP, bool BIAS, bool DBIAS>
+static int launch_queries(const Args &a, hipStream_t st) {
+  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) +
+                     (BIAS ? (DBIAS ? 5 : 1) * table_size(a.bias) * sizeof(float) : 0);
+  auto kernel = queries_kernel<T, DP, BIAS, DBIAS>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);
+  return launch_status();
+}
+template <class T, int DP, bool BIAS>
+static int launch_keys(const Args &a, hipStream_t st) {
+  constexpr int QT = tile_rows<T, DP>();
+  const size_t lds = 4 * (size_t)QT * Ops<T, DP>::kStride * sizeof(T) + 4 * QT * sizeof(float) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
+  auto kernel = keys_kernel<T, DP, BIAS>;
+  if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
+  const int64_t per_head = a.blocks - (a.sink_chunks > 0) + a.sink_chunks;
+  kernel<<<(unsigned)(per_head * a.Hk * a.B), 256, lds, st>>>(a);
+  if (int rc = launch_status()) return rc;
+  if (a.sink_chunks == 0) return PA_OK;
+  const int64_t n = (int64_t)a.B * a.Hk * 2 * 128 * a.D;
+  sink_sums_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+  return launch_status();
+}
+template <class T>
+static int backward_of(const Args &a, float *d_bias, hipStream_t st) {
+  return by_width(a.D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    const bool bias = a.bias.buckets != 0;
+    int rc = d_bias ? launch_queries<T, DP, true, true>(a, st)
+             : bias ? launch_queries<T, DP, true, false>(a, st) : launch_queries<T, DP, false, false>(a, st);
+    if (!rc && d_bias) {
+      bias_sums_kernel<<<(unsigned)(a.Hq * a.bias.buckets), 256, 0, st>>>(a.bias_parts, (int64_t)a.B * a.blocks, a.Hq, a.bias.buckets, d_bias);
+      rc = launch_status();
+    }
+    if (rc) return rc;
+    return bias ? launch_keys<T, DP, true>(a, st) : launch_keys<T, DP, false>(a, st);
+  });
+}
+
+// what the workspace holds, in floats
+struct Room {
+  int64_t delta, bias_parts, sink_parts;
+  int chunks;
+};
+static Room room_of(const Args &a, bool want_bias) {
+  Room r;
+  r.delta = ((int64_t)a.B * a.Hq * a.N + 3) / 4 * 4;
+  r.bias_parts = want_bias ? ((int64_t)a.B * a.blocks * a.Hq * a.bias.buckets + 3) / 4 * 4 : 0;
+  // parts of about 1 024 queries, which take about as long as a block of keys without sinks in a usual window
+  r.chunks = a.sinks > 0 ? (a.N + 1023) / 1024 : 0;
+  r.sink_parts = (int64_t)a.B * a.Hk * r.chunks * 2 * 128 * a.D;
+  return r;
+}
+int64_t backward_workspace_bytes(int dtype, const pa_window_params &p, bool want_bias) {
+  const Room r = room_of(make_args(dtype, p), want_bias);
+  return (r.delta + r.bias_parts + r.sink_parts) * (int64_t)sizeof(float);
+}
+int backward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, const void *y, const float *stats,
+             const pa_heads &dy, void *dq, void *dk, void *dv, float *d_bias, void *workspace, hipStream_t st) {
+  Args a = make_args(dtype, p);
+  const Room r = room_of(a, d_bias != nullptr);
+  a.q = make_view(dtype, q, p.D), a.k = make_view(dtype, k, p.D), a.v = make_view(dtype, v, p.D), a.dy = make_view(dtype, dy, p.D);
+  a.saved_y = y, a.saved_stats = stats;
+  a.dq = dq, a.dk = dk, a.dv = dv;
+  a.delta = static_cast<float *>(workspace);
+  a.bias_parts = a.delta + r.delta;
+  a.sink_parts = a.bias_parts + r.bias_parts;
+  a.sink_chunks = r.chunks;
+  for (const void *out : {y, (const void *)dq, (const void *)dk, (const void *)dv}) a.out_units = a.out_units && reinterpret_cast<uintptr_t>(out) % 16 == 0;
+  return dtype == PA_F32 ? backward_of<float>(a, d_bias, st) : backward_of<bf16>(a, d_bias, st);
+}
+
+}  // namespace window
+}  // namespace pa

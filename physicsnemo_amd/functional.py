@@ -6,6 +6,7 @@ kernels on torch's current stream.  `params` is the dict produced by
 """
 from __future__ import annotations
 
+from bisect import bisect_right
 from contextlib import nullcontext
 from ctypes import byref
 from functools import lru_cache
@@ -1401,4 +1402,235 @@ def gated_mlp_int8(x, w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, 
         params = _lib.PaInt8GatedParams(*map(_lib.ptr, (w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, b_down)))
         _lib.check(lib.pa_int8_gated(dtype, rows, C, F, byref(params), code, x.data_ptr(), _lib.ptr(residual), y.data_ptr(),
                                      workspace.data_ptr(), nbytes, _lib.current_stream_ptr(x.device)), "pa_int8_gated")
+    return y
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention of points over their neighbours in an order of the points
+# ---------------------------------------------------------------------------------------------------------------------
+
+_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_SEQ_LIMITS = dict(D=128, sinks=128, buckets=256, distance=2048)
+
+
+def _heads_of(t, what: str, device, dtype, shape):
+    """`t` (B, N, heads, D) as the library takes it: any strides as long as a head's channels are neighbours."""
+    if not t.is_cuda:
+        _need_cuda(t)
+    if t.device != device:
+        raise ValueError(f"all tensors have to be on the input's device ({device}), got {what} on {t.device}")
+    if t.dtype != dtype or t.shape != shape:
+        raise ValueError(f"{what} has to be {dtype} of shape {tuple(shape)}, got {t.dtype} of shape {tuple(t.shape)}")
+    batch, row, head, last = t.stride()
+    if last != 1 and shape[-1] != 1:
+        raise ValueError(f"the last axis of {what} has to be contiguous, its stride is {last}")
+    return _lib.PaHeads(t.data_ptr(), batch, row, head)
+
+
+def _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved):
+    """(params, q and k as heads) of the norm_rotate functions after checking that the arguments belong together."""
+    if q.ndim != 4 or k.ndim != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q and k have to be (B, N, heads, D) alike, got {tuple(q.shape)} and {tuple(k.shape)}")
+    B, N, Hq, D = q.shape
+    views = _heads_of(q, "q", q.device, q.dtype, q.shape), _heads_of(k, "k", q.device, q.dtype, k.shape)
+    if (positions is None) != (frequencies is None):
+        raise ValueError("positions and frequencies are given together")
+    _lib.dtype_code(q.dtype)
+    if not norm and not (q_weight is None and k_weight is None):
+        raise ValueError("weights belong to the norm: there are none without it")
+    _together(q.new_empty(0), positions, frequencies, q_weight, k_weight)
+    _expect(q_weight, "q_weight", (D,), torch.float32)
+    _expect(k_weight, "k_weight", (D,), torch.float32)
+    if D == 0 or Hq == 0 or k.shape[2] == 0 or D > _SEQ_LIMITS["D"]:
+        raise ValueError(f"heads of 1 to {_SEQ_LIMITS['D']} channels are served, one of each at least, got {tuple(q.shape)} and {tuple(k.shape)}")
+    axes = rotated = position_batch = kind = 0
+    if positions is not None:
+        if frequencies.ndim not in (1, 2) or frequencies.dtype != torch.float32:
+            raise ValueError(f"frequencies have to be float32 (pairs) or (axes, pairs), got {frequencies.dtype} of shape {tuple(frequencies.shape)}")
+        axes, rotated = (1 if frequencies.ndim == 1 else frequencies.shape[0]), 2 * frequencies.shape[-1]
+        if not 1 <= axes <= 8 or rotated > D:
+            raise ValueError(f"one to eight axes and at most half as many pairs as channels, got {axes} and {rotated // 2} for {D} channels")
+        if positions.dtype not in _POSITION_TYPES:
+            raise ValueError(f"positions have to be int32, int64 or float32, got {positions.dtype}")
+        shape = tuple(positions.shape)
+        if shape not in ((N, axes), (B, N, axes)) and (axes > 1 or shape not in ((N,), (B, N))):
+            raise ValueError(f"positions have to be {(N, axes)} or {(B, N, axes)}, with one axis also {(N,)} or {(B, N)}, got {shape}")
+        position_batch = 0 if shape in ((N, axes), (N,)) else N * axes
+        kind = _POSITION_TYPES[positions.dtype]
+    params = _lib.PaRotateParams(B, N, Hq, k.shape[2], D, rotated, axes, position_batch, kind, int(bool(interleaved)), int(bool(norm)), float(eps),
+                                 *map(_lib.ptr, (positions, frequencies, q_weight, k_weight)))
+    return params, *views
+
+
+def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, frequencies=None, eps: float = 1e-6, norm: bool = True,
+                interleaved: bool = False):
+    """Queries and keys before attention, (B, N, heads, D) each: every head's channels divided by the root of their mean square plus eps and
+    multiplied by the weight (D) float32 (None: ones), then turned by the angles of their positions; (q, k), contiguous.
+
+    positions (N) or (B, N) int32, int64 or float32 with frequencies (pairs) float32: pair p turns by position frequency_p; several
+    numbers a position, (N, axes) or (B, N, axes) with frequencies (axes, pairs): by the sum over them, formed without loss for far positions.  Pairs are channels (p, p + pairs),
+    with `interleaved` (2 p, 2 p + 1); channels behind 2 pairs are left as they are.  Without positions there is no turn, with norm = False no
+    norm.  q, k bfloat16 or float32, of any strides with contiguous channels (views of one projection), up to 128 channels a head."""
+    params, qv, kv = _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if q.shape[0] * q.shape[1]:
+        with _on(q.device):
+            _lib.check(_lib.load().pa_norm_rotate(_lib.dtype_code(q.dtype), byref(params), byref(qv), byref(kv), out[0].data_ptr(),
+                                                  out[1].data_ptr(), _lib.current_stream_ptr(q.device)), "pa_norm_rotate")
+    return out
+
+
+def norm_rotate_backward(d_q, d_k, q, k, q_weight=None, k_weight=None, positions=None, frequencies=None, eps: float = 1e-6, norm: bool = True,
+                         interleaved: bool = False, wanted=(True,) * 4):
+    """(dq, dk, d q_weight, d k_weight) of `norm_rotate` from the gradients of its results; `wanted` says which of the four are formed,
+    the others (and the weights' without a norm) are None."""
+    params, qv, kv = _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved)
+    gq, gk = _heads_of(d_q, "d_q", q.device, q.dtype, q.shape), _heads_of(d_k, "d_k", q.device, q.dtype, k.shape)
+    wanted = [bool(w) for w in wanted[:2]] + [bool(w) and norm for w in wanted[2:]]
+    empty = q.shape[0] * q.shape[1] == 0
+    make = torch.zeros if empty else torch.empty
+    kinds = ((q.shape, q.dtype), (k.shape, q.dtype), (q.shape[3:], torch.float32), (q.shape[3:], torch.float32))
+    out = tuple(make(s, dtype=t, device=q.device) if w else None for (s, t), w in zip(kinds, wanted))
+    if empty or not any(wanted):
+        return out
+    lib, code = _lib.load(), _lib.dtype_code(q.dtype)
+    with _on(q.device):
+        nbytes = _sized(lib.pa_norm_rotate_backward_workspace_bytes(code, byref(params)), "pa_norm_rotate_backward_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _lib.check(lib.pa_norm_rotate_backward(code, byref(params), byref(qv), byref(kv), byref(gq), byref(gk), *map(_lib.ptr, out),
+                                               workspace.data_ptr(), nbytes, _lib.current_stream_ptr(q.device)), "pa_norm_rotate_backward")
+    return out
+
+
+def _bound(value, what: str) -> int:
+    if value is None:
+        return -1
+    if int(value) != value or value < 0:
+        raise ValueError(f"{what} has to be a whole number from 0 on or None for no bound, got {value}")
+    return int(value)
+
+
+def _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance):
+    """(params, q, k and v as heads) of the window attention functions after checking that the arguments belong together."""
+    if q.ndim != 4 or k.ndim != 4 or k.shape[0] != q.shape[0] or k.shape[1] != N or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q, k and v have to be (B, N, heads, D) alike, got {tuple(q.shape)} and {tuple(k.shape)}")
+    B, _, Hq, D = q.shape
+    Hk = k.shape[2]
+    if Hk == 0 or Hq % Hk or Hq == 0 or not 1 <= D <= _SEQ_LIMITS["D"]:
+        raise ValueError(f"query heads have to be a multiple of the key heads, of 1 to {_SEQ_LIMITS['D']} channels, got {tuple(q.shape)} and {tuple(k.shape)}")
+    views = [_heads_of(q, "q", q.device, q.dtype, q.shape)] + [_heads_of(t, n, q.device, q.dtype, k.shape) for t, n in ((k, "k"), (v, "v"))]
+    _lib.dtype_code(q.dtype)
+    left, right = _bound(window[0], "the window's reach back"), _bound(window[1], "the window's reach ahead")
+    sinks = _bound(sinks, "the number of first points")
+    if sinks < 0 or sinks > _SEQ_LIMITS["sinks"]:
+        raise ValueError(f"0 to {_SEQ_LIMITS['sinks']} first points can stay visible, got {sinks}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"scale has to be positive, got {scale}")
+    _together(q.new_empty(0), lengths, bias)
+    _expect(lengths, "lengths", (B,), torch.int32)
+    buckets = distance = 0
+    if bias is not None:
+        if bias.ndim != 2 or bias.dtype != torch.float32 or bias.shape[1] != Hq:
+            raise ValueError(f"bias has to be float32 (buckets, {Hq}), got {bias.dtype} of shape {tuple(bias.shape)}")
+        buckets, distance = bias.shape[0], int(max_distance)
+        relative_buckets((), buckets, distance, both=right != 0)  # refuses what does not go together
+    return _lib.PaWindowParams(B, N, Hq, Hk, D, left, right, sinks, buckets, distance, scale, _lib.ptr(lengths), _lib.ptr(bias)), *views
+
+
+@lru_cache(maxsize=64)
+def _bucket_borders(side: int, distance: int) -> tuple:
+    """The least distance of each of a side's buckets: whole numbers, found without rounding."""
+    exact = side // 2
+    rest, borders = side - exact, list(range(exact))
+    for b in range(rest):
+        d = max(exact, int(exact * (distance / exact) ** (b / rest)) - 1)
+        while d ** rest * exact ** b < distance ** b * exact ** rest:
+            d += 1
+        borders.append(d)
+    return tuple(borders)
+
+
+def relative_buckets(offsets, buckets: int, max_distance: int, both: bool = True) -> list:
+    """Bucket of each offset j - i as `window_attention` counts them.  n buckets for j <= i (n = buckets / 2 if `both`, else all), and if
+    `both` as many for j > i behind them; distances below E = n // 2 have one each, the others share the rest: E + b from
+    E (max_distance / E)^(b / (n - E)) on, and nothing changes from max_distance on."""
+    side = buckets // 2 if both else buckets
+    if side < 2 or (both and buckets % 2) or buckets > _SEQ_LIMITS["buckets"]:
+        raise ValueError(f"2 to {_SEQ_LIMITS['buckets']} buckets, with a reach ahead 4 and an even number, got {buckets}")
+    if not side // 2 < max_distance <= _SEQ_LIMITS["distance"]:
+        raise ValueError(f"max_distance has to be more than {side // 2} for {buckets} buckets and at most {_SEQ_LIMITS['distance']}, got {max_distance}")
+    borders = _bucket_borders(side, max_distance) if len(offsets) else ()
+    return [bisect_right(borders, min(abs(o), max_distance)) - 1 + (side if o > 0 and both else 0) for o in offsets]
+
+
+def window_attention(q, k, v, window=(None, None), sinks: int = 0, scale: float | None = None, lengths=None, bias=None, max_distance: int = 128,
+                     return_stats: bool = False):
+    """y_i = sum_j p_ij v_j, p_i the softmax of scale q_i . k_j + bias[bucket(j - i)] over the points j that i sees: from i - window[0] to
+    i + window[1] (None: no bound) and, of those before the window, the first `sinks` points.
+
+    q (B, N, Hq, D), k and v (B, N, Hk, D) with Hk a divisor of Hq (query head h reads key head h // (Hq // Hk)), bfloat16 or float32, of any
+    strides with contiguous channels, D up to 128; scale None: 1 / sqrt(D).  lengths (B) int32 on the device: how many points each sequence
+    has, the rows behind them are not read and zero in the result.  bias (buckets, Hq) float32, added by distance (`relative_buckets`, with a side of their own
+    for j > i unless window[1] is 0).  A point that sees nothing, or only biases of -inf, has zeros.  With `return_stats` the softmax's denominators (log2,
+    (B, Hq, N) float32), which the backward pass reads, come too."""
+    B, N = q.shape[:2] if q.ndim == 4 else (0, 0)
+    params, *views = _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance)
+    y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    stats = torch.empty(B, q.shape[2], N, dtype=torch.float32, device=q.device) if return_stats else None
+    if B * N:
+        with _on(q.device):
+            _lib.check(_lib.load().pa_window_attention(_lib.dtype_code(q.dtype), byref(params), *map(byref, views), y.data_ptr(), _lib.ptr(stats),
+                                                       _lib.current_stream_ptr(q.device)), "pa_window_attention")
+    return (y, stats) if return_stats else y
+
+
+def window_attention_backward(dy, q, k, v, y, stats, window=(None, None), sinks: int = 0, scale: float | None = None, lengths=None, bias=None,
+                              max_distance: int = 128, need_bias: bool = True):
+    """(dq, dk, dv, d bias) of `window_attention` from the gradient of its result, the result and its stats; d bias None without a bias or
+    where it is not wanted."""
+    B, N = q.shape[:2] if q.ndim == 4 else (0, 0)
+    params, *views = _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance)
+    grad = _heads_of(dy, "dy", q.device, q.dtype, q.shape)
+    _together(y, stats)
+    _expect(y, "y", q.shape, q.dtype)
+    _expect(stats, "stats", (B, q.shape[2], N), torch.float32)
+    if y.device != q.device:
+        raise ValueError(f"all tensors have to be on the input's device ({q.device}), got y on {y.device}")
+    empty, need_bias = B * N == 0, need_bias and bias is not None
+    make = torch.zeros if empty else torch.empty
+    out = [make(t.shape, dtype=q.dtype, device=q.device) for t in (q, k, v)]
+    out.append(make(bias.shape, dtype=torch.float32, device=q.device) if need_bias else None)
+    if empty:
+        return tuple(out)
+    lib, code = _lib.load(), _lib.dtype_code(q.dtype)
+    with _on(q.device):
+        nbytes = _sized(lib.pa_window_attention_backward_workspace_bytes(code, byref(params), int(need_bias)),
+                        "pa_window_attention_backward_workspace_bytes")
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        _lib.check(lib.pa_window_attention_backward(code, byref(params), *map(byref, views), y.data_ptr(), stats.data_ptr(), byref(grad),
+                                                    *map(_lib.ptr, out), workspace.data_ptr(), nbytes, _lib.current_stream_ptr(q.device)),
+                   "pa_window_attention_backward")
+    return tuple(out)
+
+
+def window_attention_step(q, k, v, lengths, left: int | None = None, sinks: int = 0, scale: float | None = None, bias=None,
+                          max_distance: int = 128):
+    """`window_attention` with window (left, 0) for the newest points alone: q (B, T, Hq, D) of the last T points of each sequence, k and v
+    (B, capacity, Hk, D) of all its points so far, these included; lengths (B) int32 on the device says how many they are.  Query t is point
+    lengths - T + t (zeros where that is before the first).  Reads what the window leaves visible and nothing else.  For inference: it has no gradient."""
+    if q.ndim != 4 or k.ndim != 4 or lengths is None:
+        raise ValueError("q has to be (B, T, heads, D), k and v (B, capacity, heads, D), and lengths is needed")
+    params, *views = _window_call(q, k, v, k.shape[1], (left, 0), sinks, scale, lengths, bias, max_distance)
+    T = q.shape[1]
+    if T > k.shape[1]:
+        raise ValueError(f"{T} new points do not fit a capacity of {k.shape[1]}")
+    y = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.shape[0] * T:
+        lib, code = _lib.load(), _lib.dtype_code(q.dtype)
+        with _on(q.device):
+            nbytes = _sized(lib.pa_window_attention_step_workspace_bytes(code, byref(params), T), "pa_window_attention_step_workspace_bytes")
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            _lib.check(lib.pa_window_attention_step(code, byref(params), T, *map(byref, views), y.data_ptr(), workspace.data_ptr(), nbytes,
+                                                    _lib.current_stream_ptr(q.device)), "pa_window_attention_step")
     return y
