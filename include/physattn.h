@@ -802,7 +802,8 @@ int pa_norm_rotate_backward(int dtype, const pa_rotate_params *p, const pa_heads
 
 /* y_i = sum_j p_ij v_j, p_i the softmax over the visible j of scale q_i . k_j + bias[bucket(j - i), head], for points i of a sequence:
  * j is visible to i if j <= i + right and (j >= i - left or j < sinks) and both lie in the sequence.  Query head h reads key head
- * h / (Hq / Hk).  A row that sees nothing, or only scores of -inf, is zero, and so are its gradients.
+ * h / (Hq / Hk).  A bias of -65536 or less hides its distances as -inf does, one above 65536 counts as that.  A row that sees nothing is zero, and so are its
+ * gradients.  What i does not see has no part in y_i, infinities and NaN included.
  * Buckets of the distance d = |j - i|, n = buckets of them for j <= i where right is 0; else n = buckets / 2 for j <= i and as many for j > i
  * behind them.  With E = n / 2: d < E has bucket d, others E + the largest b < n - E with d >= E (distance / E)^(b / (n - E)). */
 #define PA_MAX_WINDOW_N (1ll << 29)

@@ -26,7 +26,8 @@ HIPCC_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 # flags of single files; the reason stands at the top of the file
-FILE_FLAGS = {"pa_layer_point.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "pa_gated_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {"pa_layer_point.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "pa_gated_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+              "pa_window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "pa_window_bwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _headers_mtime() -> float:

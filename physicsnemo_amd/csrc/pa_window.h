@@ -32,7 +32,7 @@ constexpr int kNoBound = 1 << 30;  // past every distance: positions stay below 
 struct View {
   const void *data;
   int64_t batch, row, head;
-  bool units;  // every row of a head is whole 16-byte units on 16-byte boundaries
+  bool plain;  // see Stage
 };
 struct BiasArgs {
   const float *table;  // (buckets, Hq)
@@ -57,7 +57,6 @@ struct Args {
   float *delta, *bias_parts, *sink_parts;
   int blocks;       // query (key) blocks of a sequence
   int sink_chunks;  // parts of the queries of a key block with sinks
-  bool out_units;   // rows of the results are whole 16-byte units
 };
 
 __device__ __forceinline__ int length_of(const Args &a, int b) {
@@ -92,15 +91,16 @@ __device__ __forceinline__ int bucket_of_offset(const BiasArgs &b, int off) {  /
 constexpr int kPad = 64;
 __host__ __device__ inline int table_low(const BiasArgs &b) { return b.distance + kPad; }
 __host__ __device__ inline int table_size(const BiasArgs &b) { return b.distance + 2 * kPad + 1 + (b.both ? b.distance : 0); }
-// to log2 units; finite values stay finite, so that a bias of the lowest float leaves what the softmax of such scores is
-__device__ __forceinline__ float bias_log2(float v) {
-  const float s = v * kLog2e;
-  return fabsf(v) < INFINITY ? fminf(fmaxf(s, -3.0e38f), 3.0e38f) : s;
+// A bias as the products start from it, in units of q . k: z = q . k + bias / scale, and a weight is exp2(c z - ..).  Biases of -2^16 and less
+// hide as -inf does, and none is above 2^16: a float32 score keeps nothing of q . k beside larger ones, nor does the sum that the backward
+// pass reads, the logarithm of the denominator with the reference.
+__device__ __forceinline__ float bias_start(float v, float c) {
+  return v <= -65536.f ? -INFINITY : (v > 65536.f ? 65536.f : v) * (kLog2e / c);
 }
 __device__ __forceinline__ void fill_bias_table(const Args &a, int head, float *lds) {
   const int low = table_low(a.bias), n = table_size(a.bias);
   for (int u = threadIdx.x; u < n; u += blockDim.x)
-    lds[u] = bias_log2(a.bias.table[(int64_t)bucket_of_offset(a.bias, u - low) * a.Hq + head]);
+    lds[u] = bias_start(a.bias.table[(int64_t)bucket_of_offset(a.bias, u - low) * a.Hq + head], a.c);
 }
 // where a 32 x 32 tile's offsets lie, least and most of them
 enum Reach { kNear, kFarBehind, kFarAhead };
@@ -110,15 +110,65 @@ __device__ __forceinline__ Reach reach_of(const BiasArgs &b, int least, int most
   return kNear;
 }
 
-// ---- visibility of 32 keys from k0 for 32 queries from q0 ----
-enum Sight { kNone, kSome, kAll };
-__device__ __forceinline__ Sight sight_of(const Args &a, int len, int q0, int k0) {
-  if (k0 >= len || q0 >= len || k0 > q0 + 31 + a.right || (k0 + 31 < q0 - a.left && k0 >= a.sinks)) return kNone;
-  if (k0 + 31 < len && q0 + 31 < len && k0 + 31 <= q0 + a.right && (k0 >= q0 + 31 - a.left || k0 + 31 < a.sinks)) return kAll;
-  return kSome;
+// ---- visibility of n keys from k0 for the 32 queries from q0: none of it, or what has to be hidden ----
+enum : int { kAll = 0, kEarly = 1, kLate = 2, kNone = 4 };  // kEarly: keys before a query's window, kLate: behind it, or one of both outside the sequence
+__device__ __forceinline__ int sight_of(const Args &a, int len, int q0, int k0, int n) {
+  const int k1 = k0 + n - 1, q1 = q0 + 31;
+  if (k0 >= len || q0 >= len || k0 > q1 + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) return kNone;
+  return (k0 < q1 - a.left && k1 >= a.sinks ? kEarly : 0) | (k1 > q0 + a.right || k1 >= len || q1 >= len ? kLate : 0);
 }
-__device__ __forceinline__ bool sees(const Args &a, int len, int i, int j) {
-  return j < len && i < len && j <= i + a.right && (j >= i - a.left || j < a.sinks);
+// The rows that lie in a lane's sight: low .. high, and those below `first`
+struct Span {
+  int low, high, first;
+  // of which of a tile's rows, 16 of the 32 from r0 on, a lane holds: bit r for row r0 + rowmap(r, g)
+  __device__ __forceinline__ uint32_t seen(int r0, int g) const {
+    const int lo = low - r0 - 4 * g, hi = high - r0 - 4 * g, of_first = first - r0 - 4 * g;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int n = 8 * (r >> 2) + (r & 3);
+      bits |= ((n >= lo && n <= hi) || n < of_first) ? 1u << r : 0u;
+    }
+    return bits;
+  }
+};
+// what query i sees
+__device__ __forceinline__ Span keys_of(const Args &a, int len, int i) {
+  Span s;
+  s.high = i + a.right < len - 1 ? i + a.right : len - 1;
+  if (i < 0 || i >= len) s.high = -1;
+  s.low = i - a.left > 0 ? i - a.left : 0;
+  s.first = a.sinks < s.high + 1 ? a.sinks : s.high + 1;
+  return s;
+}
+// the queries that see key j; of a sink all from low on
+__device__ __forceinline__ Span queries_of(const Args &a, int len, int j) {
+  Span s;
+  s.low = j - a.right > 0 ? j - a.right : 0;
+  s.high = j + a.left < len - 1 && j >= a.sinks ? j + a.left : len - 1;
+  if (j >= len) s.high = -1;
+  s.first = 0;
+  return s;
+}
+// z <- instead where the row is out of sight, on the sides that are asked for; `first`: some of the tile's rows may be seen as first ones
+template <bool FIRST>
+__device__ __forceinline__ void hide_low(f32x16 &z, const Span &span, int r0, int g, float instead) {
+  const int lo = span.low - r0 - 4 * g, of_first = span.first - r0 - 4 * g;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int n = 8 * (r >> 2) + (r & 3);
+    z[r] = n >= lo || (FIRST && n < of_first) ? z[r] : instead;
+  }
+}
+__device__ __forceinline__ void hide_high(f32x16 &z, const Span &span, int r0, int g, float instead) {
+  const int hi = span.high - r0 - 4 * g;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 8 * (r >> 2) + (r & 3) <= hi ? z[r] : instead;
+}
+__device__ __forceinline__ void hide(f32x16 &z, const Span &span, bool low, bool high, bool first, int r0, int g, float instead) {
+  if (low && first) hide_low<true>(z, span, r0, g, instead);
+  else if (low) hide_low<false>(z, span, r0, g, instead);
+  if (high) hide_high(z, span, r0, g, instead);
 }
 
 // The key tiles of kt rows that queries from q0 to q1 of a sequence see: those of the sinks, then those of the window
@@ -139,14 +189,18 @@ struct Tiles {
 // ---- rows and their products ----
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// eight (bf16) or four (float32) neighbouring channels of a row, zeros from D on
+// eight (bf16) or four (float32) neighbouring channels of a row, zeros from D on; rows may start on any element
+typedef u32x4 unit_at4 __attribute__((aligned(4)));
+typedef u32x4 unit_at2 __attribute__((aligned(2)));
 template <class T>
-__device__ __forceinline__ u32x4 load_piece(const T *row, int col, int D, bool units) {
+using Piece = typename std::conditional<sizeof(T) == 4, unit_at4, unit_at2>::type;
+template <class T>
+__device__ __forceinline__ u32x4 load_piece(const T *row, int col, int D) {
   constexpr int V = 16 / sizeof(T);
   u32x4 w = {0u, 0u, 0u, 0u};
-  if (units) {
-    if (col < D) w = *reinterpret_cast<const u32x4 *>(row + col);
-  } else {
+  if (col + V <= D) {
+    w = *reinterpret_cast<const Piece<T> *>(row + col);
+  } else if (col < D) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       if constexpr (sizeof(T) == 2) w[j / 2] |= (col + j < D ? (uint32_t)row[col + j].bits : 0u) << (16 * (j & 1));
@@ -154,6 +208,30 @@ __device__ __forceinline__ u32x4 load_piece(const T *row, int col, int D, bool u
     }
   }
   return w;
+}
+// the same without a branch where D is whole pieces (PLAIN); zeros where not `there`: the row itself has to be readable all the same
+template <bool PLAIN, class T>
+__device__ __forceinline__ u32x4 load_some(const T *row, int col, int D, bool there) {
+  u32x4 w;
+  if constexpr (PLAIN) w = *reinterpret_cast<const Piece<T> *>(row + (col < D ? col : 0));
+  else w = load_piece(row, col, D);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = there && col < D ? w[k] : 0u;
+  return w;
+}
+template <class T>
+__device__ __forceinline__ void store_piece(T *row, int col, int D, const u32x4 &w) {
+  constexpr int V = 16 / sizeof(T);
+  if (col + V <= D) {
+    *reinterpret_cast<Piece<T> *>(row + col) = w;
+  } else if (col < D) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (col + j >= D) continue;
+      if constexpr (sizeof(T) == 2) row[col + j].bits = (uint16_t)(w[j / 2] >> (16 * (j & 1)));
+      else row[col + j] = __uint_as_float(w[j]);
+    }
+  }
 }
 
 template <class T, int DP>
@@ -168,14 +246,19 @@ struct Ops<bf16, DP> {
   struct Weights {
     u32x4 v[2];
   };
-  static __device__ __forceinline__ Rows rows(const bf16 *row, bool there, int D, bool units, int g) {
+  // row n of a head's 0 .. limit - 1, zeros where not `there` (and from channel D on)
+  template <bool PLAIN>
+  static __device__ __forceinline__ Rows rows(const bf16 *head, int64_t stride, int n, int limit, bool there, int D, int g) {
+    const bf16 *const row = head + (n < 0 ? 0 : n < limit ? n : limit - 1) * stride;
     Rows r;
 #pragma unroll
-    for (int kk = 0; kk < DP / 16; ++kk) {
-      r.v[kk] = u32x4{0u, 0u, 0u, 0u};
-      if (there) r.v[kk] = load_piece(row, 16 * kk + 8 * g, D, units);
-    }
+    for (int kk = 0; kk < DP / 16; ++kk) r.v[kk] = load_some<PLAIN>(row, 16 * kk + 8 * g, D, there);
     return r;
+  }
+  // Waits for the rows here: left to their first use, inside the loop, the wait would be for the next tile's loads, too
+  static __device__ __forceinline__ void settle(Rows &r) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) asm volatile("" : "+v"(r.v[kk]));
   }
   static __device__ __forceinline__ float dot(const Rows &x, const Rows &y) {  // of this lane's channels
     float s = 0.f;
@@ -202,6 +285,35 @@ struct Ops<bf16, DP> {
     return acc;
   }
   static __device__ __forceinline__ Weights pack(const f32x16 &v) { return {{mfma::pack_half<0>(v), mfma::pack_half<1>(v)}}; }
+  // sum of this lane's weights as they are multiplied
+  static __device__ __forceinline__ float sum(const Weights &w) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
+    float s[2] = {};
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t word = w.v[q][k];
+        s[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, word), ones, s[q], false);
+      }
+    return s[0] + s[1];
+  }
+  // whether any of the 32 rows of lds holds an infinity or NaN: times zero it is NaN
+  static __device__ __forceinline__ bool wild(const bf16 *lds, int lane) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 zeros = {(__bf16)0.f, (__bf16)0.f};
+    const u32x4 *p = reinterpret_cast<const u32x4 *>(lds + (lane & 31) * kStride + (lane >> 5) * (DP / 2));
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint32_t word = p[k][n];
+        s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, word), zeros, s, false);
+      }
+    return __any(s != s);
+  }
   // acc[channel][column] += sum over the 32 rows of lds.  The transposing read: in a group of 16 lanes, lane l addresses four
   // channels 4 (l % 4) .. of row l / 4 and receives channel l of the four rows.
   static __device__ __forceinline__ void outcome(const bf16 *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
@@ -232,12 +344,13 @@ struct Ops<float, DP> {
   struct Weights {
     f32x16 v;
   };
-  static __device__ __forceinline__ Rows rows(const float *row, bool there, int D, bool units, int g) {
+  template <bool PLAIN>
+  static __device__ __forceinline__ Rows rows(const float *head, int64_t stride, int n, int limit, bool there, int D, int g) {
+    const float *const row = head + (n < 0 ? 0 : n < limit ? n : limit - 1) * stride;
     Rows r;
 #pragma unroll
     for (int k = 0; k < DP / 8; ++k) {
-      u32x4 w = {0u, 0u, 0u, 0u};
-      if (there) w = load_piece(row, g * (DP / 2) + 4 * k, D, units);
+      const u32x4 w = load_some<PLAIN>(row, g * (DP / 2) + 4 * k, D, there);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t b = w[j];
@@ -245,6 +358,10 @@ struct Ops<float, DP> {
       }
     }
     return r;
+  }
+  static __device__ __forceinline__ void settle(Rows &r) {
+#pragma unroll
+    for (int k = 0; k < DP / 2; ++k) asm volatile("" : "+v"(r.v[k]));
   }
   static __device__ __forceinline__ float dot(const Rows &x, const Rows &y) {
     float s = 0.f;
@@ -268,6 +385,21 @@ struct Ops<float, DP> {
     return acc;
   }
   static __device__ __forceinline__ Weights pack(const f32x16 &v) { return {v}; }
+  static __device__ __forceinline__ float sum(const Weights &w) {
+    float s[2] = {};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r & 1] += w.v[r];
+    return s[0] + s[1];
+  }
+  static __device__ __forceinline__ bool wild(const float *lds, int lane) {
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(lds + (lane & 31) * kStride + (lane >> 5) * (DP / 2));
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 8; ++k)
+#pragma unroll
+      for (int n = 0; n < 4; ++n) s = fmaf(p[k][n], 0.f, s);
+    return __any(s != s);
+  }
   static __device__ __forceinline__ void outcome(const float *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
     const float *p = lds + 4 * (lane >> 5) * kStride + (lane & 31);
 #pragma unroll
@@ -278,19 +410,55 @@ struct Ops<float, DP> {
   }
 };
 
-// ROWS rows of DP channels on their way from memory to LDS by THREADS threads: loaded into registers, written later
-template <class T, int DP, int ROWS, int THREADS>
+// acc[channel][column] += sum over the rows of lds that the column's lanes see, one by one: what is not seen has no part in it, whatever it
+// holds.  For tiles with infinities or NaN that some queries see and some do not.
+template <class T, int DP>
+__device__ __forceinline__ void outcome_of_seen(const T *lds, f32x16 w, uint32_t seen, int lane, f32x16 (&acc)[DP / 32]) {
+  const int g = lane >> 5;
+#pragma unroll 1
+  for (int r = 0; r < 16; ++r, seen >>= 1) {
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      const float weight = __shfl(w[0], (lane & 31) + 32 * half, 64);
+      const bool there = __shfl((int)seen, (lane & 31) + 32 * half, 64) & 1;
+      const T *const row = lds + rowmap(r, half) * Ops<T, DP>::kStride;
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float x = load_as_f32(row + 32 * db + rowmap(k, g));
+          acc[db][k] = there ? fmaf(weight, x, acc[db][k]) : acc[db][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 15; ++k) w[k] = w[k + 1];  // the next row's weight, without an index into registers
+  }
+}
+
+// ROWS rows of DP channels on their way from memory to LDS by THREADS threads: loaded into registers, written later.  PLAIN rows come by
+// buffer loads: a lane's offset in a tile never changes, the tile's place is in scalar registers, and what lies outside reads as zero without a
+// comparison.  Others by element where a piece is not whole.
+template <class T, int DP, bool PLAIN, int ROWS, int THREADS>
 struct Stage {
   static constexpr int V = 16 / sizeof(T), PER_ROW = DP / V, UNITS = ROWS * PER_ROW / THREADS;
-  static_assert(ROWS * PER_ROW % THREADS == 0, "whole units a thread");
+  static_assert(ROWS * PER_ROW % THREADS == 0 && THREADS % PER_ROW == 0, "whole units a thread");
   u32x4 w[UNITS];
-  // rows first .. first + ROWS - 1 of a head; zeros outside 0 .. limit - 1
+  // rows first .. first + ROWS - 1 of a head, of which 0 .. limit - 1 are there
   __device__ __forceinline__ void load(const View &view, const T *head, int first, int limit, int D, int tid) {
+    if constexpr (PLAIN) {
+      const int left = limit - first, bytes = (int)view.row * (int)sizeof(T), col = tid % PER_ROW * V;
+      const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<T *>(head + first * view.row), 0, left <= 0 ? 0 : (left < ROWS ? left : ROWS) * bytes, 0x00027000);
+      const int at = col < D ? tid / PER_ROW * bytes + col * (int)sizeof(T) : 0x7ffffff0;
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-      const int at = tid + u * THREADS, row = first + at / PER_ROW, col = at % PER_ROW * V;
-      w[u] = u32x4{0u, 0u, 0u, 0u};
-      if (row >= 0 && row < limit) w[u] = load_piece(head + row * view.row, col, D, view.units);
+      for (int u = 0; u < UNITS; ++u) w[u] = __builtin_amdgcn_raw_buffer_load_b128(src, at, u * (THREADS / PER_ROW) * bytes, 0);
+    } else {
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int at = tid + u * THREADS, row = first + at / PER_ROW, col = at % PER_ROW * V;
+        w[u] = u32x4{0u, 0u, 0u, 0u};
+        if (row < limit) w[u] = load_piece(head + row * view.row, col, D);
+      }
     }
   }
   __device__ __forceinline__ void store(T *lds, int tid) const {
@@ -309,35 +477,23 @@ __device__ __forceinline__ const T *head_of(const View &v, int b, int h) {
 
 // acc[channel][lane's row] to the row, scaled; zeros where not `some`
 template <class T, int DP>
-__device__ __forceinline__ void store_rows(f32x16 (&acc)[DP / 32], float scale, bool some, T *row, bool there, int D, bool units, int g) {
+__device__ __forceinline__ void store_rows(f32x16 (&acc)[DP / 32], float scale, bool some, T *row, bool there, int D, int g) {
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[db][r] = some ? acc[db][r] * scale : 0.f;
     if constexpr (sizeof(T) == 2) {
-      if (units) {
-        u32x4 s0, s1;
-        mfma::tile_natural(acc[db], s0, s1);
-        const int col = 32 * db + 16 * g;
-        uint16_t *out = reinterpret_cast<uint16_t *>(row);
-        if (there && col < D) *reinterpret_cast<u32x4 *>(out + col) = s0;
-        if (there && col + 8 < D) *reinterpret_cast<u32x4 *>(out + col + 8) = s1;
-        continue;
-      }
+      u32x4 s0, s1;
+      mfma::tile_natural(acc[db], s0, s1);
+      if (there) store_piece(row, 32 * db + 16 * g, D, s0), store_piece(row, 32 * db + 16 * g + 8, D, s1);
     } else {
-      if (units) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int col = 32 * db + 8 * q + 4 * g;
-          if (there && col < D) *reinterpret_cast<f32x4 *>(row + col) = f32x4{acc[db][4 * q], acc[db][4 * q + 1], acc[db][4 * q + 2], acc[db][4 * q + 3]};
-        }
-        continue;
+      for (int q = 0; q < 4; ++q) {
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(acc[db][4 * q + j]);
+        if (there) store_piece(row, 32 * db + 8 * q + 4 * g, D, w);
       }
-    }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int col = 32 * db + rowmap(r, g);
-      if (there && col < D) store_from_f32(row + col, acc[db][r]);
     }
   }
 }
@@ -357,17 +513,23 @@ constexpr int tile_rows() {
   return sizeof(T) == 4 && DP == 128 ? 32 : 64;
 }
 
-// f(std::integral_constant<int, DP>{}) for the padded width of D channels
+// f(std::integral_constant<int, DP>{}, std::bool_constant<PLAIN>{}) for the padded width of D channels
 template <class F>
-int by_width(int D, F &&f) {
-  if (D <= 32) return f(std::integral_constant<int, 32>{});
-  if (D <= 64) return f(std::integral_constant<int, 64>{});
-  return f(std::integral_constant<int, 128>{});
+int by_width(int D, bool plain, F &&f) {
+  auto with = [&](auto dp) { return plain ? f(dp, std::true_type{}) : f(dp, std::false_type{}); };
+  if (D <= 32) return with(std::integral_constant<int, 32>{});
+  if (D <= 64) return with(std::integral_constant<int, 64>{});
+  return with(std::integral_constant<int, 128>{});
 }
 
 // host
-Args make_args(int dtype, const pa_window_params &p);
-View make_view(int dtype, const pa_heads &h, int64_t D);
+Args make_args(const pa_window_params &p);
+// rows that the buffer loads take: whole 16-byte pieces on 4-byte boundaries, rows apart and no further than 2^31 bytes a tile
+inline View make_view(const pa_heads &h, int64_t D, int64_t elem) {
+  const bool plain = D * elem % 16 == 0 && reinterpret_cast<uintptr_t>(h.data) % 4 == 0 && h.batch * elem % 4 == 0 && h.row * elem % 4 == 0 &&
+                     h.head * elem % 4 == 0 && h.row >= D && h.row <= (1 << 20);
+  return {h.data, h.batch, h.row, h.head, plain};
+}
 
 }  // namespace window
 }  // namespace pa

@@ -13,40 +13,7 @@
 namespace pa {
 namespace window {
 
-constexpr float kSlack = 8.f;  // log2: how far scores may rise above the reference maximum before sums are scaled again
-
-// The softmax of a wave's queries so far, and the values' sum under it
-template <int DB>
-struct Running {
-  f32x16 o[DB];
-  float m, l, off;  // reference maximum in units of z, this lane's share of the sum, -m cc (0 while nothing was seen)
-  __device__ __forceinline__ void start() {
-    zero(o);
-    m = -INFINITY, l = 0.f, off = 0.f;
-  }
-  // a tile's largest z of this lane's query: scales what is summed where it is far above the reference (for the whole wave at once)
-  __device__ __forceinline__ void raise(float most, float cc) {
-    if (!__any(most > m + kSlack / cc)) return;
-    const float now = fmaxf(m, most);
-    const float ref = now == -INFINITY ? 0.f : now;
-    const float alpha = __builtin_amdgcn_exp2f((m - ref) * cc);
-    m = now, off = -ref * cc;
-    l *= alpha;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-  }
-  __device__ __forceinline__ void weigh(f32x16 &z, float cc) {
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], cc, off));
-      sum += z[r];
-    }
-    l += sum;
-  }
-};
+constexpr float kMost = 65536.f, kSlack = 16.f;  // how far a tile's weights, log2 of a weight may rise above the reference before all is scaled again
 
 __device__ __forceinline__ float most_of(const f32x16 &z) {
   float m = z[0];
@@ -55,30 +22,102 @@ __device__ __forceinline__ float most_of(const f32x16 &z) {
   return m;
 }
 
-// bias (in log2 units, z with it) and mask of a tile of keys from k0 for the query at position i of a wave from q0
+// The softmax of a wave's queries so far, and the values' sum under it.  The reference is not the largest score so far but one that none has
+// passed by much: only a tile whose weights sum up past kMost is looked through for its maximum and taken again, and the first ones,
+// until every query has seen something.
+template <class T, int DP>
+struct Running {
+  using O = Ops<T, DP>;
+  f32x16 o[DP / 32];
+  float m, l, off;  // reference in units of z, this lane's share of the sum, -m c (0 while nothing was seen)
+  bool fresh;       // for the whole wave: some query has seen nothing yet
+  __device__ __forceinline__ void start(bool live) {
+    zero(o);
+    m = live ? -INFINITY : 0.f, l = 0.f, off = 0.f;
+    fresh = true;
+  }
+  // for the queries that need it, so that none depends on which others are in its wave
+  __device__ __forceinline__ void raise(float most, bool need, float c) {
+    const float now = need ? fmaxf(m, most) : m, ref = now == -INFINITY ? 0.f : now;
+    const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
+    m = now, off = -ref * c;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+  }
+  // z -> weights
+  template <int S>
+  __device__ __forceinline__ float weigh(f32x16 (&z)[S], typename O::Weights (&w)[S], float c) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) z[s][r] = __builtin_amdgcn_exp2f(fmaf(z[s][r], c, off));
+      w[s] = O::pack(z[s]);
+      sum += O::sum(w[s]);
+    }
+    return sum;
+  }
+  template <int S>
+  __device__ __forceinline__ float highest(const f32x16 (&z)[S]) const {
+    float most = most_of(z[0]);
+#pragma unroll
+    for (int s = 1; s < S; ++s) most = fmaxf(most, most_of(z[s]));
+    return half_max(most);
+  }
+  // the weights of a tile that all queries see all of; scores(z) forms its z
+  template <int S, class F>
+  __device__ __forceinline__ void weights_of_all(typename O::Weights (&w)[S], float c, F &&scores) {
+    f32x16 z[S];
+    scores(z);
+    if (__builtin_expect(fresh, 0)) raise(highest(z), m == -INFINITY, c), fresh = false;
+    float sum = weigh(z, w, c);
+    if (__builtin_expect(__any(!(sum <= kMost)), 0)) {
+      const bool need = half_max(sum <= kMost ? 0.f : 1.f) > 0.f;
+      scores(z);
+      raise(highest(z), need, c);
+      sum = weigh(z, w, c);
+    }
+    l += sum;
+  }
+  // those of a tile in which some is hidden (z = -inf)
+  __device__ __forceinline__ typename O::Weights weights_of_some(f32x16 (&z)[1], float c) {
+    const float most = highest(z);
+    const bool need = m == -INFINITY || !(most * c + off <= kSlack);
+    if (__any(need)) raise(most, need, c);
+    typename O::Weights w[1];
+    l += weigh(z, w, c);
+    if (fresh) fresh = __any(m == -INFINITY);
+    return w[0];
+  }
+};
+
+// z as the products start from it: the bias of a tile of keys from k0 for the query at position i of a wave from q0, or zero
 template <bool BIAS>
-__device__ __forceinline__ void dress(const Args &a, int len, Sight sight, f32x16 &z, int q0, int i, int k0, int g, const float *table) {
+__device__ __forceinline__ f32x16 start_of(const Args &a, int q0, int i, int k0, int g, const float *table) {
+  f32x16 z;
   if constexpr (BIAS) {
     const Reach reach = reach_of(a.bias, k0 - q0 - 31, k0 + 31 - q0);
-    const int low = table_low(a.bias);
     if (reach == kNear) {
-      const float *t = table + (k0 + 4 * g - i + low);
+      const float *t = table + (k0 + 4 * g - i + table_low(a.bias));
 #pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[8 * (r >> 2) + (r & 3)]);
+      for (int r = 0; r < 16; ++r) z[r] = t[8 * (r >> 2) + (r & 3)];
     } else {
       const float far = reach == kFarBehind ? table[0] : table[table_size(a.bias) - 1];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+      for (int r = 0; r < 16; ++r) z[r] = far;
     }
-  }
-  if (sight == kSome) {
+  } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = sees(a, len, i, k0 + rowmap(r, g)) ? z[r] : -INFINITY;
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
   }
+  return z;
 }
 
-template <class T, int DP, bool BIAS>
-__global__ __launch_bounds__(256) void forward_kernel(Args a) {
+template <class T, int DP, bool PLAIN, bool BIAS>
+__global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forward_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
@@ -88,16 +127,17 @@ __global__ __launch_bounds__(256) void forward_kernel(Args a) {
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
   using O = Ops<T, DP>;
-  Running<DP / 32> run;
-  run.start();
-  const float cc = BIAS ? 1.f : a.c;
+  Running<T, DP> run;
+  run.start(me < len);
   if (q0 < len) {
-    const typename O::Rows own = O::rows(head_of<T>(a.q, b, h) + me * a.q.row, me < len, a.D, a.q.units, g);
+    typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
+    O::settle(own);
+    const Span span = keys_of(a, len, me);
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
     if constexpr (BIAS) fill_bias_table(a, h, table);
-    Stage<T, DP, KT, 256> ks, vs;
+    Stage<T, DP, PLAIN, KT, 256> ks, vs;
     if (list.count > 0) {
       ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
       vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
@@ -113,28 +153,25 @@ __global__ __launch_bounds__(256) void forward_kernel(Args a) {
         vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
       }
       const int k0 = list[n] * KT;
-      f32x16 z[SUB];
-      Sight sight[SUB];
-      float most = -INFINITY;
-      bool any = false;
+      if (sight_of(a, len, qw, k0, KT) == kAll) {
+        typename O::Weights w[SUB];
+        run.weights_of_all(w, a.c, [&](f32x16 (&z)[SUB]) {
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        sight[s] = sight_of(a, len, qw, k0 + 32 * s);
-        if (sight[s] == kNone) continue;
-        any = true;
+          for (int s = 0; s < SUB; ++s) z[s] = O::scores(kt + 32 * s * O::kStride, own, i, g, start_of<BIAS>(a, qw, me, k0 + 32 * s, g, table));
+        });
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[s][r] = 0.f;
-        z[s] = O::scores(kt + 32 * s * O::kStride, own, i, g, z[s]);
-        dress<BIAS>(a, len, sight[s], z[s], qw, me, k0 + 32 * s, g, table);
-        most = fmaxf(most, most_of(z[s]));
-      }
-      if (any) {
-        run.raise(half_max(most), cc);
-#pragma unroll
+        for (int s = 0; s < SUB; ++s) O::outcome(vt + 32 * s * O::kStride, w[s], lane, run.o);
+      } else {
+#pragma unroll 1
         for (int s = 0; s < SUB; ++s) {
-          if (sight[s] == kNone) continue;
-          run.weigh(z[s], cc);
-          O::outcome(vt + 32 * s * O::kStride, O::pack(z[s]), lane, run.o);
+          const int r0 = k0 + 32 * s, sight = sight_of(a, len, qw, r0, 32);
+          if (sight == kNone) continue;
+          f32x16 z[1] = {O::scores(kt + 32 * s * O::kStride, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table))};
+          hide(z[0], span, sight & kEarly, sight & kLate, r0 < a.sinks, r0, g, -INFINITY);
+          const typename O::Weights w = run.weights_of_some(z, a.c);
+          const T *const rows = vt + 32 * s * O::kStride;
+          if (__builtin_expect(sight != kAll && O::wild(rows, lane), 0)) outcome_of_seen<T, DP>(rows, z[0], span.seen(r0, g), lane, run.o);
+          else O::outcome(rows, w, lane, run.o);
         }
       }
       if (n + 1 < list.count) {
@@ -147,7 +184,7 @@ __global__ __launch_bounds__(256) void forward_kernel(Args a) {
   const float l = half_sum(run.l);
   const bool some = me < len && l != 0.f;
   T *const row = static_cast<T *>(a.y) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
-  store_rows<T, DP>(run.o, 1.f / l, some, row, me < a.N, a.D, a.out_units, g);
+  store_rows<T, DP>(run.o, 1.f / l, some, row, me < a.N, a.D, g);
   if (a.stats && g == 0 && me < a.N) a.stats[((int64_t)b * a.Hq + h) * a.N + me] = some ? log2f(l) - run.off : INFINITY;
 }
 
@@ -168,7 +205,7 @@ struct StepArgs {
   float *part_o, *part_ml;  // [b][hk][column tile][part][32][DP], [..][32][2]
 };
 
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool PLAIN, bool BIAS>
 __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
   using O = Ops<T, DP>;
   constexpr int TILE = 32 * O::kStride, DB = DP / 32;
@@ -191,14 +228,15 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
   const bool mine = col < s.columns && me >= 0;
   const int t0 = ct * 32 / s.G, t1 = (ct * 32 + 31 < s.columns ? ct * 32 + 31 : s.columns - 1) / s.G;
   const int first_q = len - s.T + t0 > 0 ? len - s.T + t0 : 0, last_q = len - s.T + t1;
-  const typename O::Rows own = O::rows(head_of<T>(a.q, b, hk * s.G + gq) + t * a.q.row, mine, a.D, a.q.units, g);
+  typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, hk * s.G + gq), a.q.row, t, s.T, mine, a.D, g);
+  O::settle(own);
   const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
-  Running<DB> run;
-  run.start();
-  const float cc = BIAS ? 1.f : a.c;
+  const Span span = keys_of(a, mine ? len : 0, me);
+  Running<T, DP> run;
+  run.start(mine);
   if constexpr (BIAS) {
     for (int u = threadIdx.x; u < a.bias.buckets * s.G; u += 256)
-      biases[u] = bias_log2(a.bias.table[(int64_t)(u / s.G) * a.Hq + hk * s.G + u % s.G]);
+      biases[u] = bias_start(a.bias.table[(int64_t)(u / s.G) * a.Hq + hk * s.G + u % s.G], a.c);
     for (int u = threadIdx.x; u <= a.bias.distance; u += 256) buckets[u] = (uint8_t)bucket_of(a.bias, u);
     __syncthreads();
   }
@@ -207,10 +245,10 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
     const int by = 4 * s.parts;
     int n = part * 4 + wave;
     typename O::Rows next;
-    Stage<T, DP, 32, 64> vs;
+    Stage<T, DP, PLAIN, 32, 64> vs;
     auto fetch = [&](int at) {
       const int k0 = list[at] * 32;
-      next = O::rows(keys + (k0 + i) * a.k.row, k0 + i < len, a.D, a.k.units, g);
+      next = O::template rows<PLAIN>(keys, a.k.row, k0 + i, len, k0 + i < len, a.D, g);
       vs.load(a.v, values, k0, len, a.D, lane);
     };
     if (n < list.count) fetch(n);
@@ -218,24 +256,25 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
       const int k0 = list[n] * 32;
       vs.store(patch, lane);
       wave_meets();  // lanes read what others wrote
-      f32x16 z;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = 0.f;
-      z = O::scores(next, own, z);
+      const typename O::Rows rows = next;
       if (n + by < list.count) fetch(n + by);
-      if constexpr (BIAS) {
+      f32x16 z[1];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
+      for (int r = 0; r < 16; ++r) {
+        z[0][r] = 0.f;
+        if constexpr (BIAS) {
           int d = me - (k0 + rowmap(r, g));
           d = d < 0 ? 0 : d < a.bias.distance ? d : a.bias.distance;
-          z[r] = fmaf(z[r], a.c, biases[buckets[d] * s.G + gq]);
+          z[0][r] = biases[buckets[d] * s.G + gq];
         }
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) z[r] = mine && sees(a, len, me, k0 + rowmap(r, g)) ? z[r] : -INFINITY;
-      run.raise(half_max(most_of(z)), cc);
-      run.weigh(z, cc);
-      O::outcome(patch, O::pack(z), lane, run.o);
+      z[0] = O::scores(rows, own, z[0]);
+      const int k1 = k0 + 31;
+      const bool early = k0 < last_q - a.left, late = k1 > first_q || len - s.T + t0 < 0;
+      hide(z[0], span, early, late, k0 < a.sinks, k0, g, -INFINITY);
+      const typename O::Weights w = run.weights_of_some(z, a.c);
+      if (__builtin_expect((early || late) && O::wild(patch, lane), 0)) outcome_of_seen<T, DP>(patch, z[0], span.seen(k0, g), lane, run.o);
+      else O::outcome(patch, w, lane, run.o);
       wave_meets();
     }
   }
@@ -314,12 +353,6 @@ __global__ __launch_bounds__(256) void join_kernel(StepArgs s) {
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
-View make_view(int dtype, const pa_heads &h, int64_t D) {
-  const int64_t elem = dtype == PA_F32 ? 4 : 2, per = 16 / elem;
-  return {h.data, h.batch, h.row, h.head,
-          reinterpret_cast<uintptr_t>(h.data) % 16 == 0 && h.batch % per == 0 && h.row % per == 0 && h.head % per == 0 && D % per == 0};
-}
-
 // Whether d >= E (M / E)^(b / L), that is d^L E^b >= M^b E^L: by logarithms where they tell, else by the whole numbers themselves
 // (up to 2 048^128 128^128: 2 304 bits)
 static bool reached(int64_t d, int64_t E, int64_t M, int L, int b) {
@@ -367,7 +400,7 @@ static BiasArgs make_bias(const pa_window_params &p) {
   return b;
 }
 
-Args make_args(int dtype, const pa_window_params &p) {
+Args make_args(const pa_window_params &p) {
   Args a = {};
   a.N = (int)p.N, a.Hq = (int)p.Hq, a.Hk = (int)p.Hk, a.D = (int)p.D, a.B = (int)p.B;
   a.left = p.left < 0 || p.left >= p.N ? kNoBound : (int)p.left;
@@ -376,32 +409,32 @@ Args make_args(int dtype, const pa_window_params &p) {
   a.scale = (float)p.scale, a.c = (float)(p.scale * 1.4426950408889634);
   a.lengths = p.lengths;
   a.bias = make_bias(p);
-  a.out_units = p.D % (dtype == PA_F32 ? 4 : 8) == 0;
   a.blocks = (int)((p.N + 127) / 128);
   return a;
 }
 
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool PLAIN, bool BIAS>
 static int launch_forward(const Args &a, hipStream_t st) {
   const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
-  auto kernel = forward_kernel<T, DP, BIAS>;
+  auto kernel = forward_kernel<T, DP, PLAIN, BIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);
   return launch_status();
 }
 template <class T>
 static int forward_of(const Args &a, hipStream_t st) {
-  return by_width(a.D, [&](auto dp) {
+  return by_width(a.D, a.q.plain && a.k.plain && a.v.plain, [&](auto dp, auto plain) {
     constexpr int DP = decltype(dp)::value;
-    return a.bias.buckets ? launch_forward<T, DP, true>(a, st) : launch_forward<T, DP, false>(a, st);
+    constexpr bool PLAIN = decltype(plain)::value;
+    return a.bias.buckets ? launch_forward<T, DP, PLAIN, true>(a, st) : launch_forward<T, DP, PLAIN, false>(a, st);
   });
 }
 
 int forward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, void *y, float *stats, hipStream_t st) {
-  Args a = make_args(dtype, p);
-  a.q = make_view(dtype, q, p.D), a.k = make_view(dtype, k, p.D), a.v = make_view(dtype, v, p.D);
+  const int64_t elem = dtype == PA_F32 ? 4 : 2;
+  Args a = make_args(p);
+  a.q = make_view(q, p.D, elem), a.k = make_view(k, p.D, elem), a.v = make_view(v, p.D, elem);
   a.y = y, a.stats = stats;
-  a.out_units = a.out_units && reinterpret_cast<uintptr_t>(y) % 16 == 0;
   return dtype == PA_F32 ? forward_of<float>(a, st) : forward_of<bf16>(a, st);
 }
 
@@ -429,7 +462,7 @@ int64_t step_workspace_bytes(int, const pa_window_params &p, int64_t T, int num_
   return s.parts > 1 ? s.slots * 32 * (s.DP + 2) * (int64_t)sizeof(float) : 0;
 }
 
-template <class T, int DP>
+template <class T, int DP, bool PLAIN>
 static int launch_step(const StepArgs &s, hipStream_t st) {
   const size_t patches = 4 * 32 * Ops<T, DP>::kStride * sizeof(T), joins = 4 * 32 * DP * sizeof(float);
   size_t lds = patches > joins ? patches : joins;
@@ -437,11 +470,11 @@ static int launch_step(const StepArgs &s, hipStream_t st) {
   const int64_t base = (int64_t)s.a.B * s.a.Hk * s.column_tiles;
   int rc = 0;
   if (s.a.bias.buckets) {
-    auto kernel = step_kernel<T, DP, true>;
+    auto kernel = step_kernel<T, DP, PLAIN, true>;
     if ((rc = allow_dynamic_lds(kernel, lds))) return rc;
     kernel<<<(unsigned)(base * s.parts), 256, lds, st>>>(s);
   } else {
-    auto kernel = step_kernel<T, DP, false>;
+    auto kernel = step_kernel<T, DP, PLAIN, false>;
     if ((rc = allow_dynamic_lds(kernel, lds))) return rc;
     kernel<<<(unsigned)(base * s.parts), 256, lds, st>>>(s);
   }
@@ -454,17 +487,17 @@ int step(int dtype, const pa_window_params &p, int64_t T, const pa_heads &q, con
          int num_cu, hipStream_t st) {
   const StepPlan plan = step_plan(p, T, num_cu);
   StepArgs s = {};
-  s.a = make_args(dtype, p);
-  s.a.q = make_view(dtype, q, p.D), s.a.k = make_view(dtype, k, p.D), s.a.v = make_view(dtype, v, p.D);
+  s.a = make_args(p);
+  const int64_t elem = dtype == PA_F32 ? 4 : 2;
+  s.a.q = make_view(q, p.D, elem), s.a.k = make_view(k, p.D, elem), s.a.v = make_view(v, p.D, elem);
+  const bool plain = s.a.q.plain && s.a.k.plain && s.a.v.plain;
   s.a.y = y;
   s.T = (int)T, s.G = (int)(p.Hq / p.Hk), s.columns = (int)(T * (p.Hq / p.Hk));
   s.column_tiles = (int)plan.column_tiles, s.parts = (int)plan.parts;
   s.part_o = static_cast<float *>(workspace);
   s.part_ml = s.part_o + plan.slots * 32 * plan.DP;
-  return by_width(s.a.D, [&](auto dp) {
-    constexpr int DP = decltype(dp)::value;
-    return dtype == PA_F32 ? launch_step<float, DP>(s, st) : launch_step<bf16, DP>(s, st);
-  });
+  if (dtype == PA_F32) return by_width(s.a.D, plain, [&](auto dp, auto is_plain) { return launch_step<float, decltype(dp)::value, decltype(is_plain)::value>(s, st); });
+  return by_width(s.a.D, plain, [&](auto dp, auto is_plain) { return launch_step<bf16, decltype(dp)::value, decltype(is_plain)::value>(s, st); });
 }
 
 }  // namespace window

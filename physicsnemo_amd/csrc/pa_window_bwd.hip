@@ -12,7 +12,7 @@
 namespace pa {
 namespace window {
 
-template <class T, int DP, bool BIAS, bool DBIAS>
+template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
@@ -33,22 +33,27 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
     for (int u = lane; u < entries; u += 64) mine[u] = 0.f;
   float behind = 0.f, ahead = 0.f;
   if (q0 < len) {
-    const typename O::Rows own = O::rows(head_of<T>(a.q, b, h) + me * a.q.row, me < len, a.D, a.q.units, g);
-    const typename O::Rows dy = O::rows(head_of<T>(a.dy, b, h) + me * a.dy.row, me < len, a.D, a.dy.units, g);
+    typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
+    typename O::Rows dy = O::template rows<PLAIN>(head_of<T>(a.dy, b, h), a.dy.row, me, len, me < len, a.D, g);
+    O::settle(own), O::settle(dy);
     const int64_t at = ((int64_t)b * a.Hq + h) * a.N + me;
-    const float stat = me < len ? a.saved_stats[at] : INFINITY;
+    float stat = me < len ? a.saved_stats[at] : INFINITY;
     float delta = 0.f;
     if constexpr (!DBIAS) {
       const typename O::Rows y =
-          O::rows(static_cast<const T *>(a.saved_y) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D, me < len, a.D, a.out_units, g);
+          O::template rows<PLAIN>(static_cast<const T *>(a.saved_y) + ((int64_t)b * a.N * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, me, len, me < len, a.D, g);
       delta = half_sum(O::dot(y, dy));
     }
+    const Span span = keys_of(a, len, me);
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
-    Stage<T, DP, KT, 256> ks, vs;
+    Stage<T, DP, PLAIN, KT, 256> ks, vs;
     // one pass over the keys: f(sub-tile's keys, values, p, dp, first key)
-    auto pass = [&](auto &&f) {
+    f32x16 start;  // of dp: in the last pass less delta already
+    auto pass = [&](float from, auto &&f) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) start[r] = from;
       __syncthreads();
       if (list.count > 0) {
         ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
@@ -67,37 +72,35 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
           const int k0 = list[n] * KT + 32 * s;
-          const Sight sight = sight_of(a, len, qw, k0);
+          const int sight = sight_of(a, len, qw, k0, 32);
           if (sight == kNone) continue;
-          f32x16 z, dp;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
-          z = O::scores(kt + 32 * s * O::kStride, own, i, g, z);
-          dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
-          const Reach reach = BIAS ? reach_of(a.bias, k0 - qw - 31, k0 + 31 - qw) : kNear;
+          const T *const krows = kt + 32 * s * O::kStride;
+          f32x16 z, dp = start;
+          Reach reach = kNear;
           if constexpr (BIAS) {
-            const int low = table_low(a.bias);
+            reach = reach_of(a.bias, k0 - qw - 31, k0 + 31 - qw);
             if (reach == kNear) {
-              const float *t = table + (k0 + 4 * g - me + low);
+              const float *t = table + (k0 + 4 * g - me + table_low(a.bias));
 #pragma unroll
-              for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[8 * (r >> 2) + (r & 3)]);
+              for (int r = 0; r < 16; ++r) z[r] = t[8 * (r >> 2) + (r & 3)];
             } else {
               const float far = reach == kFarBehind ? table[0] : table[entries - 1];
 #pragma unroll
-              for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+              for (int r = 0; r < 16; ++r) z[r] = far;
             }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] = 0.f;
+          }
+          z = O::scores(krows, own, i, g, z);
+          dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
+          if (sight != kAll) {
+            hide(z, span, sight & kEarly, sight & kLate, k0 < a.sinks, k0, g, -INFINITY);
+            if (O::wild(vt + 32 * s * O::kStride, lane)) hide(dp, span, true, true, true, k0, g, 0.f);
           }
 #pragma unroll
-          for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], BIAS ? 1.f : a.c, -stat));
-          if (sight == kSome) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const bool ok = sees(a, len, me, k0 + rowmap(r, g));
-              z[r] = ok ? z[r] : 0.f;
-              dp[r] = ok ? dp[r] : 0.f;
-            }
-          }
-          f(kt + 32 * s * O::kStride, z, dp, k0, reach);
+          for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], a.c, -stat));
+          f(krows, z, dp, k0, reach, sight);
         }
         if (n + 1 < list.count) {
           ks.store(next, threadIdx.x);
@@ -107,19 +110,24 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
       }
     };
     if constexpr (DBIAS) {
-      float part = 0.f;
-      pass([&](const T *, f32x16 &p, f32x16 &dp, int, Reach) {
-        float sum = 0.f;
+      // the denominator, too: for bf16 the forward pass summed the weights as it multiplied them, rounded
+      float part = 0.f, total = 0.f;
+      pass(0.f, [&](const T *, f32x16 &p, f32x16 &dp, int, Reach, int) {
+        float sum = 0.f, weights = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum);
-        part += sum;
+        for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum), weights += p[r];
+        part += sum, total += weights;
       });
-      delta = half_sum(part);
+      total = half_sum(total);
+      if (total > 0.f) {
+        delta = half_sum(part) / total;
+        stat += log2f(total);
+      }
     }
     if (g == 0 && me < len) a.delta[at] = delta;
-    pass([&](const T *kt, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
+    pass(-delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach, int sight) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] *= dp[r] - delta;
+      for (int r = 0; r < 16; ++r) p[r] *= dp[r];
       if constexpr (DBIAS) {
         if (reach == kNear) {
           // the half-waves one after the other: within one, every lane has an offset of its own
@@ -140,11 +148,12 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           else ahead += sum;
         }
       }
-      O::outcome(kt, O::pack(p), lane, dq);
+      if (sight != kAll && O::wild(krows, lane)) outcome_of_seen<T, DP>(krows, p, span.seen(k0, g), lane, dq);
+      else O::outcome(krows, O::pack(p), lane, dq);
     });
   }
   T *const row = static_cast<T *>(a.dq) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
-  store_rows<T, DP>(dq, a.scale, me < len, row, me < a.N, a.D, a.out_units, g);
+  store_rows<T, DP>(dq, a.scale, me < len, row, me < a.N, a.D, g);
   if constexpr (DBIAS) {
     // this workgroup's share of every bucket: waves added up by offset, then offsets by bucket, one bucket a wave at a time
     __shared__ float far[2][4];
@@ -190,7 +199,7 @@ __global__ __launch_bounds__(256) void bias_sums_kernel(const float *parts, int6
 // keys_kernel: block 0 of the keys, where it holds sinks, is seen by all queries behind them: its queries are cut into sink_chunks parts, each a
 // workgroup of its own whose sums are joined by sink_sums_kernel.
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool PLAIN, bool BIAS>
 __global__ __launch_bounds__(256) void keys_kernel(Args a) {
   constexpr int QT = tile_rows<T, DP>(), SUB = QT / 32, TILE = QT * Ops<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
@@ -212,8 +221,10 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
   zero(dk);
   zero(dv);
   if (k0 < len) {
-    const typename O::Rows key = O::rows(head_of<T>(a.k, b, hk) + me * a.k.row, me < len, a.D, a.k.units, g);
-    const typename O::Rows value = O::rows(head_of<T>(a.v, b, hk) + me * a.v.row, me < len, a.D, a.v.units, g);
+    typename O::Rows key = O::template rows<PLAIN>(head_of<T>(a.k, b, hk), a.k.row, me, len, me < len, a.D, g);
+    typename O::Rows value = O::template rows<PLAIN>(head_of<T>(a.v, b, hk), a.v.row, me, len, me < len, a.D, g);
+    O::settle(key), O::settle(value);
+    const Span span = queries_of(a, len, me);
     // queries that see a key of the block: i >= j - right, and i <= j + left or j a sink
     int first = k0 - a.right > 0 ? k0 - a.right : 0, last = k0 + 127 + a.left;
     if (chunk >= 0 || last > len - 1) last = len - 1;
@@ -224,7 +235,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       t1 = t1 < chunk * each + each - 1 ? t1 : chunk * each + each - 1;
     }
     const int tiles_of_head = t1 - t0 + 1, count = tiles_of_head > 0 ? tiles_of_head * G : 0;
-    Stage<T, DP, QT, 256> qs, gs;
+    Stage<T, DP, PLAIN, QT, 256> qs, gs;
     float stat = 0.f;
     auto fetch = [&](int n) {
       const int h = hk * G + n / tiles_of_head, from = (t0 + n % tiles_of_head) * QT;
@@ -232,8 +243,10 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       gs.load(a.dy, head_of<T>(a.dy, b, h), from, len, a.D, threadIdx.x);
       if (threadIdx.x < 2 * QT) {
         const int row = from + threadIdx.x % QT;
+        // as the products start from them: less the denominator in units of z, less delta; rows that are not there weigh nothing
         const float *src = (int)threadIdx.x < QT ? a.saved_stats : a.delta;
-        stat = row < len ? src[((int64_t)b * a.Hq + h) * a.N + row] : ((int)threadIdx.x < QT ? INFINITY : 0.f);
+        const float v = src[((int64_t)b * a.Hq + h) * a.N + (row < len ? row : len - 1)];
+        stat = (int)threadIdx.x >= QT ? -v : row < len ? -v / a.c : -INFINITY;
       }
     };
     auto put = [&](int n) {
@@ -258,62 +271,58 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
 #pragma unroll
       for (int s = 0; s < SUB; ++s) {
         const int q0 = (t0 + n % tiles_of_head) * QT + 32 * s;
-        const Sight sight = sight_of(a, len, q0, kw);
+        const int sight = sight_of(a, len, q0, kw, 32);
         if (sight == kNone) continue;
+        const T *const qrows = qt + 32 * s * O::kStride, *const grows = gt + 32 * s * O::kStride;
         f32x16 z, dp;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = dp[r] = 0.f;
-        z = O::scores(qt + 32 * s * O::kStride, key, i, g, z);
-        dp = O::scores(gt + 32 * s * O::kStride, value, i, g, dp);
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 l4 = *reinterpret_cast<const f32x4 *>(lse + 32 * s + 8 * q + 4 * g), d4 = *reinterpret_cast<const f32x4 *>(delta + 32 * s + 8 * q + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[4 * q + j] = l4[j], dp[4 * q + j] = d4[j];
+        }
         if constexpr (BIAS) {
           const Reach reach = reach_of(a.bias, kw - q0 - 31, kw + 31 - q0);
-          const int low = table_low(a.bias);
           if (reach == kNear) {
-            const float *t = table + (me - q0 - 4 * g + low);
+            const float *t = table + (me - q0 - 4 * g + table_low(a.bias));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, t[-(8 * (r >> 2) + (r & 3))]);
+            for (int r = 0; r < 16; ++r) z[r] += t[-(8 * (r >> 2) + (r & 3))];
           } else {
             const float far = reach == kFarBehind ? table[0] : table[table_size(a.bias) - 1];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z[r] = fmaf(z[r], a.c, far);
+            for (int r = 0; r < 16; ++r) z[r] += far;
           }
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4 *>(lse + 32 * s + 8 * q + 4 * g);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(z[4 * q + j], BIAS ? 1.f : a.c, -l4[j]));
+        z = O::scores(qrows, key, i, g, z);
+        dp = O::scores(grows, value, i, g, dp);
+        bool wild = false;
+        if (sight != kAll) {  // a key that comes early for a query sees it late
+          hide(z, span, sight & kLate, (sight & kEarly) || q0 + 31 >= len, false, q0, g, -INFINITY);
+          wild = O::wild(grows, lane) || __any(!(fabsf(delta[32 * s + i]) < INFINITY));
+          if (wild) hide(dp, span, true, true, false, q0, g, 0.f);
         }
-        if (sight == kSome) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const bool ok = sees(a, len, q0 + rowmap(r, g), me);
-            z[r] = ok ? z[r] : 0.f;
-            dp[r] = ok ? dp[r] : 0.f;
-          }
-        }
-        O::outcome(gt + 32 * s * O::kStride, O::pack(z), lane, dv);
+        for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(z[r] * a.c);
+        if (wild) outcome_of_seen<T, DP>(grows, z, span.seen(q0, g), lane, dv);
+        else O::outcome(grows, O::pack(z), lane, dv);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f32x4 d4 = *reinterpret_cast<const f32x4 *>(delta + 32 * s + 8 * q + 4 * g);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) z[4 * q + j] *= dp[4 * q + j] - d4[j];
-        }
-        O::outcome(qt + 32 * s * O::kStride, O::pack(z), lane, dk);
+        for (int r = 0; r < 16; ++r) z[r] *= dp[r];
+        if (sight != kAll && O::wild(qrows, lane)) outcome_of_seen<T, DP>(qrows, z, span.seen(q0, g), lane, dk);
+        else O::outcome(qrows, O::pack(z), lane, dk);
       }
       if (n + 1 < count) put(n + 1);
     }
   }
   if (chunk < 0) {
     const int64_t at = (((int64_t)b * a.N + me) * a.Hk + hk) * a.D;
-    store_rows<T, DP>(dk, a.scale, me < len, static_cast<T *>(a.dk) + at, me < a.N, a.D, a.out_units, g);
-    store_rows<T, DP>(dv, 1.f, me < len, static_cast<T *>(a.dv) + at, me < a.N, a.D, a.out_units, g);
+    store_rows<T, DP>(dk, a.scale, me < len, static_cast<T *>(a.dk) + at, me < a.N, a.D, g);
+    store_rows<T, DP>(dv, 1.f, me < len, static_cast<T *>(a.dv) + at, me < a.N, a.D, g);
     return;
   }
   // [b][hk][chunk][dk, dv][128][D]
   float *const part = a.sink_parts + (((int64_t)b * a.Hk + hk) * chunks + chunk) * 2 * 128 * a.D + (32 * wave + i) * a.D;
-  store_rows<float, DP>(dk, a.scale, me < len, part, true, a.D, a.D % 4 == 0, g);
-  store_rows<float, DP>(dv, 1.f, me < len, part + 128 * a.D, true, a.D, a.D % 4 == 0, g);
+  store_rows<float, DP>(dk, a.scale, me < len, part, true, a.D, g);
+  store_rows<float, DP>(dv, 1.f, me < len, part + 128 * a.D, true, a.D, g);
 }
 
 template <class T>
@@ -333,20 +342,20 @@ __global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
 // ---------------------------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------------------------
-template <class T, int DP, bool BIAS, bool DBIAS>
+template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 static int launch_queries(const Args &a, hipStream_t st) {
   const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) +
                      (BIAS ? (DBIAS ? 5 : 1) * table_size(a.bias) * sizeof(float) : 0);
-  auto kernel = queries_kernel<T, DP, BIAS, DBIAS>;
+  auto kernel = queries_kernel<T, DP, PLAIN, BIAS, DBIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);
   return launch_status();
 }
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool PLAIN, bool BIAS>
 static int launch_keys(const Args &a, hipStream_t st) {
   constexpr int QT = tile_rows<T, DP>();
   const size_t lds = 4 * (size_t)QT * Ops<T, DP>::kStride * sizeof(T) + 4 * QT * sizeof(float) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
-  auto kernel = keys_kernel<T, DP, BIAS>;
+  auto kernel = keys_kernel<T, DP, PLAIN, BIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   const int64_t per_head = a.blocks - (a.sink_chunks > 0) + a.sink_chunks;
   kernel<<<(unsigned)(per_head * a.Hk * a.B), 256, lds, st>>>(a);
@@ -358,17 +367,18 @@ static int launch_keys(const Args &a, hipStream_t st) {
 }
 template <class T>
 static int backward_of(const Args &a, float *d_bias, hipStream_t st) {
-  return by_width(a.D, [&](auto dp) {
+  return by_width(a.D, a.q.plain && a.k.plain && a.v.plain && a.dy.plain, [&](auto dp, auto plain) {
     constexpr int DP = decltype(dp)::value;
+    constexpr bool PLAIN = decltype(plain)::value;
     const bool bias = a.bias.buckets != 0;
-    int rc = d_bias ? launch_queries<T, DP, true, true>(a, st)
-             : bias ? launch_queries<T, DP, true, false>(a, st) : launch_queries<T, DP, false, false>(a, st);
+    int rc = d_bias ? launch_queries<T, DP, PLAIN, true, true>(a, st)
+             : bias ? launch_queries<T, DP, PLAIN, true, false>(a, st) : launch_queries<T, DP, PLAIN, false, false>(a, st);
     if (!rc && d_bias) {
       bias_sums_kernel<<<(unsigned)(a.Hq * a.bias.buckets), 256, 0, st>>>(a.bias_parts, (int64_t)a.B * a.blocks, a.Hq, a.bias.buckets, d_bias);
       rc = launch_status();
     }
     if (rc) return rc;
-    return bias ? launch_keys<T, DP, true>(a, st) : launch_keys<T, DP, false>(a, st);
+    return bias ? launch_keys<T, DP, PLAIN, true>(a, st) : launch_keys<T, DP, PLAIN, false>(a, st);
   });
 }
 
@@ -387,21 +397,21 @@ static Room room_of(const Args &a, bool want_bias) {
   return r;
 }
 int64_t backward_workspace_bytes(int dtype, const pa_window_params &p, bool want_bias) {
-  const Room r = room_of(make_args(dtype, p), want_bias);
+  const Room r = room_of(make_args(p), want_bias);
   return (r.delta + r.bias_parts + r.sink_parts) * (int64_t)sizeof(float);
 }
 int backward(int dtype, const pa_window_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &v, const void *y, const float *stats,
              const pa_heads &dy, void *dq, void *dk, void *dv, float *d_bias, void *workspace, hipStream_t st) {
-  Args a = make_args(dtype, p);
+  const int64_t elem = dtype == PA_F32 ? 4 : 2;
+  Args a = make_args(p);
   const Room r = room_of(a, d_bias != nullptr);
-  a.q = make_view(dtype, q, p.D), a.k = make_view(dtype, k, p.D), a.v = make_view(dtype, v, p.D), a.dy = make_view(dtype, dy, p.D);
+  a.q = make_view(q, p.D, elem), a.k = make_view(k, p.D, elem), a.v = make_view(v, p.D, elem), a.dy = make_view(dy, p.D, elem);
   a.saved_y = y, a.saved_stats = stats;
   a.dq = dq, a.dk = dk, a.dv = dv;
   a.delta = static_cast<float *>(workspace);
   a.bias_parts = a.delta + r.delta;
   a.sink_parts = a.bias_parts + r.bias_parts;
   a.sink_chunks = r.chunks;
-  for (const void *out : {y, (const void *)dq, (const void *)dk, (const void *)dv}) a.out_units = a.out_units && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   return dtype == PA_F32 ? backward_of<float>(a, d_bias, st) : backward_of<bf16>(a, d_bias, st);
 }
 

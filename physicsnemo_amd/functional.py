@@ -1572,7 +1572,8 @@ def window_attention(q, k, v, window=(None, None), sinks: int = 0, scale: float 
     q (B, N, Hq, D), k and v (B, N, Hk, D) with Hk a divisor of Hq (query head h reads key head h // (Hq // Hk)), bfloat16 or float32, of any
     strides with contiguous channels, D up to 128; scale None: 1 / sqrt(D).  lengths (B) int32 on the device: how many points each sequence
     has, the rows behind them are not read and zero in the result.  bias (buckets, Hq) float32, added by distance (`relative_buckets`, with a side of their own
-    for j > i unless window[1] is 0).  A point that sees nothing, or only biases of -inf, has zeros.  With `return_stats` the softmax's denominators (log2,
+    for j > i unless window[1] is 0); a bias of -65536 or less hides its distances as -inf does, one above 65536 counts as that.  A point that sees nothing
+    has zeros, and what it does not see has no part in its result, infinities and NaN included.  With `return_stats` the softmax's denominators (log2,
     (B, Hq, N) float32), which the backward pass reads, come too."""
     B, N = q.shape[:2] if q.ndim == 4 else (0, 0)
     params, *views = _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance)

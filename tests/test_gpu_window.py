@@ -80,29 +80,64 @@ def test_padded_sequences(lengths, buckets, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(torch.float32).min, -1e9])
+@pytest.mark.parametrize("value", [float("-inf"), torch.finfo(torch.float32).min, -1e9, -65536.0])
 @pytest.mark.parametrize("all_of_it", [False, True])
 def test_masking_biases(value, all_of_it, dtype):
-    """Biases of -inf hide their distances, also all that a point sees; the lowest float where nothing else is left gives equal weights."""
+    """Biases of -inf and down to the lowest float hide their distances, also all that a point sees: zeros, no gradients, no NaN."""
     announce("masking", value, all_of_it, dtype)
     q, k, v, dy, bias = make(2, 150, 2, 2, 32, dtype, 8, seed=9)
     bias[:, 0] = value  # head 0: everything, or all but the point itself
     if not all_of_it:
         bias[0, 0] = 0.5
     bias[3:5, 1] = value
-    call = dict(window=(40, 40), max_distance=30)
-    want = wo.attention(q, k, v, bias=bias, dy=dy, **call)
-    y = PF.window_attention(q, k, v, bias=bias, **call)
-    if value < -1e30 or not all_of_it:  # -1e9: a float32 score keeps nothing of q . k in its 24 bits, and the oracle's 53 do
-        wo.check(y, want["y"], "y")
-    assert torch.isfinite(y).all() and (value != float("-inf") or not all_of_it or not y[:, :, 0].any())
+    compare(q, k, v, dy, bias, window=(40, 40), max_distance=30)
     leaves = [t.detach().requires_grad_(True) for t in (q, k, v, bias)]
-    grads = torch.autograd.grad(PA.window_attention(*leaves[:3], bias=leaves[3], **call), leaves, dy)
-    assert all(torch.isfinite(g).all() for g in grads)
-    if value == float("-inf"):
-        for name, g in zip(("dq", "dk", "dv", "dbias"), grads):
-            wo.check(g, want[name], name)
-        assert not grads[3][3:5, 1].any() and (not all_of_it or not grads[0][:, :, 0].any())
+    y = PA.window_attention(*leaves[:3], bias=leaves[3], window=(40, 40), max_distance=30)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert not grads[3][3:5, 1].any()
+    if all_of_it:
+        assert not any(t[:, :, 0].any() for t in (y, *grads[:3])) and not grads[3][:, 0].any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("value", [70000.0, 9000.0, -9000.0])
+def test_large_biases(value, dtype):
+    """One distance far above or below the others, by more than exp2 holds: what is above takes all, what is below nothing."""
+    announce("large", value, dtype)
+    q, k, v, dy, bias = make(1, 100, 2, 1, 16, dtype, 8, seed=3)
+    bias[1] = value
+    compare(q, k, v, dy, bias, window=(30, 30), max_distance=20)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+def test_wild_values_where_they_are_not_seen(value, dtype):
+    """Infinities and NaN in points of the sequence itself reach the points that see them and no others, forward and backward."""
+    announce("wild", value, dtype)
+    q, k, v, dy, bias = make(1, 300, 4, 2, 32, dtype, 8, seed=12)
+    call = dict(window=(37, 21), sinks=2, bias=bias, max_distance=25)
+    def all_of_it(q, k, v, dy):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        y = PA.window_attention(*leaves, **call)
+        n = torch.full((1,), 300, dtype=torch.int32, device="cuda")
+        step = PF.window_attention_step(q[:, -40:], k, v, n, left=37, sinks=2, bias=bias, max_distance=25)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy), step]
+    clean, at, want = all_of_it(q, k, v, dy), 150, wo.attention(q, k, v, dy=dy, **call)
+    i = torch.arange(300, device="cuda")
+    sees = (i >= at - 21) & (i <= at + 37)  # the queries that see the point; the keys it sees: at - 37 .. at + 21 and the sinks
+    seen = ((i >= at - 37) & (i <= at + 21)) | (i < 2)
+    near = sees[:, None] & torch.stack([((i >= a - 37) & (i <= a + 21)) | (i < 2) for a in range(300)])
+    through = near.any(0)  # keys of the queries that see the point
+    for which, touched in (("q", (i == at, i == at, seen, seen)), ("k", (sees, sees, through, through)), ("v", (sees, sees, through, i == at)),
+                           ("dy", (i < 0, i == at, seen, seen))):
+        t = {n: x.clone() for n, x in zip(("q", "k", "v", "dy"), (q, k, v, dy))}
+        t[which][0, at] = value
+        got = all_of_it(**t)
+        for n, (name, may) in enumerate(zip(("y", "dq", "dk", "dv"), touched)):
+            wo.check(got[n][0][~may], [t[0][~may] for t in want[name]], (which, name))
+            if may.any() and not (which == "v" and name == "dv"):
+                assert not torch.isfinite(got[n][0][may]).all(), (which, name)
+        assert torch.equal(got[4], clean[4])  # the step's windows lie behind the point
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])

@@ -50,10 +50,10 @@ def attention(q, k, v, window=(None, None), sinks=0, scale=None, lengths=None, b
     e_s = (D + 8) * U * scale * torch.matmul(Q.abs(), K.abs().mT) + 4 * U * s.abs()
     if bias is not None:
         add = bias_of(bias.double(), N, Nk, first, window[1], max_distance)
-        s, e_s = s + add, e_s + 4 * U * add.abs().nan_to_num(0, 0, 0).clamp(max=1e4)
+        ok = ok & (add > -65536)  # hidden
+        add = add.clamp(-65536, 65536)
+        s, e_s = s + add, e_s + 4 * U * add.abs()
     s = torch.where(ok, s, torch.full_like(s, -torch.inf))
-    if bias is not None and (bias.abs() > 1e30).any():  # where float32 scores are all the bias
-        s = torch.where(s < -1e30, torch.where(s == -torch.inf, s, torch.full_like(s, -3e38)), s)
     top = s.amax(-1, keepdim=True)
     p = torch.exp(s - torch.where(top > -torch.inf, top, torch.zeros_like(top)))
     total = p.sum(-1, keepdim=True)
