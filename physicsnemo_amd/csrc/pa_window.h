@@ -66,9 +66,9 @@ __device__ __forceinline__ int length_of(const Args &a, int b) {
 }
 
 // Workgroup -> work: consecutive work on one XCD (workgroups go round them), whose L2 then holds what neighbours share
-__device__ __forceinline__ int64_t own_work() {
-  const int64_t n = gridDim.x, id = blockIdx.x, per = n / 8, rest = n % 8, xcd = id % 8, slot = id / 8;
-  return xcd < rest ? xcd * (per + 1) + slot : rest * (per + 1) + (xcd - rest) * per + slot;
+__device__ __forceinline__ uint32_t own_work() {
+  const uint32_t n = gridDim.x, id = blockIdx.x, per = n / 8, rest = n % 8, xcd = id % 8, slot = id / 8;
+  return xcd * per + (xcd < rest ? xcd : rest) + slot;
 }
 
 // ---- bias ----
@@ -120,17 +120,7 @@ __device__ __forceinline__ int sight_of(const Args &a, int len, int q0, int k0, 
 // The rows that lie in a lane's sight: low .. high, and those below `first`
 struct Span {
   int low, high, first;
-  // of which of a tile's rows, 16 of the 32 from r0 on, a lane holds: bit r for row r0 + rowmap(r, g)
-  __device__ __forceinline__ uint32_t seen(int r0, int g) const {
-    const int lo = low - r0 - 4 * g, hi = high - r0 - 4 * g, of_first = first - r0 - 4 * g;
-    uint32_t bits = 0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int n = 8 * (r >> 2) + (r & 3);
-      bits |= ((n >= lo && n <= hi) || n < of_first) ? 1u << r : 0u;
-    }
-    return bits;
-  }
+  __device__ __forceinline__ bool sees(int r) const { return (r >= low && r <= high) || r < first; }
 };
 // what query i sees
 __device__ __forceinline__ Span keys_of(const Args &a, int len, int i) {
@@ -299,21 +289,6 @@ struct Ops<bf16, DP> {
       }
     return s[0] + s[1];
   }
-  // whether any of the 32 rows of lds holds an infinity or NaN: times zero it is NaN
-  static __device__ __forceinline__ bool wild(const bf16 *lds, int lane) {
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 zeros = {(__bf16)0.f, (__bf16)0.f};
-    const u32x4 *p = reinterpret_cast<const u32x4 *>(lds + (lane & 31) * kStride + (lane >> 5) * (DP / 2));
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) {
-        const uint32_t word = p[k][n];
-        s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, word), zeros, s, false);
-      }
-    return __any(s != s);
-  }
   // acc[channel][column] += sum over the 32 rows of lds.  The transposing read: in a group of 16 lanes, lane l addresses four
   // channels 4 (l % 4) .. of row l / 4 and receives channel l of the four rows.
   static __device__ __forceinline__ void outcome(const bf16 *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
@@ -391,15 +366,6 @@ struct Ops<float, DP> {
     for (int r = 0; r < 16; ++r) s[r & 1] += w.v[r];
     return s[0] + s[1];
   }
-  static __device__ __forceinline__ bool wild(const float *lds, int lane) {
-    const f32x4 *p = reinterpret_cast<const f32x4 *>(lds + (lane & 31) * kStride + (lane >> 5) * (DP / 2));
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < DP / 8; ++k)
-#pragma unroll
-      for (int n = 0; n < 4; ++n) s = fmaf(p[k][n], 0.f, s);
-    return __any(s != s);
-  }
   static __device__ __forceinline__ void outcome(const float *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
     const float *p = lds + 4 * (lane >> 5) * kStride + (lane & 31);
 #pragma unroll
@@ -409,31 +375,6 @@ struct Ops<float, DP> {
         acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(p[(8 * (r >> 2) + (r & 3)) * kStride + 32 * db], w.v[r], acc[db], 0, 0, 0);
   }
 };
-
-// acc[channel][column] += sum over the rows of lds that the column's lanes see, one by one: what is not seen has no part in it, whatever it
-// holds.  For tiles with infinities or NaN that some queries see and some do not.
-template <class T, int DP>
-__device__ __forceinline__ void outcome_of_seen(const T *lds, f32x16 w, uint32_t seen, int lane, f32x16 (&acc)[DP / 32]) {
-  const int g = lane >> 5;
-#pragma unroll 1
-  for (int r = 0; r < 16; ++r, seen >>= 1) {
-#pragma unroll 1
-    for (int half = 0; half < 2; ++half) {
-      const float weight = __shfl(w[0], (lane & 31) + 32 * half, 64);
-      const bool there = __shfl((int)seen, (lane & 31) + 32 * half, 64) & 1;
-      const T *const row = lds + rowmap(r, half) * Ops<T, DP>::kStride;
-#pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float x = load_as_f32(row + 32 * db + rowmap(k, g));
-          acc[db][k] = there ? fmaf(weight, x, acc[db][k]) : acc[db][k];
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 15; ++k) w[k] = w[k + 1];  // the next row's weight, without an index into registers
-  }
-}
 
 // ROWS rows of DP channels on their way from memory to LDS by THREADS threads: loaded into registers, written later.  PLAIN rows come by
 // buffer loads: a lane's offset in a tile never changes, the tile's place is in scalar registers, and what lies outside reads as zero without a
@@ -496,6 +437,41 @@ __device__ __forceinline__ void store_rows(f32x16 (&acc)[DP / 32], float scale, 
       }
     }
   }
+}
+
+// What a lane's row does not see has no part in its sum, but a product multiplies it by zero: an infinity or NaN leaves NaN.  Sums that are not
+// finite are formed again from what is seen alone, row by row, which costs its time only where there are such.
+template <int N>
+__device__ __forceinline__ bool not_finite(const f32x16 (&acc)[N]) {
+  float s = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s = fmaf(acc[n][r], 0.f, s);
+  return s != s;
+}
+// acc += weight(n, seen) row n of a head, for rows first .. last, in the lanes that see it and are `bad`
+template <class T, int DP, class F>
+__device__ __forceinline__ void add_rows(const T *head, int64_t stride, int first, int last, int D, int g, bool bad, f32x16 (&acc)[DP / 32], F &&weight) {
+#pragma unroll 1
+  for (int n = first; n <= last; ++n) {
+    bool seen;
+    const float w = weight(n, seen);
+    const T *const row = head + n * stride;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int col = 32 * db + rowmap(r, g);
+        const float x = col < D ? load_as_f32(row + col) : 0.f;
+        acc[db][r] = bad && seen ? fmaf(w, x, acc[db][r]) : acc[db][r];
+        if (r % 4 == 3) asm volatile("" ::: "memory");  // few loads at a time: this path must not cost the others registers
+      }
+  }
+}
+__device__ __forceinline__ float bias_at(const BiasArgs &b, const float *table, int off) {
+  const int low = table_low(b), at = off + low, n = table_size(b);
+  return table[at < 0 ? 0 : at < n ? at : n - 1];
 }
 
 template <int N>

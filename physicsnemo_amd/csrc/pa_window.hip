@@ -47,50 +47,38 @@ struct Running {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
   }
-  // z -> weights
-  template <int S>
-  __device__ __forceinline__ float weigh(f32x16 (&z)[S], typename O::Weights (&w)[S], float c) const {
-    float sum = 0.f;
+  // z -> weights; their sum
+  __device__ __forceinline__ float weigh(f32x16 &z, typename O::Weights &w, float c) const {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) z[s][r] = __builtin_amdgcn_exp2f(fmaf(z[s][r], c, off));
-      w[s] = O::pack(z[s]);
-      sum += O::sum(w[s]);
-    }
-    return sum;
+    for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], c, off));
+    w = O::pack(z);
+    return O::sum(w);
   }
-  template <int S>
-  __device__ __forceinline__ float highest(const f32x16 (&z)[S]) const {
-    float most = most_of(z[0]);
-#pragma unroll
-    for (int s = 1; s < S; ++s) most = fmaxf(most, most_of(z[s]));
-    return half_max(most);
-  }
-  // the weights of a tile that all queries see all of; scores(z) forms its z
-  template <int S, class F>
-  __device__ __forceinline__ void weights_of_all(typename O::Weights (&w)[S], float c, F &&scores) {
-    f32x16 z[S];
-    scores(z);
-    if (__builtin_expect(fresh, 0)) raise(highest(z), m == -INFINITY, c), fresh = false;
+  // the weights of a tile that all queries see all of; scores() forms its z
+  template <class F>
+  __device__ __forceinline__ typename O::Weights weights_of_all(float c, F &&scores) {
+    f32x16 z = scores();
+    typename O::Weights w;
+    if (__builtin_expect(fresh, 0)) raise(half_max(most_of(z)), m == -INFINITY, c), fresh = __any(m == -INFINITY);
     float sum = weigh(z, w, c);
     if (__builtin_expect(__any(!(sum <= kMost)), 0)) {
       const bool need = half_max(sum <= kMost ? 0.f : 1.f) > 0.f;
-      scores(z);
-      raise(highest(z), need, c);
+      z = scores();
+      raise(half_max(most_of(z)), need, c);
       sum = weigh(z, w, c);
     }
     l += sum;
+    return w;
   }
   // those of a tile in which some is hidden (z = -inf)
-  __device__ __forceinline__ typename O::Weights weights_of_some(f32x16 (&z)[1], float c) {
-    const float most = highest(z);
+  __device__ __forceinline__ typename O::Weights weights_of_some(f32x16 &z, float c) {
+    const float most = half_max(most_of(z));
     const bool need = m == -INFINITY || !(most * c + off <= kSlack);
     if (__any(need)) raise(most, need, c);
-    typename O::Weights w[1];
+    typename O::Weights w;
     l += weigh(z, w, c);
     if (fresh) fresh = __any(m == -INFINITY);
-    return w[0];
+    return w;
   }
 };
 
@@ -117,13 +105,13 @@ __device__ __forceinline__ f32x16 start_of(const Args &a, int q0, int i, int k0,
 }
 
 template <class T, int DP, bool PLAIN, bool BIAS>
-__global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forward_kernel(Args a) {
+__global__ __launch_bounds__(256) void forward_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
   float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
-  const int64_t work = own_work();
-  const int block = (int)(work % a.blocks), h = (int)(work / a.blocks % a.Hq), b = (int)(work / a.blocks / a.Hq);
+  const uint32_t work = own_work(), at_head = work / (uint32_t)a.blocks;
+  const int block = (int)(work - at_head * (uint32_t)a.blocks), b = (int)(at_head / (uint32_t)a.Hq), h = (int)(at_head - (uint32_t)b * (uint32_t)a.Hq);
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
   using O = Ops<T, DP>;
@@ -131,8 +119,6 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
   run.start(me < len);
   if (q0 < len) {
     typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
-    O::settle(own);
-    const Span span = keys_of(a, len, me);
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
@@ -144,6 +130,7 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       ks.store(tiles, threadIdx.x);
       vs.store(tiles + TILE, threadIdx.x);
     }
+    O::settle(own);
     __syncthreads();
     for (int n = 0; n < list.count; ++n) {
       const T *const kt = tiles + (n & 1) * 2 * TILE, *const vt = kt + TILE;
@@ -153,25 +140,19 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
         vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
       }
       const int k0 = list[n] * KT;
-      if (sight_of(a, len, qw, k0, KT) == kAll) {
-        typename O::Weights w[SUB];
-        run.weights_of_all(w, a.c, [&](f32x16 (&z)[SUB]) {
-#pragma unroll
-          for (int s = 0; s < SUB; ++s) z[s] = O::scores(kt + 32 * s * O::kStride, own, i, g, start_of<BIAS>(a, qw, me, k0 + 32 * s, g, table));
-        });
-#pragma unroll
-        for (int s = 0; s < SUB; ++s) O::outcome(vt + 32 * s * O::kStride, w[s], lane, run.o);
-      } else {
 #pragma unroll 1
-        for (int s = 0; s < SUB; ++s) {
-          const int r0 = k0 + 32 * s, sight = sight_of(a, len, qw, r0, 32);
-          if (sight == kNone) continue;
-          f32x16 z[1] = {O::scores(kt + 32 * s * O::kStride, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table))};
-          hide(z[0], span, sight & kEarly, sight & kLate, r0 < a.sinks, r0, g, -INFINITY);
+      for (int s = 0; s < SUB; ++s) {
+        const int r0 = k0 + 32 * s, sight = sight_of(a, len, qw, r0, 32);
+        const T *const krows = kt + 32 * s * O::kStride, *const vrows = vt + 32 * s * O::kStride;
+        auto scores = [&]() { return O::scores(krows, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table)); };
+        if (sight == kAll) {
+          O::outcome(vrows, run.weights_of_all(a.c, scores), lane, run.o);
+        } else if (sight != kNone) {
+          f32x16 z = scores();
+          const Span span = keys_of(a, len, me);
+          hide(z, span, sight & kEarly, sight & kLate, r0 < a.sinks, r0, g, -INFINITY);
           const typename O::Weights w = run.weights_of_some(z, a.c);
-          const T *const rows = vt + 32 * s * O::kStride;
-          if (__builtin_expect(sight != kAll && O::wild(rows, lane), 0)) outcome_of_seen<T, DP>(rows, z[0], span.seen(r0, g), lane, run.o);
-          else O::outcome(rows, w, lane, run.o);
+          O::outcome(vrows, w, lane, run.o);
         }
       }
       if (n + 1 < list.count) {
@@ -179,6 +160,22 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
         vs.store(next + TILE, threadIdx.x);
       }
       __syncthreads();
+    }
+    bool bad = not_finite(run.o);
+    if (__builtin_expect(__any(bad), 0)) {
+      bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      const Span span = keys_of(a, len, me);
+      for (int d = 0; d < DP / 32; ++d)
+        for (int r = 0; r < 16; ++r) run.o[d][r] = bad ? 0.f : run.o[d][r];
+      auto weight = [&](int j, bool &seen) {
+        seen = span.sees(j);
+        float z = half_sum(O::dot(own, O::template rows<PLAIN>(keys, a.k.row, j, len, true, a.D, g)));
+        if constexpr (BIAS) z += bias_at(a.bias, table, j - me);
+        return __builtin_amdgcn_exp2f(fmaf(z, a.c, run.off));
+      };
+      const int low = qw - a.left > 0 ? qw - a.left : 0, high = qw + 31 + a.right < len - 1 ? qw + 31 + a.right : len - 1;
+      add_rows<T, DP>(values, a.v.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, run.o, weight);
+      add_rows<T, DP>(values, a.v.row, low, high, a.D, g, bad, run.o, weight);
     }
   }
   const float l = half_sum(run.l);
@@ -258,24 +255,41 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
       wave_meets();  // lanes read what others wrote
       const typename O::Rows rows = next;
       if (n + by < list.count) fetch(n + by);
-      f32x16 z[1];
+      f32x16 z;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        z[0][r] = 0.f;
+        z[r] = 0.f;
         if constexpr (BIAS) {
           int d = me - (k0 + rowmap(r, g));
           d = d < 0 ? 0 : d < a.bias.distance ? d : a.bias.distance;
-          z[0][r] = biases[buckets[d] * s.G + gq];
+          z[r] = biases[buckets[d] * s.G + gq];
         }
       }
-      z[0] = O::scores(rows, own, z[0]);
+      z = O::scores(rows, own, z);
       const int k1 = k0 + 31;
       const bool early = k0 < last_q - a.left, late = k1 > first_q || len - s.T + t0 < 0;
-      hide(z[0], span, early, late, k0 < a.sinks, k0, g, -INFINITY);
+      hide(z, span, early, late, k0 < a.sinks, k0, g, -INFINITY);
       const typename O::Weights w = run.weights_of_some(z, a.c);
-      if (__builtin_expect((early || late) && O::wild(patch, lane), 0)) outcome_of_seen<T, DP>(patch, z[0], span.seen(k0, g), lane, run.o);
-      else O::outcome(patch, w, lane, run.o);
+      O::outcome(patch, w, lane, run.o);
       wave_meets();
+    }
+    bool bad = not_finite(run.o);
+    if (__builtin_expect(__any(bad), 0)) {
+      bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      for (int d = 0; d < DB; ++d)
+        for (int r = 0; r < 16; ++r) run.o[d][r] = bad ? 0.f : run.o[d][r];
+      for (n = part * 4 + wave; n < list.count; n += by) {
+        const int k0 = list[n] * 32, k1 = k0 + 31 < len ? k0 + 31 : len - 1;
+        add_rows<T, DP>(values, a.v.row, k0, k1, a.D, g, bad, run.o, [&](int j, bool &seen) {
+          seen = span.sees(j);
+          float z = half_sum(O::dot(own, O::template rows<PLAIN>(keys, a.k.row, j, len, true, a.D, g)));
+          if constexpr (BIAS) {
+            const int d = me - j;
+            z += biases[buckets[d < 0 ? 0 : d < a.bias.distance ? d : a.bias.distance] * s.G + gq];
+          }
+          return __builtin_amdgcn_exp2f(fmaf(z, a.c, run.off));
+        });
+      }
     }
   }
   // the four waves' results under one maximum

@@ -20,8 +20,8 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
   const int entries = BIAS ? table_size(a.bias) : 0;
   float *const sums = table + entries;  // DBIAS: [wave][offset]
-  const int64_t work = own_work();
-  const int block = (int)(work % a.blocks), h = (int)(work / a.blocks % a.Hq), b = (int)(work / a.blocks / a.Hq);
+  const uint32_t work = own_work(), at_head = work / (uint32_t)a.blocks;
+  const int block = (int)(work - at_head * (uint32_t)a.blocks), b = (int)(at_head / (uint32_t)a.Hq), h = (int)(at_head - (uint32_t)b * (uint32_t)a.Hq);
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
   using O = Ops<T, DP>;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           ks.load(a.k, keys, list[n + 1] * KT, len, a.D, threadIdx.x);
           vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
         }
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < SUB; ++s) {
           const int k0 = list[n] * KT + 32 * s;
           const int sight = sight_of(a, len, qw, k0, 32);
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
           if (sight != kAll) {
             hide(z, span, sight & kEarly, sight & kLate, k0 < a.sinks, k0, g, -INFINITY);
-            if (O::wild(vt + 32 * s * O::kStride, lane)) hide(dp, span, true, true, true, k0, g, 0.f);
+            if constexpr (DBIAS) hide(dp, span, sight & kEarly, sight & kLate, k0 < a.sinks, k0, g, 0.f);  // the bias sums take every element
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], a.c, -stat));
@@ -148,9 +148,24 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           else ahead += sum;
         }
       }
-      if (sight != kAll && O::wild(krows, lane)) outcome_of_seen<T, DP>(krows, p, span.seen(k0, g), lane, dq);
-      else O::outcome(krows, O::pack(p), lane, dq);
+      O::outcome(krows, O::pack(p), lane, dq);
     });
+    bool bad = not_finite(dq);
+    if (__builtin_expect(__any(bad), 0)) {
+      bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      for (int d = 0; d < DP / 32; ++d)
+        for (int r = 0; r < 16; ++r) dq[d][r] = bad ? 0.f : dq[d][r];
+      auto weight = [&](int j, bool &seen) {
+        seen = span.sees(j);
+        float z = half_sum(O::dot(own, O::template rows<PLAIN>(keys, a.k.row, j, len, true, a.D, g)));
+        const float by = half_sum(O::dot(dy, O::template rows<PLAIN>(values, a.v.row, j, len, true, a.D, g)));
+        if constexpr (BIAS) z += bias_at(a.bias, table, j - me);
+        return __builtin_amdgcn_exp2f(fmaf(z, a.c, -stat)) * (by - delta);
+      };
+      const int low = qw - a.left > 0 ? qw - a.left : 0, high = qw + 31 + a.right < len - 1 ? qw + 31 + a.right : len - 1;
+      add_rows<T, DP>(keys, a.k.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, dq, weight);
+      add_rows<T, DP>(keys, a.k.row, low, high, a.D, g, bad, dq, weight);
+    }
   }
   T *const row = static_cast<T *>(a.dq) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
   store_rows<T, DP>(dq, a.scale, me < len, row, me < a.N, a.D, g);
@@ -208,9 +223,9 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
   float *const table = stats + 4 * QT;
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int G = a.Hq / a.Hk, chunks = a.sink_chunks, per_head = a.blocks - (chunks > 0) + chunks;
-  const int64_t work = own_work();
-  int block = (int)(work % per_head), chunk = -1;
-  const int hk = (int)(work / per_head % a.Hk), b = (int)(work / per_head / a.Hk);
+  const uint32_t work = own_work(), at_head = work / (uint32_t)per_head;
+  int block = (int)(work - at_head * (uint32_t)per_head), chunk = -1;
+  const int b = (int)(at_head / (uint32_t)a.Hk), hk = (int)(at_head - (uint32_t)b * (uint32_t)a.Hk);
   if (chunks > 0) {
     if (block < chunks) chunk = block, block = 0;
     else block -= chunks - 1;
@@ -268,7 +283,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       const T *const qt = tiles + (n & 1) * 2 * TILE, *const gt = qt + TILE;
       const float *const lse = stats + (n & 1) * 2 * QT, *const delta = lse + QT;
       if (n + 1 < count) fetch(n + 1);
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
         const int q0 = (t0 + n % tiles_of_head) * QT + 32 * s;
         const int sight = sight_of(a, len, q0, kw, 32);
@@ -295,22 +310,40 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
         }
         z = O::scores(qrows, key, i, g, z);
         dp = O::scores(grows, value, i, g, dp);
-        bool wild = false;
-        if (sight != kAll) {  // a key that comes early for a query sees it late
+        if (sight != kAll)  // a key that comes early for a query sees it late
           hide(z, span, sight & kLate, (sight & kEarly) || q0 + 31 >= len, false, q0, g, -INFINITY);
-          wild = O::wild(grows, lane) || __any(!(fabsf(delta[32 * s + i]) < INFINITY));
-          if (wild) hide(dp, span, true, true, false, q0, g, 0.f);
-        }
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(z[r] * a.c);
-        if (wild) outcome_of_seen<T, DP>(grows, z, span.seen(q0, g), lane, dv);
-        else O::outcome(grows, O::pack(z), lane, dv);
+        O::outcome(grows, O::pack(z), lane, dv);
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] *= dp[r];
-        if (sight != kAll && O::wild(qrows, lane)) outcome_of_seen<T, DP>(qrows, z, span.seen(q0, g), lane, dk);
-        else O::outcome(qrows, O::pack(z), lane, dk);
+        O::outcome(qrows, O::pack(z), lane, dk);
       }
       if (n + 1 < count) put(n + 1);
+    }
+    bool bad = not_finite(dk) || not_finite(dv);
+    if (__builtin_expect(__any(bad), 0)) {
+      bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      for (int d = 0; d < DP / 32; ++d)
+        for (int r = 0; r < 16; ++r) dk[d][r] = bad ? 0.f : dk[d][r], dv[d][r] = bad ? 0.f : dv[d][r];
+      const int q_low = t0 * QT > kw - a.right ? t0 * QT : kw - a.right;
+      int q_high = t1 * QT + QT - 1 < len - 1 ? t1 * QT + QT - 1 : len - 1;
+      if (kw >= a.sinks && kw + 31 + a.left < q_high) q_high = kw + 31 + a.left;
+      for (int h = hk * G; h < hk * G + G; ++h) {
+        const T *const queries = head_of<T>(a.q, b, h), *const grads = head_of<T>(a.dy, b, h);
+        const int64_t first_stat = ((int64_t)b * a.Hq + h) * a.N;
+        auto p_of = [&](int n, bool &seen) {
+          seen = span.sees(n);
+          float z = half_sum(O::dot(key, O::template rows<PLAIN>(queries, a.q.row, n, len, true, a.D, g)));
+          if constexpr (BIAS) z += bias_start(a.bias.table[(int64_t)bucket_of_offset(a.bias, me - n) * a.Hq + h], a.c);
+          return __builtin_amdgcn_exp2f(fmaf(z, a.c, -a.saved_stats[first_stat + n]));
+        };
+        add_rows<T, DP>(grads, a.dy.row, q_low, q_high, a.D, g, bad, dv, p_of);
+        add_rows<T, DP>(queries, a.q.row, q_low, q_high, a.D, g, bad, dk, [&](int n, bool &seen) {
+          const float p = p_of(n, seen);
+          return p * (half_sum(O::dot(value, O::template rows<PLAIN>(grads, a.dy.row, n, len, true, a.D, g))) - a.delta[first_stat + n]);
+        });
+      }
     }
   }
   if (chunk < 0) {
