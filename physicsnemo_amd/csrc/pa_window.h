@@ -61,9 +61,12 @@ struct Args {
 
 __device__ __forceinline__ int length_of(const Args &a, int b) {
   if (!a.lengths) return a.N;
-  const int n = a.lengths[b];
+  const int n = __builtin_amdgcn_readfirstlane(a.lengths[b]);
   return n < 0 ? 0 : n > a.N ? a.N : n;
 }
+// whether it is so in some lane: a branch on this is one of the whole wave, and known as such (branches that are taken for divergent cost copies
+// of all sums that they change)
+__device__ __forceinline__ bool some_lane(bool v) { return __builtin_amdgcn_ballot_w64(v) != 0; }
 
 // Workgroup -> work: consecutive work on one XCD (workgroups go round them), whose L2 then holds what neighbours share
 __device__ __forceinline__ uint32_t own_work() {
@@ -110,12 +113,34 @@ __device__ __forceinline__ Reach reach_of(const BiasArgs &b, int least, int most
   return kNear;
 }
 
-// ---- visibility of n keys from k0 for the 32 queries from q0: none of it, or what has to be hidden ----
-enum : int { kAll = 0, kEarly = 1, kLate = 2, kNone = 4 };  // kEarly: keys before a query's window, kLate: behind it, or one of both outside the sequence
-__device__ __forceinline__ int sight_of(const Args &a, int len, int q0, int k0, int n) {
-  const int k1 = k0 + n - 1, q1 = q0 + 31;
-  if (k0 >= len || q0 >= len || k0 > q1 + a.right || (k1 < q0 - a.left && k0 >= a.sinks)) return kNone;
-  return (k0 < q1 - a.left && k1 >= a.sinks ? kEarly : 0) | (k1 > q0 + a.right || k1 >= len || q1 >= len ? kLate : 0);
+// ---- which tiles of 32 rows from r0 on a wave's 32 own rows see: some of it, or all.  Formed once, so that a tile costs a few scalar
+// comparisons (formed for each tile anew it cost 90 scalar instructions and a third of the time) ----
+struct Sights {
+  int low, high, first, full;  // some: low .. high or below `first`; all: full .. full + span
+  uint32_t span;
+  __device__ __forceinline__ bool none(int r0) const { return r0 > high || (r0 < low && r0 >= first); }
+  __device__ __forceinline__ bool all(int r0) const { return (uint32_t)(r0 - full) < span; }
+  __device__ __forceinline__ void set_full(int from, int to) {  // to: the last first row
+    full = from, span = to < from ? 0u : (uint32_t)(to - from) + 1u;
+  }
+};
+// keys for the queries from q0
+__device__ __forceinline__ Sights sights_of_queries(const Args &a, int len, int q0) {
+  Sights s;
+  const int last = q0 + 31 + a.right < len - 1 ? q0 + 31 + a.right : len - 1;
+  s.low = q0 - a.left - 31, s.high = q0 < len ? last : -1, s.first = q0 < len ? a.sinks : 0;
+  const int least = q0 + a.right < len - 1 ? q0 + a.right : len - 1;  // what the first of them sees
+  s.set_full(q0 + 31 - a.left > 0 ? q0 + 31 - a.left : 0, q0 + 31 < len ? least - 31 : -1);
+  return s;
+}
+// queries for the keys from k0
+__device__ __forceinline__ Sights sights_of_keys(const Args &a, int len, int k0) {
+  Sights s;
+  s.low = k0 - a.right - 31, s.first = 0;
+  s.high = k0 >= len ? -1 : k0 >= a.sinks && k0 + 31 + a.left < len - 1 ? k0 + 31 + a.left : len - 1;
+  const int least = k0 + 31 >= a.sinks && k0 + a.left < len - 1 ? k0 + a.left : len - 1;
+  s.set_full(k0 + 31 - a.right > 0 ? k0 + 31 - a.right : 0, k0 + 31 < len ? least - 31 : -1);
+  return s;
 }
 // The rows that lie in a lane's sight: low .. high, and those below `first`
 struct Span {
@@ -140,7 +165,7 @@ __device__ __forceinline__ Span queries_of(const Args &a, int len, int j) {
   s.first = 0;
   return s;
 }
-// z <- instead where the row is out of sight, on the sides that are asked for; `first`: some of the tile's rows may be seen as first ones
+// z <- instead where the row of a tile is out of sight; FIRST: some of its rows may be seen as first ones
 template <bool FIRST>
 __device__ __forceinline__ void hide_low(f32x16 &z, const Span &span, int r0, int g, float instead) {
   const int lo = span.low - r0 - 4 * g, of_first = span.first - r0 - 4 * g;
@@ -155,10 +180,10 @@ __device__ __forceinline__ void hide_high(f32x16 &z, const Span &span, int r0, i
 #pragma unroll
   for (int r = 0; r < 16; ++r) z[r] = 8 * (r >> 2) + (r & 3) <= hi ? z[r] : instead;
 }
-__device__ __forceinline__ void hide(f32x16 &z, const Span &span, bool low, bool high, bool first, int r0, int g, float instead) {
-  if (low && first) hide_low<true>(z, span, r0, g, instead);
-  else if (low) hide_low<false>(z, span, r0, g, instead);
-  if (high) hide_high(z, span, r0, g, instead);
+__device__ __forceinline__ void hide(f32x16 &z, const Span &span, int r0, int g, float instead) {
+  if (some_lane(span.first > r0)) hide_low<true>(z, span, r0, g, instead);
+  else if (some_lane(span.low > r0)) hide_low<false>(z, span, r0, g, instead);
+  if (some_lane(span.high < r0 + 31)) hide_high(z, span, r0, g, instead);
 }
 
 // The key tiles of kt rows that queries from q0 to q1 of a sequence see: those of the sinks, then those of the window

@@ -13,7 +13,7 @@
 namespace pa {
 namespace window {
 
-constexpr float kMost = 65536.f, kSlack = 16.f;  // how far a tile's weights, log2 of a weight may rise above the reference before all is scaled again
+constexpr float kMost = 1073741824.f, kSlack = 16.f;  // how far weights may sum up, log2 of one may lie above the reference before it is taken again
 
 __device__ __forceinline__ float most_of(const f32x16 &z) {
   float m = z[0];
@@ -22,9 +22,7 @@ __device__ __forceinline__ float most_of(const f32x16 &z) {
   return m;
 }
 
-// The softmax of a wave's queries so far, and the values' sum under it.  The reference is not the largest score so far but one that none has
-// passed by much: only a tile whose weights sum up past kMost is looked through for its maximum and taken again, and the first ones,
-// until every query has seen something.
+// The softmax of a wave's queries so far, and the values' sum under it.  A query's numbers depend on its own scores alone.
 template <class T, int DP>
 struct Running {
   using O = Ops<T, DP>;
@@ -36,8 +34,26 @@ struct Running {
     m = live ? -INFINITY : 0.f, l = 0.f, off = 0.f;
     fresh = true;
   }
-  // for the queries that need it, so that none depends on which others are in its wave
-  __device__ __forceinline__ void raise(float most, bool need, float c) {
+  // the largest score of the first tile that a query sees something of is its reference
+  __device__ __forceinline__ void refer(const f32x16 &z, float c) {
+    const float most = half_max(most_of(z));
+    m = m == -INFINITY ? most : m;
+    off = m == -INFINITY ? 0.f : -m * c;
+    fresh = some_lane(m == -INFINITY);
+  }
+  // z -> weights
+  __device__ __forceinline__ typename O::Weights weigh(f32x16 &z, float c) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], c, off));
+    const typename O::Weights w = O::pack(z);
+    l += O::sum(w);
+    return w;
+  }
+  // a larger reference where this tile's largest score asks for it, and all that is summed so far under it
+  __device__ __forceinline__ void raise(const f32x16 &z, float c) {
+    const float most = half_max(most_of(z));
+    const bool need = m == -INFINITY || !(most * c + off <= kSlack);
+    if (!some_lane(need)) return;
     const float now = need ? fmaxf(m, most) : m, ref = now == -INFINITY ? 0.f : now;
     const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
     m = now, off = -ref * c;
@@ -46,39 +62,6 @@ struct Running {
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
-  }
-  // z -> weights; their sum
-  __device__ __forceinline__ float weigh(f32x16 &z, typename O::Weights &w, float c) const {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], c, off));
-    w = O::pack(z);
-    return O::sum(w);
-  }
-  // the weights of a tile that all queries see all of; scores() forms its z
-  template <class F>
-  __device__ __forceinline__ typename O::Weights weights_of_all(float c, F &&scores) {
-    f32x16 z = scores();
-    typename O::Weights w;
-    if (__builtin_expect(fresh, 0)) raise(half_max(most_of(z)), m == -INFINITY, c), fresh = __any(m == -INFINITY);
-    float sum = weigh(z, w, c);
-    if (__builtin_expect(__any(!(sum <= kMost)), 0)) {
-      const bool need = half_max(sum <= kMost ? 0.f : 1.f) > 0.f;
-      z = scores();
-      raise(half_max(most_of(z)), need, c);
-      sum = weigh(z, w, c);
-    }
-    l += sum;
-    return w;
-  }
-  // those of a tile in which some is hidden (z = -inf)
-  __device__ __forceinline__ typename O::Weights weights_of_some(f32x16 &z, float c) {
-    const float most = half_max(most_of(z));
-    const bool need = m == -INFINITY || !(most * c + off <= kSlack);
-    if (__any(need)) raise(most, need, c);
-    typename O::Weights w;
-    l += weigh(z, w, c);
-    if (fresh) fresh = __any(m == -INFINITY);
-    return w;
   }
 };
 
@@ -105,7 +88,7 @@ __device__ __forceinline__ f32x16 start_of(const Args &a, int q0, int i, int k0,
 }
 
 template <class T, int DP, bool PLAIN, bool BIAS>
-__global__ __launch_bounds__(256) void forward_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forward_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
@@ -123,46 +106,63 @@ __global__ __launch_bounds__(256) void forward_kernel(Args a) {
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
     if constexpr (BIAS) fill_bias_table(a, h, table);
+    const Sights sights = sights_of_queries(a, len, qw);
     Stage<T, DP, PLAIN, KT, 256> ks, vs;
-    if (list.count > 0) {
-      ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
-      vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
-      ks.store(tiles, threadIdx.x);
-      vs.store(tiles + TILE, threadIdx.x);
-    }
-    O::settle(own);
-    __syncthreads();
-    for (int n = 0; n < list.count; ++n) {
-      const T *const kt = tiles + (n & 1) * 2 * TILE, *const vt = kt + TILE;
-      T *const next = tiles + ((n + 1) & 1) * 2 * TILE;
-      if (n + 1 < list.count) {
-        ks.load(a.k, keys, list[n + 1] * KT, len, a.D, threadIdx.x);
-        vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
-      }
-      const int k0 = list[n] * KT;
-#pragma unroll 1
-      for (int s = 0; s < SUB; ++s) {
-        const int r0 = k0 + 32 * s, sight = sight_of(a, len, qw, r0, 32);
-        const T *const krows = kt + 32 * s * O::kStride, *const vrows = vt + 32 * s * O::kStride;
-        auto scores = [&]() { return O::scores(krows, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table)); };
-        if (sight == kAll) {
-          O::outcome(vrows, run.weights_of_all(a.c, scores), lane, run.o);
-        } else if (sight != kNone) {
-          f32x16 z = scores();
-          const Span span = keys_of(a, len, me);
-          hide(z, span, sight & kEarly, sight & kLate, r0 < a.sinks, r0, g, -INFINITY);
-          const typename O::Weights w = run.weights_of_some(z, a.c);
-          O::outcome(vrows, w, lane, run.o);
-        }
-      }
-      if (n + 1 < list.count) {
-        ks.store(next, threadIdx.x);
-        vs.store(next + TILE, threadIdx.x);
+    auto scores = [&](const T *rows, int r0) {
+      f32x16 z = O::scores(rows, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table));
+      if (!sights.all(r0)) hide(z, keys_of(a, len, me), r0, g, -INFINITY);
+      return z;
+    };
+    // all tiles of keys, and of values if they are wanted: f(keys, values, first key) for each sub-tile in sight.  Nothing in it changes the
+    // values' sum but the products: a scaling in a branch would cost copies of the sum around every tile.
+    auto pass = [&](bool both, auto &&f) {
+      if (list.count > 0) {
+        ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
+        if (both) vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
+        O::settle(own);
+        ks.store(tiles, threadIdx.x);
+        if (both) vs.store(tiles + TILE, threadIdx.x);
       }
       __syncthreads();
+      for (int n = 0; n < list.count; ++n) {
+        const T *const kt = tiles + (n & 1) * 2 * TILE, *const vt = kt + TILE;
+        T *const next = tiles + ((n + 1) & 1) * 2 * TILE;
+        if (n + 1 < list.count) {
+          ks.load(a.k, keys, list[n + 1] * KT, len, a.D, threadIdx.x);
+          if (both) vs.load(a.v, values, list[n + 1] * KT, len, a.D, threadIdx.x);
+        }
+        const int k0 = list[n] * KT;
+#pragma unroll 1
+        for (int s = 0; s < SUB; ++s) {
+          if (sights.none(k0 + 32 * s)) continue;
+          f(kt + 32 * s * O::kStride, vt + 32 * s * O::kStride, k0 + 32 * s);
+        }
+        if (n + 1 < list.count) {
+          ks.store(next, threadIdx.x);
+          if (both) vs.store(next + TILE, threadIdx.x);
+        }
+        __syncthreads();
+      }
+    };
+    for (bool again = false;; again = true) {
+      pass(true, [&](const T *krows, const T *vrows, int r0) {
+        f32x16 z = scores(krows, r0);
+        if (__builtin_expect(run.fresh, 0)) run.refer(z, a.c);
+        O::outcome(vrows, run.weigh(z, a.c), lane, run.o);
+      });
+      // Scores far above the first ones: those queries take their largest score for the reference, and the workgroup goes over the keys again
+      const bool high = half_max(run.l <= kMost ? 0.f : 1.f) > 0.f;
+      if (again || !__syncthreads_or(high)) break;
+      float most = -INFINITY;
+      pass(false, [&](const T *krows, const T *, int r0) { most = fmaxf(most, most_of(scores(krows, r0))); });
+      most = half_max(most);
+      zero(run.o);
+      run.l = 0.f;
+      run.m = high ? most : run.m;
+      run.off = run.m == -INFINITY ? 0.f : -run.m * a.c;
     }
     bool bad = not_finite(run.o);
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
       const Span span = keys_of(a, len, me);
       for (int d = 0; d < DP / 32; ++d)
@@ -266,15 +266,14 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
         }
       }
       z = O::scores(rows, own, z);
-      const int k1 = k0 + 31;
-      const bool early = k0 < last_q - a.left, late = k1 > first_q || len - s.T + t0 < 0;
-      hide(z, span, early, late, k0 < a.sinks, k0, g, -INFINITY);
-      const typename O::Weights w = run.weights_of_some(z, a.c);
+      hide(z, span, k0, g, -INFINITY);
+      run.raise(z, a.c);
+      const typename O::Weights w = run.weigh(z, a.c);
       O::outcome(patch, w, lane, run.o);
       wave_meets();
     }
     bool bad = not_finite(run.o);
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
       for (int d = 0; d < DB; ++d)
         for (int r = 0; r < 16; ++r) run.o[d][r] = bad ? 0.f : run.o[d][r];

@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           O::template rows<PLAIN>(static_cast<const T *>(a.saved_y) + ((int64_t)b * a.N * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, me, len, me < len, a.D, g);
       delta = half_sum(O::dot(y, dy));
     }
-    const Span span = keys_of(a, len, me);
+    const Sights sights = sights_of_queries(a, len, qw);
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
@@ -72,8 +72,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
 #pragma unroll 1
         for (int s = 0; s < SUB; ++s) {
           const int k0 = list[n] * KT + 32 * s;
-          const int sight = sight_of(a, len, qw, k0, 32);
-          if (sight == kNone) continue;
+          if (sights.none(k0)) continue;
           const T *const krows = kt + 32 * s * O::kStride;
           f32x16 z, dp = start;
           Reach reach = kNear;
@@ -94,13 +93,14 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           }
           z = O::scores(krows, own, i, g, z);
           dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
-          if (sight != kAll) {
-            hide(z, span, sight & kEarly, sight & kLate, k0 < a.sinks, k0, g, -INFINITY);
-            if constexpr (DBIAS) hide(dp, span, sight & kEarly, sight & kLate, k0 < a.sinks, k0, g, 0.f);  // the bias sums take every element
+          if (!sights.all(k0)) {
+            const Span span = keys_of(a, len, me);
+            hide(z, span, k0, g, -INFINITY);
+            if constexpr (DBIAS) hide(dp, span, k0, g, 0.f);  // the bias sums take every element
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], a.c, -stat));
-          f(krows, z, dp, k0, reach, sight);
+          f(krows, z, dp, k0, reach);
         }
         if (n + 1 < list.count) {
           ks.store(next, threadIdx.x);
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
     if constexpr (DBIAS) {
       // the denominator, too: for bf16 the forward pass summed the weights as it multiplied them, rounded
       float part = 0.f, total = 0.f;
-      pass(0.f, [&](const T *, f32x16 &p, f32x16 &dp, int, Reach, int) {
+      pass(0.f, [&](const T *, f32x16 &p, f32x16 &dp, int, Reach) {
         float sum = 0.f, weights = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum = fmaf(p[r], dp[r], sum), weights += p[r];
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
       }
     }
     if (g == 0 && me < len) a.delta[at] = delta;
-    pass(-delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach, int sight) {
+    pass(-delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] *= dp[r];
       if constexpr (DBIAS) {
@@ -151,8 +151,9 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
       O::outcome(krows, O::pack(p), lane, dq);
     });
     bool bad = not_finite(dq);
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      const Span span = keys_of(a, len, me);
       for (int d = 0; d < DP / 32; ++d)
         for (int r = 0; r < 16; ++r) dq[d][r] = bad ? 0.f : dq[d][r];
       auto weight = [&](int j, bool &seen) {
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
     typename O::Rows key = O::template rows<PLAIN>(head_of<T>(a.k, b, hk), a.k.row, me, len, me < len, a.D, g);
     typename O::Rows value = O::template rows<PLAIN>(head_of<T>(a.v, b, hk), a.v.row, me, len, me < len, a.D, g);
     O::settle(key), O::settle(value);
-    const Span span = queries_of(a, len, me);
+    const Sights sights = sights_of_keys(a, len, kw);
     // queries that see a key of the block: i >= j - right, and i <= j + left or j a sink
     int first = k0 - a.right > 0 ? k0 - a.right : 0, last = k0 + 127 + a.left;
     if (chunk >= 0 || last > len - 1) last = len - 1;
@@ -286,8 +287,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
         const int q0 = (t0 + n % tiles_of_head) * QT + 32 * s;
-        const int sight = sight_of(a, len, q0, kw, 32);
-        if (sight == kNone) continue;
+        if (sights.none(q0)) continue;
         const T *const qrows = qt + 32 * s * O::kStride, *const grows = gt + 32 * s * O::kStride;
         f32x16 z, dp;
 #pragma unroll
@@ -310,8 +310,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
         }
         z = O::scores(qrows, key, i, g, z);
         dp = O::scores(grows, value, i, g, dp);
-        if (sight != kAll)  // a key that comes early for a query sees it late
-          hide(z, span, sight & kLate, (sight & kEarly) || q0 + 31 >= len, false, q0, g, -INFINITY);
+        if (!sights.all(q0)) hide(z, queries_of(a, len, me), q0, g, -INFINITY);
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(z[r] * a.c);
         O::outcome(grows, O::pack(z), lane, dv);
@@ -322,8 +321,9 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       if (n + 1 < count) put(n + 1);
     }
     bool bad = not_finite(dk) || not_finite(dv);
-    if (__builtin_expect(__any(bad), 0)) {
+    if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
+      const Span span = queries_of(a, len, me);
       for (int d = 0; d < DP / 32; ++d)
         for (int r = 0; r < 16; ++r) dk[d][r] = bad ? 0.f : dk[d][r], dv[d][r] = bad ? 0.f : dv[d][r];
       const int q_low = t0 * QT > kw - a.right ? t0 * QT : kw - a.right;
