@@ -16,6 +16,7 @@ namespace pa {
 namespace rotate {
 
 using mfma::u32x2;
+using mfma::u32x4;
 
 struct Side {
   const void *x, *dy;  // dy: backward
@@ -30,8 +31,27 @@ struct Args {
   float *partials;  // backward: [workgroup][2][D]
   int64_t points, N, position_batch;
   int Hq, Hk, D, half, axes, position_type, interleaved, norm, per_block;  // half: pairs that are turned
+  uint32_t by_heads, by_half;  // 2^32 over Hq + Hk and over half, rounded up
   float eps;
 };
+
+// where point first + n lies, first being row r0 of sequence b0: 64-bit divisions once a workgroup's pass, not once a row
+struct Spot {
+  int64_t b, r;
+};
+__device__ __forceinline__ Spot spot_of(const Args &a, const Spot &first, int n) {
+  Spot s = {first.b, first.r + n};
+  if (a.N >= a.per_block) {
+    const bool over = s.r >= a.N;
+    s.b += over, s.r -= over ? a.N : 0;
+  } else {  // N < 32
+    const uint32_t r = (uint32_t)s.r, whole = r / (uint32_t)a.N;
+    s.b += whole, s.r = r - whole * (uint32_t)a.N;
+  }
+  return s;
+}
+// n / d for n < 2^18, d <= 2^13, by = ceil(2^32 / d)
+__device__ __forceinline__ int quotient(int n, uint32_t by, int d) { return d == 1 ? n : (int)__umulhi((uint32_t)n, by); }
 
 // ---- cos and sin of a point's angle ----
 __device__ __forceinline__ double position(const Args &a, int64_t at) {
@@ -47,8 +67,8 @@ __device__ __forceinline__ double turns(double pos, double f) {
   const double u = t * hi, rest = fma(t, hi, -u) + fma(t, lo, t_rest * hi);
   return (u - rint(u)) + rest;
 }
-__device__ __forceinline__ float2 cos_sin(const Args &a, int64_t point, int p) {
-  const int64_t b = point / a.N, n = point - b * a.N, at = b * a.position_batch + n * a.axes;
+__device__ __forceinline__ float2 cos_sin(const Args &a, const Spot &spot, int p) {
+  const int64_t at = spot.b * a.position_batch + spot.r * a.axes;
   double turn = 0;
   for (int x = 0; x < a.axes; ++x) turn += turns(position(a, at + x), (double)a.frequencies[x * a.half + p]);
   const double quarters = turn * 4, whole = rint(quarters);
@@ -64,187 +84,230 @@ __device__ __forceinline__ float2 cos_sin(const Args &a, int64_t point, int p) {
   return (k & 2) ? make_float2(-c, -s) : make_float2(c, s);
 }
 
-// ---- a lane's eight channels: pairs j of (first(j), second(j)) ----
-struct Place {
-  int a[4], b[4];  // channels of the pairs, in the order the registers hold them
-  int at0, at1;    // UNITS: where the two pieces of four start
-  bool turned[4];
-};
-template <bool INTERLEAVED>
-__device__ __forceinline__ Place place_of(const Args &a, int slot, bool units) {
-  Place p;
-  p.at0 = 8 * slot, p.at1 = 8 * slot + 4;
+// ---- a lane's eight channels ----
+// kNeighbours: pairs (2 p, 2 p + 1), eight channels in a row, whole pairs.  kQuarters: pairs (p, p + half) of whole fours: four channels of the first
+// half and theirs of the second (behind the halves eight in a row).  kApart: pairs (p, p + half) of any half: eight channels in a row, their
+// partners' values through LDS.
+enum Pairs { kNeighbours, kQuarters, kApart };
+typedef u32x4 unit_at4 __attribute__((aligned(4)));
+typedef u32x4 unit_at2 __attribute__((aligned(2)));
+typedef u32x2 half_at2 __attribute__((aligned(2)));
+__device__ __forceinline__ void load4(const float *p, float *v) {
+  const u32x4 w = *reinterpret_cast<const unit_at4 *>(p);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int pair = 4 * slot + j;
-    p.turned[j] = pair < a.half;
-    if (INTERLEAVED || !p.turned[j]) {
-      p.a[j] = 2 * pair, p.b[j] = 2 * pair + 1;
-      if (!INTERLEAVED && units) p.a[j] = 8 * slot + j, p.b[j] = 8 * slot + 4 + j;  // no pairs there: any will do
-    } else {
-      p.a[j] = pair, p.b[j] = pair + a.half;
-      p.at0 = 4 * slot, p.at1 = 4 * slot + a.half;
-    }
+    const uint32_t b = w[j];
+    v[j] = __uint_as_float(b);
   }
-  return p;
 }
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void load4(const float *p, float (&v)[4]) {
-  const f32x4 w = *reinterpret_cast<const f32x4 *>(p);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = w[j];
-}
-__device__ __forceinline__ void load4(const bf16 *p, float (&v)[4]) {
-  const u32x2 w = *reinterpret_cast<const u32x2 *>(p);
+__device__ __forceinline__ void load4(const bf16 *p, float *v) {
+  const u32x2 w = *reinterpret_cast<const half_at2 *>(p);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const uint32_t b = w[j / 2];
     v[j] = __uint_as_float(j & 1 ? b & 0xffff0000u : b << 16);
   }
 }
-__device__ __forceinline__ void store4(float *p, const float (&v)[4]) {
-  f32x4 w;
+__device__ __forceinline__ void load8(const float *p, float *v) { load4(p, v), load4(p + 4, v + 4); }
+__device__ __forceinline__ void load8(const bf16 *p, float *v) {
+  const u32x4 w = *reinterpret_cast<const unit_at2 *>(p);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = v[j];
-  *reinterpret_cast<f32x4 *>(p) = w;
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t b = w[j / 2];
+    v[j] = __uint_as_float(j & 1 ? b & 0xffff0000u : b << 16);
+  }
 }
-__device__ __forceinline__ void store4(bf16 *p, const float (&v)[4]) {
+__device__ __forceinline__ void store4(float *p, const float *v) {
+  u32x4 w;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[j]);
+  *reinterpret_cast<unit_at4 *>(p) = w;
+}
+__device__ __forceinline__ void store4(bf16 *p, const float *v) {
   u32x2 w;
   w[0] = mfma::pack2(v[0], v[1]);
   w[1] = mfma::pack2(v[2], v[3]);
-  *reinterpret_cast<u32x2 *>(p) = w;
+  *reinterpret_cast<half_at2 *>(p) = w;
 }
-// UNITS: heads are whole pieces of eight channels on boundaries of four, and so are the turned halves
-template <class T, bool UNITS, bool INTERLEAVED>
-__device__ __forceinline__ void load_row(const T *row, const Place &p, int D, float (&a)[4], float (&b)[4]) {
-  if constexpr (UNITS) {
-    float lo[4] = {}, hi[4] = {};
-    if (p.a[0] < D) load4(row + p.at0, lo), load4(row + p.at1, hi);
+__device__ __forceinline__ void store8(float *p, const float *v) { store4(p, v), store4(p + 4, v + 4); }
+__device__ __forceinline__ void store8(bf16 *p, const float *v) {
+  u32x4 w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (INTERLEAVED) {
-        a[j] = j < 2 ? lo[2 * j] : hi[2 * j - 4];
-        b[j] = j < 2 ? lo[2 * j + 1] : hi[2 * j - 3];
-      } else {
-        a[j] = lo[j], b[j] = hi[j];
-      }
-    }
+  for (int j = 0; j < 4; ++j) w[j] = mfma::pack2(v[2 * j], v[2 * j + 1]);
+  *reinterpret_cast<unit_at2 *>(p) = w;
+}
+
+// where the two fours of a lane's channels start
+struct Place {
+  int at0, at1;
+};
+template <Pairs PAIRS>
+__device__ __forceinline__ Place place_of(int half, int slot) {
+  if (PAIRS == kQuarters && 4 * slot < half) return {4 * slot, 4 * slot + half};
+  return {8 * slot, 8 * slot + 4};
+}
+template <class T, Pairs PAIRS>
+__device__ __forceinline__ void load_row(const T *row, const Place &p, int D, float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  if constexpr (PAIRS == kQuarters) {  // D is whole eights
+    if (p.at0 < D) load4(row + p.at0, v), load4(row + p.at1, v + 4);
+  } else if (p.at0 + 8 <= D) {
+    load8(row + p.at0, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a[j] = p.a[j] < D ? load_as_f32(row + p.a[j]) : 0.f;
-      b[j] = p.b[j] < D ? load_as_f32(row + p.b[j]) : 0.f;
-    }
+    for (int j = 0; j < 8; ++j)
+      if (p.at0 + j < D) v[j] = load_as_f32(row + p.at0 + j);
   }
 }
-template <class T, bool UNITS, bool INTERLEAVED>
-__device__ __forceinline__ void store_row(T *row, const Place &p, int D, const float (&a)[4], const float (&b)[4]) {
-  if constexpr (UNITS) {
-    float lo[4], hi[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (INTERLEAVED) {
-        lo[j] = j & 1 ? b[j / 2] : a[j / 2];
-        hi[j] = j & 1 ? b[2 + j / 2] : a[2 + j / 2];
-      } else {
-        lo[j] = a[j], hi[j] = b[j];
-      }
-    }
-    if (p.a[0] < D) store4(row + p.at0, lo), store4(row + p.at1, hi);
+template <class T, Pairs PAIRS>
+__device__ __forceinline__ void store_row(T *row, const Place &p, int D, const float (&v)[8]) {
+  if constexpr (PAIRS == kQuarters) {
+    if (p.at0 < D) store4(row + p.at0, v), store4(row + p.at1, v + 4);
+  } else if (p.at0 + 8 <= D) {
+    store8(row + p.at0, v);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (p.a[j] < D) store_from_f32(row + p.a[j], a[j]);
-      if (p.b[j] < D) store_from_f32(row + p.b[j], b[j]);
-    }
+    for (int j = 0; j < 8; ++j)
+      if (p.at0 + j < D) store_from_f32(row + p.at0 + j, v[j]);
   }
 }
 
+// kApart: where each of a lane's channels finds its partner in the exchange and its pair in the point's turns, and which way its partner's part goes
+struct Partners {
+  int other[8], pair[8];
+  float sign[8];
+};
+__device__ __forceinline__ int spread(int c) { return c + (c >> 3); }  // a gap every eight floats spreads lanes over the banks
+template <int LANES>
+__device__ __forceinline__ Partners partners_of(int half, int slot) {
+  Partners p;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = 8 * slot + j;
+    const bool lower = c < half, turned = c < 2 * half;
+    p.other[j] = spread(!turned ? c : lower ? c + half : c - half);
+    p.pair[j] = !turned ? half : lower ? c : c - half;  // behind the pairs: one that turns nothing
+    p.sign[j] = lower ? -1.f : 1.f;
+  }
+  return p;
+}
+
+// v <- v turned by the point's angles (cs: cos and sin of its pairs), backwards with sign = -1
+template <Pairs PAIRS, int LANES>
+__device__ __forceinline__ void turn(float (&v)[8], const float2 *cs, int half, int slot, float sign, float *exchange, const Partners &p) {
+  if constexpr (PAIRS != kApart) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int a = PAIRS == kNeighbours ? 2 * j : j, b = PAIRS == kNeighbours ? 2 * j + 1 : j + 4, pair = 4 * slot + j;
+      const float2 t = pair < half ? cs[pair] : make_float2(1.f, 0.f);
+      const float x = v[a], y = v[b];
+      v[a] = x * t.x - sign * y * t.y;
+      v[b] = sign * x * t.y + y * t.x;
+    }
+  } else {
+    // the lanes of a row are lanes of one wave, whose LDS accesses happen in order
+    float *const mine = exchange + threadIdx.x / LANES * (9 * LANES + 1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine[9 * slot + j] = v[j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 t = cs[p.pair[j]];
+      v[j] = fmaf(v[j], t.x, mine[p.other[j]] * (sign * p.sign[j] * t.y));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// sum over groups of LANES neighbouring lanes, in every lane
 template <int LANES>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int off = 1; off < LANES; off <<= 1) v += __shfl_xor(v, off, 64);
+  auto step = [](float x, auto ctrl) {
+    constexpr int c = decltype(ctrl)::value;
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), c, 0xf, 0xf, true));
+  };
+  if constexpr (LANES >= 2) v = step(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1,0,3,2]
+  if constexpr (LANES >= 4) v = step(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2,3,0,1]
+  if constexpr (LANES >= 8) v = step(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  if constexpr (LANES >= 16) v = step(v, std::integral_constant<int, 0x140>{}); // row_mirror
   return v;
 }
 
-// cos and sin of per_block points from `first` on, [point][pair]
-__device__ __forceinline__ void fill_turns(const Args &a, int64_t first, int points, float2 *cs) {
+// cos and sin of the points from `first` on, [point][pair], and behind a point's pairs one that turns nothing
+__device__ __forceinline__ void fill_turns(const Args &a, const Spot &first, int points, float2 *cs) {
   for (int u = threadIdx.x; u < points * a.half; u += blockDim.x) {
-    const int n = u / a.half;
-    cs[u] = cos_sin(a, first + n, u - n * a.half);
+    const int n = quotient(u, a.by_half, a.half), p = u - n * a.half;
+    cs[n * (a.half + 1) + p] = cos_sin(a, spot_of(a, first, n), p);
   }
+  if ((int)threadIdx.x < points) cs[threadIdx.x * (a.half + 1) + a.half] = make_float2(1.f, 0.f);
 }
 
 // LANES lanes a row; a workgroup takes per_block points at a time, their rows (heads of q, then of k) one after the other
-template <class T, bool UNITS, bool INTERLEAVED, int LANES, bool BACK>
+template <class T, Pairs PAIRS, int LANES, bool BACK>
 __global__ __launch_bounds__(256) void rows_kernel(Args a) {
   extern __shared__ float2 cs[];
+  float *const exchange = reinterpret_cast<float *>(cs + a.per_block * (a.half + 1));
   const int slot = threadIdx.x % LANES, group = threadIdx.x / LANES;
   constexpr int GROUPS = 256 / LANES;
   const int H = a.Hq + a.Hk, D = a.D;
-  const Place at = place_of<INTERLEAVED>(a, slot, UNITS);
+  const Place place = place_of<PAIRS>(a.half, slot);
+  auto channel = [&](int j) { return j < 4 ? place.at0 + j : place.at1 + j - 4; };
+  const Partners partners = partners_of<LANES>(a.half, slot);
   const float inv = 1.f / (float)D;
-  float wq[2][4], wk[2][4], sq[2][4] = {}, sk[2][4] = {};  // weights, sums of their gradients: first, second of the pairs
+  float wq[8], wk[8], sq[8] = {}, sk[8] = {};  // weights, sums of their gradients
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    wq[0][j] = a.norm && a.q.weight && at.a[j] < D ? a.q.weight[at.a[j]] : 1.f;
-    wq[1][j] = a.norm && a.q.weight && at.b[j] < D ? a.q.weight[at.b[j]] : 1.f;
-    wk[0][j] = a.norm && a.k.weight && at.a[j] < D ? a.k.weight[at.a[j]] : 1.f;
-    wk[1][j] = a.norm && a.k.weight && at.b[j] < D ? a.k.weight[at.b[j]] : 1.f;
+  for (int j = 0; j < 8; ++j) {
+    wq[j] = a.norm && a.q.weight && channel(j) < D ? a.q.weight[channel(j)] : 1.f;
+    wk[j] = a.norm && a.k.weight && channel(j) < D ? a.k.weight[channel(j)] : 1.f;
   }
   for (int64_t first = (int64_t)blockIdx.x * a.per_block; first < a.points; first += (int64_t)gridDim.x * a.per_block) {
     const int points = (int)(a.points - first < a.per_block ? a.points - first : a.per_block);
     __syncthreads();  // the pass before has read its turns
-    fill_turns(a, first, points, cs);
+    const Spot start = {first / a.N, first % a.N};
+    fill_turns(a, start, points, cs);
     __syncthreads();
-    for (int row = group; row < (points * H + GROUPS - 1) / GROUPS * GROUPS; row += GROUPS) {  // all lanes: the sums exchange
-      const int n = row / H, h = row - n * H;
-      const bool live = n < points, key = h >= a.Hq;
+    const int rows = points * H;
+    for (int row = group; row < (rows + GROUPS - 1) / GROUPS * GROUPS; row += GROUPS) {  // all lanes: the sums exchange
+      const bool live = row < rows;
+      const int n = live ? quotient(row, a.by_heads, H) : 0, h = live ? row - n * H : 0;
+      const bool key = h >= a.Hq;
       const Side &s = key ? a.k : a.q;
-      const int64_t point = first + (live ? n : 0), b = point / a.N, r = point - b * a.N;
+      const Spot spot = spot_of(a, start, n);
       const int head = key ? h - a.Hq : h;
-      const T *x = static_cast<const T *>(s.x) + b * s.batch + r * s.row + head * s.head;
-      T *out = static_cast<T *>(s.out) + ((point * (key ? a.Hk : a.Hq)) + head) * D;
-      float xa[4], xb[4];
-      load_row<T, UNITS, INTERLEAVED>(x, at, live ? D : 0, xa, xb);
-      float2 turn[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) turn[j] = at.turned[j] && live ? cs[n * a.half + 4 * slot + j] : make_float2(1.f, 0.f);
+      const T *x = static_cast<const T *>(s.x) + spot.b * s.batch + spot.r * s.row + head * s.head;
+      T *out = static_cast<T *>(s.out) + ((first + n) * (key ? a.Hk : a.Hq) + head) * D;
+      float v[8], g[8];
+      load_row<T, PAIRS>(x, place, live ? D : 0, v);
+      if constexpr (BACK) load_row<T, PAIRS>(static_cast<const T *>(s.dy) + spot.b * s.dy_batch + spot.r * s.dy_row + head * s.dy_head, place, live ? D : 0, g);
       float rstd = 1.f;
       if (a.norm) {
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], sum));
-        rstd = 1.f / sqrtf(fmaf(lanes_sum<LANES>(sum), inv, a.eps));
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+        rstd = __builtin_amdgcn_rsqf(fmaf(lanes_sum<LANES>(sum), inv, a.eps));
       }
-      float ya[4], yb[4];
       if constexpr (!BACK) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float u = xa[j] * rstd * (key ? wk[0][j] : wq[0][j]), v = xb[j] * rstd * (key ? wk[1][j] : wq[1][j]);
-          ya[j] = u * turn[j].x - v * turn[j].y;
-          yb[j] = u * turn[j].y + v * turn[j].x;
-        }
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * (key ? wk[j] : wq[j]);
+        turn<PAIRS, LANES>(v, cs + n * (a.half + 1), a.half, slot, 1.f, exchange, partners);
       } else {
-        const T *dy = static_cast<const T *>(s.dy) + b * s.dy_batch + r * s.dy_row + head * s.dy_head;
-        float ga[4], gb[4];
-        load_row<T, UNITS, INTERLEAVED>(dy, at, live ? D : 0, ga, gb);
+        turn<PAIRS, LANES>(g, cs + n * (a.half + 1), a.half, slot, -1.f, exchange, partners);
         float dot = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float u = ga[j] * turn[j].x + gb[j] * turn[j].y, v = gb[j] * turn[j].x - ga[j] * turn[j].y;
-          xa[j] *= rstd, xb[j] *= rstd;
-          sq[0][j] += key ? 0.f : u * xa[j], sq[1][j] += key ? 0.f : v * xb[j];
-          sk[0][j] += key ? u * xa[j] : 0.f, sk[1][j] += key ? v * xb[j] : 0.f;
-          ga[j] = u * (key ? wk[0][j] : wq[0][j]), gb[j] = v * (key ? wk[1][j] : wq[1][j]);
-          dot = fmaf(ga[j], xa[j], fmaf(gb[j], xb[j], dot));
+        for (int j = 0; j < 8; ++j) {
+          v[j] *= rstd;
+          sq[j] += key ? 0.f : g[j] * v[j], sk[j] += key ? g[j] * v[j] : 0.f;
+          g[j] *= key ? wk[j] : wq[j];
+          dot = fmaf(g[j], v[j], dot);
         }
         const float mean = a.norm ? lanes_sum<LANES>(dot) * inv : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ya[j] = rstd * (ga[j] - xa[j] * mean), yb[j] = rstd * (gb[j] - xb[j] * mean);
+        for (int j = 0; j < 8; ++j) v[j] = rstd * (g[j] - v[j] * mean);
       }
-      if (s.out) store_row<T, UNITS, INTERLEAVED>(out, at, live ? D : 0, ya, yb);
+      if (s.out) store_row<T, PAIRS>(out, place, live ? D : 0, v);
     }
   }
   if constexpr (BACK) {
@@ -254,32 +317,27 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
     for (int side = 0; side < 2; ++side) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        share[threadIdx.x * 8 + j] = side ? sk[0][j] : sq[0][j];
-        share[threadIdx.x * 8 + 4 + j] = side ? sk[1][j] : sq[1][j];
-      }
+      for (int j = 0; j < 8; ++j) share[threadIdx.x * 8 + j] = side ? sk[j] : sq[j];
       __syncthreads();
       if ((int)threadIdx.x < LANES * 8) {
         float sum = 0.f;
-        for (int g = 0; g < GROUPS; ++g) sum += share[g * LANES * 8 + threadIdx.x];
-        const Place mine = place_of<INTERLEAVED>(a, threadIdx.x / 8, UNITS);
-        int channel = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if ((threadIdx.x & 7) == j) channel = mine.a[j];
-          if ((threadIdx.x & 7) == 4 + j) channel = mine.b[j];
-        }
-        if (channel < D) a.partials[((int64_t)blockIdx.x * 2 + side) * D + channel] = sum;
+        for (int k = 0; k < GROUPS; ++k) sum += share[k * LANES * 8 + threadIdx.x];
+        const Place mine = place_of<PAIRS>(a.half, threadIdx.x / 8);
+        const int j = threadIdx.x & 7, c = j < 4 ? mine.at0 + j : mine.at1 + j - 4;
+        if (c < D) a.partials[((int64_t)blockIdx.x * 2 + side) * D + c] = sum;
       }
     }
   }
 }
 
-template <class T, bool UNITS, bool INTERLEAVED, bool BACK>
-int launch_lanes(const Args &a, int64_t blocks, size_t lds, hipStream_t st) {
+template <class T, Pairs PAIRS, bool BACK>
+int launch_lanes(const Args &a, int64_t blocks, hipStream_t st) {
   const int slots = (a.D + 7) / 8;
   auto go = [&](auto lanes) {
-    rows_kernel<T, UNITS, INTERLEAVED, decltype(lanes)::value, BACK><<<(unsigned)blocks, 256, lds, st>>>(a);
+    constexpr int LANES = decltype(lanes)::value;
+    const size_t turns = (size_t)a.per_block * (a.half + 1) * sizeof(float2) + (PAIRS == kApart ? 256 / LANES * (9 * LANES + 1) * sizeof(float) : 0);
+    const size_t shares = BACK ? 256 * 8 * sizeof(float) : 0;
+    rows_kernel<T, PAIRS, LANES, BACK><<<(unsigned)blocks, 256, turns > shares ? turns : shares, st>>>(a);
     return launch_status();
   };
   if (slots <= 1) return go(std::integral_constant<int, 1>{});
@@ -289,28 +347,29 @@ int launch_lanes(const Args &a, int64_t blocks, size_t lds, hipStream_t st) {
   return go(std::integral_constant<int, 16>{});
 }
 template <class T, bool BACK>
-int launch_type(const Args &a, bool units, int64_t blocks, size_t lds, hipStream_t st) {
-  if (units) return a.interleaved ? launch_lanes<T, true, true, BACK>(a, blocks, lds, st) : launch_lanes<T, true, false, BACK>(a, blocks, lds, st);
-  return a.interleaved ? launch_lanes<T, false, true, BACK>(a, blocks, lds, st) : launch_lanes<T, false, false, BACK>(a, blocks, lds, st);
+int launch_type(const Args &a, int64_t blocks, hipStream_t st) {
+  if (a.interleaved || a.half == 0) return launch_lanes<T, kNeighbours, BACK>(a, blocks, st);
+  if (a.half % 4 == 0 && a.D % 8 == 0) return launch_lanes<T, kQuarters, BACK>(a, blocks, st);
+  return launch_lanes<T, kApart, BACK>(a, blocks, st);
 }
 
-// totals of the workgroups' sums: 16 columns a workgroup, their rows in 16 parts that are added up in order
+// totals of the workgroups' sums: 4 columns a workgroup, their rows in 64 parts that are joined in order
 __global__ __launch_bounds__(256) void weight_sums_kernel(const float *partials, int64_t rows, int D, float *d_q, float *d_k) {
-  __shared__ float part[16][17];
-  const int col = threadIdx.x & 15, p = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
+  __shared__ float part[64][4];
+  const int col = threadIdx.x & 3, p = threadIdx.x >> 2, c = blockIdx.x * 4 + col;
   float sum = 0.f;
-  if (c < 2 * D)
-    for (int64_t r = p; r < rows; r += 16) sum += partials[r * 2 * D + c];
+  if (c < 2 * D) {
+#pragma unroll 4
+    for (int64_t r = p; r < rows; r += 64) sum += partials[r * 2 * D + c];
+  }
   part[p][col] = sum;
-  __syncthreads();
+  for (int n = 32; n > 0; n >>= 1) {
+    __syncthreads();
+    if (p < n) part[p][col] += part[p + n][col];
+  }
   if (p != 0 || c >= 2 * D) return;
-  for (int k = 1; k < 16; ++k) sum += part[k][col];
   float *out = c < D ? d_q : d_k;
-  if (out) out[c < D ? c : c - D] = sum;
-}
-
-static bool on_fours(const pa_heads &h, size_t elem) {
-  return reinterpret_cast<uintptr_t>(h.data) % (4 * elem) == 0 && h.batch % 4 == 0 && h.row % 4 == 0 && h.head % 4 == 0;
+  if (out) out[c < D ? c : c - D] = part[0][col];
 }
 
 struct Plan {
@@ -325,11 +384,6 @@ static Plan plan_of(int64_t points, int num_cu) {
   const int64_t wanted = (points + per - 1) / per, most = (int64_t)num_cu * 8;
   return {per, wanted < most ? wanted : most};
 }
-static size_t lds_of(const Plan &plan, int half, bool back) {
-  const size_t turns = (size_t)plan.per_block * half * sizeof(float2), shares = back ? 256 * 8 * sizeof(float) : 0;
-  return turns > shares ? turns : shares;
-}
-
 static Args args_of(const pa_rotate_params &p, const pa_heads &q, const pa_heads &k) {
   Args a = {};
   a.q.x = q.data, a.q.batch = q.batch, a.q.row = q.row, a.q.head = q.head, a.q.weight = p.q_weight;
@@ -337,23 +391,17 @@ static Args args_of(const pa_rotate_params &p, const pa_heads &q, const pa_heads
   a.positions = p.positions, a.frequencies = p.frequencies;
   a.points = p.B * p.N, a.N = p.N, a.position_batch = p.position_batch;
   a.Hq = (int)p.Hq, a.Hk = (int)p.Hk, a.D = (int)p.D, a.half = (int)(p.rotated / 2), a.axes = (int)p.axes;
+  a.by_heads = (uint32_t)(((1ull << 32) + a.Hq + a.Hk - 1) / (a.Hq + a.Hk));
+  a.by_half = a.half ? (uint32_t)(((1ull << 32) + a.half - 1) / a.half) : 0;
   a.position_type = p.position_type, a.interleaved = p.interleaved, a.norm = p.norm, a.eps = (float)p.eps;
   return a;
 }
-static bool units_of(const Args &a, size_t elem) {
-  return a.D % 8 == 0 && (a.interleaved || a.half % 4 == 0) && reinterpret_cast<uintptr_t>(a.q.out) % (4 * elem) == 0 &&
-         reinterpret_cast<uintptr_t>(a.k.out) % (4 * elem) == 0;
-}
-
 int forward(int dtype, const pa_rotate_params &p, const pa_heads &q, const pa_heads &k, void *q_out, void *k_out, int num_cu, hipStream_t st) {
-  const size_t elem = dtype == PA_F32 ? 4 : 2;
   Args a = args_of(p, q, k);
   a.q.out = q_out, a.k.out = k_out;
   const Plan plan = plan_of(a.points, num_cu);
   a.per_block = plan.per_block;
-  const bool units = units_of(a, elem) && on_fours(q, elem) && on_fours(k, elem);
-  const size_t lds = lds_of(plan, a.half, false);
-  return dtype == PA_F32 ? launch_type<float, false>(a, units, plan.blocks, lds, st) : launch_type<bf16, false>(a, units, plan.blocks, lds, st);
+  return dtype == PA_F32 ? launch_type<float, false>(a, plan.blocks, st) : launch_type<bf16, false>(a, plan.blocks, st);
 }
 
 int64_t backward_workspace_bytes(const pa_rotate_params &p, int num_cu) {
@@ -361,7 +409,6 @@ int64_t backward_workspace_bytes(const pa_rotate_params &p, int num_cu) {
 }
 int backward(int dtype, const pa_rotate_params &p, const pa_heads &q, const pa_heads &k, const pa_heads &d_q, const pa_heads &d_k, void *dq,
              void *dk, float *d_q_weight, float *d_k_weight, float *workspace, int num_cu, hipStream_t st) {
-  const size_t elem = dtype == PA_F32 ? 4 : 2;
   Args a = args_of(p, q, k);
   a.q.out = dq, a.k.out = dk;
   a.q.dy = d_q.data, a.q.dy_batch = d_q.batch, a.q.dy_row = d_q.row, a.q.dy_head = d_q.head;
@@ -369,11 +416,9 @@ int backward(int dtype, const pa_rotate_params &p, const pa_heads &q, const pa_h
   const Plan plan = plan_of(a.points, num_cu);
   a.per_block = plan.per_block;
   a.partials = d_q_weight || d_k_weight ? workspace : nullptr;
-  const bool units = units_of(a, elem) && on_fours(q, elem) && on_fours(k, elem) && on_fours(d_q, elem) && on_fours(d_k, elem);
-  const size_t lds = lds_of(plan, a.half, true);
-  int rc = dtype == PA_F32 ? launch_type<float, true>(a, units, plan.blocks, lds, st) : launch_type<bf16, true>(a, units, plan.blocks, lds, st);
+  const int rc = dtype == PA_F32 ? launch_type<float, true>(a, plan.blocks, st) : launch_type<bf16, true>(a, plan.blocks, st);
   if (rc || !a.partials) return rc;
-  weight_sums_kernel<<<(unsigned)((2 * p.D + 15) / 16), 256, 0, st>>>(workspace, plan.blocks, (int)p.D, d_q_weight, d_k_weight);
+  weight_sums_kernel<<<(unsigned)((2 * p.D + 3) / 4), 256, 0, st>>>(workspace, plan.blocks, (int)p.D, d_q_weight, d_k_weight);
   return launch_status();
 }
 
