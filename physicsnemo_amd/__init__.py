@@ -13,5 +13,6 @@ from .gale import GALE, GALEBlock, GALEStructuredMesh2D, GALEStructuredMesh3D  #
 from .geotransolver import GeoTransolver, GlobalContextBuilder  # noqa: F401
 from .graphs import GraphedForward  # noqa: F401
 from .transolver import Mlp, Transolver, TransolverBlock  # noqa: F401
+from .window_attention import WindowAttention, WindowCache  # noqa: F401
 
 __version__ = "0.1.0"

@@ -26,6 +26,7 @@ from . import versions
 from .feedforward import GATED_ACTS, CounterDropout, GatedMlp, Int8Mlp, counter_dropout, plain_act
 from .physics_attention import (PhysicsAttentionBase, PhysicsAttentionIrregularMesh, PhysicsAttentionStructuredMesh2D,
                                 PhysicsAttentionStructuredMesh3D)
+from .window_attention import WindowAttention
 
 __all__ = ["Mlp", "TransolverBlock", "Transolver"]
 
@@ -130,13 +131,16 @@ class TransolverBlock(nn.Module):
 
     def __init__(self, num_heads: int, hidden_dim: int, dropout: float, act: str = "gelu", mlp_ratio: int = 4,
                  last_layer: bool = False, out_dim: int = 1, slice_num: int = 32,
-                 spatial_shape: tuple[int, ...] | None = None, use_te: bool = True, plus: bool = False):
+                 spatial_shape: tuple[int, ...] | None = None, use_te: bool = True, plus: bool = False, window: dict | None = None):
+        """`window`: options of a `WindowAttention` over the points in their order (a grid's row by row) in place of the slice attention."""
         super().__init__()
         self.last_layer = last_layer
         self.ln_1 = nn.LayerNorm(hidden_dim)
         common = dict(heads=num_heads, dim_head=hidden_dim // num_heads, dropout=dropout, slice_num=slice_num,
                       use_te=use_te, plus=plus)
-        if spatial_shape is None:
+        if window is not None:
+            self.Attn = WindowAttention(hidden_dim, heads=num_heads, dim_head=hidden_dim // num_heads, dropout=dropout, **window)
+        elif spatial_shape is None:
             self.Attn = PhysicsAttentionIrregularMesh(hidden_dim, **common)
         elif len(spatial_shape) == 2:
             self.Attn = PhysicsAttentionStructuredMesh2D(hidden_dim, spatial_shape=spatial_shape, **common)
@@ -400,13 +404,15 @@ class TransolverBlock(nn.Module):
 
 class Transolver(nn.Module):
     """Transolver model (reference :447-736) built on the HIP PhysicsAttention layer.  Beside the reference's activations
-    `act` takes "swiglu", "geglu", "reglu" and "glu": blocks with a `GatedMlp`, the preprocess Mlp with the gate's activation."""
+    `act` takes "swiglu", "geglu", "reglu" and "glu": blocks with a `GatedMlp`, the preprocess Mlp with the gate's activation; and the
+    blocks whose numbers are in `window_blocks` attend over a window of neighbours in the order of the points instead of through slices
+    (`WindowAttention` with `window_options`)."""
 
     def __init__(self, functional_dim: int, out_dim: int, embedding_dim: int | None = None, n_layers: int = 4,
                  n_hidden: int = 256, dropout: float = 0.0, n_head: int = 8, act: str = "gelu", mlp_ratio: int = 4,
                  slice_num: int = 32, unified_pos: bool = False, ref: int = 8,
                  structured_shape: None | tuple[int, ...] = None, use_te: bool = True, time_input: bool = False,
-                 plus: bool = False) -> None:
+                 plus: bool = False, window_blocks: tuple[int, ...] = (), window_options: dict | None = None) -> None:
         super().__init__()
         # constructor arguments as the reference records them for its checkpoints (core/module.py:196-223)
         self._args = dict(functional_dim=functional_dim, out_dim=out_dim, embedding_dim=embedding_dim, n_layers=n_layers,
@@ -414,6 +420,13 @@ class Transolver(nn.Module):
                           slice_num=slice_num, unified_pos=unified_pos, ref=ref,
                           structured_shape=list(structured_shape) if structured_shape is not None else None,
                           use_te=use_te, time_input=time_input, plus=plus)
+        window_blocks = tuple(int(k) for k in window_blocks)
+        if any(not 0 <= k < n_layers for k in window_blocks):
+            raise ValueError(f"window_blocks has to name blocks 0 to {n_layers - 1}, got {window_blocks}")
+        if window_blocks:  # not among the reference's arguments: in a checkpoint only where used
+            self._args.update(window_blocks=list(window_blocks), window_options=window_options)
+        elif window_options is not None:
+            raise ValueError("window_options are for the blocks in window_blocks, which names none")
         self.use_te = use_te
         if not n_hidden % n_head == 0:
             raise ValueError(
@@ -445,7 +458,8 @@ class Transolver(nn.Module):
         self.blocks = nn.ModuleList([
             TransolverBlock(num_heads=n_head, hidden_dim=n_hidden, dropout=dropout, act=act, mlp_ratio=mlp_ratio,
                             out_dim=out_dim, slice_num=slice_num, spatial_shape=structured_shape,
-                            last_layer=(i == n_layers - 1), use_te=use_te, plus=plus)
+                            last_layer=(i == n_layers - 1), use_te=use_te, plus=plus,
+                            **({"window": window_options or {}} if i in window_blocks else {}))
             for i in range(n_layers)
         ])
         self.initialize_weights()
@@ -524,6 +538,8 @@ class Transolver(nn.Module):
     def use_fp8_weights(self, enabled: bool = True):
         """Every block's large weights as fp8-e4m3 with per-output-channel scales (`TransolverBlock.use_fp8_weights`);
         the preprocess Mlp, the LayerNorms, the slice / qkv projections and the output head stay in higher precision."""
+        if enabled and any(type(block.Attn) is WindowAttention for block in self.blocks):
+            raise ValueError("fp8 weights are for models without window attention blocks")
         for block in self.blocks:
             block.use_fp8_weights(enabled)
         return self
