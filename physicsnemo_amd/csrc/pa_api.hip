@@ -2049,7 +2049,7 @@ static int check_window(int dtype, const pa_window_params *p) {
   if (!(p->scale > 1e-30 && p->scale < 1e30)) return PA_ERR_DIMS;
   if (p->D > PA_MAX_D || p->Hq > 4096 || p->N > PA_MAX_WINDOW_N || p->B > (1 << 24) || p->sinks > PA_MAX_SINKS) return PA_ERR_UNSUPPORTED;
   // one workgroup per 128 rows of a head, and as many again for the first rows of each
-  if (((p->N + 127) / 128 + (p->N + 1023) / 1024) > ((1ll << 31) - 1) / (p->Hq * p->B)) return PA_ERR_UNSUPPORTED;
+  if (((p->N + 127) / 128 + (p->N + 511) / 512) > ((1ll << 31) - 1) / (p->Hq * p->B)) return PA_ERR_UNSUPPORTED;
   if (p->buckets > 0) {
     const int64_t side = p->right != 0 ? p->buckets / 2 : p->buckets;
     if (side < 2 || (p->right != 0 && p->buckets % 2 != 0) || p->distance <= side / 2) return PA_ERR_DIMS;

@@ -56,7 +56,8 @@ struct Args {
   void *dq, *dk, *dv;
   float *delta, *bias_parts, *sink_parts;
   int blocks;       // query (key) blocks of a sequence
-  int sink_chunks;  // parts of the queries of a key block with sinks
+  int sink_chunks;  // parts of the queries of the key tiles with sinks
+  int sink_rows;    // rows of those tiles
 };
 
 __device__ __forceinline__ int length_of(const Args &a, int b) {

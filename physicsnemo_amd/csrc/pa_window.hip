@@ -419,6 +419,7 @@ Args make_args(const pa_window_params &p) {
   a.left = p.left < 0 || p.left >= p.N ? kNoBound : (int)p.left;
   a.right = p.right < 0 || p.right >= p.N ? kNoBound : (int)p.right;
   a.sinks = a.left == kNoBound ? 0 : (int)p.sinks;  // all that lies behind is seen without them
+  a.sink_rows = (a.sinks + 31) / 32 * 32;
   a.scale = (float)p.scale, a.c = (float)(p.scale * 1.4426950408889634);
   a.lengths = p.lengths;
   a.bias = make_bias(p);

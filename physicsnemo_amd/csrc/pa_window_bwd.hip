@@ -12,6 +12,29 @@
 namespace pa {
 namespace window {
 
+// Sums of a tile's score gradients by offset key - query, added to a wave's table of them (t: the offset of the tile's first key from the
+// wave's first query).  Eight keys at a time go to LDS as [diagonal][key], where 39 lanes add up a diagonal each: what a diagonal lacks at its ends is
+// never written and stays zero.  (LDS atomics, one a score, took 96 cycles an instruction: 3 000 a tile, and 150 us of the whole at 11 253 x 8 x 64.)
+constexpr int kDiagonals = 39, kDiagonal = 12;
+__device__ __forceinline__ void add_diagonals(const f32x16 &ds, float *buffer, float *t, int lane) {
+  const int i = lane & 31, g = lane >> 5;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float *const put = buffer + (4 * g - i + 31) * kDiagonal + 4 * g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put[j * kDiagonal + j] = ds[4 * q + j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // LDS accesses of a wave happen in order; this keeps the compiler from exchanging them
+    __builtin_amdgcn_wave_barrier();
+    if (lane < kDiagonals) {
+      const f32x4 *const d = reinterpret_cast<const f32x4 *>(buffer + lane * kDiagonal);
+      const f32x4 a = d[0], b = d[1];
+      t[8 * q + lane - 31] += ((a[0] + a[1]) + (a[2] + a[3])) + ((b[0] + b[1]) + (b[2] + b[3]));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
@@ -29,8 +52,12 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   zero(dq);
   if constexpr (BIAS) fill_bias_table(a, h, table);
   float *const mine = sums + wave * entries;
-  if constexpr (DBIAS)
+  // 16-byte boundaries: the tables' sizes are no multiples of four
+  float *const buffer = reinterpret_cast<float *>((reinterpret_cast<uintptr_t>(sums + 4 * entries) + 15) / 16 * 16) + wave * kDiagonals * kDiagonal;
+  if constexpr (DBIAS) {
     for (int u = lane; u < entries; u += 64) mine[u] = 0.f;
+    for (int u = lane; u < kDiagonals * kDiagonal; u += 64) buffer[u] = 0.f;
+  }
   float behind = 0.f, ahead = 0.f;
   if (q0 < len) {
     typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
@@ -50,10 +77,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
     Stage<T, DP, PLAIN, KT, 256> ks, vs;
     // one pass over the keys: f(sub-tile's keys, values, p, dp, first key)
-    f32x16 start;  // of dp: in the last pass less delta already
-    auto pass = [&](float from, auto &&f) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) start[r] = from;
+    auto pass = [&](float from, auto &&f) {  // from: what dp starts from, in the last pass less delta
       __syncthreads();
       if (list.count > 0) {
         ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
@@ -74,7 +98,9 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
           const int k0 = list[n] * KT + 32 * s;
           if (sights.none(k0)) continue;
           const T *const krows = kt + 32 * s * O::kStride;
-          f32x16 z, dp = start;
+          f32x16 z, dp;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dp[r] = from;
           Reach reach = kNear;
           if constexpr (BIAS) {
             reach = reach_of(a.bias, k0 - qw - 31, k0 + 31 - qw);
@@ -130,16 +156,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
       for (int r = 0; r < 16; ++r) p[r] *= dp[r];
       if constexpr (DBIAS) {
         if (reach == kNear) {
-          // the half-waves one after the other: within one, every lane has an offset of its own
-          float *t = mine + (k0 + 4 * g - me + table_low(a.bias));
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (g == half) {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) unsafeAtomicAdd(t + 8 * (r >> 2) + (r & 3), p[r]);
-            }
-            __builtin_amdgcn_wave_barrier();
-          }
+          add_diagonals(p, buffer, mine + (k0 - qw + table_low(a.bias)), lane);
         } else {
           float sum = 0.f;
 #pragma unroll
@@ -212,8 +229,8 @@ __global__ __launch_bounds__(256) void bias_sums_kernel(const float *parts, int6
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// keys_kernel: block 0 of the keys, where it holds sinks, is seen by all queries behind them: its queries are cut into sink_chunks parts, each a
-// workgroup of its own whose sums are joined by sink_sums_kernel.
+// keys_kernel: tiles of keys with sinks are seen by all queries behind them, which are cut into sink_chunks parts, each a workgroup of its own
+// for those tiles alone, whose sums are joined by sink_sums_kernel.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, bool PLAIN, bool BIAS>
 __global__ __launch_bounds__(256) void keys_kernel(Args a) {
@@ -223,13 +240,13 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
   float *const stats = reinterpret_cast<float *>(tiles + 4 * TILE);  // [buffer][log2 denominators, deltas][QT]
   float *const table = stats + 4 * QT;
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int G = a.Hq / a.Hk, chunks = a.sink_chunks, per_head = a.blocks - (chunks > 0) + chunks;
+  const int G = a.Hq / a.Hk, chunks = a.sink_chunks, per_head = a.blocks + chunks;
   const uint32_t work = own_work(), at_head = work / (uint32_t)per_head;
   int block = (int)(work - at_head * (uint32_t)per_head), chunk = -1;
   const int b = (int)(at_head / (uint32_t)a.Hk), hk = (int)(at_head - (uint32_t)b * (uint32_t)a.Hk);
   if (chunks > 0) {
     if (block < chunks) chunk = block, block = 0;
-    else block -= chunks - 1;
+    else block -= chunks;
   }
   const int len = length_of(a, b), k0 = block * 128, kw = k0 + 32 * wave, me = kw + i;
   using O = Ops<T, DP>;
@@ -240,7 +257,8 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
     typename O::Rows key = O::template rows<PLAIN>(head_of<T>(a.k, b, hk), a.k.row, me, len, me < len, a.D, g);
     typename O::Rows value = O::template rows<PLAIN>(head_of<T>(a.v, b, hk), a.v.row, me, len, me < len, a.D, g);
     O::settle(key), O::settle(value);
-    const Sights sights = sights_of_keys(a, len, kw);
+    Sights sights = sights_of_keys(a, len, kw);
+    if (chunks > 0 && (kw < a.sink_rows) != (chunk >= 0)) sights.high = -1;  // the other workgroups' rows
     // queries that see a key of the block: i >= j - right, and i <= j + left or j a sink
     int first = k0 - a.right > 0 ? k0 - a.right : 0, last = k0 + 127 + a.left;
     if (chunk >= 0 || last > len - 1) last = len - 1;
@@ -253,28 +271,36 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
     const int tiles_of_head = t1 - t0 + 1, count = tiles_of_head > 0 ? tiles_of_head * G : 0;
     Stage<T, DP, PLAIN, QT, 256> qs, gs;
     float stat = 0.f;
-    auto fetch = [&](int n) {
-      const int h = hk * G + n / tiles_of_head, from = (t0 + n % tiles_of_head) * QT;
+    // the tile in work and the one to fetch, counted on: a division an iteration by each of two was half of all scalar work
+    int h = hk * G, tile = t0, next_h = hk * G, next_tile = t0;
+    auto on = [&](int &head, int &at) {
+      if (++at > t1) at = t0, ++head;
+    };
+    int from = 0;
+    auto fetch = [&]() {
+      const int h = next_h;
+      from = next_tile * QT;
+      on(next_h, next_tile);
       qs.load(a.q, head_of<T>(a.q, b, h), from, len, a.D, threadIdx.x);
       gs.load(a.dy, head_of<T>(a.dy, b, h), from, len, a.D, threadIdx.x);
       if (threadIdx.x < 2 * QT) {
         const int row = from + threadIdx.x % QT;
-        // as the products start from them: less the denominator in units of z, less delta; rows that are not there weigh nothing
         const float *src = (int)threadIdx.x < QT ? a.saved_stats : a.delta;
-        const float v = src[((int64_t)b * a.Hq + h) * a.N + (row < len ? row : len - 1)];
-        stat = (int)threadIdx.x >= QT ? -v : row < len ? -v / a.c : -INFINITY;
+        stat = src[((int64_t)b * a.Hq + h) * a.N + (row < len ? row : len - 1)];
       }
     };
     auto put = [&](int n) {
       T *const to = tiles + (n & 1) * 2 * TILE;
       qs.store(to, threadIdx.x);
       gs.store(to + TILE, threadIdx.x);
-      if (threadIdx.x < 2 * QT) stats[(n & 1) * 2 * QT + threadIdx.x] = stat;
+      // as the products start from them: less the denominator in units of z, less delta; rows that are not there weigh nothing.  Here and not in
+      // fetch, where it would wait for the loads: 110 -> 99 us at 65 536 x 8 x 32, 257 keys a query.
+      if (threadIdx.x < 2 * QT)
+        stats[(n & 1) * 2 * QT + threadIdx.x] = (int)threadIdx.x >= QT ? -stat : from + (int)threadIdx.x < len ? -stat / a.c : -INFINITY;
     };
-    if (count > 0) fetch(0), put(0);
+    if (count > 0) fetch(), put(0);
     int filled = -1;
-    for (int n = 0; n < count; ++n) {
-      const int h = hk * G + n / tiles_of_head;
+    for (int n = 0; n < count; ++n, on(h, tile)) {
       if (BIAS && h != filled) {
         __syncthreads();  // the head before is done with
         fill_bias_table(a, h, table);
@@ -283,10 +309,10 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       __syncthreads();
       const T *const qt = tiles + (n & 1) * 2 * TILE, *const gt = qt + TILE;
       const float *const lse = stats + (n & 1) * 2 * QT, *const delta = lse + QT;
-      if (n + 1 < count) fetch(n + 1);
+      if (n + 1 < count) fetch();
 #pragma unroll 1
       for (int s = 0; s < SUB; ++s) {
-        const int q0 = (t0 + n % tiles_of_head) * QT + 32 * s;
+        const int q0 = tile * QT + 32 * s;
         if (sights.none(q0)) continue;
         const T *const qrows = qt + 32 * s * O::kStride, *const grows = gt + 32 * s * O::kStride;
         f32x16 z, dp;
@@ -329,7 +355,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       const int q_low = t0 * QT > kw - a.right ? t0 * QT : kw - a.right;
       int q_high = t1 * QT + QT - 1 < len - 1 ? t1 * QT + QT - 1 : len - 1;
       if (kw >= a.sinks && kw + 31 + a.left < q_high) q_high = kw + 31 + a.left;
-      for (int h = hk * G; h < hk * G + G; ++h) {
+      for (h = hk * G; h < hk * G + G; ++h) {
         const T *const queries = head_of<T>(a.q, b, h), *const grads = head_of<T>(a.dy, b, h);
         const int64_t first_stat = ((int64_t)b * a.Hq + h) * a.N;
         auto p_of = [&](int n, bool &seen) {
@@ -347,27 +373,38 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
     }
   }
   if (chunk < 0) {
+    if (kw < a.sink_rows) return;
     const int64_t at = (((int64_t)b * a.N + me) * a.Hk + hk) * a.D;
     store_rows<T, DP>(dk, a.scale, me < len, static_cast<T *>(a.dk) + at, me < a.N, a.D, g);
     store_rows<T, DP>(dv, 1.f, me < len, static_cast<T *>(a.dv) + at, me < a.N, a.D, g);
     return;
   }
-  // [b][hk][chunk][dk, dv][128][D]
-  float *const part = a.sink_parts + (((int64_t)b * a.Hk + hk) * chunks + chunk) * 2 * 128 * a.D + (32 * wave + i) * a.D;
+  // [b][hk][chunk][dk, dv][sink_rows][D]
+  if (kw >= a.sink_rows) return;
+  float *const part = a.sink_parts + (((int64_t)b * a.Hk + hk) * chunks + chunk) * 2 * a.sink_rows * a.D + (32 * wave + i) * a.D;
   store_rows<float, DP>(dk, a.scale, me < len, part, true, a.D, g);
-  store_rows<float, DP>(dv, 1.f, me < len, part + 128 * a.D, true, a.D, g);
+  store_rows<float, DP>(dv, 1.f, me < len, part + a.sink_rows * a.D, true, a.D, g);
 }
 
+// 32 neighbouring elements a workgroup, the chunks in 8 parts that are joined in order
 template <class T>
 __global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
-  const int64_t per = 2 * 128 * (int64_t)a.D, e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= (int64_t)a.B * a.Hk * per) return;
-  const int64_t head = e / per, at = e - head * per;
+  __shared__ float parts[8][32];
+  const int64_t per = 2 * a.sink_rows * (int64_t)a.D, e = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+  const bool some = e < (int64_t)a.B * a.Hk * per;
+  const int64_t head = some ? e / per : 0, at = some ? e - head * per : 0;
   const float *p = a.sink_parts + head * a.sink_chunks * per + at;
+  const int part = threadIdx.x >> 5, each = (a.sink_chunks + 7) / 8, last = part * each + each < a.sink_chunks ? part * each + each : a.sink_chunks;
   float sum = 0.f;
-  for (int c = 0; c < a.sink_chunks; ++c) sum += p[c * per];
-  const int b = (int)(head / a.Hk), hk = (int)(head % a.Hk), side = (int)(at / (128 * a.D));
-  const int row = (int)(at / a.D % 128), d = (int)(at % a.D);
+#pragma unroll 4
+  for (int c = part * each; c < last; ++c) sum += p[c * per];
+  parts[part][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (part != 0 || !some) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sum += parts[k][threadIdx.x];
+  const int b = (int)(head / a.Hk), hk = (int)(head % a.Hk), side = (int)(at / (a.sink_rows * a.D));
+  const int row = (int)(at / a.D % a.sink_rows), d = (int)(at % a.D);
   T *const out = static_cast<T *>(side ? a.dv : a.dk);
   if (row < a.N) store_from_f32(out + (((int64_t)b * a.N + row) * a.Hk + hk) * a.D + d, sum);
 }
@@ -378,7 +415,7 @@ __global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 static int launch_queries(const Args &a, hipStream_t st) {
   const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) +
-                     (BIAS ? (DBIAS ? 5 : 1) * table_size(a.bias) * sizeof(float) : 0);
+                     (BIAS ? (DBIAS ? 5 : 1) * table_size(a.bias) * sizeof(float) : 0) + (DBIAS ? 16 + 4 * kDiagonals * kDiagonal * sizeof(float) : 0);
   auto kernel = queries_kernel<T, DP, PLAIN, BIAS, DBIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);
@@ -390,12 +427,12 @@ static int launch_keys(const Args &a, hipStream_t st) {
   const size_t lds = 4 * (size_t)QT * Ops<T, DP>::kStride * sizeof(T) + 4 * QT * sizeof(float) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
   auto kernel = keys_kernel<T, DP, PLAIN, BIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
-  const int64_t per_head = a.blocks - (a.sink_chunks > 0) + a.sink_chunks;
+  const int64_t per_head = a.blocks + a.sink_chunks;
   kernel<<<(unsigned)(per_head * a.Hk * a.B), 256, lds, st>>>(a);
   if (int rc = launch_status()) return rc;
   if (a.sink_chunks == 0) return PA_OK;
-  const int64_t n = (int64_t)a.B * a.Hk * 2 * 128 * a.D;
-  sink_sums_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+  const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sink_rows * a.D;
+  sink_sums_kernel<T><<<(unsigned)((n + 31) / 32), 256, 0, st>>>(a);
   return launch_status();
 }
 template <class T>
@@ -424,9 +461,15 @@ static Room room_of(const Args &a, bool want_bias) {
   Room r;
   r.delta = ((int64_t)a.B * a.Hq * a.N + 3) / 4 * 4;
   r.bias_parts = want_bias ? ((int64_t)a.B * a.blocks * a.Hq * a.bias.buckets + 3) / 4 * 4 : 0;
-  // parts of about 1 024 queries, which take about as long as a block of keys without sinks in a usual window
-  r.chunks = a.sinks > 0 ? (a.N + 1023) / 1024 : 0;
-  r.sink_parts = (int64_t)a.B * a.Hk * r.chunks * 2 * 128 * a.D;
+  // Parts of 1 024 queries.  Where the workgroups fill the card few times over, the longest counts: there parts of about as many queries as see
+  // a block of keys without sinks (5 001 x 3 x 4 x 64, 512 keys: 98 us with parts of 640, 119 of 1 024; 65 536 x 8 x 32, 257 keys: 121 of 384, 115 of 1 024).
+  int64_t queries = 1024;
+  if ((int64_t)a.blocks * a.Hk * a.B <= 2048) {
+    queries = 128 + (int64_t)a.left + (a.right == kNoBound ? 0 : a.right);
+    queries = queries < 512 ? 512 : queries > 1024 ? 1024 : (queries + 63) / 64 * 64;
+  }
+  r.chunks = a.sinks > 0 ? (int)((a.N + queries - 1) / queries) : 0;
+  r.sink_parts = (int64_t)a.B * a.Hk * r.chunks * 2 * a.sink_rows * a.D;
   return r;
 }
 int64_t backward_workspace_bytes(int dtype, const pa_window_params &p, bool want_bias) {
