@@ -250,6 +250,13 @@ __device__ __forceinline__ void store_piece(T *row, int col, int D, const u32x4 
   }
 }
 
+__device__ __forceinline__ float sum_of(const f32x16 &v) {
+  float s[2] = {};
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r & 1] += v[r];
+  return s[0] + s[1];
+}
+
 template <class T, int DP>
 struct Ops;
 
@@ -259,6 +266,7 @@ struct Ops<bf16, DP> {
   struct Rows {
     u32x4 v[DP / 16];
   };
+  using Raw = Rows;  // as loaded
   struct Weights {
     u32x4 v[2];
   };
@@ -272,11 +280,12 @@ struct Ops<bf16, DP> {
     return r;
   }
   // Waits for the rows here: left to their first use, inside the loop, the wait would be for the next tile's loads, too
-  static __device__ __forceinline__ void settle(Rows &r) {
+  static __device__ __forceinline__ Rows settle(Raw r) {
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) asm volatile("" : "+v"(r.v[kk]));
+    return r;
   }
-  static __device__ __forceinline__ float dot(const Rows &x, const Rows &y) {  // of this lane's channels
+  static __device__ __forceinline__ float dot(const Rows &x, const Raw &y) {  // of this lane's channels
     float s = 0.f;
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk)
@@ -289,7 +298,7 @@ struct Ops<bf16, DP> {
     return s;
   }
   // acc[row of lds][lane's row] += product over the channels
-  static __device__ __forceinline__ f32x16 scores(const bf16 *lds, const Rows &own, int i, int g, f32x16 acc) {
+  static __device__ __forceinline__ f32x16 scores(const bf16 *lds, const Rows &own, int i, int g, f32x16 acc, int) {
     const u32x4 *p = reinterpret_cast<const u32x4 *>(lds + i * kStride + 8 * g);
 #pragma unroll
     for (int kk = 0; kk < DP / 16; ++kk) acc = mfma::mma(p[2 * kk], own.v[kk], acc);
@@ -302,7 +311,7 @@ struct Ops<bf16, DP> {
   }
   static __device__ __forceinline__ Weights pack(const f32x16 &v) { return {{mfma::pack_half<0>(v), mfma::pack_half<1>(v)}}; }
   // sum of this lane's weights as they are multiplied
-  static __device__ __forceinline__ float sum(const Weights &w) {
+  static __device__ __forceinline__ float sum(const Weights &w, const f32x16 &) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
     float s[2] = {};
@@ -315,6 +324,7 @@ struct Ops<bf16, DP> {
       }
     return s[0] + s[1];
   }
+  static __device__ __forceinline__ void put(bf16 *row, int col, const u32x4 &w) { *reinterpret_cast<u32x4 *>(row + col) = w; }
   // acc[channel][column] += sum over the 32 rows of lds.  The transposing read: in a group of 16 lanes, lane l addresses four
   // channels 4 (l % 4) .. of row l / 4 and receives channel l of the four rows.
   static __device__ __forceinline__ void outcome(const bf16 *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
@@ -342,6 +352,7 @@ struct Ops<float, DP> {
   struct Rows {
     float v[DP / 2];  // channels g DP / 2 ..
   };
+  using Raw = Rows;
   struct Weights {
     f32x16 v;
   };
@@ -360,9 +371,10 @@ struct Ops<float, DP> {
     }
     return r;
   }
-  static __device__ __forceinline__ void settle(Rows &r) {
+  static __device__ __forceinline__ Rows settle(Raw r) {
 #pragma unroll
     for (int k = 0; k < DP / 2; ++k) asm volatile("" : "+v"(r.v[k]));
+    return r;
   }
   static __device__ __forceinline__ float dot(const Rows &x, const Rows &y) {
     float s = 0.f;
@@ -370,7 +382,7 @@ struct Ops<float, DP> {
     for (int k = 0; k < DP / 2; ++k) s = fmaf(x.v[k], y.v[k], s);
     return s;
   }
-  static __device__ __forceinline__ f32x16 scores(const float *lds, const Rows &own, int i, int g, f32x16 acc) {
+  static __device__ __forceinline__ f32x16 scores(const float *lds, const Rows &own, int i, int g, f32x16 acc, int) {
     const f32x4 *p = reinterpret_cast<const f32x4 *>(lds + i * kStride + g * (DP / 2));
 #pragma unroll
     for (int k = 0; k < DP / 8; ++k) {
@@ -386,12 +398,8 @@ struct Ops<float, DP> {
     return acc;
   }
   static __device__ __forceinline__ Weights pack(const f32x16 &v) { return {v}; }
-  static __device__ __forceinline__ float sum(const Weights &w) {
-    float s[2] = {};
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r & 1] += w.v[r];
-    return s[0] + s[1];
-  }
+  static __device__ __forceinline__ float sum(const Weights &, const f32x16 &v) { return sum_of(v); }
+  static __device__ __forceinline__ void put(float *row, int col, const u32x4 &w) { *reinterpret_cast<u32x4 *>(row + col) = w; }
   static __device__ __forceinline__ void outcome(const float *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
     const float *p = lds + 4 * (lane >> 5) * kStride + (lane & 31);
 #pragma unroll
@@ -402,10 +410,151 @@ struct Ops<float, DP> {
   }
 };
 
+// Float32 rows for the bf16 matrix instructions: a value is three bf16 values, each the rounding of what the ones before leave over, which
+// together hold all of its 24 bits; a . b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1, and what is dropped is below 2^-24 |a| |b|.  A
+// product of 32 x 32 over 16 takes 48 passes of the matrix unit against 128 by v_mfma_f32_32x32x2_f32, and a width of 16 one step of 16 (4 x 7 225 x 8 x 16,
+// 171 keys: forward 92 -> 66 us, queries 123 -> 78, keys 156 -> 101; 20 000 x 4 x 64, 401 keys: 140 -> 98, 197 -> 131, 269 -> 175).
+struct Thirds {
+  uint32_t w[3];  // of two neighbouring values
+};
+// INNER: what is known to be finite.  Otherwise an infinity or NaN is in the first alone, so that the others give it back.
+template <bool INNER>
+__device__ __forceinline__ Thirds thirds_of(float x, float y) {
+  Thirds t;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    t.w[k] = mfma::pack2(x, y);
+    if (k == 2) break;
+    x -= __uint_as_float(t.w[k] << 16);
+    y -= __uint_as_float(t.w[k] & 0xffff0000u);
+    if (!INNER) x = x == x ? x : 0.f, y = y == y ? y : 0.f;
+  }
+  return t;
+}
+
+template <int DP>
+struct Split {
+  static constexpr int kPlane = DP + 8, kStride = 3 * kPlane / 2;  // of a row's third in LDS in bf16, of the row in floats
+  using Raw = struct {
+    u32x4 v[DP / 8];  // channels 16 k + 8 g .. + 3 and + 4 .. + 7
+  };
+  struct Rows {
+    u32x4 v[3][DP / 16];
+  };
+  struct Weights {
+    u32x4 v[3][2];
+  };
+  template <bool PLAIN>
+  static __device__ __forceinline__ Raw rows(const float *head, int64_t stride, int n, int limit, bool there, int D, int g) {
+    const float *const row = head + (n < 0 ? 0 : n < limit ? n : limit - 1) * stride;
+    Raw r;
+#pragma unroll
+    for (int k = 0; k < DP / 8; ++k) r.v[k] = load_some<PLAIN>(row, 16 * (k >> 1) + 8 * g + 4 * (k & 1), D, there);
+    return r;
+  }
+  static __device__ __forceinline__ Rows settle(const Raw &r) {
+    Rows s;
+#pragma unroll
+    for (int k = 0; k < DP / 8; ++k)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t x = r.v[k][2 * w], y = r.v[k][2 * w + 1];
+        const Thirds t = thirds_of<false>(__uint_as_float(x), __uint_as_float(y));
+#pragma unroll
+        for (int p = 0; p < 3; ++p) s.v[p][k >> 1][2 * (k & 1) + w] = t.w[p];
+      }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) asm volatile("" : "+v"(s.v[p][kk]));
+    return s;
+  }
+  static __device__ __forceinline__ float dot(const Rows &x, const Raw &y) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 8; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        float v = 0.f;
+#pragma unroll
+        for (int p = 2; p >= 0; --p) {  // exact in this order
+          const uint32_t two = x.v[p][k >> 1][2 * (k & 1) + (w >> 1)];
+          v += __uint_as_float(w & 1 ? two & 0xffff0000u : two << 16);
+        }
+        const uint32_t b = y.v[k][w];
+        s = fmaf(v, __uint_as_float(b), s);
+      }
+    return s;
+  }
+  // the small ones first
+  static __device__ __forceinline__ f32x16 products(const u32x4 (&a)[3], const u32x4 &b0, const u32x4 &b1, const u32x4 &b2, f32x16 acc) {
+    acc = mfma::mma(a[2], b0, acc);
+    acc = mfma::mma(a[0], b2, acc);
+    acc = mfma::mma(a[1], b1, acc);
+    acc = mfma::mma(a[1], b0, acc);
+    acc = mfma::mma(a[0], b1, acc);
+    return mfma::mma(a[0], b0, acc);
+  }
+  static __device__ __forceinline__ f32x16 scores(const float *lds, const Rows &own, int i, int g, f32x16 acc, int D) {
+    const uint16_t *const p = reinterpret_cast<const uint16_t *>(lds + i * kStride) + 8 * g;
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk) {
+      if (kk % 2 == 1 && 16 * kk >= D) break;  // the upper half of 32 channels is empty
+      u32x4 a[3];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) a[q] = *reinterpret_cast<const u32x4 *>(p + q * kPlane + 16 * kk);
+      acc = products(a, own.v[0][kk], own.v[1][kk], own.v[2][kk], acc);
+    }
+    return acc;
+  }
+  static __device__ __forceinline__ Weights pack(const f32x16 &v) {
+    Weights w;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const Thirds t = thirds_of<true>(v[2 * k], v[2 * k + 1]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) w.v[p][k >> 2][k & 3] = t.w[p];
+    }
+    return w;
+  }
+  static __device__ __forceinline__ float sum(const Weights &, const f32x16 &v) { return sum_of(v); }
+  static __device__ __forceinline__ void put(float *row, int col, const u32x4 &w) {
+    const uint32_t x0 = w[0], x1 = w[1], x2 = w[2], x3 = w[3];
+    const Thirds t = thirds_of<false>(__uint_as_float(x0), __uint_as_float(x1)), u = thirds_of<false>(__uint_as_float(x2), __uint_as_float(x3));
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<mfma::u32x2 *>(reinterpret_cast<uint16_t *>(row) + p * kPlane + col) = mfma::u32x2{t.w[p], u.w[p]};
+  }
+  static __device__ __forceinline__ void outcome(const float *lds, const Weights &w, int lane, f32x16 (&acc)[DP / 32]) {
+    const int l = lane & 15, h = (lane >> 4) & 1, g = lane >> 5;
+    const uint16_t *const p = reinterpret_cast<const uint16_t *>(lds + (4 * g + (l >> 2)) * kStride) + 16 * h + 4 * (l & 3);
+    typedef __attribute__((address_space(3))) s16x4 lds_piece;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        u32x4 a[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+          union {
+            s16x4 h[2];
+            u32x4 v;
+          } x;
+          x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_piece *)(p + (16 * q) * 2 * kStride + k * kPlane + 32 * db));
+          x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_piece *)(p + (16 * q + 8) * 2 * kStride + k * kPlane + 32 * db));
+          a[k] = x.v;
+        }
+        acc[db] = products(a, w.v[0][q], w.v[1][q], w.v[2][q], acc[db]);
+      }
+  }
+};
+// what the kernels over windows multiply with: float32 rows of 128 channels leave no room for thirds beside the bias tables
+template <class T, int DP>
+using WindowOps = typename std::conditional<sizeof(T) == 4 && DP <= 64, Split<(DP <= 64 ? DP : 64)>, Ops<T, DP>>::type;
+
 // ROWS rows of DP channels on their way from memory to LDS by THREADS threads: loaded into registers, written later.  PLAIN rows come by
 // buffer loads: a lane's offset in a tile never changes, the tile's place is in scalar registers, and what lies outside reads as zero without a
 // comparison.  Others by element where a piece is not whole.
-template <class T, int DP, bool PLAIN, int ROWS, int THREADS>
+template <class O, class T, int DP, bool PLAIN, int ROWS, int THREADS>
 struct Stage {
   static constexpr int V = 16 / sizeof(T), PER_ROW = DP / V, UNITS = ROWS * PER_ROW / THREADS;
   static_assert(ROWS * PER_ROW % THREADS == 0 && THREADS % PER_ROW == 0, "whole units a thread");
@@ -432,7 +581,7 @@ struct Stage {
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const int at = tid + u * THREADS;
-      *reinterpret_cast<u32x4 *>(lds + at / PER_ROW * Ops<T, DP>::kStride + at % PER_ROW * V) = w[u];
+      O::put(lds + at / PER_ROW * O::kStride, at % PER_ROW * V, w[u]);
     }
   }
 };
@@ -512,7 +661,7 @@ __device__ __forceinline__ void zero(f32x16 (&acc)[N]) {
 // channels: for one)
 template <class T, int DP>
 constexpr int tile_rows() {
-  return sizeof(T) == 4 && DP == 128 ? 32 : 64;
+  return sizeof(T) == 4 ? 32 : 64;
 }
 
 // f(std::integral_constant<int, DP>{}, std::bool_constant<PLAIN>{}) for the padded width of D channels

@@ -23,9 +23,8 @@ __device__ __forceinline__ float most_of(const f32x16 &z) {
 }
 
 // The softmax of a wave's queries so far, and the values' sum under it.  A query's numbers depend on its own scores alone.
-template <class T, int DP>
+template <class O, int DP>
 struct Running {
-  using O = Ops<T, DP>;
   f32x16 o[DP / 32];
   float m, l, off;  // reference in units of z, this lane's share of the sum, -m c (0 while nothing was seen)
   bool fresh;       // for the whole wave: some query has seen nothing yet
@@ -46,7 +45,7 @@ struct Running {
 #pragma unroll
     for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(fmaf(z[r], c, off));
     const typename O::Weights w = O::pack(z);
-    l += O::sum(w);
+    l += O::sum(w, z);
     return w;
   }
   // a larger reference where this tile's largest score asks for it, and all that is summed so far under it
@@ -89,7 +88,7 @@ __device__ __forceinline__ f32x16 start_of(const Args &a, int q0, int i, int k0,
 
 template <class T, int DP, bool PLAIN, bool BIAS>
 __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forward_kernel(Args a) {
-  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
+  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
   float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
@@ -97,19 +96,20 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
   const int block = (int)(work - at_head * (uint32_t)a.blocks), b = (int)(at_head / (uint32_t)a.Hq), h = (int)(at_head - (uint32_t)b * (uint32_t)a.Hq);
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
-  using O = Ops<T, DP>;
-  Running<T, DP> run;
+  using O = WindowOps<T, DP>;
+  Running<O, DP> run;
   run.start(me < len);
   if (q0 < len) {
-    typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
+    const typename O::Raw raw = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
+    typename O::Rows own;
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
     if constexpr (BIAS) fill_bias_table(a, h, table);
     const Sights sights = sights_of_queries(a, len, qw);
-    Stage<T, DP, PLAIN, KT, 256> ks, vs;
+    Stage<O, T, DP, PLAIN, KT, 256> ks, vs;
     auto scores = [&](const T *rows, int r0) {
-      f32x16 z = O::scores(rows, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table));
+      f32x16 z = O::scores(rows, own, i, g, start_of<BIAS>(a, qw, me, r0, g, table), a.D);
       if (!sights.all(r0)) hide(z, keys_of(a, len, me), r0, g, -INFINITY);
       return z;
     };
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       if (list.count > 0) {
         ks.load(a.k, keys, list[0] * KT, len, a.D, threadIdx.x);
         if (both) vs.load(a.v, values, list[0] * KT, len, a.D, threadIdx.x);
-        O::settle(own);
+        if (both) own = O::settle(raw);
         ks.store(tiles, threadIdx.x);
         if (both) vs.store(tiles + TILE, threadIdx.x);
       }
@@ -161,19 +161,29 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       run.m = high ? most : run.m;
       run.off = run.m == -INFINITY ? 0.f : -run.m * a.c;
     }
-    bool bad = not_finite(run.o);
+    // A score of a visible infinite key is infinite, which thirds do not give: the sum of the weights is formed again, too
+    bool bad = not_finite(run.o) || run.l * 0.f != 0.f;
     if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
       const Span span = keys_of(a, len, me);
       for (int d = 0; d < DP / 32; ++d)
         for (int r = 0; r < 16; ++r) run.o[d][r] = bad ? 0.f : run.o[d][r];
-      auto weight = [&](int j, bool &seen) {
-        seen = span.sees(j);
+      auto score = [&](int j) {
         float z = half_sum(O::dot(own, O::template rows<PLAIN>(keys, a.k.row, j, len, true, a.D, g)));
         if constexpr (BIAS) z += bias_at(a.bias, table, j - me);
-        return __builtin_amdgcn_exp2f(fmaf(z, a.c, run.off));
+        return z;
       };
       const int low = qw - a.left > 0 ? qw - a.left : 0, high = qw + 31 + a.right < len - 1 ? qw + 31 + a.right : len - 1;
+      float most = -INFINITY;
+      for (int j = a.sinks > 0 ? 0 : low; j <= high; j = j + 1 == a.sinks && low > j ? low : j + 1)
+        if (const float z = score(j); span.sees(j)) most = fmaxf(most, z);
+      if (bad) run.l = 0.f, run.m = most, run.off = most == -INFINITY ? 0.f : -most * a.c;
+      auto weight = [&](int j, bool &seen) {
+        seen = span.sees(j);
+        const float w = __builtin_amdgcn_exp2f(fmaf(score(j), a.c, run.off));
+        if (bad && seen && g == 0) run.l += w;
+        return w;
+      };
       add_rows<T, DP>(values, a.v.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, run.o, weight);
       add_rows<T, DP>(values, a.v.row, low, high, a.D, g, bad, run.o, weight);
     }
@@ -225,11 +235,10 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
   const bool mine = col < s.columns && me >= 0;
   const int t0 = ct * 32 / s.G, t1 = (ct * 32 + 31 < s.columns ? ct * 32 + 31 : s.columns - 1) / s.G;
   const int first_q = len - s.T + t0 > 0 ? len - s.T + t0 : 0, last_q = len - s.T + t1;
-  typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, hk * s.G + gq), a.q.row, t, s.T, mine, a.D, g);
-  O::settle(own);
+  const typename O::Rows own = O::settle(O::template rows<PLAIN>(head_of<T>(a.q, b, hk * s.G + gq), a.q.row, t, s.T, mine, a.D, g));
   const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
   const Span span = keys_of(a, mine ? len : 0, me);
-  Running<T, DP> run;
+  Running<O, DP> run;
   run.start(mine);
   if constexpr (BIAS) {
     for (int u = threadIdx.x; u < a.bias.buckets * s.G; u += 256)
@@ -242,7 +251,7 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
     const int by = 4 * s.parts;
     int n = part * 4 + wave;
     typename O::Rows next;
-    Stage<T, DP, PLAIN, 32, 64> vs;
+    Stage<O, T, DP, PLAIN, 32, 64> vs;
     auto fetch = [&](int at) {
       const int k0 = list[at] * 32;
       next = O::template rows<PLAIN>(keys, a.k.row, k0 + i, len, k0 + i < len, a.D, g);
@@ -429,7 +438,7 @@ Args make_args(const pa_window_params &p) {
 
 template <class T, int DP, bool PLAIN, bool BIAS>
 static int launch_forward(const Args &a, hipStream_t st) {
-  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
+  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * WindowOps<T, DP>::kStride * sizeof(T) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
   auto kernel = forward_kernel<T, DP, PLAIN, BIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   kernel<<<(unsigned)((int64_t)a.blocks * a.Hq * a.B), 256, lds, st>>>(a);

@@ -35,9 +35,15 @@ __device__ __forceinline__ void add_diagonals(const f32x16 &ds, float *buffer, f
   }
 }
 
+// Waves a SIMD: the thirds of float32 rows need 184 registers at widths to 32 (one more wave for 20 spilled ones: 4 x 7 225 x 8 x 16, queries 90 -> 78 us,
+// keys 109 -> 101) and 271 at 64 (a second wave: 20 000 x 4 x 64, 401 keys, queries 172 -> 131, keys 200 -> 175).  bf16 rows to 32 run three by
+// themselves; four spill (65 536 x 8 x 32: queries 82 -> 81, keys 99 -> 106).
+template <class T, int DP>
+constexpr int kWaves = sizeof(T) == 2 || DP == 128 ? 1 : DP == 64 ? 2 : 3;
+
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
-__global__ __launch_bounds__(256) void queries_kernel(Args a) {
-  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * Ops<T, DP>::kStride;
+__global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
+  constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
   float *const table = reinterpret_cast<float *>(tiles + 4 * TILE);
@@ -47,7 +53,7 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   const int block = (int)(work - at_head * (uint32_t)a.blocks), b = (int)(at_head / (uint32_t)a.Hq), h = (int)(at_head - (uint32_t)b * (uint32_t)a.Hq);
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
-  using O = Ops<T, DP>;
+  using O = WindowOps<T, DP>;
   f32x16 dq[DP / 32];
   zero(dq);
   if constexpr (BIAS) fill_bias_table(a, h, table);
@@ -60,22 +66,22 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
   }
   float behind = 0.f, ahead = 0.f;
   if (q0 < len) {
-    typename O::Rows own = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
-    typename O::Rows dy = O::template rows<PLAIN>(head_of<T>(a.dy, b, h), a.dy.row, me, len, me < len, a.D, g);
-    O::settle(own), O::settle(dy);
+    const typename O::Raw raw = O::template rows<PLAIN>(head_of<T>(a.q, b, h), a.q.row, me, len, me < len, a.D, g);
+    const typename O::Raw raw_dy = O::template rows<PLAIN>(head_of<T>(a.dy, b, h), a.dy.row, me, len, me < len, a.D, g);
+    const typename O::Rows own = O::settle(raw), dy = O::settle(raw_dy);
     const int64_t at = ((int64_t)b * a.Hq + h) * a.N + me;
     float stat = me < len ? a.saved_stats[at] : INFINITY;
     float delta = 0.f;
     if constexpr (!DBIAS) {
-      const typename O::Rows y =
+      const typename O::Raw y =
           O::template rows<PLAIN>(static_cast<const T *>(a.saved_y) + ((int64_t)b * a.N * a.Hq + h) * a.D, (int64_t)a.Hq * a.D, me, len, me < len, a.D, g);
-      delta = half_sum(O::dot(y, dy));
+      delta = half_sum(O::dot(dy, y));
     }
     const Sights sights = sights_of_queries(a, len, qw);
     const int hk = h / (a.Hq / a.Hk);
     const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
     const Tiles list(a, len, q0, q0 + 127 < len ? q0 + 127 : len - 1, KT);
-    Stage<T, DP, PLAIN, KT, 256> ks, vs;
+    Stage<O, T, DP, PLAIN, KT, 256> ks, vs;
     // one pass over the keys: f(sub-tile's keys, values, p, dp, first key)
     auto pass = [&](float from, auto &&f) {  // from: what dp starts from, in the last pass less delta
       __syncthreads();
@@ -117,8 +123,8 @@ __global__ __launch_bounds__(256) void queries_kernel(Args a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) z[r] = 0.f;
           }
-          z = O::scores(krows, own, i, g, z);
-          dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp);
+          z = O::scores(krows, own, i, g, z, a.D);
+          dp = O::scores(vt + 32 * s * O::kStride, dy, i, g, dp, a.D);
           if (!sights.all(k0)) {
             const Span span = keys_of(a, len, me);
             hide(z, span, k0, g, -INFINITY);
@@ -233,8 +239,8 @@ __global__ __launch_bounds__(256) void bias_sums_kernel(const float *parts, int6
 // for those tiles alone, whose sums are joined by sink_sums_kernel.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, bool PLAIN, bool BIAS>
-__global__ __launch_bounds__(256) void keys_kernel(Args a) {
-  constexpr int QT = tile_rows<T, DP>(), SUB = QT / 32, TILE = QT * Ops<T, DP>::kStride;
+__global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
+  constexpr int QT = tile_rows<T, DP>(), SUB = QT / 32, TILE = QT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][queries, gradients][QT][stride]
   float *const stats = reinterpret_cast<float *>(tiles + 4 * TILE);  // [buffer][log2 denominators, deltas][QT]
@@ -249,14 +255,14 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
     else block -= chunks;
   }
   const int len = length_of(a, b), k0 = block * 128, kw = k0 + 32 * wave, me = kw + i;
-  using O = Ops<T, DP>;
+  using O = WindowOps<T, DP>;
   f32x16 dk[DP / 32], dv[DP / 32];
   zero(dk);
   zero(dv);
   if (k0 < len) {
-    typename O::Rows key = O::template rows<PLAIN>(head_of<T>(a.k, b, hk), a.k.row, me, len, me < len, a.D, g);
-    typename O::Rows value = O::template rows<PLAIN>(head_of<T>(a.v, b, hk), a.v.row, me, len, me < len, a.D, g);
-    O::settle(key), O::settle(value);
+    const typename O::Raw raw_key = O::template rows<PLAIN>(head_of<T>(a.k, b, hk), a.k.row, me, len, me < len, a.D, g);
+    const typename O::Raw raw_value = O::template rows<PLAIN>(head_of<T>(a.v, b, hk), a.v.row, me, len, me < len, a.D, g);
+    const typename O::Rows key = O::settle(raw_key), value = O::settle(raw_value);
     Sights sights = sights_of_keys(a, len, kw);
     if (chunks > 0 && (kw < a.sink_rows) != (chunk >= 0)) sights.high = -1;  // the other workgroups' rows
     // queries that see a key of the block: i >= j - right, and i <= j + left or j a sink
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
       t1 = t1 < chunk * each + each - 1 ? t1 : chunk * each + each - 1;
     }
     const int tiles_of_head = t1 - t0 + 1, count = tiles_of_head > 0 ? tiles_of_head * G : 0;
-    Stage<T, DP, PLAIN, QT, 256> qs, gs;
+    Stage<O, T, DP, PLAIN, QT, 256> qs, gs;
     float stat = 0.f;
     // the tile in work and the one to fetch, counted on: a division an iteration by each of two was half of all scalar work
     int h = hk * G, tile = t0, next_h = hk * G, next_tile = t0;
@@ -334,8 +340,8 @@ __global__ __launch_bounds__(256) void keys_kernel(Args a) {
             for (int r = 0; r < 16; ++r) z[r] += far;
           }
         }
-        z = O::scores(qrows, key, i, g, z);
-        dp = O::scores(grows, value, i, g, dp);
+        z = O::scores(qrows, key, i, g, z, a.D);
+        dp = O::scores(grows, value, i, g, dp, a.D);
         if (!sights.all(q0)) hide(z, queries_of(a, len, me), q0, g, -INFINITY);
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(z[r] * a.c);
@@ -414,7 +420,7 @@ __global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 static int launch_queries(const Args &a, hipStream_t st) {
-  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * Ops<T, DP>::kStride * sizeof(T) +
+  const size_t lds = 4 * (size_t)tile_rows<T, DP>() * WindowOps<T, DP>::kStride * sizeof(T) +
                      (BIAS ? (DBIAS ? 5 : 1) * table_size(a.bias) * sizeof(float) : 0) + (DBIAS ? 16 + 4 * kDiagonals * kDiagonal * sizeof(float) : 0);
   auto kernel = queries_kernel<T, DP, PLAIN, BIAS, DBIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
@@ -424,7 +430,7 @@ static int launch_queries(const Args &a, hipStream_t st) {
 template <class T, int DP, bool PLAIN, bool BIAS>
 static int launch_keys(const Args &a, hipStream_t st) {
   constexpr int QT = tile_rows<T, DP>();
-  const size_t lds = 4 * (size_t)QT * Ops<T, DP>::kStride * sizeof(T) + 4 * QT * sizeof(float) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
+  const size_t lds = 4 * (size_t)QT * WindowOps<T, DP>::kStride * sizeof(T) + 4 * QT * sizeof(float) + (BIAS ? table_size(a.bias) * sizeof(float) : 0);
   auto kernel = keys_kernel<T, DP, PLAIN, BIAS>;
   if (int rc = allow_dynamic_lds(kernel, lds)) return rc;
   const int64_t per_head = a.blocks + a.sink_chunks;

@@ -141,6 +141,38 @@ def test_wild_values_where_they_are_not_seen(value, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_infinite_keys_in_sight(D, dtype):
+    """A key whose scores are all -inf weighs nothing; one whose scores are +inf leaves NaN to the points that see it, as a softmax does."""
+    announce("infinite", D, dtype)
+    q, k, v, _, bias = make(1, 150, 2, 2, D, dtype, 8, seed=4)
+    q = q.abs() + 1
+    call = dict(window=(20, 9), sinks=3, bias=bias, max_distance=12)
+    for at in (1, 70):  # a first point, which all see; a point in the middle
+        k2 = k.clone()
+        k2[0, at, :, 0] = float("-inf")
+        low = k.clone()
+        low[0, at, :, 0] = -2000.0  # weights below exp(-170)
+        y = PF.window_attention(q, k2, v, **call)
+        wo.check(y, wo.attention(q, low, v, **call)["y"], ("-inf", at))
+        k2[0, at, :, 0] = float("inf")
+        y = PF.window_attention(q, k2, v, **call)[0]
+        i = torch.arange(150, device="cuda")
+        sees = (i >= at - 9) if at < 3 else (i >= at - 9) & (i <= at + 20)
+        assert torch.isnan(y[sees]).all() and torch.isfinite(y[~sees]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("bias", [False, True])
+def test_scores_that_outgrow_the_first(bias, dtype):
+    """Scores that rise by hundreds along the window, beyond what exp2 holds: the weights of the largest, as a softmax has them."""
+    announce("outgrow", bias, dtype)
+    q, k, v, dy, table = make(2, 700, 2, 1, 32, dtype, 8, seed=6)
+    q[..., 0], k[..., 0] = 8.0, torch.linspace(-160, 160, 700, device="cuda").to(dtype)[None, :, None]  # 226 a hundred points
+    compare(q, k, v, dy, table if bias else None, window=(300, 150), sinks=2, **(dict(max_distance=20) if bias else {}))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_views(dtype):
     """Slices of one projection, shared keys (stride 0), rows off 16-byte boundaries, heads in front of rows: the results of copies."""
     announce("views", dtype)
