@@ -352,19 +352,30 @@ __global__ __launch_bounds__(256) void join_kernel(StepArgs s) {
   const int column = ct * 32 + c;
   if (column >= s.columns) return;
   const int64_t slot = work * s.parts;
+  // a part's maximum and sum a lane, so that nothing waits for the part before
+  const auto most_and_sum = [&](int p) { return reinterpret_cast<const float2 *>(s.part_ml)[(slot + p) * 32 + c]; };
   float top = -INFINITY;
-  for (int p = 0; p < s.parts; ++p) top = fmaxf(top, s.part_ml[((slot + p) * 32 + c) * 2]);
+  for (int p = lane; p < s.parts; p += 64) top = fmaxf(top, most_and_sum(p).x);
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   const float ref = top == -INFINITY ? 0.f : top;
   float total = 0.f, o[(DP + 63) / 64] = {};
-  for (int p = 0; p < s.parts; ++p) {
-    const float l = s.part_ml[((slot + p) * 32 + c) * 2 + 1];
-    if (l == 0.f) continue;
-    const float w = __builtin_amdgcn_exp2f(s.part_ml[((slot + p) * 32 + c) * 2] - ref);
-    total += l * w;
+  for (int first = 0; first < s.parts; first += 64) {
+    float w = 0.f;
+    if (first + lane < s.parts) {
+      const float2 ml = most_and_sum(first + lane);
+      if (ml.y != 0.f) w = __builtin_amdgcn_exp2f(ml.x - ref), total += ml.y * w;
+    }
+    const int count = s.parts - first < 64 ? s.parts - first : 64;
+#pragma unroll 8
+    for (int p = 0; p < count; ++p) {  // parts without a sum hold zeros
+      const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), p));
 #pragma unroll
-    for (int k = 0; k < (DP + 63) / 64; ++k)
-      if (lane + 64 * k < DP) o[k] += s.part_o[((slot + p) * 32 + c) * DP + lane + 64 * k] * w;
+      for (int k = 0; k < (DP + 63) / 64; ++k)
+        if (lane + 64 * k < DP) o[k] += s.part_o[((slot + first + p) * 32 + c) * DP + lane + 64 * k] * by;
+    }
   }
+  total = wave_sum(total);
   const int t = column / s.G, hq = hk * s.G + column - t * s.G;
 #pragma unroll
   for (int k = 0; k < (DP + 63) / 64; ++k)
