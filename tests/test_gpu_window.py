@@ -173,6 +173,20 @@ def test_scores_that_outgrow_the_first(bias, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_nan_and_the_bias_gradient(dtype):
+    """A gradient that is NaN at one point reaches the buckets of the distances that the point sees; the others stay as they were."""
+    announce("nan in d bias", dtype)
+    q, k, v, dy, bias = make(1, 90, 2, 1, 32, dtype, 16, seed=2)
+    def grad(dy):
+        leaf = bias.detach().requires_grad_(True)
+        return torch.autograd.grad(PA.window_attention(q, k, v, bias=leaf, window=(60, 0), max_distance=40), leaf, dy)[0]
+    clean, bad = grad(dy), dy.clone()
+    bad[0, 3, 0] = float("nan")  # sees distances 0 .. 3, of a bucket each
+    got = grad(bad)
+    assert torch.isnan(got[:4, 0]).all() and torch.equal(got[4:], clean[4:]) and torch.equal(got[:, 1], clean[:, 1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_views(dtype):
     """Slices of one projection, shared keys (stride 0), rows off 16-byte boundaries, heads in front of rows: the results of copies."""
     announce("views", dtype)
