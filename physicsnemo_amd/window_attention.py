@@ -32,8 +32,13 @@ class WindowCache:
             self.lengths.zero_()
             self.used = 0
         else:
+            if lengths.shape != self.lengths.shape:
+                raise ValueError(f"lengths have to be of shape {tuple(self.lengths.shape)}, got {tuple(lengths.shape)}")
+            low, high = (int(n) for n in lengths.aminmax()) if lengths.numel() else (0, 0)
+            if low < 0 or high > self.capacity:
+                raise ValueError(f"lengths have to be between 0 and {self.capacity}, got {low} to {high}")
             self.lengths.copy_(lengths)
-            self.used = int(lengths.max()) if lengths.numel() else 0
+            self.used = high
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v (B, T, heads, dim_head) behind what each sequence holds."""
@@ -83,16 +88,23 @@ class WindowAttention(nn.Module):
             self.q_norm_weight = nn.Parameter(torch.ones(dim_head))
             self.k_norm_weight = nn.Parameter(torch.ones(dim_head))
         self.bias = nn.Parameter(torch.zeros(bias_buckets, heads)) if bias_buckets else None
-        frequencies = None
-        if rotary_base is not None:
-            pairs = dim_head // 2
-            if pairs < axes:
-                raise ValueError(f"{dim_head} channels a head have {pairs} pairs, too few for {axes} axes")
-            each = pairs // axes
-            frequencies = torch.zeros(axes, each * axes)
-            for a in range(axes):
-                frequencies[a, a * each:(a + 1) * each] = float(rotary_base) ** (-torch.arange(each, dtype=torch.float64) / each)
-        self.register_buffer("frequencies", frequencies, persistent=False)
+        self.rotary_base = rotary_base
+        if rotary_base is not None and dim_head // 2 < axes:
+            raise ValueError(f"{dim_head} channels a head have {dim_head // 2} pairs, too few for {axes} axes")
+        self.register_buffer("frequencies", None if rotary_base is None else self._frequencies(), persistent=False)
+
+    def _frequencies(self) -> torch.Tensor:
+        each = self.dim_head // 2 // self.axes
+        frequencies = torch.zeros(self.axes, each * self.axes)
+        for a in range(self.axes):
+            frequencies[a, a * each:(a + 1) * each] = float(self.rotary_base) ** (-torch.arange(each, dtype=torch.float64) / each)
+        return frequencies
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.frequencies is not None:  # float32 whatever type the weights are cast to
+            self.frequencies = self._frequencies().to(self.frequencies.device)
+        return self
 
     def extra_repr(self) -> str:
         return f"heads={self.heads}, kv_heads={self.kv_heads}, window={self.window}, sinks={self.sinks}"

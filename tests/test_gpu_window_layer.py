@@ -127,6 +127,20 @@ def test_model_with_window_blocks(autocast):
         assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.any(), name
 
 
+def test_model_cast_to_bfloat16():
+    """Weights cast as a whole: the angles stay float32, the model runs and trains."""
+    announce("bf16 model")
+    torch.manual_seed(4)
+    model = pn.Transolver(functional_dim=3, out_dim=2, embedding_dim=2, n_layers=2, n_hidden=128, n_head=4, slice_num=16, use_te=False, dropout=0.0,
+                          window_blocks=(1,), window_options=dict(window=(30, 0), bias_buckets=8, max_distance=20)).cuda().to(torch.bfloat16)
+    fx, emb = (torch.randn(2, 300, n, device="cuda", dtype=torch.bfloat16) for n in (3, 2))
+    with torch.no_grad():
+        assert torch.isfinite(model.eval()(fx, emb)).all()
+    model.train()(fx, emb).float().square().mean().backward()
+    for name, p in model.blocks[1].named_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all() and p.grad.any(), name
+
+
 def test_block_with_counter_dropout_and_structured_points():
     announce("block")
     torch.manual_seed(4)

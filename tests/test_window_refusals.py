@@ -160,8 +160,21 @@ def test_the_layer_refuses():
     cache.reset(torch.tensor([1, 0], dtype=torch.int32))
     cache.append(3 * k, k)
     assert cache.k[0, 1:, 0, 0].tolist() == [3, 3] and cache.k[1, :2, 0, 0].tolist() == [3, 3]
+    for lengths in ([0, -1], [4, 0], [1]):
+        with pytest.raises(ValueError, match="lengths have to be"):
+            cache.reset(torch.tensor(lengths, dtype=torch.int32))
+    assert cache.lengths.tolist() == [3, 2] and cache.used == 3
     cache.reset()
     assert cache.used == 0 and not cache.lengths.any()
+
+
+def test_frequencies_of_a_cast_layer():
+    """The type of the weights does not round the angles."""
+    layer = pn.WindowAttention(32, heads=4, dim_head=16, axes=2)
+    own = layer.frequencies.clone()
+    for cast in (layer.to(torch.bfloat16), layer.half(), layer.double(), layer.to("meta"), layer.to_empty(device="cpu")):
+        assert layer.frequencies.dtype == torch.float32
+        assert layer.frequencies.is_meta or torch.equal(layer.frequencies, own)
 
 
 def test_models_with_window_blocks(tmp_path):
