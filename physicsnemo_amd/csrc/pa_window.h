@@ -7,7 +7,8 @@
 //   outcome  o[d][i] = sum_r X[r][d] w[r][i]         w: the weights of the tile, packed where they were formed (a C tile is a pair
 //                                                    of B operands in the order rowmap); X transposed: bf16 by the transposing LDS
 //                                                    read, float32 element by element (lanes run along d: no conflicts)
-// bf16 rows go through v_mfma_f32_32x32x16_bf16, float32 rows through v_mfma_f32_32x32x2_f32.
+// bf16 rows go through v_mfma_f32_32x32x16_bf16, and so do float32 rows to widths of 64 in the kernels over windows, three bf16 values each (Split);
+// wider ones and the steps, which are bound by memory, through v_mfma_f32_32x32x2_f32.
 #pragma once
 
 #include "pa_common.h"
@@ -625,14 +626,19 @@ __device__ __forceinline__ bool not_finite(const f32x16 (&acc)[N]) {
     for (int r = 0; r < 16; ++r) s = fmaf(acc[n][r], 0.f, s);
   return s != s;
 }
-// acc += weight(n, seen) row n of a head, for rows first .. last, in the lanes that see it and are `bad`
-template <class T, int DP, class F>
-__device__ __forceinline__ void add_rows(const T *head, int64_t stride, int first, int last, int D, int g, bool bad, f32x16 (&acc)[DP / 32], F &&weight) {
+// acc += weight(n, seen) row n of a head, for rows first .. last, in the lanes that see it and are `bad`; on(): whether a lane goes on with sums that are all NaN
+struct Nothing {
+  __device__ __forceinline__ bool operator()() const { return false; }
+};
+template <class T, int DP, class F, class W = Nothing>
+__device__ __forceinline__ void add_rows(const T *head, int64_t stride, int first, int last, int D, int g, bool bad, f32x16 (&acc)[DP / 32], F &&weight,
+                                         W &&on = W()) {
 #pragma unroll 1
   for (int n = first; n <= last; ++n) {
     bool seen;
     const float w = weight(n, seen);
     const T *const row = head + n * stride;
+    bool open = on();  // or some of the lane's sums are not NaN
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
@@ -640,8 +646,10 @@ __device__ __forceinline__ void add_rows(const T *head, int64_t stride, int firs
         const int col = 32 * db + rowmap(r, g);
         const float x = col < D ? load_as_f32(row + col) : 0.f;
         acc[db][r] = bad && seen ? fmaf(w, x, acc[db][r]) : acc[db][r];
+        open |= col < D && acc[db][r] == acc[db][r];
         if (r % 4 == 3) asm volatile("" ::: "memory");  // few loads at a time: this path must not cost the others registers
       }
+    if (!some_lane(bad && open)) return;  // NaN whatever follows: an input full of them takes no longer for it
   }
 }
 __device__ __forceinline__ float bias_at(const BiasArgs &b, const float *table, int off) {

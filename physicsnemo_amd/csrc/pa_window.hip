@@ -1,11 +1,17 @@
 // Attention of points over a window of their neighbours and a few first points, served: y_i = sum_j p_ij v_j, p_i the softmax over the
 // visible j of scale q_i . k_j (+ a bias by buckets of j - i).
 //
-// One pass over the visible keys with a running maximum and sum (in log2 units, so that a weight is one multiply-add and one exp2).
+// One pass over the visible keys, a weight one multiply-add and one exp2: a query's reference is the largest score of the first tile that it sees
+// something of, and stays.  Where scores outgrow it until the weights pass 2^30, the workgroup looks for those queries' largest scores and goes over
+// the keys once more (a running maximum would scale the values' sum in a branch, which costs copies of it around every tile: 193 -> 172 us below).
 // A wave owns 32 queries of a head, a lane one of them (with its partner 32 lanes on): the scores of a tile of keys are the rows of a
-// C tile, so that maximum and sum are per lane, and the weights go back into the product with the values as they lie.  Four waves share the
+// C tile, so that reference and sum are per lane, and the weights go back into the product with the values as they lie.  Four waves share the
 // tiles of keys and values, two buffers in LDS, the next tile's loads under the present one's products.  Tiles that a wave's
 // queries do not see are skipped, and only tiles on an edge are masked.
+//
+// What it takes: 131 072 x 8 x 32 bf16, 513 keys a query: 172 us (0.27 GB: 49 us; 69 GFLOP: 50 us; 52 vector and 16 exp2 instructions a tile of 32 x 32:
+// about 110 us at full issue, which bounds it); 3 x 9 001 x 8 over 2 x 64, 1 024 keys: 101; 4 x 7 225 x 8 x 16 float32, 171 keys: 66; with biases
+// 65 536 x 8 x 32, 257 keys: 76.  Five waves a SIMD instead of four spill (2 to 3 times as long), 64 queries a wave lose a third.
 #include "pa_window.h"
 
 #include <math.h>
@@ -161,9 +167,10 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       run.m = high ? most : run.m;
       run.off = run.m == -INFINITY ? 0.f : -run.m * a.c;
     }
-    // A score of a visible infinite key is infinite, which thirds do not give: the sum of the weights is formed again, too
-    bool bad = not_finite(run.o) || run.l * 0.f != 0.f;
+    // A score of a visible infinite key is infinite, which thirds do not give: a sum of weights that is not finite is formed again, too
+    bool again = run.l * 0.f != 0.f, bad = again || not_finite(run.o);
     if (__builtin_expect(some_lane(bad), 0)) {
+      again = half_max(again ? 1.f : 0.f) > 0.f;
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
       const Span span = keys_of(a, len, me);
       for (int d = 0; d < DP / 32; ++d)
@@ -175,17 +182,19 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       };
       const int low = qw - a.left > 0 ? qw - a.left : 0, high = qw + 31 + a.right < len - 1 ? qw + 31 + a.right : len - 1;
       float most = -INFINITY;
-      for (int j = a.sinks > 0 ? 0 : low; j <= high; j = j + 1 == a.sinks && low > j ? low : j + 1)
-        if (const float z = score(j); span.sees(j)) most = fmaxf(most, z);
-      if (bad) run.l = 0.f, run.m = most, run.off = most == -INFINITY ? 0.f : -most * a.c;
+      bool open = true;  // no score is NaN so far
+      for (int j = a.sinks > 0 ? 0 : low; j <= high && some_lane(again && open); j = j + 1 == a.sinks && low > j ? low : j + 1)
+        if (const float z = score(j); span.sees(j)) most = fmaxf(most, z), open = open && z == z;
+      if (again) run.l = 0.f, run.m = most, run.off = most == -INFINITY ? 0.f : -most * a.c;
       auto weight = [&](int j, bool &seen) {
         seen = span.sees(j);
         const float w = __builtin_amdgcn_exp2f(fmaf(score(j), a.c, run.off));
-        if (bad && seen && g == 0) run.l += w;
+        if (again && seen && g == 0) run.l += w;
         return w;
       };
-      add_rows<T, DP>(values, a.v.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, run.o, weight);
-      add_rows<T, DP>(values, a.v.row, low, high, a.D, g, bad, run.o, weight);
+      auto on = [&] { return again && g == 0 && run.l == run.l; };
+      add_rows<T, DP>(values, a.v.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, run.o, weight, on);
+      add_rows<T, DP>(values, a.v.row, low, high, a.D, g, bad, run.o, weight, on);
     }
   }
   const float l = half_sum(run.l);

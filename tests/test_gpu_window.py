@@ -187,6 +187,26 @@ def test_nan_and_the_bias_gradient(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("which", ["all", "k", "v"])
+def test_inputs_full_of_nan(which, dtype):
+    """NaN everywhere is NaN everywhere; with NaN in the values alone the weights, and so dv, are those of the scores."""
+    announce("full of nan", which, dtype)
+    q, k, v, dy, _ = make(1, 3000, 2, 1, 40, dtype, seed=8)
+    want = wo.attention(q, k, v, sinks=0, dy=dy)
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if which in ("all", name):
+            t.fill_(float("nan"))
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    y = PA.window_attention(*leaves)
+    dq, dk, dv = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.isnan(t).all() for t in (y, dq, dk))
+    if which == "v":
+        wo.check(dv, want["dv"], "dv")
+    else:
+        assert torch.isnan(dv).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_views(dtype):
     """Slices of one projection, shared keys (stride 0), rows off 16-byte boundaries, heads in front of rows: the results of copies."""
     announce("views", dtype)
