@@ -1427,6 +1427,15 @@ def _heads_of(t, what: str, device, dtype, shape):
     return _lib.PaHeads(t.data_ptr(), batch, row, head)
 
 
+def _beside(q, *others):
+    """What goes with heads of any strides: on their GPU and contiguous."""
+    others = [t for t in others if t is not None]
+    if others:
+        _together(*others)
+        if others[0].device != q.device:
+            raise ValueError(f"all tensors have to be on the input's device ({q.device}), got one on {others[0].device}")
+
+
 def _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved):
     """(params, q and k as heads) of the norm_rotate functions after checking that the arguments belong together."""
     if q.ndim != 4 or k.ndim != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
@@ -1438,7 +1447,7 @@ def _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, in
     _lib.dtype_code(q.dtype)
     if not norm and not (q_weight is None and k_weight is None):
         raise ValueError("weights belong to the norm: there are none without it")
-    _together(q.new_empty(0), positions, frequencies, q_weight, k_weight)
+    _beside(q, positions, frequencies, q_weight, k_weight)
     _expect(q_weight, "q_weight", (D,), torch.float32)
     _expect(k_weight, "k_weight", (D,), torch.float32)
     if D == 0 or Hq == 0 or k.shape[2] == 0 or D > _SEQ_LIMITS["D"]:
@@ -1527,7 +1536,7 @@ def _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance):
     scale = D ** -0.5 if scale is None else float(scale)
     if not 1e-30 < scale < 1e30:
         raise ValueError(f"scale has to be positive, got {scale}")
-    _together(q.new_empty(0), lengths, bias)
+    _beside(q, lengths, bias)
     _expect(lengths, "lengths", (B,), torch.int32)
     buckets = distance = 0
     if bias is not None:
