@@ -806,7 +806,7 @@ int pa_norm_rotate_backward(int dtype, const pa_rotate_params *p, const pa_heads
  * gradients.  What i does not see has no part in y_i, infinities and NaN included.
  * Buckets of the distance d = |j - i|, n = buckets of them for j <= i where right is 0; else n = buckets / 2 for j <= i and as many for j > i
  * behind them.  With E = n / 2: d < E has bucket d, others E + the largest b < n - E with d >= E (distance / E)^(b / (n - E)). */
-#define PA_MAX_WINDOW_N (1ll << 29)
+#define PA_MAX_WINDOW_N (1ll << 29)  /* and, in all, below 2^24 of ceil(N / 128) + ceil(N / 512) blocks x Hq x B (a launch's threads) */
 #define PA_MAX_SINKS 128
 #define PA_MAX_BUCKETS 256
 #define PA_MAX_DISTANCE 2048

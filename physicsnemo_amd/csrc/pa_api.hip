@@ -2048,8 +2048,8 @@ static int check_window(int dtype, const pa_window_params *p) {
   if (p->left < PA_NO_BOUND || p->right < PA_NO_BOUND || p->sinks < 0 || p->buckets < 0) return PA_ERR_DIMS;
   if (!(p->scale > 1e-30 && p->scale < 1e30)) return PA_ERR_DIMS;
   if (p->D > PA_MAX_D || p->Hq > 4096 || p->N > PA_MAX_WINDOW_N || p->B > (1 << 24) || p->sinks > PA_MAX_SINKS) return PA_ERR_UNSUPPORTED;
-  // one workgroup per 128 rows of a head, and as many again for the first rows of each
-  if (((p->N + 127) / 128 + (p->N + 511) / 512) > ((1ll << 31) - 1) / (p->Hq * p->B)) return PA_ERR_UNSUPPORTED;
+  // a workgroup of 256 per 128 rows of a head and up to a quarter of that for the first rows: a launch holds less than 2^32 threads
+  if (((p->N + 127) / 128 + (p->N + 511) / 512) > ((1ll << 24) - 1) / (p->Hq * p->B)) return PA_ERR_UNSUPPORTED;
   if (p->buckets > 0) {
     const int64_t side = p->right != 0 ? p->buckets / 2 : p->buckets;
     if (side < 2 || (p->right != 0 && p->buckets % 2 != 0) || p->distance <= side / 2) return PA_ERR_DIMS;
@@ -2092,7 +2092,7 @@ static int check_step(int dtype, const pa_window_params *p, int64_t T) {
   if (T <= 0 || T > p->N || p->right != 0) return PA_ERR_DIMS;
   if (!p->lengths) return PA_ERR_NULL;
   const int64_t G = p->Hq / p->Hk, tiles = (T * G + 31) / 32;
-  if (p->buckets * G > 16384 || T > (1 << 24) || tiles * 8 > ((1ll << 31) - 1) / (p->Hk * p->B)) return PA_ERR_UNSUPPORTED;
+  if (p->buckets * G > 16384 || T > (1 << 24) || tiles * 8 > ((1ll << 24) - 1) / (p->Hk * p->B)) return PA_ERR_UNSUPPORTED;
   return PA_OK;
 }
 

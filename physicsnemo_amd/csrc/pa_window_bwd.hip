@@ -404,23 +404,27 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
 template <class T>
 __global__ __launch_bounds__(256) void sink_sums_kernel(Args a) {
   __shared__ float parts[8][32];
-  const int64_t per = 2 * a.sink_rows * (int64_t)a.D, e = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-  const bool some = e < (int64_t)a.B * a.Hk * per;
-  const int64_t head = some ? e / per : 0, at = some ? e - head * per : 0;
-  const float *p = a.sink_parts + head * a.sink_chunks * per + at;
+  const int64_t per = 2 * a.sink_rows * (int64_t)a.D, all = (int64_t)a.B * a.Hk * per;
   const int part = threadIdx.x >> 5, each = (a.sink_chunks + 7) / 8, last = part * each + each < a.sink_chunks ? part * each + each : a.sink_chunks;
-  float sum = 0.f;
+  for (int64_t first = (int64_t)blockIdx.x * 32; first < all; first += (int64_t)gridDim.x * 32) {
+    const int64_t e = first + (threadIdx.x & 31);  // `per` is whole thirty-twos
+    const int64_t head = e / per, at = e - head * per;
+    const float *p = a.sink_parts + head * a.sink_chunks * per + at;
+    float sum = 0.f;
 #pragma unroll 4
-  for (int c = part * each; c < last; ++c) sum += p[c * per];
-  parts[part][threadIdx.x & 31] = sum;
-  __syncthreads();
-  if (part != 0 || !some) return;
+    for (int c = part * each; c < last; ++c) sum += p[c * per];
+    parts[part][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (part == 0) {
 #pragma unroll
-  for (int k = 1; k < 8; ++k) sum += parts[k][threadIdx.x];
-  const int b = (int)(head / a.Hk), hk = (int)(head % a.Hk), side = (int)(at / (a.sink_rows * a.D));
-  const int row = (int)(at / a.D % a.sink_rows), d = (int)(at % a.D);
-  T *const out = static_cast<T *>(side ? a.dv : a.dk);
-  if (row < a.N) store_from_f32(out + (((int64_t)b * a.N + row) * a.Hk + hk) * a.D + d, sum);
+      for (int k = 1; k < 8; ++k) sum += parts[k][threadIdx.x];
+      const int b = (int)(head / a.Hk), hk = (int)(head % a.Hk), side = (int)(at / (a.sink_rows * a.D));
+      const int row = (int)(at / a.D % a.sink_rows), d = (int)(at % a.D);
+      T *const out = static_cast<T *>(side ? a.dv : a.dk);
+      if (row < a.N) store_from_f32(out + (((int64_t)b * a.N + row) * a.Hk + hk) * a.D + d, sum);
+    }
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -446,7 +450,7 @@ static int launch_keys(const Args &a, hipStream_t st) {
   if (int rc = launch_status()) return rc;
   if (a.sink_chunks == 0) return PA_OK;
   const int64_t n = (int64_t)a.B * a.Hk * 2 * a.sink_rows * a.D;
-  sink_sums_kernel<T><<<(unsigned)((n + 31) / 32), 256, 0, st>>>(a);
+  sink_sums_kernel<T><<<(unsigned)(n / 32 < 16384 ? n / 32 : 16384), 256, 0, st>>>(a);
   return launch_status();
 }
 template <class T>

@@ -207,6 +207,14 @@ def test_inputs_full_of_nan(which, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_first_points_of_many_sequences(dtype):
+    """More sums of first points' gradients than one round of their workgroups holds."""
+    announce("many", dtype)
+    q, k, v, dy, _ = make(40, 130, 4, 4, 64, dtype, seed=1)
+    compare(q, k, v, dy, None, window=(5, 0), sinks=128)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_views(dtype):
     """Slices of one projection, shared keys (stride 0), rows off 16-byte boundaries, heads in front of rows: the results of copies."""
     announce("views", dtype)

@@ -27,7 +27,7 @@ def window(**kw):
 WINDOWS = [(dict(B=0), -2), (dict(N=0), -2), (dict(Hq=0), -2), (dict(Hk=0), -2), (dict(D=0), -2), (dict(Hq=5), -2), (dict(left=-2), -2), (dict(right=-2), -2),
            (dict(sinks=-1), -2), (dict(scale=0.0), -2), (dict(scale=-1.0), -2), (dict(scale=float("nan")), -2), (dict(scale=float("inf")), -2),
            (dict(D=129), -3), (dict(sinks=129), -3), (dict(N=(1 << 29) + 1), -3), (dict(Hq=8192, Hk=8192), -3), (dict(B=1 << 25), -3),
-           (dict(B=1 << 20, N=1 << 20), -3), (dict(buckets=-1), -2), (dict(buckets=2, distance=9, bias=P), -2), (dict(buckets=7, distance=9, bias=P), -2),
+           (dict(B=1 << 20, N=1 << 20), -3), (dict(B=1 << 21), -3), (dict(N=1 << 28, Hq=8, Hk=8, B=1), -3), (dict(buckets=-1), -2), (dict(buckets=2, distance=9, bias=P), -2), (dict(buckets=7, distance=9, bias=P), -2),
            (dict(buckets=32, distance=8, bias=P), -2), (dict(buckets=32, distance=16, right=0, bias=P), -2), (dict(buckets=258, distance=500, bias=P), -3),
            (dict(buckets=32, distance=2049, bias=P), -3), (dict(buckets=32, distance=64), -1)]
 
