@@ -553,8 +553,9 @@ template <class T, int DP>
 using WindowOps = typename std::conditional<sizeof(T) == 4 && DP <= 64, Split<(DP <= 64 ? DP : 64)>, Ops<T, DP>>::type;
 
 // ROWS rows of DP channels on their way from memory to LDS by THREADS threads: loaded into registers, written later.  PLAIN rows come by
-// buffer loads: a lane's offset in a tile never changes, the tile's place is in scalar registers, and what lies outside reads as zero without a
-// comparison.  Others by element where a piece is not whole.
+// buffer loads: a lane's offsets in a tile never change, the tile's place is in scalar registers, and what lies outside reads as zero without a
+// comparison.  All of an offset is in the vector register: the scalar one takes no part in the comparison with the buffer's size.  Others by
+// element where a piece is not whole.
 template <class O, class T, int DP, bool PLAIN, int ROWS, int THREADS>
 struct Stage {
   static constexpr int V = 16 / sizeof(T), PER_ROW = DP / V, UNITS = ROWS * PER_ROW / THREADS;
@@ -566,9 +567,11 @@ struct Stage {
       const int left = limit - first, bytes = (int)view.row * (int)sizeof(T), col = tid % PER_ROW * V;
       const __amdgpu_buffer_rsrc_t src = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<T *>(head + first * view.row), 0, left <= 0 ? 0 : (left < ROWS ? left : ROWS) * bytes, 0x00027000);
-      const int at = col < D ? tid / PER_ROW * bytes + col * (int)sizeof(T) : 0x7ffffff0;
+      // rows are below 2^22 bytes (make_view) and at most 64: what starts at 2^31 - 16 stays outside for every unit
+      uint32_t at = col < D ? (uint32_t)(tid / PER_ROW * bytes + col * (int)sizeof(T)) : 0x7ffffff0u;
+      asm volatile("" : "+v"(at));  // the units' offsets are formed here, not kept in a register each around the loop
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) w[u] = __builtin_amdgcn_raw_buffer_load_b128(src, at, u * (THREADS / PER_ROW) * bytes, 0);
+      for (int u = 0; u < UNITS; ++u) w[u] = __builtin_amdgcn_raw_buffer_load_b128(src, at + (uint32_t)(u * (THREADS / PER_ROW) * bytes), 0, 0);
     } else {
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
