@@ -184,6 +184,7 @@ struct Partners {
   float sign[8];
 };
 __device__ __forceinline__ int spread(int c) { return c + (c >> 3); }  // a gap every eight floats spreads lanes over the banks
+constexpr int kNone = 8;  // the first gap: -0, what a channel that is not turned takes from its partner, so that it stays as it is, infinite or not
 template <int LANES>
 __device__ __forceinline__ Partners partners_of(int half, int slot) {
   Partners p;
@@ -191,7 +192,7 @@ __device__ __forceinline__ Partners partners_of(int half, int slot) {
   for (int j = 0; j < 8; ++j) {
     const int c = 8 * slot + j;
     const bool lower = c < half, turned = c < 2 * half;
-    p.other[j] = spread(!turned ? c : lower ? c + half : c - half);
+    p.other[j] = !turned ? kNone : spread(lower ? c + half : c - half);
     p.pair[j] = !turned ? half : lower ? c : c - half;  // behind the pairs: one that turns nothing
     p.sign[j] = lower ? -1.f : 1.f;
   }
@@ -205,10 +206,11 @@ __device__ __forceinline__ void turn(float (&v)[8], const float2 *cs, int half, 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int a = PAIRS == kNeighbours ? 2 * j : j, b = PAIRS == kNeighbours ? 2 * j + 1 : j + 4, pair = 4 * slot + j;
-      const float2 t = pair < half ? cs[pair] : make_float2(1.f, 0.f);
+      const bool turned = pair < half;  // others stay as they are: a product with a sine of zero would make an infinity in one NaN in both
+      const float2 t = cs[turned ? pair : half];
       const float x = v[a], y = v[b];
-      v[a] = x * t.x - sign * y * t.y;
-      v[b] = sign * x * t.y + y * t.x;
+      v[a] = turned ? x * t.x - sign * y * t.y : x;
+      v[b] = turned ? sign * x * t.y + y * t.x : y;
     }
   } else {
     // the lanes of a row are lanes of one wave, whose LDS accesses happen in order
@@ -261,6 +263,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
   const Place place = place_of<PAIRS>(a.half, slot);
   auto channel = [&](int j) { return j < 4 ? place.at0 + j : place.at1 + j - 4; };
   const Partners partners = partners_of<LANES>(a.half, slot);
+  if (PAIRS == kApart && slot == 0) exchange[group * (9 * LANES + 1) + kNone] = -0.f;
   const float inv = 1.f / (float)D;
   float wq[8], wk[8], sq[8] = {}, sk[8] = {};  // weights, sums of their gradients
 #pragma unroll
