@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
         }
         const float mean = a.norm ? lanes_sum<LANES>(dot) * inv : 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = rstd * (g[j] - v[j] * mean);
+        for (int j = 0; j < 8; ++j) v[j] = a.norm ? rstd * (g[j] - v[j] * mean) : g[j];  // without the norm x has no part in it, infinite or not
       }
       if (s.out) store_row<T, PAIRS>(out, place, live ? D : 0, v);
     }

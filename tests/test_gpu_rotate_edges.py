@@ -58,3 +58,22 @@ def test_infinite_channels_under_the_norm(D, R, interleaved, dtype):
         want[0, 4, 1] = 0
         want[0, 4, 1, at] = float("nan")
         assert same(got[0], want) and torch.equal(got[1], clean[1]), at
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("value", WILD)
+@pytest.mark.parametrize("D,R,interleaved", PAIRINGS)
+def test_gradients_without_the_norm_do_not_read_the_inputs(D, R, interleaved, value, dtype):
+    """dx is dy turned back, whatever x holds."""
+    announce("without the norm", D, R, interleaved, value, dtype)
+    N = 19
+    q, k, _, _, dyq, dyk = make(2, N, 2, 1, D, dtype, seed=D + 2)
+    turn = (torch.arange(N, device="cuda"), speeds(R // 2)) if R else (None, None)
+    call = dict(norm=False, interleaved=interleaved)
+    wild = [torch.full_like(t, value) for t in (q, k)]
+    clean = PF.norm_rotate_backward(dyq, dyk, q, k, None, None, *turn, **call)
+    got = PF.norm_rotate_backward(dyq, dyk, *wild, None, None, *turn, **call)
+    assert all(torch.equal(a, b) for a, b in zip(got[:2], clean[:2]))
+    leaves = [t.requires_grad_(True) for t in wild]
+    own = torch.autograd.grad(PA.norm_rotate(*leaves, None, None, *turn, **call), leaves, [dyq, dyk])
+    assert all(torch.equal(a, b) for a, b in zip(own, clean[:2]))
