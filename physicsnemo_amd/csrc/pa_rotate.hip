@@ -296,6 +296,7 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
         rstd = __builtin_amdgcn_rsqf(fmaf(lanes_sum<LANES>(sum), inv, a.eps));
+        if (BACK && !live) rstd = 1.f;  // with eps = 0 a row of zeros is NaN: not in lanes that hold no row, which add to the weights' sums, too
       }
       if constexpr (!BACK) {
 #pragma unroll

@@ -5,7 +5,7 @@ import torch
 from gpu_util import announce
 from physicsnemo_amd import autograd as PA
 from physicsnemo_amd import functional as PF
-from test_gpu_rotate import make, speeds
+from test_gpu_rotate import compare, make, speeds
 
 pytestmark = pytest.mark.gpu
 WILD = [float("inf"), float("-inf"), float("nan")]
@@ -77,3 +77,12 @@ def test_gradients_without_the_norm_do_not_read_the_inputs(D, R, interleaved, va
     leaves = [t.requires_grad_(True) for t in wild]
     own = torch.autograd.grad(PA.norm_rotate(*leaves, None, None, *turn, **call), leaves, [dyq, dyk])
     assert all(torch.equal(a, b) for a, b in zip(own, clean[:2]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,N,Hq,Hk,D", [(1, 1, 1, 1, 8), (1, 5, 3, 1, 32), (2, 7, 2, 2, 33), (1, 1031, 3, 2, 64), (3, 2, 1, 1, 128)])
+def test_no_eps(B, N, Hq, Hk, D, dtype):
+    """eps = 0: rows that are not zero have their norm, and weight gradients sum them alone, also where rows do not fill a workgroup."""
+    announce("no eps", B, N, Hq, Hk, D, dtype)
+    q, k, wq, wk, dyq, dyk = make(B, N, Hq, Hk, D, dtype, seed=N)
+    compare(q, k, wq, wk, torch.arange(N, device="cuda"), speeds(D // 2), dyq, dyk, eps=0.0)
