@@ -772,7 +772,8 @@ typedef struct pa_heads {
 } pa_heads;
 
 /* Queries and keys normalised and turned: u = x (mean_d x^2 + eps)^(-1/2) weight, then pair p of u's channels, (a, b), becomes
- * (a cos t - b sin t, a sin t + b cos t), t = sum_a positions[b, n, a] frequencies[a, p] (rounded only once it is within one turn).
+ * (a cos t - b sin t, a sin t + b cos t), t = sum_a positions[b, n, a] frequencies[a, p] (rounded only once it is within one turn;
+ * a pair with a product past 2^78, or with a whole position past 2^53, is NaN).
  * Pairs: (p, p + rotated / 2), with `interleaved` (2 p, 2 p + 1); channels behind `rotated` are not turned. */
 #define PA_POS_I32 0
 #define PA_POS_I64 1

@@ -2,8 +2,9 @@
 //   u = x r w,  r = (mean_d x^2 + eps)^(-1/2);  y = T u, T turning pair p of the channels by t_p = sum_a pos_a f_{a,p}
 //   g = T^-1 dy;  dw = sum g x r;  dx = r (t - xh mean_d(t xh)),  t = g w,  xh = x r
 // Angles of far positions: t / (2 pi) is formed as a product of two doubles with the rounding of the first one carried along, and
-// only what is left of it after whole quarter turns is rounded to float32, so that cos and sin are good to 2e-7 for every position
-// that a float32 or a 53-bit integer holds.  Sums, norms and the turn are float32; a result is rounded once.
+// only what is left of it after whole quarter turns is rounded to float32, so that cos and sin are good to 2.4e-7 (4 u) while every pos_a f_{a,p} is
+// within 2^78 (error of the turn: 2^-107 of the product, 4e-8 at 2^79 in all) and whole positions within 2^53.  What lies further out is NaN.  Sums,
+// norms and the turn are float32; a result is rounded once.
 //
 // Bound by HBM: two element accesses forward, three backward.  A workgroup forms cos and sin of its points once, in LDS, for all heads
 // (a double-precision product and two polynomials per angle, for Hq + Hk rows of use); a lane holds eight channels of a row, its pairs
@@ -59,9 +60,14 @@ __device__ __forceinline__ Spot spot_of(const Args &a, const Spot &first, int n)
 __device__ __forceinline__ int quotient(int n, uint32_t by, int d) { return d == 1 ? n : (int)__umulhi((uint32_t)n, by); }
 
 // ---- cos and sin of a point's angle ----
+constexpr int64_t kMostWhole = 1ll << 53;
+constexpr double kMostAngle = 0x1p78;
 __device__ __forceinline__ double position(const Args &a, int64_t at) {
   if (a.position_type == PA_POS_F32) return (double)static_cast<const float *>(a.positions)[at];
-  if (a.position_type == PA_POS_I64) return (double)static_cast<const int64_t *>(a.positions)[at];
+  if (a.position_type == PA_POS_I64) {
+    const int64_t n = static_cast<const int64_t *>(a.positions)[at];
+    return n <= kMostWhole && n >= -kMostWhole ? (double)n : __builtin_nan("");
+  }
   return (double)static_cast<const int32_t *>(a.positions)[at];
 }
 // pos f in turns, less whole turns
@@ -70,7 +76,7 @@ __device__ __forceinline__ double turns(double pos, double f) {
   constexpr double hi = 0x1.45f306dc9c883p-3, lo = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
   const double t = pos * f, t_rest = fma(pos, f, -t);
   const double u = t * hi, rest = fma(t, hi, -u) + fma(t, lo, t_rest * hi);
-  return (u - rint(u)) + rest;
+  return fabs(t) <= kMostAngle ? (u - rint(u)) + rest : __builtin_nan("");
 }
 __device__ __forceinline__ float2 cos_sin(const Args &a, const Spot &spot, int p) {
   const int64_t at = spot.b * a.position_batch + spot.r * a.axes;

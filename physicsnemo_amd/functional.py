@@ -1477,7 +1477,8 @@ def norm_rotate(q, k, q_weight=None, k_weight=None, positions=None, frequencies=
     multiplied by the weight (D) float32 (None: ones), then turned by the angles of their positions; (q, k), contiguous.
 
     positions (N) or (B, N) int32, int64 or float32 with frequencies (pairs) float32: pair p turns by position frequency_p; several
-    numbers a position, (N, axes) or (B, N, axes) with frequencies (axes, pairs): by the sum over them, formed without loss for far positions.  Pairs are channels (p, p + pairs),
+    numbers a position, (N, axes) or (B, N, axes) with frequencies (axes, pairs): by the sum over them, formed without loss for far positions (to products
+    of 2^78 and whole positions of 2^53; pairs further out are NaN).  Pairs are channels (p, p + pairs),
     with `interleaved` (2 p, 2 p + 1); channels behind 2 pairs are left as they are.  Without positions there is no turn, with norm = False no
     norm.  q, k bfloat16 or float32, of any strides with contiguous channels (views of one projection), up to 128 channels a head."""
     params, qv, kv = _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, interleaved)

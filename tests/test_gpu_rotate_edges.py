@@ -86,3 +86,49 @@ def test_no_eps(B, N, Hq, Hk, D, dtype):
     announce("no eps", B, N, Hq, Hk, D, dtype)
     q, k, wq, wk, dyq, dyk = make(B, N, Hq, Hk, D, dtype, seed=N)
     compare(q, k, wq, wk, torch.arange(N, device="cuda"), speeds(D // 2), dyq, dyk, eps=0.0)
+
+
+TWO_PI = "6.283185307179586476925286766559005768394338798750211641949889184615632812572417997256069650684234135964296173026564613294187689219"
+
+
+@pytest.mark.parametrize("kind,far", [(torch.float32, 2.0 ** 40), (torch.float32, -(2.0 ** 62)), (torch.float32, 2.0 ** 77), (torch.float32, -(2.0 ** 77)),
+                                      (torch.int64, 2 ** 53 - 4), (torch.int64, -(2 ** 53))])
+@pytest.mark.parametrize("axes", [1, 3])
+def test_angles_far_out(axes, kind, far):
+    """To the last product that is served, against angles reduced with 120 digits: the turn's own error is below 2^-25 there, sincos and its argument's
+    rounding leave less than the rest of 4 u (u = 2^-24)."""
+    import math
+    from decimal import Decimal, getcontext
+    getcontext().prec = 120
+    announce("far out", axes, kind, far)
+    f = torch.stack([speeds(8) / 2 ** a for a in range(axes)])
+    steps = torch.arange(3 * axes, device="cuda").view(3, axes)
+    positions = far * (1 + steps.float() * 2.0 ** -5) if kind == torch.float32 else far + steps % 4
+    positions = positions.to(kind)
+    assert positions.double().abs().max() <= (2.0 ** 78 if kind == torch.float32 else 2.0 ** 53)
+    angle = [[float(sum(Decimal(p) * Decimal(w[c]) for p, w in zip(row, f.tolist())) % Decimal(TWO_PI)) for c in range(8)]
+             for row in ([[Decimal(v) for v in row] for row in positions.tolist()])]
+    want_c, want_s = (torch.tensor([[fn(a) for a in row] for row in angle], dtype=torch.float64) for fn in (math.cos, math.sin))
+    one = torch.zeros(1, 3, 1, 16, device="cuda")
+    one[..., :8] = 1
+    q, _ = PF.norm_rotate(one, one, positions=positions, frequencies=f, norm=False)
+    got = q[0, :, 0].double().cpu()
+    assert (got[:, :8] - want_c).abs().max() <= 4 * 2.0 ** -24 and (got[:, 8:] - want_s).abs().max() <= 4 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("kind,far", [(torch.float32, 2.0 ** 79), (torch.float32, -3e38), (torch.float32, float("inf")), (torch.float32, float("nan")),
+                                      (torch.int64, 2 ** 53 + 1), (torch.int64, -(2 ** 63)), (torch.int64, 2 ** 63 - 1)])
+def test_angles_too_far_out(kind, far):
+    """NaN, not a wrong turn, in the pairs that it concerns; other points and channels behind the pairs as ever."""
+    announce("too far out", kind, far)
+    q, k, _, _, _, _ = make(1, 5, 1, 1, 12, torch.float32, seed=1)
+    f = torch.tensor([1.0, 0.5, 0.5, 0.0], device="cuda")
+    positions = torch.tensor([3, 1, 4, 1, 5], device="cuda").to(kind)
+    clean = PF.norm_rotate(q, k, None, None, positions, f)[0]
+    positions[2] = far
+    got = PF.norm_rotate(q, k, None, None, positions, f)[0]
+    keep = [0, 1, 3, 4]
+    assert torch.equal(got[:, keep], clean[:, keep]) and torch.equal(got[..., 8:], clean[..., 8:])
+    touched = got[0, 2, 0, :8].isnan().view(2, 4)
+    all_of_it = kind == torch.int64 or not abs(far) < float("inf")
+    assert touched[:, 0].all() and bool(touched[:, 3].all()) == all_of_it and torch.equal(touched[0], touched[1])
