@@ -20,6 +20,8 @@ namespace pa {
 namespace window {
 
 constexpr float kMost = 1073741824.f, kSlack = 16.f;  // how far weights may sum up, log2 of one may lie above the reference before it is taken again
+// how far from 0 log2 of the reference's own weight may lie: -m c is rounded, at scores of 1e9 to tens and at 1e11 past what a float32 weight holds
+constexpr float kSlip = 64.f;
 
 __device__ __forceinline__ float most_of(const f32x16 &z) {
   float m = z[0];
@@ -92,8 +94,10 @@ __device__ __forceinline__ f32x16 start_of(const Args &a, int q0, int i, int k0,
   return z;
 }
 
+// Waves a SIMD: bf16 rows to 32 run four, which the bound keeps; float32 rows of 64 take up to 14 registers more than two waves leave where they are
+// not held to two.
 template <class T, int DP, bool PLAIN, bool BIAS>
-__global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forward_kernel(Args a) {
+__global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : DP == 64 && sizeof(T) == 4 ? 2 : 1) void forward_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
@@ -167,8 +171,10 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       run.m = high ? most : run.m;
       run.off = run.m == -INFINITY ? 0.f : -run.m * a.c;
     }
-    // A score of a visible infinite key is infinite, which thirds do not give: a sum of weights that is not finite is formed again, too
-    bool again = run.l * 0.f != 0.f, bad = again || not_finite(run.o);
+    // A score of a visible infinite key is infinite, which thirds do not give: a sum of weights that is not finite is formed again, too, and so is one
+    // whose reference weighs far from one
+    const bool slips = run.m != -INFINITY && !(fabsf(fmaf(run.m, a.c, run.off)) <= kSlip);
+    bool again = run.l * 0.f != 0.f || slips, bad = again || not_finite(run.o);
     if (__builtin_expect(some_lane(bad), 0)) {
       again = half_max(again ? 1.f : 0.f) > 0.f;
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
@@ -186,9 +192,10 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : 1) void forwa
       for (int j = a.sinks > 0 ? 0 : low; j <= high && some_lane(again && open); j = j + 1 == a.sinks && low > j ? low : j + 1)
         if (const float z = score(j); span.sees(j)) most = fmaxf(most, z), open = open && z == z;
       if (again) run.l = 0.f, run.m = most, run.off = most == -INFINITY ? 0.f : -most * a.c;
+      const float ref = run.m == -INFINITY ? 0.f : run.m;
       auto weight = [&](int j, bool &seen) {
         seen = span.sees(j);
-        const float w = __builtin_amdgcn_exp2f(fmaf(score(j), a.c, run.off));
+        const float z = score(j), w = __builtin_amdgcn_exp2f(again ? (z - ref) * a.c : fmaf(z, a.c, run.off));
         if (again && seen && g == 0) run.l += w;
         return w;
       };

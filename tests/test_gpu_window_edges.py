@@ -38,3 +38,46 @@ def test_rows_behind_sequences_are_not_read(D, buckets, dtype):
 
     for a, b in zip(all_of_it(0.0), all_of_it(float("nan"))):
         assert torch.isfinite(a[a != float("inf")]).all() and torch.equal(a, b)
+
+
+def one_hot(size, N, D, dtype, falling, twice):
+    """Scores of up to about `size` in steps of its 128th at the scale D^-0.5, formed without rounding: q, k, v and, for a window of everything up to a point
+    (first points of it included), what a softmax of such scores leaves: the value of the largest, or the mean of the two that are largest."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    draw = lambda: torch.randn(1, N, 2, D, generator=gen, device="cuda").to(dtype)
+    q, k, v, dy = torch.zeros_like(draw()), torch.zeros_like(draw()), draw(), draw()
+    step = torch.arange(N, device="cuda") % 64
+    if falling:
+        step = step.flip(0)
+    if twice:
+        step = step // 2 * 2
+    root = 2.0 ** round(torch.tensor(size * D ** 0.5).double().log2().item() / 2)
+    q[..., 0], k[..., 0] = root, (root * (1 + step / 128))[None, :, None].to(dtype)
+    return q, k, v, dy, step
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("twice", [False, True])
+@pytest.mark.parametrize("falling", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e8, 3e9, 3e10, 1e11, 1e20, 2e37])
+def test_scores_of_any_size(size, falling, twice, D, dtype):
+    """Scores that are finite in float32 have their softmax: gaps of a 128th of the size, 780 and more, leave the largest alone.  A value is weighed and
+    divided by its weight: r of itself and 8 u; the mean of two as well."""
+    announce("size", size, falling, twice, D, dtype)
+    N, back = 200, 50
+    q, k, v, _, step = one_hot(size, N, D, dtype, falling, twice)
+    i = torch.arange(N, device="cuda")
+    ok = (i[None] <= i[:, None]) & (i[None] >= i[:, None] - back)
+    best = torch.where(ok, step[None], -1).amax(1, keepdim=True)
+    w = (ok & (step[None] == best)).double()
+    w /= w.sum(1, keepdim=True)
+    V = v[0].double()
+    want, size_of = torch.einsum("ij,jhd->ihd", w, V), torch.einsum("ij,jhd->ihd", w, V.abs())
+    r = torch.finfo(dtype).eps / 2
+    tol = r * want.abs() + 8 * wo.U * size_of
+    y = PF.window_attention(q, k, v, window=(back, 0))
+    if float(q[..., 0].max()) * float(k[..., 0].min()) >= 2.0 ** 128:  # 2e37 at 128 channels: q . k is past float32, every score infinite
+        assert y.isnan().all()
+    else:
+        assert ((y[0].double() - want).abs() <= tol).all()
