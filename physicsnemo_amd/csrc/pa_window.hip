@@ -56,19 +56,41 @@ struct Running {
     l += O::sum(w, z);
     return w;
   }
+};
+
+// The same with the largest score so far for the reference, for the steps, which memory bounds: a weight costs a subtraction more, and is right for scores of
+// any size.
+template <class O, int DP>
+struct Raising {
+  f32x16 o[DP / 32];
+  float m, l, ref;  // reference in units of z, this lane's share of the sum, m or 0 while nothing was seen
+  __device__ __forceinline__ void start(bool live) {
+    zero(o);
+    m = live ? -INFINITY : 0.f, l = 0.f, ref = 0.f;
+  }
   // a larger reference where this tile's largest score asks for it, and all that is summed so far under it
   __device__ __forceinline__ void raise(const f32x16 &z, float c) {
     const float most = half_max(most_of(z));
-    const bool need = m == -INFINITY || !(most * c + off <= kSlack);
+    const bool need = m == -INFINITY || !((most - ref) * c <= kSlack);
     if (!some_lane(need)) return;
-    const float now = need ? fmaxf(m, most) : m, ref = now == -INFINITY ? 0.f : now;
+    const float now = need ? fmaxf(m, most) : m;
+    ref = now == -INFINITY ? 0.f : now;
     const float alpha = __builtin_amdgcn_exp2f((m - ref) * c);
-    m = now, off = -ref * c;
+    m = now;
     l *= alpha;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+  }
+  __device__ __forceinline__ float weight(float z, float c) const { return __builtin_amdgcn_exp2f((z - ref) * c); }
+  // z -> weights
+  __device__ __forceinline__ typename O::Weights weigh(f32x16 &z, float c) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = weight(z[r], c);
+    const typename O::Weights w = O::pack(z);
+    l += O::sum(w, z);
+    return w;
   }
 };
 
@@ -254,7 +276,7 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
   const typename O::Rows own = O::settle(O::template rows<PLAIN>(head_of<T>(a.q, b, hk * s.G + gq), a.q.row, t, s.T, mine, a.D, g));
   const T *const keys = head_of<T>(a.k, b, hk), *const values = head_of<T>(a.v, b, hk);
   const Span span = keys_of(a, mine ? len : 0, me);
-  Running<O, DP> run;
+  Raising<O, DP> run;
   run.start(mine);
   if constexpr (BIAS) {
     for (int u = threadIdx.x; u < a.bias.buckets * s.G; u += 256)
@@ -311,14 +333,14 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
             const int d = me - j;
             z += biases[buckets[d < 0 ? 0 : d < a.bias.distance ? d : a.bias.distance] * s.G + gq];
           }
-          return __builtin_amdgcn_exp2f(fmaf(z, a.c, run.off));
+          return run.weight(z, a.c);
         });
       }
     }
   }
   // the four waves' results under one maximum
   const float l = half_sum(run.l);
-  if (g == 0) most_of_wave[wave][i] = l != 0.f ? -run.off : -INFINITY, sum_of_wave[wave][i] = l;
+  if (g == 0) most_of_wave[wave][i] = l != 0.f ? run.ref : -INFINITY, sum_of_wave[wave][i] = l;
   __syncthreads();  // and all patches have been read
   float top = -INFINITY;
 #pragma unroll
@@ -327,8 +349,8 @@ __global__ __launch_bounds__(256) void step_kernel(StepArgs s) {
   float total = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w)
-    if (sum_of_wave[w][i] != 0.f) total += sum_of_wave[w][i] * __builtin_amdgcn_exp2f(most_of_wave[w][i] - ref);
-  const float scale = l != 0.f ? __builtin_amdgcn_exp2f(-run.off - ref) : 0.f;
+    if (sum_of_wave[w][i] != 0.f) total += sum_of_wave[w][i] * __builtin_amdgcn_exp2f((most_of_wave[w][i] - ref) * a.c);
+  const float scale = l != 0.f ? __builtin_amdgcn_exp2f((run.ref - ref) * a.c) : 0.f;
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -380,7 +402,7 @@ __global__ __launch_bounds__(256) void join_kernel(StepArgs s) {
     float w = 0.f;
     if (first + lane < s.parts) {
       const float2 ml = most_and_sum(first + lane);
-      if (ml.y != 0.f) w = __builtin_amdgcn_exp2f(ml.x - ref), total += ml.y * w;
+      if (ml.y != 0.f) w = __builtin_amdgcn_exp2f((ml.x - ref) * a.c), total += ml.y * w;
     }
     const int count = s.parts - first < 64 ? s.parts - first : 64;
 #pragma unroll 8

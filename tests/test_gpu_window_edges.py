@@ -81,3 +81,31 @@ def test_scores_of_any_size(size, falling, twice, D, dtype):
         assert y.isnan().all()
     else:
         assert ((y[0].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("twice", [False, True])
+@pytest.mark.parametrize("falling", [False, True])
+@pytest.mark.parametrize("size", [1e5, 1e8, 3e9, 3e10, 1e11, 1e20, 2e37])
+def test_steps_over_scores_of_any_size(size, falling, twice, D, dtype):
+    """The same over a cache, in one part and in several, whose references differ."""
+    announce("step of size", size, falling, twice, D, dtype)
+    for N, back in ((200, 50), (3000, None)):
+        q, k, v, _, step = one_hot(size, N, D, dtype, falling, twice)
+        if back is None:  # every part has a largest of its own, all of them another
+            step = torch.arange(N, device="cuda") * 64 // N
+            step = step.flip(0) if falling else step
+            k[..., 0] = (float(q[0, 0, 0, 0]) * (1 + step / 128))[None, :, None].to(dtype)
+        n = torch.tensor([N], dtype=torch.int32, device="cuda")
+        ok = torch.ones(N, dtype=torch.bool, device="cuda") if back is None else torch.arange(N, device="cuda") >= N - 1 - back
+        w = (ok & (step == step[ok].max())).double()
+        w /= w.sum()
+        V = v[0].double()
+        want, size_of = torch.einsum("j,jhd->hd", w, V), torch.einsum("j,jhd->hd", w, V.abs())
+        tol = torch.finfo(dtype).eps / 2 * want.abs() + (16 + int(w.gt(0).sum())) * wo.U * size_of
+        y = PF.window_attention_step(q[:, -1:], k, v, n, left=back)
+        if float(q[..., 0].max()) * float(k[..., 0].min()) >= 2.0 ** 128:
+            assert y.isnan().all()
+        else:
+            assert ((y[0, 0].double() - want).abs() <= tol).all(), N
