@@ -821,7 +821,9 @@ typedef struct pa_window_params {
   const float *bias;         /* (buckets, Hq) */
 } pa_window_params;
 #define PA_NO_BOUND (-1)
-/* stats: (B, Hq, N) float32 for the backward pass, log2 of the softmax's denominators, or NULL. */
+/* stats: (B, Hq, N) float32 for the backward pass, log2 of the softmax's denominators (sums of 2^(score log2 e)), or NULL.  That pass forms the weights
+ * again from them, with relative errors of up to |score| 2^-22; where one is past 2^22 (scores of 2.9e6) it is NaN, and so are the gradients that its
+ * point has a part in. */
 int pa_window_attention(int dtype, const pa_window_params *p, const pa_heads *q, const pa_heads *k, const pa_heads *v, void *y,
                         float *stats, void *stream);
 /* Its gradients from dy, the inputs, y and stats: dq, dk, dv (contiguous, in dtype), d_bias (buckets, Hq) float32 or NULL.  Sums in a fixed order. */

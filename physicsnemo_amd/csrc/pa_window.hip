@@ -22,6 +22,9 @@ namespace window {
 constexpr float kMost = 1073741824.f, kSlack = 16.f;  // how far weights may sum up, log2 of one may lie above the reference before it is taken again
 // how far from 0 log2 of the reference's own weight may lie: -m c is rounded, at scores of 1e9 to tens and at 1e11 past what a float32 weight holds
 constexpr float kSlip = 64.f;
+// what the backward pass takes: past 2^22 the denominator's float32 logarithm, with the reference in it, is off by a quarter and more, and with it
+// all weights of the row
+constexpr float kMostStat = 4194304.f;
 
 __device__ __forceinline__ float most_of(const f32x16 &z) {
   float m = z[0];
@@ -230,7 +233,10 @@ __global__ __launch_bounds__(256, DP == 32 && sizeof(T) == 2 ? 4 : DP == 64 && s
   const bool some = me < len && l != 0.f;
   T *const row = static_cast<T *>(a.y) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
   store_rows<T, DP>(run.o, 1.f / l, some, row, me < a.N, a.D, g);
-  if (a.stats && g == 0 && me < a.N) a.stats[((int64_t)b * a.Hq + h) * a.N + me] = some ? log2f(l) - run.off : INFINITY;
+  if (a.stats && g == 0 && me < a.N) {
+    const float stat = log2f(l) - run.off;
+    a.stats[((int64_t)b * a.Hq + h) * a.N + me] = !some ? INFINITY : fabsf(stat) <= kMostStat ? stat : __builtin_nanf("");
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------

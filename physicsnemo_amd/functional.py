@@ -1584,7 +1584,8 @@ def window_attention(q, k, v, window=(None, None), sinks: int = 0, scale: float 
     has, the rows behind them are not read and zero in the result.  bias (buckets, Hq) float32, added by distance (`relative_buckets`, with a side of their own
     for j > i unless window[1] is 0); a bias of -65536 or less hides its distances as -inf does, one above 65536 counts as that.  A point that sees nothing
     has zeros, and what it does not see has no part in its result, infinities and NaN included.  With `return_stats` the softmax's denominators (log2,
-    (B, Hq, N) float32), which the backward pass reads, come too."""
+    (B, Hq, N) float32), which the backward pass reads, come too; it forms the weights again with relative errors of up to |score| 2^-22, and where scores
+    pass 2.9e6 the denominator and the gradients that the point has a part in are NaN."""
     B, N = q.shape[:2] if q.ndim == 4 else (0, 0)
     params, *views = _window_call(q, k, v, N, window, sinks, scale, lengths, bias, max_distance)
     y = torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -109,3 +109,43 @@ def test_steps_over_scores_of_any_size(size, falling, twice, D, dtype):
             assert y.isnan().all()
         else:
             assert ((y[0, 0].double() - want).abs() <= tol).all(), N
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("buckets", [0, 8])
+def test_gradients_of_scores_past_the_denominators(buckets, D, dtype):
+    """A point whose scores are past what the kept denominator holds: NaN in its gradient and in those of the keys that it sees, not wrong ones; all others
+    as they were."""
+    announce("past the denominators", buckets, D, dtype)
+    N, at = 200, 120
+    q, k, v, dy, bias = make(1, N, 2, 2, D, dtype, buckets, seed=D)
+    k[..., 0] = k[..., 0].abs() + 0.5  # its scores are all of one sign
+    call = dict(window=(30, 10), sinks=2, bias=bias, max_distance=12)
+
+    def all_of_it(q):
+        y, stats = PF.window_attention(q, k, v, return_stats=True, **call)
+        return y, stats, PF.window_attention_backward(dy, q, k, v, y, stats, **call)
+
+    clean, q2 = all_of_it(q), q.clone()
+    i = torch.arange(N, device="cuda")
+    seen = ((i >= at - 30) & (i <= at + 10)) | (i < 2)
+    for size in (1e8, -1e8, 1e12, 1e30):
+        q2[0, at, 1] = 0
+        q2[0, at, 1, 0] = size
+        y, stats, (dq, dk, dv, db) = all_of_it(q2)
+        assert torch.isfinite(y).all() and stats[0, 1, at].isnan() and int(stats.isnan().sum()) == 1
+        assert dq[0, at, 1].isnan().all() and torch.equal(dq[0, i != at], clean[2][0][0, i != at])
+        for got, was in ((dk, clean[2][1]), (dv, clean[2][2])):
+            assert got[0, seen, 1].isnan().all() and torch.equal(got[0, ~seen], was[0, ~seen]) and torch.equal(got[:, :, 0], was[:, :, 0])
+        if buckets:
+            assert torch.equal(db[:, 0], clean[2][3][:, 0]) and db[0, 1].isnan()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("falling", [False, True])
+@pytest.mark.parametrize("size", [1e3, 1e4, 1e5])
+def test_gradients_of_large_scores(size, falling, dtype):
+    announce("gradients of size", size, falling, dtype)
+    q, k, v, dy, _ = one_hot(size, 200, 32, dtype, falling, True)
+    compare(q, k, v, dy, None, window=(50, 0))
