@@ -45,6 +45,13 @@ __device__ __forceinline__ void add_diagonals(const f32x16 &ds, float *buffer, f
 template <class T, int DP>
 constexpr int kWaves = sizeof(T) == 2 || DP == 128 ? 1 : DP == 64 ? 2 : 3;
 
+// Products that start from -delta, or from a denominator, are rounded differently, always to the same side, and sums over long windows keep that: with queries
+// of mean 8 (6 000 points, 4 001 keys, 128 channels) dk and dv of float32 rows were 6.5e-6 off, 2.2e-6 to 2.7e-6 with the differences taken behind the products,
+// where a plain float32 form has 1.7e-6 and 3.3e-6; the far buckets' gradients 1.4e-5, now 1.4e-6 (3 x 5 001 x 8 x 64).  It costs 4 us of the 101 of
+// the key pass at 4 x 7 225 x 8 x 16.  bf16 rows start from them: their p and ds are rounded to 2^-9.
+template <class T>
+constexpr bool kDifferencesAfter = sizeof(T) == 4;
+
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
 __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * WindowOps<T, DP>::kStride;
@@ -58,6 +65,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
   const int lane = threadIdx.x & 63, i = lane & 31, g = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int len = length_of(a, b), q0 = block * 128, qw = q0 + 32 * wave, me = qw + i;
   using O = WindowOps<T, DP>;
+  constexpr bool kAfter = DBIAS || kDifferencesAfter<T>;
   f32x16 dq[DP / 32];
   zero(dq);
   if constexpr (BIAS) fill_bias_table(a, h, table);
@@ -161,11 +169,9 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
       }
     }
     if (g == 0 && me < len) a.delta[at] = delta;
-    // The bias sums take dp as the first pass had it: started from -delta the products are rounded differently, always to the same side, and the
-    // sums of the far buckets are off by 1.4e-5 instead of 1.4e-6 (3 x 5 001 x 8 x 64).
-    pass(DBIAS ? 0.f : -delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
+    pass(kAfter ? 0.f : -delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] *= DBIAS ? dp[r] - delta : dp[r];
+      for (int r = 0; r < 16; ++r) p[r] *= kAfter ? dp[r] - delta : dp[r];
       if constexpr (DBIAS)
         if (!sights.all(k0)) hide(p, keys_of(a, len, me), k0, g, 0.f);  // where delta is NaN
       if constexpr (DBIAS) {
@@ -264,6 +270,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
   }
   const int len = length_of(a, b), k0 = block * 128, kw = k0 + 32 * wave, me = kw + i;
   using O = WindowOps<T, DP>;
+  constexpr bool kAfter = kDifferencesAfter<T>;
   f32x16 dk[DP / 32], dv[DP / 32];
   zero(dk);
   zero(dv);
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
       // as the products start from them: less the denominator in units of z, less delta; rows that are not there weigh nothing.  Here and not in
       // fetch, where it would wait for the loads: 110 -> 99 us at 65 536 x 8 x 32, 257 keys a query.
       if (threadIdx.x < 2 * QT)
-        stats[(n & 1) * 2 * QT + threadIdx.x] = (int)threadIdx.x >= QT ? -stat : from + (int)threadIdx.x < len ? -stat / a.c : -INFINITY;
+        stats[(n & 1) * 2 * QT + threadIdx.x] = (int)threadIdx.x >= QT ? -stat : from + (int)threadIdx.x < len ? (kAfter ? -stat : -stat / a.c) : -INFINITY;
     };
     if (count > 0) fetch(), put(0);
     int filled = -1;
@@ -330,11 +337,17 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
         if (sights.none(q0)) continue;
         const T *const qrows = qt + 32 * s * O::kStride, *const grows = gt + 32 * s * O::kStride;
         f32x16 z, dp;
+        const auto rows_of = [&](const float *p, int q) { return *reinterpret_cast<const f32x4 *>(p + 32 * s + 8 * q + 4 * g); };
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 l4 = *reinterpret_cast<const f32x4 *>(lse + 32 * s + 8 * q + 4 * g), d4 = *reinterpret_cast<const f32x4 *>(delta + 32 * s + 8 * q + 4 * g);
+          if constexpr (kAfter) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) z[4 * q + j] = l4[j], dp[4 * q + j] = d4[j];
+            for (int j = 0; j < 4; ++j) z[4 * q + j] = dp[4 * q + j] = 0.f;
+          } else {
+            const f32x4 l4 = rows_of(lse, q), d4 = rows_of(delta, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[4 * q + j] = l4[j], dp[4 * q + j] = d4[j];
+          }
         }
         if constexpr (BIAS) {
           const Reach reach = reach_of(a.bias, kw - q0 - 31, kw + 31 - q0);
@@ -350,9 +363,17 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
         }
         z = O::scores(qrows, key, i, g, z, a.D);
         dp = O::scores(grows, value, i, g, dp, a.D);
-        if (!sights.all(q0)) hide(z, queries_of(a, len, me), q0, g, -INFINITY);
+        if constexpr (kAfter) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(z[r] * a.c);
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 l4 = rows_of(lse, q), d4 = rows_of(delta, q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[4 * q + j] = fmaf(z[4 * q + j], a.c, l4[j]), dp[4 * q + j] += d4[j];
+          }
+        }
+        if (!sights.all(q0)) hide(z, queries_of(a, len, me), q0, g, -INFINITY);  // behind what may be NaN
+#pragma unroll
+        for (int r = 0; r < 16; ++r) z[r] = __builtin_amdgcn_exp2f(kAfter ? z[r] : z[r] * a.c);
         O::outcome(grows, O::pack(z), lane, dv);
 #pragma unroll
         for (int r = 0; r < 16; ++r) z[r] *= dp[r];
