@@ -345,6 +345,8 @@ struct Ops<bf16, DP> {
         acc[db] = mfma::mma(x.v, w.v[q], acc[db]);
       }
   }
+  // the same good to 2^-8 of the weights and the rows
+  static __device__ __forceinline__ void outcome_coarse(const bf16 *lds, const f32x16 &v, int lane, f32x16 (&acc)[DP / 32]) { outcome(lds, pack(v), lane, acc); }
 };
 
 template <int DP>
@@ -409,6 +411,7 @@ struct Ops<float, DP> {
       for (int r = 0; r < 16; ++r)
         acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(p[(8 * (r >> 2) + (r & 3)) * kStride + 32 * db], w.v[r], acc[db], 0, 0, 0);
   }
+  static __device__ __forceinline__ void outcome_coarse(const float *lds, const f32x16 &v, int lane, f32x16 (&acc)[DP / 32]) { outcome(lds, pack(v), lane, acc); }
 };
 
 // Float32 rows for the bf16 matrix instructions: a value is three bf16 values, each the rounding of what the ones before leave over, which
@@ -545,6 +548,25 @@ struct Split {
           a[k] = x.v;
         }
         acc[db] = products(a, w.v[0][q], w.v[1][q], w.v[2][q], acc[db]);
+      }
+  }
+  // of the first parts alone
+  static __device__ __forceinline__ void outcome_coarse(const float *lds, const f32x16 &v, int lane, f32x16 (&acc)[DP / 32]) {
+    const int l = lane & 15, h = (lane >> 4) & 1, g = lane >> 5;
+    const uint16_t *const p = reinterpret_cast<const uint16_t *>(lds + (4 * g + (l >> 2)) * kStride) + 16 * h + 4 * (l & 3);
+    const u32x4 w[2] = {mfma::pack_half<0>(v), mfma::pack_half<1>(v)};
+    typedef __attribute__((address_space(3))) s16x4 lds_piece;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        union {
+          s16x4 h[2];
+          u32x4 v;
+        } x;
+        x.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_piece *)(p + (16 * q) * 2 * kStride + 32 * db));
+        x.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_piece *)(p + (16 * q + 8) * 2 * kStride + 32 * db));
+        acc[db] = mfma::mma(x.v, w[q], acc[db]);
       }
   }
 };

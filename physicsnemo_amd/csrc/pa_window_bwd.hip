@@ -9,8 +9,13 @@
 // vector instructions and registers, three waves a SIMD, bound both); 4 x 7 225 x 8 x 16 float32, 171 keys: 78 and 101; with the bias gradient, 3 x 5 001 x 8
 // over 4 x 64, 512 keys: 119 (four products a tile, not three) and 91 to 96.
 //
-// delta from y carries the roundings of the weights and of y (2^-9 of |dy| |v| for bf16), which is what dq, dk and dv of that type are
-// rounded to.  The bias gradient is float32, and its sums cancel: where it is wanted, the first kernel sums p dp before it goes over the keys again.
+// delta from y carries y's rounding (2^-9 of |dy| |v| for bf16), and with a delta that is off by e a query's score gradients sum up to e, not to zero: dq is
+// off by e times the mean of its keys, which may be many times what is left of dq where the keys and values have means of their own.  So the sum of
+// ds, as it is multiplied, and the mean key sum_j p_ij k_j are summed along; what the one leaves of the other is taken off dq, and the sum before its rounding is
+// added to delta for the second kernel.  Keys and values of mean 8 (6 000 points, 4 001 keys of 32 channels): dq in bf16 3.7 off, now 0.0024, dk 0.0145, now 0.0023; in float32 1.2e-3, now
+// 4.5e-6, a plain form 1.4e-4.  It costs a product in seven (65 536 x 8 x 32: queries 82 -> 96 us; float32
+// 4 x 7 225 x 8 x 16: 78 -> 90).
+// The bias gradient is float32, and sums single ds: where it is wanted, the first kernel sums p dp before it goes over the keys again.
 #include "pa_window.h"
 
 namespace pa {
@@ -39,11 +44,14 @@ __device__ __forceinline__ void add_diagonals(const f32x16 &ds, float *buffer, f
   }
 }
 
-// Waves a SIMD: the thirds of float32 rows need 184 registers at widths to 32 (one more wave for 20 spilled ones: 4 x 7 225 x 8 x 16, queries 90 -> 78 us,
-// keys 109 -> 101) and 271 at 64 (a second wave: 20 000 x 4 x 64, 401 keys, queries 172 -> 131, keys 200 -> 175).  bf16 rows to 32 run three by
-// themselves; four spill (65 536 x 8 x 32: queries 82 -> 81, keys 99 -> 106).
+// Waves a SIMD.  queries_kernel: bf16 rows to 32 run three by themselves (of odd pieces for ten spilled registers), to 64 two; the thirds of float32 rows take
+// 200 registers at widths to 32 (a third wave for 35 spilled ones) and 320 at 64 (a second wave).  keys_kernel: bf16 rows to 32 run four by themselves
+// without biases and three with them; float32 rows need 184 at widths to 32 and 271 at 64 (4 x 7 225 x 8 x 16: a third wave takes 109 to 101 us;
+// 20 000 x 4 x 64, 401 keys: a second one 200 to 175).  Rows of 128 run one: 350 to 450 registers.
+template <int DP>
+constexpr int kWavesOfQueries = DP == 128 ? 1 : DP == 64 ? 2 : 3;
 template <class T, int DP>
-constexpr int kWaves = sizeof(T) == 2 || DP == 128 ? 1 : DP == 64 ? 2 : 3;
+constexpr int kWavesOfKeys = sizeof(T) == 2 || DP == 128 ? 1 : DP == 64 ? 2 : 3;
 
 // Products that start from -delta, or from a denominator, are rounded differently, always to the same side, and sums over long windows keep that: with queries
 // of mean 8 (6 000 points, 4 001 keys, 128 channels) dk and dv of float32 rows were 6.5e-6 off, 2.2e-6 to 2.7e-6 with the differences taken behind the products,
@@ -53,7 +61,7 @@ template <class T>
 constexpr bool kDifferencesAfter = sizeof(T) == 4;
 
 template <class T, int DP, bool PLAIN, bool BIAS, bool DBIAS>
-__global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
+__global__ __launch_bounds__(256, kWavesOfQueries<DP>) void queries_kernel(Args a) {
   constexpr int KT = tile_rows<T, DP>(), SUB = KT / 32, TILE = KT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][keys, values][KT][stride]
@@ -168,8 +176,11 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
         stat += log2f(total);
       }
     }
-    if (g == 0 && me < len) a.delta[at] = delta;
+    float exact = 0.f, rest = 0.f;  // the sum of ds, for delta; the sum of ds as it is multiplied; `mean`: sum p k, good to 2^-8, which is enough beside a rest that is small itself
+    f32x16 mean[DP / 32];
+    zero(mean);
     pass(kAfter ? 0.f : -delta, [&](const T *krows, f32x16 &p, f32x16 &dp, int k0, Reach reach) {
+      O::outcome_coarse(krows, p, lane, mean);
 #pragma unroll
       for (int r = 0; r < 16; ++r) p[r] *= kAfter ? dp[r] - delta : dp[r];
       if constexpr (DBIAS)
@@ -185,9 +196,14 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
           else ahead += sum;
         }
       }
-      O::outcome(krows, O::pack(p), lane, dq);
+      const typename O::Weights ds = O::pack(p);
+      rest += O::sum(ds, p);
+      if constexpr (sizeof(T) == 2) exact += sum_of(p);
+      O::outcome(krows, ds, lane, dq);
     });
-    bool bad = not_finite(dq);
+    rest = half_sum(rest);
+    exact = sizeof(T) == 2 ? half_sum(exact) : rest;
+    bool bad = not_finite(dq) || not_finite(mean) || rest * 0.f != 0.f;
     if (__builtin_expect(some_lane(bad), 0)) {
       bad = half_max(bad ? 1.f : 0.f) > 0.f;
       const Span span = keys_of(a, len, me);
@@ -201,9 +217,21 @@ __global__ __launch_bounds__(256, (kWaves<T, DP>)) void queries_kernel(Args a) {
         return __builtin_amdgcn_exp2f(fmaf(z, a.c, -stat)) * (by - delta);
       };
       const int low = qw - a.left > 0 ? qw - a.left : 0, high = qw + 31 + a.right < len - 1 ? qw + 31 + a.right : len - 1;
+      float own_rest = 0.f;  // delta from what is seen alone
+      for (int j = a.sinks > 0 ? 0 : low; j <= high && some_lane(bad && own_rest == own_rest); j = j + 1 == a.sinks && low > j ? low : j + 1) {
+        bool seen;
+        const float w = weight(j, seen);
+        own_rest += seen ? w : 0.f;
+      }
+      if (bad) delta += own_rest, exact = 0.f;
       add_rows<T, DP>(keys, a.k.row, 0, (a.sinks < low ? a.sinks : low) - 1, a.D, g, bad, dq, weight);
       add_rows<T, DP>(keys, a.k.row, low, high, a.D, g, bad, dq, weight);
     }
+    if (g == 0 && me < len) a.delta[at] = stat == stat ? delta + exact : 0.f;  // 0: the weights are NaN, and where there are none no NaN of delta's meets them
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dq[d][r] = bad ? dq[d][r] : fmaf(-rest, mean[d][r], dq[d][r]);
   }
   T *const row = static_cast<T *>(a.dq) + (((int64_t)b * a.N + me) * a.Hq + h) * a.D;
   store_rows<T, DP>(dq, a.scale, me < len, row, me < a.N, a.D, g);
@@ -253,7 +281,7 @@ __global__ __launch_bounds__(256) void bias_sums_kernel(const float *parts, int6
 // for those tiles alone, whose sums are joined by sink_sums_kernel.
 // ---------------------------------------------------------------------------------------------------------------
 template <class T, int DP, bool PLAIN, bool BIAS>
-__global__ __launch_bounds__(256, (kWaves<T, DP>)) void keys_kernel(Args a) {
+__global__ __launch_bounds__(256, (kWavesOfKeys<T, DP>)) void keys_kernel(Args a) {
   constexpr int QT = tile_rows<T, DP>(), SUB = QT / 32, TILE = QT * WindowOps<T, DP>::kStride;
   extern __shared__ u32x4 lds_raw[];
   T *const tiles = reinterpret_cast<T *>(lds_raw);  // [buffer][queries, gradients][QT][stride]

@@ -58,3 +58,15 @@ def test_sums_that_a_start_would_bias(means, D):
         print(f"{name} {own:.2e} {plain:.2e}", flush=True)
         if name in ("dk", "dv"):
             assert own <= 2 * plain + 16 * U, (name, own, plain)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [16, 32, 40, 64, 128])
+@pytest.mark.parametrize("means", MEANS)
+def test_means_far_from_zero(means, D, dtype, bias):
+    """delta from a rounded result, and score gradients that are rounded before they meet the keys, leave multiples of the means behind."""
+    announce("means", means, D, dtype, bias)
+    for name, (own, plain) in errors(means, D, dtype, bias).items():
+        print(f"{name} {own:.2e} {plain:.2e}", flush=True)
+        assert own <= 2 * plain + (16 * U if dtype == F32 else 2.0 ** -8), (name, own, plain)
