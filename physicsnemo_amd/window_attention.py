@@ -184,6 +184,9 @@ class WindowAttention(nn.Module):
 
     def forward_block(self, x: torch.Tensor, residual: torch.Tensor, ln: nn.LayerNorm | None):
         """self(x) + residual and, with `ln`, its LayerNorm, for a block that is served."""
+        if x.is_cuda and self._in_float32(x):
+            with torch.autocast("cuda", enabled=False):  # the sum as well, as in the other layers
+                return self.forward_block(x.float(), residual.float(), ln)
         y = self.forward(x).to(residual.dtype).contiguous()
         if ln is None:
             return PF.residual_layernorm(y, residual=residual.contiguous())

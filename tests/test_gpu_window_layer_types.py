@@ -1,0 +1,51 @@
+"""The window attention layer in float16, which it computes as float32, and what a served block does around it."""
+import pytest
+import torch
+
+import physicsnemo_amd as pn
+from gpu_util import announce
+
+pytestmark = pytest.mark.gpu
+HALF = 2.0 ** -11
+
+
+def model(blocks, **options):
+    torch.manual_seed(3)
+    return pn.Transolver(functional_dim=3, out_dim=2, embedding_dim=2, n_layers=3, n_hidden=64, n_head=4, slice_num=16, use_te=False, dropout=0.0,
+                         window_blocks=blocks, window_options=dict(window=(30, 30), sinks=2, bias_buckets=8, max_distance=20), **options).cuda()
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+@pytest.mark.parametrize("blocks", [(0,), (0, 1, 2), (1,), (2,)])
+def test_model_under_float16_autocast(blocks):
+    """Served, also where the first block attends over a window, and as it is trained.  Against float32: every Linear of the way (preprocess 2, six in the
+    blocks' MLPs, head) rounds its inputs and its result by 2^-11, nine of them, each once more for what comes from the one before."""
+    announce("float16 autocast", blocks)
+    net = model(blocks)
+    fx, emb = (torch.randn(2, 300, n, device="cuda") for n in (3, 2))
+    with torch.no_grad():
+        want = net.eval()(fx, emb)
+        with torch.autocast("cuda", torch.float16):
+            served = net(fx, emb)
+    with torch.autocast("cuda", torch.float16):
+        trained = net.train()(fx, emb)
+    assert rel(served, want) < 18 * HALF and rel(trained.detach(), want) < 18 * HALF
+    trained.float().square().mean().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in net.blocks.parameters())
+
+
+def test_the_sum_with_the_residual_is_not_rounded():
+    """float16 autocast: a float32 residual meets the layer's float32 result."""
+    announce("residual")
+    block = model((0,)).blocks[0].eval()
+    x, residual = (torch.randn(2, 100, 64, device="cuda") for _ in range(2))
+    with torch.no_grad():
+        want = block.Attn.forward_block(x, residual, block.ln_mlp1[0])
+        with torch.autocast("cuda", torch.float16):
+            got = block.Attn.forward_block(x, residual, block.ln_mlp1[0])
+            of_half = block.Attn.forward_block(x, residual.half(), block.ln_mlp1[0])
+    assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(got, want))
+    assert all(a.dtype == torch.float32 and rel(a, b) < 2 * HALF for a, b in zip(of_half, want))
