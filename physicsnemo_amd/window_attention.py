@@ -187,7 +187,7 @@ class WindowAttention(nn.Module):
         if x.is_cuda and self._in_float32(x):
             with torch.autocast("cuda", enabled=False):  # the sum as well, as in the other layers
                 return self.forward_block(x.float(), residual.float(), ln)
-        y = self.forward(x).to(residual.dtype).contiguous()
+        y = self(x).to(residual.dtype).contiguous()
         if ln is None:
             return PF.residual_layernorm(y, residual=residual.contiguous())
         return PF.residual_layernorm(y, residual=residual.contiguous(), ln_weight=ln.weight.detach().float().contiguous(),

@@ -49,3 +49,25 @@ def test_the_sum_with_the_residual_is_not_rounded():
             of_half = block.Attn.forward_block(x, residual.half(), block.ln_mlp1[0])
     assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(got, want))
     assert all(a.dtype == torch.float32 and rel(a, b) < 2 * HALF for a, b in zip(of_half, want))
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_hooks_of_the_layer(half):
+    """They observe and change the layer's result in a served block as in a trained one."""
+    announce("hooks", half)
+    block = pn.TransolverBlock(4, 64, 0.0, use_te=False, window=dict(window=(12, 12))).cuda()
+    fx, seen = torch.randn(2, 120, 64, device="cuda"), []
+    def run():
+        with torch.autocast("cuda", torch.float16, enabled=half):
+            return block(fx)
+    with torch.no_grad():
+        plain = block.eval() and run()
+        first = block.Attn.register_forward_hook(lambda m, i, o: seen.append(o.shape))
+        assert torch.equal(run(), plain) and len(seen) == 1
+        first.remove()
+        block.Attn.register_forward_hook(lambda m, i, o: o * 0)
+        block.Attn.register_forward_pre_hook(lambda m, i: seen.append(i[0].shape))
+        served = run()
+    trained = block.train()(fx) if not half else run()
+    without = fx + block.ln_mlp1[1](block.ln_mlp1[0](fx))
+    assert len(seen) == 3 and rel(served, without) < (18 * HALF if half else 1e-5) and rel(trained.detach(), without.detach()) < (18 * HALF if half else 1e-5)
