@@ -118,6 +118,10 @@ class WindowAttention(nn.Module):
         return torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
 
     def _projected(self, lin: nn.Linear, x: torch.Tensor, needs_grad: bool) -> torch.Tensor:
+        if (x.dtype == torch.float32 and type(lin) is nn.Linear and lin.weight.dtype == torch.float16 and PA.unhooked(lin) and
+                not torch.is_autocast_enabled("cuda")):  # weights of a float16 layer, which is computed in float32
+            if needs_grad or lin.in_features > 512:
+                return nn.functional.linear(x, lin.weight.float(), lin.bias.float())
         if needs_grad:
             return PA.linear_as_autocast(x, lin)
         if x.dtype in (torch.float32, torch.bfloat16) and type(lin) is nn.Linear and lin.in_features <= 512 and PA.unhooked(lin):

@@ -71,3 +71,37 @@ def test_hooks_of_the_layer(half):
     trained = block.train()(fx) if not half else run()
     without = fx + block.ln_mlp1[1](block.ln_mlp1[0](fx))
     assert len(seen) == 3 and rel(served, without) < (18 * HALF if half else 1e-5) and rel(trained.detach(), without.detach()) < (18 * HALF if half else 1e-5)
+
+
+@pytest.mark.parametrize("dim,heads,dim_head", [(48, 4, 16), (640, 4, 160 // 2), (64, 9, 64)])
+@pytest.mark.parametrize("autocast", [False, True])
+def test_layers_in_float16(autocast, dim, heads, dim_head):
+    """Cast as a whole and given float16, or under autocast: float32 inside, results and gradients rounded once, by 2^-11 at most.  Layers of more
+    inputs than the row kernels hold, too.  Float32 sums of up to 640 terms: 2 x 640 u on either side's results, which the bound leaves room for."""
+    announce("float16", autocast, dim, heads, dim_head)
+    torch.manual_seed(5)
+    layer = pn.WindowAttention(dim, heads=heads, dim_head=dim_head, window=(20, 9), sinks=1, bias_buckets=8, max_distance=20).cuda()
+    torch.nn.init.normal_(layer.bias)
+    with torch.no_grad():
+        for p in layer.parameters():
+            p.copy_(p.half().float())
+    x, dy = (torch.randn(2, 90, dim, device="cuda").half() for _ in range(2))
+    lengths = torch.tensor([90, 41], dtype=torch.int32, device="cuda")
+
+    def run(layer, x, **kw):
+        with torch.no_grad():
+            served = layer(x, **kw)
+        x = x.detach().requires_grad_(True)
+        out = layer(x, **kw)
+        grads = torch.autograd.grad(out, [x, *layer.parameters()], dy.to(out.dtype))
+        return served, out.detach(), grads
+    want = run(layer, x.float(), lengths=lengths)
+    if autocast:
+        with torch.autocast("cuda", torch.float16):
+            got = run(layer, x.float(), lengths=lengths)
+    else:
+        got = run(layer.half(), x, lengths=lengths)
+    assert got[0].dtype == got[1].dtype == torch.float16
+    assert rel(got[0], want[0]) < 1.5 * HALF and rel(got[1], want[1]) < 1.5 * HALF
+    for (name, _), a, b in zip([("x", None), *layer.named_parameters()], got[2], want[2]):
+        assert a.dtype == (torch.float32 if autocast else torch.float16) and rel(a, b) < 1.5 * HALF, (name, rel(a, b))
