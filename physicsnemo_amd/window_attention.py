@@ -198,9 +198,10 @@ class WindowAttention(nn.Module):
                                      ln_bias=ln.bias.detach().float().contiguous(), ln_eps=ln.eps)
 
     def cache(self, batch: int, capacity: int, dtype: torch.dtype | None = None) -> WindowCache:
-        """An empty cache for `step`, in the type that the layer's inputs will have."""
+        """An empty cache for `step`, in the type that the layer's inputs will have, by default its weights' (float32 for float16)."""
         weight = self.in_project_qkv.weight
-        return WindowCache(batch, capacity, self.kv_heads, self.dim_head, dtype or weight.dtype, weight.device)
+        dtype = dtype or weight.dtype
+        return WindowCache(batch, capacity, self.kv_heads, self.dim_head, torch.float32 if dtype == torch.float16 else dtype, weight.device)
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, cache: WindowCache, positions: torch.Tensor | None = None) -> torch.Tensor:
@@ -208,7 +209,12 @@ class WindowAttention(nn.Module):
         all points so far.  For layers that look back only (window[1] = 0); positions as for `forward`, by default the places behind the cache."""
         if self.window[1] != 0:
             raise ValueError("step is for a layer whose window has no reach ahead")
+        if x.is_cuda and self._in_float32(x):
+            with torch.autocast("cuda", enabled=False):
+                return self.step(x.float(), cache, positions).to(torch.float16)
         x = self._prepared(x)
+        if x.numel() == 0:
+            return x.new_zeros(*x.shape[:-1], self.out_linear.out_features)
         if self.frequencies is not None and positions is None and self.axes == 1:
             positions = cache.lengths[:, None].long() + torch.arange(x.shape[1], device=x.device)
         q, k, v = self._qkv(x, self._positions(x, positions), False)

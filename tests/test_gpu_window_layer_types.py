@@ -105,3 +105,32 @@ def test_layers_in_float16(autocast, dim, heads, dim_head):
     assert rel(got[0], want[0]) < 1.5 * HALF and rel(got[1], want[1]) < 1.5 * HALF
     for (name, _), a, b in zip([("x", None), *layer.named_parameters()], got[2], want[2]):
         assert a.dtype == (torch.float32 if autocast else torch.float16) and rel(a, b) < 1.5 * HALF, (name, rel(a, b))
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_steps_in_float16(autocast):
+    """A cache of float32, the rows of the whole layer, rounded once (float32 sums in another order: 2^-18 beside 2^-11)."""
+    announce("float16 steps", autocast)
+    torch.manual_seed(6)
+    layer = pn.WindowAttention(64, heads=4, dim_head=32, window=(24, 0), sinks=2, kv_heads=2, bias_buckets=8, max_distance=20).cuda()
+    torch.nn.init.normal_(layer.bias)
+    layer = layer if autocast else layer.half()
+    x = torch.randn(3, 40, 64, device="cuda")
+    x = x if autocast else x.half()
+    with torch.no_grad(), torch.autocast("cuda", torch.float16, enabled=autocast):
+        whole, cache = layer(x), layer.cache(3, 40)
+        rows = [layer.step(x[:, a:b], cache) for a, b in ((0, 17), (17, 18), (18, 18), (18, 19), (19, 40))]
+    assert cache.k.dtype == torch.float32 and cache.lengths.tolist() == [40] * 3 and cache.used == 40
+    assert all(r.dtype == torch.float16 for r in rows) and rel(torch.cat(rows, 1), whole) < HALF + 2.0 ** -18
+    assert layer.cache(1, 1, torch.float16).k.dtype == torch.float32 and layer.cache(1, 1, torch.bfloat16).k.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, torch.bfloat16])
+def test_steps_of_nothing(dtype):
+    """No sequences or no new points: empty results, a cache as it was."""
+    announce("nothing", dtype)
+    layer = pn.WindowAttention(64, heads=4, dim_head=32, window=(24, 0)).cuda().to(dtype)
+    for batch, points in ((0, 3), (2, 0), (0, 0)):
+        cache = layer.cache(batch, 5)
+        y = layer.step(torch.zeros(batch, points, 64, device="cuda", dtype=dtype), cache)
+        assert y.shape == (batch, points, 64) and y.dtype == dtype and cache.used == 0 and not cache.lengths.any()
