@@ -140,6 +140,8 @@ class TransolverBlock(nn.Module):
                       use_te=use_te, plus=plus)
         if window is not None:
             self.Attn = WindowAttention(hidden_dim, heads=num_heads, dim_head=hidden_dim // num_heads, dropout=dropout, **window)
+            if self.Attn.rotary_base is not None and self.Attn.axes != 1:
+                raise ValueError(f"a block turns by the places of its points in their order, one number each: axes has to be 1, got {self.Attn.axes}")
         elif spatial_shape is None:
             self.Attn = PhysicsAttentionIrregularMesh(hidden_dim, **common)
         elif len(spatial_shape) == 2:
