@@ -1410,7 +1410,7 @@ def gated_mlp_int8(x, w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, 
 # ---------------------------------------------------------------------------------------------------------------------
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-_SEQ_LIMITS = dict(D=128, sinks=128, buckets=256, distance=2048)
+_SEQ_LIMITS = dict(D=128, sinks=128, buckets=256, distance=2048, axes=8)
 
 
 def _heads_of(t, what: str, device, dtype, shape):
@@ -1457,7 +1457,7 @@ def _rotate_call(q, k, q_weight, k_weight, positions, frequencies, eps, norm, in
         if frequencies.ndim not in (1, 2) or frequencies.dtype != torch.float32:
             raise ValueError(f"frequencies have to be float32 (pairs) or (axes, pairs), got {frequencies.dtype} of shape {tuple(frequencies.shape)}")
         axes, rotated = (1 if frequencies.ndim == 1 else frequencies.shape[0]), 2 * frequencies.shape[-1]
-        if not 1 <= axes <= 8 or rotated > D:
+        if not 1 <= axes <= _SEQ_LIMITS["axes"] or rotated > D:
             raise ValueError(f"one to eight axes and at most half as many pairs as channels, got {axes} and {rotated // 2} for {D} channels")
         if positions.dtype not in _POSITION_TYPES:
             raise ValueError(f"positions have to be int32, int64 or float32, got {positions.dtype}")

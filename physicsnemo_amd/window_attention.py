@@ -77,6 +77,13 @@ class WindowAttention(nn.Module):
             raise ValueError(f"window has to be (back, ahead), got {window!r}")
         for reach, what in zip(self.window, ("reach back", "reach ahead")):
             PF._bound(reach, f"the window's {what}")
+        limits = PF._SEQ_LIMITS
+        if not 1 <= dim_head <= limits["D"]:
+            raise ValueError(f"heads of 1 to {limits['D']} channels are served, got {dim_head}")
+        if PF._bound(sinks, "the number of first points") not in range(limits["sinks"] + 1):
+            raise ValueError(f"0 to {limits['sinks']} first points can stay visible, got {sinks}")
+        if rotary_base is not None and (rotary_base <= 0 or axes not in range(1, limits["axes"] + 1)):
+            raise ValueError(f"a rotation has a positive base and one to {limits['axes']} axes, got {rotary_base} and {axes}")
         self.heads, self.kv_heads, self.dim_head, self.sinks, self.axes, self.max_distance = heads, kv_heads, dim_head, sinks, axes, max_distance
         if bias_buckets:
             PF.relative_buckets((), bias_buckets, max_distance, both=self.window[1] != 0)
