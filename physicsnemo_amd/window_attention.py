@@ -42,7 +42,10 @@ class WindowCache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v (B, T, heads, dim_head) behind what each sequence holds."""
-        T = k.shape[1]
+        batch, _, heads, channels = self.k.shape
+        T = k.shape[1] if k.ndim == 4 else 0
+        if k.shape != v.shape or k.shape != (batch, T, heads, channels):
+            raise ValueError(f"keys and values have to be {(batch, 'T', heads, channels)}, got {tuple(k.shape)} and {tuple(v.shape)}")
         if self.used + T > self.capacity:
             raise ValueError(f"the cache holds {self.used} of {self.capacity} points: no room for {T} more")
         rows = self.lengths[:, None].long() + torch.arange(T, device=k.device)

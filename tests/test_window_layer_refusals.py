@@ -31,3 +31,17 @@ def test_layers_at_the_limits():
     for options in (dict(sinks=128), dict(sinks=0), dict(dim_head=128), dict(dim_head=1, rotary_base=None), dict(dim_head=16, axes=8), dict(axes=0, rotary_base=None)):
         layer = pn.WindowAttention(32, **{"heads": 4, "dim_head": 8, **options})
         assert layer.frequencies is None or torch.isfinite(layer.frequencies).all()
+
+
+def test_rows_that_do_not_go_into_a_cache():
+    """Refused, and the cache is as it was: rows of one sequence went into the first for all of them."""
+    cache = pn.WindowCache(2, 5, 3, 4, torch.float32, "cpu")
+    cache.append(torch.ones(2, 1, 3, 4), torch.ones(2, 1, 3, 4))
+    good = torch.full((2, 2, 3, 4), 7.0)
+    for bad in (good[:1], good[:, :, :1], good[..., :2], good[0], torch.zeros(3, 2, 3, 4)):
+        for k, v in ((bad, bad), (good, bad), (bad, good)):
+            with pytest.raises(ValueError, match="keys and values"):
+                cache.append(k, v)
+    assert cache.used == 1 and cache.lengths.tolist() == [1, 1] and not cache.k[:, 1:].any() and not cache.v[:, 1:].any()
+    cache.append(good, good)
+    assert cache.lengths.tolist() == [3, 3] and bool(cache.k[:, 1:3].eq(7).all())
