@@ -1410,6 +1410,7 @@ def gated_mlp_int8(x, w_gate, s_gate, b_gate, w_up, s_up, b_up, w_down, s_down, 
 # ---------------------------------------------------------------------------------------------------------------------
 
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+MAX_STEP_BIASES = 16384  # that a step holds on chip: buckets x query heads of a key head
 _SEQ_LIMITS = dict(D=128, sinks=128, buckets=256, distance=2048, axes=8)
 
 
@@ -1630,11 +1631,14 @@ def window_attention_step(q, k, v, lengths, left: int | None = None, sinks: int 
                           max_distance: int = 128):
     """`window_attention` with window (left, 0) for the newest points alone: q (B, T, Hq, D) of the last T points of each sequence, k and v
     (B, capacity, Hk, D) of all its points so far, these included; lengths (B) int32 on the device says how many they are.  Query t is point
-    lengths - T + t (zeros where that is before the first).  Reads what the window leaves visible and nothing else.  For inference: it has no gradient."""
+    lengths - T + t (zeros where that is before the first).  Reads what the window leaves visible and nothing else.  At most MAX_STEP_BIASES biases, buckets
+    times the query heads of a key head.  For inference: it has no gradient."""
     if q.ndim != 4 or k.ndim != 4 or lengths is None:
         raise ValueError("q has to be (B, T, heads, D), k and v (B, capacity, heads, D), and lengths is needed")
     params, *views = _window_call(q, k, v, k.shape[1], (left, 0), sinks, scale, lengths, bias, max_distance)
     T = q.shape[1]
+    if bias is not None and bias.numel() // k.shape[2] > MAX_STEP_BIASES:
+        raise ValueError(f"at most {MAX_STEP_BIASES} biases a key head, got {tuple(bias.shape)} over {k.shape[2]}")
     if T > k.shape[1]:
         raise ValueError(f"{T} new points do not fit a capacity of {k.shape[1]}")
     y = torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -219,6 +219,9 @@ class WindowAttention(nn.Module):
         all points so far.  For layers that look back only (window[1] = 0); positions as for `forward`, by default the places behind the cache."""
         if self.window[1] != 0:
             raise ValueError("step is for a layer whose window has no reach ahead")
+        shared = self.heads // self.kv_heads
+        if self.bias is not None and self.bias.shape[0] * shared > PF.MAX_STEP_BIASES:  # before the cache changes
+            raise ValueError(f"step takes {PF.MAX_STEP_BIASES} biases a key head, got {self.bias.shape[0]} of {shared} query heads")
         if x.is_cuda and self._in_float32(x):
             with torch.autocast("cuda", enabled=False):
                 return self.step(x.float(), cache, positions).to(torch.float16)

@@ -45,3 +45,11 @@ def test_rows_that_do_not_go_into_a_cache():
     assert cache.used == 1 and cache.lengths.tolist() == [1, 1] and not cache.k[:, 1:].any() and not cache.v[:, 1:].any()
     cache.append(good, good)
     assert cache.lengths.tolist() == [3, 3] and bool(cache.k[:, 1:3].eq(7).all())
+
+
+def test_steps_that_are_refused_leave_the_cache():
+    layer = pn.WindowAttention(32, heads=128, dim_head=2, kv_heads=1, window=(9, 0), rotary_base=None, qk_norm=False, bias_buckets=256, max_distance=2048)
+    cache = layer.cache(1, 4)
+    with pytest.raises(ValueError, match="biases"):
+        layer.step(torch.zeros(1, 1, 32), cache)
+    assert cache.used == 0 and not cache.lengths.any()
