@@ -149,3 +149,38 @@ def test_gradients_of_large_scores(size, falling, dtype):
     announce("gradients of size", size, falling, dtype)
     q, k, v, dy, _ = one_hot(size, 200, 32, dtype, falling, True)
     compare(q, k, v, dy, None, window=(50, 0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("buckets", [0, 12])
+@pytest.mark.parametrize("D", [24, 64, 128])
+@pytest.mark.parametrize("scale", [0.03, 1.0, 3.0])
+def test_scales(scale, D, buckets, dtype):
+    """The caller's scale, in values, all gradients, and steps."""
+    announce("scale", scale, D, buckets, dtype)
+    q, k, v, dy, bias = make(2, 210, 4, 2, D, dtype, buckets, seed=D)
+    call = dict(sinks=3, scale=scale, max_distance=30)
+    q = q * min(1.0, D ** -0.5 / scale * 2)  # scores of a softmax that is not one-hot
+    lengths = torch.tensor([210, 133], dtype=torch.int32, device="cuda")
+    for right in (0, 25):
+        compare(q, k, v, dy, bias, window=(60, right), lengths=lengths, **call)
+    want = wo.attention(q[:, -7:], k, v, window=(60, 0), lengths=lengths, bias=bias, first=lengths.long() - 7, **call)["y"]
+    wo.check(PF.window_attention_step(q[:, -7:], k, v, lengths, left=60, bias=bias, **call), want, "step")
+    other = PF.window_attention(q, k, v, window=(60, 0), bias=bias, **{**call, "scale": 2 * scale})
+    assert not torch.equal(other, PF.window_attention(q, k, v, window=(60, 0), bias=bias, **call))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [1e-29, 1e-12, 1e12, 1e29])
+def test_scales_at_their_limits(scale, dtype):
+    """Inputs that make up for it: the results of ordinary ones, exactly so for scales and inputs that differ by powers of two."""
+    announce("far scale", scale, dtype)
+    q, k, v, dy, _ = make(1, 150, 2, 1, 32, dtype, 0, seed=3)
+    power = 2.0 ** round(torch.tensor(scale).double().log2().item())
+    call = dict(window=(40, 20), sinks=2)
+    def all_of_it(q, scale):
+        y, stats = PF.window_attention(q, k, v, scale=scale, return_stats=True, **call)
+        return y, *PF.window_attention_backward(dy, q, k, v, y, stats, scale=scale, **call)[:3]
+    want, got = all_of_it(q, 0.25), all_of_it(q / power, 0.25 * power)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+    wo.check(got[1].double() / power, (want[1].double(), torch.finfo(dtype).eps * want[1].double().abs()), "dq")
