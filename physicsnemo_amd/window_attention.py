@@ -201,6 +201,10 @@ class WindowAttention(nn.Module):
         if x.is_cuda and self._in_float32(x):
             with torch.autocast("cuda", enabled=False):  # the sum as well, as in the other layers
                 return self.forward_block(x.float(), residual.float(), ln)
+        if x.numel() == 0:
+            y = self(x)
+            y = y + residual.to(y.dtype)
+            return y if ln is None else (y, y.clone())
         y = self(x).to(residual.dtype).contiguous()
         if ln is None:
             return PF.residual_layernorm(y, residual=residual.contiguous())

@@ -134,3 +134,20 @@ def test_steps_of_nothing(dtype):
         cache = layer.cache(batch, 5)
         y = layer.step(torch.zeros(batch, points, 64, device="cuda", dtype=dtype), cache)
         assert y.shape == (batch, points, 64) and y.dtype == dtype and cache.used == 0 and not cache.lengths.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, torch.bfloat16])
+def test_served_blocks_of_nothing(dtype):
+    """The layer's part of a block without points, and a model on a grid without samples under float16 autocast, as with slices."""
+    announce("block of nothing", dtype)
+    block = pn.TransolverBlock(4, 64, 0.0, use_te=False, window=dict(window=(5, 5))).cuda().eval()
+    x = torch.zeros(2, 0, 64, device="cuda", dtype=dtype)
+    with torch.no_grad():
+        for got in (*block.Attn.forward_block(x, x, block.ln_mlp1[0]), block.Attn.forward_block(x, x, None)):
+            assert got.shape == x.shape and got.dtype == (torch.float32 if dtype == torch.float16 else dtype)
+    for blocks in ((), (0, 2)):
+        torch.manual_seed(1)
+        net = pn.Transolver(functional_dim=3, out_dim=2, embedding_dim=2, n_layers=3, n_hidden=64, n_head=4, slice_num=16, use_te=False, structured_shape=(6, 7),
+                            window_blocks=blocks, window_options=dict(window=(5, 5)) if blocks else None).cuda().eval()
+        with torch.no_grad(), torch.autocast("cuda", torch.float16):
+            assert net(torch.zeros(0, 42, 3, device="cuda"), torch.zeros(0, 42, 2, device="cuda")).shape == (0, 42, 2)
