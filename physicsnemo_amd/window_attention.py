@@ -111,9 +111,10 @@ class WindowAttention(nn.Module):
         return frequencies
 
     def _apply(self, fn, recurse=True):
+        own = self.frequencies
         super()._apply(fn, recurse)
-        if self.frequencies is not None:  # float32 whatever type the weights are cast to
-            self.frequencies = self._frequencies().to(self.frequencies.device)
+        if own is not None:  # float32 whatever type the weights are cast to; on the meta device they have no values to keep
+            self.frequencies = (self._frequencies() if own.is_meta else own).to(self.frequencies.device)
         return self
 
     def extra_repr(self) -> str:

@@ -53,3 +53,14 @@ def test_steps_that_are_refused_leave_the_cache():
     with pytest.raises(ValueError, match="biases"):
         layer.step(torch.zeros(1, 1, 32), cache)
     assert cache.used == 0 and not cache.lengths.any()
+
+
+def test_frequencies_of_the_callers_stay():
+    """Those that a user sets go along with the layer like its weights."""
+    layer = pn.WindowAttention(32, heads=4, dim_head=16)
+    own = torch.linspace(0.1, 2.0, 8)[None]
+    layer.frequencies = own.clone()
+    for _ in (layer.to(torch.bfloat16), layer.half(), layer.double(), layer.cpu()):
+        assert layer.frequencies.dtype == torch.float32 and torch.equal(layer.frequencies, own)
+    model = torch.nn.Sequential(layer).to(torch.bfloat16)
+    assert torch.equal(model[0].frequencies, own)
