@@ -132,11 +132,12 @@ class WindowAttention(nn.Module):
         if (x.dtype == torch.float32 and type(lin) is nn.Linear and lin.weight.dtype == torch.float16 and PA.unhooked(lin) and
                 not torch.is_autocast_enabled("cuda")):  # weights of a float16 layer, which is computed in float32
             if needs_grad or lin.in_features > 512:
-                return nn.functional.linear(x, lin.weight.float(), lin.bias.float())
+                return nn.functional.linear(x, lin.weight.float(), None if lin.bias is None else lin.bias.float())
         if needs_grad:
             return PA.linear_as_autocast(x, lin)
         if x.dtype in (torch.float32, torch.bfloat16) and type(lin) is nn.Linear and lin.in_features <= 512 and PA.unhooked(lin):
-            return PF.linear(x, lin.weight.to(x.dtype).contiguous(), lin.bias.float().contiguous())
+            bias = lin.weight.new_zeros(lin.out_features, dtype=torch.float32) if lin.bias is None else lin.bias.float().contiguous()
+            return PF.linear(x, lin.weight.to(x.dtype).contiguous(), bias)
         return lin(x).to(x.dtype)
 
     def _qkv(self, x: torch.Tensor, positions, needs_grad: bool):

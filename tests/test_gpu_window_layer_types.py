@@ -151,3 +151,17 @@ def test_served_blocks_of_nothing(dtype):
                             window_blocks=blocks, window_options=dict(window=(5, 5)) if blocks else None).cuda().eval()
         with torch.no_grad(), torch.autocast("cuda", torch.float16):
             assert net(torch.zeros(0, 42, 3, device="cuda"), torch.zeros(0, 42, 2, device="cuda")).shape == (0, 42, 2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, torch.bfloat16])
+def test_projections_without_a_bias(dtype):
+    """A layer whose Linears were exchanged for such serves as it trains."""
+    announce("no biases", dtype)
+    torch.manual_seed(7)
+    layer = pn.WindowAttention(32, heads=4, dim_head=8, window=(9, 9))
+    layer.in_project_qkv, layer.out_linear = torch.nn.Linear(32, 96, bias=False), torch.nn.Linear(32, 32, bias=False)
+    layer, x = layer.cuda().to(dtype), torch.randn(2, 50, 32, device="cuda").to(dtype)
+    with torch.no_grad():
+        served = layer(x)
+    trained = layer(x)
+    assert trained.requires_grad and rel(served, trained.detach()) < 8 * torch.finfo(dtype).eps  # two products' roundings, and what they do to a softmax
