@@ -11,7 +11,7 @@
 // whole, so that the turn needs no neighbour and the norm three or four lane exchanges (halves that are no multiple of four go through LDS).
 //
 // What it takes: 131 072 x 16 rows of 32 bf16, 30 channels turned: 85 us (0.27 GB: 49; 230 vector instructions a row of four lanes and the angles in
-// double precision, 66 % of the issue slots); 4 x 7 225 x 16 x 16 float32, all turned: 14 forward, 21 backward (11 and 17 at the copy's rate).  The next row
+// double precision, 68 % of the issue slots); 4 x 7 225 x 16 x 16 float32, all turned: 15 forward, 21 backward (11 and 17 at the copy's rate).  The next row
 // loaded ahead gives 4 us of the 85 for eight registers; a point's heads one after the other by the same lanes, its turns in registers, 7, but
 // one point costs 5.1 instead of 4.3 and the backward pass 21.2 instead of 20.8: neither is kept.
 #include "pa_common.h"

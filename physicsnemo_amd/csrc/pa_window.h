@@ -417,7 +417,8 @@ struct Ops<float, DP> {
 // Float32 rows for the bf16 matrix instructions: a value is three bf16 values, each the rounding of what the ones before leave over, which
 // together hold all of its 24 bits; a . b is a1 b1 + a1 b2 + a2 b1 + a2 b2 + a1 b3 + a3 b1, and what is dropped is below 2^-24 |a| |b|.  A
 // product of 32 x 32 over 16 takes 48 passes of the matrix unit against 128 by v_mfma_f32_32x32x2_f32, and a width of 16 one step of 16 (4 x 7 225 x 8 x 16,
-// 171 keys: forward 92 -> 66 us, queries 123 -> 78, keys 156 -> 101; 20 000 x 4 x 64, 401 keys: 140 -> 98, 197 -> 131, 269 -> 175).
+// 171 keys, when it was taken: forward 92 -> 66 us, queries 123 -> 78, keys 156 -> 101, today 67, 91, 108; 20 000 x 4 x 64, 401 keys: 140 -> 98, 197 -> 131,
+// 269 -> 175, today 93, 161, 184).
 struct Thirds {
   uint32_t w[3];  // of two neighbouring values
 };
@@ -672,7 +673,7 @@ __device__ __forceinline__ void add_rows(const T *head, int64_t stride, int firs
         const float x = col < D ? load_as_f32(row + col) : 0.f;
         acc[db][r] = bad && seen ? fmaf(w, x, acc[db][r]) : acc[db][r];
         open |= col < D && acc[db][r] == acc[db][r];
-        if (r % 4 == 3) asm volatile("" ::: "memory");  // few loads at a time: this path must not cost the others registers
+        if (r % 4 == 3) asm volatile("" ::: "memory");  // few loads at a time, to cost the paths beside it fewer registers
       }
     if (!some_lane(bad && open)) return;  // NaN whatever follows: an input full of them takes no longer for it
   }

@@ -9,9 +9,9 @@
 // tiles of keys and values, two buffers in LDS, the next tile's loads under the present one's products.  Tiles that a wave's
 // queries do not see are skipped, and only tiles on an edge are masked.
 //
-// What it takes: 131 072 x 8 x 32 bf16, 513 keys a query: 172 us (0.27 GB: 49 us; 69 GFLOP: 50 us; 52 vector and 16 exp2 instructions a tile of 32 x 32:
-// about 110 us at full issue, which bounds it); 3 x 9 001 x 8 over 2 x 64, 1 024 keys: 101; 4 x 7 225 x 8 x 16 float32, 171 keys: 66; with biases
-// 65 536 x 8 x 32, 257 keys: 76.  Five waves a SIMD instead of four spill (2 to 3 times as long), 64 queries a wave lose a third.
+// What it takes: 131 072 x 8 x 32 bf16, 513 keys a query: 174 us (0.27 GB: 49 us; 69 GFLOP: 50 us; 52 vector and 16 exp2 instructions a tile of 32 x 32:
+// about 110 us at full issue, which bounds it; 66 % of the issue slots, matrix pipes 20 %); 3 x 9 001 x 8 over 2 x 64, 1 024 keys: 98; 4 x 7 225 x 8 x 16 float32,
+// 171 keys: 67; with biases 65 536 x 8 x 32, 257 keys: 77.  Five waves a SIMD instead of four spill (2 to 3 times as long), 64 queries a wave lose a third.
 #include "pa_window.h"
 
 #include <math.h>

@@ -5,16 +5,16 @@
 // (delta, dq, d bias), keys_kernel owns 32 keys a wave and goes over the queries that see them and over the query heads that share
 // them (dk, dv).
 //
-// What it takes: 65 536 x 8 x 32 bf16, 257 keys a query and 8 sinks: queries 82 us, keys 99 (0.27 GB in all: 49; the seven products' 45 GFLOP of ten: 33;
-// vector instructions and registers, three waves a SIMD, bound both); 4 x 7 225 x 8 x 16 float32, 171 keys: 78 and 101; with the bias gradient, 3 x 5 001 x 8
-// over 4 x 64, 512 keys: 119 (four products a tile, not three) and 91 to 96.
+// What it takes: 65 536 x 8 x 32 bf16, 257 keys a query and 8 sinks: queries 97 us, keys 100 (0.27 GB in all: 49; the eight products' 71 GFLOP: 52;
+// vector instructions and registers, three and four waves a SIMD, bound them: 60 and 50 % of the issue slots, matrix pipes 21); 4 x 7 225 x 8 x 16 float32,
+// 171 keys: 91 and 108; with the bias gradient, 3 x 5 001 x 8 over 4 x 64, 512 keys: 121 to 127 (six products a tile, not four) and 93.
 //
 // delta from y carries y's rounding (2^-9 of |dy| |v| for bf16), and with a delta that is off by e a query's score gradients sum up to e, not to zero: dq is
 // off by e times the mean of its keys, which may be many times what is left of dq where the keys and values have means of their own.  So the sum of
 // ds, as it is multiplied, and the mean key sum_j p_ij k_j are summed along; what the one leaves of the other is taken off dq, and the sum before its rounding is
 // added to delta for the second kernel.  Keys and values of mean 8 (6 000 points, 4 001 keys of 32 channels): dq in bf16 3.7 off, now 0.0024, dk 0.0145, now 0.0023; in float32 1.2e-3, now
-// 4.5e-6, a plain form 1.4e-4.  It costs a product in seven (65 536 x 8 x 32: queries 82 -> 96 us; float32
-// 4 x 7 225 x 8 x 16: 78 -> 90).
+// 4.5e-6, a plain form 1.4e-4.  It costs an eighth product beside seven (65 536 x 8 x 32: queries 82 -> 97 us; float32
+// 4 x 7 225 x 8 x 16: 78 -> 91; 20 000 x 4 x 64, 401 keys: 131 -> 161).
 // The bias gradient is float32, and sums single ds: where it is wanted, the first kernel sums p dp before it goes over the keys again.
 #include "pa_window.h"
 
@@ -46,8 +46,8 @@ __device__ __forceinline__ void add_diagonals(const f32x16 &ds, float *buffer, f
 
 // Waves a SIMD.  queries_kernel: bf16 rows to 32 run three by themselves (of odd pieces for ten spilled registers), to 64 two; the thirds of float32 rows take
 // 200 registers at widths to 32 (a third wave for 35 spilled ones) and 320 at 64 (a second wave).  keys_kernel: bf16 rows to 32 run four by themselves
-// without biases and three with them; float32 rows need 184 at widths to 32 and 271 at 64 (4 x 7 225 x 8 x 16: a third wave takes 109 to 101 us;
-// 20 000 x 4 x 64, 401 keys: a second one 200 to 175).  Rows of 128 run one: 350 to 450 registers.
+// without biases and three with them; float32 rows need 184 at widths to 32 and 271 at 64 (a third wave took 4 x 7 225 x 8 x 16 from 109 to 101 us, a second one
+// 20 000 x 4 x 64, 401 keys, from 200 to 175; with the differences behind the products 108 and 184).  Rows of 128 run one: 350 to 450 registers.
 template <int DP>
 constexpr int kWavesOfQueries = DP == 128 ? 1 : DP == 64 ? 2 : 3;
 template <class T, int DP>
